@@ -1,0 +1,280 @@
+// Paged attention of single tokens whose requests share their first positions, for any element type, head sizes (<= 512,
+// keys and values may differ in width), group and page size: the kernels of the 32-bit path, and of sizes the tensor-core
+// kernel (attention_shared_tc.cu) refuses; and the list of what is shared, which both read.
+//
+// Softmax attention over any cut of a row's keys comes together from each piece's maximum m, sum l = sum e^(z - m) and
+// accumulator o = sum e^(z - m) v:  m = max m_i,  l = sum l_i e^(m_i - m),  o = sum o_i e^(m_i - m),  and the row's answer is
+// o / l (l + e^(sink - m) under a sink). So the positions that a group of requests shares are one piece, or several, attended
+// to by all of the group's rows at once: their keys and values are read once for the group and not once a request. What a request holds
+// of its own makes more pieces. Everything is held in float32.
+//
+// Pieces are written as [requests, heads, places, width] (m in log2 units), a request's shared ones first, and a kernel of a
+// block per request and head puts them together, adds the sink, takes the difference of two maps or the gate.
+//
+// A block of four warps owns up to 32 rows (request, query head) of one key/value head and walks its keys in tiles of 32: a
+// warp has eight of the rows, a lane scores one key for them and then owns output dims lane, lane + 32, ...
+#include "common.cuh"
+
+namespace {
+
+constexpr int ROWS = 32, WARPS = 4, PER_WARP = ROWS / WARPS, TILE = 32;
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr int ITEM_INTS = 8;  // of the list of shared pieces (see SharedAttention)
+
+}  // namespace
+
+// What the kernels are handed. The list `plan` holds, ints: starts[requests] (the positions that a request shares), parts[requests] (the
+// pieces that these were cut into), members[...] (request numbers, group by group), then `items` of ITEM_INTS ints:
+// (request whose pages are read, place of the group's first member in `members`, first row, rows, key/value head, first key,
+// last key + 1, piece); rows < 1: nothing to do.
+struct SharedAttention {
+  const void *q, *k_pages, *v_pages, *gate;
+  void* out;
+  const int *block_table, *cu_seqlens, *seq_lens, *plan;
+  const float* sink;
+  float *part_o, *part_ml;
+  int* err;
+  long long page_stride;
+  int requests, members, items, max_parts, chunk_keys, max_chunks, gate_stride, max_pages, num_pages, nq, nkv, d, dv, page_size, maps;
+  float scale, softcap;
+  MapDifference difference;
+};
+
+namespace {
+
+template <typename T, int MOST>
+__global__ void __launch_bounds__(32 * WARPS)
+shared_pieces_kernel(const __grid_constant__ SharedAttention a) {
+  constexpr int ACC = MOST / 32;
+  pdl_wait();
+  pdl_launch_dependents();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int group = a.nq / a.nkv, width4 = (a.d + 3) / 4;
+  const int stride = 4 * width4 + ((width4 & 1) ? 0 : 4);  // 4 modulo 8 floats: eight lanes' 16 bytes lie in different banks
+  const int *starts = a.plan, *parts = starts + a.requests, *members = parts + a.requests;
+  int table_of, first_member, row0, rows, kvh, lo, hi, part;
+  if ((int)blockIdx.x < a.items) {
+    const int* item = members + a.members + ITEM_INTS * blockIdx.x;
+    table_of = item[0], first_member = item[1], row0 = item[2], rows = item[3], kvh = item[4], lo = item[5], hi = item[6], part = item[7];
+  } else {
+    // A chunk of what a request holds of its own.
+    int at = blockIdx.x - a.items;
+    const int chunk = at % a.max_chunks;
+    at /= a.max_chunks;
+    const int blocks = (group + ROWS - 1) / ROWS;
+    row0 = at % blocks * ROWS;
+    at /= blocks;
+    kvh = at % a.nkv;
+    table_of = at / a.nkv;
+    first_member = -1;
+    rows = min(ROWS, group - row0);
+    lo = starts[table_of] + chunk * a.chunk_keys, hi = min(lo + a.chunk_keys, a.seq_lens[table_of]);
+    part = parts[table_of] + chunk;
+  }
+  if (rows < 1 || lo >= hi) return;
+
+  extern __shared__ __align__(16) float smem[];
+  float* qs = smem;                    // [ROWS][stride]
+  float* ks = qs + ROWS * stride;      // [TILE][stride]
+  float* vs = ks + TILE * stride;      // [TILE][dv]
+  auto place = [&](int r, int& request, int& head) {
+    const int row = row0 + r;
+    request = first_member < 0 ? table_of : members[first_member + row / group];
+    head = kvh * group + row % group;
+  };
+  const T* q = (const T*)a.q;
+  for (int i = tid; i < ROWS * stride; i += 32 * WARPS) {
+    const int r = i / stride, c = i - r * stride;
+    float v = 0.f;
+    if (r < rows && c < a.d) {
+      int request, head;
+      place(r, request, head);
+      v = to_f32(q[((size_t)a.cu_seqlens[request] * a.nq + head) * a.d + c]);
+    }
+    qs[i] = v;
+  }
+  for (int i = tid; i < TILE * stride; i += 32 * WARPS) ks[i] = 0.f;  // the dims beyond d stay zero
+  float m[PER_WARP], l[PER_WARP], acc[PER_WARP][ACC];
+#pragma unroll
+  for (int x = 0; x < PER_WARP; ++x) {
+    m[x] = -INFINITY, l[x] = 0.f;
+#pragma unroll
+    for (int k = 0; k < ACC; ++k) acc[x][k] = 0.f;
+  }
+  const int* table = a.block_table + (size_t)table_of * a.max_pages;
+  const T *k_pages = (const T*)a.k_pages, *v_pages = (const T*)a.v_pages;
+  const float pre = a.softcap > 0.f ? a.scale / a.softcap : a.scale * LOG2E, cap = a.softcap * LOG2E;
+  for (int key0 = lo; key0 < hi; key0 += TILE) {
+    __syncthreads();  // the tile before has been read
+    const int keys = min(TILE, hi - key0);
+    // A warp brings every fourth key. Rows past the last key hold zeros, whatever the cache has there.
+    bool bad = false;
+    for (int k = warp; k < TILE; k += WARPS) {
+      const int pos = key0 + k;
+      const int page = k < keys ? table[pos / a.page_size] : -1;
+      const bool there = page >= 0 && page < a.num_pages;
+      bad |= k < keys && !there;
+      const long long at = (long long)page * a.page_stride;
+      const int off = kvh * a.page_size + pos % a.page_size;
+      for (int c = lane; c < a.d; c += 32) ks[k * stride + c] = there ? to_f32(k_pages[at + (long long)off * a.d + c]) : 0.f;
+      for (int c = lane; c < a.dv; c += 32) vs[k * a.dv + c] = there ? to_f32(v_pages[at + (long long)off * a.dv + c]) : 0.f;
+    }
+    if (bad && lane == 0) atomicOr(a.err, OMNIA_ERR_PAGE);
+    __syncthreads();
+    float s[PER_WARP];
+#pragma unroll
+    for (int x = 0; x < PER_WARP; ++x) s[x] = 0.f;
+    const float4* k4 = reinterpret_cast<const float4*>(ks + lane * stride);
+    for (int c = 0; c < width4; ++c) {
+      const float4 k = k4[c];
+#pragma unroll
+      for (int x = 0; x < PER_WARP; ++x) {
+        if (warp + WARPS * x >= rows) break;
+        const float4 v = reinterpret_cast<const float4*>(qs + (warp + WARPS * x) * stride)[c];
+        s[x] = fmaf(v.x, k.x, fmaf(v.y, k.y, fmaf(v.z, k.z, fmaf(v.w, k.w, s[x]))));
+      }
+    }
+#pragma unroll
+    for (int x = 0; x < PER_WARP; ++x) {
+      if (warp + WARPS * x >= rows) break;
+      float z = a.softcap > 0.f ? cap * tanhf(s[x] * pre) : s[x] * pre;
+      if (lane >= keys) z = -INFINITY;
+      const float top = fmaxf(m[x], warp_max(z));
+      const float base = top == -INFINITY ? 0.f : top;
+      const float p = exp2f(z - base), alpha = m[x] == -INFINITY ? 0.f : exp2f(m[x] - base);
+      m[x] = top;
+      l[x] = l[x] * alpha + warp_sum(p);
+#pragma unroll
+      for (int k = 0; k < ACC; ++k) acc[x][k] *= alpha;
+      s[x] = p;
+    }
+    for (int k = 0; k < keys; ++k) {
+      float v[ACC];
+#pragma unroll
+      for (int i = 0; i < ACC; ++i) v[i] = lane + 32 * i < a.dv ? vs[k * a.dv + lane + 32 * i] : 0.f;
+#pragma unroll
+      for (int x = 0; x < PER_WARP; ++x) {
+        if (warp + WARPS * x >= rows) break;
+        const float p = __shfl_sync(0xffffffffu, s[x], k);
+#pragma unroll
+        for (int i = 0; i < ACC; ++i) acc[x][i] = fmaf(p, v[i], acc[x][i]);
+      }
+    }
+  }
+  const int places = a.max_parts + a.max_chunks;
+#pragma unroll
+  for (int x = 0; x < PER_WARP; ++x) {
+    const int r = warp + WARPS * x;
+    if (r >= rows) break;
+    int request, head;
+    place(r, request, head);
+    const size_t at = ((size_t)request * a.nq + head) * places + part;
+#pragma unroll
+    for (int i = 0; i < ACC; ++i)
+      if (lane + 32 * i < a.dv) a.part_o[at * a.dv + lane + 32 * i] = acc[x][i];
+    if (lane == 0) a.part_ml[2 * at] = m[x], a.part_ml[2 * at + 1] = l[x];
+  }
+}
+
+// grid (heads that come out, requests), 128 threads: a request's pieces put together in ascending order.
+template <typename T>
+__global__ void __launch_bounds__(128)
+shared_merge_kernel(const __grid_constant__ SharedAttention a) {
+  __shared__ float scratch[33];
+  pdl_wait();
+  pdl_launch_dependents();
+  const int request = blockIdx.y, tid = threadIdx.x;
+  const int own = a.seq_lens[request] - a.plan[request];
+  if (a.seq_lens[request] < 1) return;
+  const int count = min(a.plan[a.requests + request], a.max_parts) + max(0, min((own + a.chunk_keys - 1) / a.chunk_keys, a.max_chunks));
+  const int places = a.max_parts + a.max_chunks;
+  const size_t token = (size_t)a.cu_seqlens[request];
+  constexpr int PER_THREAD = 4;  // widths of at most 512
+  float map[2][PER_THREAD];
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    if (which >= a.maps) break;
+    const int head = blockIdx.x * a.maps + which;
+    const size_t at = ((size_t)request * a.nq + head) * places;
+    const float *ml = a.part_ml + 2 * at, *o = a.part_o + at * a.dv;
+    float top = -INFINITY, total = 0.f;
+    for (int i = 0; i < count; ++i) top = fmaxf(top, ml[2 * i]);
+#pragma unroll
+    for (int v = 0; v < PER_THREAD; ++v) map[which][v] = 0.f;
+    for (int i = 0; i < count; ++i) {
+      const float w = ml[2 * i] == -INFINITY ? 0.f : exp2f(ml[2 * i] - top);
+      total += ml[2 * i + 1] * w;
+#pragma unroll
+      for (int v = 0; v < PER_THREAD; ++v)
+        if (tid + 128 * v < a.dv) map[which][v] += o[(size_t)i * a.dv + tid + 128 * v] * w;
+    }
+    if (a.sink != nullptr && top != -INFINITY) total += exp2f(a.sink[head] * LOG2E - top);
+    const float inv = total > 0.f ? 1.f / total : 0.f;
+#pragma unroll
+    for (int v = 0; v < PER_THREAD; ++v) map[which][v] *= inv;
+  }
+  T* out = (T*)a.out;
+  if (a.maps == 2) {
+    float ss = 0.f;
+#pragma unroll
+    for (int v = 0; v < PER_THREAD; ++v) {
+      map[0][v] = tid + 128 * v < a.difference.dv ? map[0][v] - a.difference.lambda * map[1][v] : 0.f;
+      ss += map[0][v] * map[0][v];
+    }
+    const float f = rsqrtf(block_sum(ss, scratch) / (float)a.difference.dv + a.difference.eps) * a.difference.factor;
+    T* row = out + (token * (a.nq / 2) + blockIdx.x) * a.difference.dv;
+#pragma unroll
+    for (int v = 0; v < PER_THREAD; ++v)
+      if (tid + 128 * v < a.difference.dv) row[tid + 128 * v] = from_f32<T>(map[0][v] * f);
+    return;
+  }
+  const T* gate = a.gate ? (const T*)a.gate + token * a.gate_stride + (size_t)blockIdx.x * a.dv : nullptr;
+#pragma unroll
+  for (int v = 0; v < PER_THREAD; ++v) {
+    const int dim = tid + 128 * v;
+    if (dim >= a.dv) break;
+    float y = map[0][v];
+    if (gate) y *= 1.f / (1.f + expf(-to_f32(gate[dim])));
+    out[(token * a.nq + blockIdx.x) * a.dv + dim] = from_f32<T>(y);
+  }
+}
+
+template <typename T, int MOST>
+int launch_pieces(const SharedAttention& a, long long blocks, size_t smem, cudaStream_t stream) {
+  static bool configured[64] = {};
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) return (int)cudaErrorInvalidDevice;
+  if (!configured[device]) {
+    const cudaError_t e = cudaFuncSetAttribute(shared_pieces_kernel<T, MOST>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+    if (e != cudaSuccess) return (int)e;
+    configured[device] = true;
+  }
+  launch_pdl(shared_pieces_kernel<T, MOST>, dim3((unsigned)blocks), 32 * WARPS, smem, stream, a);
+  return OMNIA_LAUNCH_RESULT();
+}
+
+}  // namespace
+
+extern "C" int omnia_shared_attention(const SharedAttention* given, int dtype, cudaStream_t stream) {
+  const SharedAttention a = *given;
+  if (a.requests == 0) return 0;
+  if (a.requests < 0 || a.requests > 65535 || a.members < 0 || a.items < 0 || a.nkv < 1 || a.nq < 1 || a.nq % a.nkv || a.d < 1 || a.d > 512 ||
+      a.dv < 1 || a.dv > 512 || a.page_size < 1 || a.max_pages < 1 || a.num_pages < 1 || a.max_parts < 0 || a.max_chunks < 0 ||
+      a.chunk_keys < 1 || a.softcap < 0.f || (a.maps != 1 && a.maps != 2) ||
+      (a.maps == 2 && (a.nq % 2 || a.gate || a.sink || a.difference.dv < 1 || a.difference.dv > a.dv)))
+    return (int)cudaErrorInvalidValue;
+  const int group = a.nq / a.nkv, width4 = (a.d + 3) / 4, stride = 4 * width4 + ((width4 & 1) ? 0 : 4);
+  const long long blocks = a.items + (long long)a.requests * a.nkv * ((group + ROWS - 1) / ROWS) * a.max_chunks;
+  if (blocks > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
+  const size_t smem = (size_t)((ROWS + TILE) * stride + TILE * a.dv) * sizeof(float);
+  const int most = a.d > a.dv ? a.d : a.dv;
+  OMNIA_DISPATCH_DTYPE(dtype, {
+    if (blocks > 0) {
+      const int code = most <= 64 ? launch_pieces<T, 64>(a, blocks, smem, stream) : most <= 128 ? launch_pieces<T, 128>(a, blocks, smem, stream)
+                     : most <= 256 ? launch_pieces<T, 256>(a, blocks, smem, stream) : launch_pieces<T, 512>(a, blocks, smem, stream);
+      if (code != 0) return code;
+    }
+    launch_pdl(shared_merge_kernel<T>, dim3(a.nq / a.maps, a.requests), 128, 0, stream, a);
+  });
+  return OMNIA_LAUNCH_RESULT();
+}

@@ -655,8 +655,8 @@ def decode_fusable(proj: torch.Tensor, nq: int, nkv: int, d: int, inv_freq: torc
                    kv: KVView, step: StepContext) -> bool:
     """Whether the decode attention kernel can take the projected rows as they are: a step of
     single tokens, bfloat16, a head size that is a multiple of 32, rotated whole or not at all,
-    and a cache entry that this layer writes."""
-    return (step.decode_only and proj.is_cuda and kv.writes and d % 32 == 0
+    a cache entry that this layer writes, and no positions shared by several requests that are read once for all."""
+    return (step.decode_only and not shared_applies(step, kv) and proj.is_cuda and kv.writes and d % 32 == 0
             and (inv_freq is None or 2 * inv_freq.shape[0] == d) and proj.shape[1] % 2 == 0
             and tiled_attention_supported(proj.dtype, nq, nkv, d))
 
@@ -671,6 +671,124 @@ class MapDifference:
     eps: float
     factor: float
     dv: int
+
+
+class _MapDifferenceArgs(ctypes.Structure):
+    _fields_ = [("lam", c_float), ("eps", c_float), ("factor", c_float), ("dv", c_int)]
+
+
+class _SharedArgs(ctypes.Structure):  # SharedAttention in attention_shared.cu
+    _fields_ = [(name, c_void_p) for name in ("q", "k_pages", "v_pages", "gate", "out", "block_table", "cu_seqlens", "seq_lens", "plan",
+                                              "sink", "part_o", "part_ml", "err")] + \
+               [("page_stride", c_longlong)] + \
+               [(name, c_int) for name in ("requests", "members", "items", "max_parts", "chunk_keys", "max_chunks", "gate_stride", "max_pages",
+                                           "num_pages", "nq", "nkv", "d", "dv", "page_size", "maps")] + \
+               [("scale", c_float), ("softcap", c_float), ("difference", _MapDifferenceArgs)]
+
+
+SHARED_ROWS, SHARED_TILE = 32, 32
+"""Rows of a block and keys of a tile of the kernel for any shape (attention_shared.cu)."""
+
+
+@dataclass(frozen=True)
+class SharedPlan:
+    """How a step's shared positions are cut: `parts` pieces of a group's positions, `items` (block of rows, key/value head, piece) in
+    all, `members` places of the list of requests. Made from the groups' sizes rounded up (`shared_shape`), so that
+    a captured step takes the same plan until a group has lost half of its requests."""
+
+    parts: tuple[int, ...]
+    blocks: tuple[int, ...]  # of rows, a group
+    members: int
+    items: int
+
+
+def shared_shape(shared) -> tuple[tuple[int, int], ...]:
+    """(positions, requests rounded up to a power of two) of every group: what a plan is made from."""
+    return tuple((positions, 1 << max(len(members) - 1, 0).bit_length()) for positions, members in shared)
+
+
+def shared_plan(shape: tuple[tuple[int, int], ...], group: int, nkv: int, block_rows: int, tile: int, least: int, places: int) -> SharedPlan:
+    """`group` query heads to each of `nkv` key/value heads, `block_rows` rows and tiles of `tile` keys to a block; pieces of at least `least`
+    tiles, as many as keep all items within the `places` that the GPU runs at a time (one a group where even that is more)."""
+    tiles = [-(-positions // tile) for positions, _ in shape]
+    blocks = [-(-count * group // block_rows) for _, count in shape]
+    items = lambda size: sum(b * nkv * -(-t // size) for b, t in zip(blocks, tiles))  # noqa: E731
+    lo, hi = least, max([least, *tiles])
+    while lo < hi:  # the least size with which all items fit
+        mid = (lo + hi) // 2
+        lo, hi = (lo, mid) if items(mid) <= places else (mid + 1, hi)
+    return SharedPlan(tuple(-(-t // lo) for t in tiles), tuple(blocks), sum(count for _, count in shape), items(lo))
+
+
+def shared_list(step: StepContext, plan: SharedPlan, group: int, nkv: int, block_rows: int, tile: int) -> np.ndarray:
+    """The list that the kernels read (`SharedAttention` in attention_shared.cu)."""
+    n = step.num_seqs
+    out = np.zeros(2 * n + plan.members + 8 * plan.items, dtype=np.int32)
+    items = out[2 * n + plan.members:].reshape(-1, 8)
+    seen: set[int] = set()
+    first = at = 0
+    for (positions, members), parts, blocks, (_, room) in zip(step.shared, plan.parts, plan.blocks, shared_shape(step.shared)):
+        if positions < 1 or not members or not seen.isdisjoint(members) or len(set(members)) < len(members) or \
+                min(members) < 0 or max(members) >= n:
+            raise KernelError("requests share at least one position, each in one group of the step's requests")
+        if step.seq_lens_host and any(m < len(step.seq_lens_host) and step.seq_lens_host[m] <= positions for m in members):
+            raise KernelError("a request holds more positions than it shares")
+        seen.update(members)
+        out[list(members)] = positions
+        out[[n + m for m in members]] = parts
+        out[2 * n + first: 2 * n + first + len(members)] = members
+        tiles = -(-positions // tile)
+        cuts = [tiles * i // parts * tile for i in range(parts)] + [positions]
+        for b in range(blocks):
+            rows = max(0, min(block_rows, len(members) * group - b * block_rows))
+            block = items[at: at + nkv * parts].reshape(nkv, parts, 8)
+            block[:, :, 0], block[:, :, 1], block[:, :, 2], block[:, :, 3] = members[0], first, b * block_rows, rows
+            block[:, :, 4] = np.arange(nkv)[:, None]
+            block[:, :, 5], block[:, :, 6], block[:, :, 7] = cuts[:-1], cuts[1:], np.arange(parts)
+            at += nkv * parts
+        first += room
+    return out
+
+
+def shared_applies(step: StepContext, kv: KVView, run: int = 0) -> bool:
+    """Whether a layer's attention reads shared positions once for their group: a step of single tokens, every position in sight."""
+    return bool(getattr(step, "shared", ())) and step.decode_only and not kv.window and not run
+
+
+def _own_longest(step: StepContext) -> int:
+    """The most positions that a request of the step holds beyond those that it shares."""
+    if step.max_own is not None:
+        return step.max_own
+    starts = {m: positions for positions, members in step.shared for m in members}
+    return max((n - starts.get(r, 0) for r, n in enumerate(step.seq_lens_host)), default=0)
+
+
+def _shared_attention(q: torch.Tensor, kv: KVView, step: StepContext, scale: float, gate_ptr, gate_stride: int, sink: torch.Tensor | None,
+                      softcap: float, difference: "MapDifference | None", out: torch.Tensor) -> torch.Tensor:
+    """`paged_attention` of a step whose requests share positions (`StepContext.shared`): a group's shared positions as pieces for all of its
+    rows, each request's own in chunks, both put together at the end."""
+    device = q.device
+    _, nq, d = q.shape
+    k_ptr, v_ptr, page_stride, nkv, _, dv = kv_layout(kv)
+    group, sms, n = nq // nkv, sm_count(device), step.num_seqs
+    own = width_bucket(-(-_own_longest(step) // kv.page_size)) * kv.page_size
+    chunk, _ = decode_plan(n, nkv, own, sms)
+    plan = shared_plan(shared_shape(step.shared), group, nkv, SHARED_ROWS, SHARED_TILE, 4, 4 * sms)
+    key = ("shared", group, nkv, SHARED_ROWS, SHARED_TILE, plan)
+    listed = _step_list(step, key, lambda st: shared_list(st, plan, group, nkv, SHARED_ROWS, SHARED_TILE), device)
+    max_parts, max_chunks = max(plan.parts), -(-own // chunk)
+    part_o, part_ml = _step_buffers(step, device, {
+        "attention_part_o": (n * nq * (max_parts + max_chunks) * dv, torch.float32, False),
+        "attention_part_ml": (n * nq * (max_parts + max_chunks) * 2, torch.float32, False)})
+    last = _MapDifferenceArgs(0.0, 0.0, 0.0, 0) if difference is None else \
+        _MapDifferenceArgs(difference.lam, difference.eps, difference.factor, difference.dv)
+    args = _SharedArgs(_ptr(q), k_ptr, v_ptr, gate_ptr, _ptr(out), _ptr(kv.block_table), _ptr(step.cu_seqlens), _ptr(step.seq_lens), _ptr(listed),
+                       _ptr(sink), _ptr(part_o), _ptr(part_ml), _ptr(error_word(device)), page_stride, n, plan.members, plan.items, max_parts, chunk,
+                       max_chunks, gate_stride, kv.block_table.shape[1], kv.pages.shape[0], nq, nkv, d, dv, kv.page_size,
+                       1 if difference is None else 2, scale, softcap, last)
+    fn = _function("attention_shared", "omnia_shared_attention", [c_void_p, c_int, c_void_p])
+    _check(fn(ctypes.byref(args), _code(q.dtype), _stream()), "shared_attention")
+    return out
 
 
 def paged_attention(q: torch.Tensor | None, kv: KVView, step: StepContext, scale: float,
@@ -729,6 +847,10 @@ def paged_attention(q: torch.Tensor | None, kv: KVView, step: StepContext, scale
     run, softcap = int(chunk or 0), float(softcap or 0.0)
     if run and keep:
         raise KernelError("a mask of runs keeps no first positions")
+    if shared_applies(step, kv, run):
+        if projection is not None:
+            raise KernelError("attention over shared positions takes queries, not projected rows")
+        return _shared_attention(q, kv, step, scale, gate_ptr, gate_stride, sink, softcap, difference, out)
     if dv != d or not tiled_attention_supported(q.dtype, nq, nkv, d):
         if projection is not None:
             raise KernelError("the generic attention kernel takes queries, not projected rows")
@@ -903,6 +1025,57 @@ def fill_slots(tensors: list[tuple[torch.Tensor, torch.Tensor | None]], slots: l
         for j in range(0, len(slots), FILL_SLOTS):
             some = (c_int * len(slots[j: j + FILL_SLOTS]))(*slots[j: j + FILL_SLOTS])
             _check(fn(to, start, size, len(part), some, len(some), _stream()), "fill_slots")
+
+
+def _move_array(moves, columns: int, most_from: int, most_to: int, same: bool, what: str) -> np.ndarray:
+    """Moves (from, to, ...) as an int32 array; numbers in range, no two with one end, and in one tensor no move's end another's beginning."""
+    held = np.asarray(moves, dtype=np.int64).reshape(-1, columns)
+    if held.shape[0]:
+        src, dst = held[:, 0], held[:, 1]
+        if int(src.min()) < 0 or int(src.max()) >= most_from or int(dst.min()) < 0 or int(dst.max()) >= most_to:
+            raise KernelError(f"{what}: a move's number lies outside the tensor")
+        ends = set(dst.tolist())
+        if len(ends) < held.shape[0]:
+            raise KernelError(f"{what}: two moves end in the same place")
+        if same and not ends.isdisjoint(src.tolist()):
+            raise KernelError(f"{what}: a move ends where another begins")
+    return np.ascontiguousarray(held, dtype=np.int32)
+
+
+def copy_pages(pages: torch.Tensor, rows: tuple[tuple[int, int], ...], page_size: int, moves, to: torch.Tensor | None = None) -> torch.Tensor:
+    """In place: of every layer's pages (`pages` [layers, pages, ...], contiguous), the first `count` stored rows of page `src` to
+    page `dst`, for every (src, dst, count) of `moves`. `rows`: what a page holds, the `(heads, width)` of a `KVSpec`, each a block
+    [heads, page_size, width]. `to`: another such tensor (as many layers, other pages, of the same type and page shape) that the
+    pages go to. No two moves may end in the same page, and within one tensor none where another begins. -> the tensor written"""
+    to = pages if to is None else to
+    if not pages.is_contiguous() or not to.is_contiguous() or pages.dtype != to.dtype or pages.device != to.device or \
+            pages.shape[:1] + pages.shape[2:] != to.shape[:1] + to.shape[2:]:
+        raise KernelError("copy_pages takes contiguous tensors of the same layers, page shape, type and device")
+    item, elements = pages.element_size(), pages.shape[2:].numel()
+    if sum(h * w for h, w in rows) * page_size != elements:
+        raise KernelError(f"pages of {elements} elements do not hold {page_size} rows of {rows}")
+    held = _move_array(moves, 3, pages.shape[1], to.shape[1], pages.data_ptr() == to.data_ptr(), "copy_pages")
+    if held.shape[0] and (int(held[:, 2].min()) < 0 or int(held[:, 2].max()) > page_size):
+        raise KernelError(f"copy_pages: a move of more rows than a page's {page_size}, or fewer than none")
+    fn = _function("cache_copy", "omnia_copy_pages", [c_void_p, c_void_p, c_longlong, c_longlong, c_int, c_longlong, c_int, c_void_p, c_void_p,
+                                                      c_int, c_void_p, c_int, c_void_p])
+    heads, width = (c_int * len(rows))(*(h for h, _ in rows)), (c_int * len(rows))(*(w * item for _, w in rows))
+    _check(fn(_ptr(pages), _ptr(to), pages.stride(0) * item, to.stride(0) * item, pages.shape[0], elements * item, page_size, heads, width,
+              len(rows), held.ctypes.data, held.shape[0], _stream()), "copy_pages")
+    return to
+
+
+def copy_slots(tensors: list[torch.Tensor], moves) -> None:
+    """In place: row `src` of every tensor (contiguous, of whatever type) to its row `dst`, for every (src, dst) of `moves`. No
+    two moves may end in the same row, none where another begins."""
+    if any(not t.is_contiguous() or t.dim() < 1 for t in tensors):
+        raise KernelError("copy_slots takes contiguous tensors")
+    least = min((t.shape[0] for t in tensors), default=0)
+    held = _move_array(moves, 2, least, least, True, "copy_slots")
+    fn = _function("cache_copy", "omnia_copy_slots", [c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p])
+    to = (c_void_p * len(tensors))(*(t.data_ptr() for t in tensors))
+    size = (c_longlong * len(tensors))(*(t[0].numel() * t.element_size() if t.shape[0] else 0 for t in tensors))
+    _check(fn(to, size, len(tensors), held.ctypes.data, held.shape[0], _stream()), "copy_slots")
 
 
 SKINNY_ROWS = 16

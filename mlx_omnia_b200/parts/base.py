@@ -345,6 +345,10 @@ class StepContext:
     groups: dict[int, tuple[torch.Tensor, torch.Tensor]]  # group -> (block_table, slot_mapping)
     workspace: Any = None
     model_state: "dict[str, torch.Tensor] | None" = None  # the embedding's named per-request state
+    # Which requests share their first positions, in the same pages or in copies of them: (positions, requests of the step) for
+    # each group, no request in two. Attention without a window may then read a group's shared positions once for all of it.
+    shared: "tuple[tuple[int, tuple[int, ...]], ...]" = ()
+    max_own: int | None = None  # a bound of what a request holds beyond its shared positions (None: from seq_lens_host)
 
 
 @dataclass
