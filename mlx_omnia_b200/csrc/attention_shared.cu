@@ -13,32 +13,14 @@
 //
 // A block of four warps owns up to 32 rows (request, query head) of one key/value head and walks its keys in tiles of 32: a
 // warp has eight of the rows, a lane scores one key for them and then owns output dims lane, lane + 32, ...
-#include "common.cuh"
+#include "attention_shared.cuh"
 
 namespace {
 
 constexpr int ROWS = 32, WARPS = 4, PER_WARP = ROWS / WARPS, TILE = 32;
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr int ITEM_INTS = 8;  // of the list of shared pieces (see SharedAttention)
 
 }  // namespace
-
-// What the kernels are handed. The list `plan` holds, ints: starts[requests] (the positions that a request shares), parts[requests] (the
-// pieces that these were cut into), members[...] (request numbers, group by group), then `items` of ITEM_INTS ints:
-// (request whose pages are read, place of the group's first member in `members`, first row, rows, key/value head, first key,
-// last key + 1, piece); rows < 1: nothing to do.
-struct SharedAttention {
-  const void *q, *k_pages, *v_pages, *gate;
-  void* out;
-  const int *block_table, *cu_seqlens, *seq_lens, *plan;
-  const float* sink;
-  float *part_o, *part_ml;
-  int* err;
-  long long page_stride;
-  int requests, members, items, max_parts, chunk_keys, max_chunks, gate_stride, max_pages, num_pages, nq, nkv, d, dv, page_size, maps;
-  float scale, softcap;
-  MapDifference difference;
-};
 
 namespace {
 
@@ -54,7 +36,7 @@ shared_pieces_kernel(const __grid_constant__ SharedAttention a) {
   const int *starts = a.plan, *parts = starts + a.requests, *members = parts + a.requests;
   int table_of, first_member, row0, rows, kvh, lo, hi, part;
   if ((int)blockIdx.x < a.items) {
-    const int* item = members + a.members + ITEM_INTS * blockIdx.x;
+    const int* item = members + a.members + SHARED_ITEM_INTS * blockIdx.x;
     table_of = item[0], first_member = item[1], row0 = item[2], rows = item[3], kvh = item[4], lo = item[5], hi = item[6], part = item[7];
   } else {
     // A chunk of what a request holds of its own.

@@ -1,0 +1,407 @@
+// The shared positions of attention_shared.cu in bfloat16 on the 5th-generation tensor cores: a group's keys and values are
+// fetched once and attended to by the rows of all its requests. Compiled for one head size and one group size:
+//   -DHEAD_DIM=64|128   -DGROUP=g (query heads per key/value head, g <= 16)
+//
+// Floor: the shared keys and values once (4 D bytes a position and key/value head) at the memory's rate, or the
+// products' 4 D operations a row and position, whichever is more: 256 rows are where the two meet.
+//
+// A block has an SM, one key/value head, one run of keys (an item of the list) and up to 256 rows, in two slots of 128, which are two
+// softmax chains that know nothing of one another: each has a score tile of 128 columns and an accumulator in tensor memory, a
+// warp that issues its products and four warps of a thread a row:
+//   S = Q K^T   tcgen05.mma (M 128, N 128) over the head size
+//   softmax     two passes over the scores, 32 at a time; P, rounded to bfloat16, takes the scores' place; the exponent's
+//               offset follows a row's maximum lazily, and only then is the accumulator rescaled
+//   O += P V    tcgen05.mma (M 128, N head size), P read from tensor memory
+// One chain alone would wait for its own products and loads half of the time; two fill each other's gaps. With more
+// than 128 rows a slot has half of them and both see every tile of keys; with fewer both hold the same rows and take the tiles
+// in turn, and the two states are brought together at the end. The rows are gathered from wherever the requests' tokens lie.
+// Keys and values come by TMA, a box of 16 keys x 64 dims, into rings of stages of 128 keys.
+#ifndef HEAD_DIM
+#define HEAD_DIM 128
+#endif
+#ifndef GROUP
+#define GROUP 2
+#endif
+
+#include "attention_tcgen05.cuh"
+#include "attention_shared.cuh"
+namespace {
+
+constexpr int D = HEAD_DIM;
+static_assert(D == 64 || D == 128, "head sizes 64 and 128");
+static_assert(GROUP >= 1 && GROUP <= 16, "group size must be 1..16");
+constexpr int DH = D / 64;               // 64-wide halves of a head
+constexpr int BM = 128, BN = 128;        // rows of a slot, keys of a tile
+constexpr int SLOT_ROWS = BM / GROUP * GROUP;
+// Seven tiles of shared memory: the rows (one tile where both slots hold the same, else two), the rest but the last two for
+// keys, two for values. A stage's loads, products and barriers go by one order of tiles; where the slots take turns each has stages
+// of its own (the even or the odd ones), filled by a warp of its own: a stage that both used would complete a phase which the slower
+// slot has yet to wait for.
+constexpr int TILES = 7, V_STAGES = 2, K_STAGES = 4;  // (three for keys where there are two tiles of rows)
+constexpr int SOFTMAX_THREADS = 256;     // warps 0-3 slot 0, 4-7 slot 1
+constexpr int WARP_MMA = 8, WARP_K = 10, WARP_V = 12, FEEDERS = 2;  // one issuer a slot; two warps feed each ring in turns
+constexpr int THREADS = 32 * 14;
+constexpr uint32_t HALF_BYTES = 128 * 128;   // 128 rows of 128 bytes
+constexpr uint32_t TILE_BYTES = DH * HALF_BYTES;
+constexpr uint32_t BOX_BYTES = 16 * 128;     // 16 keys x 64 dims
+constexpr uint32_t TMEM_COLS = 512, O_COL = 2 * BN;  // two score tiles, then two accumulators
+
+__device__ __forceinline__ void softmax_sync() { asm volatile("bar.sync 1, %0;" ::"n"(SOFTMAX_THREADS) : "memory"); }
+
+}  // namespace
+
+__global__ void __launch_bounds__(THREADS, 1)
+shared_pieces_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_constant__ SharedAttention a) {
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  if (smem_u32(smem_raw) & 1023u) {  // the swizzled tiles need a base on 1024 bytes
+    if (threadIdx.x == 0) atomicOr(a.err, OMNIA_ERR_TIMEOUT);
+    return;
+  }
+  unsigned char* q_s = smem_raw;
+  unsigned char* v_s = q_s + (TILES - V_STAGES) * TILE_BYTES;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(v_s + V_STAGES * TILE_BYTES);
+  // bars: q_full | k_full[] | k_empty[] | v_full[] | v_empty[] | s_full[2] | p_full[2] | o_done[2]
+  constexpr int BARS = 1 + 2 * K_STAGES + 2 * V_STAGES + 6;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + BARS);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+  float* row_ml = reinterpret_cast<float*>(tmem_holder + 2);  // [2][128][2]: a slot's offset and sum, for the other one
+  const int warp = omnia_warp_index(), lane = threadIdx.x & 31;
+  const uint32_t q_full = smem_u32(bars), k_full0 = q_full + 8, k_empty0 = k_full0 + 8 * K_STAGES, v_full0 = k_empty0 + 8 * K_STAGES,
+                 v_empty0 = v_full0 + 8 * V_STAGES, s_full0 = v_empty0 + 8 * V_STAGES, p_full0 = s_full0 + 16, o_done0 = p_full0 + 16;
+  if (warp == WARP_MMA) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)), "r"(TMEM_COLS));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+  }
+  // From here on what earlier kernels wrote is read; the launch is a programmatic dependent one.
+  pdl_wait();
+  pdl_launch_dependents();
+  const int *members = a.plan + 2 * a.requests, *item = members + a.members + SHARED_ITEM_INTS * blockIdx.x;
+  const int table_of = item[0], first_member = item[1], row0 = item[2], rows = item[3], kvh = item[4], lo = item[5], hi = item[6], part = item[7];
+  const bool turns = rows <= SLOT_ROWS;           // both slots hold the same rows and take the tiles in turn
+  const int k_stages = turns ? K_STAGES : K_STAGES - 1;
+  unsigned char* k_s = v_s - k_stages * TILE_BYTES;
+  const int tiles = rows < 1 ? 0 : (hi - lo + BN - 1) / BN;
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, SOFTMAX_THREADS);
+    const int readers = turns ? 1 : 2;
+    for (int s = 0; s < K_STAGES; ++s) mbar_init(k_full0 + 8 * s, 1), mbar_init(k_empty0 + 8 * s, readers);
+    for (int s = 0; s < V_STAGES; ++s) mbar_init(v_full0 + 8 * s, 1), mbar_init(v_empty0 + 8 * s, readers);
+    for (int s = 0; s < 2; ++s) mbar_init(s_full0 + 8 * s, 1), mbar_init(p_full0 + 8 * s, BM), mbar_init(o_done0 + 8 * s, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem_base = *tmem_holder;
+  int issued = -1;  // the last tile that this warp has asked for
+
+  if (warp >= WARP_K) {
+    // ---- producers: two warps a ring take turns with its stages; a lane looks up a box's page, one lane asks for the boxes ----
+    const int which = warp >= WARP_V ? 1 : 0, turn = warp - (which ? WARP_V : WARP_K), stages = which ? V_STAGES : k_stages;
+    const int* table = a.block_table + (size_t)table_of * a.max_pages;
+    const uint32_t full0 = which ? v_full0 : k_full0, empty0 = which ? v_empty0 : k_empty0;
+    auto lookup = [&](int j) {  // the page of this lane's 16 keys of tile j (-2: none that the item reads)
+      const int pos = lo + j * BN + lane * 16;
+      return lane < BN / 16 && j < tiles && pos < hi ? table[pos / a.page_size] : -2;
+    };
+    bool ok = true;
+    int page_cur = lookup(turn);
+    for (int j = turn; j < tiles; j += FEEDERS) {
+      const int page_next = lookup(j + FEEDERS), s = j % stages, pos = lo + j * BN + lane * 16;
+      if (lane == 0 && j >= stages) ok = mbar_wait(empty0 + 8 * s, ((j / stages) & 1) ^ 1, abort_flag);
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+      if (!ok) break;
+      bool load = page_cur != -2;
+      if (load && (page_cur < 0 || page_cur >= a.num_pages)) atomicOr(a.err, OMNIA_ERR_PAGE), load = false;
+      const uint32_t loaded = __ballot_sync(0xffffffffu, load);
+      const int mine = load ? ((page_cur * 2 + which) * a.nkv + kvh) * a.page_size + pos % a.page_size : 0;
+      int y[BN / 16];
+#pragma unroll
+      for (int x = 0; x < BN / 16; ++x) y[x] = __shfl_sync(0xffffffffu, mine, x);
+      if (omnia_elect_one()) {
+        mbar_expect_tx(full0 + 8 * s, __popc(loaded) * DH * BOX_BYTES);
+        const uint32_t dst = smem_u32((which ? v_s : k_s) + s * TILE_BYTES);
+#pragma unroll
+        for (int x = 0; x < BN / 16; ++x)
+          if ((loaded >> x) & 1u)
+#pragma unroll
+            for (int half = 0; half < DH; ++half)
+              tma_load_2d(dst + half * HALF_BYTES + x * BOX_BYTES, &map_kv, full0 + 8 * s, half * 64, y[x]);
+      }
+      __syncwarp();
+      issued = j;
+      page_cur = page_next;
+    }
+  } else if (warp >= WARP_MMA) {
+    // ---- issuer of a slot's products -----------------------------------------------------------------------------------
+    const int slot = warp - WARP_MMA;
+    if (tiles > 0 && omnia_elect_one()) {
+      constexpr uint32_t instr_s = idesc(BM, BN, false), instr_o = idesc(BM, D, true);
+      const uint64_t q_desc = desc_k_major(smem_u32(q_s + (turns ? 0 : slot) * TILE_BYTES));
+      const uint32_t s_tmem = tmem_base + slot * BN, o_tmem = tmem_base + O_COL + slot * D;
+      uint32_t accumulate = 0;
+      bool ok = mbar_wait(q_full, 0, abort_flag);
+      const int step = turns ? 2 : 1;
+      for (int j = turns ? slot : 0, t = 0; j < tiles && ok; j += step, ++t) {
+        const int ks = j % k_stages, vs = j % V_STAGES;
+        // The score tile is free: the product that read P from it is done.
+        ok = mbar_wait(k_full0 + 8 * ks, (j / k_stages) & 1, abort_flag) &&
+             (t == 0 || mbar_wait(o_done0 + 8 * slot, (t & 1) ^ 1, abort_flag));
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint64_t k_desc = desc_k_major(smem_u32(k_s + ks * TILE_BYTES));
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk)
+          umma(s_tmem, q_desc + (((kk / 4) * HALF_BYTES + (kk % 4) * 32) >> 4), k_desc + (((kk / 4) * HALF_BYTES + (kk % 4) * 32) >> 4), instr_s,
+               kk != 0);
+        umma_commit(s_full0 + 8 * slot);
+        umma_commit(k_empty0 + 8 * ks);
+        ok = mbar_wait(v_full0 + 8 * vs, (j / V_STAGES) & 1, abort_flag) && mbar_wait(p_full0 + 8 * slot, t & 1, abort_flag);
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint64_t v_desc = desc_mn_major(smem_u32(v_s + vs * TILE_BYTES), HALF_BYTES);
+        const int groups = min(BN, hi - lo - j * BN + 15) / 16;  // boxes that were loaded: the rest of the stage is stale
+        for (int kk = 0; kk < groups; ++kk) {
+          // P: 16 keys are eight columns of packed pairs, in the place of those keys' first eight scores
+          umma_ts(o_tmem, s_tmem + kk * 16, v_desc + ((kk * BOX_BYTES) >> 4), instr_o, accumulate);
+          accumulate = 1;
+        }
+        umma_commit(o_done0 + 8 * slot);
+        umma_commit(v_empty0 + 8 * vs);
+      }
+    }
+  } else {
+    // ---- softmax: a thread a row of its slot -----------------------------------------------------------------------------
+    const int slot = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;
+    auto place = [&](int r, int& request, int& head) {
+      request = members[first_member + (row0 + r) / GROUP];
+      head = kvh * GROUP + (row0 + r) % GROUP;
+    };
+    // The rows' queries, 16 bytes a load, into the swizzled tiles (16-byte pieces of a row exchanged by the row's number).
+    if (tiles > 0) {
+      const bf16* q = (const bf16*)a.q;
+      const int first_row = turns ? 0 : slot * SLOT_ROWS;
+      unsigned char* tile = q_s + (turns ? 0 : slot) * TILE_BYTES;
+      constexpr int PIECES = D / 8;
+      for (int i = turns ? threadIdx.x : threadIdx.x & 127; i < BM * PIECES; i += turns ? 256 : 128) {
+        const int r = i / PIECES, piece = i % PIECES;
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        if (r < SLOT_ROWS && first_row + r < rows) {
+          int request, head;
+          place(first_row + r, request, head);
+          v = *reinterpret_cast<const uint4*>(q + ((size_t)a.cu_seqlens[request] * a.nq + head) * D + piece * 8);
+        }
+        *reinterpret_cast<uint4*>(tile + (piece / 8) * HALF_BYTES + r * 128 + (((piece % 8) ^ (r & 7)) << 4)) = v;
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      mbar_arrive(q_full);
+    }
+    const int my_row = turns ? row : slot * SLOT_ROWS + row;   // among the item's rows
+    const bool live = row < SLOT_ROWS && my_row < rows;
+    const uint32_t lane_field = (uint32_t)(quarter * 32) << 16;
+    const uint32_t s_addr = tmem_base + lane_field + slot * BN, o_addr = tmem_base + lane_field + O_COL + slot * D;
+    const bool capped = a.softcap > 0.f;
+    const float pre = capped ? a.scale / a.softcap : 1.f, cap = a.softcap, sl2 = capped ? LOG2E : a.scale * LOG2E;
+    float m = -INFINITY, l = 0.f;  // in units of scores
+    bool ok = true;
+    int done = 0;
+    for (int j = turns ? slot : 0; j < tiles; j += turns ? 2 : 1, ++done) {
+      ok = __all_sync(0xffffffffu, mbar_wait(s_full0 + 8 * slot, done & 1, abort_flag));
+      if (!ok) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const int seen = min(BN, hi - lo - j * BN);  // keys of this tile; the columns beyond hold whatever the stage held
+      float tile_max = -INFINITY;
+#pragma unroll 1
+      for (int c = 0; c < BN; c += 32) {
+        uint32_t v[32];
+        tmem_load32(s_addr + c, v);
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        if (c + 32 <= seen) {
+          float part4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int i = 0; i < 32; ++i) part4[i & 3] = fmaxf(part4[i & 3], __uint_as_float(v[i]));
+          tile_max = fmaxf(tile_max, fmaxf(fmaxf(part4[0], part4[1]), fmaxf(part4[2], part4[3])));
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (c + i < seen) tile_max = fmaxf(tile_max, __uint_as_float(v[i]));
+        }
+      }
+      if (capped) tile_max = cap * tanhf(tile_max * pre);  // (it rises with the score)
+      float alpha = 1.f;
+      if (tile_max > m) {
+        if (m == -INFINITY) {
+          m = tile_max;
+        } else if ((tile_max - m) * sl2 > RESCALE_STEP) {
+          alpha = fast_exp2((m - tile_max) * sl2);
+          l *= alpha;
+          m = tile_max;
+        }
+      }
+      if (done > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+        // (The products so far are done: the issuer waited for them before it issued these scores.)
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+          uint32_t o[32];
+          tmem_load32(o_addr + c, o);
+          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+          tmem_store32(o_addr + c, o);
+        }
+      }
+      const float offset = m == -INFINITY ? 0.f : m * sl2;
+      float sums[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+      for (int c = 0; c < BN; c += 32) {
+        uint32_t v[32], packed[16];
+        tmem_load32(s_addr + c, v);
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        if (capped)
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(cap * tanhf(__uint_as_float(v[i]) * pre));
+        const int left = seen - c;
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+          float p0 = fast_exp2(fmaf(__uint_as_float(v[i]), sl2, -offset)), p1 = fast_exp2(fmaf(__uint_as_float(v[i + 1]), sl2, -offset));
+          if (left < 32) p0 = i < left ? p0 : 0.f, p1 = i + 1 < left ? p1 : 0.f;
+          sums[(i >> 1) & 3] += p0 + p1;
+          packed[i / 2] = pack_bf16(p0, p1);
+        }
+        tmem_store8(s_addr + c, packed);
+        tmem_store8(s_addr + c + 16, packed + 8);
+      }
+      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+      l += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+      if (seen & 15) {
+        // The last box reaches past the last key. Its rows of V beyond get no weight, but what they hold need not be a number
+        // (0 x NaN is NaN): they are cleared once the stage has landed, by both slots where both read it.
+        const int vs = j % V_STAGES;
+        ok = __all_sync(0xffffffffu, mbar_wait(v_full0 + 8 * vs, (j / V_STAGES) & 1, abort_flag));
+        if (!ok) break;
+        const int r1 = (seen + 15) & ~15;
+        for (int i = row; i < (r1 - seen) * DH * 8; i += BM) {
+          const int piece = i & 7, h = (i >> 3) % DH, r = seen + (i >> 3) / DH;
+          *reinterpret_cast<uint4*>(v_s + vs * TILE_BYTES + h * HALF_BYTES + r * 128 + piece * 16) = make_uint4(0u, 0u, 0u, 0u);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      }
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      mbar_arrive(p_full0 + 8 * slot);
+    }
+    // ---- the slot's piece: maximum (log2 units), sum, accumulator ---------------------------------------------------------
+    if (ok && done > 0) ok = __all_sync(0xffffffffu, mbar_wait(o_done0 + 8 * slot, (done - 1) & 1, abort_flag));
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const float top = m == -INFINITY ? -INFINITY : m * sl2;
+    const int places = a.max_parts + a.max_chunks;
+    size_t at = 0;
+    if (live) {
+      int request, head;
+      place(my_row, request, head);
+      at = ((size_t)request * a.nq + head) * places + part;
+    }
+    if (!turns) {
+      if (ok && live) a.part_ml[2 * at] = top, a.part_ml[2 * at + 1] = l;
+#pragma unroll 1
+      for (int c = 0; ok && c < D; c += 32) {
+        uint32_t o[32];
+        tmem_load32(o_addr + c, o);
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        if (live)
+#pragma unroll
+          for (int i = 0; i < 32; i += 4)
+            *reinterpret_cast<uint4*>(a.part_o + at * D + c + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+      }
+    } else {
+      // Both slots' states of a row become one: each slot finishes half of the dims, and gives the other the rest by way of the
+      // K ring, which nobody reads any more (both slots' last products are done once both are past the barrier; the
+      // loads have all landed, since products have read them). A slot without a tile has nothing in its accumulator.
+      row_ml[(slot * BM + row) * 2] = top, row_ml[(slot * BM + row) * 2 + 1] = l;
+      softmax_sync();
+      const float other_top = row_ml[((slot ^ 1) * BM + row) * 2], other_l = row_ml[((slot ^ 1) * BM + row) * 2 + 1];
+      const float both = fmaxf(top, other_top);
+      const float w = top == -INFINITY ? 0.f : fast_exp2(top - both), other_w = other_top == -INFINITY ? 0.f : fast_exp2(other_top - both);
+      constexpr int HALF = D / 2;
+      float* give = reinterpret_cast<float*>(k_s);  // [2][HALF][128]: dim after dim, so a warp's rows lie side by side
+      if (done > 0 && ok) {
+#pragma unroll 1
+        for (int c = 0; c < HALF; c += 32) {
+          uint32_t o[32];
+          tmem_load32(o_addr + (slot ^ 1) * HALF + c, o);
+          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+          for (int i = 0; i < 32; ++i) give[(slot * HALF + c + i) * BM + row] = __uint_as_float(o[i]);
+        }
+      } else {
+        for (int i = 0; i < HALF; ++i) give[(slot * HALF + i) * BM + row] = 0.f;
+      }
+      softmax_sync();
+      if (ok && live) {
+        if (slot == 0) a.part_ml[2 * at] = both, a.part_ml[2 * at + 1] = l * w + other_l * other_w;
+      }
+#pragma unroll 1
+      for (int c = 0; ok && c < HALF; c += 32) {
+        uint32_t o[32];
+        tmem_load32(o_addr + slot * HALF + c, o);
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        if (live) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) {
+            float y[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              y[e] = (done > 0 ? __uint_as_float(o[i + e]) * w : 0.f) + give[((slot ^ 1) * HALF + c + i + e) * BM + row] * other_w;
+            *reinterpret_cast<float4*>(a.part_o + at * D + slot * HALF + c + i) = make_float4(y[0], y[1], y[2], y[3]);
+          }
+        }
+      }
+    }
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (*abort_flag && warp >= WARP_K && lane == 0) {
+    // Given up: what this warp has asked for must land before the block's shared memory goes away. (Its last copies, one a stage; a
+    // stage that the ring's other warp has filled since reads as not complete, so the wait is short.)
+    const int stages = warp >= WARP_V ? V_STAGES : k_stages;
+    const uint32_t full0 = warp >= WARP_V ? v_full0 : k_full0;
+    for (int j = issued; j >= 0 && j > issued - stages; j -= FEEDERS)
+      for (uint32_t i = 0; i < WAIT_LIMIT / 1024 && !mbar_try(full0 + 8 * (j % stages), (j / stages) & 1); ++i) {
+      }
+  }
+  if (warp == WARP_MMA) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS));
+  if (threadIdx.x == 0 && *abort_flag) atomicOr(a.err, OMNIA_ERR_TIMEOUT);
+}
+
+// ---- host side -------------------------------------------------------------------------------
+
+// The pieces of all items. Pages [num_pages, 2, nkv, page_size, D], page_size a multiple of 16; q [tokens, nq, D]; an item has at most
+// 2 * (128 / GROUP) * GROUP rows, its first key is a multiple of 16.
+extern "C" int omnia_shared_pieces_tc(const SharedAttention* given, cudaStream_t stream) {
+  const SharedAttention a = *given;
+  if (a.items == 0) return 0;
+  if (a.items < 0 || a.requests < 1 || a.members < 1 || a.nq != a.nkv * GROUP || a.d != D || a.dv != D || a.page_size < 16 || a.page_size % 16 ||
+      a.max_pages < 1 || a.num_pages < 1 || ((uintptr_t)a.q & 15) || ((uintptr_t)a.k_pages & 15) || ((uintptr_t)a.part_o & 15) || a.softcap < 0.f ||
+      (long long)a.num_pages * 2 * a.nkv * a.page_size > 0x7fffffffLL)
+    return (int)cudaErrorInvalidValue;
+  EncodeTiled encode = encode_tiled();
+  if (encode == nullptr) return (int)cudaErrorNotSupported;
+  CUtensorMap map_kv;
+  const cuuint64_t dims[2] = {(cuuint64_t)D, (cuuint64_t)a.num_pages * 2 * a.nkv * a.page_size};
+  const cuuint64_t strides[1] = {(cuuint64_t)D * 2};
+  const cuuint32_t box[2] = {64, 16}, elem[2] = {1, 1};
+  if (encode(&map_kv, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(a.k_pages), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+    return (int)cudaErrorInvalidValue;
+  constexpr size_t smem = TILES * (size_t)TILE_BYTES + 256 + 4 * BM * sizeof(float);
+  static bool configured[64] = {};
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) return (int)cudaErrorInvalidDevice;
+  if (!configured[device]) {
+    const cudaError_t e = cudaFuncSetAttribute(shared_pieces_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return (int)e;
+    configured[device] = true;
+  }
+  launch_pdl(shared_pieces_tc_kernel, dim3(a.items), THREADS, smem, stream, map_kv, a);
+  return OMNIA_LAUNCH_RESULT();
+}

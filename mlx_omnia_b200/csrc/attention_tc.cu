@@ -29,6 +29,8 @@
 // softcap * tanh(s / softcap) ahead of the softmax).
 // Compiled with -DMAPS=2, two neighbouring query heads are the two maps of one head of differential
 // attention, and what is written is their difference (see MapDifference), [tokens, nq / 2, dv].
+// Compiled with -DSHARED=1, the decode kernel takes only the positions that a request does not share with others, and merges its
+// partials behind those of the shared ones (attention_shared.cuh); the file then holds that one entry point and no other.
 #include "common.cuh"
 
 #include <type_traits>
@@ -41,6 +43,12 @@
 #endif
 #ifndef MAPS
 #define MAPS 1
+#endif
+#ifndef SHARED
+#define SHARED 0
+#endif
+#if SHARED
+#include "attention_shared.cuh"
 #endif
 
 namespace {
@@ -609,7 +617,11 @@ attention_decode_kernel(const bf16* q, const bf16* __restrict__ pages,
                         int listed_before, int max_pages,
                         int num_pages, int nq, int nkv, int page_size, int window, float scale,
                         const FusedQK fused, int keep_first, const float* __restrict__ sink, int run, float softcap,
-                        const MapDifference difference, int beside, int* err) {
+                        const MapDifference difference, int beside, int* err
+#if SHARED
+                        , const int* shared, int max_parts
+#endif
+                        ) {
   // In the fused mode nothing up to the query fragments depends on the kernel before this one
   // (the lengths and tables were copied in before the step began, the keys and values of earlier
   // tokens were written in earlier steps), so the block's start and its first loads of the cache
@@ -633,6 +645,7 @@ attention_decode_kernel(const bf16* q, const bf16* __restrict__ pages,
     if (run > 0 && pos >= 0) first = max(first, pos - pos % run);
     return first;
   };
+  int parts = 0;  // partials of shared positions ahead of this request's own
   // What this block does: request `request` of the call, which is request `seq` of the step; keys lo..hi, the `chunk`th of
   // the request's `chunks` runs of keys, whose partials lie one after the other.
   int request = blockIdx.z, kvh = blockIdx.y, chunk = blockIdx.x, chunks = 0, seq = 0, pos = -1, first = 0, lo = 0, hi = -1;
@@ -652,6 +665,9 @@ attention_decode_kernel(const bf16* q, const bf16* __restrict__ pages,
     seq = seq_ids ? seq_ids[request] : request;
     pos = seq_lens[seq] - 1;
     first = first_key(pos);
+#if SHARED
+    first = max(first, shared[seq]), parts = min(shared[gridDim.z + seq], max_parts);  // (all of the step's requests: no index list)
+#endif
     const int c0 = first / chunk_keys;  // blocks count from the first chunk in sight: a window needs a window's worth of them
     lo = max(first, (c0 + chunk) * chunk_keys), hi = min(pos, (c0 + chunk + 1) * chunk_keys - 1);
     if (pos < 0 || lo > hi) {
@@ -659,6 +675,9 @@ attention_decode_kernel(const bf16* q, const bf16* __restrict__ pages,
       return;
     }
     chunks = pos / chunk_keys - c0 + 1;
+#if SHARED
+    max_chunks += max_parts;  // (of the partials' places, from here on)
+#endif
     part_o += (size_t)request * nq * max_chunks * D, part_ml += (size_t)request * nq * max_chunks * 2;
   }
   // The chunk that holds the window's first key also takes the kept first positions below the
@@ -906,7 +925,7 @@ attention_decode_kernel(const bf16* q, const bf16* __restrict__ pages,
   for (int r = 0; r < 2; ++r) {
     const int row = (lane >> 2) + 8 * r;
     if (row >= GROUP) continue;
-    const size_t slot = (size_t)(kvh * GROUP + row) * max_chunks + chunk;
+    const size_t slot = (size_t)(kvh * GROUP + row) * max_chunks + parts + chunk;
     float* dst = WARPS == 1 ? part_o + slot * D : merge + ((size_t)warp * GROUP + row) * (D + 2);
 #pragma unroll
     for (int j = 0; j < NT_O; ++j) {
@@ -943,7 +962,7 @@ attention_decode_kernel(const bf16* q, const bf16* __restrict__ pages,
         sum += src[w * APART + D + 1] * weight;
         acc += src[w * APART + dim] * weight;
       }
-      const size_t slot = (size_t)(kvh * GROUP + row) * max_chunks + chunk;
+      const size_t slot = (size_t)(kvh * GROUP + row) * max_chunks + parts + chunk;
       part_o[slot * D + dim] = acc;
       if (dim == 0) {
         part_ml[slot * 2] = top;
@@ -971,6 +990,8 @@ attention_decode_kernel(const bf16* q, const bf16* __restrict__ pages,
   }
   OMNIA_TRACE_BLOCK(6);
   if (ticket != chunks - 1) return;
+  if (SHARED && beside) pdl_wait();  // the shared positions' partials come from the kernel that this one runs beside
+  chunks += parts;
   // Two heads at a time (their loads travel together; one at a time where a head's rows would not
   // fit in registers twice), then the odd one.
   constexpr int TOGETHER = MAPS == 2 || (D <= 128 && GROUP > 1) ? 2 : 1;
@@ -990,11 +1011,12 @@ attention_decode_kernel(const bf16* q, const bf16* __restrict__ pages,
   }
   if (threadIdx.x == 0) *counter = 0;  // for the next launch
   OMNIA_TRACE_BLOCK(7);
-  if (beside) pdl_wait();
+  if (beside && !SHARED) pdl_wait();
 }
 
 // ---------------------------------------------------------------------------------------
 
+#if !SHARED
 extern "C" int omnia_attention_tc_info(int* head_dim, int* group, int* tokens_per_block) {
   *head_dim = HEAD_DIM;
   *group = GROUP;
@@ -1034,11 +1056,15 @@ typedef void (*DecodeKernel)(const bf16*, const bf16*, const int*, const int*, c
                              int, bf16*, int, int, const DecodePiece*, int, int, int, int, int, int, int, int, float, const FusedQK, int, const float*, int, float,
                              const MapDifference, int, int*);
 
+#endif  // !SHARED
+
 // Shared memory of an SM, the most a block may ask for, and what a block costs beside its dynamic
 // part (the system's kilobyte and the kernel's static arrays). Both decode entry points allow the
 // kernels the same dynamic size, so neither undoes the other's setting.
-constexpr size_t SM_SHARED = 228 * 1024, BLOCK_MOST = 227 * 1024, BLOCK_OVERHEAD = 1024 + 5 * 1024;
+[[maybe_unused]] constexpr size_t SM_SHARED = 228 * 1024;
+constexpr size_t BLOCK_MOST = 227 * 1024, BLOCK_OVERHEAD = 1024 + 5 * 1024;
 
+#if !SHARED
 // proj non-null selects the fused mode: the kernel first does the step's QK-norm (eps < 0: none),
 // rotation (inv_freq: head_dim / 2 inverse frequencies, or null) and cache write from the
 // projected rows [tokens, stride] with q, k, v heads at q_col, k_col, v_col, and q is not read.
@@ -1213,3 +1239,47 @@ extern "C" int omnia_attention_decode_tc_static(const void* q, const void* pages
   if (e != cudaSuccess) snprintf(static_error, sizeof static_error, "launch: %s", cudaGetErrorString(e));
   return (int)e;
 }
+
+#else  // SHARED
+
+// Attention of a step of single tokens over what each request holds beyond its shared positions, and the merge with the shared
+// positions' partials (attention_shared_tc.cu, the launch before this one where `items` is not zero): chunks of chunk_keys keys at fixed
+// positions, `warps` warps (1 or 4) a block. tickets [requests, nkv] are zero and left so. All requests of the step, rows of the
+// call's head size and group.
+extern "C" int omnia_attention_decode_shared(const SharedAttention* given, int* tickets, int warps, cudaStream_t stream) {
+  const SharedAttention a = *given;
+  if (a.requests == 0) return 0;
+  if (MAPS != a.maps || (MAPS == 2 && (a.gate != nullptr || a.sink != nullptr || a.difference.dv < 1 || a.difference.dv > D)))
+    return (int)cudaErrorInvalidValue;
+  if (a.requests < 0 || a.requests > 65535 || a.nkv < 1 || a.nq != a.nkv * GROUP || a.d != D || a.dv != D || a.chunk_keys <= 0 || a.chunk_keys % DECODE_BN != 0 ||
+      a.max_chunks < 1 || a.max_parts < 0 || a.max_pages < 1 || a.num_pages < 1 || a.page_size < 1 || a.softcap < 0.f || (warps != 1 && warps != 4))
+    return (int)cudaErrorInvalidValue;
+  const int sms = omnia_sm_count();
+  const long long blocks = (long long)a.max_chunks * a.nkv * a.requests;
+  const bool deep = warps == 4 && blocks <= sms && (size_t)(8 * 2 * DECODE_BN) * ROW * sizeof(bf16) <= BLOCK_MOST - BLOCK_OVERHEAD;
+  const size_t smem = (size_t)((warps == 1 ? DECODE_STAGES : deep ? 8 : 4) * 2 * DECODE_BN) * ROW * sizeof(bf16);
+  static bool configured[64] = {};
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) return (int)cudaErrorInvalidDevice;
+  const auto kernel = a.softcap > 0.f ? (warps == 1 ? attention_decode_kernel<1, DECODE_STAGES, true>
+                                                    : deep ? attention_decode_kernel<4, 2, true> : attention_decode_kernel<4, 1, true>)
+                                      : (warps == 1 ? attention_decode_kernel<1, DECODE_STAGES, false>
+                                                    : deep ? attention_decode_kernel<4, 2, false> : attention_decode_kernel<4, 1, false>);
+  if (!configured[device]) {
+    const decltype(kernel) all[] = {attention_decode_kernel<1, DECODE_STAGES, false>, attention_decode_kernel<1, DECODE_STAGES, true>,
+                                    attention_decode_kernel<4, 1, false>, attention_decode_kernel<4, 1, true>,
+                                    attention_decode_kernel<4, 2, false>, attention_decode_kernel<4, 2, true>};
+    for (const auto each : all) {
+      const cudaError_t e = cudaFuncSetAttribute(each, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(BLOCK_MOST - BLOCK_OVERHEAD));
+      if (e != cudaSuccess) return (int)e;
+    }
+    configured[device] = true;
+  }
+  launch_pdl(kernel, dim3(a.max_chunks, a.nkv, a.requests), warps * 32, smem, stream, (const bf16*)a.q, (const bf16*)a.k_pages,
+             a.block_table, a.cu_seqlens, a.seq_lens, (const int*)nullptr, a.part_o, a.part_ml, tickets, (const bf16*)a.gate, a.gate_stride,
+             (bf16*)a.out, a.chunk_keys, a.max_chunks, (const DecodePiece*)nullptr, 0, 0, a.max_pages, a.num_pages, a.nq, a.nkv,
+             a.page_size, 0, a.scale, FusedQK{}, 0, a.sink, 0, a.softcap, a.difference, a.items > 0 ? 1 : 0, a.err, a.plan, a.max_parts);
+  return OMNIA_LAUNCH_RESULT();
+}
+
+#endif

@@ -772,22 +772,33 @@ def _shared_attention(q: torch.Tensor, kv: KVView, step: StepContext, scale: flo
     k_ptr, v_ptr, page_stride, nkv, _, dv = kv_layout(kv)
     group, sms, n = nq // nkv, sm_count(device), step.num_seqs
     own = width_bucket(-(-_own_longest(step) // kv.page_size)) * kv.page_size
-    chunk, _ = decode_plan(n, nkv, own, sms)
-    plan = shared_plan(shared_shape(step.shared), group, nkv, SHARED_ROWS, SHARED_TILE, 4, 4 * sms)
-    key = ("shared", group, nkv, SHARED_ROWS, SHARED_TILE, plan)
-    listed = _step_list(step, key, lambda st: shared_list(st, plan, group, nkv, SHARED_ROWS, SHARED_TILE), device)
-    max_parts, max_chunks = max(plan.parts), -(-own // chunk)
-    part_o, part_ml = _step_buffers(step, device, {
-        "attention_part_o": (n * nq * (max_parts + max_chunks) * dv, torch.float32, False),
-        "attention_part_ml": (n * nq * (max_parts + max_chunks) * 2, torch.float32, False)})
+    chunk, warps = decode_plan(n, nkv, own, sms)
+    tensor_cores = dv == d and scale > 0 and tcgen05_attention_supported(q.dtype, nq, nkv, d, kv.page_size)
+    rows, tile, least, places = (2 * (128 // group) * group, 128, 1, sms) if tensor_cores else (SHARED_ROWS, SHARED_TILE, 4, 4 * sms)
+    plan = shared_plan(shared_shape(step.shared), group, nkv, rows, tile, least, places)
+    listed = _step_list(step, ("shared", group, nkv, rows, tile, plan), lambda st: shared_list(st, plan, group, nkv, rows, tile), device)
+    # (The tensor-core kernel's chunks lie at fixed positions, so a request's may be one more than its positions fill.)
+    max_parts, max_chunks = max(plan.parts), -(-own // chunk) + int(tensor_cores)
+    places = n * nq * (max_parts + max_chunks)
+    part_o, part_ml = _step_buffers(step, device, {"attention_part_o": (places * dv, torch.float32, False),
+                                                   "attention_part_ml": (places * 2, torch.float32, False)})
     last = _MapDifferenceArgs(0.0, 0.0, 0.0, 0) if difference is None else \
         _MapDifferenceArgs(difference.lam, difference.eps, difference.factor, difference.dv)
     args = _SharedArgs(_ptr(q), k_ptr, v_ptr, gate_ptr, _ptr(out), _ptr(kv.block_table), _ptr(step.cu_seqlens), _ptr(step.seq_lens), _ptr(listed),
                        _ptr(sink), _ptr(part_o), _ptr(part_ml), _ptr(error_word(device)), page_stride, n, plan.members, plan.items, max_parts, chunk,
                        max_chunks, gate_stride, kv.block_table.shape[1], kv.pages.shape[0], nq, nkv, d, dv, kv.page_size,
                        1 if difference is None else 2, scale, softcap, last)
-    fn = _function("attention_shared", "omnia_shared_attention", [c_void_p, c_int, c_void_p])
-    _check(fn(ctypes.byref(args), _code(q.dtype), _stream()), "shared_attention")
+    if not tensor_cores:
+        fn = _function("attention_shared", "omnia_shared_attention", [c_void_p, c_int, c_void_p])
+        _check(fn(ctypes.byref(args), _code(q.dtype), _stream()), "shared_attention")
+        return out
+    tickets, = _step_buffers(step, device, {"attention_tickets": (n * nkv, torch.int32, True)})
+    defines = {"HEAD_DIM": d, "GROUP": group}
+    fn = _function("attention_shared_tc", "omnia_shared_pieces_tc", [c_void_p, c_void_p], defines)
+    _check(fn(ctypes.byref(args), _stream()), "shared_pieces")
+    fn = _function("attention_tc", "omnia_attention_decode_shared", [c_void_p, c_void_p, c_int, c_void_p],
+                   defines | {"SHARED": 1} | ({} if difference is None else {"MAPS": 2}))
+    _check(fn(ctypes.byref(args), _ptr(tickets), warps, _stream()), "attention_decode_shared")
     return out
 
 
