@@ -9,12 +9,12 @@
 // softmax chains that know nothing of one another: each has a score tile of 128 columns and an accumulator in tensor memory, a
 // warp that issues its products and four warps of a thread a row:
 //   S = Q K^T   tcgen05.mma (M 128, N 128) over the head size
-//   softmax     two passes over the scores, 32 at a time; P, rounded to bfloat16, takes the scores' place; the exponent's
+//   softmax     a row's 128 scores in registers at once; P, rounded to bfloat16, takes the scores' place; the exponent's
 //               offset follows a row's maximum lazily, and only then is the accumulator rescaled
 //   O += P V    tcgen05.mma (M 128, N head size), P read from tensor memory
 // One chain alone would wait for its own products and loads half of the time; two fill each other's gaps. With more
 // than 128 rows a slot has half of them and both see every tile of keys; with fewer both hold the same rows and take the tiles
-// in turn, and the two states are brought together at the end. The rows are gathered from wherever the requests' tokens lie.
+// in turn, and the two states are brought together at the end. The rows are gathered from wherever the requests' tokens lie, by TMA.
 // Keys and values come by TMA, a box of 16 keys x 64 dims, into rings of stages of 128 keys.
 #ifndef HEAD_DIM
 #define HEAD_DIM 128
@@ -39,19 +39,42 @@ constexpr int SLOT_ROWS = BM / GROUP * GROUP;
 // slot has yet to wait for.
 constexpr int TILES = 7, V_STAGES = 2, K_STAGES = 4;  // (three for keys where there are two tiles of rows)
 constexpr int SOFTMAX_THREADS = 256;     // warps 0-3 slot 0, 4-7 slot 1
-constexpr int WARP_MMA = 8, WARP_K = 10, WARP_V = 12, FEEDERS = 2;  // one issuer a slot; two warps feed each ring in turns
-constexpr int THREADS = 32 * 14;
+constexpr int SLOT_MEMBERS = BM / GROUP, Q_MEMBERS = 8;  // requests of a slot's rows, of a box of queries
+constexpr int WARP_MMA = 8, WARP_K = 10, WARP_V = 12, WARP_Q = 14, FEEDERS = 2;  // one issuer a slot; two warps feed each ring in turns
+constexpr int THREADS = 512;             // (a warp has nothing to do)
+// Registers a thread, by warpgroup: the slots' softmax holds a row's 128 scores. Together they are what the block is launched with.
+constexpr int SLOT_REGS = 192, OTHER_REGS = 64;
+static_assert(2 * SLOT_REGS + 2 * OTHER_REGS == 4 * (65536 / THREADS), "a register split's sum is the launch's");
 constexpr uint32_t HALF_BYTES = 128 * 128;   // 128 rows of 128 bytes
 constexpr uint32_t TILE_BYTES = DH * HALF_BYTES;
 constexpr uint32_t BOX_BYTES = 16 * 128;     // 16 keys x 64 dims
 constexpr uint32_t TMEM_COLS = 512, O_COL = 2 * BN;  // two score tiles, then two accumulators
 
+// mbar_wait without a time to sleep for: a warp that asks for one wakes up later.
+__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  if (omnia_mbar_test(bar, parity)) return true;
+  for (uint32_t i = 0; i < WAIT_LIMIT; ++i) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if (done) return true;
+    if ((i & 63) == 63 && *abort_flag) return false;
+  }
+  *abort_flag = 1;
+  return false;
+}
 __device__ __forceinline__ void softmax_sync() { asm volatile("bar.sync 1, %0;" ::"n"(SOFTMAX_THREADS) : "memory"); }
 
 }  // namespace
 
 __global__ void __launch_bounds__(THREADS, 1)
-shared_pieces_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_constant__ SharedAttention a) {
+shared_pieces_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_constant__ CUtensorMap map_q,
+                        const __grid_constant__ CUtensorMap map_q8, const __grid_constant__ SharedAttention a) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   if (smem_u32(smem_raw) & 1023u) {  // the swizzled tiles need a base on 1024 bytes
     if (threadIdx.x == 0) atomicOr(a.err, OMNIA_ERR_TIMEOUT);
@@ -82,11 +105,11 @@ shared_pieces_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid
   unsigned char* k_s = v_s - k_stages * TILE_BYTES;
   const int tiles = rows < 1 ? 0 : (hi - lo + BN - 1) / BN;
   if (threadIdx.x == 0) {
-    mbar_init(q_full, SOFTMAX_THREADS);
+    mbar_init(q_full, 1);
     const int readers = turns ? 1 : 2;
     for (int s = 0; s < K_STAGES; ++s) mbar_init(k_full0 + 8 * s, 1), mbar_init(k_empty0 + 8 * s, readers);
     for (int s = 0; s < V_STAGES; ++s) mbar_init(v_full0 + 8 * s, 1), mbar_init(v_empty0 + 8 * s, readers);
-    for (int s = 0; s < 2; ++s) mbar_init(s_full0 + 8 * s, 1), mbar_init(p_full0 + 8 * s, BM), mbar_init(o_done0 + 8 * s, 1);
+    for (int s = 0; s < 2; ++s) mbar_init(s_full0 + 8 * s, 1), mbar_init(p_full0 + 8 * s, BM / 32), mbar_init(o_done0 + 8 * s, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -96,7 +119,34 @@ shared_pieces_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid
   const uint32_t tmem_base = *tmem_holder;
   int issued = -1;  // the last tile that this warp has asked for
 
-  if (warp >= WARP_K) {
+  if (warp >= WARP_MMA) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
+  if (warp > WARP_Q) {
+    // (nothing)
+  } else if (warp == WARP_Q) {
+    // ---- the rows' queries, a box the group's rows of a request x 64 dims, or of eight requests that are neighbours in the step (a box takes its
+    // issuer 40 ns). The rows of a tile that hold nothing are whatever was there: no other row learns of it. --------------------------------
+    const int count = rows / GROUP, first = first_member + row0 / GROUP;
+    if (tiles > 0) {
+      if (omnia_elect_one()) mbar_expect_tx(q_full, rows * DH * 128);
+      __syncwarp();
+      for (int m0 = 0; m0 < count; m0 += 32) {
+        const int some = min(32, count - m0), mine = lane < some ? a.cu_seqlens[members[first + m0 + lane]] : -1;  // tokens
+        const uint32_t follow = __ballot_sync(0xffffffffu, __shfl_down_sync(0xffffffffu, mine, 1) == mine + 1 && lane + 1 < some);
+        constexpr uint32_t ALL = (1u << (Q_MEMBERS - 1)) - 1;
+        for (int m = 0; m < some;) {
+          const int token = __shfl_sync(0xffffffffu, mine, m), member = m0 + m, slot = member / SLOT_MEMBERS, at = member % SLOT_MEMBERS;
+          const bool eight = m + Q_MEMBERS <= some && at + Q_MEMBERS <= SLOT_MEMBERS && ((follow >> m) & ALL) == ALL;
+          if (omnia_elect_one())
+#pragma unroll
+            for (int half = 0; half < DH; ++half)
+              tma_load_3d(smem_u32(q_s) + slot * TILE_BYTES + half * HALF_BYTES + at * GROUP * 128, eight ? &map_q8 : &map_q, q_full, half * 64,
+                          kvh * GROUP, token);
+          __syncwarp();
+          m += eight ? Q_MEMBERS : 1;
+        }
+      }
+    }
+  } else if (warp >= WARP_K) {
     // ---- producers: two warps a ring take turns with its stages; a lane looks up a box's page, one lane asks for the boxes ----
     const int which = warp >= WARP_V ? 1 : 0, turn = warp - (which ? WARP_V : WARP_K), stages = which ? V_STAGES : k_stages;
     const int* table = a.block_table + (size_t)table_of * a.max_pages;
@@ -109,7 +159,7 @@ shared_pieces_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid
     int page_cur = lookup(turn);
     for (int j = turn; j < tiles; j += FEEDERS) {
       const int page_next = lookup(j + FEEDERS), s = j % stages, pos = lo + j * BN + lane * 16;
-      if (lane == 0 && j >= stages) ok = mbar_wait(empty0 + 8 * s, ((j / stages) & 1) ^ 1, abort_flag);
+      if (lane == 0 && j >= stages) ok = wait_for(empty0 + 8 * s, ((j / stages) & 1) ^ 1, abort_flag);
       ok = __shfl_sync(0xffffffffu, ok, 0);
       if (!ok) break;
       bool load = page_cur != -2;
@@ -141,13 +191,13 @@ shared_pieces_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid
       const uint64_t q_desc = desc_k_major(smem_u32(q_s + (turns ? 0 : slot) * TILE_BYTES));
       const uint32_t s_tmem = tmem_base + slot * BN, o_tmem = tmem_base + O_COL + slot * D;
       uint32_t accumulate = 0;
-      bool ok = mbar_wait(q_full, 0, abort_flag);
+      bool ok = wait_for(q_full, 0, abort_flag);
       const int step = turns ? 2 : 1;
       for (int j = turns ? slot : 0, t = 0; j < tiles && ok; j += step, ++t) {
         const int ks = j % k_stages, vs = j % V_STAGES;
         // The score tile is free: the product that read P from it is done.
-        ok = mbar_wait(k_full0 + 8 * ks, (j / k_stages) & 1, abort_flag) &&
-             (t == 0 || mbar_wait(o_done0 + 8 * slot, (t & 1) ^ 1, abort_flag));
+        ok = wait_for(k_full0 + 8 * ks, (j / k_stages) & 1, abort_flag) &&
+             (t == 0 || wait_for(o_done0 + 8 * slot, (t & 1) ^ 1, abort_flag));
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const uint64_t k_desc = desc_k_major(smem_u32(k_s + ks * TILE_BYTES));
@@ -157,14 +207,16 @@ shared_pieces_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid
                kk != 0);
         umma_commit(s_full0 + 8 * slot);
         umma_commit(k_empty0 + 8 * ks);
-        ok = mbar_wait(v_full0 + 8 * vs, (j / V_STAGES) & 1, abort_flag) && mbar_wait(p_full0 + 8 * slot, t & 1, abort_flag);
+        ok = wait_for(v_full0 + 8 * vs, (j / V_STAGES) & 1, abort_flag) && wait_for(p_full0 + 8 * slot, t & 1, abort_flag);
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const uint64_t v_desc = desc_mn_major(smem_u32(v_s + vs * TILE_BYTES), HALF_BYTES);
         const int groups = min(BN, hi - lo - j * BN + 15) / 16;  // boxes that were loaded: the rest of the stage is stale
-        for (int kk = 0; kk < groups; ++kk) {
-          // P: 16 keys are eight columns of packed pairs, in the place of those keys' first eight scores
-          umma_ts(o_tmem, s_tmem + kk * 16, v_desc + ((kk * BOX_BYTES) >> 4), instr_o, accumulate);
+#pragma unroll
+        for (int kk = 0; kk < BN / 16; ++kk) {
+          if (kk >= groups) break;
+          // P: 16 keys are eight columns of packed pairs
+          umma_ts(o_tmem, s_tmem + kk * 8, v_desc + ((kk * BOX_BYTES) >> 4), instr_o, accumulate);
           accumulate = 1;
         }
         umma_commit(o_done0 + 8 * slot);
@@ -172,115 +224,107 @@ shared_pieces_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid
       }
     }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SLOT_REGS));
     // ---- softmax: a thread a row of its slot -----------------------------------------------------------------------------
     const int slot = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;
     auto place = [&](int r, int& request, int& head) {
       request = members[first_member + (row0 + r) / GROUP];
       head = kvh * GROUP + (row0 + r) % GROUP;
     };
-    // The rows' queries, 16 bytes a load, into the swizzled tiles (16-byte pieces of a row exchanged by the row's number).
-    if (tiles > 0) {
-      const bf16* q = (const bf16*)a.q;
-      const int first_row = turns ? 0 : slot * SLOT_ROWS;
-      unsigned char* tile = q_s + (turns ? 0 : slot) * TILE_BYTES;
-      constexpr int PIECES = D / 8;
-      for (int i = turns ? threadIdx.x : threadIdx.x & 127; i < BM * PIECES; i += turns ? 256 : 128) {
-        const int r = i / PIECES, piece = i % PIECES;
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (r < SLOT_ROWS && first_row + r < rows) {
-          int request, head;
-          place(first_row + r, request, head);
-          v = *reinterpret_cast<const uint4*>(q + ((size_t)a.cu_seqlens[request] * a.nq + head) * D + piece * 8);
-        }
-        *reinterpret_cast<uint4*>(tile + (piece / 8) * HALF_BYTES + r * 128 + (((piece % 8) ^ (r & 7)) << 4)) = v;
-      }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      mbar_arrive(q_full);
-    }
     const int my_row = turns ? row : slot * SLOT_ROWS + row;   // among the item's rows
     const bool live = row < SLOT_ROWS && my_row < rows;
     const uint32_t lane_field = (uint32_t)(quarter * 32) << 16;
     const uint32_t s_addr = tmem_base + lane_field + slot * BN, o_addr = tmem_base + lane_field + O_COL + slot * D;
     const bool capped = a.softcap > 0.f;
-    const float pre = capped ? a.scale / a.softcap : 1.f, cap = a.softcap, sl2 = capped ? LOG2E : a.scale * LOG2E;
-    float m = -INFINITY, l = 0.f;  // in units of scores
+    const float cap = a.softcap * LOG2E, twice = capped ? 2.f * a.scale / a.softcap * LOG2E : 0.f, unit = capped ? 1.f : a.scale * LOG2E;
+    float m = -INFINITY, l = 0.f;  // the row's offset (log2 units), its sum against it
     bool ok = true;
     int done = 0;
-    for (int j = turns ? slot : 0; j < tiles; j += turns ? 2 : 1, ++done) {
-      ok = __all_sync(0xffffffffu, mbar_wait(s_full0 + 8 * slot, done & 1, abort_flag));
-      if (!ok) break;
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const int seen = min(BN, hi - lo - j * BN);  // keys of this tile; the columns beyond hold whatever the stage held
-      float tile_max = -INFINITY;
-#pragma unroll 1
-      for (int c = 0; c < BN; c += 32) {
-        uint32_t v[32];
-        tmem_load32(s_addr + c, v);
-        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-        if (c + 32 <= seen) {
-          float part4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-          for (int i = 0; i < 32; ++i) part4[i & 3] = fmaxf(part4[i & 3], __uint_as_float(v[i]));
-          tile_max = fmaxf(tile_max, fmaxf(fmaxf(part4[0], part4[1]), fmaxf(part4[2], part4[3])));
-        } else {
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (c + i < seen) tile_max = fmaxf(tile_max, __uint_as_float(v[i]));
-        }
+    // The turn ahead of the first tile works on whatever tensor memory holds, and leaves it in the accumulator, which the first product
+    // overwrites: it fetches the code, a straight line of some thousand instructions that every launch finds cold, while the first
+    // tile is on its way (without it a block's first tile took 3 us).
+    const int step = turns ? 2 : 1, j0 = turns ? slot : 0;
+    for (int j = tiles > j0 ? j0 - step : tiles; j < tiles; j += step) {
+      const bool dry = j < j0;
+      if (!dry) {
+        ok = __all_sync(0xffffffffu, wait_for(s_full0 + 8 * slot, done & 1, abort_flag));
+        if (!ok) break;
       }
-      if (capped) tile_max = cap * tanhf(tile_max * pre);  // (it rises with the score)
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const int seen = dry ? BN : min(BN, hi - lo - j * BN);  // keys of this tile; the columns beyond hold whatever the stage held
+      // All of the row's scores at once: a load from tensor memory takes some 0.35 us to arrive.
+      float z[BN];
+      {
+        uint32_t raw[BN];
+#pragma unroll
+        for (int c = 0; c < BN; c += 32) tmem_load32(s_addr + c, raw + c);
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+        for (int c = 0; c < BN; ++c) z[c] = __uint_as_float(raw[c]);
+      }
+      if (seen < BN) {
+#pragma unroll
+        for (int c = 0; c < BN; ++c) z[c] = c < seen ? z[c] : -INFINITY;
+      }
+      if (capped) {  // c tanh(x) = c - 2 c / (1 + e^2x), in log2 units
+#pragma unroll
+        for (int c = 0; c < BN; ++c) z[c] = z[c] == -INFINITY ? z[c] : fmaf(-2.f * cap, fast_rcp(1.f + fast_exp2(z[c] * twice)), cap);
+      }
+      float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int c = 0; c < BN; ++c) tops[c & 3] = fmaxf(tops[c & 3], z[c]);
+      const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * unit;
+      // The offset follows the row's maximum lazily: what was summed is brought to a new one only when the scores have outgrown the old.
       float alpha = 1.f;
-      if (tile_max > m) {
+      if (top > m) {
         if (m == -INFINITY) {
-          m = tile_max;
-        } else if ((tile_max - m) * sl2 > RESCALE_STEP) {
-          alpha = fast_exp2((m - tile_max) * sl2);
+          m = top;
+        } else if (top - m > RESCALE_STEP) {
+          alpha = fast_exp2(m - top);
           l *= alpha;
-          m = tile_max;
+          m = top;
         }
       }
       if (done > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
         // (The products so far are done: the issuer waited for them before it issued these scores.)
 #pragma unroll 1
-        for (int c = 0; c < D; c += 32) {
-          uint32_t o[32];
-          tmem_load32(o_addr + c, o);
+        for (int c = 0; c < D; c += 8) {
+          uint32_t o[8];
+          tmem_load8(o_addr + c, o);
           asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-          tmem_store32(o_addr + c, o);
+          for (int i = 0; i < 8; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+          tmem_store8(o_addr + c, o);
         }
       }
-      const float offset = m == -INFINITY ? 0.f : m * sl2;
+      const float offset = m == -INFINITY ? 0.f : m;
       float sums[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 1
-      for (int c = 0; c < BN; c += 32) {
-        uint32_t v[32], packed[16];
-        tmem_load32(s_addr + c, v);
-        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-        if (capped)
+      // The weights, in pairs, take the place of the first half of the row's scores.
 #pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(cap * tanhf(__uint_as_float(v[i]) * pre));
-        const int left = seen - c;
+      for (int c0 = 0; c0 < BN; c0 += 64) {
+        uint32_t packed[32];
 #pragma unroll
-        for (int i = 0; i < 32; i += 2) {
-          float p0 = fast_exp2(fmaf(__uint_as_float(v[i]), sl2, -offset)), p1 = fast_exp2(fmaf(__uint_as_float(v[i + 1]), sl2, -offset));
-          if (left < 32) p0 = i < left ? p0 : 0.f, p1 = i + 1 < left ? p1 : 0.f;
-          sums[(i >> 1) & 3] += p0 + p1;
-          packed[i / 2] = pack_bf16(p0, p1);
+        for (int c = 0; c < 64; c += 2) {
+          const float p0 = fast_exp2(fmaf(z[c0 + c], unit, -offset)), p1 = fast_exp2(fmaf(z[c0 + c + 1], unit, -offset));
+          sums[c & 2] += p0, sums[(c & 2) + 1] += p1;
+          packed[c / 2] = pack_bf16(p0, p1);
         }
-        tmem_store8(s_addr + c, packed);
-        tmem_store8(s_addr + c + 16, packed + 8);
+        tmem_store32((dry ? o_addr : s_addr) + c0 / 2, packed);
       }
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+      if (dry) {
+        m = -INFINITY, l = 0.f;
+        continue;
+      }
       l += (sums[0] + sums[1]) + (sums[2] + sums[3]);
       if (seen & 15) {
         // The last box reaches past the last key. Its rows of V beyond get no weight, but what they hold need not be a number
         // (0 x NaN is NaN): they are cleared once the stage has landed, by both slots where both read it.
         const int vs = j % V_STAGES;
-        ok = __all_sync(0xffffffffu, mbar_wait(v_full0 + 8 * vs, (j / V_STAGES) & 1, abort_flag));
+        ok = __all_sync(0xffffffffu, wait_for(v_full0 + 8 * vs, (j / V_STAGES) & 1, abort_flag));
         if (!ok) break;
         const int r1 = (seen + 15) & ~15;
+#pragma unroll 1
         for (int i = row; i < (r1 - seen) * DH * 8; i += BM) {
           const int piece = i & 7, h = (i >> 3) % DH, r = seen + (i >> 3) / DH;
           *reinterpret_cast<uint4*>(v_s + vs * TILE_BYTES + h * HALF_BYTES + r * 128 + piece * 16) = make_uint4(0u, 0u, 0u, 0u);
@@ -288,12 +332,14 @@ shared_pieces_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-      mbar_arrive(p_full0 + 8 * slot);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(p_full0 + 8 * slot);
+      ++done;
     }
     // ---- the slot's piece: maximum (log2 units), sum, accumulator ---------------------------------------------------------
-    if (ok && done > 0) ok = __all_sync(0xffffffffu, mbar_wait(o_done0 + 8 * slot, (done - 1) & 1, abort_flag));
+    if (ok && done > 0) ok = __all_sync(0xffffffffu, wait_for(o_done0 + 8 * slot, (done - 1) & 1, abort_flag));
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    const float top = m == -INFINITY ? -INFINITY : m * sl2;
+    const float top = m;
     const int places = a.max_parts + a.max_chunks;
     size_t at = 0;
     if (live) {
@@ -393,6 +439,19 @@ extern "C" int omnia_shared_pieces_tc(const SharedAttention* given, cudaStream_t
   if (encode(&map_kv, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(a.k_pages), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
     return (int)cudaErrorInvalidValue;
+  // Queries [tokens, nq, D]: a box is the group's rows of one token, or of eight, x 64 dims.
+  CUtensorMap map_q, map_q8;
+  const cuuint64_t q_dims[3] = {(cuuint64_t)D, (cuuint64_t)a.nq, (cuuint64_t)a.requests};
+  const cuuint64_t q_strides[2] = {(cuuint64_t)D * 2, (cuuint64_t)a.nq * D * 2};
+  cuuint32_t q_box[3] = {64, GROUP, 1};
+  const cuuint32_t q_elem[3] = {1, 1, 1};
+  for (int tokens = 1; tokens <= Q_MEMBERS; tokens += Q_MEMBERS - 1) {
+    q_box[2] = tokens;
+    if (encode(tokens == 1 ? &map_q : &map_q8, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(a.q), q_dims, q_strides, q_box, q_elem,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+      return (int)cudaErrorInvalidValue;
+  }
   constexpr size_t smem = TILES * (size_t)TILE_BYTES + 256 + 4 * BM * sizeof(float);
   static bool configured[64] = {};
   int device = 0;
@@ -402,6 +461,6 @@ extern "C" int omnia_shared_pieces_tc(const SharedAttention* given, cudaStream_t
     if (e != cudaSuccess) return (int)e;
     configured[device] = true;
   }
-  launch_pdl(shared_pieces_tc_kernel, dim3(a.items), THREADS, smem, stream, map_kv, a);
+  launch_pdl(shared_pieces_tc_kernel, dim3(a.items), THREADS, smem, stream, map_kv, map_q, map_q8, a);
   return OMNIA_LAUNCH_RESULT();
 }

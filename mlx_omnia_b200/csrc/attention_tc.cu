@@ -1061,8 +1061,7 @@ typedef void (*DecodeKernel)(const bf16*, const bf16*, const int*, const int*, c
 // Shared memory of an SM, the most a block may ask for, and what a block costs beside its dynamic
 // part (the system's kilobyte and the kernel's static arrays). Both decode entry points allow the
 // kernels the same dynamic size, so neither undoes the other's setting.
-[[maybe_unused]] constexpr size_t SM_SHARED = 228 * 1024;
-constexpr size_t BLOCK_MOST = 227 * 1024, BLOCK_OVERHEAD = 1024 + 5 * 1024;
+constexpr size_t SM_SHARED = 228 * 1024, BLOCK_MOST = 227 * 1024, BLOCK_OVERHEAD = 1024 + 5 * 1024;
 
 #if !SHARED
 // proj non-null selects the fused mode: the kernel first does the step's QK-norm (eps < 0: none),
@@ -1257,7 +1256,7 @@ extern "C" int omnia_attention_decode_shared(const SharedAttention* given, int* 
   const int sms = omnia_sm_count();
   const long long blocks = (long long)a.max_chunks * a.nkv * a.requests;
   const bool deep = warps == 4 && blocks <= sms && (size_t)(8 * 2 * DECODE_BN) * ROW * sizeof(bf16) <= BLOCK_MOST - BLOCK_OVERHEAD;
-  const size_t smem = (size_t)((warps == 1 ? DECODE_STAGES : deep ? 8 : 4) * 2 * DECODE_BN) * ROW * sizeof(bf16);
+  size_t smem = (size_t)((warps == 1 ? DECODE_STAGES : deep ? 8 : 4) * 2 * DECODE_BN) * ROW * sizeof(bf16);
   static bool configured[64] = {};
   int device = 0;
   if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) return (int)cudaErrorInvalidDevice;
@@ -1274,6 +1273,11 @@ extern "C" int omnia_attention_decode_shared(const SharedAttention* given, int* 
       if (e != cudaSuccess) return (int)e;
     }
     configured[device] = true;
+  }
+  {  // (spread over the SMs, as the other entry point's blocks are: those that the kernel beside this one leaves)
+    const int left = sms - a.items > sms / 4 ? sms - a.items : sms / 4;
+    const size_t room = SM_SHARED / (size_t)((blocks + left - 1) / left);
+    if (room > smem + BLOCK_OVERHEAD) smem = (room > BLOCK_MOST ? BLOCK_MOST : room) - BLOCK_OVERHEAD;
   }
   launch_pdl(kernel, dim3(a.max_chunks, a.nkv, a.requests), warps * 32, smem, stream, (const bf16*)a.q, (const bf16*)a.k_pages,
              a.block_table, a.cu_seqlens, a.seq_lens, (const int*)nullptr, a.part_o, a.part_ml, tickets, (const bf16*)a.gate, a.gate_stride,

@@ -763,42 +763,95 @@ def _own_longest(step: StepContext) -> int:
     return max((n - starts.get(r, 0) for r, n in enumerate(step.seq_lens_host)), default=0)
 
 
-def _shared_attention(q: torch.Tensor, kv: KVView, step: StepContext, scale: float, gate_ptr, gate_stride: int, sink: torch.Tensor | None,
-                      softcap: float, difference: "MapDifference | None", out: torch.Tensor) -> torch.Tensor:
-    """`paged_attention` of a step whose requests share positions (`StepContext.shared`): a group's shared positions as pieces for all of its
-    rows, each request's own in chunks, both put together at the end."""
-    device = q.device
-    _, nq, d = q.shape
-    k_ptr, v_ptr, page_stride, nkv, _, dv = kv_layout(kv)
-    group, sms, n = nq // nkv, sm_count(device), step.num_seqs
+@dataclass
+class _SharedCall:
+    """What a step's layers of one cache layout tell the kernels alike, and the memory that this names."""
+
+    args: _SharedArgs
+    launch: Callable[[], int]
+    held: list[torch.Tensor]
+
+
+SHARED_TILE_NS, OWN_GBS = 1000, 4500
+"""What a tile of 128 shared keys takes a block of the tensor-core kernel, and the rate at which the decode kernel reads what requests hold of
+their own: how many SMs shared positions get follows from the two, since the kernels run beside one another."""
+
+
+def shared_size(shape: tuple[tuple[int, int], ...], group: int, nkv: int, block_rows: int, own_bytes: int, sms: int) -> int:
+    """Tiles of a piece of the tensor-core kernel: as many as one SM does in the time that all of them need for everything."""
+    tiles = sum(-(-count * group // block_rows) * nkv * -(-positions // 128) for positions, count in shape)
+    return max(1, -(-(tiles + own_bytes * sms // (OWN_GBS * SHARED_TILE_NS)) // sms))
+
+
+def _shared_call(step: StepContext, kv: KVView, nq: int, nkv: int, d: int, dv: int, dtype: torch.dtype, device: torch.device, positive: bool,
+                 maps: int) -> _SharedCall:
+    """Made once a step and layout; the layers' own pointers are filled in by every call. Scratch memory is the step's own: two steps on two
+    streams do not meet in it."""
+    if step.workspace is None:
+        step.workspace = {}
+    num_pages, max_pages = kv.pages.shape[0], kv.block_table.shape[1]
+    key = ("shared_call", step.shared, nq, nkv, d, dv, kv.page_size, num_pages, max_pages, dtype, positive, maps)
+    call = step.workspace.get(key)
+    if call is not None:
+        return call
+    group, sms, n, shape = nq // nkv, sm_count(device), step.num_seqs, shared_shape(step.shared)
+    if any(positions > max_pages * kv.page_size for positions, _ in step.shared):
+        raise KernelError("a group shares more positions than a block table holds")
     own = width_bucket(-(-_own_longest(step) // kv.page_size)) * kv.page_size
     chunk, warps = decode_plan(n, nkv, own, sms)
-    tensor_cores = dv == d and scale > 0 and tcgen05_attention_supported(q.dtype, nq, nkv, d, kv.page_size)
-    rows, tile, least, places = (2 * (128 // group) * group, 128, 1, sms) if tensor_cores else (SHARED_ROWS, SHARED_TILE, 4, 4 * sms)
-    plan = shared_plan(shared_shape(step.shared), group, nkv, rows, tile, least, places)
-    listed = _step_list(step, ("shared", group, nkv, rows, tile, plan), lambda st: shared_list(st, plan, group, nkv, rows, tile), device)
-    # (The tensor-core kernel's chunks lie at fixed positions, so a request's may be one more than its positions fill.)
+    tensor_cores = positive and dv == d and tcgen05_attention_supported(dtype, nq, nkv, d, kv.page_size)
+    if tensor_cores:
+        rows, tile, places = 2 * (128 // group) * group, 128, sms
+        least = shared_size(shape, group, nkv, rows, n * own * nkv * (d + dv) * 2 // 2, sms)
+    else:
+        rows, tile, least, places = SHARED_ROWS, SHARED_TILE, 2, 4 * sms
+    plan = shared_plan(shape, group, nkv, rows, tile, least, places)
+    listed = _step_list(step, ("shared", step.shared, group, nkv, rows, tile, plan), lambda st: shared_list(st, plan, group, nkv, rows, tile), device)
+    # (The decode kernel's chunks lie at fixed positions, so a request's may be one more than its positions fill.)
     max_parts, max_chunks = max(plan.parts), -(-own // chunk) + int(tensor_cores)
-    places = n * nq * (max_parts + max_chunks)
-    part_o, part_ml = _step_buffers(step, device, {"attention_part_o": (places * dv, torch.float32, False),
-                                                   "attention_part_ml": (places * 2, torch.float32, False)})
-    last = _MapDifferenceArgs(0.0, 0.0, 0.0, 0) if difference is None else \
-        _MapDifferenceArgs(difference.lam, difference.eps, difference.factor, difference.dv)
-    args = _SharedArgs(_ptr(q), k_ptr, v_ptr, gate_ptr, _ptr(out), _ptr(kv.block_table), _ptr(step.cu_seqlens), _ptr(step.seq_lens), _ptr(listed),
-                       _ptr(sink), _ptr(part_o), _ptr(part_ml), _ptr(error_word(device)), page_stride, n, plan.members, plan.items, max_parts, chunk,
-                       max_chunks, gate_stride, kv.block_table.shape[1], kv.pages.shape[0], nq, nkv, d, dv, kv.page_size,
-                       1 if difference is None else 2, scale, softcap, last)
-    if not tensor_cores:
-        fn = _function("attention_shared", "omnia_shared_attention", [c_void_p, c_int, c_void_p])
-        _check(fn(ctypes.byref(args), _code(q.dtype), _stream()), "shared_attention")
-        return out
-    tickets, = _step_buffers(step, device, {"attention_tickets": (n * nkv, torch.int32, True)})
-    defines = {"HEAD_DIM": d, "GROUP": group}
-    fn = _function("attention_shared_tc", "omnia_shared_pieces_tc", [c_void_p, c_void_p], defines)
-    _check(fn(ctypes.byref(args), _stream()), "shared_pieces")
-    fn = _function("attention_tc", "omnia_attention_decode_shared", [c_void_p, c_void_p, c_int, c_void_p],
-                   defines | {"SHARED": 1} | ({} if difference is None else {"MAPS": 2}))
-    _check(fn(ctypes.byref(args), _ptr(tickets), warps, _stream()), "attention_decode_shared")
+    count = n * nq * (max_parts + max_chunks)
+    held = [listed, torch.empty(count, dv, device=device), torch.empty(count, 2, device=device)]
+    args = _SharedArgs(cu_seqlens=_ptr(step.cu_seqlens), seq_lens=_ptr(step.seq_lens), plan=_ptr(listed), part_o=_ptr(held[1]), part_ml=_ptr(held[2]),
+                       err=_ptr(error_word(device)), page_stride=kv_layout(kv)[2], requests=n, members=plan.members, items=plan.items,
+                       max_parts=max_parts, chunk_keys=chunk, max_chunks=max_chunks, max_pages=max_pages, num_pages=num_pages, nq=nq, nkv=nkv,
+                       d=d, dv=dv, page_size=kv.page_size, maps=maps)
+    at = ctypes.byref(args)
+    if tensor_cores:
+        defines = {"HEAD_DIM": d, "GROUP": group}
+        pieces = _function("attention_shared_tc", "omnia_shared_pieces_tc", [c_void_p, c_void_p], defines)
+        decode = _function("attention_tc", "omnia_attention_decode_shared", [c_void_p, c_void_p, c_int, c_void_p],
+                           defines | {"SHARED": 1} | ({} if maps == 1 else {"MAPS": 2}))
+        held.append(torch.zeros(n * nkv, dtype=torch.int32, device=device))
+        tickets = _ptr(held[3])
+
+        def launch() -> int:
+            stream = _stream()
+            return pieces(at, stream) or decode(at, tickets, warps, stream)
+    else:
+        generic, code = _function("attention_shared", "omnia_shared_attention", [c_void_p, c_int, c_void_p]), _code(dtype)
+        launch = lambda: generic(at, code, _stream())  # noqa: E731
+    call = step.workspace[key] = _SharedCall(args, launch, held)
+    return call
+
+
+def _shared_attention(q: torch.Tensor, kv: KVView, step: StepContext, scale: float, gate: torch.Tensor | None, gate_col: int,
+                      sink: torch.Tensor | None, softcap: float, difference: "MapDifference | None") -> torch.Tensor:
+    """`paged_attention` of a step whose requests share positions (`StepContext.shared`): a group's shared positions as pieces for all of its
+    rows, each request's own in chunks, both put together at the end."""
+    tokens, nq, d = q.shape
+    k_ptr, v_ptr, _, nkv, _, dv = kv_layout(kv)
+    call = _shared_call(step, kv, nq, nkv, d, dv, q.dtype, q.device, scale > 0, 1 if difference is None else 2)
+    out = torch.empty(tokens, nq * dv if difference is None else nq // 2 * difference.dv, dtype=q.dtype, device=q.device)
+    args = call.args
+    args.q, args.k_pages, args.v_pages, args.out, args.block_table = q.data_ptr(), k_ptr, v_ptr, out.data_ptr(), kv.block_table.data_ptr()
+    if gate is None:
+        args.gate, args.gate_stride = None, 0
+    else:
+        args.gate, args.gate_stride = gate.data_ptr() + gate_col * gate.element_size(), gate.shape[1]
+    args.sink, args.scale, args.softcap = _ptr(sink), scale, softcap
+    if difference is not None:
+        args.difference = _MapDifferenceArgs(difference.lam, difference.eps, difference.factor, difference.dv)
+    _check(call.launch(), "shared_attention")
     return out
 
 
@@ -849,6 +902,10 @@ def paged_attention(q: torch.Tensor | None, kv: KVView, step: StepContext, scale
     if difference is not None and (nq % 2 or gate is not None or sink is not None or projection is not None
                                    or not 1 <= difference.dv <= dv):
         raise KernelError("a difference of maps takes pairs of query heads, no gate, no sink and no projected rows")
+    if shared_applies(step, kv, int(chunk or 0)):
+        if projection is not None:
+            raise KernelError("attention over shared positions takes queries, not projected rows")
+        return _shared_attention(q, kv, step, scale, gate, gate_col, sink, float(softcap or 0.0), difference)
     last = (0.0, 0.0, 0.0, 0) if difference is None else (difference.lam, difference.eps, difference.factor, difference.dv)
     out = torch.empty(tokens, nq * dv if difference is None else nq // 2 * difference.dv, dtype=q.dtype, device=q.device)
     gate_ptr = None if gate is None else gate.data_ptr() + gate_col * gate.element_size()
@@ -858,10 +915,6 @@ def paged_attention(q: torch.Tensor | None, kv: KVView, step: StepContext, scale
     run, softcap = int(chunk or 0), float(softcap or 0.0)
     if run and keep:
         raise KernelError("a mask of runs keeps no first positions")
-    if shared_applies(step, kv, run):
-        if projection is not None:
-            raise KernelError("attention over shared positions takes queries, not projected rows")
-        return _shared_attention(q, kv, step, scale, gate_ptr, gate_stride, sink, softcap, difference, out)
     if dv != d or not tiled_attention_supported(q.dtype, nq, nkv, d):
         if projection is not None:
             raise KernelError("the generic attention kernel takes queries, not projected rows")
