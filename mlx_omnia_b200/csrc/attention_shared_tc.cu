@@ -193,6 +193,9 @@ shared_pieces_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid
       uint32_t accumulate = 0;
       bool ok = wait_for(q_full, 0, abort_flag);
       const int step = turns ? 2 : 1;
+      // The second slot begins when the first one's first weights are there: its exponentials then run while the other one's products do, and
+      // not beside the other one's exponentials.
+      if (slot == 1 && tiles > 1 && ok) ok = wait_for(p_full0, 0, abort_flag);
       for (int j = turns ? slot : 0, t = 0; j < tiles && ok; j += step, ++t) {
         const int ks = j % k_stages, vs = j % V_STAGES;
         // The score tile is free: the product that read P from it is done.
@@ -336,72 +339,69 @@ shared_pieces_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid
       if (lane == 0) mbar_arrive(p_full0 + 8 * slot);
       ++done;
     }
-    // ---- the slot's piece: maximum (log2 units), sum, accumulator ---------------------------------------------------------
+    // ---- the slot's piece: offset, sum, accumulator. The accumulators' rows go through shared memory (all of it but the barriers: both slots'
+    // products are done behind the first barrier, and every load has landed, since products have read it), so that a warp writes a row
+    // of 512 bytes at a time: a thread a row wrote 16 bytes here and there, 3 us of a block's end and 8 where both slots have rows. -------
     if (ok && done > 0) ok = __all_sync(0xffffffffu, wait_for(o_done0 + 8 * slot, (done - 1) & 1, abort_flag));
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    const float top = m;
-    const int places = a.max_parts + a.max_chunks;
-    size_t at = 0;
-    if (live) {
-      int request, head;
-      place(my_row, request, head);
-      at = ((size_t)request * a.nq + head) * places + part;
+    constexpr int STRIDE = D + 4;  // floats: eight lanes' 16 bytes lie in different banks
+    float* stage = reinterpret_cast<float*>(smem_raw) + (turns ? 0 : slot) * BM * STRIDE;
+    static_assert(2 * BM * STRIDE * sizeof(float) <= TILES * TILE_BYTES, "both slots' rows fit where the tiles were");
+    float both = m, w = 1.f;  // of a row whose two slots' states become one: the offset, and what this slot's state counts
+    if (turns) row_ml[(slot * BM + row) * 2] = m, row_ml[(slot * BM + row) * 2 + 1] = l;
+    softmax_sync();
+    if (turns) {
+      const float other_m = row_ml[((slot ^ 1) * BM + row) * 2], other_l = row_ml[((slot ^ 1) * BM + row) * 2 + 1];
+      both = fmaxf(m, other_m);
+      w = m == -INFINITY ? 0.f : fast_exp2(m - both);
+      l = l * w + (other_m == -INFINITY ? 0.f : other_l * fast_exp2(other_m - both));
     }
-    if (!turns) {
-      if (ok && live) a.part_ml[2 * at] = top, a.part_ml[2 * at + 1] = l;
+    const int places = a.max_parts + a.max_chunks;
+    auto place_of = [&](int r) {  // of row r of the item
+      int request, head;
+      place(r, request, head);
+      return ((size_t)request * a.nq + head) * places + part;
+    };
+    if (ok && live && (!turns || slot == 0)) {
+      const size_t at = place_of(my_row);
+      a.part_ml[2 * at] = both, a.part_ml[2 * at + 1] = l;
+    }
+    // This slot's rows, weighted, to the stage; where the rows are both slots', the second slot's first.
+    auto put_rows = [&](bool add) {
 #pragma unroll 1
-      for (int c = 0; ok && c < D; c += 32) {
+      for (int c = 0; c < D; c += 32) {
         uint32_t o[32];
-        tmem_load32(o_addr + c, o);
-        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-        if (live)
-#pragma unroll
-          for (int i = 0; i < 32; i += 4)
-            *reinterpret_cast<uint4*>(a.part_o + at * D + c + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-      }
-    } else {
-      // Both slots' states of a row become one: each slot finishes half of the dims, and gives the other the rest by way of the
-      // K ring, which nobody reads any more (both slots' last products are done once both are past the barrier; the
-      // loads have all landed, since products have read them). A slot without a tile has nothing in its accumulator.
-      row_ml[(slot * BM + row) * 2] = top, row_ml[(slot * BM + row) * 2 + 1] = l;
-      softmax_sync();
-      const float other_top = row_ml[((slot ^ 1) * BM + row) * 2], other_l = row_ml[((slot ^ 1) * BM + row) * 2 + 1];
-      const float both = fmaxf(top, other_top);
-      const float w = top == -INFINITY ? 0.f : fast_exp2(top - both), other_w = other_top == -INFINITY ? 0.f : fast_exp2(other_top - both);
-      constexpr int HALF = D / 2;
-      float* give = reinterpret_cast<float*>(k_s);  // [2][HALF][128]: dim after dim, so a warp's rows lie side by side
-      if (done > 0 && ok) {
-#pragma unroll 1
-        for (int c = 0; c < HALF; c += 32) {
-          uint32_t o[32];
-          tmem_load32(o_addr + (slot ^ 1) * HALF + c, o);
+        if (done > 0) {
+          tmem_load32(o_addr + c, o);
           asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-          for (int i = 0; i < 32; ++i) give[(slot * HALF + c + i) * BM + row] = __uint_as_float(o[i]);
         }
-      } else {
-        for (int i = 0; i < HALF; ++i) give[(slot * HALF + i) * BM + row] = 0.f;
-      }
-      softmax_sync();
-      if (ok && live) {
-        if (slot == 0) a.part_ml[2 * at] = both, a.part_ml[2 * at + 1] = l * w + other_l * other_w;
-      }
-#pragma unroll 1
-      for (int c = 0; ok && c < HALF; c += 32) {
-        uint32_t o[32];
-        tmem_load32(o_addr + slot * HALF + c, o);
-        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-        if (live) {
+        float4* to = reinterpret_cast<float4*>(stage + row * STRIDE + c);
 #pragma unroll
-          for (int i = 0; i < 32; i += 4) {
-            float y[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              y[e] = (done > 0 ? __uint_as_float(o[i + e]) * w : 0.f) + give[((slot ^ 1) * HALF + c + i + e) * BM + row] * other_w;
-            *reinterpret_cast<float4*>(a.part_o + at * D + slot * HALF + c + i) = make_float4(y[0], y[1], y[2], y[3]);
+        for (int i = 0; i < 8; ++i) {
+          float4 y = add ? to[i] : make_float4(0.f, 0.f, 0.f, 0.f);
+          if (done > 0) {  // (a slot without a tile has nothing in its accumulator)
+            y.x = fmaf(__uint_as_float(o[4 * i]), w, y.x), y.y = fmaf(__uint_as_float(o[4 * i + 1]), w, y.y);
+            y.z = fmaf(__uint_as_float(o[4 * i + 2]), w, y.z), y.w = fmaf(__uint_as_float(o[4 * i + 3]), w, y.w);
           }
+          to[i] = y;
         }
       }
+    };
+    if (turns) {
+      if (slot == 1) put_rows(false);
+      softmax_sync();
+      if (slot == 0) put_rows(true);
+      softmax_sync();
+    } else {
+      put_rows(false);
+      __syncwarp();
+    }
+    // Rows out: a warp's own 32, or 16 of the rows that were both slots'.
+    const int r0 = turns ? warp * 16 : quarter * 32, r1 = min(r0 + (turns ? 16 : 32), min(SLOT_ROWS, rows - (turns ? 0 : slot * SLOT_ROWS)));
+#pragma unroll 4
+    for (int r = r0; r < r1; ++r) {
+      const size_t at = place_of((turns ? 0 : slot * SLOT_ROWS) + r);
+      if (ok && lane < D / 4) reinterpret_cast<float4*>(a.part_o + at * D)[lane] = reinterpret_cast<const float4*>(stage + r * STRIDE)[lane];
     }
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");

@@ -772,15 +772,16 @@ class _SharedCall:
     held: list[torch.Tensor]
 
 
-SHARED_TILE_NS, OWN_GBS = 1000, 4500
-"""What a tile of 128 shared keys takes a block of the tensor-core kernel, and the rate at which the decode kernel reads what requests hold of
-their own: how many SMs shared positions get follows from the two, since the kernels run beside one another."""
+SHARED_TILE_NS, OWN_GBS = (1450, 2600), 4500
+"""What a tile of 128 shared keys takes a block of the tensor-core kernel (up to 128 rows, up to 256), and the rate at which the decode kernel
+reads what requests hold of their own: how many SMs shared positions get follows from these, since the kernels run beside one another."""
 
 
 def shared_size(shape: tuple[tuple[int, int], ...], group: int, nkv: int, block_rows: int, own_bytes: int, sms: int) -> int:
     """Tiles of a piece of the tensor-core kernel: as many as one SM does in the time that all of them need for everything."""
-    tiles = sum(-(-count * group // block_rows) * nkv * -(-positions // 128) for positions, count in shape)
-    return max(1, -(-(tiles + own_bytes * sms // (OWN_GBS * SHARED_TILE_NS)) // sms))
+    cost = lambda count: SHARED_TILE_NS[count * group > block_rows // 2]  # noqa: E731
+    work = sum(-(-count * group // block_rows) * nkv * -(-positions // 128) * cost(count) for positions, count in shape)
+    return max(1, -(-(work + own_bytes * sms // OWN_GBS) // (sms * max(cost(count) for _, count in shape))))
 
 
 def _shared_call(step: StepContext, kv: KVView, nq: int, nkv: int, d: int, dv: int, dtype: torch.dtype, device: torch.device, positive: bool,
