@@ -419,7 +419,109 @@ shared_pieces_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid
   if (threadIdx.x == 0 && *abort_flag) atomicOr(a.err, OMNIA_ERR_TIMEOUT);
 }
 
+// ---- the pieces of a request and key/value head, put together: grid (nkv, requests) --------------------------------------------
+// A warp has a head's pieces, or every second, fourth, ... of them: eight maxima, sums and accumulators (16 bytes a lane) on their way at once. The
+// group's heads (eight at a time) end side by side in shared memory, where the gate, or the difference of two maps, is taken.
+constexpr int MERGE_WARPS = 8, MERGE_HEADS = GROUP < MERGE_WARPS ? GROUP : MERGE_WARPS, HEAD_WARPS = MERGE_WARPS / MERGE_HEADS;
+__global__ void __launch_bounds__(32 * MERGE_WARPS)
+shared_merge_tc_kernel(const __grid_constant__ SharedAttention a) {
+  __shared__ __align__(16) float part[MERGE_HEADS][HEAD_WARPS][D];
+  __shared__ float tops[MERGE_HEADS][HEAD_WARPS], sums[MERGE_HEADS][HEAD_WARPS];
+  pdl_wait();
+  pdl_launch_dependents();
+  const int kvh = blockIdx.x, request = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int start = a.plan[request], parts = min(a.plan[a.requests + request], a.max_parts), pos = a.seq_lens[request] - 1;
+  const size_t token = (size_t)a.cu_seqlens[request];
+  if (pos < 0) return;
+  const int places = a.max_parts + a.max_chunks, pieces = parts + (pos < start ? 0 : pos / a.chunk_keys - start / a.chunk_keys + 1);
+  for (int h0 = 0; h0 < GROUP; h0 += MERGE_HEADS) {
+    const int h = warp / HEAD_WARPS, sub = warp % HEAD_WARPS, r = h0 + h;
+    if (h < MERGE_HEADS && r < GROUP) {
+      const size_t first = ((size_t)request * a.nq + kvh * GROUP + r) * places;
+      float top = -INFINITY, l = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+      for (int p0 = sub; p0 < pieces; p0 += 8 * HEAD_WARPS) {
+        float2 ml[8];
+        float4 x[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const int p = p0 + u * HEAD_WARPS;
+          ml[u] = make_float2(-INFINITY, 0.f), x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (p < pieces) {
+            ml[u] = __ldcg(reinterpret_cast<const float2*>(a.part_ml) + first + p);
+            if (lane < D / 4) x[u] = __ldcg(reinterpret_cast<const float4*>(a.part_o + (first + p) * D) + lane);
+          }
+        }
+        float now = top;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) now = fmaxf(now, ml[u].x);
+        const float keep = top == -INFINITY ? 0.f : exp2f(top - now);
+        l *= keep, acc.x *= keep, acc.y *= keep, acc.z *= keep, acc.w *= keep;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const float w = ml[u].x == -INFINITY ? 0.f : exp2f(ml[u].x - now);
+          l = fmaf(ml[u].y, w, l);
+          acc.x = fmaf(x[u].x, w, acc.x), acc.y = fmaf(x[u].y, w, acc.y), acc.z = fmaf(x[u].z, w, acc.z), acc.w = fmaf(x[u].w, w, acc.w);
+        }
+        top = now;
+      }
+      if (lane < D / 4) *reinterpret_cast<float4*>(&part[h][sub][4 * lane]) = acc;
+      if (lane == 0) tops[h][sub] = top, sums[h][sub] = l;
+    }
+    __syncthreads();
+    bf16* out = (bf16*)a.out;
+    const int heads = min(MERGE_HEADS, GROUP - h0);
+    auto value = [&](int h, int dim) {
+      float top = -INFINITY, l = 0.f, v = 0.f;
+#pragma unroll
+      for (int x = 0; x < HEAD_WARPS; ++x) top = fmaxf(top, tops[h][x]);
+      if (top == -INFINITY) return 0.f;  // nothing seen
+#pragma unroll
+      for (int x = 0; x < HEAD_WARPS; ++x) {
+        const float w = tops[h][x] == -INFINITY ? 0.f : exp2f(tops[h][x] - top);
+        l = fmaf(sums[h][x], w, l), v = fmaf(part[h][x][dim], w, v);
+      }
+      if (a.sink != nullptr) l += exp2f(a.sink[kvh * GROUP + h0 + h] * LOG2E - top);
+      return v / l;
+    };
+    if (a.maps == 1) {
+      for (int x = threadIdx.x; x < heads * D; x += 32 * MERGE_WARPS) {
+        const int head = kvh * GROUP + h0 + x / D;
+        float y = value(x / D, x % D);
+        if (a.gate) y *= 1.f / (1.f + expf(-__bfloat162float(((const bf16*)a.gate)[token * a.gate_stride + (size_t)head * D + x % D])));
+        out[(token * a.nq + head) * D + x % D] = __float2bfloat16_rn(y);
+      }
+    } else if (2 * warp + 1 < heads) {  // a warp a pair of maps
+      float d[D / 32], ss = 0.f;
+#pragma unroll
+      for (int k = 0; k < D / 32; ++k) {
+        const int dim = lane + 32 * k;
+        d[k] = dim < a.difference.dv ? value(2 * warp, dim) - a.difference.lambda * value(2 * warp + 1, dim) : 0.f;
+        ss += d[k] * d[k];
+      }
+      const float f = rsqrtf(warp_sum(ss) / (float)a.difference.dv + a.difference.eps) * a.difference.factor;
+#pragma unroll
+      for (int k = 0; k < D / 32; ++k)
+        if (lane + 32 * k < a.difference.dv)
+          out[(token * (a.nq / 2) + (kvh * GROUP + h0) / 2 + warp) * a.difference.dv + lane + 32 * k] = __float2bfloat16_rn(d[k] * f);
+    }
+    __syncthreads();
+  }
+}
+
 // ---- host side -------------------------------------------------------------------------------
+
+// What the two kernels of a step's shared and own positions have left, put together.
+extern "C" int omnia_shared_merge_tc(const SharedAttention* given, cudaStream_t stream) {
+  const SharedAttention a = *given;
+  if (a.requests == 0) return 0;
+  if (a.requests < 0 || a.requests > 65535 || a.nkv < 1 || a.nq != a.nkv * GROUP || a.d != D || a.dv != D || a.chunk_keys < 1 || (a.maps != 1 && a.maps != 2) ||
+      (a.maps == 2 && (GROUP % 2 || a.gate || a.sink || a.difference.dv < 1 || a.difference.dv > D)) || ((uintptr_t)a.part_o & 15) || ((uintptr_t)a.part_ml & 7))
+    return (int)cudaErrorInvalidValue;
+  launch_pdl(shared_merge_tc_kernel, dim3(a.nkv, a.requests), 32 * MERGE_WARPS, 0, stream, a);
+  return OMNIA_LAUNCH_RESULT();
+}
 
 // The pieces of all items. Pages [num_pages, 2, nkv, page_size, D], page_size a multiple of 16; q [tokens, nq, D]; an item has at most
 // 2 * (128 / GROUP) * GROUP rows, its first key is a multiple of 16.

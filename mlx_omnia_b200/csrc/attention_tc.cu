@@ -619,7 +619,7 @@ attention_decode_kernel(const bf16* q, const bf16* __restrict__ pages,
                         const FusedQK fused, int keep_first, const float* __restrict__ sink, int run, float softcap,
                         const MapDifference difference, int beside, int* err
 #if SHARED
-                        , const int* shared, int max_parts
+                        , const int* shared, int max_parts, int merge_here
 #endif
                         ) {
   // In the fused mode nothing up to the query fragments depends on the kernel before this one
@@ -970,6 +970,12 @@ attention_decode_kernel(const bf16* q, const bf16* __restrict__ pages,
       }
     }
   }
+#if SHARED
+  if (!merge_here) {  // (one block waits for the kernel beside this one, so that whoever comes next comes after both)
+    if (beside && blockIdx.x + blockIdx.y + blockIdx.z == 0) pdl_wait();
+    return;
+  }
+#endif
   // Whoever finishes last merges: publish the partial, take a ticket, and if it is the last
   // one of this (request, head group), read all partials back and write the output. The ticket is drawn with release
   // and acquire at once: with it the thread's own and, through the barrier, the block's writes are given out, and the other blocks'
@@ -1243,7 +1249,8 @@ extern "C" int omnia_attention_decode_tc_static(const void* q, const void* pages
 
 // Attention of a step of single tokens over what each request holds beyond its shared positions, and the merge with the shared
 // positions' partials (attention_shared_tc.cu, the launch before this one where `items` is not zero): chunks of chunk_keys keys at fixed
-// positions, `warps` warps (1 or 4) a block. tickets [requests, nkv] are zero and left so. All requests of the step, rows of the
+// positions, `warps` warps (1 or 4) a block. tickets [requests, nkv] are zero and left so; without them the partials are
+// left for omnia_shared_merge_tc. All requests of the step, rows of the
 // call's head size and group.
 extern "C" int omnia_attention_decode_shared(const SharedAttention* given, int* tickets, int warps, cudaStream_t stream) {
   const SharedAttention a = *given;
@@ -1282,7 +1289,7 @@ extern "C" int omnia_attention_decode_shared(const SharedAttention* given, int* 
   launch_pdl(kernel, dim3(a.max_chunks, a.nkv, a.requests), warps * 32, smem, stream, (const bf16*)a.q, (const bf16*)a.k_pages,
              a.block_table, a.cu_seqlens, a.seq_lens, (const int*)nullptr, a.part_o, a.part_ml, tickets, (const bf16*)a.gate, a.gate_stride,
              (bf16*)a.out, a.chunk_keys, a.max_chunks, (const DecodePiece*)nullptr, 0, 0, a.max_pages, a.num_pages, a.nq, a.nkv,
-             a.page_size, 0, a.scale, FusedQK{}, 0, a.sink, 0, a.softcap, a.difference, a.items > 0 ? 1 : 0, a.err, a.plan, a.max_parts);
+             a.page_size, 0, a.scale, FusedQK{}, 0, a.sink, 0, a.softcap, a.difference, a.items > 0 ? 1 : 0, a.err, a.plan, a.max_parts, tickets != nullptr ? 1 : 0);
   return OMNIA_LAUNCH_RESULT();
 }
 

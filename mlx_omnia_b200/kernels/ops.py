@@ -10,7 +10,10 @@ names the element type of activations, matrices and cache pages; the residual st
 
 from __future__ import annotations
 
+import array
 import ctypes
+import itertools
+import math
 from ctypes import c_float, c_int, c_longlong, c_void_p
 
 import dataclasses
@@ -750,9 +753,9 @@ def shared_list(step: StepContext, plan: SharedPlan, group: int, nkv: int, block
     return out
 
 
-def shared_applies(step: StepContext, kv: KVView, run: int = 0) -> bool:
+def shared_applies(step: StepContext, kv: KVView) -> bool:
     """Whether a layer's attention reads shared positions once for their group: a step of single tokens, every position in sight."""
-    return bool(getattr(step, "shared", ())) and step.decode_only and not kv.window and not run
+    return bool(getattr(step, "shared", ())) and step.decode_only and not kv.window
 
 
 def _own_longest(step: StepContext) -> int:
@@ -770,11 +773,20 @@ class _SharedCall:
     args: _SharedArgs
     launch: Callable[[], int]
     held: list[torch.Tensor]
+    columns: int  # of the result
+    values: int  # bytes from the keys of a page to its values
 
 
 SHARED_TILE_NS, OWN_GBS = (1450, 2600), 4500
 """What a tile of 128 shared keys takes a block of the tensor-core kernel (up to 128 rows, up to 256), and the rate at which the decode kernel
 reads what requests hold of their own: how many SMs shared positions get follows from these, since the kernels run beside one another."""
+
+
+SHARED_MERGE_GROUP, SHARED_MERGE_PARTS = 4, 8
+"""From so many query heads a key/value head and pieces of shared positions on, a request's pieces are put together by a kernel of its own and not by
+the decode kernel's last block of the request, which has a warp for all of the group's heads. B200, us, that block / a kernel: four heads, 64
+requests of 65,536 shared positions 158 / 141, 16 of 32,768 50.4 / 45.6, 32 of 16,384 28.4 / 26.8; two heads, 64 of 2,051 35.2 / 38.9, 8 of
+4,096 14.5 / 15.6."""
 
 
 def shared_size(shape: tuple[tuple[int, int], ...], group: int, nkv: int, block_rows: int, own_bytes: int, sms: int) -> int:
@@ -784,17 +796,16 @@ def shared_size(shape: tuple[tuple[int, int], ...], group: int, nkv: int, block_
     return max(1, -(-(work + own_bytes * sms // OWN_GBS) // (sms * max(cost(count) for _, count in shape))))
 
 
-def _shared_call(step: StepContext, kv: KVView, nq: int, nkv: int, d: int, dv: int, dtype: torch.dtype, device: torch.device, positive: bool,
-                 maps: int) -> _SharedCall:
+def _shared_call(step: StepContext, kv: KVView, q: torch.Tensor, positive: bool, difference: "MapDifference | None") -> _SharedCall:
     """Made once a step and layout; the layers' own pointers are filled in by every call. Scratch memory is the step's own: two steps on two
     streams do not meet in it."""
-    if step.workspace is None:
-        step.workspace = {}
-    num_pages, max_pages = kv.pages.shape[0], kv.block_table.shape[1]
-    key = ("shared_call", step.shared, nq, nkv, d, dv, kv.page_size, num_pages, max_pages, dtype, positive, maps)
-    call = step.workspace.get(key)
-    if call is not None:
-        return call
+    device, dtype, (_, nq, d) = q.device, q.dtype, q.shape
+    k_ptr, v_ptr, _, nkv, _, dv = kv_layout(kv)
+    num_pages, max_pages, maps = kv.pages.shape[0], kv.block_table.shape[1], 1 if difference is None else 2
+    if difference is not None and not (nq % 2 == 0 and 1 <= difference.dv <= dv):
+        raise KernelError("a difference of maps takes pairs of query heads, and no more values than the cache has")
+    if kv.pages.dtype != dtype or not q.is_contiguous() or step.num_tokens != step.num_seqs or q.shape[0] != step.num_seqs:
+        raise KernelError("attention over shared positions takes a token a request, queries that are contiguous and of the cache's type")
     group, sms, n, shape = nq // nkv, sm_count(device), step.num_seqs, shared_shape(step.shared)
     if any(positions > max_pages * kv.page_size for positions, _ in step.shared):
         raise KernelError("a group shares more positions than a block table holds")
@@ -822,29 +833,39 @@ def _shared_call(step: StepContext, kv: KVView, nq: int, nkv: int, d: int, dv: i
         pieces = _function("attention_shared_tc", "omnia_shared_pieces_tc", [c_void_p, c_void_p], defines)
         decode = _function("attention_tc", "omnia_attention_decode_shared", [c_void_p, c_void_p, c_int, c_void_p],
                            defines | {"SHARED": 1} | ({} if maps == 1 else {"MAPS": 2}))
-        held.append(torch.zeros(n * nkv, dtype=torch.int32, device=device))
-        tickets = _ptr(held[3])
+        if group >= SHARED_MERGE_GROUP and max_parts >= SHARED_MERGE_PARTS:
+            merge = _function("attention_shared_tc", "omnia_shared_merge_tc", [c_void_p, c_void_p], defines)
 
-        def launch() -> int:
-            stream = _stream()
-            return pieces(at, stream) or decode(at, tickets, warps, stream)
+            def launch() -> int:
+                stream = _stream()
+                return pieces(at, stream) or decode(at, None, warps, stream) or merge(at, stream)
+        else:
+            held.append(torch.zeros(n * nkv, dtype=torch.int32, device=device))
+            tickets = _ptr(held[3])
+
+            def launch() -> int:
+                stream = _stream()
+                return pieces(at, stream) or decode(at, tickets, warps, stream)
     else:
         generic, code = _function("attention_shared", "omnia_shared_attention", [c_void_p, c_int, c_void_p]), _code(dtype)
         launch = lambda: generic(at, code, _stream())  # noqa: E731
-    call = step.workspace[key] = _SharedCall(args, launch, held)
-    return call
+    return _SharedCall(args, launch, held, nq * dv if difference is None else nq // 2 * difference.dv, v_ptr - k_ptr)
 
 
 def _shared_attention(q: torch.Tensor, kv: KVView, step: StepContext, scale: float, gate: torch.Tensor | None, gate_col: int,
                       sink: torch.Tensor | None, softcap: float, difference: "MapDifference | None") -> torch.Tensor:
     """`paged_attention` of a step whose requests share positions (`StepContext.shared`): a group's shared positions as pieces for all of its
     rows, each request's own in chunks, both put together at the end."""
-    tokens, nq, d = q.shape
-    k_ptr, v_ptr, _, nkv, _, dv = kv_layout(kv)
-    call = _shared_call(step, kv, nq, nkv, d, dv, q.dtype, q.device, scale > 0, 1 if difference is None else 2)
-    out = torch.empty(tokens, nq * dv if difference is None else nq // 2 * difference.dv, dtype=q.dtype, device=q.device)
-    args = call.args
-    args.q, args.k_pages, args.v_pages, args.out, args.block_table = q.data_ptr(), k_ptr, v_ptr, out.data_ptr(), kv.block_table.data_ptr()
+    pages, table = kv.pages, kv.block_table
+    if step.workspace is None:
+        step.workspace = {}
+    key = ("shared_call", step.shared, q.shape, q.dtype, pages.shape, table.shape, kv.page_size, kv.spec, scale > 0, difference)
+    call = step.workspace.get(key)
+    if call is None:
+        call = step.workspace[key] = _shared_call(step, kv, q, scale > 0, difference)
+    out = torch.empty(q.shape[0], call.columns, dtype=q.dtype, device=q.device)
+    args, base = call.args, pages.data_ptr()
+    args.q, args.k_pages, args.v_pages, args.out, args.block_table = q.data_ptr(), base, base + call.values, out.data_ptr(), table.data_ptr()
     if gate is None:
         args.gate, args.gate_stride = None, 0
     else:
@@ -889,6 +910,12 @@ def paged_attention(q: torch.Tensor | None, kv: KVView, step: StepContext, scale
     decode kernel when every request brings one token; otherwise the tcgen05 prefill kernel
     (head sizes 64 and 128, pages of a multiple of 16) or the mma.sync prefill kernel. Other
     cases (the 32-bit path among them) run on the generic kernel."""
+    if getattr(step, "shared", ()) and step.decode_only and not chunk and not (kv.window if window == -1 else window):
+        if projection is not None:
+            raise KernelError("attention over shared positions takes queries, not projected rows")
+        if difference is not None and (gate is not None or sink is not None):
+            raise KernelError("a difference of maps takes no gate and no sink")
+        return _shared_attention(q, kv, step, scale, gate, gate_col, sink, float(softcap or 0.0), difference)
     if projection is not None:
         tokens, nq, d = projection.rows.shape[0], projection.nq, projection.d
         q = projection.rows  # for its dtype and device only
@@ -903,10 +930,6 @@ def paged_attention(q: torch.Tensor | None, kv: KVView, step: StepContext, scale
     if difference is not None and (nq % 2 or gate is not None or sink is not None or projection is not None
                                    or not 1 <= difference.dv <= dv):
         raise KernelError("a difference of maps takes pairs of query heads, no gate, no sink and no projected rows")
-    if shared_applies(step, kv, int(chunk or 0)):
-        if projection is not None:
-            raise KernelError("attention over shared positions takes queries, not projected rows")
-        return _shared_attention(q, kv, step, scale, gate, gate_col, sink, float(softcap or 0.0), difference)
     last = (0.0, 0.0, 0.0, 0) if difference is None else (difference.lam, difference.eps, difference.factor, difference.dv)
     out = torch.empty(tokens, nq * dv if difference is None else nq // 2 * difference.dv, dtype=q.dtype, device=q.device)
     gate_ptr = None if gate is None else gate.data_ptr() + gate_col * gate.element_size()
@@ -1092,19 +1115,19 @@ def fill_slots(tensors: list[tuple[torch.Tensor, torch.Tensor | None]], slots: l
             _check(fn(to, start, size, len(part), some, len(some), _stream()), "fill_slots")
 
 
-def _move_array(moves, columns: int, most_from: int, most_to: int, same: bool, what: str) -> np.ndarray:
-    """Moves (from, to, ...) as an int32 array; numbers in range, no two with one end, and in one tensor no move's end another's beginning."""
-    held = np.asarray(moves, dtype=np.int64).reshape(-1, columns)
-    if held.shape[0]:
-        src, dst = held[:, 0], held[:, 1]
-        if int(src.min()) < 0 or int(src.max()) >= most_from or int(dst.min()) < 0 or int(dst.max()) >= most_to:
+def _move_array(moves, most_from: int, most_to: int, same: bool, what: str) -> array.array:
+    """Moves (from, to, ...) as ints one after the other; numbers in range, no two with one end, and in one tensor no move's end another's
+    beginning."""
+    if len(moves):
+        src, dst, *_ = zip(*moves)
+        if min(src) < 0 or max(src) >= most_from or min(dst) < 0 or max(dst) >= most_to:
             raise KernelError(f"{what}: a move's number lies outside the tensor")
-        ends = set(dst.tolist())
-        if len(ends) < held.shape[0]:
+        ends = set(dst)
+        if len(ends) < len(dst):
             raise KernelError(f"{what}: two moves end in the same place")
-        if same and not ends.isdisjoint(src.tolist()):
+        if same and not ends.isdisjoint(src):
             raise KernelError(f"{what}: a move ends where another begins")
-    return np.ascontiguousarray(held, dtype=np.int32)
+    return array.array("i", itertools.chain.from_iterable(moves))
 
 
 def copy_pages(pages: torch.Tensor, rows: tuple[tuple[int, int], ...], page_size: int, moves, to: torch.Tensor | None = None) -> torch.Tensor:
@@ -1112,21 +1135,23 @@ def copy_pages(pages: torch.Tensor, rows: tuple[tuple[int, int], ...], page_size
     page `dst`, for every (src, dst, count) of `moves`. `rows`: what a page holds, the `(heads, width)` of a `KVSpec`, each a block
     [heads, page_size, width]. `to`: another such tensor (as many layers, other pages, of the same type and page shape) that the
     pages go to. No two moves may end in the same page, and within one tensor none where another begins. -> the tensor written"""
+    shape, item = pages.shape, pages.element_size()
     to = pages if to is None else to
-    if not pages.is_contiguous() or not to.is_contiguous() or pages.dtype != to.dtype or pages.device != to.device or \
-            pages.shape[:1] + pages.shape[2:] != to.shape[:1] + to.shape[2:]:
+    if not pages.is_contiguous() or (to is not pages and (not to.is_contiguous() or pages.dtype != to.dtype or pages.device != to.device or
+                                                          shape[:1] + shape[2:] != to.shape[:1] + to.shape[2:])):
         raise KernelError("copy_pages takes contiguous tensors of the same layers, page shape, type and device")
-    item, elements = pages.element_size(), pages.shape[2:].numel()
+    elements = math.prod(shape[2:])
     if sum(h * w for h, w in rows) * page_size != elements:
         raise KernelError(f"pages of {elements} elements do not hold {page_size} rows of {rows}")
-    held = _move_array(moves, 3, pages.shape[1], to.shape[1], pages.data_ptr() == to.data_ptr(), "copy_pages")
-    if held.shape[0] and (int(held[:, 2].min()) < 0 or int(held[:, 2].max()) > page_size):
-        raise KernelError(f"copy_pages: a move of more rows than a page's {page_size}, or fewer than none")
+    address, to_address = pages.data_ptr(), to.data_ptr()
+    held = _move_array(moves, shape[1], to.shape[1], address == to_address, "copy_pages")
+    if len(held) != 3 * len(moves) or (held and not 0 <= min(held[2::3]) <= max(held[2::3]) <= page_size):
+        raise KernelError(f"copy_pages: moves of (from, to, rows), of no more rows than a page's {page_size}")
     fn = _function("cache_copy", "omnia_copy_pages", [c_void_p, c_void_p, c_longlong, c_longlong, c_int, c_longlong, c_int, c_void_p, c_void_p,
                                                       c_int, c_void_p, c_int, c_void_p])
     heads, width = (c_int * len(rows))(*(h for h, _ in rows)), (c_int * len(rows))(*(w * item for _, w in rows))
-    _check(fn(_ptr(pages), _ptr(to), pages.stride(0) * item, to.stride(0) * item, pages.shape[0], elements * item, page_size, heads, width,
-              len(rows), held.ctypes.data, held.shape[0], _stream()), "copy_pages")
+    _check(fn(address, to_address, shape[1] * elements * item, to.shape[1] * elements * item, shape[0], elements * item, page_size, heads, width,
+              len(rows), held.buffer_info()[0], len(moves), _stream()), "copy_pages")
     return to
 
 
@@ -1136,11 +1161,13 @@ def copy_slots(tensors: list[torch.Tensor], moves) -> None:
     if any(not t.is_contiguous() or t.dim() < 1 for t in tensors):
         raise KernelError("copy_slots takes contiguous tensors")
     least = min((t.shape[0] for t in tensors), default=0)
-    held = _move_array(moves, 2, least, least, True, "copy_slots")
+    held = _move_array(moves, least, least, True, "copy_slots")
+    if len(held) != 2 * len(moves):
+        raise KernelError("copy_slots: moves of (from, to)")
     fn = _function("cache_copy", "omnia_copy_slots", [c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p])
     to = (c_void_p * len(tensors))(*(t.data_ptr() for t in tensors))
-    size = (c_longlong * len(tensors))(*(t[0].numel() * t.element_size() if t.shape[0] else 0 for t in tensors))
-    _check(fn(to, size, len(tensors), held.ctypes.data, held.shape[0], _stream()), "copy_slots")
+    size = (c_longlong * len(tensors))(*(t.numel() // max(t.shape[0], 1) * t.element_size() for t in tensors))
+    _check(fn(to, size, len(tensors), held.buffer_info()[0], len(moves), _stream()), "copy_slots")
 
 
 SKINNY_ROWS = 16
