@@ -27,7 +27,7 @@ namespace {
 template <typename T, int MOST>
 __global__ void __launch_bounds__(32 * WARPS)
 shared_pieces_kernel(const __grid_constant__ SharedAttention a) {
-  constexpr int ACC = MOST / 32;
+  constexpr int ACC = MOST / 32, AT_ONCE = ACC < 4 ? ACC : 4;
   pdl_wait();
   pdl_launch_dependents();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -89,19 +89,43 @@ shared_pieces_kernel(const __grid_constant__ SharedAttention a) {
   for (int key0 = lo; key0 < hi; key0 += TILE) {
     __syncthreads();  // the tile before has been read
     const int keys = min(TILE, hi - key0);
-    // A warp brings every fourth key. Rows past the last key hold zeros, whatever the cache has there.
-    bool bad = false;
-    for (int k = warp; k < TILE; k += WARPS) {
-      const int pos = key0 + k;
-      const int page = k < keys ? table[pos / a.page_size] : -1;
-      const bool there = page >= 0 && page < a.num_pages;
-      bad |= k < keys && !there;
-      const long long at = (long long)page * a.page_stride;
-      const int off = kvh * a.page_size + pos % a.page_size;
-      for (int c = lane; c < a.d; c += 32) ks[k * stride + c] = there ? to_f32(k_pages[at + (long long)off * a.d + c]) : 0.f;
-      for (int c = lane; c < a.dv; c += 32) vs[k * a.dv + c] = there ? to_f32(v_pages[at + (long long)off * a.dv + c]) : 0.f;
+    // A lane looks a key's page up; then a warp brings every fourth key, the loads of 128 columns of all of its keys and values on their way
+    // together. Rows past the last key hold zeros, whatever the cache has there.
+    int page = -1;
+    if (lane < keys) {
+      page = table[(key0 + lane) / a.page_size];
+      if (page < 0 || page >= a.num_pages) page = -1;
     }
-    if (bad && lane == 0) atomicOr(a.err, OMNIA_ERR_PAGE);
+    if (warp == 0 && __any_sync(0xffffffffu, lane < keys && page < 0) && lane == 0) atomicOr(a.err, OMNIA_ERR_PAGE);
+    const T *k_rows[PER_WARP], *v_rows[PER_WARP];
+#pragma unroll
+    for (int x = 0; x < PER_WARP; ++x) {
+      const int k = warp + WARPS * x, from = __shfl_sync(0xffffffffu, page, k);
+      const long long at = (long long)from * a.page_stride;
+      const int off = kvh * a.page_size + (key0 + k) % a.page_size;
+      k_rows[x] = from < 0 ? nullptr : k_pages + at + (long long)off * a.d;
+      v_rows[x] = from < 0 ? nullptr : v_pages + at + (long long)off * a.dv;
+    }
+#pragma unroll 1
+    for (int c0 = lane; c0 < MOST; c0 += 32 * AT_ONCE) {
+      T k[PER_WARP][AT_ONCE], v[PER_WARP][AT_ONCE];
+#pragma unroll
+      for (int x = 0; x < PER_WARP; ++x)
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) {
+          const int c = c0 + 32 * i;
+          k[x][i] = k_rows[x] != nullptr && c < a.d ? k_rows[x][c] : from_f32<T>(0.f);
+          v[x][i] = v_rows[x] != nullptr && c < a.dv ? v_rows[x][c] : from_f32<T>(0.f);
+        }
+#pragma unroll
+      for (int x = 0; x < PER_WARP; ++x)
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) {
+          const int c = c0 + 32 * i;
+          if (c < a.d) ks[(warp + WARPS * x) * stride + c] = to_f32(k[x][i]);
+          if (c < a.dv) vs[(warp + WARPS * x) * a.dv + c] = to_f32(v[x][i]);
+        }
+    }
     __syncthreads();
     float s[PER_WARP];
 #pragma unroll

@@ -538,7 +538,7 @@ __device__ __forceinline__ void merge_chunks(const float* __restrict__ part_o, c
 #pragma unroll
       for (int k = 0; k < PER_LANE; ++k) {
         const int dim = lane + 32 * k;
-        d[k] = dim < D ? stage[dim] - difference.lambda * stage[D + dim] : 0.f;
+        d[k] = dim < difference.dv ? stage[dim] - difference.lambda * stage[D + dim] : 0.f;
         ss += d[k] * d[k];
       }
       const float f = rsqrtf(warp_sum(ss) / (float)difference.dv + difference.eps) * difference.factor;

@@ -659,7 +659,7 @@ def decode_fusable(proj: torch.Tensor, nq: int, nkv: int, d: int, inv_freq: torc
     """Whether the decode attention kernel can take the projected rows as they are: a step of
     single tokens, bfloat16, a head size that is a multiple of 32, rotated whole or not at all,
     a cache entry that this layer writes, and no positions shared by several requests that are read once for all."""
-    return (step.decode_only and not shared_applies(step, kv) and proj.is_cuda and kv.writes and d % 32 == 0
+    return (step.decode_only and not shared_applies(step, kv, nq) and proj.is_cuda and kv.writes and d % 32 == 0
             and (inv_freq is None or 2 * inv_freq.shape[0] == d) and proj.shape[1] % 2 == 0
             and tiled_attention_supported(proj.dtype, nq, nkv, d))
 
@@ -695,9 +695,9 @@ SHARED_ROWS, SHARED_TILE = 32, 32
 
 @dataclass(frozen=True)
 class SharedPlan:
-    """How a step's shared positions are cut: `parts` pieces of a group's positions, `items` (block of rows, key/value head, piece) in
+    """How a step's shared positions are cut: up to `parts` pieces of a group's positions, `items` (block of rows, key/value head, piece) in
     all, `members` places of the list of requests. Made from the groups' sizes rounded up (`shared_shape`), so that
-    a captured step takes the same plan until a group has lost half of its requests."""
+    a captured step serves groups of about one size."""
 
     parts: tuple[int, ...]
     blocks: tuple[int, ...]  # of rows, a group
@@ -706,8 +706,18 @@ class SharedPlan:
 
 
 def shared_shape(shared) -> tuple[tuple[int, int], ...]:
-    """(positions, requests rounded up to a power of two) of every group: what a plan is made from."""
-    return tuple((positions, 1 << max(len(members) - 1, 0).bit_length()) for positions, members in shared)
+    """(positions, requests) of every group, what a plan is made from: positions in tiles of 128, rounded up to four significant bits,
+    and requests to a power of two."""
+    shape = []
+    for positions, members in shared:
+        tiles = max(-(-positions // 128), 1)
+        unit = 1 << max(tiles.bit_length() - 4, 0)
+        shape.append((-(-tiles // unit) * unit * 128, 1 << max(len(members) - 1, 0).bit_length()))
+    return tuple(shape)
+
+
+def _shape_of(step: StepContext) -> tuple[tuple[int, int], ...]:
+    return shared_shape(step.shared) if step.shared_shape is None else step.shared_shape
 
 
 def shared_plan(shape: tuple[tuple[int, int], ...], group: int, nkv: int, block_rows: int, tile: int, least: int, places: int) -> SharedPlan:
@@ -728,34 +738,74 @@ def shared_list(step: StepContext, plan: SharedPlan, group: int, nkv: int, block
     n = step.num_seqs
     out = np.zeros(2 * n + plan.members + 8 * plan.items, dtype=np.int32)
     items = out[2 * n + plan.members:].reshape(-1, 8)
-    seen: set[int] = set()
+    shape = _shape_of(step)
+    if step.shared and shared_shape(step.shared) != shape:
+        raise KernelError("the groups of a step have another shape than it was captured for")
     first = at = 0
-    for (positions, members), parts, blocks, (_, room) in zip(step.shared, plan.parts, plan.blocks, shared_shape(step.shared)):
-        if positions < 1 or not members or not seen.isdisjoint(members) or len(set(members)) < len(members) or \
-                min(members) < 0 or max(members) >= n:
-            raise KernelError("requests share at least one position, each in one group of the step's requests")
-        if step.seq_lens_host and any(m < len(step.seq_lens_host) and step.seq_lens_host[m] <= positions for m in members):
-            raise KernelError("a request holds more positions than it shares")
-        seen.update(members)
+    for (positions, members), most, blocks, (_, room) in zip(step.shared, plan.parts, plan.blocks, shape):
+        tiles = -(-positions // tile)
+        parts = min(most, tiles)  # a piece without positions would leave nothing behind
         out[list(members)] = positions
         out[[n + m for m in members]] = parts
         out[2 * n + first: 2 * n + first + len(members)] = members
-        tiles = -(-positions // tile)
         cuts = [tiles * i // parts * tile for i in range(parts)] + [positions]
         for b in range(blocks):
             rows = max(0, min(block_rows, len(members) * group - b * block_rows))
-            block = items[at: at + nkv * parts].reshape(nkv, parts, 8)
+            block = items[at: at + nkv * most].reshape(nkv, most, 8)[:, :parts]
             block[:, :, 0], block[:, :, 1], block[:, :, 2], block[:, :, 3] = members[0], first, b * block_rows, rows
             block[:, :, 4] = np.arange(nkv)[:, None]
             block[:, :, 5], block[:, :, 6], block[:, :, 7] = cuts[:-1], cuts[1:], np.arange(parts)
-            at += nkv * parts
+            at += nkv * most
         first += room
     return out
 
 
-def shared_applies(step: StepContext, kv: KVView) -> bool:
-    """Whether a layer's attention reads shared positions once for their group: a step of single tokens, every position in sight."""
-    return bool(getattr(step, "shared", ())) and step.decode_only and not kv.window
+def shares(step: StepContext) -> bool:
+    """Whether requests of the step share positions, or may when it is replayed."""
+    return bool(getattr(step, "shared", ()) or getattr(step, "shared_shape", None))
+
+
+def check_shared(step: StepContext) -> None:
+    """Groups of at least one position, of requests of this step that hold more than they share, each in one group. (Looked at once a step.)"""
+    if step.workspace is None:
+        step.workspace = {}
+    key = ("shared_checked", step.shared, step.num_seqs, tuple(step.seq_lens_host))
+    if key in step.workspace:
+        return
+    seen: set[int] = set()
+    for positions, members in step.shared:
+        if positions < 1 or not members or not seen.isdisjoint(members) or len(set(members)) < len(members) or min(members) < 0 or \
+                max(members) >= step.num_seqs:
+            raise KernelError("requests share at least one position, each in one group of the step's requests")
+        if step.seq_lens_host and any(m < len(step.seq_lens_host) and step.seq_lens_host[m] <= positions for m in members):
+            raise KernelError("a request holds more positions than it shares")
+        seen.update(members)
+    step.workspace[key] = True
+
+
+SHARED_LEAST_BYTES = 24 << 20
+"""Shared positions are read once for a group where that saves so many bytes a layer of the tensor-core kernels, which are two or three launches in
+place of one. B200, us, shared / each for itself: 16/8 heads of 128, 8 requests of 1,000 + 30 positions (29 MB) 7.4 / 8.4, of 500 (14 MB) 7.5 / 7.3,
+2 of 4,000 + 400 (16 MB) 8.7 / 8.7, of 200 6.5 / 4.4; 16/4 heads, 32 of 500 (32 MB) 8.7 / 9.4; 6/2 heads of 64, 32 of 2,000 (32 MB) 7.5 / 8.4, of 500
+(8 MB) 7.0 / 6.1. The kernel for other types and sizes is the faster one from the first positions on (32 bits, 16/8 heads of 128, 2 requests of 64 + 30
+positions 13.7 / 43.5, 16 of 100 + 30 37 / 61): the ordinary kernel for these walks a request's keys in one block. It is not where bfloat16 of other
+head sizes has a tensor-core decode kernel to itself (8/2 heads of 256, 32 of 4,000 + 100 137 / 54; 8/8 of 96, 81 / 46), so that stays."""
+
+
+def shared_applies(step: StepContext, kv: KVView, nq: int, window: int | None = -1) -> bool:
+    """Whether a layer's attention reads shared positions once for their group: a step of single tokens, every position in sight, and enough of
+    them (`SHARED_LEAST_BYTES`; requests rounded up as in `shared_shape`, so that a captured step decides as it did)."""
+    if not shares(step) or not step.decode_only or (kv.window if window == -1 else window):
+        return False
+    if kv.spec is not None and (kv.spec.stride != 1 or kv.spec.chunk):
+        return False
+    _, _, _, nkv, d, dv = kv_layout(kv)
+    if d != dv or not tiled_attention_supported(kv.pages.dtype, nq, nkv, d):
+        return True
+    if not tcgen05_attention_supported(kv.pages.dtype, nq, nkv, d, kv.page_size):
+        return False
+    saved = sum(positions * (count - 1) for positions, count in _shape_of(step))
+    return saved * nkv * (d + dv) * kv.pages.element_size() >= SHARED_LEAST_BYTES
 
 
 def _own_longest(step: StepContext) -> int:
@@ -806,11 +856,12 @@ def _shared_call(step: StepContext, kv: KVView, q: torch.Tensor, positive: bool,
         raise KernelError("a difference of maps takes pairs of query heads, and no more values than the cache has")
     if kv.pages.dtype != dtype or not q.is_contiguous() or step.num_tokens != step.num_seqs or q.shape[0] != step.num_seqs:
         raise KernelError("attention over shared positions takes a token a request, queries that are contiguous and of the cache's type")
-    group, sms, n, shape = nq // nkv, sm_count(device), step.num_seqs, shared_shape(step.shared)
+    group, sms, n, shape = nq // nkv, sm_count(device), step.num_seqs, _shape_of(step)
     if any(positions > max_pages * kv.page_size for positions, _ in step.shared):
         raise KernelError("a group shares more positions than a block table holds")
     own = width_bucket(-(-_own_longest(step) // kv.page_size)) * kv.page_size
     chunk, warps = decode_plan(n, nkv, own, sms)
+    # (The tensor-core kernel looks for its maximum before it scales.)
     tensor_cores = positive and dv == d and tcgen05_attention_supported(dtype, nq, nkv, d, kv.page_size)
     if tensor_cores:
         rows, tile, places = 2 * (128 // group) * group, 128, sms
@@ -818,7 +869,7 @@ def _shared_call(step: StepContext, kv: KVView, q: torch.Tensor, positive: bool,
     else:
         rows, tile, least, places = SHARED_ROWS, SHARED_TILE, 2, 4 * sms
     plan = shared_plan(shape, group, nkv, rows, tile, least, places)
-    listed = _step_list(step, ("shared", step.shared, group, nkv, rows, tile, plan), lambda st: shared_list(st, plan, group, nkv, rows, tile), device)
+    listed = _step_list(step, ("shared", group, nkv, rows, tile, plan, () if step.shared_shape is not None else step.shared), lambda st: shared_list(st, plan, group, nkv, rows, tile), device)
     # (The decode kernel's chunks lie at fixed positions, so a request's may be one more than its positions fill.)
     max_parts, max_chunks = max(plan.parts), -(-own // chunk) + int(tensor_cores)
     count = n * nq * (max_parts + max_chunks)
@@ -857,9 +908,8 @@ def _shared_attention(q: torch.Tensor, kv: KVView, step: StepContext, scale: flo
     """`paged_attention` of a step whose requests share positions (`StepContext.shared`): a group's shared positions as pieces for all of its
     rows, each request's own in chunks, both put together at the end."""
     pages, table = kv.pages, kv.block_table
-    if step.workspace is None:
-        step.workspace = {}
-    key = ("shared_call", step.shared, q.shape, q.dtype, pages.shape, table.shape, kv.page_size, kv.spec, scale > 0, difference)
+    own = tuple(step.seq_lens_host) if step.max_own is None else step.max_own
+    key = ("shared_call", step.shared if step.shared_shape is None else step.shared_shape, own, q.shape, q.dtype, pages.shape, table.shape, kv.page_size, kv.spec, scale > 0, difference)
     call = step.workspace.get(key)
     if call is None:
         call = step.workspace[key] = _shared_call(step, kv, q, scale > 0, difference)
@@ -910,7 +960,9 @@ def paged_attention(q: torch.Tensor | None, kv: KVView, step: StepContext, scale
     decode kernel when every request brings one token; otherwise the tcgen05 prefill kernel
     (head sizes 64 and 128, pages of a multiple of 16) or the mma.sync prefill kernel. Other
     cases (the 32-bit path among them) run on the generic kernel."""
-    if getattr(step, "shared", ()) and step.decode_only and not chunk and not (kv.window if window == -1 else window):
+    if shares(step):
+        check_shared(step)
+    if not chunk and shared_applies(step, kv, q.shape[1] if projection is None else projection.nq, window):
         if projection is not None:
             raise KernelError("attention over shared positions takes queries, not projected rows")
         if difference is not None and (gate is not None or sink is not None):
