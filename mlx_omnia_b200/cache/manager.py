@@ -22,6 +22,14 @@ position has left a page's run behind. Pages that hold
 one of the first `keep_first` positions of such a group are kept until the request ends. All pages
 return when the request ends. Freed pages are handed out again, last freed first.
 
+A request may be *forked* (`CacheManager.fork`): the new one holds the first positions of the old
+one. Whole pages of these are then in both requests' block tables (the pool counts the references, a page
+is free again once the last is given back; nobody writes to a page that is in two tables, since
+positions only grow), the rows in the page that they end in are copied to a page of its own, and so is
+per-request state. Which requests share what (`SharedRun`) is kept with them, so that a step of
+single tokens can read shared positions once for all of them. `CacheManager.resize` gives the pools another
+number of pages while requests live: what is held moves to the front of the new ones.
+
 Beside the pages there are *state slots*: a request holds one slot number for its
 whole life, and every entry that declares a `StateSpec` has a tensor
 `[slots + 1, *shape]` indexed by it (an entry that declares several by name has one
@@ -55,12 +63,12 @@ class CacheError(RuntimeError):
 
 
 class PagePool:
-    """Page numbers 0..count-1; a stack of free ones (last freed, first reused)."""
+    """Page numbers 0..count-1, each held so many times; a stack of free ones (last freed, first reused)."""
 
     def __init__(self, count: int) -> None:
         self.count = count
         self._free = list(range(count - 1, -1, -1))
-        self._held = [False] * count
+        self._held = [0] * count
 
     @property
     def free(self) -> int:
@@ -70,19 +78,39 @@ class PagePool:
         if not self._free:
             raise CacheError("no free page")
         page = self._free.pop()
-        self._held[page] = True
+        self._held[page] = 1
         return page
+
+    def share(self, page: int) -> None:
+        """Hold a page once more; it is free after as many `give`s."""
+        if not 0 <= page < self.count or not self._held[page]:
+            raise CacheError(f"page {page} is not held and cannot be shared")
+        self._held[page] += 1
 
     def give(self, page: int) -> None:
         if not 0 <= page < self.count:
             raise CacheError(f"page {page} is not in a pool of {self.count}")
         if not self._held[page]:
             raise CacheError(f"page {page} is freed twice")
-        self._held[page] = False
-        self._free.append(page)
+        self._held[page] -= 1
+        if not self._held[page]:
+            self._free.append(page)
 
     def held(self) -> list[int]:
         return [p for p, h in enumerate(self._held) if h]
+
+    def references(self, page: int) -> int:
+        return self._held[page]
+
+    def resized(self, count: int) -> "tuple[PagePool, dict[int, int]]":
+        """A pool of `count` pages that holds what this one does, from page 0 on, and where each held page went."""
+        to = {page: i for i, page in enumerate(self.held())}
+        if len(to) > count:
+            raise CacheError(f"{len(to)} pages are held, which a pool of {count} does not take")
+        pool = PagePool(count)
+        for page in to:
+            pool._held[pool.take()] = self._held[page]
+        return pool, to
 
 
 @dataclass
@@ -91,6 +119,13 @@ class Group:
     entries: list[int]  # schedule entries stored in this group, in tensor order
     pool: PagePool
     pages: torch.Tensor | None  # [entries, pages, rows, heads, page_size, width] or [entries, pages, elements]
+
+
+@dataclass(eq=False, frozen=True)
+class SharedRun:
+    """The first `positions` positions that forks of one request hold alike; requests of one run carry the same object."""
+
+    positions: int
 
 
 @dataclass
@@ -105,6 +140,7 @@ class RequestCache:
     # int32 copies of `tables` (capacity grown by doubling; entries beyond len(tables[g]) are -1),
     # so that a step lays its block tables out with array copies instead of Python loops
     arrays: list[np.ndarray] = field(default_factory=list)
+    runs: list[SharedRun] = field(default_factory=list)  # what it shares with others, shortest first
 
     def table_array(self, group: int) -> np.ndarray:
         return self.arrays[group][: len(self.tables[group])]
@@ -163,16 +199,14 @@ class CacheManager:
                     self.initial_state[entry] = start.expand(1, *need.state.shape)[0].contiguous()
             if getattr(need, "block_state", None):
                 self.block_state[entry] = {name: slots_of(spec) for name, spec in need.block_state.items()}
+        self.has_state = bool(model_state) or any(need.state is not None or getattr(need, "block_state", None) for need in needs)
         # State that belongs to the model and to no schedule entry (an embedding that looks at the token before).
         self.model_state: dict[str, torch.Tensor] = \
             {name: slots_of(spec) for name, spec in (model_state or {}).items()} if allocate else {}
         self.requests: dict[str, RequestCache] = {}
 
-    def reset_slots(self, slots: list[int]) -> None:
-        """Set the state of `slots` (of requests about to run their first step) to its start:
-        the mixer's `initial_state()` where it gave one, zeros everywhere else."""
-        if not slots or not (self.state or self.block_state or self.model_state):
-            return
+    def state_tensors(self) -> list[tuple[torch.Tensor, torch.Tensor | None]]:
+        """Every tensor indexed by state slots, with what a slot starts as (None: zeros)."""
         held: list[tuple[torch.Tensor, torch.Tensor | None]] = [(t, None) for t in self.model_state.values()]
         for entry in sorted(set(self.state) | set(self.block_state)):
             own = self.state.get(entry)
@@ -181,6 +215,14 @@ class CacheManager:
             elif own is not None:
                 held.append((own, self.initial_state.get(entry)))
             held += [(t, None) for t in self.block_state.get(entry, {}).values()]
+        return held
+
+    def reset_slots(self, slots: list[int]) -> None:
+        """Set the state of `slots` (of requests about to run their first step) to its start:
+        the mixer's `initial_state()` where it gave one, zeros everywhere else."""
+        if not slots or not (self.state or self.block_state or self.model_state):
+            return
+        held = self.state_tensors()
         if held and held[0][0].is_cuda:
             from mlx_omnia_b200.kernels import ops
 
@@ -253,6 +295,114 @@ class CacheManager:
                 table.append(page)
         request.tokens += new_tokens
 
+    # -- forks -------------------------------------------------------------------------
+    def fork_pages(self, positions: int) -> list[int]:
+        """Pages each group takes for a fork at `positions`: the one that these end in, where they do not fill it."""
+        return [int(g.spec.stored(positions) > self._whole_pages(i, positions) * self.page_size) for i, g in enumerate(self.groups)]
+
+    def _whole_pages(self, group: int, positions: int) -> int:
+        """Pages of `group` that `positions` positions fill: no later position is written to them."""
+        return positions // self.groups[group].spec.stride // self.page_size
+
+    def why_not_fork(self, request: RequestCache, positions: int) -> str | None:
+        """Why `request` cannot be forked at `positions` (None: it can; pages and slots may still be short)."""
+        if not 1 <= positions <= request.tokens:
+            return f"a fork takes between 1 and the {request.tokens} positions that request {request.request_id!r} holds, not {positions}"
+        if request.tokens == positions:
+            return None
+        if self.has_state:
+            return f"the state of request {request.request_id!r} is that of {request.tokens} positions, not of {positions}"
+        for g, (group, table) in enumerate(zip(self.groups, request.tables)):
+            spec = group.spec
+            if positions % spec.stride:
+                return f"a stored row of {spec.stride} positions has gone on past position {positions}"
+            dead = max(spec.dead_below(positions), 0) // spec.stride // self.page_size if spec.forgets else 0
+            kept = -(-spec.stored(spec.keep_first) // self.page_size) if spec.keep_first else 0
+            if any(page < 0 and (i < kept or i >= dead) for i, page in enumerate(table[: self.pages_for(g, positions)])):
+                return f"positions that a request of {positions} reads were given back"
+        return None
+
+    def fork(self, request: RequestCache, request_id: str, positions: int | None = None) -> RequestCache:
+        """Open `request_id` with the first `positions` positions of `request` (None: all of them) as its own. Whole pages are
+        shared, the rest and the state are copied (on the current stream). Nothing is taken when it cannot be done (CacheError)."""
+        positions = request.tokens if positions is None else positions
+        why = self.why_not_fork(request, positions)
+        if why is not None:
+            raise CacheError(why)
+        need = self.fork_pages(positions)
+        for n, group in zip(need, self.groups):
+            if n > group.pool.free:
+                raise CacheError(f"group {group.spec} needs {n} pages, {group.pool.free} free")
+        new = self.open(request_id)
+        new.tokens, new.fresh = positions, request.fresh
+        for g, (n, group, table) in enumerate(zip(need, self.groups, request.tables)):
+            whole = self._whole_pages(g, positions)
+            mine = list(table[:whole])
+            for page in mine:
+                if page >= 0:
+                    group.pool.share(page)
+            if n and table[whole] < 0:
+                mine.append(-1)  # the page that they end in holds nothing that can still be read
+            elif n:
+                mine.append(group.pool.take())
+                if group.pages is not None:
+                    self._copy_rows(group, table[whole], mine[-1], group.spec.stored(positions) - whole * self.page_size)
+            new.tables[g] = mine
+            if len(mine) > len(new.arrays[g]):
+                new.arrays[g] = np.full(2 * len(mine), -1, dtype=np.int32)
+            new.arrays[g][: len(mine)] = mine
+        tensors = [t for t, _ in self.state_tensors()]
+        if tensors and tensors[0].is_cuda:
+            from mlx_omnia_b200.kernels import ops
+
+            ops.copy_slots(tensors, [(request.slot, new.slot)])
+        else:
+            for tensor in tensors:
+                tensor[new.slot] = tensor[request.slot]
+        run = next((r for r in request.runs if r.positions == positions), None)
+        if run is None:
+            run = SharedRun(positions)
+            request.runs = sorted([*request.runs, run], key=lambda r: r.positions)
+        new.runs = [r for r in request.runs if r.positions <= positions]
+        return new
+
+    def _copy_rows(self, group: Group, page: int, to: int, rows: int) -> None:
+        if group.pages.is_cuda:
+            from mlx_omnia_b200.kernels import ops
+
+            ops.copy_pages(group.pages, group.spec.rows, self.page_size, [(page, to, rows)])
+            return
+        flat, at = group.pages.flatten(2), 0
+        for heads, width in group.spec.rows:
+            size = heads * self.page_size * width
+            block = flat[:, :, at: at + size].unflatten(2, (heads, self.page_size, width))
+            block[:, to, :, :rows] = block[:, page, :, :rows]
+            at += size
+
+    def resize(self, pages_per_group: "int | dict[KVSpec, int]") -> None:
+        """Give every group's pool another number of pages, more or fewer, while requests live: what is held moves to the front of a
+        new tensor. CacheError, and nothing changed, where a pool would not take what it holds. No step may be in flight, and
+        steps captured on the old tensors are dead afterwards (`StepRunner.forget_graphs`)."""
+        counts = [pages_per_group[g.spec] if isinstance(pages_per_group, dict) else pages_per_group for g in self.groups]
+        if any(count < 1 for count in counts):
+            raise ValueError("a pool has at least one page")
+        pools = [group.pool.resized(count) for group, count in zip(self.groups, counts)]
+        for g, (group, (pool, to)) in enumerate(zip(self.groups, pools)):
+            if group.pages is not None:
+                old = group.pages
+                new = torch.zeros(old.shape[0], pool.count, *old.shape[2:], dtype=old.dtype, device=old.device)
+                if old.is_cuda:
+                    from mlx_omnia_b200.kernels import ops
+
+                    ops.copy_pages(old, group.spec.rows, self.page_size, [(a, b, self.page_size) for a, b in to.items()], to=new)
+                elif to:
+                    new[:, list(to.values())] = old[:, list(to)]
+                group.pages = new
+            group.pool = pool
+            for request in self.requests.values():
+                table = [to.get(page, -1) for page in request.tables[g]]
+                request.tables[g], request.arrays[g][: len(table)] = table, table
+
     def slot_of(self, request: RequestCache, group: int, position: int) -> int:
         row = position // self.groups[group].spec.stride
         page = request.tables[group][row // self.page_size]
@@ -300,16 +450,23 @@ class CacheManager:
         return self.groups[g].pages[index]
 
     def check(self) -> None:
-        """Every page is either free or in exactly one table (used by tests)."""
+        """Every page is either free or in as many tables as it is held times, at one place in all of them, and forks apart no
+        request writes to it (used by tests)."""
         for g, group in enumerate(self.groups):
-            seen: dict[int, str] = {}
+            seen: dict[int, list[tuple[int, str]]] = {}
             for request in self.requests.values():
-                for page in request.tables[g]:
+                for place, page in enumerate(request.tables[g]):
                     if page < 0:
                         continue
-                    if page in seen:
-                        raise CacheError(f"page {page} of group {g} is held by {seen[page]!r} and {request.request_id!r}")
-                    seen[page] = request.request_id
+                    holders = seen.setdefault(page, [])
+                    shared = max((r.positions for r in request.runs), default=0)
+                    if holders and (holders[0][0] != place or holders[-1][1] == request.request_id or
+                                    place >= self._whole_pages(g, shared)):
+                        raise CacheError(f"page {page} of group {g} is held by {holders[-1][1]!r} and {request.request_id!r}")
+                    holders.append((place, request.request_id))
+            for page, holders in seen.items():
+                if group.pool.references(page) != len(holders):
+                    raise CacheError(f"page {page} of group {g} is held {group.pool.references(page)} times, by {len(holders)} tables")
             if sorted(seen) != group.pool.held():
                 raise CacheError(f"group {g}: pages in tables {sorted(seen)} differ from pages taken {group.pool.held()}")
             if len(seen) + group.pool.free != group.pool.count:

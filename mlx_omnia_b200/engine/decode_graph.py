@@ -3,7 +3,8 @@
 A step in which every request brings one token launches some three hundred small
 kernels; issued one by one from Python they cost more host time than the GPU needs to
 run them. Such steps are therefore captured once per *bucket* (requests rounded up to
-a power of two, block-table width rounded up to three significant bits) and replayed: the
+a power of two, block-table width rounded up to three significant bits; where requests share
+positions, the rounded sizes of their groups and of what each holds beyond them) and replayed: the
 host writes the step's metadata into one pinned buffer, one copy brings it to the
 device buffer the captured kernels read, and the graph runs. Rows beyond the live
 requests are padding: sequence length 0, cache slot -1, position -1, which every kernel
@@ -53,7 +54,7 @@ from dataclasses import dataclass
 import numpy as np
 import torch
 
-from mlx_omnia_b200.engine.step import StepLayout
+from mlx_omnia_b200.engine.step import StepLayout, shared_positions
 from mlx_omnia_b200.kernels import ops
 from mlx_omnia_b200.parts.base import StepContext
 
@@ -100,14 +101,14 @@ class _Captured:
 class DecodeGraphs:
     def __init__(self, runner) -> None:
         self.runner = runner
-        self.captured: dict[tuple[int, int], _Captured] = {}  # in order of last use, oldest first
+        self.captured: dict[tuple, _Captured] = {}  # in order of last use, oldest first
         self.replays = 0
 
     @staticmethod
     def supported(model) -> bool:
         return all(getattr(block.mixer, "graph_safe", False) for block in model.blocks)
 
-    def _capture(self, batch: int, width: int) -> _Captured:
+    def _capture(self, batch: int, width: int, shape: tuple = (), own: int | None = None) -> _Captured:
         runner = self.runner
         device = runner.runtime.device
         layout = StepLayout(batch, batch, batch, [width] * len(runner.cache.groups))
@@ -116,7 +117,7 @@ class DecodeGraphs:
         # Kernels that need scratch memory keep it in the workspace, for as long as the graph lives.
         step = layout.context(dev, q_lens=[1] * batch, seq_lens_host=[], max_q_len=1,
                               max_seq_len=width * runner.cache.page_size, decode_only=True,
-                              workspace={"private": True})
+                              workspace={"private": True}, shared_shape=shape or None, max_own=own)
         # Padding everywhere, so the warm-up and the capture touch no page.
         layout.fill(host_tensor.numpy(), runner.cache, [], [], np.arange(batch, dtype=np.int32))
         dev.copy_(host_tensor)
@@ -133,15 +134,15 @@ class DecodeGraphs:
             logits = runner.model.forward(step, layers)
         return _Captured(graph, step, layout, host_tensor, dev, logits, ops.launches - before)
 
-    def _graph_for(self, batch: int, width: int) -> _Captured:
-        key = (batch, width)
+    def _graph_for(self, *key) -> _Captured:
+        """`key`: requests and table width, then (where requests share positions) the groups' shape and what a request holds beyond them."""
         captured = self.captured.pop(key, None)
         if captured is None:
             while len(self.captured) >= MAX_GRAPHS:
                 oldest = next(iter(self.captured))
                 torch.cuda.synchronize(self.runner.runtime.device)  # nothing of it is still running
                 del self.captured[oldest]
-            captured = self._capture(batch, width)
+            captured = self._capture(*key)
         self.captured[key] = captured  # most recently used last
         return captured
 
@@ -154,7 +155,12 @@ class DecodeGraphs:
         starts = runner.take_pages(entries)
         batch = _bucket(len(entries))
         width = ops.width_bucket(max(max((len(t) for t in e.request.tables), default=0) for e in entries))
-        captured = self._graph_for(batch, width)
+        shared, beyond = shared_positions(entries), ()
+        if shared:
+            page, starts_of = runner.cache.page_size, {i: positions for positions, which in shared for i in which}
+            own = max(s + 1 - starts_of.get(i, 0) for i, s in enumerate(starts))
+            beyond = (ops.shared_shape(shared), ops.width_bucket(-(-own // page)) * page)
+        captured = self._graph_for(batch, width, *beyond)
         if captured.copied is not None:
             captured.copied.synchronize()  # the pinned buffer is free to be written again
         captured.layout.fill(captured.host_tensor.numpy(), runner.cache, entries, starts,
@@ -162,6 +168,9 @@ class DecodeGraphs:
         captured.device.copy_(captured.host_tensor, non_blocking=True)
         if device_tokens is not None:
             captured.step.token_ids[: len(entries)].copy_(device_tokens[: len(entries)])
+        if shared:
+            captured.step.shared = shared
+            ops.fill_step_lists(captured.step)
         if captured.copied is None:
             captured.copied = torch.cuda.Event()
         captured.copied.record()

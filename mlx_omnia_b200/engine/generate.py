@@ -12,6 +12,7 @@ read of the chosen tokens per step.
 
 from __future__ import annotations
 
+import dataclasses
 import itertools
 import secrets
 from collections.abc import Iterator, Sequence
@@ -73,6 +74,12 @@ class _Launched:
     copied: "torch.cuda.Event | None" = None  # recorded behind that copy
 
 
+def common_start(prompts: Sequence[Sequence[int]]) -> int:
+    """How many first tokens all of the prompts have in common."""
+    first, last = min(prompts, default=()), max(prompts, default=())  # whatever these two share, all between them do
+    return next((i for i, (a, b) in enumerate(zip(first, last)) if a != b), min(len(first), len(last)))
+
+
 class Generator:
     """Continuous batching over one `Engine`."""
 
@@ -90,7 +97,11 @@ class Generator:
         self._token_slot = 0
         self.pipelined = True  # launch the next decode step before reading this one's tokens
 
-    def add(self, prompt: Sequence[int], options: GenerationOptions, request_id: str | None = None) -> Request:
+    def add(self, prompt: Sequence[int], options: GenerationOptions, request_id: str | None = None, *,
+            leader: Request | None = None, fork_at: int | None = None) -> Request:
+        """Add a request. With a `leader`, a request whose prompt begins with the same `fork_at` tokens (None: as many as the two have in
+        common; all but the last of this prompt at most), those are not read again but taken over from it, and steps of single tokens
+        read their keys and values once for both."""
         prompt = [int(t) for t in prompt]
         vocab = self.engine.vocab_size
         if any(not 0 <= t < vocab for t in prompt):
@@ -101,6 +112,9 @@ class Generator:
         stop = options.stop if options.stop is not None else self.default_stop
         params = options.params()
         request = Request(request_id or f"req-{next(self._ids)}", prompt, max(budget, 0), params, frozenset(stop))
+        if leader is not None:
+            request.fork_at = common_start([leader.prompt, prompt[:-1]]) if fork_at is None else int(fork_at)
+            request.leader = leader if request.fork_at or fork_at is not None else None
         request.meter = options.meter if options.meter is not None else Meter()
         request.meter.begin(len(prompt))
         self.scheduler.add(request)
@@ -217,15 +231,47 @@ class Generator:
             self._in_flight = None
         return self._finalize(launched)
 
+    def resize_cache(self, tokens: int) -> None:
+        """Give the page pools of a running engine room for `tokens` positions, more or fewer: what live requests hold is kept
+        (CacheError where it would not fit). The step in flight is finished first; captured steps are made anew."""
+        if self._in_flight is not None:
+            raise ValueError("a step is in flight; drain() it and read its outputs first")
+        engine = self.engine
+        if any(r.max_tokens + len(r.prompt) > tokens for r in [*self.scheduler.running, *self.scheduler.waiting]):
+            raise ValueError(f"a live request may grow past {tokens} tokens")
+        engine.cache.resize(-(-tokens // engine.cache.page_size))
+        engine.cache_tokens, self.scheduler.capacity = tokens, engine.cache.capacity_tokens()
+        engine.runner.forget_graphs()
+
     def run(self) -> None:
         """Step until every request has finished."""
         while not self.scheduler.idle or self._in_flight is not None:
             if not self.step() and self._in_flight is None and not self.scheduler.running and self.scheduler.waiting:
                 raise RuntimeError("the scheduler can admit nothing: the cache pool is too small")
 
-    def generate(self, prompts: Sequence[Sequence[int]], options: GenerationOptions) -> list[list[int]]:
-        """Generate for all prompts together; returns the generated ids per prompt."""
-        requests = [self.add(p, options) for p in prompts]
+    def generate(self, prompts: Sequence[Sequence[int]], options: GenerationOptions, *, samples: int = 1,
+                 share: bool = False) -> list[list[int]]:
+        """Generate for all prompts together; returns the generated ids per prompt.
+
+        `samples`: answers to every prompt, one after the other in what is returned. The prompt is read once, and every answer
+        goes on from there with draws of its own (the sampler's seed + i for answer i where a seed is given).
+        `share`: tokens that all of the prompts begin with are read once for all of them. Either way the answers' steps read the keys and
+        values of what they share once for all, which rounds otherwise than reading them request by request: in bfloat16 an answer may part from
+        the one that its prompt has by itself where two tokens are as good as equal."""
+        if samples < 1:
+            raise ValueError("samples must be at least 1")
+        prompts = [[int(t) for t in p] for p in prompts]
+        start = common_start([p[:-1] for p in prompts]) if share and len(prompts) > 1 else 0
+        requests: list[Request] = []
+        for prompt in prompts:
+            follows = {"leader": requests[0], "fork_at": start} if requests and start else {}
+            first = self.add(prompt, options, **follows)
+            requests.append(first)
+            for i in range(1, samples):
+                seed = options.sampler.seed
+                draws = options if seed is None else \
+                    dataclasses.replace(options, sampler=dataclasses.replace(options.sampler, seed=seed + i))
+                requests.append(self.add(prompt, draws, leader=first))
         self.run()
         ops.raise_on_error(self.engine.runtime.device)
         return [r.generated for r in requests]
@@ -263,9 +309,10 @@ class LanguageModel:
             if request.status != "finished":
                 self.generator.abort(request.request_id)
 
-    def generate(self, inputs: Sequence, options: GenerationOptions) -> list[list[int]]:
-        """Generate for several prompts in one continuous batch; ids per prompt."""
-        return self.generator.generate([self._ids(p) for p in inputs], options)
+    def generate(self, inputs: Sequence, options: GenerationOptions, *, samples: int = 1, share: bool = False) -> list[list[int]]:
+        """Generate for several prompts in one continuous batch; ids per prompt, `samples` answers to each one after the other. What the
+        answers to a prompt (and with `share` all prompts) have in common is read and kept once: see `Generator.generate`."""
+        return self.generator.generate([self._ids(p) for p in inputs], options, samples=samples, share=share)
 
 
 def load(model: str | Path, *, dtype=None, quantize=None, page_size: int = 16, cache_tokens: int | None = None,

@@ -17,6 +17,13 @@ exceeds the pool is refused when it is added; `max_tokens` is cut to what the po
 can hold, as the reference cuts it to the context limit
 (src/mlx_omnia/engine/language.py:407-409).
 
+A request may *follow* another (`Request.leader`, `Request.fork_at`): it has the other's first `fork_at`
+tokens, and rather than read them again it is forked from it (`CacheManager.fork`) when it is
+admitted. The leader's portion is cut there, so that it stands at that very position when its followers
+are admitted (per-request state can be copied at no other); a follower at the head of the queue waits for its leader to
+get there. A leader that cannot be forked any more (it has ended, or has gone on and its model keeps
+state) leaves its followers to read their tokens like any other request.
+
 A request ends when it samples a stop token (which is not emitted, as in
 src/mlx_omnia/engine/batching.py:653-655), when it has generated `max_tokens`
 (src/mlx_omnia/engine/batching.py:667), or when it is aborted; its pages and slot go
@@ -55,6 +62,8 @@ class Request:
     preemptions: int = 0
     order: int = 0
     meter: object | None = None  # an engine.meter.Meter, filled by the generation loop
+    leader: "Request | None" = None  # the request that this one is forked from when it is admitted
+    fork_at: int = 0  # ... with so many of its first tokens, which both have
 
     @property
     def tokens(self) -> list[int]:
@@ -121,6 +130,10 @@ class Scheduler:
         if len(request.prompt) >= self.capacity:
             raise ValueError(f"a prompt of {len(request.prompt)} tokens does not fit the cache pool of "
                              f"{self.capacity} tokens")
+        if request.leader is not None:
+            at = request.fork_at
+            if not 1 <= at < len(request.prompt) or request.prompt[:at] != request.leader.prompt[:at]:
+                raise ValueError("a request follows one whose prompt begins with the same tokens, one or more and not all of its own")
         request.max_tokens = min(request.max_tokens, self.capacity - len(request.prompt))
         request.order = next(self._order)
         request.status = "waiting"
@@ -175,6 +188,35 @@ class Scheduler:
         for g in range(len(reserved)):
             reserved[g] += self.cache.pages_for(g, held + count) - self.cache.pages_for(g, held)
 
+    def _portion(self, request: Request, budget: int) -> int:
+        """The next tokens of `request` within the budget, no further than where a waiting request is to be forked from it."""
+        count = min(request.pending, budget)
+        for follower in self.waiting:
+            if follower.leader is request and request.computed < follower.fork_at:
+                count = min(count, follower.fork_at - request.computed)
+        return count
+
+    def _fork(self, request: Request, reserved: list[int]) -> bool | None:
+        """Make a follower a fork of its leader, or of another follower of it that holds as much. True: done; False: not yet;
+        None: it follows nobody any more."""
+        leader, at = request.leader, request.fork_at
+        if leader.status == "waiting" and (leader in self.waiting or leader in self.running):
+            return False
+        if leader.cache is not None and leader.computed < at:
+            return False
+        donors = [leader] + [r for r in self.running if r.leader is leader and r.fork_at >= at]
+        donor = next((r for r in donors if r.cache is not None and self.cache.why_not_fork(r.cache, at) is None), None)
+        if donor is None:
+            request.leader = None
+            return None
+        grow = [self.cache.pages_for(g, at + 1) - self.cache.pages_for(g, at) for g in range(len(reserved))]
+        if any(n + more > group.pool.free - r
+               for n, more, group, r in zip(self.cache.fork_pages(at), grow, self.cache.groups, reserved)):
+            return False
+        request.cache = self.cache.fork(donor.cache, request.request_id, at)
+        request.computed = at
+        return True
+
     def plan(self) -> StepPlan:
         reserved = [0] * len(self.cache.groups)
         entries: list[PlannedEntry] = []
@@ -212,7 +254,7 @@ class Scheduler:
                               key=lambda r: r.order):
             if budget < 1:
                 break
-            count = self._affordable(request, min(request.pending, budget), reserved)
+            count = self._affordable(request, self._portion(request, budget), reserved)
             if count < 1:
                 continue
             entries.append(PlannedEntry(request, request.computed, count, count == request.pending))
@@ -224,14 +266,18 @@ class Scheduler:
             request = self.waiting[0]
             if any(request is p for p in preempted):
                 break  # it lost its pages in this very plan
-            count = self._affordable(request, min(request.pending, budget), reserved)
+            forked = None if request.leader is None else self._fork(request, reserved)
+            if forked is False:
+                break
+            count = self._affordable(request, self._portion(request, budget), reserved)
             if count < 1:
                 break
             self.waiting.popleft()
-            request.cache = self.cache.open(request.request_id)
+            if request.cache is None:
+                request.cache = self.cache.open(request.request_id)
             request.status = "running"
             self.running.append(request)
-            entries.append(PlannedEntry(request, 0, count, count == request.pending))
+            entries.append(PlannedEntry(request, request.computed, count, count == request.pending))
             self._reserve(request, count, reserved)
             budget -= count
         return StepPlan(entries, preempted)

@@ -31,6 +31,22 @@ class StepEntry:
     want: list[int] = field(default_factory=list)  # indices into `tokens`
 
 
+def shared_positions(entries: list[StepEntry]) -> tuple[tuple[int, tuple[int, ...]], ...]:
+    """Which entries' requests share their first positions: (positions, entries) of each group of two or more, the largest first. A
+    request that shares several runs of positions goes with the longest that another entry, not in a group yet, shares too."""
+    members: dict = {}
+    for i, entry in enumerate(entries):
+        for run in entry.request.runs:
+            members.setdefault(run, []).append(i)
+    found, taken = [], set()
+    for run in sorted(members, key=lambda run: -run.positions):
+        which = tuple(i for i in members[run] if i not in taken)
+        if len(which) > 1:
+            found.append((run.positions, which))
+            taken.update(which)
+    return tuple(sorted(found, key=lambda group: (-group[0], -len(group[1]))))
+
+
 class StepLayout:
     """Where each field of a step's metadata sits in one buffer of int32 words, so that one
     copy brings all of it to the device. A layout is made for `tokens` rows of the batch,
@@ -114,14 +130,22 @@ class StepRunner:
     def __init__(self, model: DecoderModel, cache: CacheManager, runtime: Runtime, cuda_graphs: bool = False) -> None:
         self.model, self.cache, self.runtime = model, cache, runtime
         self.steps_run = 0
+        self.cuda_graphs = cuda_graphs
         self.graphs = self.mixed_graphs = None
-        if cuda_graphs and runtime.device.type == "cuda":
-            from mlx_omnia_b200.engine.decode_graph import DecodeGraphs, MixedGraphs
+        self.forget_graphs()
 
-            if DecodeGraphs.supported(model):
-                self.graphs = DecodeGraphs(self)
-                if MixedGraphs.supported(model):
-                    self.mixed_graphs = MixedGraphs(self)
+    def forget_graphs(self) -> None:
+        """Drop every captured step (they hold the addresses of the cache's tensors) and begin anew."""
+        if not self.cuda_graphs or self.runtime.device.type != "cuda":
+            return
+        from mlx_omnia_b200.engine.decode_graph import DecodeGraphs, MixedGraphs
+
+        if self.graphs is not None:
+            torch.cuda.synchronize(self.runtime.device)  # nothing of them is still running
+        if DecodeGraphs.supported(self.model):
+            self.graphs = DecodeGraphs(self)
+            if MixedGraphs.supported(self.model):
+                self.mixed_graphs = MixedGraphs(self)
 
     # -- metadata ----------------------------------------------------------------------
     def take_pages(self, entries: list[StepEntry]) -> list[int]:
@@ -160,8 +184,9 @@ class StepRunner:
         host_tensor = torch.empty(layout.words, dtype=torch.int32, pin_memory=pinned)
         q_lens, held = layout.fill(host_tensor.numpy(), cache, entries, starts, rows)
         device = host_tensor.to(self.runtime.device, non_blocking=True) if pinned else host_tensor
+        single = all(q == 1 for q in q_lens)
         return layout.context(device, q_lens=q_lens, seq_lens_host=held, max_q_len=max(q_lens),
-                              max_seq_len=max(held), decode_only=all(q == 1 for q in q_lens))
+                              max_seq_len=max(held), decode_only=single, shared=shared_positions(entries) if single else ())
 
     def _shrink(self, request: RequestCache, count: int) -> None:
         """Undo a `grow` of `count` tokens that no kernel has used."""

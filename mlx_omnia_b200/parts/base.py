@@ -348,7 +348,10 @@ class StepContext:
     # Which requests share their first positions, in the same pages or in copies of them: (positions, requests of the step) for
     # each group, no request in two. Attention without a window may then read a group's shared positions once for all of it.
     shared: "tuple[tuple[int, tuple[int, ...]], ...]" = ()
-    max_own: int | None = None  # a bound of what a request holds beyond its shared positions (None: from seq_lens_host)
+    # Of a captured step, which is replayed with other groups: what they amount to, rounded up (`kernels.ops.shared_shape`), and a bound
+    # of what a request holds beyond its shared positions. None: from `shared` and `seq_lens_host`.
+    shared_shape: "tuple[tuple[int, int], ...] | None" = None
+    max_own: int | None = None
 
 
 @dataclass
