@@ -427,14 +427,27 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS)
 shared_merge_tc_kernel(const __grid_constant__ SharedAttention a) {
   __shared__ __align__(16) float part[MERGE_HEADS][HEAD_WARPS][D];
   __shared__ float tops[MERGE_HEADS][HEAD_WARPS], sums[MERGE_HEADS][HEAD_WARPS];
-  pdl_wait();
-  pdl_launch_dependents();
+  // The kernel before this one lets it begin only after its own wait for whatever came before, so lengths, list and gates are there.
   const int kvh = blockIdx.x, request = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int start = a.plan[request], parts = min(a.plan[a.requests + request], a.max_parts), pos = a.seq_lens[request] - 1;
   const size_t token = (size_t)a.cu_seqlens[request];
+  constexpr int MINE = (MERGE_HEADS * D + 32 * MERGE_WARPS - 1) / (32 * MERGE_WARPS);
+  float gates[MINE];
+  auto ask_for_gates = [&](int h0) {
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) {
+      const int x = threadIdx.x + i * 32 * MERGE_WARPS;
+      if (a.gate != nullptr && x < min(MERGE_HEADS, GROUP - h0) * D)
+        gates[i] = __bfloat162float(((const bf16*)a.gate)[token * a.gate_stride + (size_t)(kvh * GROUP + h0) * D + x]);
+    }
+  };
+  ask_for_gates(0);
+  pdl_wait();
+  pdl_launch_dependents();
   if (pos < 0) return;
   const int places = a.max_parts + a.max_chunks, pieces = parts + (pos < start ? 0 : pos / a.chunk_keys - start / a.chunk_keys + 1);
   for (int h0 = 0; h0 < GROUP; h0 += MERGE_HEADS) {
+    if (h0 > 0) ask_for_gates(h0);
     const int h = warp / HEAD_WARPS, sub = warp % HEAD_WARPS, r = h0 + h;
     if (h < MERGE_HEADS && r < GROUP) {
       const size_t first = ((size_t)request * a.nq + kvh * GROUP + r) * places;
@@ -486,11 +499,13 @@ shared_merge_tc_kernel(const __grid_constant__ SharedAttention a) {
       return v / l;
     };
     if (a.maps == 1) {
-      for (int x = threadIdx.x; x < heads * D; x += 32 * MERGE_WARPS) {
-        const int head = kvh * GROUP + h0 + x / D;
+#pragma unroll
+      for (int i = 0; i < MINE; ++i) {
+        const int x = threadIdx.x + i * 32 * MERGE_WARPS;
+        if (x >= heads * D) break;
         float y = value(x / D, x % D);
-        if (a.gate) y *= 1.f / (1.f + expf(-__bfloat162float(((const bf16*)a.gate)[token * a.gate_stride + (size_t)head * D + x % D])));
-        out[(token * a.nq + head) * D + x % D] = __float2bfloat16_rn(y);
+        if (a.gate != nullptr) y *= 1.f / (1.f + expf(-gates[i]));
+        out[(token * a.nq + kvh * GROUP + h0) * D + x] = __float2bfloat16_rn(y);
       }
     } else if (2 * warp + 1 < heads) {  // a warp a pair of maps
       float d[D / 32], ss = 0.f;

@@ -619,7 +619,7 @@ attention_decode_kernel(const bf16* q, const bf16* __restrict__ pages,
                         const FusedQK fused, int keep_first, const float* __restrict__ sink, int run, float softcap,
                         const MapDifference difference, int beside, int* err
 #if SHARED
-                        , const int* shared, int max_parts, int merge_here
+                        , const int* shared, int requests, int members, int items, int max_parts, int merge_here
 #endif
                         ) {
   // In the fused mode nothing up to the query fragments depends on the kernel before this one
@@ -646,6 +646,14 @@ attention_decode_kernel(const bf16* q, const bf16* __restrict__ pages,
     return first;
   };
   int parts = 0;  // partials of shared positions ahead of this request's own
+#if SHARED
+  // A block behind the requests' takes an item of the list: shared positions for up to sixteen rows of a group's requests.
+  constexpr int ROWS = 16;
+  int rows = GROUP, row0 = 0;
+  const int* group_members = nullptr;
+#else
+  constexpr int ROWS = GROUP, rows = GROUP;
+#endif
   // What this block does: request `request` of the call, which is request `seq` of the step; keys lo..hi, the `chunk`th of
   // the request's `chunks` runs of keys, whose partials lie one after the other.
   int request = blockIdx.z, kvh = blockIdx.y, chunk = blockIdx.x, chunks = 0, seq = 0, pos = -1, first = 0, lo = 0, hi = -1;
@@ -661,12 +669,23 @@ attention_decode_kernel(const bf16* q, const bf16* __restrict__ pages,
     first = first_key(pos);
     max_chunks = pieces;
     part_o += (size_t)mine.before * D, part_ml += (size_t)mine.before * 2;  // the heads' partials lie `pieces` apart
+#if SHARED
+  } else if (request >= requests) {
+    const int at = ((request - requests) * gridDim.y + kvh) * gridDim.x + chunk;
+    if (at >= items) return;
+    const int* item = shared + 2 * requests + members + SHARED_ITEM_INTS * at;
+    seq = item[0], group_members = shared + 2 * requests + item[1], row0 = item[2], rows = item[3], kvh = item[4], lo = item[5], hi = item[6] - 1;
+    chunk = item[7];
+    if (rows < 1 || lo > hi) return;
+    first = lo;
+    max_chunks += max_parts;
+#endif
   } else {
     seq = seq_ids ? seq_ids[request] : request;
     pos = seq_lens[seq] - 1;
     first = first_key(pos);
 #if SHARED
-    first = max(first, shared[seq]), parts = min(shared[gridDim.z + seq], max_parts);  // (all of the step's requests: no index list)
+    first = max(first, shared[seq]), parts = min(shared[requests + seq], max_parts);  // (all of the step's requests: no index list)
 #endif
     const int c0 = first / chunk_keys;  // blocks count from the first chunk in sight: a window needs a window's worth of them
     lo = max(first, (c0 + chunk) * chunk_keys), hi = min(pos, (c0 + chunk + 1) * chunk_keys - 1);
@@ -775,6 +794,18 @@ attention_decode_kernel(const bf16* q, const bf16* __restrict__ pages,
   {
     const int g = lane >> 2, t = lane & 3;
     const bf16* q_src = fused.proj ? fused.proj + token * fused.stride + fused.q_col : q + token * nq * D;
+#if SHARED
+    const bf16* q_rows[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int row = min(g + 8 * r, rows - 1);
+      const int head = group_members == nullptr ? row : (row0 + row) % GROUP;
+      const size_t of = group_members == nullptr ? token : (size_t)cu_seqlens[group_members[(row0 + row) / GROUP]];
+      q_rows[r] = q + (of * nq + kvh * GROUP + head) * D;
+    }
+#else
+    const bf16* q_rows[2] = {q_src + (size_t)(kvh * GROUP + g) * D, q_src + (size_t)(kvh * GROUP + g + 8) * D};
+#endif
 #pragma unroll
     for (int kstep = 0; kstep < KSTEPS; ++kstep) {
 #pragma unroll
@@ -782,8 +813,8 @@ attention_decode_kernel(const bf16* q, const bf16* __restrict__ pages,
         const int dim = kstep * 16 + half * 8 + 2 * t;
         unsigned lo_row = 0u, hi_row = 0u;
         if (dim < D) {
-          if (g < GROUP) lo_row = __ldcg(reinterpret_cast<const unsigned*>(q_src + (size_t)(kvh * GROUP + g) * D + dim));
-          if (g + 8 < GROUP) hi_row = __ldcg(reinterpret_cast<const unsigned*>(q_src + (size_t)(kvh * GROUP + g + 8) * D + dim));
+          if (g < rows) lo_row = __ldcg(reinterpret_cast<const unsigned*>(q_rows[0] + dim));
+          if (g + 8 < rows) hi_row = __ldcg(reinterpret_cast<const unsigned*>(q_rows[1] + dim));
         }
         qf[kstep][2 * half] = lo_row;
         qf[kstep][2 * half + 1] = hi_row;
@@ -851,7 +882,7 @@ attention_decode_kernel(const bf16* q, const bf16* __restrict__ pages,
   for (int r = 0; r < 2; ++r) {
     const int row = (lane >> 2) + 8 * r;
     row_lo[r] = lo;
-    row_hi[r] = row < GROUP ? hi : -1;
+    row_hi[r] = row < rows ? hi : -1;
   }
   const float sl2 = CAPPED && softcap > 0.f ? LOG2E : scale * LOG2E;
   const float pre = CAPPED && softcap > 0.f ? scale / softcap : 0.f;
@@ -919,14 +950,21 @@ attention_decode_kernel(const bf16* q, const bf16* __restrict__ pages,
   const int t = lane & 3;
   // The rows' states go to the block's partial: straight from the registers of a lone warp, or
   // (several warps) through shared memory, where warp 0 merges them, every lane its own dims.
-  float* merge = reinterpret_cast<float*>(smem_raw);  // [WARPS][GROUP][D + 2]: accumulator, max (log2 units), sum
+  float* merge = reinterpret_cast<float*>(smem_raw);  // [WARPS][ROWS][D + 2]: accumulator, max (log2 units), sum
+  auto place = [&](int row) {  // of a row's partial
+#if SHARED
+    if (group_members != nullptr)
+      return ((size_t)group_members[(row0 + row) / GROUP] * nq + kvh * GROUP + (row0 + row) % GROUP) * max_chunks + chunk;
+#endif
+    return (size_t)(kvh * GROUP + row) * max_chunks + parts + chunk;
+  };
   if (WARPS > 1) __syncthreads();                     // every warp is done with its tiles
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
     const int row = (lane >> 2) + 8 * r;
-    if (row >= GROUP) continue;
-    const size_t slot = (size_t)(kvh * GROUP + row) * max_chunks + parts + chunk;
-    float* dst = WARPS == 1 ? part_o + slot * D : merge + ((size_t)warp * GROUP + row) * (D + 2);
+    if (row >= rows) continue;
+    const size_t slot = place(row);
+    float* dst = WARPS == 1 ? part_o + slot * D : merge + ((size_t)warp * ROWS + row) * (D + 2);
 #pragma unroll
     for (int j = 0; j < NT_O; ++j) {
       const int dim = 8 * j + 2 * t;
@@ -947,12 +985,12 @@ attention_decode_kernel(const bf16* q, const bf16* __restrict__ pages,
   if (WARPS > 1) {
     __syncthreads();
 #pragma unroll
-    for (int i0 = 0; i0 < GROUP * D; i0 += WARPS * 32) {
+    for (int i0 = 0; i0 < ROWS * D; i0 += WARPS * 32) {
       const int i = i0 + threadIdx.x;
-      if (i >= GROUP * D) break;
+      if (i >= rows * D) break;
       const int row = i / D, dim = i - row * D;
-      const float* src = merge + (size_t)row * (D + 2);  // the first warp's; the others' lie GROUP rows apart
-      constexpr int APART = GROUP * (D + 2);
+      const float* src = merge + (size_t)row * (D + 2);  // the first warp's; the others' lie ROWS rows apart
+      constexpr int APART = ROWS * (D + 2);
       float top = -INFINITY, sum = 0.f, acc = 0.f;
 #pragma unroll
       for (int w = 0; w < WARPS; ++w) top = fmaxf(top, src[w * APART + D]);
@@ -962,7 +1000,7 @@ attention_decode_kernel(const bf16* q, const bf16* __restrict__ pages,
         sum += src[w * APART + D + 1] * weight;
         acc += src[w * APART + dim] * weight;
       }
-      const size_t slot = (size_t)(kvh * GROUP + row) * max_chunks + parts + chunk;
+      const size_t slot = place(row);
       part_o[slot * D + dim] = acc;
       if (dim == 0) {
         part_ml[slot * 2] = top;
@@ -1250,18 +1288,20 @@ extern "C" int omnia_attention_decode_tc_static(const void* q, const void* pages
 // Attention of a step of single tokens over what each request holds beyond its shared positions, and the merge with the shared
 // positions' partials (attention_shared_tc.cu, the launch before this one where `items` is not zero): chunks of chunk_keys keys at fixed
 // positions, `warps` warps (1 or 4) a block. tickets [requests, nkv] are zero and left so; without them the partials are
-// left for omnia_shared_merge_tc. All requests of the step, rows of the
-// call's head size and group.
-extern "C" int omnia_attention_decode_shared(const SharedAttention* given, int* tickets, int warps, cudaStream_t stream) {
+// left for omnia_shared_merge_tc. With `rows` the list's items, of up to 16 rows each, are more blocks of this kernel, and nothing
+// runs before it (no tickets then). All requests of the step, rows of the call's head size and group.
+extern "C" int omnia_attention_decode_shared(const SharedAttention* given, int* tickets, int warps, int rows, cudaStream_t stream) {
   const SharedAttention a = *given;
   if (a.requests == 0) return 0;
   if (MAPS != a.maps || (MAPS == 2 && (a.gate != nullptr || a.sink != nullptr || a.difference.dv < 1 || a.difference.dv > D)))
     return (int)cudaErrorInvalidValue;
   if (a.requests < 0 || a.requests > 65535 || a.nkv < 1 || a.nq != a.nkv * GROUP || a.d != D || a.dv != D || a.chunk_keys <= 0 || a.chunk_keys % DECODE_BN != 0 ||
-      a.max_chunks < 1 || a.max_parts < 0 || a.max_pages < 1 || a.num_pages < 1 || a.page_size < 1 || a.softcap < 0.f || (warps != 1 && warps != 4))
+      a.max_chunks < 1 || a.max_parts < 0 || a.max_pages < 1 || a.num_pages < 1 || a.page_size < 1 || a.softcap < 0.f || (warps != 1 && warps != 4) ||
+      a.items < 0 || a.members < 0 || (rows && tickets != nullptr))
     return (int)cudaErrorInvalidValue;
-  const int sms = omnia_sm_count();
-  const long long blocks = (long long)a.max_chunks * a.nkv * a.requests;
+  const int sms = omnia_sm_count(), layer = a.max_chunks * a.nkv, more = rows ? (a.items + layer - 1) / layer : 0;
+  if (more > 65535 - a.requests) return (int)cudaErrorInvalidValue;
+  const long long blocks = (long long)layer * a.requests + (rows ? a.items : 0);
   const bool deep = warps == 4 && blocks <= sms && (size_t)(8 * 2 * DECODE_BN) * ROW * sizeof(bf16) <= BLOCK_MOST - BLOCK_OVERHEAD;
   size_t smem = (size_t)((warps == 1 ? DECODE_STAGES : deep ? 8 : 4) * 2 * DECODE_BN) * ROW * sizeof(bf16);
   static bool configured[64] = {};
@@ -1282,14 +1322,14 @@ extern "C" int omnia_attention_decode_shared(const SharedAttention* given, int* 
     configured[device] = true;
   }
   {  // (spread over the SMs, as the other entry point's blocks are: those that the kernel beside this one leaves)
-    const int left = sms - a.items > sms / 4 ? sms - a.items : sms / 4;
+    const int left = rows ? sms : sms - a.items > sms / 4 ? sms - a.items : sms / 4;
     const size_t room = SM_SHARED / (size_t)((blocks + left - 1) / left);
     if (room > smem + BLOCK_OVERHEAD) smem = (room > BLOCK_MOST ? BLOCK_MOST : room) - BLOCK_OVERHEAD;
   }
-  launch_pdl(kernel, dim3(a.max_chunks, a.nkv, a.requests), warps * 32, smem, stream, (const bf16*)a.q, (const bf16*)a.k_pages,
+  launch_pdl(kernel, dim3(a.max_chunks, a.nkv, a.requests + more), warps * 32, smem, stream, (const bf16*)a.q, (const bf16*)a.k_pages,
              a.block_table, a.cu_seqlens, a.seq_lens, (const int*)nullptr, a.part_o, a.part_ml, tickets, (const bf16*)a.gate, a.gate_stride,
              (bf16*)a.out, a.chunk_keys, a.max_chunks, (const DecodePiece*)nullptr, 0, 0, a.max_pages, a.num_pages, a.nq, a.nkv,
-             a.page_size, 0, a.scale, FusedQK{}, 0, a.sink, 0, a.softcap, a.difference, a.items > 0 ? 1 : 0, a.err, a.plan, a.max_parts, tickets != nullptr ? 1 : 0);
+             a.page_size, 0, a.scale, FusedQK{}, 0, a.sink, 0, a.softcap, a.difference, a.items > 0 && !rows ? 1 : 0, a.err, a.plan, a.requests, a.members, a.items, a.max_parts, tickets != nullptr ? 1 : 0);
   return OMNIA_LAUNCH_RESULT();
 }
 

@@ -784,12 +784,13 @@ def check_shared(step: StepContext) -> None:
 
 
 SHARED_LEAST_BYTES = 24 << 20
-"""Shared positions are read once for a group where that saves so many bytes a layer of the tensor-core kernels, which are two or three launches in
-place of one. B200, us, shared / each for itself: 16/8 heads of 128, 8 requests of 1,000 + 30 positions (29 MB) 7.4 / 8.4, of 500 (14 MB) 7.5 / 7.3,
-2 of 4,000 + 400 (16 MB) 8.7 / 8.7, of 200 6.5 / 4.4; 16/4 heads, 32 of 500 (32 MB) 8.7 / 9.4; 6/2 heads of 64, 32 of 2,000 (32 MB) 7.5 / 8.4, of 500
-(8 MB) 7.0 / 6.1. The kernel for other types and sizes is the faster one from the first positions on (32 bits, 16/8 heads of 128, 2 requests of 64 + 30
-positions 13.7 / 43.5, 16 of 100 + 30 37 / 61): the ordinary kernel for these walks a request's keys in one block. It is not where bfloat16 of other
-head sizes has a tensor-core decode kernel to itself (8/2 heads of 256, 32 of 4,000 + 100 137 / 54; 8/8 of 96, 81 / 46), so that stays."""
+"""Shared positions are read once for a group where that saves so many bytes a layer of the tensor-core kernels: these are two or three launches in
+place of one, and that one also takes the projected rows as they are (2 to 3 us of a kernel ahead of it). B200, us, shared / each for itself: 16/8 heads
+of 128, 2 requests of 200 + 8 positions (0.8 MB) 7.9 / 6.5, 8 of 300 + 30 (9 MB) 10.6 / 10.4, 4 of 1,000 + 30 (12 MB) 10.5 / 10.8, 2 of 4,000 + 500 (16 MB)
+11.9 / 13.4, 8 of 1,000 + 30 (29 MB) 11.1 / 12.4, 16 of 1,000 + 30 (61 MB) 12.1 / 18.7; 6/2 heads of 64, 8 of 4,000 + 30 (14 MB) 9.9 / 9.7, of
+16,000 (57 MB) 16.2 / 19.6. The kernel for other types and sizes is the faster one from the first positions on (32 bits, 16/8 heads of 128, 2 requests of
+64 + 30 positions 13.7 / 43.5, 16 of 100 + 30 37 / 61): the ordinary kernel for these walks a request's keys in one block. It is not where bfloat16 of
+other head sizes has a tensor-core decode kernel to itself (8/2 heads of 256, 32 of 4,000 + 100 137 / 54; 8/8 of 96, 81 / 46), so that stays."""
 
 
 def shared_applies(step: StepContext, kv: KVView, nq: int, window: int | None = -1) -> bool:
@@ -839,6 +840,33 @@ requests of 65,536 shared positions 158 / 141, 16 of 32,768 50.4 / 45.6, 32 of 1
 4,096 14.5 / 15.6."""
 
 
+ROWS_MOST_BYTES = 20 << 20
+"""Up to so many bytes a layer, read once for every sixteen rows of a group, the decode kernel takes shared positions too, as more blocks of its own
+launch: its blocks begin and end sooner, the tensor-core kernel's read a position once for 128 or 256 rows. B200, us, decode kernel / that: 16/8 heads of
+128, 8 requests of 4,096 + 256 positions (17 MB) 13.7 / 14.5, 16 of 1,000 + 500 (8 MB) 14.9 / 16.2, of 4,000 + 500 (33 MB) 19.1 / 16.7; 32/8 heads, 16 of
+1,000 + 30 (16 MB) 13.5 / 14.8, 8 of 4,000 + 30 (33 MB) 16.3 / 15.4; 16/4, 8 of 4,000 + 30 (16 MB) 14.3 / 14.7; 6/2 heads of 64, three groups of 21 (11
+MB) 12.6 / 17.9, 64 of 4,000 + 30 (27 MB) 14.6 / 16.0, 16 of 16,000 + 500 (33 MB) 17.2 / 15.9."""
+
+
+def rows_in_decode(shape: tuple[tuple[int, int], ...], group: int, position_bytes: int) -> bool:
+    """`position_bytes`: a layer's keys and values of a position."""
+    rows = 16 // group * group
+    return sum(-(-count * group // rows) * positions for positions, count in shape) * position_bytes <= ROWS_MOST_BYTES
+
+
+def rows_chunk(shape: tuple[tuple[int, int], ...], group: int, nkv: int, requests: int, own: int, sms: int) -> int:
+    """Keys of a block of the decode kernel that takes shared positions too: what costs least, in tiles of 32 keys, where a block's beginning and end
+    are another four and an SM runs six blocks at a time (the groups' rounded sizes make blocks without work, so part of a wave counts as
+    that part). 8 requests of 4,096 + 256 positions, us at 64, 128, 192, 256 keys: 15.3, 14.3, 15.1, 16.5; three groups of 21: 12.7, 12.5, 14.8, 15.5."""
+    rows = 16 // group * group
+
+    def cost(chunk: int) -> float:
+        blocks = nkv * (sum(-(-count * group // rows) * -(-positions // chunk) for positions, count in shape) + requests * -(-own // chunk))
+        return max(1.0, blocks / (6 * sms)) * (4 + chunk // 32)
+
+    return min(range(128, 1025, 64), key=cost)
+
+
 def shared_size(shape: tuple[tuple[int, int], ...], group: int, nkv: int, block_rows: int, own_bytes: int, sms: int) -> int:
     """Tiles of a piece of the tensor-core kernel: as many as one SM does in the time that all of them need for everything."""
     cost = lambda count: SHARED_TILE_NS[count * group > block_rows // 2]  # noqa: E731
@@ -863,7 +891,12 @@ def _shared_call(step: StepContext, kv: KVView, q: torch.Tensor, positive: bool,
     chunk, warps = decode_plan(n, nkv, own, sms)
     # (The tensor-core kernel looks for its maximum before it scales.)
     tensor_cores = positive and dv == d and tcgen05_attention_supported(dtype, nq, nkv, d, kv.page_size)
-    if tensor_cores:
+    in_decode = tensor_cores and rows_in_decode(shape, group, nkv * (d + dv) * q.element_size())
+    if in_decode:
+        rows, tile, warps, places = 16 // group * group, 32, 1, 1 << 30
+        chunk = rows_chunk(shape, group, nkv, n, own, sms)
+        least = chunk // tile
+    elif tensor_cores:
         rows, tile, places = 2 * (128 // group) * group, 128, sms
         least = shared_size(shape, group, nkv, rows, n * own * nkv * (d + dv) * 2 // 2, sms)
     else:
@@ -882,21 +915,24 @@ def _shared_call(step: StepContext, kv: KVView, q: torch.Tensor, positive: bool,
     if tensor_cores:
         defines = {"HEAD_DIM": d, "GROUP": group}
         pieces = _function("attention_shared_tc", "omnia_shared_pieces_tc", [c_void_p, c_void_p], defines)
-        decode = _function("attention_tc", "omnia_attention_decode_shared", [c_void_p, c_void_p, c_int, c_void_p],
+        decode = _function("attention_tc", "omnia_attention_decode_shared", [c_void_p, c_void_p, c_int, c_int, c_void_p],
                            defines | {"SHARED": 1} | ({} if maps == 1 else {"MAPS": 2}))
-        if group >= SHARED_MERGE_GROUP and max_parts >= SHARED_MERGE_PARTS:
-            merge = _function("attention_shared_tc", "omnia_shared_merge_tc", [c_void_p, c_void_p], defines)
-
+        merge = _function("attention_shared_tc", "omnia_shared_merge_tc", [c_void_p, c_void_p], defines)
+        if in_decode:
             def launch() -> int:
                 stream = _stream()
-                return pieces(at, stream) or decode(at, None, warps, stream) or merge(at, stream)
+                return decode(at, None, warps, 1, stream) or merge(at, stream)
+        elif group >= SHARED_MERGE_GROUP and max_parts >= SHARED_MERGE_PARTS:
+            def launch() -> int:
+                stream = _stream()
+                return pieces(at, stream) or decode(at, None, warps, 0, stream) or merge(at, stream)
         else:
             held.append(torch.zeros(n * nkv, dtype=torch.int32, device=device))
             tickets = _ptr(held[3])
 
             def launch() -> int:
                 stream = _stream()
-                return pieces(at, stream) or decode(at, tickets, warps, stream)
+                return pieces(at, stream) or decode(at, tickets, warps, 0, stream)
     else:
         generic, code = _function("attention_shared", "omnia_shared_attention", [c_void_p, c_int, c_void_p]), _code(dtype)
         launch = lambda: generic(at, code, _stream())  # noqa: E731

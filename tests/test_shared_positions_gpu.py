@@ -29,6 +29,14 @@ def share_whatever_there_is(monkeypatch):
     monkeypatch.setattr(ops, "SHARED_LEAST_BYTES", 0)
 
 
+@pytest.fixture(params=["tiles of the tensor-core kernel", "rows of the decode kernel", "by size"])
+def way(request, monkeypatch):
+    """Both kernels that take shared positions of bfloat16, at every size."""
+    most = {"tiles of the tensor-core kernel": 0, "rows of the decode kernel": 1 << 60}.get(request.param)
+    if most is not None:
+        monkeypatch.setattr(ops, "ROWS_MOST_BYTES", most)
+
+
 def ints(values):
     return torch.tensor(values, dtype=torch.int32, device="cuda")
 
@@ -177,20 +185,20 @@ GROUPS = {
 
 @pytest.mark.parametrize("groups", GROUPS, ids=str)
 @pytest.mark.parametrize("layout", LAYOUTS)
-def test_attention(layout, groups):
+def test_attention(layout, groups, way):
     nq, nkv, d, dtype, page = LAYOUTS[layout]
     check(make(nq, nkv, d, dtype, page, GROUPS[groups], seed=len(layout)))
 
 
 @pytest.mark.parametrize("options", [{"gate": True}, {"sink": True}, {"softcap": 3.0}, {"gate": True, "sink": True, "softcap": 30.0}], ids=str)
 @pytest.mark.parametrize("layout", LAYOUTS)
-def test_gates_sinks_and_caps(layout, options):
+def test_gates_sinks_and_caps(layout, options, way):
     nq, nkv, d, dtype, page = LAYOUTS[layout]
     check(make(nq, nkv, d, dtype, page, [(333, [1, 66, 20]), (64, [64, 1])], seed=3), **options)
 
 
 @pytest.mark.parametrize("layout", ["16/8x128", "8/4x64", "8/1x64", "8/1x24 f32", "4/2x128 f32"])
-def test_the_difference_of_two_maps(layout):
+def test_the_difference_of_two_maps(layout, way):
     nq, nkv, d, dtype, page = LAYOUTS[layout]
     last = ops.MapDifference(0.7, 1e-5, 0.4, d - 4)
     check(make(nq, nkv, d, dtype, page, [(333, [1, 66, 20]), (64, [64, 1])], seed=3), difference=last)
@@ -203,13 +211,13 @@ def test_values_of_another_width(nq, nkv, d, dv, dtype):
 
 @pytest.mark.parametrize("layout", ["16/8x128", "32/8x128", "6/2x64", "32/2x128"])
 @pytest.mark.parametrize("positions,members,own", [(9000, 3, 40), (2051, 64, 100), (5000, 150, 9), (20000, 33, 2)])
-def test_long_positions_and_many_rows(layout, positions, members, own):
+def test_long_positions_and_many_rows(layout, positions, members, own, way):
     nq, nkv, d, dtype, page = LAYOUTS[layout]
     check(make(nq, nkv, d, dtype, page, [(positions, [1 + (7 * i) % own for i in range(members)])], alone=(700, 1)), gate=True)
 
 
 @pytest.mark.parametrize("layout", ["16/8x128", "6/2x64", "8/1x24 f32"])
-def test_scores_far_apart(layout):
+def test_scores_far_apart(layout, way):
     """Weights that a single key takes, and maxima that move from tile to tile."""
     nq, nkv, d, dtype, page = LAYOUTS[layout]
     check(make(nq, nkv, d, dtype, page, [(1500, [1, 300]), (777, [50, 2, 9])], seed=5, spread=12.0), sink=True)
@@ -217,13 +225,13 @@ def test_scores_far_apart(layout):
 
 @pytest.mark.parametrize("layout", ["16/8x128", "6/2x64", "8/1x24 f32"])
 @pytest.mark.parametrize("scale", [1e-4, 1.0, -0.1])
-def test_scales(layout, scale):
+def test_scales(layout, scale, way):
     nq, nkv, d, dtype, page = LAYOUTS[layout]
     check(make(nq, nkv, d, dtype, page, [(300, [1, 90])], seed=6), scale)
 
 
 @pytest.mark.parametrize("layout", ["16/8x128", "2/2x64", "8/1x24 f32"])
-def test_what_no_request_holds_does_not_matter(layout):
+def test_what_no_request_holds_does_not_matter(layout, way):
     """The pages' unused rows are NaN above; infinities and the lowest numbers there give the same bits."""
     nq, nkv, d, dtype, page = LAYOUTS[layout]
     case = make(nq, nkv, d, dtype, page, [(203, [1, 30, 77])], seed=7)
@@ -235,7 +243,7 @@ def test_what_no_request_holds_does_not_matter(layout):
 
 
 @pytest.mark.parametrize("layout", ["16/8x128", "32/8x128", "34/1x64 f32"])
-def test_the_same_call_gives_the_same_bits(layout):
+def test_the_same_call_gives_the_same_bits(layout, way):
     nq, nkv, d, dtype, page = LAYOUTS[layout]
     case = make(nq, nkv, d, dtype, page, [(4111, [1, 300, 12, 64, 5])], seed=8)
     n, first = len(case.lengths), None
@@ -246,7 +254,7 @@ def test_the_same_call_gives_the_same_bits(layout):
 
 
 @pytest.mark.parametrize("layout", ["16/8x128", "8/1x24 f32"])
-def test_pages_beyond_32_bits_of_elements(layout):
+def test_pages_beyond_32_bits_of_elements(layout, way):
     """Pages whose elements are counted in more than 31 bits: the held pages are moved to the end of a tensor of that many."""
     nq, nkv, d, dtype, page = LAYOUTS[layout]
     case = make(nq, nkv, d, dtype, page, [(203, [1, 30, 77])], seed=9)
@@ -260,7 +268,7 @@ def test_pages_beyond_32_bits_of_elements(layout):
 
 
 @pytest.mark.parametrize("layout", ["16/8x128", "4/2x128 f32"])
-def test_on_another_stream(layout):
+def test_on_another_stream(layout, way):
     nq, nkv, d, dtype, page = LAYOUTS[layout]
     case = make(nq, nkv, d, dtype, page, [(2000, [1, 300, 12])], seed=10)
     side = torch.cuda.Stream()
@@ -278,7 +286,7 @@ def test_on_another_stream(layout):
 
 
 @pytest.mark.parametrize("layout", ["16/8x128", "32/8x128", "8/1x24 f32"])
-def test_a_captured_step_serves_other_groups(layout):
+def test_a_captured_step_serves_other_groups(layout, way):
     nq, nkv, d, dtype, page = LAYOUTS[layout]
     cases = [make(nq, nkv, d, dtype, page, [(positions, [1 + (3 * i) % 50 for i in range(members)])], alone=(9,) * alone, padding=1, seed=seed)
              for seed, positions, members, alone in ((1, 1290, 7, 2), (2, 1400, 5, 4), (3, 1282, 8, 1))]
