@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import array
 import ctypes
+import functools
 import itertools
 import math
 from ctypes import c_float, c_int, c_longlong, c_void_p
@@ -324,6 +325,7 @@ def width_bucket(pages: int) -> int:
     return -(-pages // step) * step
 
 
+@functools.lru_cache(maxsize=4096)
 def decode_plan(requests: int, nkv: int, longest: int, sms: int) -> tuple[int, int]:
     """(keys per block, warps per block) of the decode attention kernel for `requests` requests
     (rounded up to a power of two, as a captured graph's batch is) of `nkv` key/value heads whose
@@ -362,6 +364,7 @@ PIECE_REQUESTS, PIECE_TILES, PIECE_INTS = 256, 5, 8
 attention runs by such a list, and the ints of a piece (`DecodePiece` in common.cuh)."""
 
 
+@functools.lru_cache(maxsize=4096)
 def decode_places(requests: int, nkv: int, longest: int, sms: int, d: int = 128) -> tuple[int, int]:
     """(blocks a key/value head that the GPU holds at a time, rounds of them that there may be) where a decode step's
     attention runs by a list of pieces (`omnia_decode_pieces`); (0, 0) where it keeps to `decode_plan`'s chunks. `requests` is
@@ -828,11 +831,6 @@ class _SharedCall:
     values: int  # bytes from the keys of a page to its values
 
 
-SHARED_TILE_NS, OWN_GBS = (1450, 2600), 4500
-"""What a tile of 128 shared keys takes a block of the tensor-core kernel (up to 128 rows, up to 256), and the rate at which the decode kernel
-reads what requests hold of their own: how many SMs shared positions get follows from these, since the kernels run beside one another."""
-
-
 SHARED_MERGE_GROUP, SHARED_MERGE_PARTS = 4, 8
 """From so many query heads a key/value head and pieces of shared positions on, a request's pieces are put together by a kernel of its own and not by
 the decode kernel's last block of the request, which has a warp for all of the group's heads. B200, us, that block / a kernel: four heads, 64
@@ -867,11 +865,29 @@ def rows_chunk(shape: tuple[tuple[int, int], ...], group: int, nkv: int, request
     return min(range(128, 1025, 64), key=cost)
 
 
+SHARED_TILE_US, SHARED_BLOCK_US, OWN_GBS, OWN_US = (2.0, 3.3), 6.0, 6000, 5.0
+"""What a tile of 128 shared keys takes a block of the tensor-core kernel (up to 128 rows, up to 256) while the decode kernel runs beside it, what a block
+takes besides, the rate at which the decode kernel reads what requests hold of their own and what it takes besides. Fitted to twelve
+shapes timed at every number of pieces: the plans made from these are the best or within 3 % for nine of them (64 answers to 65,536
+positions + 1,024: 120 blocks of 35 tiles 130 us, 152 of 27 133, 104 of 40 139), within 10 % for the rest (96 of 6,000 + 1,200: 32 blocks 87, 56 78, 16 108)."""
+
+
+@functools.lru_cache(maxsize=256)
 def shared_size(shape: tuple[tuple[int, int], ...], group: int, nkv: int, block_rows: int, own_bytes: int, sms: int) -> int:
-    """Tiles of a piece of the tensor-core kernel: as many as one SM does in the time that all of them need for everything."""
-    cost = lambda count: SHARED_TILE_NS[count * group > block_rows // 2]  # noqa: E731
-    work = sum(-(-count * group // block_rows) * nkv * -(-positions // 128) * cost(count) for positions, count in shape)
-    return max(1, -(-(work + own_bytes * sms // OWN_GBS) // (sms * max(cost(count) for _, count in shape))))
+    """Tiles of a piece of the tensor-core kernel: with which the GPU is done soonest, its SMs taken together or the longest block, whichever ends
+    later; a block an SM at most."""
+    groups = [(-(-count * group // block_rows) * nkv, positions // 128, SHARED_TILE_US[count * group > block_rows // 2]) for positions, count in shape]
+    longest = max(tiles for _, tiles, _ in groups)
+    best, best_us = longest, None
+    for size in sorted({-(-longest // parts) for parts in range(1, min(longest, sms) + 1)}, reverse=True):
+        pieces = [blocks * -(-tiles // size) for blocks, tiles, _ in groups]
+        if best_us is not None and sum(pieces) > sms:
+            break
+        work = sum(n * SHARED_BLOCK_US + blocks * tiles * us for n, (blocks, tiles, us) in zip(pieces, groups))
+        us = max(work / sms + OWN_US + own_bytes / (1000 * OWN_GBS), *(SHARED_BLOCK_US + us * min(size, tiles) for _, tiles, us in groups))
+        if best_us is None or us <= best_us:
+            best, best_us = size, us
+    return best
 
 
 def _shared_call(step: StepContext, kv: KVView, q: torch.Tensor, positive: bool, difference: "MapDifference | None") -> _SharedCall:
@@ -1203,11 +1219,14 @@ def fill_slots(tensors: list[tuple[torch.Tensor, torch.Tensor | None]], slots: l
             _check(fn(to, start, size, len(part), some, len(some), _stream()), "fill_slots")
 
 
-def _move_array(moves, most_from: int, most_to: int, same: bool, what: str) -> array.array:
+def _move_array(moves, columns: int, most_from: int, most_to: int, same: bool, what: str) -> array.array:
     """Moves (from, to, ...) as ints one after the other; numbers in range, no two with one end, and in one tensor no move's end another's
     beginning."""
-    if len(moves):
-        src, dst, *_ = zip(*moves)
+    held = list(itertools.chain.from_iterable(moves))
+    if len(held) != columns * len(moves):
+        raise KernelError(f"{what}: moves of (from, to{', rows' if columns == 3 else ''})")
+    if held:
+        src, dst = held[0::columns], held[1::columns]
         if min(src) < 0 or max(src) >= most_from or min(dst) < 0 or max(dst) >= most_to:
             raise KernelError(f"{what}: a move's number lies outside the tensor")
         ends = set(dst)
@@ -1215,7 +1234,10 @@ def _move_array(moves, most_from: int, most_to: int, same: bool, what: str) -> a
             raise KernelError(f"{what}: two moves end in the same place")
         if same and not ends.isdisjoint(src):
             raise KernelError(f"{what}: a move ends where another begins")
-    return array.array("i", itertools.chain.from_iterable(moves))
+    return array.array("i", held)  # (of a list: of anything else it takes three times as long)
+
+
+_COPY_PAGES = [c_void_p, c_void_p, c_longlong, c_longlong, c_int, c_longlong, c_int, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p]
 
 
 def copy_pages(pages: torch.Tensor, rows: tuple[tuple[int, int], ...], page_size: int, moves, to: torch.Tensor | None = None) -> torch.Tensor:
@@ -1226,20 +1248,22 @@ def copy_pages(pages: torch.Tensor, rows: tuple[tuple[int, int], ...], page_size
     shape, item = pages.shape, pages.element_size()
     to = pages if to is None else to
     if not pages.is_contiguous() or (to is not pages and (not to.is_contiguous() or pages.dtype != to.dtype or pages.device != to.device or
-                                                          shape[:1] + shape[2:] != to.shape[:1] + to.shape[2:])):
+                                                          shape[0] != to.shape[0] or shape[2:] != to.shape[2:])):
         raise KernelError("copy_pages takes contiguous tensors of the same layers, page shape, type and device")
     elements = math.prod(shape[2:])
     if sum(h * w for h, w in rows) * page_size != elements:
         raise KernelError(f"pages of {elements} elements do not hold {page_size} rows of {rows}")
     address, to_address = pages.data_ptr(), to.data_ptr()
-    held = _move_array(moves, shape[1], to.shape[1], address == to_address, "copy_pages")
-    if len(held) != 3 * len(moves) or (held and not 0 <= min(held[2::3]) <= max(held[2::3]) <= page_size):
-        raise KernelError(f"copy_pages: moves of (from, to, rows), of no more rows than a page's {page_size}")
-    fn = _function("cache_copy", "omnia_copy_pages", [c_void_p, c_void_p, c_longlong, c_longlong, c_int, c_longlong, c_int, c_void_p, c_void_p,
-                                                      c_int, c_void_p, c_int, c_void_p])
-    heads, width = (c_int * len(rows))(*(h for h, _ in rows)), (c_int * len(rows))(*(w * item for _, w in rows))
-    _check(fn(address, to_address, shape[1] * elements * item, to.shape[1] * elements * item, shape[0], elements * item, page_size, heads, width,
-              len(rows), held.buffer_info()[0], len(moves), _stream()), "copy_pages")
+    held = _move_array(moves, 3, shape[1], to.shape[1], address == to_address, "copy_pages")
+    if held:
+        counts = held[2::3]
+        if min(counts) < 0 or max(counts) > page_size:
+            raise KernelError(f"copy_pages: a move of no more rows than a page's {page_size}")
+    kinds = array.array("i", [h for h, _ in rows] + [w * item for _, w in rows])  # heads, then bytes of a row
+    at = kinds.buffer_info()[0]
+    _check(_function("cache_copy", "omnia_copy_pages", _COPY_PAGES)(
+        address, to_address, shape[1] * elements * item, to.shape[1] * elements * item, shape[0], elements * item, page_size, at,
+        at + len(rows) * kinds.itemsize, len(rows), held.buffer_info()[0], len(moves), _stream()), "copy_pages")
     return to
 
 
@@ -1249,9 +1273,7 @@ def copy_slots(tensors: list[torch.Tensor], moves) -> None:
     if any(not t.is_contiguous() or t.dim() < 1 for t in tensors):
         raise KernelError("copy_slots takes contiguous tensors")
     least = min((t.shape[0] for t in tensors), default=0)
-    held = _move_array(moves, least, least, True, "copy_slots")
-    if len(held) != 2 * len(moves):
-        raise KernelError("copy_slots: moves of (from, to)")
+    held = _move_array(moves, 2, least, least, True, "copy_slots")
     fn = _function("cache_copy", "omnia_copy_slots", [c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p])
     to = (c_void_p * len(tensors))(*(t.data_ptr() for t in tensors))
     size = (c_longlong * len(tensors))(*(t.numel() // max(t.shape[0], 1) * t.element_size() for t in tensors))
