@@ -31,7 +31,7 @@ constexpr int D = HEAD_DIM;
 static_assert(D == 64 || D == 128, "head sizes 64 and 128");
 static_assert(GROUP >= 1 && GROUP <= 16, "group size must be 1..16");
 constexpr int DH = D / 64;               // 64-wide halves of a head
-constexpr int BM = 128, BN = 128;        // rows of a slot, keys of a tile
+constexpr int BM = 128, BN = 128, HALF = 64;  // rows of a slot, keys of a tile, of the halves that are worked on
 constexpr int SLOT_ROWS = BM / GROUP * GROUP;
 // Seven tiles of shared memory: the rows (one tile where both slots hold the same, else two), the rest but the last two for
 // keys, two for values. A stage's loads, products and barriers go by one order of tiles; where the slots take turns each has stages
@@ -83,14 +83,15 @@ shared_pieces_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid
   unsigned char* q_s = smem_raw;
   unsigned char* v_s = q_s + (TILES - V_STAGES) * TILE_BYTES;
   uint64_t* bars = reinterpret_cast<uint64_t*>(v_s + V_STAGES * TILE_BYTES);
-  // bars: q_full | k_full[] | k_empty[] | v_full[] | v_empty[] | s_full[2] | p_full[2] | o_done[2]
-  constexpr int BARS = 1 + 2 * K_STAGES + 2 * V_STAGES + 6;
+  // bars: q_full | k_full[] | k_empty[] | v_full[] | v_empty[] | s_full[2][2] | p_full[2][2] | o_done[2][2] (slot, half) | began
+  constexpr int BARS = 1 + 2 * K_STAGES + 2 * V_STAGES + 13;
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + BARS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
   float* row_ml = reinterpret_cast<float*>(tmem_holder + 2);  // [2][128][2]: a slot's offset and sum, for the other one
   const int warp = omnia_warp_index(), lane = threadIdx.x & 31;
   const uint32_t q_full = smem_u32(bars), k_full0 = q_full + 8, k_empty0 = k_full0 + 8 * K_STAGES, v_full0 = k_empty0 + 8 * K_STAGES,
-                 v_empty0 = v_full0 + 8 * V_STAGES, s_full0 = v_empty0 + 8 * V_STAGES, p_full0 = s_full0 + 16, o_done0 = p_full0 + 16;
+                 v_empty0 = v_full0 + 8 * V_STAGES, s_full0 = v_empty0 + 8 * V_STAGES, p_full0 = s_full0 + 32, o_done0 = p_full0 + 32,
+                 began = o_done0 + 32;
   if (warp == WARP_MMA) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)), "r"(TMEM_COLS));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
@@ -109,7 +110,8 @@ shared_pieces_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid
     const int readers = turns ? 1 : 2;
     for (int s = 0; s < K_STAGES; ++s) mbar_init(k_full0 + 8 * s, 1), mbar_init(k_empty0 + 8 * s, readers);
     for (int s = 0; s < V_STAGES; ++s) mbar_init(v_full0 + 8 * s, 1), mbar_init(v_empty0 + 8 * s, readers);
-    for (int s = 0; s < 2; ++s) mbar_init(s_full0 + 8 * s, 1), mbar_init(p_full0 + 8 * s, BM / 32), mbar_init(o_done0 + 8 * s, 1);
+    for (int s = 0; s < 4; ++s) mbar_init(s_full0 + 8 * s, 1), mbar_init(p_full0 + 8 * s, BM / 32), mbar_init(o_done0 + 8 * s, 1);
+    mbar_init(began, BM / 32);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -118,6 +120,12 @@ shared_pieces_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem_base = *tmem_holder;
   int issued = -1;  // the last tile that this warp has asked for
+  // A slot's sequence of half tiles: half u is the (u & 1)th of the tile j0 + (u >> 1) * step.
+  const int step = turns ? 2 : 1;
+  auto halves_of = [&](int j0) {
+    const int mine = tiles > j0 ? (tiles - j0 + step - 1) / step : 0, last = j0 + (mine - 1) * step;
+    return mine < 1 ? 0 : 2 * mine - (hi - lo - last * BN <= HALF ? 1 : 0);
+  };
 
   if (warp >= WARP_MMA) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
   if (warp > WARP_Q) {
@@ -185,45 +193,52 @@ shared_pieces_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid
     }
   } else if (warp >= WARP_MMA) {
     // ---- issuer of a slot's products -----------------------------------------------------------------------------------
-    const int slot = warp - WARP_MMA;
-    if (tiles > 0 && omnia_elect_one()) {
-      constexpr uint32_t instr_s = idesc(BM, BN, false), instr_o = idesc(BM, D, true);
+    const int slot = warp - WARP_MMA, j0 = turns ? slot : 0, halves = halves_of(j0);
+    if (halves > 0 && omnia_elect_one()) {
+      constexpr uint32_t instr_s = idesc(BM, HALF, false), instr_o = idesc(BM, D, true);
       const uint64_t q_desc = desc_k_major(smem_u32(q_s + (turns ? 0 : slot) * TILE_BYTES));
       const uint32_t s_tmem = tmem_base + slot * BN, o_tmem = tmem_base + O_COL + slot * D;
       uint32_t accumulate = 0;
       bool ok = wait_for(q_full, 0, abort_flag);
-      const int step = turns ? 2 : 1;
       // The second slot begins when the first one's first weights are there: its exponentials then run while the other one's products do, and
       // not beside the other one's exponentials.
-      if (slot == 1 && tiles > 1 && ok) ok = wait_for(p_full0, 0, abort_flag);
-      for (int j = turns ? slot : 0, t = 0; j < tiles && ok; j += step, ++t) {
-        const int ks = j % k_stages, vs = j % V_STAGES;
-        // The score tile is free: the product that read P from it is done.
-        ok = wait_for(k_full0 + 8 * ks, (j / k_stages) & 1, abort_flag) &&
-             (t == 0 || wait_for(o_done0 + 8 * slot, (t & 1) ^ 1, abort_flag));
-        if (!ok) break;
+      if (slot == 1 && tiles > 1 && ok) ok = wait_for(began, 0, abort_flag);
+      auto scores = [&](int u) {
+        const int h = u & 1, j = j0 + (u >> 1) * step, ks = j % k_stages;
+        if (h == 0) ok = wait_for(k_full0 + 8 * ks, (j / k_stages) & 1, abort_flag);
+        if (!ok) return;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint64_t k_desc = desc_k_major(smem_u32(k_s + ks * TILE_BYTES));
+        const uint64_t k_desc = desc_k_major(smem_u32(k_s + ks * TILE_BYTES + h * (HALF * 128)));
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk)
-          umma(s_tmem, q_desc + (((kk / 4) * HALF_BYTES + (kk % 4) * 32) >> 4), k_desc + (((kk / 4) * HALF_BYTES + (kk % 4) * 32) >> 4), instr_s,
-               kk != 0);
-        umma_commit(s_full0 + 8 * slot);
-        umma_commit(k_empty0 + 8 * ks);
-        ok = wait_for(v_full0 + 8 * vs, (j / V_STAGES) & 1, abort_flag) && wait_for(p_full0 + 8 * slot, t & 1, abort_flag);
+          umma(s_tmem + h * HALF, q_desc + (((kk / 4) * HALF_BYTES + (kk % 4) * 32) >> 4), k_desc + (((kk / 4) * HALF_BYTES + (kk % 4) * 32) >> 4),
+               instr_s, kk != 0);
+        umma_commit(s_full0 + 8 * (2 * slot + h));
+        if (h == 1 || u == halves - 1) umma_commit(k_empty0 + 8 * ks);
+      };
+      if (ok) scores(0);
+      if (ok && halves > 1) scores(1);
+      for (int u = 0; u < halves && ok; ++u) {
+        const int h = u & 1, t = u >> 1, j = j0 + t * step, vs = j % V_STAGES;
+        ok = (h == 1 || wait_for(v_full0 + 8 * vs, (j / V_STAGES) & 1, abort_flag)) && wait_for(p_full0 + 8 * (2 * slot + h), t & 1, abort_flag);
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const uint64_t v_desc = desc_mn_major(smem_u32(v_s + vs * TILE_BYTES), HALF_BYTES);
-        const int groups = min(BN, hi - lo - j * BN + 15) / 16;  // boxes that were loaded: the rest of the stage is stale
+        const int groups = min(HALF, hi - lo - j * BN - h * HALF + 15) / 16;  // boxes that were loaded: the rest of the stage is stale
 #pragma unroll
-        for (int kk = 0; kk < BN / 16; ++kk) {
+        for (int kk = 0; kk < HALF / 16; ++kk) {
           if (kk >= groups) break;
           // P: 16 keys are eight columns of packed pairs
-          umma_ts(o_tmem, s_tmem + kk * 8, v_desc + ((kk * BOX_BYTES) >> 4), instr_o, accumulate);
+          umma_ts(o_tmem, s_tmem + h * HALF + kk * 8, v_desc + (((h * (HALF / 16) + kk) * BOX_BYTES) >> 4), instr_o, accumulate);
           accumulate = 1;
         }
-        umma_commit(o_done0 + 8 * slot);
-        umma_commit(v_empty0 + 8 * vs);
+        umma_commit(o_done0 + 8 * (2 * slot + h));
+        if (h == 1 || u == halves - 1) umma_commit(v_empty0 + 8 * vs);
+        // The half's columns are free once its weights have been read.
+        if (u + 2 < halves) {
+          ok = wait_for(o_done0 + 8 * (2 * slot + h), t & 1, abort_flag);
+          if (ok) scores(u + 2);
+        }
       }
     }
   } else {
@@ -246,36 +261,38 @@ shared_pieces_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid
     // The turn ahead of the first tile works on whatever tensor memory holds, and leaves it in the accumulator, which the first product
     // overwrites: it fetches the code, a straight line of some thousand instructions that every launch finds cold, while the first
     // tile is on its way (without it a block's first tile took 3 us).
-    const int step = turns ? 2 : 1, j0 = turns ? slot : 0;
-    for (int j = tiles > j0 ? j0 - step : tiles; j < tiles; j += step) {
-      const bool dry = j < j0;
+    const int j0 = turns ? slot : 0, halves = halves_of(j0);
+    for (int u = halves > 0 ? -1 : 0; u < halves; ++u) {
+      const bool dry = u < 0;
+      const int h = dry ? 0 : u & 1, t = u >> 1, j = j0 + t * step;
+      const uint32_t half_addr = s_addr + h * HALF;
       if (!dry) {
-        ok = __all_sync(0xffffffffu, wait_for(s_full0 + 8 * slot, done & 1, abort_flag));
+        ok = __all_sync(0xffffffffu, wait_for(s_full0 + 8 * (2 * slot + h), t & 1, abort_flag));
         if (!ok) break;
       }
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const int seen = dry ? BN : min(BN, hi - lo - j * BN);  // keys of this tile; the columns beyond hold whatever the stage held
+      const int seen = dry ? HALF : min(HALF, hi - lo - j * BN - h * HALF);  // keys of this half; the columns beyond hold whatever the stage held
       // All of the row's scores at once: a load from tensor memory takes some 0.35 us to arrive.
-      float z[BN];
+      float z[HALF];
       {
-        uint32_t raw[BN];
+        uint32_t raw[HALF];
 #pragma unroll
-        for (int c = 0; c < BN; c += 32) tmem_load32(s_addr + c, raw + c);
+        for (int c = 0; c < HALF; c += 32) tmem_load32(half_addr + c, raw + c);
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-        for (int c = 0; c < BN; ++c) z[c] = __uint_as_float(raw[c]);
+        for (int c = 0; c < HALF; ++c) z[c] = __uint_as_float(raw[c]);
       }
-      if (seen < BN) {
+      if (seen < HALF) {
 #pragma unroll
-        for (int c = 0; c < BN; ++c) z[c] = c < seen ? z[c] : -INFINITY;
+        for (int c = 0; c < HALF; ++c) z[c] = c < seen ? z[c] : -INFINITY;
       }
       if (capped) {  // c tanh(x) = c - 2 c / (1 + e^2x), in log2 units
 #pragma unroll
-        for (int c = 0; c < BN; ++c) z[c] = z[c] == -INFINITY ? z[c] : fmaf(-2.f * cap, fast_rcp(1.f + fast_exp2(z[c] * twice)), cap);
+        for (int c = 0; c < HALF; ++c) z[c] = z[c] == -INFINITY ? z[c] : fmaf(-2.f * cap, fast_rcp(1.f + fast_exp2(z[c] * twice)), cap);
       }
       float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int c = 0; c < BN; ++c) tops[c & 3] = fmaxf(tops[c & 3], z[c]);
+      for (int c = 0; c < HALF; ++c) tops[c & 3] = fmaxf(tops[c & 3], z[c]);
       const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * unit;
       // The offset follows the row's maximum lazily: what was summed is brought to a new one only when the scores have outgrown the old.
       float alpha = 1.f;
@@ -289,7 +306,10 @@ shared_pieces_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid
         }
       }
       if (done > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
-        // (The products so far are done: the issuer waited for them before it issued these scores.)
+        // The products so far, the half before this one's among them, have to be done; the next one's wait for this warp.
+        ok = __all_sync(0xffffffffu, wait_for(o_done0 + 8 * (2 * slot + (h ^ 1)), ((u - 1) >> 1) & 1, abort_flag));
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
         for (int c = 0; c < D; c += 8) {
           uint32_t o[8];
@@ -302,18 +322,15 @@ shared_pieces_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid
       }
       const float offset = m == -INFINITY ? 0.f : m;
       float sums[4] = {0.f, 0.f, 0.f, 0.f};
-      // The weights, in pairs, take the place of the first half of the row's scores.
+      // The weights, in pairs, take the place of the first half of these scores.
+      uint32_t packed[HALF / 2];
 #pragma unroll
-      for (int c0 = 0; c0 < BN; c0 += 64) {
-        uint32_t packed[32];
-#pragma unroll
-        for (int c = 0; c < 64; c += 2) {
-          const float p0 = fast_exp2(fmaf(z[c0 + c], unit, -offset)), p1 = fast_exp2(fmaf(z[c0 + c + 1], unit, -offset));
-          sums[c & 2] += p0, sums[(c & 2) + 1] += p1;
-          packed[c / 2] = pack_bf16(p0, p1);
-        }
-        tmem_store32((dry ? o_addr : s_addr) + c0 / 2, packed);
+      for (int c = 0; c < HALF; c += 2) {
+        const float p0 = fast_exp2(fmaf(z[c], unit, -offset)), p1 = fast_exp2(fmaf(z[c + 1], unit, -offset));
+        sums[c & 2] += p0, sums[(c & 2) + 1] += p1;
+        packed[c / 2] = pack_bf16(p0, p1);
       }
+      tmem_store32(dry ? o_addr : half_addr, packed);
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       if (dry) {
         m = -INFINITY, l = 0.f;
@@ -329,20 +346,23 @@ shared_pieces_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid
         const int r1 = (seen + 15) & ~15;
 #pragma unroll 1
         for (int i = row; i < (r1 - seen) * DH * 8; i += BM) {
-          const int piece = i & 7, h = (i >> 3) % DH, r = seen + (i >> 3) / DH;
-          *reinterpret_cast<uint4*>(v_s + vs * TILE_BYTES + h * HALF_BYTES + r * 128 + piece * 16) = make_uint4(0u, 0u, 0u, 0u);
+          const int piece = i & 7, side = (i >> 3) % DH, r = h * HALF + seen + (i >> 3) / DH;
+          *reinterpret_cast<uint4*>(v_s + vs * TILE_BYTES + side * HALF_BYTES + r * 128 + piece * 16) = make_uint4(0u, 0u, 0u, 0u);
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
-      if (lane == 0) mbar_arrive(p_full0 + 8 * slot);
+      if (lane == 0) {
+        mbar_arrive(p_full0 + 8 * (2 * slot + h));
+        if (u == 0 && slot == 0) mbar_arrive(began);
+      }
       ++done;
     }
     // ---- the slot's piece: offset, sum, accumulator. The accumulators' rows go through shared memory (all of it but the barriers: both slots'
     // products are done behind the first barrier, and every load has landed, since products have read it), so that a warp writes a row
     // of 512 bytes at a time: a thread a row wrote 16 bytes here and there, 3 us of a block's end and 8 where both slots have rows. -------
-    if (ok && done > 0) ok = __all_sync(0xffffffffu, wait_for(o_done0 + 8 * slot, (done - 1) & 1, abort_flag));
+    if (ok && done > 0) ok = __all_sync(0xffffffffu, wait_for(o_done0 + 8 * (2 * slot + ((done - 1) & 1)), ((done - 1) >> 1) & 1, abort_flag));
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     constexpr int STRIDE = D + 4;  // floats: eight lanes' 16 bytes lie in different banks
     float* stage = reinterpret_cast<float*>(smem_raw) + (turns ? 0 : slot) * BM * STRIDE;
@@ -415,6 +435,9 @@ shared_pieces_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid
       for (uint32_t i = 0; i < WAIT_LIMIT / 1024 && !mbar_try(full0 + 8 * (j % stages), (j / stages) & 1); ++i) {
       }
   }
+  if (*abort_flag && warp == WARP_Q && lane == 0 && tiles > 0)
+    for (uint32_t i = 0; i < WAIT_LIMIT / 1024 && !mbar_try(q_full, 0); ++i) {
+    }
   if (warp == WARP_MMA) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS));
   if (threadIdx.x == 0 && *abort_flag) atomicOr(a.err, OMNIA_ERR_TIMEOUT);
 }
