@@ -865,11 +865,11 @@ def rows_chunk(shape: tuple[tuple[int, int], ...], group: int, nkv: int, request
     return min(range(128, 1025, 64), key=cost)
 
 
-SHARED_TILE_US, SHARED_BLOCK_US, OWN_GBS, OWN_US = (2.0, 3.3), 6.0, 6000, 5.0
+SHARED_TILE_US, SHARED_BLOCK_US, OWN_GBS, OWN_US = (1.45, 3.3), 8.0, 6000, 5.0
 """What a tile of 128 shared keys takes a block of the tensor-core kernel (up to 128 rows, up to 256) while the decode kernel runs beside it, what a block
-takes besides, the rate at which the decode kernel reads what requests hold of their own and what it takes besides. Fitted to twelve
-shapes timed at every number of pieces: the plans made from these are the best or within 3 % for nine of them (64 answers to 65,536
-positions + 1,024: 120 blocks of 35 tiles 130 us, 152 of 27 133, 104 of 40 139), within 10 % for the rest (96 of 6,000 + 1,200: 32 blocks 87, 56 78, 16 108)."""
+takes besides, the rate at which the decode kernel reads what requests hold of their own and what it takes besides. Fitted to eighteen
+shapes timed at every number of pieces: the plans made from these are 3 % behind the best on average and 10 % at most (64 answers to 65,536
+positions + 1,024: 120 blocks of 35 tiles 119 us, 112 of 37 116, 152 of 27 121; 96 of 6,000 + 1,200: 32 blocks 84, 56 76, 16 103)."""
 
 
 @functools.lru_cache(maxsize=256)
