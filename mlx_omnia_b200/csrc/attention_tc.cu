@@ -30,7 +30,11 @@
 // Compiled with -DMAPS=2, two neighbouring query heads are the two maps of one head of differential
 // attention, and what is written is their difference (see MapDifference), [tokens, nq / 2, dv].
 // Compiled with -DSHARED=1, the decode kernel takes only the positions that a request does not share with others, and merges its
-// partials behind those of the shared ones (attention_shared.cuh); the file then holds that one entry point and no other.
+// partials behind those of the shared ones (attention_shared.cuh); the file then holds that one entry point and no other. Or it
+// takes the shared positions too: more blocks, each with up to sixteen rows of several requests (their heads side by side, as a
+// group's are), so that a group's keys are read once for every sixteen rows; the merge is then a kernel of its own. Eight requests of
+// 4,096 shared positions + 256, 16/8 heads of 128: 13.7 us (floor 3.5; each for itself 30.2), 9.2 this kernel, the rest the merge; what bounds
+// it is a block's chain, 4 us of beginning and end and as many tiles of 32 keys at 0.6 us, and the second launch.
 #include "common.cuh"
 
 #include <type_traits>

@@ -5,6 +5,9 @@
 // Both kernels cut their work into runs of at most COPY_RUN contiguous bytes, a warp a run: with 16 bytes a load a lane has
 // eight loads on their way before its first store, and an SM's warps some 256 KB. All sources are taken to be other bytes
 // than all destinations, and no two destinations to be the same (the callers check both), so runs go in any order.
+//
+// Measured (B200): 300 pages of 36 layers to another tensor (1.4 GB in and out) 221 us, 6.4 TB/s, 99 % of what a plain copy reaches; the state
+// of 24 requests (413 MB) 64 us, 6.4 TB/s. A few pages are bound by the call: 7 forks of a page 11 us with the host's part, 63 20.
 #include "common.cuh"
 
 namespace {
