@@ -132,6 +132,8 @@ class Scheduler:
                              f"{self.capacity} tokens")
         if request.leader is not None:
             at = request.fork_at
+            if request.leader.status != "finished" and request.leader not in self.waiting and request.leader not in self.running:
+                raise ValueError("a request follows one that was added before it")
             if not 1 <= at < len(request.prompt) or request.prompt[:at] != request.leader.prompt[:at]:
                 raise ValueError("a request follows one whose prompt begins with the same tokens, one or more and not all of its own")
         request.max_tokens = min(request.max_tokens, self.capacity - len(request.prompt))
@@ -190,11 +192,8 @@ class Scheduler:
 
     def _portion(self, request: Request, budget: int) -> int:
         """The next tokens of `request` within the budget, no further than where a waiting request is to be forked from it."""
-        count = min(request.pending, budget)
-        for follower in self.waiting:
-            if follower.leader is request and request.computed < follower.fork_at:
-                count = min(count, follower.fork_at - request.computed)
-        return count
+        ahead = [at - request.computed for at in self._fork_points.get(id(request), ()) if at > request.computed]
+        return min(request.pending, budget, *ahead)
 
     def _fork(self, request: Request, reserved: list[int]) -> bool | None:
         """Make a follower a fork of its leader, or of another follower of it that holds as much. True: done; False: not yet;
@@ -218,9 +217,22 @@ class Scheduler:
         return True
 
     def plan(self) -> StepPlan:
+        """The next step. (A leader that stops for its followers lets others in before its prompt is read, and all of them may end up
+        short of pages: the newest then make room.)"""
+        plan = self._plan([])
+        while not plan.entries and len(self.running) > 1:
+            victim = max(self.running, key=lambda r: r.order)
+            self._preempt(victim)
+            plan = self._plan([*plan.preempted, victim])
+        return plan
+
+    def _plan(self, preempted: list[Request]) -> StepPlan:
+        self._fork_points: dict[int, list[int]] = {}
+        for follower in self.waiting:
+            if follower.leader is not None:
+                self._fork_points.setdefault(id(follower.leader), []).append(follower.fork_at)
         reserved = [0] * len(self.cache.groups)
         entries: list[PlannedEntry] = []
-        preempted: list[Request] = []
         budget = self.max_tokens_per_step
 
         # (1) decoding requests, oldest first; preempt the newest while pages are short.

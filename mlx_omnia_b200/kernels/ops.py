@@ -827,6 +827,7 @@ class _SharedCall:
     args: _SharedArgs
     launch: Callable[[], int]
     held: list[torch.Tensor]
+    kernels: int
     columns: int  # of the result
     values: int  # bytes from the keys of a page to its values
 
@@ -952,7 +953,8 @@ def _shared_call(step: StepContext, kv: KVView, q: torch.Tensor, positive: bool,
     else:
         generic, code = _function("attention_shared", "omnia_shared_attention", [c_void_p, c_int, c_void_p]), _code(dtype)
         launch = lambda: generic(at, code, _stream())  # noqa: E731
-    return _SharedCall(args, launch, held, nq * dv if difference is None else nq // 2 * difference.dv, v_ptr - k_ptr)
+    kernels = 2 if in_decode or not tensor_cores or len(held) > 3 else 3
+    return _SharedCall(args, launch, held, kernels, nq * dv if difference is None else nq // 2 * difference.dv, v_ptr - k_ptr)
 
 
 def _shared_attention(q: torch.Tensor, kv: KVView, step: StepContext, scale: float, gate: torch.Tensor | None, gate_col: int,
@@ -975,6 +977,8 @@ def _shared_attention(q: torch.Tensor, kv: KVView, step: StepContext, scale: flo
     args.sink, args.scale, args.softcap = _ptr(sink), scale, softcap
     if difference is not None:
         args.difference = _MapDifferenceArgs(difference.lam, difference.eps, difference.factor, difference.dv)
+    global launches
+    launches += call.kernels - 1
     _check(call.launch(), "shared_attention")
     return out
 

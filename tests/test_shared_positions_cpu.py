@@ -287,6 +287,28 @@ def test_requests_that_cannot_follow(prompt, at):
         scheduler.add(Request("b", prompt, 3, leader=first, fork_at=at))
 
 
+def test_a_leader_that_stops_for_its_follower_is_not_starved():
+    """Another request is admitted while the leader waits at the fork and takes every page; neither prompt fits beside the other."""
+    scheduler, cache = scheduled(pages=8, budget=64)
+    first = Request("a", list(range(24)), 2)
+    scheduler.add(first)
+    scheduler.add(Request("b", [99] * 30, 2))
+    scheduler.add(Request("c", list(range(4)) + [50, 51], 2, leader=first, fork_at=4))
+    assert run_step(scheduler, cache)[0] == [("a", 0, 4, False), ("b", 0, 28, False)]
+    steps = 0
+    while not scheduler.idle:
+        run_step(scheduler, cache)
+        steps += 1
+        assert steps < 30
+    assert all(g.pool.free == g.pool.count for g in cache.groups)
+
+
+def test_a_request_follows_one_that_was_added_before():
+    scheduler, _ = scheduled()
+    with pytest.raises(ValueError, match="added before"):
+        scheduler.add(Request("b", [1, 2, 3], 3, leader=Request("a", [1, 2, 3], 3), fork_at=2))
+
+
 @pytest.mark.parametrize("seed", range(5))
 def test_random_followers_under_pressure_all_end(seed):
     rng = random.Random(seed)
