@@ -16,8 +16,8 @@
 //
 // Floor: the shared keys and values once, each request's own once. What bounds it is neither these nor its multiplications but a tile's
 // chain (table, rows, scores, weights), which four blocks an SM fill in part: 12 requests of 1,001 shared positions and up to 65 of
-// their own, 8/1 heads of 24 in 32 bits, 37 us (0.3 MB), where each request for itself takes 299. With a lookup of the table and a trip to
-// memory a key, as it was, 48.
+// their own, 8/1 heads of 24 in 32 bits, 17 us (0.3 MB), where each request for itself takes 299. With a lookup of the table and a trip to
+// memory a key 48, without these 37; the rest was rows one after the other, and a merge a load at a time.
 #include "attention_shared.cuh"
 
 namespace {
@@ -28,6 +28,66 @@ constexpr float LOG2E = 1.4426950408889634f;
 }  // namespace
 
 namespace {
+
+// A tile of up to 32 keys for N of a warp's rows (every WARPS-th row of the block), all at once and without a branch between them, so that their
+// reductions overlap. Rows beyond the block's hold zeros and are written nowhere.
+template <int N, int ACC>
+__device__ __forceinline__ void attend_rows(const float* q, const float* ks, const float* vs, int stride, int width4, int dv, int keys, bool capped,
+                                            float pre, float cap, float* m, float* l, float (*acc)[ACC]) {
+  const int lane = threadIdx.x & 31;
+  float s[N];
+#pragma unroll
+  for (int x = 0; x < N; ++x) s[x] = 0.f;
+  const float4* k4 = reinterpret_cast<const float4*>(ks + lane * stride);
+#pragma unroll 2
+  for (int c = 0; c < width4; ++c) {
+    const float4 k = k4[c];
+#pragma unroll
+    for (int x = 0; x < N; ++x) {
+      const float4 v = reinterpret_cast<const float4*>(q + WARPS * x * stride)[c];
+      s[x] = fmaf(v.x, k.x, fmaf(v.y, k.y, fmaf(v.z, k.z, fmaf(v.w, k.w, s[x]))));
+    }
+  }
+  float top[N], sum[N];
+#pragma unroll
+  for (int x = 0; x < N; ++x) {
+    s[x] = capped ? cap * tanhf(s[x] * pre) : s[x] * pre;
+    if (lane >= keys) s[x] = -INFINITY;
+    top[x] = s[x];
+  }
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1)
+#pragma unroll
+    for (int x = 0; x < N; ++x) top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], off));
+#pragma unroll
+  for (int x = 0; x < N; ++x) {
+    top[x] = fmaxf(m[x], top[x]);
+    const float base = top[x] == -INFINITY ? 0.f : top[x];
+    const float alpha = m[x] == -INFINITY ? 0.f : exp2f(m[x] - base);
+    s[x] = sum[x] = exp2f(s[x] - base);
+    m[x] = top[x], l[x] *= alpha;
+#pragma unroll
+    for (int k = 0; k < ACC; ++k) acc[x][k] *= alpha;
+  }
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1)
+#pragma unroll
+    for (int x = 0; x < N; ++x) sum[x] += __shfl_xor_sync(0xffffffffu, sum[x], off);
+#pragma unroll
+  for (int x = 0; x < N; ++x) l[x] += sum[x];
+#pragma unroll 4
+  for (int k = 0; k < TILE; ++k) {  // (keys past the last have no weight, and zeros for values)
+    float v[ACC];
+#pragma unroll
+    for (int i = 0; i < ACC; ++i) v[i] = lane + 32 * i < dv ? vs[k * dv + lane + 32 * i] : 0.f;
+#pragma unroll
+    for (int x = 0; x < N; ++x) {
+      const float p = __shfl_sync(0xffffffffu, s[x], k);
+#pragma unroll
+      for (int i = 0; i < ACC; ++i) acc[x][i] = fmaf(p, v[i], acc[x][i]);
+    }
+  }
+}
 
 template <typename T, int MOST>
 __global__ void __launch_bounds__(32 * WARPS)
@@ -132,45 +192,10 @@ shared_pieces_kernel(const __grid_constant__ SharedAttention a) {
         }
     }
     __syncthreads();
-    float s[PER_WARP];
-#pragma unroll
-    for (int x = 0; x < PER_WARP; ++x) s[x] = 0.f;
-    const float4* k4 = reinterpret_cast<const float4*>(ks + lane * stride);
-    for (int c = 0; c < width4; ++c) {
-      const float4 k = k4[c];
-#pragma unroll
-      for (int x = 0; x < PER_WARP; ++x) {
-        if (warp + WARPS * x >= rows) break;
-        const float4 v = reinterpret_cast<const float4*>(qs + (warp + WARPS * x) * stride)[c];
-        s[x] = fmaf(v.x, k.x, fmaf(v.y, k.y, fmaf(v.z, k.z, fmaf(v.w, k.w, s[x]))));
-      }
-    }
-#pragma unroll
-    for (int x = 0; x < PER_WARP; ++x) {
-      if (warp + WARPS * x >= rows) break;
-      float z = a.softcap > 0.f ? cap * tanhf(s[x] * pre) : s[x] * pre;
-      if (lane >= keys) z = -INFINITY;
-      const float top = fmaxf(m[x], warp_max(z));
-      const float base = top == -INFINITY ? 0.f : top;
-      const float p = exp2f(z - base), alpha = m[x] == -INFINITY ? 0.f : exp2f(m[x] - base);
-      m[x] = top;
-      l[x] = l[x] * alpha + warp_sum(p);
-#pragma unroll
-      for (int k = 0; k < ACC; ++k) acc[x][k] *= alpha;
-      s[x] = p;
-    }
-    for (int k = 0; k < keys; ++k) {
-      float v[ACC];
-#pragma unroll
-      for (int i = 0; i < ACC; ++i) v[i] = lane + 32 * i < a.dv ? vs[k * a.dv + lane + 32 * i] : 0.f;
-#pragma unroll
-      for (int x = 0; x < PER_WARP; ++x) {
-        if (warp + WARPS * x >= rows) break;
-        const float p = __shfl_sync(0xffffffffu, s[x], k);
-#pragma unroll
-        for (int i = 0; i < ACC; ++i) acc[x][i] = fmaf(p, v[i], acc[x][i]);
-      }
-    }
+    if (rows > 2 * WARPS)
+      attend_rows<PER_WARP, ACC>(qs + warp * stride, ks, vs, stride, width4, a.dv, keys, a.softcap > 0.f, pre, cap, m, l, acc);
+    else
+      attend_rows<2, ACC>(qs + warp * stride, ks, vs, stride, width4, a.dv, keys, a.softcap > 0.f, pre, cap, m, l, acc);
   }
   const int places = a.max_parts + a.max_chunks;
 #pragma unroll
@@ -197,6 +222,7 @@ shared_merge_kernel(const __grid_constant__ SharedAttention a) {
   const int request = blockIdx.y, tid = threadIdx.x;
   const int own = a.seq_lens[request] - a.plan[request];
   if (a.seq_lens[request] < 1) return;
+  if (own > a.max_chunks * (long long)a.chunk_keys && blockIdx.x == 0 && tid == 0) atomicOr(a.err, OMNIA_ERR_WORK);  // more than the step was laid out for
   const int count = min(a.plan[a.requests + request], a.max_parts) + max(0, min((own + a.chunk_keys - 1) / a.chunk_keys, a.max_chunks));
   const int places = a.max_parts + a.max_chunks;
   const size_t token = (size_t)a.cu_seqlens[request];
@@ -209,15 +235,30 @@ shared_merge_kernel(const __grid_constant__ SharedAttention a) {
     const size_t at = ((size_t)request * a.nq + head) * places;
     const float *ml = a.part_ml + 2 * at, *o = a.part_o + at * a.dv;
     float top = -INFINITY, total = 0.f;
-    for (int i = 0; i < count; ++i) top = fmaxf(top, ml[2 * i]);
 #pragma unroll
     for (int v = 0; v < PER_THREAD; ++v) map[which][v] = 0.f;
-    for (int i = 0; i < count; ++i) {
-      const float w = ml[2 * i] == -INFINITY ? 0.f : exp2f(ml[2 * i] - top);
-      total += ml[2 * i + 1] * w;
+    // Rounds of 32 pieces: a lane has one's maximum and sum; then eight accumulators on their way at a time.
+    for (int done = 0; done < count; done += 32) {
+      const int some = min(32, count - done), lane = tid & 31;
+      const float m = lane < some ? __ldcg(ml + 2 * (done + lane)) : -INFINITY, l = lane < some ? __ldcg(ml + 2 * (done + lane) + 1) : 0.f;
+      const float now = fmaxf(top, warp_max(m)), keep = top == -INFINITY ? 0.f : exp2f(top - now);
+      const float w = m == -INFINITY ? 0.f : exp2f(m - now);
+      total = total * keep + warp_sum(l * w);
 #pragma unroll
-      for (int v = 0; v < PER_THREAD; ++v)
-        if (tid + 128 * v < a.dv) map[which][v] += o[(size_t)i * a.dv + tid + 128 * v] * w;
+      for (int v = 0; v < PER_THREAD; ++v) map[which][v] *= keep;
+      top = now;
+      for (int i0 = 0; i0 < some; i0 += 8) {
+#pragma unroll
+        for (int v = 0; v < PER_THREAD; ++v) {
+          if (128 * v >= a.dv) break;
+          const int dim = tid + 128 * v;
+          float x[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] = i0 + i < some && dim < a.dv ? __ldcg(o + (size_t)(done + i0 + i) * a.dv + dim) : 0.f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) map[which][v] = fmaf(x[i], __shfl_sync(0xffffffffu, w, i0 + i), map[which][v]);
+        }
+      }
     }
     if (a.sink != nullptr && top != -INFINITY) total += exp2f(a.sink[head] * LOG2E - top);
     const float inv = total > 0.f ? 1.f / total : 0.f;

@@ -38,13 +38,15 @@ constexpr int D = HEAD_DIM;
 static_assert(D == 64 || D == 128, "head sizes 64 and 128");
 static_assert(GROUP >= 1 && GROUP <= 16, "group size must be 1..16");
 constexpr int DH = D / 64;               // 64-wide halves of a head
+constexpr int BAR_BYTES = 384;           // of shared memory, for barriers
 constexpr int BM = 128, BN = 128, HALF = 64;  // rows of a slot, keys of a tile, of the halves that are worked on
 constexpr int SLOT_ROWS = BM / GROUP * GROUP;
-// Seven tiles of shared memory: the rows (one tile where both slots hold the same, else two), the rest but the last two for
-// keys, two for values. A stage's loads, products and barriers go by one order of tiles; where the slots take turns each has stages
-// of its own (the even or the odd ones), filled by a warp of its own: a stage that both used would complete a phase which the slower
-// slot has yet to wait for.
-constexpr int TILES = 7, V_STAGES = 2, K_STAGES = 4;  // (three for keys where there are two tiles of rows)
+// Seven tiles of shared memory: the rows (one tile where both slots hold the same, else two), the rest in stages of a half tile, as many for keys
+// as for values: five each that both slots read, or, where the slots take turns with the tiles, three each a slot, of its own halves: a stage
+// that both used in turns would complete a phase which the slower slot has yet to wait for. (Whole tiles, four stages for keys and two for
+// values, left a slot that takes turns one stage of values, asked for when the weights were already on their way: 16 requests of 32,768
+// positions 45.3 us, so 44.6; 4 of 65,536 63.5 and 59.0.)
+constexpr int TILES = 7, OWN_STAGES = 3, BOTH_STAGES = 5, MOST_STAGES = 2 * OWN_STAGES;
 constexpr int SOFTMAX_THREADS = 256;     // warps 0-3 slot 0, 4-7 slot 1
 constexpr int SLOT_MEMBERS = BM / GROUP, Q_MEMBERS = 8;  // requests of a slot's rows, of a box of queries
 constexpr int WARP_MMA = 8, WARP_K = 10, WARP_V = 12, WARP_Q = 14, FEEDERS = 2;  // one issuer a slot; two warps feed each ring in turns
@@ -55,6 +57,9 @@ static_assert(2 * SLOT_REGS + 2 * OTHER_REGS == 4 * (65536 / THREADS), "a regist
 constexpr uint32_t HALF_BYTES = 128 * 128;   // 128 rows of 128 bytes
 constexpr uint32_t TILE_BYTES = DH * HALF_BYTES;
 constexpr uint32_t BOX_BYTES = 16 * 128;     // 16 keys x 64 dims
+constexpr uint32_t SIDE_BYTES = HALF * 128, STAGE_BYTES = DH * SIDE_BYTES;  // of half a tile of keys or values
+static_assert(TILE_BYTES + 2 * MOST_STAGES * STAGE_BYTES <= TILES * TILE_BYTES && 2 * TILE_BYTES + 2 * BOTH_STAGES * STAGE_BYTES <= TILES * TILE_BYTES,
+              "rows and stages fit");
 constexpr uint32_t TMEM_COLS = 512, O_COL = 2 * BN;  // two score tiles, then two accumulators
 
 // mbar_wait without a time to sleep for: a warp that asks for one wakes up later.
@@ -88,16 +93,16 @@ shared_pieces_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid
     return;
   }
   unsigned char* q_s = smem_raw;
-  unsigned char* v_s = q_s + (TILES - V_STAGES) * TILE_BYTES;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(v_s + V_STAGES * TILE_BYTES);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(q_s + TILES * TILE_BYTES);
   // bars: q_full | k_full[] | k_empty[] | v_full[] | v_empty[] | s_full[2][2] | p_full[2][2] | o_done[2][2] (slot, half) | began
-  constexpr int BARS = 1 + 2 * K_STAGES + 2 * V_STAGES + 13;
+  constexpr int BARS = 1 + 4 * MOST_STAGES + 13;
+  static_assert(BARS * 8 + 8 <= BAR_BYTES, "barriers and the two words behind them");
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + BARS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
   float* row_ml = reinterpret_cast<float*>(tmem_holder + 2);  // [2][128][2]: a slot's offset and sum, for the other one
   const int warp = omnia_warp_index(), lane = threadIdx.x & 31;
-  const uint32_t q_full = smem_u32(bars), k_full0 = q_full + 8, k_empty0 = k_full0 + 8 * K_STAGES, v_full0 = k_empty0 + 8 * K_STAGES,
-                 v_empty0 = v_full0 + 8 * V_STAGES, s_full0 = v_empty0 + 8 * V_STAGES, p_full0 = s_full0 + 32, o_done0 = p_full0 + 32,
+  const uint32_t q_full = smem_u32(bars), k_full0 = q_full + 8, k_empty0 = k_full0 + 8 * MOST_STAGES, v_full0 = k_empty0 + 8 * MOST_STAGES,
+                 v_empty0 = v_full0 + 8 * MOST_STAGES, s_full0 = v_empty0 + 8 * MOST_STAGES, p_full0 = s_full0 + 32, o_done0 = p_full0 + 32,
                  began = o_done0 + 32;
   if (warp == WARP_MMA) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)), "r"(TMEM_COLS));
@@ -109,14 +114,15 @@ shared_pieces_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid
   const int *members = a.plan + 2 * a.requests, *item = members + a.members + SHARED_ITEM_INTS * blockIdx.x;
   const int table_of = item[0], first_member = item[1], row0 = item[2], rows = item[3], kvh = item[4], lo = item[5], hi = item[6], part = item[7];
   const bool turns = rows <= SLOT_ROWS;           // both slots hold the same rows and take the tiles in turn
-  const int k_stages = turns ? K_STAGES : K_STAGES - 1;
-  unsigned char* k_s = v_s - k_stages * TILE_BYTES;
+  const int stages = turns ? OWN_STAGES : BOTH_STAGES;  // of a ring
+  unsigned char* k_s = q_s + (turns ? 1 : 2) * TILE_BYTES;
+  unsigned char* v_s = k_s + (turns ? MOST_STAGES : BOTH_STAGES) * STAGE_BYTES;
   const int tiles = rows < 1 ? 0 : (hi - lo + BN - 1) / BN;
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
     const int readers = turns ? 1 : 2;
-    for (int s = 0; s < K_STAGES; ++s) mbar_init(k_full0 + 8 * s, 1), mbar_init(k_empty0 + 8 * s, readers);
-    for (int s = 0; s < V_STAGES; ++s) mbar_init(v_full0 + 8 * s, 1), mbar_init(v_empty0 + 8 * s, readers);
+    for (int s = 0; s < MOST_STAGES; ++s) mbar_init(k_full0 + 8 * s, 1), mbar_init(k_empty0 + 8 * s, readers);
+    for (int s = 0; s < MOST_STAGES; ++s) mbar_init(v_full0 + 8 * s, 1), mbar_init(v_empty0 + 8 * s, readers);
     for (int s = 0; s < 4; ++s) mbar_init(s_full0 + 8 * s, 1), mbar_init(p_full0 + 8 * s, BM / 32), mbar_init(o_done0 + 8 * s, 1);
     mbar_init(began, BM / 32);
     *abort_flag = 0;
@@ -126,13 +132,17 @@ shared_pieces_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem_base = *tmem_holder;
-  int issued = -1;  // the last tile that this warp has asked for
+  int issued = -1;  // the last half tile that this warp has asked for
   // A slot's sequence of half tiles: half u is the (u & 1)th of the tile j0 + (u >> 1) * step.
   const int step = turns ? 2 : 1;
   auto halves_of = [&](int j0) {
     const int mine = tiles > j0 ? (tiles - j0 + step - 1) / step : 0, last = j0 + (mine - 1) * step;
     return mine < 1 ? 0 : 2 * mine - (hi - lo - last * BN <= HALF ? 1 : 0);
   };
+  auto first_of = [&](int j0, int u) { return lo + (j0 + (u >> 1) * step) * BN + (u & 1) * HALF; };  // its first key
+  // Half u's stage, and the parity of the phase in which it is full.
+  auto stage_of = [&](int slot, int u) { return (turns ? slot * OWN_STAGES : 0) + u % stages; };
+  auto phase_of = [&](int u) { return (u / stages) & 1; };
 
   if (warp >= WARP_MMA) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
   if (warp > WARP_Q) {
@@ -162,40 +172,41 @@ shared_pieces_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid
       }
     }
   } else if (warp >= WARP_K) {
-    // ---- producers: two warps a ring take turns with its stages; a lane looks up a box's page, one lane asks for the boxes ----
-    const int which = warp >= WARP_V ? 1 : 0, turn = warp - (which ? WARP_V : WARP_K), stages = which ? V_STAGES : k_stages;
+    // ---- producers: two warps a ring, one a slot or taking turns; a lane looks up a box's page, one lane asks for the boxes ----
+    const int which = warp >= WARP_V ? 1 : 0, turn = warp - (which ? WARP_V : WARP_K), j0 = turns ? turn : 0, halves = halves_of(j0);
     const int* table = a.block_table + (size_t)table_of * a.max_pages;
     const uint32_t full0 = which ? v_full0 : k_full0, empty0 = which ? v_empty0 : k_empty0;
-    auto lookup = [&](int j) {  // the page of this lane's 16 keys of tile j (-2: none that the item reads)
-      const int pos = lo + j * BN + lane * 16;
-      return lane < BN / 16 && j < tiles && pos < hi ? table[pos / a.page_size] : -2;
+    const int u0 = turns ? 0 : turn, du = turns ? 1 : FEEDERS;
+    auto lookup = [&](int u) {  // the page of this lane's 16 keys of half u (-2: none that the item reads)
+      const int pos = first_of(j0, u) + lane * 16;
+      return lane < HALF / 16 && u < halves && pos < hi ? table[pos / a.page_size] : -2;
     };
     bool ok = true;
-    int page_cur = lookup(turn);
-    for (int j = turn; j < tiles; j += FEEDERS) {
-      const int page_next = lookup(j + FEEDERS), s = j % stages, pos = lo + j * BN + lane * 16;
-      if (lane == 0 && j >= stages) ok = wait_for(empty0 + 8 * s, ((j / stages) & 1) ^ 1, abort_flag);
+    int page_cur = lookup(u0);
+    for (int u = u0; u < halves; u += du) {
+      const int page_next = lookup(u + du), s = stage_of(turn, u), pos = first_of(j0, u) + lane * 16;
+      if (lane == 0 && u >= stages) ok = wait_for(empty0 + 8 * s, phase_of(u) ^ 1, abort_flag);
       ok = __shfl_sync(0xffffffffu, ok, 0);
       if (!ok) break;
       bool load = page_cur != -2;
       if (load && (page_cur < 0 || page_cur >= a.num_pages)) atomicOr(a.err, OMNIA_ERR_PAGE), load = false;
       const uint32_t loaded = __ballot_sync(0xffffffffu, load);
       const int mine = load ? ((page_cur * 2 + which) * a.nkv + kvh) * a.page_size + pos % a.page_size : 0;
-      int y[BN / 16];
+      int y[HALF / 16];
 #pragma unroll
-      for (int x = 0; x < BN / 16; ++x) y[x] = __shfl_sync(0xffffffffu, mine, x);
+      for (int x = 0; x < HALF / 16; ++x) y[x] = __shfl_sync(0xffffffffu, mine, x);
       if (omnia_elect_one()) {
         mbar_expect_tx(full0 + 8 * s, __popc(loaded) * DH * BOX_BYTES);
-        const uint32_t dst = smem_u32((which ? v_s : k_s) + s * TILE_BYTES);
+        const uint32_t dst = smem_u32((which ? v_s : k_s) + s * STAGE_BYTES);
 #pragma unroll
-        for (int x = 0; x < BN / 16; ++x)
+        for (int x = 0; x < HALF / 16; ++x)
           if ((loaded >> x) & 1u)
 #pragma unroll
-            for (int half = 0; half < DH; ++half)
-              tma_load_2d(dst + half * HALF_BYTES + x * BOX_BYTES, &map_kv, full0 + 8 * s, half * 64, y[x]);
+            for (int side = 0; side < DH; ++side)
+              tma_load_2d(dst + side * SIDE_BYTES + x * BOX_BYTES, &map_kv, full0 + 8 * s, side * 64, y[x]);
       }
       __syncwarp();
-      issued = j;
+      issued = u;
       page_cur = page_next;
     }
   } else if (warp >= WARP_MMA) {
@@ -211,36 +222,36 @@ shared_pieces_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid
       // not beside the other one's exponentials.
       if (slot == 1 && tiles > 1 && ok) ok = wait_for(began, 0, abort_flag);
       auto scores = [&](int u) {
-        const int h = u & 1, j = j0 + (u >> 1) * step, ks = j % k_stages;
-        if (h == 0) ok = wait_for(k_full0 + 8 * ks, (j / k_stages) & 1, abort_flag);
+        const int h = u & 1, s = stage_of(slot, u);
+        ok = wait_for(k_full0 + 8 * s, phase_of(u), abort_flag);
         if (!ok) return;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint64_t k_desc = desc_k_major(smem_u32(k_s + ks * TILE_BYTES + h * (HALF * 128)));
+        const uint64_t k_desc = desc_k_major(smem_u32(k_s + s * STAGE_BYTES));
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk)
-          umma(s_tmem + h * HALF, q_desc + (((kk / 4) * HALF_BYTES + (kk % 4) * 32) >> 4), k_desc + (((kk / 4) * HALF_BYTES + (kk % 4) * 32) >> 4),
+          umma(s_tmem + h * HALF, q_desc + (((kk / 4) * HALF_BYTES + (kk % 4) * 32) >> 4), k_desc + (((kk / 4) * SIDE_BYTES + (kk % 4) * 32) >> 4),
                instr_s, kk != 0);
         umma_commit(s_full0 + 8 * (2 * slot + h));
-        if (h == 1 || u == halves - 1) umma_commit(k_empty0 + 8 * ks);
+        umma_commit(k_empty0 + 8 * s);
       };
       if (ok) scores(0);
       if (ok && halves > 1) scores(1);
       for (int u = 0; u < halves && ok; ++u) {
-        const int h = u & 1, t = u >> 1, j = j0 + t * step, vs = j % V_STAGES;
-        ok = (h == 1 || wait_for(v_full0 + 8 * vs, (j / V_STAGES) & 1, abort_flag)) && wait_for(p_full0 + 8 * (2 * slot + h), t & 1, abort_flag);
+        const int h = u & 1, t = u >> 1, s = stage_of(slot, u);
+        ok = wait_for(v_full0 + 8 * s, phase_of(u), abort_flag) && wait_for(p_full0 + 8 * (2 * slot + h), t & 1, abort_flag);
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint64_t v_desc = desc_mn_major(smem_u32(v_s + vs * TILE_BYTES), HALF_BYTES);
-        const int groups = min(HALF, hi - lo - j * BN - h * HALF + 15) / 16;  // boxes that were loaded: the rest of the stage is stale
+        const uint64_t v_desc = desc_mn_major(smem_u32(v_s + s * STAGE_BYTES), SIDE_BYTES);
+        const int groups = min(HALF, hi - first_of(j0, u) + 15) / 16;  // boxes that were loaded: the rest of the stage is stale
 #pragma unroll
         for (int kk = 0; kk < HALF / 16; ++kk) {
           if (kk >= groups) break;
           // P: 16 keys are eight columns of packed pairs
-          umma_ts(o_tmem, s_tmem + h * HALF + kk * 8, v_desc + (((h * (HALF / 16) + kk) * BOX_BYTES) >> 4), instr_o, accumulate);
+          umma_ts(o_tmem, s_tmem + h * HALF + kk * 8, v_desc + ((kk * BOX_BYTES) >> 4), instr_o, accumulate);
           accumulate = 1;
         }
         umma_commit(o_done0 + 8 * (2 * slot + h));
-        if (h == 1 || u == halves - 1) umma_commit(v_empty0 + 8 * vs);
+        umma_commit(v_empty0 + 8 * s);
         // The half's columns are free once its weights have been read.
         if (u + 2 < halves) {
           ok = wait_for(o_done0 + 8 * (2 * slot + h), t & 1, abort_flag);
@@ -271,14 +282,14 @@ shared_pieces_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid
     const int j0 = turns ? slot : 0, halves = halves_of(j0);
     for (int u = halves > 0 ? -1 : 0; u < halves; ++u) {
       const bool dry = u < 0;
-      const int h = dry ? 0 : u & 1, t = u >> 1, j = j0 + t * step;
+      const int h = dry ? 0 : u & 1, t = u >> 1;
       const uint32_t half_addr = s_addr + h * HALF;
       if (!dry) {
         ok = __all_sync(0xffffffffu, wait_for(s_full0 + 8 * (2 * slot + h), t & 1, abort_flag));
         if (!ok) break;
       }
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const int seen = dry ? HALF : min(HALF, hi - lo - j * BN - h * HALF);  // keys of this half; the columns beyond hold whatever the stage held
+      const int seen = dry ? HALF : min(HALF, hi - first_of(j0, u));  // keys of this half; the columns beyond hold whatever the stage held
       // All of the row's scores at once: a load from tensor memory takes some 0.35 us to arrive.
       float z[HALF];
       {
@@ -347,14 +358,14 @@ shared_pieces_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid
       if (seen & 15) {
         // The last box reaches past the last key. Its rows of V beyond get no weight, but what they hold need not be a number
         // (0 x NaN is NaN): they are cleared once the stage has landed, by both slots where both read it.
-        const int vs = j % V_STAGES;
-        ok = __all_sync(0xffffffffu, wait_for(v_full0 + 8 * vs, (j / V_STAGES) & 1, abort_flag));
+        const int s = stage_of(slot, u);
+        ok = __all_sync(0xffffffffu, wait_for(v_full0 + 8 * s, phase_of(u), abort_flag));
         if (!ok) break;
         const int r1 = (seen + 15) & ~15;
 #pragma unroll 1
         for (int i = row; i < (r1 - seen) * DH * 8; i += BM) {
-          const int piece = i & 7, side = (i >> 3) % DH, r = h * HALF + seen + (i >> 3) / DH;
-          *reinterpret_cast<uint4*>(v_s + vs * TILE_BYTES + side * HALF_BYTES + r * 128 + piece * 16) = make_uint4(0u, 0u, 0u, 0u);
+          const int piece = i & 7, side = (i >> 3) % DH, r = seen + (i >> 3) / DH;
+          *reinterpret_cast<uint4*>(v_s + s * STAGE_BYTES + side * SIDE_BYTES + r * 128 + piece * 16) = make_uint4(0u, 0u, 0u, 0u);
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       }
@@ -433,13 +444,13 @@ shared_pieces_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
-  if (*abort_flag && warp >= WARP_K && lane == 0) {
+  if (*abort_flag && warp >= WARP_K && warp < WARP_Q && lane == 0) {
     // Given up: what this warp has asked for must land before the block's shared memory goes away. (Its last copies, one a stage; a
     // stage that the ring's other warp has filled since reads as not complete, so the wait is short.)
-    const int stages = warp >= WARP_V ? V_STAGES : k_stages;
     const uint32_t full0 = warp >= WARP_V ? v_full0 : k_full0;
-    for (int j = issued; j >= 0 && j > issued - stages; j -= FEEDERS)
-      for (uint32_t i = 0; i < WAIT_LIMIT / 1024 && !mbar_try(full0 + 8 * (j % stages), (j / stages) & 1); ++i) {
+    const int turn = warp - (warp >= WARP_V ? WARP_V : WARP_K);
+    for (int u = issued; u >= 0 && u > issued - stages; u -= turns ? 1 : FEEDERS)
+      for (uint32_t i = 0; i < WAIT_LIMIT / 1024 && !mbar_try(full0 + 8 * stage_of(turn, u), phase_of(u)); ++i) {
       }
   }
   if (*abort_flag && warp == WARP_Q && lane == 0 && tiles > 0)
@@ -475,7 +486,7 @@ shared_merge_tc_kernel(const __grid_constant__ SharedAttention a) {
   pdl_wait();
   pdl_launch_dependents();
   if (pos < 0) return;
-  const int places = a.max_parts + a.max_chunks, pieces = parts + (pos < start ? 0 : pos / a.chunk_keys - start / a.chunk_keys + 1);
+  const int places = a.max_parts + a.max_chunks, pieces = parts + (pos < start ? 0 : min(pos / a.chunk_keys - start / a.chunk_keys + 1, a.max_chunks));
   for (int h0 = 0; h0 < GROUP; h0 += MERGE_HEADS) {
     if (h0 > 0) ask_for_gates(h0);
     const int h = warp / HEAD_WARPS, sub = warp % HEAD_WARPS, r = h0 + h;
@@ -599,7 +610,7 @@ extern "C" int omnia_shared_pieces_tc(const SharedAttention* given, cudaStream_t
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
       return (int)cudaErrorInvalidValue;
   }
-  constexpr size_t smem = TILES * (size_t)TILE_BYTES + 256 + 4 * BM * sizeof(float);
+  constexpr size_t smem = TILES * (size_t)TILE_BYTES + BAR_BYTES + 4 * BM * sizeof(float);
   static bool configured[64] = {};
   int device = 0;
   if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) return (int)cudaErrorInvalidDevice;

@@ -699,6 +699,10 @@ attention_decode_kernel(const bf16* q, const bf16* __restrict__ pages,
     }
     chunks = pos / chunk_keys - c0 + 1;
 #if SHARED
+    if (chunks > max_chunks) {  // more of its own than the step was laid out for
+      chunks = max_chunks;
+      if (threadIdx.x == 0) atomicOr(err, OMNIA_ERR_WORK);
+    }
     max_chunks += max_parts;  // (of the partials' places, from here on)
 #endif
     part_o += (size_t)request * nq * max_chunks * D, part_ml += (size_t)request * nq * max_chunks * 2;

@@ -149,7 +149,7 @@ class Scheduler:
         for request in list(self.waiting):
             if request.request_id == request_id:
                 self.waiting.remove(request)
-                request.status, request.finish_reason = "finished", "abort"
+                request.status, request.finish_reason, request.leader = "finished", "abort", None
                 return request
         return None
 
@@ -173,7 +173,7 @@ class Scheduler:
             request.cache = None
         if request in self.running:
             self.running.remove(request)
-        request.status, request.finish_reason = "finished", reason
+        request.status, request.finish_reason, request.leader = "finished", reason, None
 
     def _affordable(self, request: Request, wanted: int, reserved: list[int]) -> int:
         """The largest portion <= wanted whose pages are free in every group, `reserved`

@@ -792,7 +792,7 @@ place of one, and that one also takes the projected rows as they are (2 to 3 us 
 of 128, 2 requests of 200 + 8 positions (0.8 MB) 7.9 / 6.5, 8 of 300 + 30 (9 MB) 10.6 / 10.4, 4 of 1,000 + 30 (12 MB) 10.5 / 10.8, 2 of 4,000 + 500 (16 MB)
 11.9 / 13.4, 8 of 1,000 + 30 (29 MB) 11.1 / 12.4, 16 of 1,000 + 30 (61 MB) 12.1 / 18.7; 6/2 heads of 64, 8 of 4,000 + 30 (14 MB) 9.9 / 9.7, of
 16,000 (57 MB) 16.2 / 19.6. The kernel for other types and sizes is the faster one from the first positions on (32 bits, 16/8 heads of 128, 2 requests of
-64 + 30 positions 13.7 / 43.5, 16 of 100 + 30 37 / 61): the ordinary kernel for these walks a request's keys in one block. It is not where bfloat16 of
+64 + 30 positions 8.0 / 43.3, 16 of 100 + 30 20.7 / 61.3): the ordinary kernel for these walks a request's keys in one block. It is not where bfloat16 of
 other head sizes has a tensor-core decode kernel to itself (8/2 heads of 256, 32 of 4,000 + 100 137 / 54; 8/8 of 96, 81 / 46), so that stays."""
 
 
@@ -816,6 +816,8 @@ def _own_longest(step: StepContext) -> int:
     """The most positions that a request of the step holds beyond those that it shares."""
     if step.max_own is not None:
         return step.max_own
+    if not step.seq_lens_host:
+        return step.max_seq_len  # lengths that the host does not know
     starts = {m: positions for positions, members in step.shared for m in members}
     return max((n - starts.get(r, 0) for r, n in enumerate(step.seq_lens_host)), default=0)
 
@@ -967,6 +969,8 @@ def _shared_attention(q: torch.Tensor, kv: KVView, step: StepContext, scale: flo
     call = step.workspace.get(key)
     if call is None:
         call = step.workspace[key] = _shared_call(step, kv, q, scale > 0, difference)
+    if q.data_ptr() & 15:
+        q = q.clone()  # the tensor-core kernel's queries come by TMA, from 16-byte boundaries
     out = torch.empty(q.shape[0], call.columns, dtype=q.dtype, device=q.device)
     args, base = call.args, pages.data_ptr()
     args.q, args.k_pages, args.v_pages, args.out, args.block_table = q.data_ptr(), base, base + call.values, out.data_ptr(), table.data_ptr()

@@ -348,6 +348,36 @@ def test_a_page_that_is_not_there_is_an_error():
             ops.raise_on_error(case.q.device)
 
 
+@pytest.mark.parametrize("layout", ["16/8x128", "8/1x24 f32"])
+def test_more_of_its_own_than_a_step_was_laid_out_for_is_an_error(layout, way):
+    nq, nkv, d, dtype, page = LAYOUTS[layout]
+    case = make(nq, nkv, d, dtype, page, [(200, [1, 1900])], alone=())
+    case.step.max_own = 64
+    ops.paged_attention(case.q, case.kv, case.step, 0.1)
+    with pytest.raises(ops.KernelError):
+        ops.raise_on_error(case.q.device)
+    case.step.workspace, case.step.max_own = None, None
+    check(case)
+
+
+@pytest.mark.parametrize("layout", ["16/8x128", "8/1x24 f32"])
+def test_lengths_that_the_host_does_not_know(layout, way):
+    nq, nkv, d, dtype, page = LAYOUTS[layout]
+    case = make(nq, nkv, d, dtype, page, [(200, [1, 1900, 30])])
+    case.step.seq_lens_host = []
+    check(case)
+
+
+@pytest.mark.parametrize("layout", ["16/8x128", "6/2x64"])
+def test_queries_off_a_16_byte_boundary(layout, way):
+    nq, nkv, d, dtype, page = LAYOUTS[layout]
+    case = make(nq, nkv, d, dtype, page, [(200, [1, 190, 30])])
+    held = torch.empty(case.q.numel() + 1, dtype=dtype, device="cuda")
+    held[1:] = case.q.flatten()
+    case.q = held[1:].view_as(case.q)
+    check(case)
+
+
 # -- copies -------------------------------------------------------------------------------------------------------------
 def bits(shape, dtype, seed=0):
     g = torch.Generator(device="cuda").manual_seed(seed)
