@@ -213,15 +213,16 @@ shared_pieces_kernel(const __grid_constant__ SharedAttention a) {
 }
 
 // grid (heads that come out, requests), 128 threads: a request's pieces put together in ascending order.
+// What a request holds of its own was cut from its first such position on or (`fixed`: by the decode kernel) at multiples of chunk_keys.
 template <typename T>
 __global__ void __launch_bounds__(128)
-shared_merge_kernel(const __grid_constant__ SharedAttention a) {
+shared_merge_kernel(const __grid_constant__ SharedAttention a, int fixed) {
   __shared__ float scratch[33];
   pdl_wait();
   pdl_launch_dependents();
   const int request = blockIdx.y, tid = threadIdx.x;
-  const int own = a.seq_lens[request] - a.plan[request];
   if (a.seq_lens[request] < 1) return;
+  const int start = a.plan[request], own = a.seq_lens[request] - (fixed ? start / a.chunk_keys * a.chunk_keys : start);
   if (own > a.max_chunks * (long long)a.chunk_keys && blockIdx.x == 0 && tid == 0) atomicOr(a.err, OMNIA_ERR_WORK);  // more than the step was laid out for
   const int count = min(a.plan[a.requests + request], a.max_parts) + max(0, min((own + a.chunk_keys - 1) / a.chunk_keys, a.max_chunks));
   const int places = a.max_parts + a.max_chunks;
@@ -307,6 +308,18 @@ int launch_pieces(const SharedAttention& a, long long blocks, size_t smem, cudaS
 
 }  // namespace
 
+// The pieces that the decode kernel has left (omnia_attention_decode_shared with `rows`), of any width.
+extern "C" int omnia_shared_merge(const SharedAttention* given, int dtype, cudaStream_t stream) {
+  const SharedAttention a = *given;
+  if (a.requests == 0) return 0;
+  if (a.requests < 0 || a.requests > 65535 || a.nkv < 1 || a.nq < 1 || a.nq % a.nkv || a.dv < 1 || a.dv > 512 || a.max_parts < 0 || a.max_chunks < 0 ||
+      a.chunk_keys < 1 || (a.maps != 1 && a.maps != 2) ||
+      (a.maps == 2 && (a.nq % 2 || a.gate || a.sink || a.difference.dv < 1 || a.difference.dv > a.dv)))
+    return (int)cudaErrorInvalidValue;
+  OMNIA_DISPATCH_DTYPE(dtype, launch_pdl(shared_merge_kernel<T>, dim3(a.nq / a.maps, a.requests), 128, 0, stream, a, 1));
+  return OMNIA_LAUNCH_RESULT();
+}
+
 extern "C" int omnia_shared_attention(const SharedAttention* given, int dtype, cudaStream_t stream) {
   const SharedAttention a = *given;
   if (a.requests == 0) return 0;
@@ -326,7 +339,7 @@ extern "C" int omnia_shared_attention(const SharedAttention* given, int dtype, c
                      : most <= 256 ? launch_pieces<T, 256>(a, blocks, smem, stream) : launch_pieces<T, 512>(a, blocks, smem, stream);
       if (code != 0) return code;
     }
-    launch_pdl(shared_merge_kernel<T>, dim3(a.nq / a.maps, a.requests), 128, 0, stream, a);
+    launch_pdl(shared_merge_kernel<T>, dim3(a.nq / a.maps, a.requests), 128, 0, stream, a, 0);
   });
   return OMNIA_LAUNCH_RESULT();
 }

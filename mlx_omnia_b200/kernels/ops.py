@@ -806,8 +806,8 @@ def shared_applies(step: StepContext, kv: KVView, nq: int, window: int | None = 
     _, _, _, nkv, d, dv = kv_layout(kv)
     if d != dv or not tiled_attention_supported(kv.pages.dtype, nq, nkv, d):
         return True
-    if not tcgen05_attention_supported(kv.pages.dtype, nq, nkv, d, kv.page_size):
-        return False
+    if nq // nkv > 8 and not tcgen05_attention_supported(kv.pages.dtype, nq, nkv, d, kv.page_size):
+        return False  # sixteen rows are one request's
     saved = sum(positions * (count - 1) for positions, count in _shape_of(step))
     return saved * nkv * (d + dv) * kv.pages.element_size() >= SHARED_LEAST_BYTES
 
@@ -910,7 +910,8 @@ def _shared_call(step: StepContext, kv: KVView, q: torch.Tensor, positive: bool,
     chunk, warps = decode_plan(n, nkv, own, sms)
     # (The tensor-core kernel looks for its maximum before it scales.)
     tensor_cores = positive and dv == d and tcgen05_attention_supported(dtype, nq, nkv, d, kv.page_size)
-    in_decode = tensor_cores and rows_in_decode(shape, group, nkv * (d + dv) * q.element_size())
+    in_decode = rows_in_decode(shape, group, nkv * (d + dv) * q.element_size()) if tensor_cores else \
+        positive and dv == d and tiled_attention_supported(dtype, nq, nkv, d)
     if in_decode:
         rows, tile, warps, places = 16 // group * group, 32, 1, 1 << 30
         chunk = rows_chunk(shape, group, nkv, n, own, sms)
@@ -923,7 +924,7 @@ def _shared_call(step: StepContext, kv: KVView, q: torch.Tensor, positive: bool,
     plan = shared_plan(shape, group, nkv, rows, tile, least, places)
     listed = _step_list(step, ("shared", group, nkv, rows, tile, plan, () if step.shared_shape is not None else step.shared), lambda st: shared_list(st, plan, group, nkv, rows, tile), device)
     # (The decode kernel's chunks lie at fixed positions, so a request's may be one more than its positions fill.)
-    max_parts, max_chunks = max(plan.parts), -(-own // chunk) + int(tensor_cores)
+    max_parts, max_chunks = max(plan.parts), -(-own // chunk) + int(tensor_cores or in_decode)
     count = n * nq * (max_parts + max_chunks)
     held = [listed, torch.empty(count, dv, device=device), torch.empty(count, 2, device=device)]
     args = _SharedArgs(cu_seqlens=_ptr(step.cu_seqlens), seq_lens=_ptr(step.seq_lens), plan=_ptr(listed), part_o=_ptr(held[1]), part_ml=_ptr(held[2]),
@@ -931,11 +932,12 @@ def _shared_call(step: StepContext, kv: KVView, q: torch.Tensor, positive: bool,
                        max_parts=max_parts, chunk_keys=chunk, max_chunks=max_chunks, max_pages=max_pages, num_pages=num_pages, nq=nq, nkv=nkv,
                        d=d, dv=dv, page_size=kv.page_size, maps=maps)
     at = ctypes.byref(args)
-    if tensor_cores:
+    if tensor_cores or in_decode:
         defines = {"HEAD_DIM": d, "GROUP": group}
-        pieces = _function("attention_shared_tc", "omnia_shared_pieces_tc", [c_void_p, c_void_p], defines)
         decode = _function("attention_tc", "omnia_attention_decode_shared", [c_void_p, c_void_p, c_int, c_int, c_void_p],
                            defines | {"SHARED": 1} | ({} if maps == 1 else {"MAPS": 2}))
+    if tensor_cores:
+        pieces = _function("attention_shared_tc", "omnia_shared_pieces_tc", [c_void_p, c_void_p], defines)
         merge = _function("attention_shared_tc", "omnia_shared_merge_tc", [c_void_p, c_void_p], defines)
         if in_decode:
             def launch() -> int:
@@ -952,6 +954,12 @@ def _shared_call(step: StepContext, kv: KVView, q: torch.Tensor, positive: bool,
             def launch() -> int:
                 stream = _stream()
                 return pieces(at, stream) or decode(at, tickets, warps, 0, stream)
+    elif in_decode:
+        merge_any, code = _function("attention_shared", "omnia_shared_merge", [c_void_p, c_int, c_void_p]), _code(dtype)
+
+        def launch() -> int:
+            stream = _stream()
+            return decode(at, None, warps, 1, stream) or merge_any(at, code, stream)
     else:
         generic, code = _function("attention_shared", "omnia_shared_attention", [c_void_p, c_int, c_void_p]), _code(dtype)
         launch = lambda: generic(at, code, _stream())  # noqa: E731

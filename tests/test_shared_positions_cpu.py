@@ -430,7 +430,8 @@ def test_where_sharing_applies():
     eight = (4096, tuple(range(8)))
     assert applies((eight,)) and not applies(()) and not applies((eight,), window=64) and not applies((eight,), decode_only=False)
     assert not applies(((200, (0, 1)),)) and applies(((200, (0, 1)),), dtype=torch.float32)
-    assert not applies((eight,), d=96) and not applies((eight,), page=8) and applies((eight,), nq=8 * 17)
+    assert applies((eight,), d=96) and applies((eight,), page=8) and applies((eight,), nq=8 * 17)
+    assert not applies((eight,), d=96, nq=8 * 9) and not applies(((200, (0, 1)),), d=96)
     assert not applies((eight,), spec=KVSpec(((8, 128), (8, 128)), chunk=64))
     assert not applies((eight,), spec=KVSpec(((8, 128), (8, 128)), stride=2))
 

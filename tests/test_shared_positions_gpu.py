@@ -174,8 +174,8 @@ LAYOUTS = {
     "32/2x128": (32, 2, 128, BF16, 16), "8/1x64": (8, 1, 64, BF16, 64), "8/4x64": (8, 4, 64, BF16, 16),
     "8/1x24 f32": (8, 1, 24, F32, 8), "4/2x128 f32": (4, 2, 128, F32, 16), "5/5x7 f32": (5, 5, 7, F32, 3), "34/1x64 f32": (34, 1, 64, F32, 16),
     "3/1x256 f32": (3, 1, 256, F32, 16), "2/1x512 f32": (2, 1, 512, F32, 4), "34/2x64": (34, 2, 64, BF16, 16),
+    "16/8x128 p8": (16, 8, 128, BF16, 8), "8/8x96": (8, 8, 96, BF16, 16), "8/2x256": (8, 2, 256, BF16, 16), "6/2x24": (6, 2, 24, BF16, 5),
 }
-TC = [name for name in LAYOUTS if "f32" not in name and not name.startswith("34")]
 GROUPS = {
     "one position": [(1, [1, 1, 7])], "a page": [(16, [1, 2])], "inside a page": [(17, [3, 1, 40]), (30, [1, 1])],
     "a tile and its ends": [(127, [1, 5]), (128, [2, 2]), (129, [1, 130])], "many pieces": [(1111, [9, 1, 200, 77, 64])],
@@ -197,7 +197,7 @@ def test_gates_sinks_and_caps(layout, options, way):
     check(make(nq, nkv, d, dtype, page, [(333, [1, 66, 20]), (64, [64, 1])], seed=3), **options)
 
 
-@pytest.mark.parametrize("layout", ["16/8x128", "8/4x64", "8/1x64", "8/1x24 f32", "4/2x128 f32"])
+@pytest.mark.parametrize("layout", ["16/8x128", "8/4x64", "8/1x64", "8/1x24 f32", "4/2x128 f32", "8/2x256"])
 def test_the_difference_of_two_maps(layout, way):
     nq, nkv, d, dtype, page = LAYOUTS[layout]
     last = ops.MapDifference(0.7, 1e-5, 0.4, d - 4)
@@ -285,7 +285,7 @@ def test_on_another_stream(layout, way):
     assert torch.equal(check(case)[: len(case.lengths)], got[: len(case.lengths)])
 
 
-@pytest.mark.parametrize("layout", ["16/8x128", "32/8x128", "8/1x24 f32"])
+@pytest.mark.parametrize("layout", ["16/8x128", "32/8x128", "8/1x24 f32", "8/8x96"])
 def test_a_captured_step_serves_other_groups(layout, way):
     nq, nkv, d, dtype, page = LAYOUTS[layout]
     cases = [make(nq, nkv, d, dtype, page, [(positions, [1 + (3 * i) % 50 for i in range(members)])], alone=(9,) * alone, padding=1, seed=seed)
@@ -348,7 +348,7 @@ def test_a_page_that_is_not_there_is_an_error():
             ops.raise_on_error(case.q.device)
 
 
-@pytest.mark.parametrize("layout", ["16/8x128", "8/1x24 f32"])
+@pytest.mark.parametrize("layout", ["16/8x128", "8/1x24 f32", "8/8x96"])
 def test_more_of_its_own_than_a_step_was_laid_out_for_is_an_error(layout, way):
     nq, nkv, d, dtype, page = LAYOUTS[layout]
     case = make(nq, nkv, d, dtype, page, [(200, [1, 1900])], alone=())
