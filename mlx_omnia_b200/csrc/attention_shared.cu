@@ -218,15 +218,16 @@ template <typename T>
 __global__ void __launch_bounds__(128)
 shared_merge_kernel(const __grid_constant__ SharedAttention a, int fixed) {
   __shared__ float scratch[33];
+  // The kernel before this one lets it begin only after its own wait for whatever came before, so lengths and list are there.
+  const int request = blockIdx.y, tid = threadIdx.x, length = a.seq_lens[request], start = a.plan[request], parts = a.plan[a.requests + request];
+  const size_t token = (size_t)a.cu_seqlens[request];
   pdl_wait();
   pdl_launch_dependents();
-  const int request = blockIdx.y, tid = threadIdx.x;
-  if (a.seq_lens[request] < 1) return;
-  const int start = a.plan[request], own = a.seq_lens[request] - (fixed ? start / a.chunk_keys * a.chunk_keys : start);
+  if (length < 1) return;
+  const int own = length - (fixed ? start / a.chunk_keys * a.chunk_keys : start);
   if (own > a.max_chunks * (long long)a.chunk_keys && blockIdx.x == 0 && tid == 0) atomicOr(a.err, OMNIA_ERR_WORK);  // more than the step was laid out for
-  const int count = min(a.plan[a.requests + request], a.max_parts) + max(0, min((own + a.chunk_keys - 1) / a.chunk_keys, a.max_chunks));
+  const int count = min(parts, a.max_parts) + max(0, min((own + a.chunk_keys - 1) / a.chunk_keys, a.max_chunks));
   const int places = a.max_parts + a.max_chunks;
-  const size_t token = (size_t)a.cu_seqlens[request];
   constexpr int PER_THREAD = 4;  // widths of at most 512
   float map[2][PER_THREAD];
 #pragma unroll
@@ -238,7 +239,7 @@ shared_merge_kernel(const __grid_constant__ SharedAttention a, int fixed) {
     float top = -INFINITY, total = 0.f;
 #pragma unroll
     for (int v = 0; v < PER_THREAD; ++v) map[which][v] = 0.f;
-    // Rounds of 32 pieces: a lane has one's maximum and sum; then eight accumulators on their way at a time.
+    // Rounds of 32 pieces: a lane has one's maximum and sum; then sixteen accumulators on their way at a time.
     for (int done = 0; done < count; done += 32) {
       const int some = min(32, count - done), lane = tid & 31;
       const float m = lane < some ? __ldcg(ml + 2 * (done + lane)) : -INFINITY, l = lane < some ? __ldcg(ml + 2 * (done + lane) + 1) : 0.f;
@@ -248,16 +249,16 @@ shared_merge_kernel(const __grid_constant__ SharedAttention a, int fixed) {
 #pragma unroll
       for (int v = 0; v < PER_THREAD; ++v) map[which][v] *= keep;
       top = now;
-      for (int i0 = 0; i0 < some; i0 += 8) {
+      for (int i0 = 0; i0 < some; i0 += 16) {
 #pragma unroll
         for (int v = 0; v < PER_THREAD; ++v) {
           if (128 * v >= a.dv) break;
           const int dim = tid + 128 * v;
-          float x[8];
+          float x[16];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] = i0 + i < some && dim < a.dv ? __ldcg(o + (size_t)(done + i0 + i) * a.dv + dim) : 0.f;
+          for (int i = 0; i < 16; ++i) x[i] = i0 + i < some && dim < a.dv ? __ldcg(o + (size_t)(done + i0 + i) * a.dv + dim) : 0.f;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) map[which][v] = fmaf(x[i], __shfl_sync(0xffffffffu, w, i0 + i), map[which][v]);
+          for (int i = 0; i < 16; ++i) map[which][v] = fmaf(x[i], __shfl_sync(0xffffffffu, w, i0 + i), map[which][v]);
         }
       }
     }
