@@ -791,9 +791,9 @@ SHARED_LEAST_BYTES = 24 << 20
 place of one, and that one also takes the projected rows as they are (2 to 3 us of a kernel ahead of it). B200, us, shared / each for itself: 16/8 heads
 of 128, 2 requests of 200 + 8 positions (0.8 MB) 7.9 / 6.5, 8 of 300 + 30 (9 MB) 10.6 / 10.4, 4 of 1,000 + 30 (12 MB) 10.5 / 10.8, 2 of 4,000 + 500 (16 MB)
 11.9 / 13.4, 8 of 1,000 + 30 (29 MB) 11.1 / 12.4, 16 of 1,000 + 30 (61 MB) 12.1 / 18.7; 6/2 heads of 64, 8 of 4,000 + 30 (14 MB) 9.9 / 9.7, of
-16,000 (57 MB) 16.2 / 19.6. The kernel for other types and sizes is the faster one from the first positions on (32 bits, 16/8 heads of 128, 2 requests of
-64 + 30 positions 8.0 / 43.3, 16 of 100 + 30 20.7 / 61.3): the ordinary kernel for these walks a request's keys in one block. It is not where bfloat16 of
-other head sizes has a tensor-core decode kernel to itself (8/2 heads of 256, 32 of 4,000 + 100 137 / 54; 8/8 of 96, 81 / 46), so that stays."""
+16,000 (57 MB) 16.2 / 19.6; 8/2 heads of 256, 32 of 300 + 100 (19 MB) 19.0 / 19.0, of 4,000 (254 MB) 38 / 81; 8/8 of 96, 8 of 1,000 + 100 (21 MB) 10.3 / 11.4. The
+kernel for other types and sizes is the faster one from the first positions on (32 bits, 16/8 heads of 128, 2 requests of 64 + 30 positions 11.8 /
+64.5, 16 of 100 + 30 30.7 / 91.9): the ordinary kernel for these walks a request's keys in one block."""
 
 
 def shared_applies(step: StepContext, kv: KVView, nq: int, window: int | None = -1) -> bool:
