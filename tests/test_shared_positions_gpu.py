@@ -4,6 +4,7 @@ answers that share a prompt, on the GPU, against plain 64-bit attention and plai
 from __future__ import annotations
 
 import dataclasses
+import importlib
 import math
 import random
 
@@ -14,6 +15,7 @@ import plain_impl
 import tiny_configs
 from mlx_omnia_b200 import GenerationOptions, load
 from mlx_omnia_b200.cache import CacheManager
+from mlx_omnia_b200.engine.engine import Engine, EngineArgs
 from mlx_omnia_b200.engine.generate import Generator
 from mlx_omnia_b200.kernels import ops
 from mlx_omnia_b200.parts.base import KVSpec, KVView, StateSpec, StepContext
@@ -558,3 +560,23 @@ def test_a_running_engine_whose_cache_is_resized(tmp_path):
     generator.run()
     ops.raise_on_error(model.engine.runtime.device)
     assert [r.generated for r in requests] == [plain_impl.greedy_generate(raw, weights, p, 12) for p in prompts]
+
+
+@pytest.mark.parametrize("graphs", [True, False])
+@pytest.mark.parametrize("family,name", [("bobarax", "K"), ("bobarax", "L"), ("dolutar", "P"), ("dolutar", "Q"), ("fokalorn", "X"), ("fokalorn", "Y"), ("gisudra", "G"),
+                                         ("gisudra", "H"), ("narezen", "P"), ("narezen", "Q"), ("rinirax", "S"), ("rinirax", "T")])
+def test_families_with_state_windows_and_latents(family, name, graphs):
+    """Recurrent state is copied at the fork, windows and runs share what they still hold: greedy answers that share are those of requests
+    of their own, in 32 bits."""
+    configs = importlib.import_module(f"{family}_configs")
+    raw = configs.config(name)
+    engine = Engine.from_tensors(raw, configs.tensors(name), EngineArgs(dtype="float32", page_size=4, cache_tokens=1024, max_requests=8, cuda_graphs=graphs))
+    generator = Generator(engine, max_tokens_per_step=16)
+    start = configs.prompt(27, engine.vocab_size, 5)
+    prompts = [start + configs.prompt(n, engine.vocab_size, n) for n in (1, 6)]
+    options = GenerationOptions(max_tokens=9, stop=())
+    alone = [generator.generate([p], options)[0] for p in prompts]
+    assert generator.generate(prompts, options, samples=3) == [ids for ids in alone for _ in range(3)]
+    assert generator.generate(prompts, options, samples=2, share=True) == [ids for ids in alone for _ in range(2)]
+    assert not engine.cache.requests
+    engine.cache.check()
