@@ -102,6 +102,7 @@ class DecodeGraphs:
     def __init__(self, runner) -> None:
         self.runner = runner
         self.captured: dict[tuple, _Captured] = {}  # in order of last use, oldest first
+        self.each_for_itself: set[tuple] = set()  # shapes of groups that no layer reads shared positions once for
         self.replays = 0
 
     @staticmethod
@@ -143,6 +144,12 @@ class DecodeGraphs:
                 torch.cuda.synchronize(self.runner.runtime.device)  # nothing of it is still running
                 del self.captured[oldest]
             captured = self._capture(*key)
+            if len(key) > 2 and not any(isinstance(k, tuple) and k[0] == "shared_call" for k in captured.step.workspace):
+                self.each_for_itself.add(key[2])  # the same step as without groups
+                key = key[:2]
+                if key in self.captured:
+                    torch.cuda.synchronize(self.runner.runtime.device)
+                    del self.captured[key]
         self.captured[key] = captured  # most recently used last
         return captured
 
@@ -156,10 +163,12 @@ class DecodeGraphs:
         batch = _bucket(len(entries))
         width = ops.width_bucket(max(max((len(t) for t in e.request.tables), default=0) for e in entries))
         shared, beyond = shared_positions(entries), ()
+        if shared and ops.shared_shape(shared) in self.each_for_itself:
+            shared = ()
         if shared:
-            page, starts_of = runner.cache.page_size, {i: positions for positions, which in shared for i in which}
+            starts_of = {i: positions for positions, which in shared for i in which}
             own = max(s + 1 - starts_of.get(i, 0) for i, s in enumerate(starts))
-            beyond = (ops.shared_shape(shared), ops.width_bucket(-(-own // page)) * page)
+            beyond = (ops.shared_shape(shared), ops.own_bucket(own, runner.cache.page_size))
         captured = self._graph_for(batch, width, *beyond)
         if captured.copied is not None:
             captured.copied.synchronize()  # the pinned buffer is free to be written again

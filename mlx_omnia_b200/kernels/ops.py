@@ -709,12 +709,12 @@ class SharedPlan:
 
 
 def shared_shape(shared) -> tuple[tuple[int, int], ...]:
-    """(positions, requests) of every group, what a plan is made from: positions in tiles of 128, rounded up to four significant bits,
-    and requests to a power of two."""
+    """(positions, requests) of every group, what a plan is made from: positions in tiles of 128, rounded up to three significant bits
+    (as the widths of block tables are, which captured steps are kept by too), and requests to a power of two."""
     shape = []
     for positions, members in shared:
         tiles = max(-(-positions // 128), 1)
-        unit = 1 << max(tiles.bit_length() - 4, 0)
+        unit = 1 << max(tiles.bit_length() - 3, 0)
         shape.append((-(-tiles // unit) * unit * 128, 1 << max(len(members) - 1, 0).bit_length()))
     return tuple(shape)
 
@@ -822,6 +822,15 @@ def _own_longest(step: StepContext) -> int:
     return max((n - starts.get(r, 0) for r, n in enumerate(step.seq_lens_host)), default=0)
 
 
+def own_bucket(positions: int, page_size: int) -> int:
+    """Positions that requests hold beyond what they share, in pages rounded up to two significant bits, at least eight: what plans are made for. (A
+    step is captured anew for every such number, and it grows from nothing: with three bits a prompt's answers of 512 tokens were nine
+    captures instead of five.)"""
+    pages = max(-(-positions // page_size), 8)
+    unit = 1 << max(pages.bit_length() - 2, 0)
+    return -(-pages // unit) * unit * page_size
+
+
 @dataclass
 class _SharedCall:
     """What a step's layers of one cache layout tell the kernels alike, and the memory that this names."""
@@ -906,7 +915,7 @@ def _shared_call(step: StepContext, kv: KVView, q: torch.Tensor, positive: bool,
     group, sms, n, shape = nq // nkv, sm_count(device), step.num_seqs, _shape_of(step)
     if any(positions > max_pages * kv.page_size for positions, _ in step.shared):
         raise KernelError("a group shares more positions than a block table holds")
-    own = width_bucket(-(-_own_longest(step) // kv.page_size)) * kv.page_size
+    own = own_bucket(_own_longest(step), kv.page_size)
     chunk, warps = decode_plan(n, nkv, own, sms)
     # (The tensor-core kernel looks for its maximum before it scales.)
     tensor_cores = positive and dv == d and tcgen05_attention_supported(dtype, nq, nkv, d, kv.page_size)
