@@ -18,11 +18,12 @@
 // Keys and values come by TMA, a box of 16 keys x 64 dims, into rings of stages of 128 keys.
 //
 // Measured (B200, 32/8 heads of 128): 64 requests of 65,536 shared positions and up to 1,024 of their own, with the decode kernel beside,
-// 119 us a layer (floor 68, memory; each request for itself 2,600); 96 of 30,000 + 64 84 us (floor 28, memory; products 48), 16 of
-// 32,768 + 500 45 (24). A tile of 128 keys takes a block 2.3 to 2.6 us with 256 rows: of that the tensor pipe is busy 44 %, the exponentials'
-// unit 48 %, the schedulers 49 %: what bounds it is the chain of a slot's half, load from tensor memory, maximum, exponentials, store, of
-// which two run side by side. With whole tiles of 128 keys and their scores' product between two softmaxes a tile took 3.3 us;
-// asking for the next half's scores ahead of this one's exponentials made it half a microsecond longer.
+// 118 us a layer (floor 68, memory; each request for itself 2,600); 96 of 30,000 + 64 84 us (floor 28, memory; products 48), 16 of
+// 32,768 + 500 45 (24). A tile of 128 keys takes a block 2.3 to 2.6 us with 256 rows. Of that the products take 1.8: a step of 16 dims is 76
+// cycles where it scores 64 keys and 102 where it scores 128, since its 128 rows come out of shared memory each time, a step of 16 keys of
+// the second product 52 to 77. Whole tiles of 128 keys have the cheaper scores but wait for them between two softmaxes: 3.3 us. The
+// softmax itself has room (exponentials' unit 48 %, schedulers 49 %): two teams of warps a slot, one a half, made it slower (96 of 30,000: 84 us,
+// so 91), and so did asking for the next half's scores ahead of this one's exponentials (96).
 #ifndef HEAD_DIM
 #define HEAD_DIM 128
 #endif
