@@ -683,7 +683,7 @@ class _MapDifferenceArgs(ctypes.Structure):
     _fields_ = [("lam", c_float), ("eps", c_float), ("factor", c_float), ("dv", c_int)]
 
 
-class _SharedArgs(ctypes.Structure):  # SharedAttention in attention_shared.cu
+class _SharedArgs(ctypes.Structure):  # SharedAttention in attention_shared.cuh
     _fields_ = [(name, c_void_p) for name in ("q", "k_pages", "v_pages", "gate", "out", "block_table", "cu_seqlens", "seq_lens", "plan",
                                               "sink", "part_o", "part_ml", "err")] + \
                [("page_stride", c_longlong)] + \
@@ -737,7 +737,7 @@ def shared_plan(shape: tuple[tuple[int, int], ...], group: int, nkv: int, block_
 
 
 def shared_list(step: StepContext, plan: SharedPlan, group: int, nkv: int, block_rows: int, tile: int) -> np.ndarray:
-    """The list that the kernels read (`SharedAttention` in attention_shared.cu)."""
+    """The list that the kernels read (`SharedAttention` in attention_shared.cuh)."""
     n = step.num_seqs
     out = np.zeros(2 * n + plan.members + 8 * plan.items, dtype=np.int32)
     items = out[2 * n + plan.members:].reshape(-1, 8)
@@ -1029,6 +1029,11 @@ def paged_attention(q: torch.Tensor | None, kv: KVView, step: StepContext, scale
 
     `difference`: two neighbouring query heads are the two maps of one head, and [tokens, nq / 2 * difference.dv] is
     what their difference gives; no gate and no sink then. Taken by the same kernels as runs and capped scores.
+
+    In a step of single tokens whose requests share their first positions (`StepContext.shared`) a layer without a window and
+    without runs reads these once for a group of requests, where that pays (`shared_applies`): every option but `projection` is taken
+    there too. Which kernel, and how the work is cut, follows from the groups' rounded sizes, so results are the same for a step of the same shape,
+    captured or not; they round otherwise than each request's by itself.
 
     With `projection` (only where `decode_fusable` holds) q is not given: the kernel makes the
     queries and the new keys and values from the projected rows, and writes the latter to the cache.
