@@ -1249,25 +1249,33 @@ def fill_slots(tensors: list[tuple[torch.Tensor, torch.Tensor | None]], slots: l
             _check(fn(to, start, size, len(part), some, len(some), _stream()), "fill_slots")
 
 
+_WRONG_MOVES = {1: "a move's number lies outside the tensor", 2: "two moves end in the same place", 3: "a move ends where another begins",
+                4: "no memory to check the moves with"}
+
+
 def _move_array(moves, columns: int, most_from: int, most_to: int, same: bool, what: str) -> array.array:
     """Moves (from, to, ...) as ints one after the other; numbers in range, no two with one end, and in one tensor no move's end another's
     beginning."""
     held = list(itertools.chain.from_iterable(moves))
     if len(held) != columns * len(moves):
         raise KernelError(f"{what}: moves of (from, to{', rows' if columns == 3 else ''})")
-    if held:
-        src, dst = held[0::columns], held[1::columns]
-        if min(src) < 0 or max(src) >= most_from or min(dst) < 0 or max(dst) >= most_to:
-            raise KernelError(f"{what}: a move's number lies outside the tensor")
-        ends = set(dst)
-        if len(ends) < len(dst):
-            raise KernelError(f"{what}: two moves end in the same place")
-        if same and not ends.isdisjoint(src):
-            raise KernelError(f"{what}: a move ends where another begins")
-    return array.array("i", held)  # (of a list: of anything else it takes three times as long)
+    try:
+        held = array.array("i", held)  # (of a list: of anything else it takes three times as long)
+    except OverflowError:
+        raise KernelError(f"{what}: {_WRONG_MOVES[1]}") from None
+    wrong = _copy_functions()[0](held.buffer_info()[0], columns, len(moves), most_from, most_to, same)
+    if wrong:
+        raise KernelError(f"{what}: {_WRONG_MOVES[wrong]}")
+    return held
 
 
-_COPY_PAGES = [c_void_p, c_void_p, c_longlong, c_longlong, c_int, c_longlong, c_int, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p]
+@functools.cache
+def _copy_functions() -> tuple:
+    """omnia_check_moves, omnia_copy_pages, omnia_copy_slots (looked up once: a copy of a few pages is bound by the host)."""
+    return (_function("cache_copy", "omnia_check_moves", [c_void_p, c_int, c_int, c_int, c_int, c_int]),
+            _function("cache_copy", "omnia_copy_pages", [c_void_p, c_void_p, c_longlong, c_longlong, c_int, c_longlong, c_int, c_void_p, c_void_p,
+                                                         c_int, c_void_p, c_int, c_void_p]),
+            _function("cache_copy", "omnia_copy_slots", [c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p]))
 
 
 def copy_pages(pages: torch.Tensor, rows: tuple[tuple[int, int], ...], page_size: int, moves, to: torch.Tensor | None = None) -> torch.Tensor:
@@ -1291,7 +1299,7 @@ def copy_pages(pages: torch.Tensor, rows: tuple[tuple[int, int], ...], page_size
             raise KernelError(f"copy_pages: a move of no more rows than a page's {page_size}")
     kinds = array.array("i", [h for h, _ in rows] + [w * item for _, w in rows])  # heads, then bytes of a row
     at = kinds.buffer_info()[0]
-    _check(_function("cache_copy", "omnia_copy_pages", _COPY_PAGES)(
+    _check(_copy_functions()[1](
         address, to_address, shape[1] * elements * item, to.shape[1] * elements * item, shape[0], elements * item, page_size, at,
         at + len(rows) * kinds.itemsize, len(rows), held.buffer_info()[0], len(moves), _stream()), "copy_pages")
     return to
@@ -1304,7 +1312,7 @@ def copy_slots(tensors: list[torch.Tensor], moves) -> None:
         raise KernelError("copy_slots takes contiguous tensors")
     least = min((t.shape[0] for t in tensors), default=0)
     held = _move_array(moves, 2, least, least, True, "copy_slots")
-    fn = _function("cache_copy", "omnia_copy_slots", [c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p])
+    fn = _copy_functions()[2]
     to = (c_void_p * len(tensors))(*(t.data_ptr() for t in tensors))
     size = (c_longlong * len(tensors))(*(t.numel() // max(t.shape[0], 1) * t.element_size() for t in tensors))
     _check(fn(to, size, len(tensors), held.buffer_info()[0], len(moves), _stream()), "copy_slots")

@@ -435,6 +435,7 @@ def test_what_copies_of_pages_refuse():
     refuses("outside", [(6, 0, 1)])
     refuses("outside", [(0, 6, 1)])
     refuses("outside", [(-1, 0, 1)])
+    refuses("outside", [(1 << 40, 0, 1)])
     refuses("the same place", [(0, 2, 1), (1, 2, 1)])
     refuses("another begins", [(0, 2, 1), (2, 3, 1)])
     refuses("another begins", [(1, 1, 4)])
