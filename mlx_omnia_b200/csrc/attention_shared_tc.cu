@@ -15,7 +15,7 @@
 // One chain alone would wait for its own products and loads half of the time; two fill each other's gaps. With more
 // than 128 rows a slot has half of them and both see every tile of keys; with fewer both hold the same rows and take the tiles
 // in turn, and the two states are brought together at the end. The rows are gathered from wherever the requests' tokens lie, by TMA.
-// Keys and values come by TMA, a box of 16 keys x 64 dims, into rings of stages of 128 keys.
+// Keys and values come by TMA, a box of 16 keys x 64 dims, into rings of stages of 64 keys.
 //
 // Measured (B200, 32/8 heads of 128): 64 requests of 65,536 shared positions and up to 1,024 of their own, with the decode kernel beside,
 // 118 us a layer (floor 68, memory; each request for itself 2,600); 96 of 30,000 + 64 84 us (floor 28, memory; products 48), 16 of
@@ -52,7 +52,7 @@ constexpr int SOFTMAX_THREADS = 256;     // warps 0-3 slot 0, 4-7 slot 1
 constexpr int SLOT_MEMBERS = BM / GROUP, Q_MEMBERS = 8;  // requests of a slot's rows, of a box of queries
 constexpr int WARP_MMA = 8, WARP_K = 10, WARP_V = 12, WARP_Q = 14, FEEDERS = 2;  // one issuer a slot; two warps feed each ring in turns
 constexpr int THREADS = 512;             // (a warp has nothing to do)
-// Registers a thread, by warpgroup: the slots' softmax holds a row's 128 scores. Together they are what the block is launched with.
+// Registers a thread, by warpgroup: the slots' softmax holds a row's 64 scores and the pairs made of them. Together they are what the block is launched with.
 constexpr int SLOT_REGS = 192, OTHER_REGS = 64;
 static_assert(2 * SLOT_REGS + 2 * OTHER_REGS == 4 * (65536 / THREADS), "a register split's sum is the launch's");
 constexpr uint32_t HALF_BYTES = 128 * 128;   // 128 rows of 128 bytes
