@@ -381,15 +381,18 @@ class CacheManager:
 
     def resize(self, pages_per_group: "int | dict[KVSpec, int]") -> None:
         """Give every group's pool another number of pages, more or fewer, while requests live: what is held moves to the front of a
-        new tensor. CacheError, and nothing changed, where a pool would not take what it holds. No step may be in flight, and
+        new tensor (old and new ones of all groups exist side by side meanwhile). CacheError where a pool would not take what it holds;
+        then, and where an allocation or a copy fails, nothing has changed. No step may be in flight, and
         steps captured on the old tensors are dead afterwards (`StepRunner.forget_graphs`)."""
         counts = [pages_per_group[g.spec] if isinstance(pages_per_group, dict) else pages_per_group for g in self.groups]
         if any(count < 1 for count in counts):
             raise ValueError("a pool has at least one page")
         pools = [group.pool.resized(count) for group, count in zip(self.groups, counts)]
-        for g, (group, (pool, to)) in enumerate(zip(self.groups, pools)):
-            if group.pages is not None:
-                old = group.pages
+        # Every group's new tensor is made and filled ahead of the first change: an allocation that fails leaves all as it was.
+        tensors: list[torch.Tensor | None] = []
+        for group, (pool, to) in zip(self.groups, pools):
+            old, new = group.pages, None
+            if old is not None:
                 new = torch.zeros(old.shape[0], pool.count, *old.shape[2:], dtype=old.dtype, device=old.device)
                 if old.is_cuda:
                     from mlx_omnia_b200.kernels import ops
@@ -397,8 +400,9 @@ class CacheManager:
                     ops.copy_pages(old, group.spec.rows, self.page_size, [(a, b, self.page_size) for a, b in to.items()], to=new)
                 elif to:
                     new[:, list(to.values())] = old[:, list(to)]
-                group.pages = new
-            group.pool = pool
+            tensors.append(new)
+        for g, (group, (pool, to), new) in enumerate(zip(self.groups, pools, tensors)):
+            group.pool, group.pages = pool, new
             for request in self.requests.values():
                 table = [to.get(page, -1) for page in request.tables[g]]
                 request.tables[g], request.arrays[g][: len(table)] = table, table

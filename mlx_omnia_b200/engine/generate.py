@@ -239,9 +239,9 @@ class Generator:
         engine = self.engine
         if any(r.max_tokens + len(r.prompt) > tokens for r in [*self.scheduler.running, *self.scheduler.waiting]):
             raise ValueError(f"a live request may grow past {tokens} tokens")
+        engine.runner.forget_graphs()  # ahead of the change: none outlives the tensors it was captured on, and their memory is free for the new ones
         engine.cache.resize(-(-tokens // engine.cache.page_size))
         engine.cache_tokens, self.scheduler.capacity = tokens, engine.cache.capacity_tokens()
-        engine.runner.forget_graphs()
 
     def run(self) -> None:
         """Step until every request has finished."""

@@ -178,6 +178,41 @@ def test_resizing_keeps_what_is_held(specs, pages):
     cache.check()
 
 
+def failing_at(monkeypatch, count):
+    """`torch.zeros` runs out of memory at its `count`th call from here on."""
+    calls, zeros = [], torch.zeros
+
+    def fake(*args, **options):
+        calls.append(1)
+        if len(calls) == count:
+            raise torch.OutOfMemoryError("no memory")
+        return zeros(*args, **options)
+
+    monkeypatch.setattr(torch, "zeros", fake)
+
+
+@pytest.mark.parametrize("specs", [(FULL, WINDOW), (UNEQUAL, FULL, STRIDED)])
+def test_a_resize_that_runs_out_of_memory_changes_nothing(specs, monkeypatch):
+    cache = manager(specs)
+    a = cache.open("a")
+    write(cache, a, 7, 1)
+    write(cache, cache.fork(a, "b"), 2, 2)
+
+    def everything():
+        return ([(g.pool.count, g.pool.held(), g.pages.data_ptr(), g.pages.clone()) for g in cache.groups],
+                [(r.tokens, [list(t) for t in r.tables], [x.tolist() for x in r.arrays]) for r in cache.requests.values()])
+
+    before = everything()
+    failing_at(monkeypatch, len(specs))
+    with pytest.raises(torch.OutOfMemoryError):
+        cache.resize(40)
+    monkeypatch.undo()
+    after = everything()
+    assert after[1] == before[1] and [x[:3] for x in after[0]] == [x[:3] for x in before[0]]
+    assert all(torch.equal(x[3], y[3]) for x, y in zip(after[0], before[0]))
+    cache.check()
+
+
 @pytest.mark.parametrize("seed", range(6))
 def test_random_lives_lose_no_page(seed):
     rng = random.Random(seed)
@@ -495,3 +530,24 @@ def test_a_cache_resized_between_steps_changes_no_answer(cpu_ops):
         generator.resize_cache(16)
     generator.run()
     assert [r.generated for r in requests] == [plain_impl.greedy_generate(raw, weights, p, 8) for p in prompts]
+
+
+def test_captured_steps_are_gone_ahead_of_a_resize_that_fails(cpu_ops, monkeypatch):
+    engine, raw, weights = engine_for("B")
+    assert len(engine.cache.groups) > 1
+    generator = Generator(engine)
+    prompt = tiny_configs.prompt(13, engine.vocab_size, 43)
+    request = generator.add(prompt, GenerationOptions(max_tokens=8, stop=()))
+    generator.step()
+    first, at_the_time = [g.pages.data_ptr() for g in engine.cache.groups], []
+    monkeypatch.setattr(engine.runner, "forget_graphs", lambda: at_the_time.append([g.pages.data_ptr() for g in engine.cache.groups]))
+    with monkeypatch.context() as patch:
+        failing_at(patch, len(engine.cache.groups))
+        with pytest.raises(torch.OutOfMemoryError):
+            generator.resize_cache(96)
+    assert at_the_time == [first] and engine.cache_tokens == 256 and generator.scheduler.capacity == engine.cache.capacity_tokens() == 256
+    assert [g.pages.data_ptr() for g in engine.cache.groups] == first
+    generator.resize_cache(96)
+    assert at_the_time == [first, first] and generator.scheduler.capacity == 96
+    generator.run()
+    assert request.generated == plain_impl.greedy_generate(raw, weights, prompt, 8)
