@@ -324,7 +324,8 @@ class CacheManager:
 
     def fork(self, request: RequestCache, request_id: str, positions: int | None = None) -> RequestCache:
         """Open `request_id` with the first `positions` positions of `request` (None: all of them) as its own. Whole pages are
-        shared, the rest and the state are copied (on the current stream). Nothing is taken when it cannot be done (CacheError)."""
+        shared, the rest and the state are copied (on the current stream). Nothing is taken when it cannot be done (CacheError), or when a
+        copy fails."""
         positions = request.tokens if positions is None else positions
         why = self.why_not_fork(request, positions)
         if why is not None:
@@ -334,20 +335,33 @@ class CacheManager:
             if n > group.pool.free:
                 raise CacheError(f"group {group.spec} needs {n} pages, {group.pool.free} free")
         new = self.open(request_id)
+        try:
+            self._take_over(request, new, positions, need)
+        except BaseException:
+            self.close(request_id)  # what it had taken by then
+            raise
+        run = next((r for r in request.runs if r.positions == positions), None)
+        if run is None:
+            run = SharedRun(positions)
+            request.runs = sorted([*request.runs, run], key=lambda r: r.positions)
+        new.runs = [r for r in request.runs if r.positions <= positions]
+        return new
+
+    def _take_over(self, request: RequestCache, new: RequestCache, positions: int, need: list[int]) -> None:
+        """Pages, rows and state of a fork. (Its table names a page as soon as it is held, so that closing it gives all of them back.)"""
         new.tokens, new.fresh = positions, request.fresh
         for g, (n, group, table) in enumerate(zip(need, self.groups, request.tables)):
-            whole = self._whole_pages(g, positions)
-            mine = list(table[:whole])
-            for page in mine:
+            whole, mine = self._whole_pages(g, positions), new.tables[g]
+            for page in table[:whole]:
                 if page >= 0:
                     group.pool.share(page)
+                mine.append(page)
             if n and table[whole] < 0:
                 mine.append(-1)  # the page that they end in holds nothing that can still be read
             elif n:
                 mine.append(group.pool.take())
                 if group.pages is not None:
                     self._copy_rows(group, table[whole], mine[-1], group.spec.stored(positions) - whole * self.page_size)
-            new.tables[g] = mine
             if len(mine) > len(new.arrays[g]):
                 new.arrays[g] = np.full(2 * len(mine), -1, dtype=np.int32)
             new.arrays[g][: len(mine)] = mine
@@ -359,12 +373,6 @@ class CacheManager:
         else:
             for tensor in tensors:
                 tensor[new.slot] = tensor[request.slot]
-        run = next((r for r in request.runs if r.positions == positions), None)
-        if run is None:
-            run = SharedRun(positions)
-            request.runs = sorted([*request.runs, run], key=lambda r: r.positions)
-        new.runs = [r for r in request.runs if r.positions <= positions]
-        return new
 
     def _copy_rows(self, group: Group, page: int, to: int, rows: int) -> None:
         if group.pages.is_cuda:

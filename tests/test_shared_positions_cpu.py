@@ -151,6 +151,36 @@ def test_a_fork_takes_nothing_when_pages_or_slots_are_short():
     cache.check()
 
 
+@pytest.mark.parametrize("fails", ["rows of the first group", "rows of the second group", "state"])
+def test_a_fork_whose_copy_fails_leaves_nothing_behind(fails, monkeypatch):
+    cache = manager((FULL, WINDOW), state=True)
+    a = cache.open("a")
+    write(cache, a, 7, 1)
+    tables, calls, copy = [list(t) for t in a.tables], [], CacheManager._copy_rows
+
+    def copy_rows(self, *args):
+        calls.append(1)
+        if len(calls) == (1 if fails == "rows of the first group" else 2):
+            raise ops.KernelError("a copy failed")
+        copy(self, *args)
+
+    def state_tensors(self):
+        raise ops.KernelError("a copy failed")
+
+    with monkeypatch.context() as patch:
+        if fails == "state":
+            patch.setattr(CacheManager, "state_tensors", state_tensors)
+        else:
+            patch.setattr(CacheManager, "_copy_rows", copy_rows)
+        with pytest.raises(ops.KernelError, match="a copy failed"):
+            cache.fork(a, "b")
+    assert list(cache.requests) == ["a"] and cache.slots.held() == [a.slot] and a.runs == [] and a.tables == tables
+    cache.check()
+    b = cache.fork(a, "b")  # the name, the slot and the pages are free
+    assert [held(cache, b, g, p) for g in (0, 1) for p in range(7)] == 2 * [1000 + p for p in range(7)]
+    cache.check()
+
+
 @pytest.mark.parametrize("specs", [(FULL, WINDOW), (UNEQUAL, FULL)])
 @pytest.mark.parametrize("pages", [9, 60])
 def test_resizing_keeps_what_is_held(specs, pages):
