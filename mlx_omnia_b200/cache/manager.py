@@ -308,6 +308,10 @@ class CacheManager:
         """Why `request` cannot be forked at `positions` (None: it can; pages and slots may still be short)."""
         if not 1 <= positions <= request.tokens:
             return f"a fork takes between 1 and the {request.tokens} positions that request {request.request_id!r} holds, not {positions}"
+        # (The page that they end in is the fork's to write on, so its first rows have to be there. None is given back while it can be written to.)
+        if any(n and table[self._whole_pages(g, positions)] < 0
+               for g, (n, table) in enumerate(zip(self.fork_pages(positions), request.tables))):
+            return f"the page that position {positions - 1} of request {request.request_id!r} lies in was given back"
         if request.tokens == positions:
             return None
         if self.has_state:
@@ -356,9 +360,7 @@ class CacheManager:
                 if page >= 0:
                     group.pool.share(page)
                 mine.append(page)
-            if n and table[whole] < 0:
-                mine.append(-1)  # the page that they end in holds nothing that can still be read
-            elif n:
+            if n:
                 mine.append(group.pool.take())
                 if group.pages is not None:
                     self._copy_rows(group, table[whole], mine[-1], group.spec.stored(positions) - whole * self.page_size)

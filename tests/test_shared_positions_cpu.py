@@ -181,6 +181,19 @@ def test_a_fork_whose_copy_fails_leaves_nothing_behind(fails, monkeypatch):
     cache.check()
 
 
+@pytest.mark.parametrize("positions", [7, 6])
+def test_a_fork_needs_the_page_that_it_goes_on_in(positions):
+    cache = manager((FULL, WINDOW))
+    a = cache.open("a")
+    write(cache, a, 7, 1)
+    cache.groups[1].pool.give(a.tables[1][1])
+    a.tables[1][1] = a.arrays[1][1] = -1
+    with pytest.raises(CacheError, match="given back"):
+        cache.fork(a, "b", positions)
+    assert list(cache.requests) == ["a"]
+    cache.check()
+
+
 @pytest.mark.parametrize("specs", [(FULL, WINDOW), (UNEQUAL, FULL)])
 @pytest.mark.parametrize("pages", [9, 60])
 def test_resizing_keeps_what_is_held(specs, pages):
