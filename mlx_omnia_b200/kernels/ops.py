@@ -916,18 +916,19 @@ def _shared_call(step: StepContext, kv: KVView, q: torch.Tensor, positive: bool,
     if any(positions > max_pages * kv.page_size for positions, _ in step.shared):
         raise KernelError("a group shares more positions than a block table holds")
     own = own_bucket(_own_longest(step), kv.page_size)
-    chunk, warps = decode_plan(n, nkv, own, sms)
+    batch = 1 << max(n - 1, 0).bit_length()  # as a captured step's: the work is cut alike, so the bits are the same
+    chunk, warps = decode_plan(batch, nkv, own, sms)
     # (The tensor-core kernel looks for its maximum before it scales.)
     tensor_cores = positive and dv == d and tcgen05_attention_supported(dtype, nq, nkv, d, kv.page_size)
     in_decode = rows_in_decode(shape, group, nkv * (d + dv) * q.element_size()) if tensor_cores else \
         positive and dv == d and tiled_attention_supported(dtype, nq, nkv, d)
     if in_decode:
         rows, tile, warps, places = 16 // group * group, 32, 1, 1 << 30
-        chunk = rows_chunk(shape, group, nkv, n, own, sms)
+        chunk = rows_chunk(shape, group, nkv, batch, own, sms)
         least = chunk // tile
     elif tensor_cores:
         rows, tile, places = 2 * (128 // group) * group, 128, sms
-        least = shared_size(shape, group, nkv, rows, n * own * nkv * (d + dv) * 2 // 2, sms)
+        least = shared_size(shape, group, nkv, rows, batch * own * nkv * (d + dv) * 2 // 2, sms)
     else:
         rows, tile, least, places = SHARED_ROWS, SHARED_TILE, 2, 4 * sms
     plan = shared_plan(shape, group, nkv, rows, tile, least, places)
@@ -1032,8 +1033,8 @@ def paged_attention(q: torch.Tensor | None, kv: KVView, step: StepContext, scale
 
     In a step of single tokens whose requests share their first positions (`StepContext.shared`) a layer without a window and
     without runs reads these once for a group of requests, where that pays (`shared_applies`): every option but `projection` is taken
-    there too. Which kernel, and how the work is cut, follows from the groups' rounded sizes, so results are the same for a step of the same shape,
-    captured or not; they round otherwise than each request's by itself.
+    there too. Which kernel, and how the work is cut, follows from rounded numbers: the groups' sizes, the requests, what these hold beyond the
+    groups. So a step has the same results captured or not; they round otherwise than each request's by itself.
 
     With `projection` (only where `decode_fusable` holds) q is not given: the kernel makes the
     queries and the new keys and values from the projected rows, and writes the latter to the cache.

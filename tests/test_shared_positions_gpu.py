@@ -318,6 +318,33 @@ def test_a_captured_step_serves_other_groups(layout, way):
         torch.cuda.synchronize()
 
 
+@pytest.mark.parametrize("layout,positions,owns", [("16/8x128", 1000, [2000 - 7 * i for i in range(17)]), ("16/8x128", 1000, [1000 - 9 * i for i in range(9)]),
+                                                   ("32/8x128", 9000, [900 - 3 * i for i in range(33)]), ("6/2x64", 1290, [1500 - i for i in range(19)]),
+                                                   ("8/2x256", 2000, [1100 - 5 * i for i in range(9)]), ("8/1x24 f32", 700, [900 - 4 * i for i in range(11)])])
+def test_a_captured_step_has_the_bits_of_one_that_is_not(layout, positions, owns, way):
+    """Requests rounded up to a power of two, as the engine's captured steps are, and what they hold beyond the group to a bound."""
+    nq, nkv, d, dtype, page = LAYOUTS[layout]
+    case = make(nq, nkv, d, dtype, page, [(positions, owns)], alone=(), padding=0, seed=11)
+    eager = check(case)
+    n = len(owns)
+    batch, width = 1 << (n - 1).bit_length(), ops.width_bucket(case.kv.block_table.shape[1])
+    q, table = torch.zeros(batch, nq, d, dtype=dtype, device="cuda"), ints([[-1] * width] * batch)
+    step = dataclasses.replace(case.step, num_tokens=batch, num_seqs=batch, cu_seqlens=ints(list(range(batch + 1))), seq_lens=ints([0] * batch),
+                               seq_lens_host=[], shared=(), shared_shape=ops.shared_shape(case.step.shared), max_own=ops.own_bucket(max(owns), page),
+                               max_seq_len=width * page, workspace={"private": True})
+    kv = dataclasses.replace(case.kv, block_table=table)
+    ops.paged_attention(q, kv, step, d ** -0.5)  # nobody holds anything: the lists and the scratch memory are made
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.paged_attention(q, kv, step, d ** -0.5)
+    q[:n], table[:n, : case.kv.block_table.shape[1]], step.seq_lens[:n], step.shared = case.q, case.kv.block_table, case.step.seq_lens, case.step.shared
+    ops.fill_step_lists(step)
+    graph.replay()
+    assert torch.equal(out[:n], eager)
+    ops.raise_on_error(q.device)
+
+
 def test_what_attention_over_shared_positions_refuses():
     case = make(16, 8, 128, BF16, 16, [(64, [1, 30]), (40, [2, 2])], alone=())
 
