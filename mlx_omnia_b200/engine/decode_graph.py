@@ -102,7 +102,6 @@ class DecodeGraphs:
     def __init__(self, runner) -> None:
         self.runner = runner
         self.captured: dict[tuple, _Captured] = {}  # in order of last use, oldest first
-        self.each_for_itself: set[tuple] = set()  # shapes of groups that no layer reads shared positions once for
         self.replays = 0
 
     @staticmethod
@@ -118,7 +117,7 @@ class DecodeGraphs:
         # Kernels that need scratch memory keep it in the workspace, for as long as the graph lives.
         step = layout.context(dev, q_lens=[1] * batch, seq_lens_host=[], max_q_len=1,
                               max_seq_len=width * runner.cache.page_size, decode_only=True,
-                              workspace={"private": True}, shared_shape=shape or None, max_own=own)
+                              workspace={"private": True, "attention_layers": set()}, shared_shape=shape or None, max_own=own)
         # Padding everywhere, so the warm-up and the capture touch no page.
         layout.fill(host_tensor.numpy(), runner.cache, [], [], np.arange(batch, dtype=np.int32))
         dev.copy_(host_tensor)
@@ -144,12 +143,7 @@ class DecodeGraphs:
                 torch.cuda.synchronize(self.runner.runtime.device)  # nothing of it is still running
                 del self.captured[oldest]
             captured = self._capture(*key)
-            if len(key) > 2 and not any(isinstance(k, tuple) and k[0] == "shared_call" for k in captured.step.workspace):
-                self.each_for_itself.add(key[2])  # the same step as without groups
-                key = key[:2]
-                if key in self.captured:
-                    torch.cuda.synchronize(self.runner.runtime.device)
-                    del self.captured[key]
+            self.runner.know_layers(captured.step)
         self.captured[key] = captured  # most recently used last
         return captured
 
@@ -163,12 +157,14 @@ class DecodeGraphs:
         batch = _bucket(len(entries))
         width = ops.width_bucket(max(max((len(t) for t in e.request.tables), default=0) for e in entries))
         shared, beyond = shared_positions(entries), ()
-        if shared and ops.shared_shape(shared) in self.each_for_itself:
-            shared = ()
         if shared:
-            starts_of = {i: positions for positions, which in shared for i in which}
-            own = max(s + 1 - starts_of.get(i, 0) for i, s in enumerate(starts))
-            beyond = (ops.shared_shape(shared), ops.own_bucket(own, runner.cache.page_size))
+            shape = ops.shared_shape(shared)
+            if any(ops.sharing_pays(layer, shape) for layer in runner.attention_layers):
+                starts_of = {i: positions for positions, which in shared for i in which}
+                own = max(s + 1 - starts_of.get(i, 0) for i, s in enumerate(starts))
+                beyond = (shape, ops.own_bucket(own, runner.cache.page_size))
+            else:
+                shared = ()  # the same step as without groups: no shape of theirs is captured
         captured = self._graph_for(batch, width, *beyond)
         if captured.copied is not None:
             captured.copied.synchronize()  # the pinned buffer is free to be written again

@@ -130,6 +130,7 @@ class StepRunner:
     def __init__(self, model: DecoderModel, cache: CacheManager, runtime: Runtime, cuda_graphs: bool = False) -> None:
         self.model, self.cache, self.runtime = model, cache, runtime
         self.steps_run = 0
+        self.attention_layers: set = set()  # kinds (`ops.AttentionLayer`) that the model was seen to run
         self.cuda_graphs = cuda_graphs
         self.graphs = self.mixed_graphs = None
         self.forget_graphs()
@@ -146,6 +147,11 @@ class StepRunner:
             self.graphs = DecodeGraphs(self)
             if MixedGraphs.supported(self.model):
                 self.mixed_graphs = MixedGraphs(self)
+
+    def know_layers(self, step: StepContext) -> None:
+        """Note which kinds of attention layers a step has run. (Every step runs all of them, and requests share positions that a step has read, so
+        they are known by the time that a captured step is asked whether it pays to read these once.)"""
+        self.attention_layers |= (step.workspace or {}).get("attention_layers", set())
 
     # -- metadata ----------------------------------------------------------------------
     def take_pages(self, entries: list[StepEntry]) -> list[int]:
@@ -230,7 +236,10 @@ class StepRunner:
                 logits = self.mixed_graphs.run(shape, entries, copy)
             else:
                 step = self.build_context(entries)
+                if not self.attention_layers:
+                    step.workspace = {"attention_layers": set()}
                 logits = self.model.forward(step, self.layer_contexts(step))
+                self.know_layers(step)
         for entry in entries:
             entry.request.fresh = False
             self.cache.release_behind_window(entry.request)

@@ -796,20 +796,43 @@ kernel for other types and sizes is the faster one from the first positions on (
 64.5, 16 of 100 + 30 30.7 / 91.9): the ordinary kernel for these walks a request's keys in one block."""
 
 
-def shared_applies(step: StepContext, kv: KVView, nq: int, window: int | None = -1) -> bool:
-    """Whether a layer's attention reads shared positions once for their group: a step of single tokens, every position in sight, and enough of
-    them (`SHARED_LEAST_BYTES`; requests rounded up as in `shared_shape`, so that a captured step decides as it did)."""
-    if not shares(step) or not step.decode_only or (kv.window if window == -1 else window):
-        return False
-    if kv.spec is not None and (kv.spec.stride != 1 or kv.spec.chunk):
-        return False
+@dataclass(frozen=True)
+class AttentionLayer:
+    """What of a layer decides whether its attention reads shared positions once for their group."""
+
+    nq: int
+    nkv: int
+    d: int
+    dv: int
+    dtype: torch.dtype
+    page_size: int
+    every: bool  # every position in sight and stored by itself: no window, no runs, no strides
+
+
+def attention_layer(kv: KVView, nq: int, window: int | None = -1) -> AttentionLayer:
     _, _, _, nkv, d, dv = kv_layout(kv)
-    if d != dv or not tiled_attention_supported(kv.pages.dtype, nq, nkv, d):
+    every = not (kv.window if window == -1 else window) and (kv.spec is None or (kv.spec.stride == 1 and not kv.spec.chunk))
+    return AttentionLayer(nq, nkv, d, dv, kv.pages.dtype, kv.page_size, every)
+
+
+def sharing_pays(layer: AttentionLayer, shape: tuple[tuple[int, int], ...]) -> bool:
+    """Whether such a layer reads groups of this `shared_shape` once: every position in sight, and enough of them (`SHARED_LEAST_BYTES`). Asked by
+    the layers of a step, and by the runner ahead of a captured one."""
+    if not layer.every:
+        return False
+    nkv, d, dv = layer.nkv, layer.d, layer.dv
+    if d != dv or not tiled_attention_supported(layer.dtype, layer.nq, nkv, d):
         return True
-    if nq // nkv > 8 and not tcgen05_attention_supported(kv.pages.dtype, nq, nkv, d, kv.page_size):
+    if layer.nq // nkv > 8 and not tcgen05_attention_supported(layer.dtype, layer.nq, nkv, d, layer.page_size):
         return False  # sixteen rows are one request's
-    saved = sum(positions * (count - 1) for positions, count in _shape_of(step))
-    return saved * nkv * (d + dv) * kv.pages.element_size() >= SHARED_LEAST_BYTES
+    saved = sum(positions * (count - 1) for positions, count in shape)
+    return saved * nkv * (d + dv) * layer.dtype.itemsize >= SHARED_LEAST_BYTES
+
+
+def shared_applies(step: StepContext, kv: KVView, nq: int, window: int | None = -1) -> bool:
+    """Whether a layer's attention reads shared positions once for their group: a step of single tokens, and `sharing_pays` (for rounded
+    groups, so that a captured step decides as it did)."""
+    return shares(step) and step.decode_only and sharing_pays(attention_layer(kv, nq, window), _shape_of(step))
 
 
 def _own_longest(step: StepContext) -> int:
@@ -1043,6 +1066,8 @@ def paged_attention(q: torch.Tensor | None, kv: KVView, step: StepContext, scale
     decode kernel when every request brings one token; otherwise the tcgen05 prefill kernel
     (head sizes 64 and 128, pages of a multiple of 16) or the mma.sync prefill kernel. Other
     cases (the 32-bit path among them) run on the generic kernel."""
+    if step.workspace and "attention_layers" in step.workspace:  # the runner wants to know
+        step.workspace["attention_layers"].add(attention_layer(kv, q.shape[1] if projection is None else projection.nq, window))
     if shares(step):
         check_shared(step)
     if not chunk and shared_applies(step, kv, q.shape[1] if projection is None else projection.nq, window):

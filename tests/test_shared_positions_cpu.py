@@ -514,6 +514,40 @@ def test_where_sharing_applies():
     assert not applies((eight,), spec=KVSpec(((8, 128), (8, 128)), stride=2))
 
 
+class Planned(Exception):
+    pass
+
+
+@pytest.mark.parametrize("positions,members,alone,windowed,pays", [(300, 4, 3, False, False), (4096, 8, 0, False, True), (4096, 8, 0, True, False),
+                                                                   (40000, 2, 1, False, True)])
+def test_a_captured_step_has_no_groups_where_no_layer_reads_them_once(positions, members, alone, windowed, pays, monkeypatch):
+    """What a step is kept by is decided ahead of its capture: where no layer gains by groups, by what the same step without them is."""
+    from mlx_omnia_b200.engine.decode_graph import DecodeGraphs
+
+    spec = KVSpec.keys_and_values(8, 128, None)
+    cache = manager((spec,), pages=6000, page_size=16, max_requests=16, allocate=False)
+    leader = cache.open("leader")
+    cache.grow(leader, positions)
+    requests = [leader] + [cache.fork(leader, f"f{i}") for i in range(members - 1)] + [cache.open(f"a{i}") for i in range(alone)]
+    for request in requests[members:]:
+        cache.grow(request, 50)
+    runner = SimpleNamespace(cache=cache, attention_layers={ops.AttentionLayer(16, 8, 128, 128, torch.bfloat16, 16, not windowed)},
+                             take_pages=lambda entries: [e.request.tokens for e in entries])
+    graphs, keys = DecodeGraphs(runner), []
+
+    def graph_for(*key):
+        keys.append(key)
+        raise Planned
+
+    monkeypatch.setattr(graphs, "_graph_for", graph_for)
+    entries = [StepEntry(r, [1], [0]) for r in requests]
+    with pytest.raises(Planned):
+        graphs.run(entries)
+    batch, width = 1 << (len(requests) - 1).bit_length(), ops.width_bucket(-(-positions // 16))
+    shape = ops.shared_shape(shared_positions(entries))
+    assert keys == [(batch, width, shape, ops.own_bucket(51 if alone else 1, 16)) if pays else (batch, width)]
+
+
 # -- answers ----------------------------------------------------------------------------------------------------------
 def engine_for(name, cache_tokens=256, page_size=4, max_requests=4):
     raw, weights = tiny_configs.config(name), tiny_configs.tensors(name)

@@ -560,6 +560,21 @@ def test_greedy_answers_that_share_equal_plain(tmp_path, name, page, graphs):
     model.engine.cache.check()
 
 
+def test_groups_that_no_layer_gains_by_cost_no_capture(tmp_path, monkeypatch):
+    """Answers to several short prompts under the rule that a user has: every capture is one that a step without groups would make, and is kept."""
+    monkeypatch.undo()
+    assert ops.SHARED_LEAST_BYTES > 1 << 20
+    write_folder(tmp_path / "m", "C")
+    model = load(tmp_path / "m", page_size=16, cache_tokens=8192, max_requests=16, max_tokens_per_step=512)
+    graphs, keys = model.engine.runner.graphs, []
+    capture = graphs._capture
+    monkeypatch.setattr(graphs, "_capture", lambda *key: keys.append(key) or capture(*key))
+    prompts = [tiny_configs.prompt(60 + 50 * i, 777, i) for i in range(4)]
+    assert len(model.generate(prompts, GenerationOptions(max_tokens=40, stop=()), samples=4)) == 16
+    assert keys and all(len(key) == 2 for key in keys)
+    assert len(keys) == len(set(keys)) == len(graphs.captured)
+
+
 def test_answers_in_bfloat16_choose_what_is_nearly_best(tmp_path):
     raw, weights = write_folder(tmp_path / "m", "C")
     model = load(tmp_path / "m", page_size=16, cache_tokens=4096, max_requests=16, max_tokens_per_step=64)
