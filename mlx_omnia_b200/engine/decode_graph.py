@@ -158,11 +158,11 @@ class DecodeGraphs:
         width = ops.width_bucket(max(max((len(t) for t in e.request.tables), default=0) for e in entries))
         shared, beyond = shared_positions(entries), ()
         if shared:
+            starts_of = {i: positions for positions, which in shared for i in which}
+            own = ops.own_bucket(max(s + 1 - starts_of.get(i, 0) for i, s in enumerate(starts)), runner.cache.page_size)
             shape = ops.shared_shape(shared)
-            if any(ops.sharing_pays(layer, shape) for layer in runner.attention_layers):
-                starts_of = {i: positions for positions, which in shared for i in which}
-                own = max(s + 1 - starts_of.get(i, 0) for i, s in enumerate(starts))
-                beyond = (shape, ops.own_bucket(own, runner.cache.page_size))
+            if any(ops.sharing_pays(layer, shape, batch, own) for layer in runner.attention_layers):
+                beyond = (shape, own)
             else:
                 shared = ()  # the same step as without groups: no shape of theirs is captured
         captured = self._graph_for(batch, width, *beyond)

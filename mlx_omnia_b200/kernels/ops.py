@@ -796,6 +796,15 @@ kernel for other types and sizes is the faster one from the first positions on (
 64.5, 16 of 100 + 30 30.7 / 91.9): the ordinary kernel for these walks a request's keys in one block."""
 
 
+SHARED_OWN_BYTES, SHARED_OWN_MOST = 40 << 20, 1000 << 20
+"""In a pass that line lies as much higher again for every so many bytes a layer that requests hold beyond what they share, up to so many (counted as requests,
+rounded up to a power of two, times the most that one holds, `own_bucket`: what a captured step is kept by). The ordinary kernel then runs by a list of equal pieces
+(`decode_places`), the one beside shared positions walks chunks, which costs every request of the step, in a group or not. B200, 16/8
+heads of 128, shared / each for itself, us a layer: 2 requests of 6,200 shared positions beside 60 of up to 6,000 134 / 117; 8 of 1,000 + 200 beside 8 of up to 3,000
+29.5 / 17.6; 8 of 4,000 + 200 beside 56 of up to 3,000 100 / 76, of 8,000 93 / 91; 64 of 512 + up to 1,954 72 / 57; 64 of 2,051 + up to 694 35 / 83. Fitted
+to 9,355 random steps in six layouts: a layer takes 1.014 times the better way's time on average, with the line where it lies outside of a pass 1.069."""
+
+
 @dataclass(frozen=True)
 class AttentionLayer:
     """What of a layer decides whether its attention reads shared positions once for their group."""
@@ -815,9 +824,10 @@ def attention_layer(kv: KVView, nq: int, window: int | None = -1) -> AttentionLa
     return AttentionLayer(nq, nkv, d, dv, kv.pages.dtype, kv.page_size, every)
 
 
-def sharing_pays(layer: AttentionLayer, shape: tuple[tuple[int, int], ...]) -> bool:
-    """Whether such a layer reads groups of this `shared_shape` once: every position in sight, and enough of them (`SHARED_LEAST_BYTES`). Asked by
-    the layers of a step, and by the runner ahead of a captured one."""
+def sharing_pays(layer: AttentionLayer, shape: tuple[tuple[int, int], ...], requests: int = 0, own: int = 0) -> bool:
+    """Whether such a layer reads groups of this `shared_shape` once: every position in sight, and enough of them (`SHARED_LEAST_BYTES`) for what
+    the step's requests hold beyond them, `own` positions (`own_bucket`) at most (`SHARED_OWN_BYTES`; 0 outside of a pass, where the ordinary
+    kernel has no list). Asked by the layers of a step, and by the runner ahead of a captured one."""
     if not layer.every:
         return False
     nkv, d, dv = layer.nkv, layer.d, layer.dv
@@ -825,14 +835,19 @@ def sharing_pays(layer: AttentionLayer, shape: tuple[tuple[int, int], ...]) -> b
         return True
     if layer.nq // nkv > 8 and not tcgen05_attention_supported(layer.dtype, layer.nq, nkv, d, layer.page_size):
         return False  # sixteen rows are one request's
-    saved = sum(positions * (count - 1) for positions, count in shape)
-    return saved * nkv * (d + dv) * layer.dtype.itemsize >= SHARED_LEAST_BYTES
+    position = nkv * (d + dv) * layer.dtype.itemsize
+    saved = sum(positions * (count - 1) for positions, count in shape) * position
+    beyond = (1 << max(requests - 1, 0).bit_length()) * own * position
+    return saved >= SHARED_LEAST_BYTES * (1 + min(beyond, SHARED_OWN_MOST) / SHARED_OWN_BYTES)
 
 
 def shared_applies(step: StepContext, kv: KVView, nq: int, window: int | None = -1) -> bool:
     """Whether a layer's attention reads shared positions once for their group: a step of single tokens, and `sharing_pays` (for rounded
-    groups, so that a captured step decides as it did)."""
-    return shares(step) and step.decode_only and sharing_pays(attention_layer(kv, nq, window), _shape_of(step))
+    numbers, so that a captured step decides as it did)."""
+    if not shares(step) or not step.decode_only:
+        return False
+    requests, own = (step.num_seqs, own_bucket(_own_longest(step), kv.page_size)) if in_pass(step) else (0, 0)
+    return sharing_pays(attention_layer(kv, nq, window), _shape_of(step), requests, own)
 
 
 def _own_longest(step: StepContext) -> int:
@@ -841,8 +856,11 @@ def _own_longest(step: StepContext) -> int:
         return step.max_own
     if not step.seq_lens_host:
         return step.max_seq_len  # lengths that the host does not know
-    starts = {m: positions for positions, members in step.shared for m in members}
-    return max((n - starts.get(r, 0) for r, n in enumerate(step.seq_lens_host)), default=0)
+    kept = step.workspace["pass"] if in_pass(step) else {}
+    if "own_longest" not in kept:
+        starts = {m: positions for positions, members in step.shared for m in members}
+        kept["own_longest"] = max((n - starts.get(r, 0) for r, n in enumerate(step.seq_lens_host)), default=0)
+    return kept["own_longest"]
 
 
 def own_bucket(positions: int, page_size: int) -> int:

@@ -514,6 +514,36 @@ def test_where_sharing_applies():
     assert not applies((eight,), spec=KVSpec(((8, 128), (8, 128)), stride=2))
 
 
+@pytest.mark.parametrize("groups,alone,pays", [
+    ([(6200, [100, 100])], [6000 - 60 * i for i in range(60)], False), ([(1000, [200] * 8)], [3000 - 90 * i for i in range(8)], False),
+    ([(4000, [200] * 8)], [3000] * 56, False), ([(512, [1 + 31 * i for i in range(64)])], [], False),
+    ([(2051, [1 + 11 * i for i in range(64)])], [], True), ([(4096, [256] * 8)], [], True), ([(30000, [200] * 16)], [3000] * 16, True),
+    ([(6200, [10, 10])], [], True)])
+def test_sharing_is_weighed_against_what_requests_hold_of_their_own(groups, alone, pays):
+    """Inside of a pass, where what a step's requests hold of their own would run by a list of equal pieces."""
+    lengths, shared = [], []
+    for positions, owns in groups:
+        shared.append((positions, tuple(range(len(lengths), len(lengths) + len(owns)))))
+        lengths += [positions + own for own in owns]
+    lengths += alone
+    step = step_of(lengths, tuple(shared))
+    pages = torch.empty(1, 2, 8, 16, 128, dtype=torch.bfloat16, device="meta")
+    kv = SimpleNamespace(pages=pages, spec=None, page_size=16, window=None)
+    assert ops.shared_applies(step, kv, 16)
+    ops.begin_pass(step)
+    assert ops.shared_applies(step, kv, 16) == pays
+    # A captured step of such numbers decides alike.
+    batch = 1 << (len(lengths) - 1).bit_length()
+    own = ops.own_bucket(max([own for _, owns in groups for own in owns] + alone), 16)
+    captured = step_of([0] * batch, (), shared_shape=ops.shared_shape(shared), max_own=own)
+    captured.seq_lens_host = []
+    ops.begin_pass(captured)
+    assert ops.shared_applies(captured, kv, 16) == pays == ops.sharing_pays(ops.attention_layer(kv, 16), ops.shared_shape(shared), len(lengths), own)
+    # Other types and widths have no list.
+    pages = torch.empty(1, 2, 8, 16, 128, device="meta")
+    assert ops.shared_applies(step, SimpleNamespace(pages=pages, spec=None, page_size=16, window=None), 16)
+
+
 class Planned(Exception):
     pass
 
