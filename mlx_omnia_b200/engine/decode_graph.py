@@ -34,9 +34,17 @@ of many lengths most shapes come once or twice: capturing at the second coming, 
 as wide as the pool, made such a stream twice as slow as launching every step kernel by
 kernel.)
 
+Steps of groups. What a capture costs, a step that reads shared positions once gains back in ten
+steps (64 requests of 65,536 positions) to thousands (four groups of four answers), and where several
+groups come and go their sizes do so within a few dozen steps. So every shape of groups has an
+account: each of its steps adds what it gains or would have gained, and its graph (one for every
+bound of what requests hold beyond the groups) is captured when that amounts to a capture, which
+is taken off. Until then the step runs as one without groups, which needs nothing of them and whose
+results round otherwise (`ops.paged_attention`).
+
 The kernels and the model code are the same as in an uncaptured step; only the way
 they are launched differs, so logits agree bit for bit with an eager step of the same
-bucket. Capture is used only when every mixer of the model declares `graph_safe`
+bucket, of groups or without. Capture is used only when every mixer of the model declares `graph_safe`
 (no host-side loops over requests).
 
 The reference compiles its one-token forward per (mode, batch, capacity) with
@@ -59,6 +67,9 @@ from mlx_omnia_b200.kernels import ops
 from mlx_omnia_b200.parts.base import StepContext
 
 MAX_GRAPHS = 24
+CAPTURE_GAINS = 1152
+"""What a capture of a step of groups costs, in `ops.SHARED_LEAST_BYTES` (24 MB) of a layer's reading: 60 to 200 ms for 28 layers, some 4.5 ms a layer, in which
+it reads 28 GB."""
 
 
 @contextlib.contextmanager
@@ -102,6 +113,7 @@ class DecodeGraphs:
     def __init__(self, runner) -> None:
         self.runner = runner
         self.captured: dict[tuple, _Captured] = {}  # in order of last use, oldest first
+        self.gained: dict[tuple, float] = {}  # by groups' shape: what its steps gain or would have (`ops.sharing_gain`), less its captures
         self.replays = 0
 
     @staticmethod
@@ -117,7 +129,7 @@ class DecodeGraphs:
         # Kernels that need scratch memory keep it in the workspace, for as long as the graph lives.
         step = layout.context(dev, q_lens=[1] * batch, seq_lens_host=[], max_q_len=1,
                               max_seq_len=width * runner.cache.page_size, decode_only=True,
-                              workspace={"private": True, "attention_layers": set()}, shared_shape=shape or None, max_own=own)
+                              workspace={"private": True} | runner.ask_for_layers(), shared_shape=shape or None, max_own=own)
         # Padding everywhere, so the warm-up and the capture touch no page.
         layout.fill(host_tensor.numpy(), runner.cache, [], [], np.arange(batch, dtype=np.int32))
         dev.copy_(host_tensor)
@@ -126,6 +138,7 @@ class DecodeGraphs:
         side.wait_stream(torch.cuda.current_stream(device))
         with torch.cuda.stream(side):
             runner.model.forward(step, layers)  # warm-up: loads kernels, sizes library workspaces
+        runner.know_layers(step)
         torch.cuda.current_stream(device).wait_stream(side)
         torch.cuda.synchronize(device)
         graph = torch.cuda.CUDAGraph()
@@ -143,9 +156,21 @@ class DecodeGraphs:
                 torch.cuda.synchronize(self.runner.runtime.device)  # nothing of it is still running
                 del self.captured[oldest]
             captured = self._capture(*key)
-            self.runner.know_layers(captured.step)
         self.captured[key] = captured  # most recently used last
         return captured
+
+    def _affords(self, key: tuple, gain: float) -> bool:
+        """Whether a step of groups runs as one: its graph is there, or the steps of this shape, this one among them, are worth its capture."""
+        shape = key[2]
+        if len(self.gained) > 4096:
+            self.gained.clear()
+        self.gained[shape] = self.gained.get(shape, 0.0) + gain
+        if key in self.captured:
+            return True
+        if self.gained[shape] < CAPTURE_GAINS * ops.SHARED_LEAST_BYTES:
+            return False
+        self.gained[shape] -= CAPTURE_GAINS * ops.SHARED_LEAST_BYTES
+        return True
 
     # -- one step ----------------------------------------------------------------------
     def run(self, entries, copy: bool = True, device_tokens: torch.Tensor | None = None) -> torch.Tensor:
@@ -161,10 +186,13 @@ class DecodeGraphs:
             starts_of = {i: positions for positions, which in shared for i in which}
             own = ops.own_bucket(max(s + 1 - starts_of.get(i, 0) for i, s in enumerate(starts)), runner.cache.page_size)
             shape = ops.shared_shape(shared)
-            if any(ops.sharing_pays(layer, shape, batch, own) for layer in runner.attention_layers):
+            gains = [(count, ops.sharing_gain(layer, shape, batch, own)) for layer, count in runner.attention_layers.items()]
+            # A layer's, over all of the model's: those that read for each request, and those without attention, are captured too.
+            gain = sum(count * g for count, g in gains if g >= 0) / len(runner.cache.needs)
+            if any(g >= 0 for _, g in gains) and self._affords((batch, width, shape, own), gain):
                 beyond = (shape, own)
             else:
-                shared = ()  # the same step as without groups: no shape of theirs is captured
+                shared = ()  # the same step as without groups
         captured = self._graph_for(batch, width, *beyond)
         if captured.copied is not None:
             captured.copied.synchronize()  # the pinned buffer is free to be written again

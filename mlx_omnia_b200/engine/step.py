@@ -14,6 +14,7 @@ engine's own design.
 
 from __future__ import annotations
 
+from collections import Counter
 from dataclasses import dataclass, field
 
 import numpy as np
@@ -130,7 +131,7 @@ class StepRunner:
     def __init__(self, model: DecoderModel, cache: CacheManager, runtime: Runtime, cuda_graphs: bool = False) -> None:
         self.model, self.cache, self.runtime = model, cache, runtime
         self.steps_run = 0
-        self.attention_layers: set = set()  # kinds (`ops.AttentionLayer`) that the model was seen to run
+        self.attention_layers: Counter = Counter()  # kinds (`ops.AttentionLayer`) that a step was seen to run, and how often
         self.cuda_graphs = cuda_graphs
         self.graphs = self.mixed_graphs = None
         self.forget_graphs()
@@ -148,10 +149,13 @@ class StepRunner:
             if MixedGraphs.supported(self.model):
                 self.mixed_graphs = MixedGraphs(self)
 
+    def ask_for_layers(self) -> dict:
+        """A step's workspace, in which attention notes its layers until these are known. (Every step runs all of them, and requests share positions
+        that a step has read, so they are known by the time that a captured step is asked whether it pays to read these once.)"""
+        return {} if self.attention_layers else {"attention_layers": Counter()}
+
     def know_layers(self, step: StepContext) -> None:
-        """Note which kinds of attention layers a step has run. (Every step runs all of them, and requests share positions that a step has read, so
-        they are known by the time that a captured step is asked whether it pays to read these once.)"""
-        self.attention_layers |= (step.workspace or {}).get("attention_layers", set())
+        self.attention_layers = step.workspace.pop("attention_layers", self.attention_layers)
 
     # -- metadata ----------------------------------------------------------------------
     def take_pages(self, entries: list[StepEntry]) -> list[int]:
@@ -236,8 +240,7 @@ class StepRunner:
                 logits = self.mixed_graphs.run(shape, entries, copy)
             else:
                 step = self.build_context(entries)
-                if not self.attention_layers:
-                    step.workspace = {"attention_layers": set()}
+                step.workspace = self.ask_for_layers()
                 logits = self.model.forward(step, self.layer_contexts(step))
                 self.know_layers(step)
         for entry in entries:

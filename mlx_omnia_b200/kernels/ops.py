@@ -824,21 +824,26 @@ def attention_layer(kv: KVView, nq: int, window: int | None = -1) -> AttentionLa
     return AttentionLayer(nq, nkv, d, dv, kv.pages.dtype, kv.page_size, every)
 
 
-def sharing_pays(layer: AttentionLayer, shape: tuple[tuple[int, int], ...], requests: int = 0, own: int = 0) -> bool:
-    """Whether such a layer reads groups of this `shared_shape` once: every position in sight, and enough of them (`SHARED_LEAST_BYTES`) for what
-    the step's requests hold beyond them, `own` positions (`own_bucket`) at most (`SHARED_OWN_BYTES`; 0 outside of a pass, where the ordinary
-    kernel has no list). Asked by the layers of a step, and by the runner ahead of a captured one."""
+def sharing_gain(layer: AttentionLayer, shape: tuple[tuple[int, int], ...], requests: int = 0, own: int = 0) -> float:
+    """What such a layer gains by reading groups of this `shared_shape` once, in bytes that it would else have read (below zero: it loses, and reads for
+    each request): every position in sight, and more of them saved than the line (`SHARED_LEAST_BYTES`), which lies the higher the more the step's requests
+    hold beyond them, `own` positions (`own_bucket`) at most (`SHARED_OWN_BYTES`; 0 outside of a pass, where the ordinary kernel has no list)."""
     if not layer.every:
-        return False
+        return -1.0
     nkv, d, dv = layer.nkv, layer.d, layer.dv
     if d != dv or not tiled_attention_supported(layer.dtype, layer.nq, nkv, d):
-        return True
+        return 12.0 * SHARED_LEAST_BYTES  # (50 us at the least, see there)
     if layer.nq // nkv > 8 and not tcgen05_attention_supported(layer.dtype, layer.nq, nkv, d, layer.page_size):
-        return False  # sixteen rows are one request's
+        return -1.0  # sixteen rows are one request's
     position = nkv * (d + dv) * layer.dtype.itemsize
     saved = sum(positions * (count - 1) for positions, count in shape) * position
     beyond = (1 << max(requests - 1, 0).bit_length()) * own * position
-    return saved >= SHARED_LEAST_BYTES * (1 + min(beyond, SHARED_OWN_MOST) / SHARED_OWN_BYTES)
+    return saved - SHARED_LEAST_BYTES * (1 + min(beyond, SHARED_OWN_MOST) / SHARED_OWN_BYTES)
+
+
+def sharing_pays(layer: AttentionLayer, shape: tuple[tuple[int, int], ...], requests: int = 0, own: int = 0) -> bool:
+    """Whether such a layer reads groups of this shape once. Asked by the layers of a step, and by the runner ahead of a captured one."""
+    return sharing_gain(layer, shape, requests, own) >= 0
 
 
 def shared_applies(step: StepContext, kv: KVView, nq: int, window: int | None = -1) -> bool:
@@ -1085,7 +1090,7 @@ def paged_attention(q: torch.Tensor | None, kv: KVView, step: StepContext, scale
     (head sizes 64 and 128, pages of a multiple of 16) or the mma.sync prefill kernel. Other
     cases (the 32-bit path among them) run on the generic kernel."""
     if step.workspace and "attention_layers" in step.workspace:  # the runner wants to know
-        step.workspace["attention_layers"].add(attention_layer(kv, q.shape[1] if projection is None else projection.nq, window))
+        step.workspace["attention_layers"][attention_layer(kv, q.shape[1] if projection is None else projection.nq, window)] += 1
     if shares(step):
         check_shared(step)
     if not chunk and shared_applies(step, kv, q.shape[1] if projection is None else projection.nq, window):

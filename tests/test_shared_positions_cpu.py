@@ -3,6 +3,7 @@ scheduler does with followers, the lists that the attention kernels read, and an
 
 from __future__ import annotations
 
+import math
 import random
 from types import SimpleNamespace
 
@@ -552,8 +553,10 @@ class Planned(Exception):
                                                                    (40000, 2, 1, False, True)])
 def test_a_captured_step_has_no_groups_where_no_layer_reads_them_once(positions, members, alone, windowed, pays, monkeypatch):
     """What a step is kept by is decided ahead of its capture: where no layer gains by groups, by what the same step without them is."""
+    from mlx_omnia_b200.engine import decode_graph
     from mlx_omnia_b200.engine.decode_graph import DecodeGraphs
 
+    monkeypatch.setattr(decode_graph, "CAPTURE_GAINS", 0)
     spec = KVSpec.keys_and_values(8, 128, None)
     cache = manager((spec,), pages=6000, page_size=16, max_requests=16, allocate=False)
     leader = cache.open("leader")
@@ -561,7 +564,7 @@ def test_a_captured_step_has_no_groups_where_no_layer_reads_them_once(positions,
     requests = [leader] + [cache.fork(leader, f"f{i}") for i in range(members - 1)] + [cache.open(f"a{i}") for i in range(alone)]
     for request in requests[members:]:
         cache.grow(request, 50)
-    runner = SimpleNamespace(cache=cache, attention_layers={ops.AttentionLayer(16, 8, 128, 128, torch.bfloat16, 16, not windowed)},
+    runner = SimpleNamespace(cache=cache, attention_layers={ops.AttentionLayer(16, 8, 128, 128, torch.bfloat16, 16, not windowed): 1},
                              take_pages=lambda entries: [e.request.tokens for e in entries])
     graphs, keys = DecodeGraphs(runner), []
 
@@ -576,6 +579,46 @@ def test_a_captured_step_has_no_groups_where_no_layer_reads_them_once(positions,
     batch, width = 1 << (len(requests) - 1).bit_length(), ops.width_bucket(-(-positions // 16))
     shape = ops.shared_shape(shared_positions(entries))
     assert keys == [(batch, width, shape, ops.own_bucket(51 if alone else 1, 16)) if pays else (batch, width)]
+
+
+def test_a_shape_of_groups_is_captured_when_its_steps_are_worth_it(monkeypatch):
+    from mlx_omnia_b200.engine.decode_graph import CAPTURE_GAINS, DecodeGraphs
+
+    cache = manager((KVSpec.keys_and_values(8, 128, None),), pages=6000, page_size=16, max_requests=16, allocate=False)
+    layer = ops.AttentionLayer(16, 8, 128, 128, torch.bfloat16, 16, True)
+    graphs, keys = DecodeGraphs(SimpleNamespace(cache=cache, attention_layers={layer: 1}, take_pages=lambda entries: [e.request.tokens for e in entries])), []
+
+    def graph_for(*key):
+        keys.append(key)
+        graphs.captured[key] = None
+        raise Planned
+
+    monkeypatch.setattr(graphs, "_graph_for", graph_for)
+
+    def steps(entries, count):
+        del keys[:]
+        for _ in range(count):
+            with pytest.raises(Planned):
+                graphs.run(entries)
+        return [len(key) > 2 for key in keys]
+
+    leader = cache.open("leader")
+    cache.grow(leader, 16000)
+    entries = [StepEntry(r, [1], [0]) for r in [leader] + [cache.fork(leader, f"f{i}") for i in range(7)]]
+    shape = ops.shared_shape(shared_positions(entries))
+    gain = ops.sharing_gain(layer, shape, 8, ops.own_bucket(1, 16))
+    first = math.ceil(CAPTURE_GAINS * ops.SHARED_LEAST_BYTES / gain)
+    assert 10 < first < 100
+    assert steps(entries, 3 * first) == [False] * (first - 1) + [True] * (2 * first + 1)
+    # What the shape has gained since pays for the graph of the next bound of what requests hold of their own.
+    for entry in entries:
+        cache.grow(entry.request, 200)
+    assert steps(entries, 2) == [True, True]
+    # Another shape has an account of its own.
+    assert steps(entries[:4], 2) == [False, False]
+    graphs.gained |= {i: 1.0 for i in range(5000)}
+    steps(entries, 1)
+    assert len(graphs.gained) == 1
 
 
 # -- answers ----------------------------------------------------------------------------------------------------------
