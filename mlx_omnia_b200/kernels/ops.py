@@ -879,7 +879,8 @@ def own_bucket(positions: int, page_size: int) -> int:
 
 @dataclass
 class _SharedCall:
-    """What a step's layers of one cache layout tell the kernels alike, and the memory that this names."""
+    """What a step's layers of one cache layout tell the kernels alike, and the memory that this names (its own: what a caller hands over is taken
+    anew by every call)."""
 
     args: _SharedArgs
     launch: Callable[[], int]
@@ -978,12 +979,12 @@ def _shared_call(step: StepContext, kv: KVView, q: torch.Tensor, positive: bool,
     else:
         rows, tile, least, places = SHARED_ROWS, SHARED_TILE, 2, 4 * sms
     plan = shared_plan(shape, group, nkv, rows, tile, least, places)
-    listed = _step_list(step, ("shared", group, nkv, rows, tile, plan, () if step.shared_shape is not None else step.shared), lambda st: shared_list(st, plan, group, nkv, rows, tile), device)
+    listed = _step_list(step, ("shared", n, group, nkv, rows, tile, plan, () if step.shared_shape is not None else step.shared), lambda st: shared_list(st, plan, group, nkv, rows, tile), device)
     # (The decode kernel's chunks lie at fixed positions, so a request's may be one more than its positions fill.)
     max_parts, max_chunks = max(plan.parts), -(-own // chunk) + int(tensor_cores or in_decode)
     count = n * nq * (max_parts + max_chunks)
     held = [listed, torch.empty(count, dv, device=device), torch.empty(count, 2, device=device)]
-    args = _SharedArgs(cu_seqlens=_ptr(step.cu_seqlens), seq_lens=_ptr(step.seq_lens), plan=_ptr(listed), part_o=_ptr(held[1]), part_ml=_ptr(held[2]),
+    args = _SharedArgs(plan=_ptr(listed), part_o=_ptr(held[1]), part_ml=_ptr(held[2]),
                        err=_ptr(error_word(device)), page_stride=kv_layout(kv)[2], requests=n, members=plan.members, items=plan.items,
                        max_parts=max_parts, chunk_keys=chunk, max_chunks=max_chunks, max_pages=max_pages, num_pages=num_pages, nq=nq, nkv=nkv,
                        d=d, dv=dv, page_size=kv.page_size, maps=maps)
@@ -1028,7 +1029,7 @@ def _shared_attention(q: torch.Tensor, kv: KVView, step: StepContext, scale: flo
     """`paged_attention` of a step whose requests share positions (`StepContext.shared`): a group's shared positions as pieces for all of its
     rows, each request's own in chunks, both put together at the end."""
     pages, table = kv.pages, kv.block_table
-    own = tuple(step.seq_lens_host) if step.max_own is None else step.max_own
+    own = (tuple(step.seq_lens_host) or step.max_seq_len) if step.max_own is None else step.max_own
     key = ("shared_call", step.shared if step.shared_shape is None else step.shared_shape, own, q.shape, q.dtype, pages.shape, table.shape, kv.page_size, kv.spec, scale > 0, difference)
     call = step.workspace.get(key)
     if call is None:
@@ -1043,6 +1044,7 @@ def _shared_attention(q: torch.Tensor, kv: KVView, step: StepContext, scale: flo
     else:
         args.gate, args.gate_stride = gate.data_ptr() + gate_col * gate.element_size(), gate.shape[1]
     args.sink, args.scale, args.softcap = _ptr(sink), scale, softcap
+    args.cu_seqlens, args.seq_lens = _ptr(step.cu_seqlens), _ptr(step.seq_lens)
     if difference is not None:
         args.difference = _MapDifferenceArgs(difference.lam, difference.eps, difference.factor, difference.dv)
     global launches

@@ -3,6 +3,7 @@ scheduler does with followers, the lists that the attention kernels read, and an
 
 from __future__ import annotations
 
+import dataclasses
 import math
 import random
 from types import SimpleNamespace
@@ -20,7 +21,7 @@ from mlx_omnia_b200.engine.generate import Generator, LanguageModel, common_star
 from mlx_omnia_b200.engine.scheduler import Request, Scheduler
 from mlx_omnia_b200.engine.step import StepEntry, shared_positions
 from mlx_omnia_b200.kernels import ops
-from mlx_omnia_b200.parts.base import KVSpec, StateSpec, StepContext
+from mlx_omnia_b200.parts.base import KVSpec, KVView, StateSpec, StepContext
 from mlx_omnia_b200.parts.model import CacheNeed
 
 FULL, WINDOW = KVSpec.keys_and_values(2, 4, None), KVSpec.keys_and_values(2, 4, 10)
@@ -543,6 +544,55 @@ def test_sharing_is_weighed_against_what_requests_hold_of_their_own(groups, alon
     # Other types and widths have no list.
     pages = torch.empty(1, 2, 8, 16, 128, device="meta")
     assert ops.shared_applies(step, SimpleNamespace(pages=pages, spec=None, page_size=16, window=None), 16)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_every_call_reads_the_lengths_and_the_list_of_its_own_step(dtype, monkeypatch):
+    """Steps that share a workspace (`dataclasses.replace`) keep plans and scratch memory with it, and no tensor of one another's."""
+    calls = []
+
+    def function(library, name, argtypes, defines=None):
+        def run(at, *rest):
+            if not calls or calls[-1] is not at:
+                calls.append(at)
+            return 0
+
+        return run
+
+    monkeypatch.setattr(ops, "_function", function)
+    monkeypatch.setattr(ops, "_stream", lambda: 0)
+    monkeypatch.setattr(ops, "sm_count", lambda device: 148)
+    monkeypatch.setattr(ops, "error_word", lambda device: torch.zeros(1, dtype=torch.int32))
+    monkeypatch.setattr(ops, "SHARED_LEAST_BYTES", 0)
+    monkeypatch.setattr(ops, "_ints_to_device", lambda values, device: torch.as_tensor(values))
+
+    def ints(values):
+        return torch.tensor(values, dtype=torch.int32)
+
+    step = step_of([300, 280, 290], ((256, (0, 1, 2)),))
+    step.cu_seqlens, step.seq_lens = ints([0, 1, 2, 3]), ints([300, 280, 290])
+    spec = KVSpec.keys_and_values(2, 64, None)
+    kv = KVView(torch.zeros(64, 2, 2, 16, 64, dtype=dtype), ints([[0] * 20] * 4), torch.zeros(4, dtype=torch.int64), 16, None, spec=spec)
+
+    def run(step):
+        q = torch.zeros(step.num_seqs, 4, 64, dtype=dtype)
+        ops.paged_attention(q, kv, step, 0.1)
+        args = calls[-1]._obj
+        assert (args.cu_seqlens, args.seq_lens) == (step.cu_seqlens.data_ptr(), step.seq_lens.data_ptr()) and args.requests == step.num_seqs
+        held = next(call for call in step.workspace.values() if isinstance(call, ops._SharedCall) and call.args is args).held[0]
+        assert args.plan == held.data_ptr()
+        return held.tolist()
+
+    first = run(step)
+    other = dataclasses.replace(step, seq_lens=ints([299, 279, 289]), cu_seqlens=ints([0, 1, 2, 3]))
+    assert other.workspace is step.workspace and run(other) == first and run(step) == first
+    more = dataclasses.replace(step, num_seqs=4, num_tokens=4, cu_seqlens=ints([0, 1, 2, 3, 4]), seq_lens=ints([300, 280, 290, 5]))
+    assert run(more)[:8] == [256, 256, 256, 0, *first[3:6], 0]
+    # Lengths that the host does not know: what the step is laid out for follows from its bound.
+    for longest in (300, 1200):
+        run(dataclasses.replace(step, seq_lens_host=[], max_seq_len=longest))
+        args = calls[-1]._obj
+        assert args.max_chunks * args.chunk_keys >= longest
 
 
 class Planned(Exception):
