@@ -1333,7 +1333,8 @@ def copy_pages(pages: torch.Tensor, rows: tuple[tuple[int, int], ...], page_size
     """In place: of every layer's pages (`pages` [layers, pages, ...], contiguous), the first `count` stored rows of page `src` to
     page `dst`, for every (src, dst, count) of `moves`. `rows`: what a page holds, the `(heads, width)` of a `KVSpec`, each a block
     [heads, page_size, width]. `to`: another such tensor (as many layers, other pages, of the same type and page shape) that the
-    pages go to. No two moves may end in the same page, and within one tensor none where another begins. -> the tensor written"""
+    pages go to, and that shares no memory with `pages`. No two moves may end in the same page, and within one tensor none where another
+    begins. -> the tensor written"""
     shape, item = pages.shape, pages.element_size()
     to = pages if to is None else to
     if not pages.is_contiguous() or (to is not pages and (not to.is_contiguous() or pages.dtype != to.dtype or pages.device != to.device or
@@ -1343,7 +1344,11 @@ def copy_pages(pages: torch.Tensor, rows: tuple[tuple[int, int], ...], page_size
     if sum(h * w for h, w in rows) * page_size != elements:
         raise KernelError(f"pages of {elements} elements do not hold {page_size} rows of {rows}")
     address, to_address = pages.data_ptr(), to.data_ptr()
-    held = _move_array(moves, 3, shape[1], to.shape[1], address == to_address, "copy_pages")
+    # Page numbers of the two name the same places where they begin together and their layers do; else nothing of one may lie in the other.
+    same = address == to_address and (shape[1] == to.shape[1] or shape[0] <= 1)
+    if not same and address < to_address + to.numel() * item and to_address < address + pages.numel() * item:
+        raise KernelError("copy_pages takes two tensors that do not overlap, or one")
+    held = _move_array(moves, 3, shape[1], to.shape[1], same, "copy_pages")
     if held:
         counts = held[2::3]
         if min(counts) < 0 or max(counts) > page_size:

@@ -196,6 +196,22 @@ def test_a_fork_needs_the_page_that_it_goes_on_in(positions):
     cache.check()
 
 
+def test_pages_are_not_copied_between_tensors_that_overlap(monkeypatch):
+    monkeypatch.setattr(ops, "_stream", lambda: 0)
+    pages, row = torch.zeros(1, 8, 2 * 2 * 8 * 4), ((2, 8), (2, 8))
+    for source, to in ((pages[:, :6], pages[:, 1:7]), (pages[:, 2:], pages[:, :3]), (pages[:, :5], pages[:, 4:])):
+        with pytest.raises(ops.KernelError, match="overlap"):
+            ops.copy_pages(source, row, 4, [(0, 1, 4)], to=to)
+    layers = torch.zeros(24, 128)
+    with pytest.raises(ops.KernelError, match="overlap"):  # page 8 of one layer is page 0 of the next
+        ops.copy_pages(layers[:16].view(2, 8, 128), row, 4, [(0, 1, 4)], to=layers.view(2, 12, 128))
+    with pytest.raises(ops.KernelError, match="another begins"):
+        ops.copy_pages(pages[:, :5], row, 4, [(0, 1, 4), (1, 2, 4)], to=pages)
+    # Nothing to move: neighbours and one tensor seen twice are taken.
+    assert ops.copy_pages(pages[:, :4], row, 4, [], to=pages[:, 4:]).data_ptr() == pages[:, 4:].data_ptr()
+    ops.copy_pages(pages, row, 4, [], to=pages[:, :5])
+
+
 @pytest.mark.parametrize("specs", [(FULL, WINDOW), (UNEQUAL, FULL)])
 @pytest.mark.parametrize("pages", [9, 60])
 def test_resizing_keeps_what_is_held(specs, pages):
