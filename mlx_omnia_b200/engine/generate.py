@@ -233,7 +233,8 @@ class Generator:
 
     def resize_cache(self, tokens: int) -> None:
         """Give the page pools of a running engine room for `tokens` positions, more or fewer: what live requests hold is kept
-        (CacheError where it would not fit). The step in flight is finished first; captured steps are made anew."""
+        (CacheError where it would not fit, and nothing changed). A step in flight, which steady decoding leaves behind every `step()`, is a ValueError:
+        `drain()` first, and read the outputs that it returns. Captured steps are made anew."""
         if self._in_flight is not None:
             raise ValueError("a step is in flight; drain() it and read its outputs first")
         engine = self.engine

@@ -605,6 +605,33 @@ def test_a_running_engine_whose_cache_is_resized(tmp_path):
     assert [r.generated for r in requests] == [plain_impl.greedy_generate(raw, weights, p, 12) for p in prompts]
 
 
+def test_a_pipelined_engine_is_drained_ahead_of_a_resize(tmp_path):
+    raw, weights = write_folder(tmp_path / "m", "B")
+    model = load(tmp_path / "m", dtype="float32", page_size=8, cache_tokens=512, max_requests=4, max_tokens_per_step=64)
+    generator: Generator = model.generator
+    assert generator.pipelined
+    prompts = [tiny_configs.prompt(n, 1000, 30 + n) for n in (5, 33)]
+    requests = [generator.add(p, GenerationOptions(max_tokens=12, stop=())) for p in prompts]
+    in_flight = 0
+    for tokens in (256, 96, 2000):
+        generator.step()
+        generator.step()
+        if generator._in_flight is not None:
+            in_flight += 1
+            pages = [g.pages.data_ptr() for g in model.engine.cache.groups]
+            with pytest.raises(ValueError, match="in flight"):
+                generator.resize_cache(tokens)
+            assert [g.pages.data_ptr() for g in model.engine.cache.groups] == pages
+        held = sum(len(r.generated) for r in requests)
+        assert sum(output.token is not None for output in generator.drain()) == sum(len(r.generated) for r in requests) - held
+        generator.resize_cache(tokens)
+        model.engine.cache.check()
+    assert in_flight
+    generator.run()
+    ops.raise_on_error(model.engine.runtime.device)
+    assert [r.generated for r in requests] == [plain_impl.greedy_generate(raw, weights, p, 12) for p in prompts]
+
+
 @pytest.mark.parametrize("graphs", [True, False])
 @pytest.mark.parametrize("family,name", [("bobarax", "K"), ("bobarax", "L"), ("dolutar", "P"), ("dolutar", "Q"), ("fokalorn", "X"), ("fokalorn", "Y"), ("gisudra", "G"),
                                          ("gisudra", "H"), ("narezen", "P"), ("narezen", "Q"), ("rinirax", "S"), ("rinirax", "T")])
