@@ -225,7 +225,8 @@ shared_merge_kernel(const __grid_constant__ SharedAttention a, int fixed) {
   pdl_launch_dependents();
   if (length < 1) return;
   const int own = length - (fixed ? start / a.chunk_keys * a.chunk_keys : start);
-  if (own > a.max_chunks * (long long)a.chunk_keys && blockIdx.x == 0 && tid == 0) atomicOr(a.err, OMNIA_ERR_WORK);  // more than the step was laid out for
+  // More than the step was laid out for, or no more than is shared.
+  if ((own > a.max_chunks * (long long)a.chunk_keys || length <= start) && blockIdx.x == 0 && tid == 0) atomicOr(a.err, OMNIA_ERR_WORK);
   const int count = min(parts, a.max_parts) + max(0, min((own + a.chunk_keys - 1) / a.chunk_keys, a.max_chunks));
   const int places = a.max_parts + a.max_chunks;
   constexpr int PER_THREAD = 4;  // widths of at most 512

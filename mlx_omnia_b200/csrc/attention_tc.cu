@@ -694,7 +694,11 @@ attention_decode_kernel(const bf16* q, const bf16* __restrict__ pages,
     const int c0 = first / chunk_keys;  // blocks count from the first chunk in sight: a window needs a window's worth of them
     lo = max(first, (c0 + chunk) * chunk_keys), hi = min(pos, (c0 + chunk + 1) * chunk_keys - 1);
     if (pos < 0 || lo > hi) {
-      if (early || (beside && pos < 0)) pdl_wait();
+#if SHARED
+      // A request that holds no more than it shares: lengths that the host did not know. Its row is not written.
+      if (pos >= 0 && pos < first && chunk == 0 && threadIdx.x == 0) atomicOr(err, OMNIA_ERR_WORK);
+#endif
+      if (early || (beside && pos < first)) pdl_wait();
       return;
     }
     chunks = pos / chunk_keys - c0 + 1;

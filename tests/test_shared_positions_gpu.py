@@ -397,6 +397,22 @@ def test_lengths_that_the_host_does_not_know(layout, way):
     check(case)
 
 
+@pytest.mark.parametrize("layout", ["16/8x128", "32/8x128", "8/1x24 f32", "8/8x96", "34/2x64"])
+@pytest.mark.parametrize("wrong", [200, 150, 1])
+def test_lengths_no_longer_than_what_is_shared_are_an_error(layout, wrong, way):
+    """Where the host knows the lengths it refuses these; where it does not, the kernels say so."""
+    nq, nkv, d, dtype, page = LAYOUTS[layout]
+    case = make(nq, nkv, d, dtype, page, [(200, [1, 190, 30])])
+    lengths = case.step.seq_lens.clone()
+    member = case.step.shared[0][1][1]
+    case.step.seq_lens_host, case.step.seq_lens[member] = [], wrong
+    ops.paged_attention(case.q, case.kv, case.step, 0.1)
+    with pytest.raises(ops.KernelError):
+        ops.raise_on_error(case.q.device)
+    case.step.seq_lens.copy_(lengths)
+    check(case)
+
+
 @pytest.mark.parametrize("layout", ["16/8x128", "6/2x64"])
 def test_queries_off_a_16_byte_boundary(layout, way):
     nq, nkv, d, dtype, page = LAYOUTS[layout]
