@@ -301,13 +301,13 @@ shared_pieces_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid
 #pragma unroll
         for (int c = 0; c < HALF; ++c) z[c] = __uint_as_float(raw[c]);
       }
+      if (capped) {  // c tanh(x) = c - 2 c / (1 + e^2x), in log2 units (a score that is infinite has the cap, of its sign)
+#pragma unroll
+        for (int c = 0; c < HALF; ++c) z[c] = fmaf(-2.f * cap, fast_rcp(1.f + fast_exp2(z[c] * twice)), cap);
+      }
       if (seen < HALF) {
 #pragma unroll
         for (int c = 0; c < HALF; ++c) z[c] = c < seen ? z[c] : -INFINITY;
-      }
-      if (capped) {  // c tanh(x) = c - 2 c / (1 + e^2x), in log2 units
-#pragma unroll
-        for (int c = 0; c < HALF; ++c) z[c] = z[c] == -INFINITY ? z[c] : fmaf(-2.f * cap, fast_rcp(1.f + fast_exp2(z[c] * twice)), cap);
       }
       float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll

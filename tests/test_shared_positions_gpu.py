@@ -232,6 +232,33 @@ def test_scales(layout, scale, way):
     check(make(nq, nkv, d, dtype, page, [(300, [1, 90])], seed=6), scale)
 
 
+@pytest.mark.parametrize("layout", ["16/8x128", "32/8x128", "6/2x64", "8/1x24 f32", "34/2x64"])
+@pytest.mark.parametrize("cap", [0.5, 3.0])
+def test_capped_scores_beyond_what_float32_holds(layout, cap, way):
+    """Scores of +-2^128 and more are infinite in float32, and capped all the same: keys weigh e^c or e^-c by their sign.
+
+    A weight is off by the exponential's and the cap's 2^-20 (see `plain`), their sum likewise; sums and joins 600 * 2^-24; in bfloat16 the weights' and
+    the answer's rounding, 2^-8 each."""
+    nq, nkv, d, dtype, page = LAYOUTS[layout]
+    case = make(nq, nkv, d, dtype, page, [(700, [1, 30, 77])], seed=12)
+    case.q = torch.full_like(case.q, 2.0 ** 64)
+    # The same sign all over a position's key: the sign of its first dim.
+    elements = nkv * d * page
+    k_view = case.kv.pages.view(case.kv.pages.shape[0], -1)[:, :elements].view(-1, nkv, page, d)
+    sign = torch.where(k_view[..., :1] < 0, -1.0, 1.0).to(dtype)
+    k_view.copy_(torch.where(torch.isnan(k_view), k_view, sign * 2.0 ** 64))
+    got = ops.paged_attention(case.q, case.kv, case.step, d ** -0.5, softcap=cap)
+    ops.raise_on_error(case.q.device)
+    half = dtype == BF16
+    for r, (k, v) in enumerate(zip(case.ks, case.vs)):
+        p = torch.softmax(torch.where(k[..., 0] < 0, -cap, cap).double(), 0)  # [positions, nkv]
+        out, most = torch.einsum("pk,pkd->kd", p, v), torch.einsum("pk,pkd->kd", p, v.abs())
+        off = 2 * (cap * 2.0 ** -20 + 2.0 ** -20) + 600 * 2.0 ** -24 + (2.0 ** -8 if half else 0.0)
+        bound = off * most + ((2.0 ** -8 if half else 2.0 ** -24) + 2.0 ** -20) * out.abs() + 1e-30
+        mine = got[r].double().view(nkv, nq // nkv, -1)
+        assert float(((mine - out[:, None]).abs() / bound[:, None]).max()) <= 1.0
+
+
 @pytest.mark.parametrize("layout", ["16/8x128", "2/2x64", "8/1x24 f32"])
 def test_what_no_request_holds_does_not_matter(layout, way):
     """The pages' unused rows are NaN above; infinities and the lowest numbers there give the same bits."""
