@@ -19,7 +19,7 @@ from ctypes import c_float, c_int, c_longlong, c_void_p
 
 import dataclasses
 from dataclasses import dataclass
-from typing import Callable
+from typing import Callable, NamedTuple
 
 import numpy as np
 import torch
@@ -805,8 +805,7 @@ heads of 128, shared / each for itself, us a layer: 2 requests of 6,200 shared p
 to 9,355 random steps in six layouts: a layer takes 1.014 times the better way's time on average, with the line where it lies outside of a pass 1.069."""
 
 
-@dataclass(frozen=True)
-class AttentionLayer:
+class AttentionLayer(NamedTuple):
     """What of a layer decides whether its attention reads shared positions once for their group."""
 
     nq: int
@@ -819,26 +818,32 @@ class AttentionLayer:
 
 
 def attention_layer(kv: KVView, nq: int, window: int | None = -1) -> AttentionLayer:
-    _, _, _, nkv, d, dv = kv_layout(kv)
-    every = not (kv.window if window == -1 else window) and (kv.spec is None or (kv.spec.stride == 1 and not kv.spec.chunk))
-    return AttentionLayer(nq, nkv, d, dv, kv.pages.dtype, kv.page_size, every)
+    pages, spec = kv.pages, kv.spec
+    (nkv, d), (_, dv) = spec.rows if spec is not None else ((pages.shape[2], pages.shape[4]),) * 2
+    every = not (kv.window if window == -1 else window) and (spec is None or (spec.stride == 1 and not spec.chunk))
+    return AttentionLayer(nq, nkv, d, dv, pages.dtype, kv.page_size, every)
 
 
 def sharing_gain(layer: AttentionLayer, shape: tuple[tuple[int, int], ...], requests: int = 0, own: int = 0) -> float:
     """What such a layer gains by reading groups of this `shared_shape` once, in bytes that it would else have read (below zero: it loses, and reads for
     each request): every position in sight, and more of them saved than the line (`SHARED_LEAST_BYTES`), which lies the higher the more the step's requests
     hold beyond them, `own` positions (`own_bucket`) at most (`SHARED_OWN_BYTES`; 0 outside of a pass, where the ordinary kernel has no list)."""
-    if not layer.every:
+    nq, nkv, d, dv, dtype, page_size, every = layer
+    if not every:
         return -1.0
-    nkv, d, dv = layer.nkv, layer.d, layer.dv
-    if d != dv or not tiled_attention_supported(layer.dtype, layer.nq, nkv, d):
+    if d != dv or not tiled_attention_supported(dtype, nq, nkv, d):
         return 12.0 * SHARED_LEAST_BYTES  # (50 us at the least, see there)
-    if layer.nq // nkv > 8 and not tcgen05_attention_supported(layer.dtype, layer.nq, nkv, d, layer.page_size):
+    if nq // nkv > 8 and not tcgen05_attention_supported(dtype, nq, nkv, d, page_size):
         return -1.0  # sixteen rows are one request's
-    position = nkv * (d + dv) * layer.dtype.itemsize
-    saved = sum(positions * (count - 1) for positions, count in shape) * position
-    beyond = (1 << max(requests - 1, 0).bit_length()) * own * position
-    return saved - SHARED_LEAST_BYTES * (1 + min(beyond, SHARED_OWN_MOST) / SHARED_OWN_BYTES)
+    position = nkv * (d + dv) * dtype.itemsize
+    saved = 0
+    for positions, count in shape:
+        saved += positions * (count - 1)
+    least = SHARED_LEAST_BYTES
+    if own:
+        beyond = (1 << max(requests - 1, 0).bit_length()) * own * position
+        least *= 1 + min(beyond, SHARED_OWN_MOST) / SHARED_OWN_BYTES
+    return saved * position - least
 
 
 def sharing_pays(layer: AttentionLayer, shape: tuple[tuple[int, int], ...], requests: int = 0, own: int = 0) -> bool:
