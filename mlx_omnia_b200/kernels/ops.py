@@ -768,13 +768,15 @@ def shares(step: StepContext) -> bool:
     return bool(getattr(step, "shared", ()) or getattr(step, "shared_shape", None))
 
 
-def check_shared(step: StepContext) -> None:
-    """Groups of at least one position, of requests of this step that hold more than they share, each in one group. (Looked at once a step.)"""
+def check_shared(step: StepContext) -> tuple[tuple[int, int], ...]:
+    """Groups of at least one position, of requests of this step that hold more than they share, each in one group. (Looked at once a step.) -> the
+    groups' shape"""
     if step.workspace is None:
         step.workspace = {}
     key = ("shared_checked", step.shared, step.num_seqs, tuple(step.seq_lens_host))
-    if key in step.workspace:
-        return
+    shape = step.workspace.get(key)
+    if shape is not None:
+        return shape if step.shared_shape is None else step.shared_shape
     seen: set[int] = set()
     for positions, members in step.shared:
         if positions < 1 or not members or not seen.isdisjoint(members) or len(set(members)) < len(members) or min(members) < 0 or \
@@ -783,7 +785,8 @@ def check_shared(step: StepContext) -> None:
         if step.seq_lens_host and any(m < len(step.seq_lens_host) and step.seq_lens_host[m] <= positions for m in members):
             raise KernelError("a request holds more positions than it shares")
         seen.update(members)
-    step.workspace[key] = True
+    shape = step.workspace[key] = shared_shape(step.shared)
+    return shape if step.shared_shape is None else step.shared_shape
 
 
 SHARED_LEAST_BYTES = 24 << 20
@@ -824,40 +827,50 @@ def attention_layer(kv: KVView, nq: int, window: int | None = -1) -> AttentionLa
     return AttentionLayer(nq, nkv, d, dv, pages.dtype, kv.page_size, every)
 
 
+def _reads_once(layer: AttentionLayer) -> bool | None:
+    """Whether such a layer reads any group once; None where that goes by the groups' sizes."""
+    nq, nkv, d, dv, dtype, page_size, every = layer
+    if not every:
+        return False
+    if d != dv or not tiled_attention_supported(dtype, nq, nkv, d):
+        return True
+    if nq // nkv > 8 and not tcgen05_attention_supported(dtype, nq, nkv, d, page_size):
+        return False  # sixteen rows are one request's
+    return None
+
+
 def sharing_gain(layer: AttentionLayer, shape: tuple[tuple[int, int], ...], requests: int = 0, own: int = 0) -> float:
     """What such a layer gains by reading groups of this `shared_shape` once, in bytes that it would else have read (below zero: it loses, and reads for
     each request): every position in sight, and more of them saved than the line (`SHARED_LEAST_BYTES`), which lies the higher the more the step's requests
     hold beyond them, `own` positions (`own_bucket`) at most (`SHARED_OWN_BYTES`; 0 outside of a pass, where the ordinary kernel has no list)."""
-    nq, nkv, d, dv, dtype, page_size, every = layer
-    if not every:
-        return -1.0
-    if d != dv or not tiled_attention_supported(dtype, nq, nkv, d):
-        return 12.0 * SHARED_LEAST_BYTES  # (50 us at the least, see there)
-    if nq // nkv > 8 and not tcgen05_attention_supported(dtype, nq, nkv, d, page_size):
-        return -1.0  # sixteen rows are one request's
-    position = nkv * (d + dv) * dtype.itemsize
-    saved = 0
+    any_group = _reads_once(layer)
+    if any_group is not None:
+        return 12.0 * SHARED_LEAST_BYTES if any_group else -1.0  # (50 us at the least, see there)
+    return _bytes_gained(layer, shape, requests, own)
+
+
+def _bytes_gained(layer: AttentionLayer, shape: tuple[tuple[int, int], ...], requests: int, own: int) -> float:
+    _, nkv, d, dv, dtype, _, _ = layer
+    position, saved, least = nkv * (d + dv) * dtype.itemsize, 0, SHARED_LEAST_BYTES
     for positions, count in shape:
         saved += positions * (count - 1)
-    least = SHARED_LEAST_BYTES
     if own:
         beyond = (1 << max(requests - 1, 0).bit_length()) * own * position
         least *= 1 + min(beyond, SHARED_OWN_MOST) / SHARED_OWN_BYTES
     return saved * position - least
 
 
-def sharing_pays(layer: AttentionLayer, shape: tuple[tuple[int, int], ...], requests: int = 0, own: int = 0) -> bool:
-    """Whether such a layer reads groups of this shape once. Asked by the layers of a step, and by the runner ahead of a captured one."""
-    return sharing_gain(layer, shape, requests, own) >= 0
-
-
-def shared_applies(step: StepContext, kv: KVView, nq: int, window: int | None = -1) -> bool:
-    """Whether a layer's attention reads shared positions once for their group: a step of single tokens, and `sharing_pays` (for rounded
-    numbers, so that a captured step decides as it did)."""
+def shared_applies(step: StepContext, kv: KVView, nq: int, window: int | None = -1, shape: tuple[tuple[int, int], ...] | None = None) -> bool:
+    """Whether a layer's attention reads shared positions once for their group: a step of single tokens, and no loss by `sharing_gain` (for
+    rounded numbers, so that a captured step decides as it did). `shape`: the groups', where the caller has it."""
     if not shares(step) or not step.decode_only:
         return False
-    requests, own = (step.num_seqs, own_bucket(_own_longest(step), kv.page_size)) if in_pass(step) else (0, 0)
-    return sharing_pays(attention_layer(kv, nq, window), _shape_of(step), requests, own)
+    layer = attention_layer(kv, nq, window)
+    any_group = _reads_once(layer)
+    if any_group is not None:
+        return any_group
+    own = own_bucket(_own_longest(step), kv.page_size) if in_pass(step) else 0
+    return _bytes_gained(layer, _shape_of(step) if shape is None else shape, step.num_seqs, own) >= 0
 
 
 def _own_longest(step: StepContext) -> int:
@@ -1098,9 +1111,8 @@ def paged_attention(q: torch.Tensor | None, kv: KVView, step: StepContext, scale
     cases (the 32-bit path among them) run on the generic kernel."""
     if step.workspace and "attention_layers" in step.workspace:  # the runner wants to know
         step.workspace["attention_layers"][attention_layer(kv, q.shape[1] if projection is None else projection.nq, window)] += 1
-    if shares(step):
-        check_shared(step)
-    if not chunk and shared_applies(step, kv, q.shape[1] if projection is None else projection.nq, window):
+    shape = check_shared(step) if shares(step) else ()
+    if shape and not chunk and shared_applies(step, kv, q.shape[1] if projection is None else projection.nq, window, shape):
         if projection is not None:
             raise KernelError("attention over shared positions takes queries, not projected rows")
         if difference is not None and (gate is not None or sink is not None):

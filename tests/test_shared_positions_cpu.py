@@ -556,7 +556,8 @@ def test_sharing_is_weighed_against_what_requests_hold_of_their_own(groups, alon
     captured = step_of([0] * batch, (), shared_shape=ops.shared_shape(shared), max_own=own)
     captured.seq_lens_host = []
     ops.begin_pass(captured)
-    assert ops.shared_applies(captured, kv, 16) == pays == ops.sharing_pays(ops.attention_layer(kv, 16), ops.shared_shape(shared), len(lengths), own)
+    gain = ops.sharing_gain(ops.attention_layer(kv, 16), ops.shared_shape(shared), len(lengths), own)
+    assert ops.shared_applies(captured, kv, 16) == pays == (gain >= 0)
     # Other types and widths have no list.
     pages = torch.empty(1, 2, 8, 16, 128, device="meta")
     assert ops.shared_applies(step, SimpleNamespace(pages=pages, spec=None, page_size=16, window=None), 16)
