@@ -9,8 +9,9 @@
 // softmax chains that know nothing of one another: each has a score tile of 128 columns and an accumulator in tensor memory, a
 // warp that issues its products and four warps of a thread a row. A slot works on halves of 64 keys, two of which have their columns:
 //   S = Q K^T   tcgen05.mma (M 128, N 64) over the head size, while the half before is weighted
-//   softmax     a row's 64 scores in registers at once; P, rounded to bfloat16, takes the scores' place; the exponent's
-//               offset follows a row's maximum lazily, and only then is the accumulator rescaled
+//   softmax     a row's 64 scores in registers at once; P takes the scores' place, rounded to bfloat16 as the product with V wants it (the
+//               sum is of what was not rounded; outputs are off by 0.0023 of their size, where rounding them alone gives 0.0017);
+//               the exponent's offset follows a row's maximum lazily, and only then is the accumulator rescaled
 //   O += P V    tcgen05.mma (M 128, N head size), P read from tensor memory
 // One chain alone would wait for its own products and loads half of the time; two fill each other's gaps. With more
 // than 128 rows a slot has half of them and both see every tile of keys; with fewer both hold the same rows and take the tiles
@@ -18,11 +19,11 @@
 // Keys and values come by TMA, a box of 16 keys x 64 dims, into rings of stages of 64 keys.
 //
 // Measured (B200, 32/8 heads of 128): 64 requests of 65,536 shared positions and up to 1,024 of their own, with the decode kernel beside,
-// 118 us a layer (floor 68, memory; each request for itself 2,600); 96 of 30,000 + 64 84 us (floor 28, memory; products 48), 16 of
+// 117 us a layer (floor 68, memory; each request for itself 2,600); 96 of 30,000 + 64 83 us (floor 28, memory; products 48), 16 of
 // 32,768 + 500 45 (24). A tile of 128 keys takes a block 2.3 to 2.6 us with 256 rows. Of that the products take 1.8: a step of 16 dims is 76
 // cycles where it scores 64 keys and 102 where it scores 128, since its 128 rows come out of shared memory each time, a step of 16 keys of
 // the second product 52 to 77. Whole tiles of 128 keys have the cheaper scores but wait for them between two softmaxes: 3.3 us. The
-// softmax itself has room (exponentials' unit 48 %, schedulers 49 %): two teams of warps a slot, one a half, made it slower (96 of 30,000: 84 us,
+// softmax itself has room (exponentials' unit 55 %, schedulers 56 % on the busiest SM): two teams of warps a slot, one a half, made it slower (96 of 30,000: 84 us,
 // so 91), and so did asking for the next half's scores ahead of this one's exponentials (96).
 #ifndef HEAD_DIM
 #define HEAD_DIM 128

@@ -257,8 +257,9 @@ class Generator:
         `samples`: answers to every prompt, one after the other in what is returned. The prompt is read once, and every answer
         goes on from there with draws of its own (the sampler's seed + i for answer i where a seed is given).
         `share`: tokens that all of the prompts begin with are read once for all of them. Either way the answers' steps read the keys and
-        values of what they share once for all, which rounds otherwise than reading them request by request: in bfloat16 an answer may part from
-        the one that its prompt has by itself where two tokens are as good as equal."""
+        values of what they share once for all where that pays (on captured steps: when their graph is worth its capture, which depends on the steps
+        before), and this rounds otherwise than reading them request by request: in bfloat16 an answer may part from the one that its prompt has by
+        itself, or had in another call, where two tokens are as good as equal."""
         if samples < 1:
             raise ValueError("samples must be at least 1")
         prompts = [[int(t) for t in p] for p in prompts]
