@@ -245,9 +245,12 @@ class MixedGraphs:
         self.seen: dict[tuple, int] = {}
         self.captured: dict[tuple, _Captured] = {}  # in order of last use, oldest first
         self.replays = 0
-        cache = runner.cache
-        # No block table is wider than the longest request the pools can hold.
-        self.widest = [cache.pages_for(g, cache.capacity_tokens()) for g in range(len(cache.groups))]
+
+    @property
+    def widest(self) -> list[int]:
+        """No block table is wider than the longest request the pools can hold (as they are now: a cache is resized between steps)."""
+        cache = self.runner.cache
+        return [cache.pages_for(g, cache.capacity_tokens()) for g in range(len(cache.groups))]
 
     @staticmethod
     def supported(model) -> bool:

@@ -274,6 +274,18 @@ def test_a_resize_that_runs_out_of_memory_changes_nothing(specs, monkeypatch):
     cache.check()
 
 
+def test_block_tables_of_captured_mixed_steps_are_as_wide_as_a_resized_cache():
+    from mlx_omnia_b200.engine.decode_graph import MixedGraphs
+
+    cache = manager((FULL, STRIDED), pages=10, page_size=4)
+    graphs = MixedGraphs(SimpleNamespace(cache=cache))
+    assert graphs.widest == [10, 4]  # 40 positions
+    cache.resize(50)
+    assert graphs.widest == [50, 17]
+    cache.resize(3)
+    assert graphs.widest == [3, 1]
+
+
 @pytest.mark.parametrize("seed", range(6))
 def test_random_lives_lose_no_page(seed):
     rng = random.Random(seed)

@@ -675,6 +675,24 @@ def test_a_pipelined_engine_is_drained_ahead_of_a_resize(tmp_path):
     assert [r.generated for r in requests] == [plain_impl.greedy_generate(raw, weights, p, 12) for p in prompts]
 
 
+def test_a_cache_that_has_grown_takes_longer_prompts_in_captured_mixed_steps(tmp_path):
+    """A prompt longer than the first pools held is read in portions beside a decoding request, in steps of one shape."""
+    raw, weights = write_folder(tmp_path / "m", "A")
+    model = load(tmp_path / "m", dtype="float32", page_size=4, cache_tokens=128, max_requests=4, max_tokens_per_step=17)
+    generator: Generator = model.generator
+    generator.resize_cache(2048)
+    vocab = raw["text_config"]["vocab_size"]
+    prompts = [tiny_configs.prompt(n, vocab, 50 + n) for n in (9, 700)]
+    requests = [generator.add(p, GenerationOptions(max_tokens=60, stop=())) for p in prompts]
+    generator.run()
+    ops.raise_on_error(model.engine.runtime.device)
+    assert model.engine.runner.mixed_graphs.replays > 10
+    for request, prompt in zip(requests, prompts):
+        logits = plain_impl.forward(raw, weights, prompt + request.generated)[len(prompt) - 1: -1]
+        chosen = logits[torch.arange(60), torch.tensor(request.generated)]
+        assert float((logits.max(dim=-1).values - chosen).max()) <= 1e-4 * float(logits.abs().max())
+
+
 @pytest.mark.parametrize("graphs", [True, False])
 @pytest.mark.parametrize("family,name", [("bobarax", "K"), ("bobarax", "L"), ("dolutar", "P"), ("dolutar", "Q"), ("fokalorn", "X"), ("fokalorn", "Y"), ("gisudra", "G"),
                                          ("gisudra", "H"), ("narezen", "P"), ("narezen", "Q"), ("rinirax", "S"), ("rinirax", "T")])
