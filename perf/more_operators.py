@@ -561,7 +561,8 @@ def run(state):
 
     if case["op"] == "tables":
         lists = [ops.PageLists(pages, starts, width, stride) for pages, starts, width, stride in s["lists"]]
-        made = ops.step_tables(s["held"], s["brought"], lists, case["page"], s["tokens"], parents=s["parents"], most=s["most"])
+        made = ops.step_tables(s["held"], s["brought"], lists, case["page"], s["tokens"], parents=s["parents"],
+                               most=s["most"] if case["trees"] else None)
         return {"positions": made.positions, "cu_seqlens": made.cu_seqlens, "seq_lens": made.seq_lens,
                 "ancestors": None if made.tree is None else made.tree.ancestors, "groups": made.groups}
     if case["op"] == "attention":
