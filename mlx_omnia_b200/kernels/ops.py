@@ -25,7 +25,7 @@ import numpy as np
 import torch
 
 from mlx_omnia_b200.csrc.build import load_library
-from mlx_omnia_b200.parts.base import KVView, StepContext
+from mlx_omnia_b200.parts.base import KVView, StepContext, StepTree
 
 _DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1}
 
@@ -1102,6 +1102,9 @@ def paged_attention(q: torch.Tensor | None, kv: KVView, step: StepContext, scale
     there too. Which kernel, and how the work is cut, follows from rounded numbers: the groups' sizes, the requests, what these hold beyond the
     groups. So a step has the same results captured or not; they round otherwise than each request's by itself.
 
+    In a step of drafted trees (`StepContext.tree`) a token sees what its request holds and, of what the request brings, what its row of the
+    tree names (`tree_attention`); no difference of maps and no projected rows then.
+
     With `projection` (only where `decode_fusable` holds) q is not given: the kernel makes the
     queries and the new keys and values from the projected rows, and writes the latter to the cache.
 
@@ -1111,6 +1114,11 @@ def paged_attention(q: torch.Tensor | None, kv: KVView, step: StepContext, scale
     cases (the 32-bit path among them) run on the generic kernel."""
     if step.workspace and "attention_layers" in step.workspace:  # the runner wants to know
         step.workspace["attention_layers"][attention_layer(kv, q.shape[1] if projection is None else projection.nq, window)] += 1
+    if step.tree is not None:
+        if projection is not None or difference is not None:
+            raise KernelError("attention of drafted trees takes queries, and no difference of maps")
+        return tree_attention(q, kv, step, scale, gate=gate, gate_col=gate_col, sink=sink, window=window, keep_first=keep_first, chunk=chunk,
+                              softcap=softcap)
     shape = check_shared(step) if shares(step) else ()
     if shape and not chunk and shared_applies(step, kv, q.shape[1] if projection is None else projection.nq, window, shape):
         if projection is not None:
@@ -1255,6 +1263,250 @@ def paged_attention(q: torch.Tensor | None, kv: KVView, step: StepContext, scale
               kv.window or 0, scale, keep, _ptr(sink), run, softcap, *last, err, _stream()), "attention_prefill")
     if single is not None:
         single_tokens(True)
+    return out
+
+
+# ------------------------------------------------------------------------------------
+# Steps that read drafted tokens (csrc/drafted.cu, csrc/attention_tree*.cu)
+
+MOST_DRAFTED = 256
+"""Tokens that a request brings to a step of drafted trees at most: eight words of bits, a thread each."""
+
+
+def _here(what: str, *tensors: "torch.Tensor | None") -> int:
+    """The index of the device that all of the tensors lie on, which has to be the current one (a launch goes to its stream)."""
+    index = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and (not t.is_cuda or t.get_device() != index):
+            raise KernelError(f"{what} takes tensors on the current CUDA device ({index}), not on {t.device}")
+    return index
+
+
+def _flat(what: str, name: str, t: torch.Tensor, dtype: torch.dtype, *shape: "int | None") -> torch.Tensor:
+    """`t`, if it is contiguous, of this type and of this shape (None: any size)."""
+    if t.dtype != dtype or t.dim() != len(shape) or not t.is_contiguous() or any(n is not None and m != n for m, n in zip(t.shape, shape)):
+        raise KernelError(f"{what}: {name} is a contiguous {dtype} tensor of {[('any' if n is None else n) for n in shape]}, not {t.dtype} {list(t.shape)}")
+    return t
+
+
+@dataclass(frozen=True)
+class PageLists:
+    """Which physical pages requests hold in one group of caches: `pages` (int32, one dimension) has each request's from `starts[request]`
+    (int64) on, in the order of its positions, -1 where one was given back; lists one behind the other, or the rows of a table that a program
+    keeps. The block table that is made of them has `width` columns; `stride` positions share a stored row."""
+
+    pages: torch.Tensor
+    starts: torch.Tensor
+    width: int
+    stride: int = 1
+
+
+@dataclass(frozen=True)
+class StepTables:
+    """What `step_tables` makes: the fields of a `StepContext` and, for each group, (block table, slot mapping)."""
+
+    positions: torch.Tensor
+    cu_seqlens: torch.Tensor
+    seq_lens: torch.Tensor
+    groups: list[tuple[torch.Tensor, torch.Tensor]]
+    tree: StepTree | None
+
+
+class _TableGroup(ctypes.Structure):
+    _fields_ = [(name, c_void_p) for name in ("pages", "starts", "table", "slots")] + [("count", c_longlong), ("width", c_int), ("stride", c_int)]
+
+
+class _StepTablesArgs(ctypes.Structure):
+    _fields_ = [(name, c_void_p) for name in ("held", "brought", "parents", "positions", "cu_seqlens", "seq_lens", "ancestors", "err")] + \
+               [(name, c_int) for name in ("requests", "tokens", "page_size", "words", "groups")] + [("group", _TableGroup * 8)]
+
+
+def step_tables(held: torch.Tensor, brought: torch.Tensor, lists: "list[PageLists]", page_size: int, tokens: int,
+                parents: torch.Tensor | None = None, most: int | None = None) -> StepTables:
+    """The tables of a step whose requests hold `held` positions (int32 [requests]; below 0: a request that is there for the step's shape only) and
+    bring `brought` tokens (int32 [requests], none allowed), stored behind those: made on the GPU, in one launch, from numbers that may be known
+    there only. `tokens`: rows of the batch, at least as many as are brought; those behind the last request's have position and slot -1.
+
+    With `most` (the most tokens that a request brings, 256 at most) the step is one of drafted trees: `parents` (int32 [tokens]) names for each
+    token the one of its own request's that it goes on from (an earlier one; -1: it goes on from what is held; no `parents`: each from the one ahead
+    of it), a token's position is `held` plus the number of tokens on its way, and `tree` names what it sees. Slots go by the order in which tokens
+    are brought, whatever their positions.
+
+    A list too short or a table too narrow for its request, more tokens than rows, a parent that is no earlier token: the error word, and
+    -1 in the request's tables (`raise_on_error`)."""
+    what = "step_tables"
+    n = held.shape[0]
+    _here(what, held, brought, parents, *(t for x in lists for t in (x.pages, x.starts)))
+    _flat(what, "held", held, torch.int32, None)
+    _flat(what, "brought", brought, torch.int32, n)
+    words = 0
+    if most is not None:
+        if not 1 <= most <= MOST_DRAFTED:
+            raise KernelError(f"{what}: a request brings 1 to {MOST_DRAFTED} drafted tokens, not {most}")
+        words = -(-most // 32)
+    if parents is not None:
+        if most is None:
+            raise KernelError(f"{what}: parents go with `most`, the most tokens that a request brings")
+        _flat(what, "parents", parents, torch.int32, tokens)
+    if not 1 <= n <= 65534 or tokens < 0 or page_size < 1 or len(lists) > 8:
+        raise KernelError(f"{what} takes 1 to 65,534 requests, pages of a token or more and up to eight groups")
+    args = _StepTablesArgs(held=held.data_ptr(), brought=brought.data_ptr(), parents=_ptr(parents), requests=n, tokens=tokens, page_size=page_size,
+                           words=words, groups=len(lists))
+    # One buffer: the slots (8 bytes each) first, then all that has 4.
+    sizes = [2 * tokens] * len(lists) + [tokens, n + 1, n, tokens * words] + [n * x.width for x in lists]
+    for x in lists:
+        _flat(what, "pages", x.pages, torch.int32, None)
+        _flat(what, "starts", x.starts, torch.int64, n)
+        if x.width < 1 or x.stride < 1 or (x.stride > 1 and most is not None):
+            raise KernelError(f"{what}: tables have a column or more, and drafted tokens a stored row each")
+    parts = torch.empty(sum(sizes), dtype=torch.int32, device=held.device).split(sizes)
+    count = len(lists)
+    positions, cu_seqlens, seq_lens, ancestors = parts[count: count + 4]
+    args.positions, args.cu_seqlens, args.seq_lens = positions.data_ptr(), cu_seqlens.data_ptr(), seq_lens.data_ptr()
+    args.ancestors, args.err = ancestors.data_ptr() if words else None, error_word(held.device).data_ptr()
+    groups = []
+    for i, x in enumerate(lists):
+        slots, table = parts[i], parts[count + 4 + i]
+        args.group[i] = _TableGroup(x.pages.data_ptr(), x.starts.data_ptr(), table.data_ptr(), slots.data_ptr(), x.pages.shape[0], x.width, x.stride)
+        groups.append((table.view(n, x.width), slots.view(torch.int64)))
+    fn = _function("drafted", "omnia_step_tables", [c_void_p, c_void_p])
+    _check(fn(ctypes.addressof(args), _stream()), what)
+    return StepTables(positions, cu_seqlens, seq_lens, groups, StepTree(ancestors.view(tokens, words)) if words else None)
+
+
+@dataclass(frozen=True)
+class Accepted:
+    """What of a step's drafted tokens is kept: `path` int32 [requests, 32 * words], the kept ones' numbers within their request's, in order, -1
+    behind them; `kept` int32 [requests], how many; `tokens` int32 [requests], what was chosen behind the last of them (-1: none was brought)."""
+
+    path: torch.Tensor
+    kept: torch.Tensor
+    tokens: torch.Tensor
+
+
+def accept_drafts(chosen: torch.Tensor, token_ids: torch.Tensor, tree: StepTree, cu_seqlens: torch.Tensor) -> Accepted:
+    """Which drafted tokens the model agrees with: from a request's first token, which is known, on to the one that was chosen behind it
+    (`chosen` int32 [tokens]: for every row of the step what its logits gave), as long as that was drafted there, of equal ones the first. Sampled
+    choices keep the model's distribution: each is a draw from its own row, whatever was drafted."""
+    what = "accept_drafts"
+    _here(what, chosen, token_ids, tree.ancestors, cu_seqlens)
+    tokens, words = tree.ancestors.shape if tree.ancestors.dim() == 2 else (0, 0)
+    _flat(what, "ancestors", tree.ancestors, torch.int32, None, None)
+    _flat(what, "chosen", chosen, torch.int32, tokens)
+    _flat(what, "token_ids", token_ids, torch.int32, tokens)
+    _flat(what, "cu_seqlens", cu_seqlens, torch.int32, None)
+    n = cu_seqlens.shape[0] - 1
+    if n < 1 or not 1 <= words <= MOST_DRAFTED // 32:
+        raise KernelError(f"{what} takes a request or more, of {MOST_DRAFTED} tokens at most")
+    path, kept, last = torch.empty(n * (32 * words + 2), dtype=torch.int32, device=chosen.device).split([n * 32 * words, n, n])
+    fn = _function("drafted", "omnia_accept_drafts", [c_void_p] * 4 + [c_int, c_int] + [c_void_p] * 3 + [c_int, c_void_p, c_void_p])
+    _check(fn(chosen.data_ptr(), token_ids.data_ptr(), tree.ancestors.data_ptr(), cu_seqlens.data_ptr(), n, words, path.data_ptr(), kept.data_ptr(),
+              last.data_ptr(), tokens, error_word(chosen.device).data_ptr(), _stream()), what)
+    return Accepted(path.view(n, 32 * words), kept, last)
+
+
+def keep_rows(pages: torch.Tensor, rows: tuple[tuple[int, int], ...], page_size: int, block_table: torch.Tensor, held: torch.Tensor,
+              accepted: Accepted) -> torch.Tensor:
+    """In place: of every layer's pages (`pages` [layers, pages, ...], contiguous, of whatever type; `rows`: what a page holds, as for
+    `copy_pages`), the i-th kept token's rows go to where the i-th token behind the request's `held` positions (int32 [requests]; below 0: nothing) is
+    stored. Other drafted tokens' rows are what they were, or a kept one's. -> `pages`"""
+    what = "keep_rows"
+    _here(what, pages, block_table, held, accepted.path, accepted.kept)
+    _flat(what, "block_table", block_table, torch.int32, None, None)
+    n, width = block_table.shape
+    _flat(what, "held", held, torch.int32, n)
+    _flat(what, "path", accepted.path, torch.int32, n, None)
+    _flat(what, "kept", accepted.kept, torch.int32, n)
+    shape, item = pages.shape, pages.element_size()
+    elements = math.prod(shape[2:])
+    if not pages.is_contiguous() or pages.dim() < 3 or not 1 <= len(rows) <= 8 or sum(h * w for h, w in rows) * page_size != elements:
+        raise KernelError(f"{what} takes contiguous pages that hold {page_size} rows of {rows}")
+    if not 1 <= accepted.path.shape[1] <= MOST_DRAFTED:
+        raise KernelError(f"{what} takes paths of 1 to {MOST_DRAFTED} tokens")
+    heads, sizes = (c_int * len(rows))(*(h for h, _ in rows)), (c_int * len(rows))(*(w * item for _, w in rows))
+    fn = _function("drafted", "omnia_keep_rows", [c_void_p, c_longlong, c_longlong, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_int,
+                                                  c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p])
+    _check(fn(pages.data_ptr(), shape[1] * elements * item, elements * item, shape[0], shape[1], page_size, heads, sizes, len(rows),
+              block_table.data_ptr(), width, held.data_ptr(), accepted.path.data_ptr(), accepted.kept.data_ptr(), n, accepted.path.shape[1],
+              error_word(pages.device).data_ptr(), _stream()), what)
+    return pages
+
+
+class _TreeArgs(ctypes.Structure):  # TreeAttention in attention_tree.cuh
+    _fields_ = [(name, c_void_p) for name in ("q", "k_pages", "v_pages", "gate", "out", "block_table", "cu_seqlens", "seq_lens", "positions",
+                                              "ancestors", "sink", "part_o", "part_ml", "err")] + [("page_stride", c_longlong)] + \
+               [(name, c_int) for name in ("tokens", "requests", "max_pages", "num_pages", "nq", "nkv", "d", "dv", "page_size", "gate_stride", "words",
+                                           "window", "keep", "run", "chunk", "parts")] + [("scale", c_float), ("softcap", c_float)]
+
+
+@functools.lru_cache(maxsize=4096)
+def tree_plan(tiles: int, keys: int, step: int, places: int) -> tuple[int, int]:
+    """(keys a block walks, blocks to a tile of rows) of attention over `keys` keys by `tiles` tiles of rows, in chunks of a multiple of `step` keys: as many
+    blocks as have a place at a time, no chunk shorter than four steps."""
+    parts = max(1, min(places // max(tiles, 1), -(-keys // (4 * step))))
+    chunk = -(-keys // (parts * step)) * step
+    return chunk, -(-keys // chunk)
+
+
+def tree_attention(q: torch.Tensor, kv: KVView, step: StepContext, scale: float, gate: torch.Tensor | None = None, gate_col: int = 0,
+                   sink: torch.Tensor | None = None, window: int | None = -1, keep_first: int | None = None, chunk: int | None = None,
+                   softcap: float | None = None) -> torch.Tensor:
+    """Attention of the step's tokens where requests bring trees of drafted ones (`StepContext.tree`): a token sees the positions that its request
+    holds and the tokens that its row of the tree names, whose keys and values are stored behind those in the order in which they are brought.
+    `gate`, `sink`, `window`, `keep_first`, `chunk`, `softcap` as for `paged_attention`, by the tokens' positions. A token that sees nothing
+    has zeros. -> [tokens, nq * dv] (rows behind the last request's are not written)"""
+    what = "tree_attention"
+    tree = step.tree
+    if tree is None:
+        raise KernelError(f"{what} takes a step of drafted trees")
+    if q.dim() != 3 or not q.is_contiguous():
+        raise KernelError(f"{what} takes contiguous queries [tokens, heads, width]")
+    tokens, nq, d = q.shape
+    k_ptr, v_ptr, page_stride, nkv, dk, dv = kv_layout(kv)
+    code = _code(q.dtype)
+    pages, table, n = kv.pages, kv.block_table, step.num_seqs
+    if dk != d or nq % nkv or pages.dtype != q.dtype or not 1 <= d <= 512 or not 1 <= dv <= 512 or not pages.is_contiguous():
+        raise KernelError(f"{what}: {nq} heads of {d} ({q.dtype}) do not go with a cache of {nkv} heads of {dk} and {dv} ({pages.dtype})")
+    if kv.spec is not None and kv.spec.stride != 1:
+        raise KernelError(f"{what} takes a cache of a row for every position")
+    _here(what, q, pages, table, tree.ancestors, step.cu_seqlens, step.seq_lens, step.positions, gate, sink)
+    _flat(what, "ancestors", tree.ancestors, torch.int32, tokens, None)
+    _flat(what, "positions", step.positions, torch.int32, tokens)
+    _flat(what, "block_table", table, torch.int32, n, None)
+    _flat(what, "cu_seqlens", step.cu_seqlens, torch.int32, n + 1)
+    _flat(what, "seq_lens", step.seq_lens, torch.int32, n)
+    words = tree.ancestors.shape[1]
+    if not 1 <= step.max_q_len <= 32 * words <= MOST_DRAFTED:
+        raise KernelError(f"{what}: a request brings up to {step.max_q_len} tokens, the tree has {words} words for each ({MOST_DRAFTED} tokens at most)")
+    if gate is not None and (gate.dtype != q.dtype or gate.dim() != 2 or gate.stride(1) != 1 or gate.shape[0] != tokens or
+                             gate.shape[1] < gate_col + nq * dv or gate_col < 0):
+        raise KernelError(f"{what}: the gate's {nq * dv} columns from {gate_col} on lie outside rows of {list(gate.shape)}")
+    if sink is not None:
+        _flat(what, "sink", sink, torch.float32, nq)
+    window = (kv.window if window == -1 else window) or 0
+    keep = (kv.keep_first if keep_first is None else keep_first) if window else 0
+    run = int(chunk or 0)
+    if run and keep:
+        raise KernelError("a mask of runs keeps no first positions")
+    out = torch.empty(tokens, nq * dv, dtype=q.dtype, device=q.device)
+    if tokens == 0:
+        return out
+    a = _TreeArgs(q.data_ptr(), k_ptr, v_ptr, None if gate is None else gate.data_ptr() + gate_col * gate.element_size(), out.data_ptr(),
+                  table.data_ptr(), step.cu_seqlens.data_ptr(), step.seq_lens.data_ptr(), step.positions.data_ptr(), tree.ancestors.data_ptr(),
+                  _ptr(sink), None, None, error_word(q.device).data_ptr(), page_stride, tokens, n, table.shape[1], pages.shape[0], nq, nkv, d, dv,
+                  kv.page_size, 0 if gate is None else gate.stride(0), words, window, keep, run, 0, 0, scale, float(softcap or 0.0))
+    # What the longest request can see: the plan is made for that, and from numbers that a captured step knows too.
+    keys = min(max(step.max_seq_len, 1), window + keep + step.max_q_len if window else 1 << 30, run + step.max_q_len if run else 1 << 30)
+    tiles = -(-step.max_q_len * (nq // nkv) // 32) * n * nkv
+    a.chunk, a.parts = tree_plan(tiles, keys, 64, 2 * sm_count(q.device))
+    if a.parts > 1:
+        parts = torch.empty(a.parts * tokens * nq * (dv + 2), dtype=torch.float32, device=q.device)
+        a.part_o, a.part_ml = parts.data_ptr(), parts.data_ptr() + a.parts * tokens * nq * dv * 4
+    fn = _function("attention_tree", "omnia_tree_attention", [c_void_p, c_int, c_int, c_void_p])
+    _check(fn(ctypes.addressof(a), step.max_q_len, code, _stream()), what)
+    if a.parts > 1:
+        fn = _function("attention_tree", "omnia_tree_merge", [c_void_p, c_int, c_void_p])
+        _check(fn(ctypes.addressof(a), code, _stream()), what)
     return out
 
 
@@ -1814,6 +2066,151 @@ def sample(logits: torch.Tensor, temperature: torch.Tensor, top_k: torch.Tensor,
     _check(fn(_ptr(logits), logits.stride(0), rows, vocab, _ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(min_p),
               _ptr(penalty), _ptr(history), 0 if history is None else history.shape[1], _ptr(seeds), _ptr(draws),
               _ptr(out), _stream()), "sample")
+    return out
+
+
+# ------------------------------------------------------------------------------------
+# What a caller's options do to logits (csrc/logits.cu)
+
+
+@dataclass(frozen=True)
+class TokenHistory:
+    """Requests' texts: `tokens` (int32, one dimension) has request r's `lengths[r]` tokens from `starts[r]` on, the first `prompts[r]` of which
+    were given to it and the rest generated (`starts` int64, the others int32 [requests])."""
+
+    tokens: torch.Tensor
+    starts: torch.Tensor
+    lengths: torch.Tensor
+    prompts: torch.Tensor
+
+
+@dataclass(frozen=True)
+class LogitBias:
+    """What requests add to tokens' logits: request r's entries are `starts[r]` to `starts[r + 1]` (int32 [requests + 1]) of `ids` (int32) and
+    `values` (float32); of an id that is named twice, both count."""
+
+    ids: torch.Tensor
+    values: torch.Tensor
+    starts: torch.Tensor
+
+
+@dataclass(frozen=True)
+class TokenMasks:
+    """Which tokens are allowed: `words` int32 [masks, at least vocab / 32], a bit a token (the lowest of word 0 first), and `rows` int32 [rows], the
+    mask of each row of logits (-1: none)."""
+
+    words: torch.Tensor
+    rows: torch.Tensor
+
+
+@dataclass(frozen=True)
+class DraftedRows:
+    """Rows of logits that belong to drafted tokens: `rows` int32 [rows of logits], each one's row of the step, whose tree, token ids and
+    cu_seqlens these are. A request's history then ends ahead of what it brings to the step, and each row's text goes on with the tokens on its
+    way through the tree, its own the last."""
+
+    tree: StepTree
+    token_ids: torch.Tensor
+    cu_seqlens: torch.Tensor
+    rows: torch.Tensor
+
+
+class _AdjustArgs(ctypes.Structure):  # AdjustLogits in logits.cu
+    _fields_ = [(name, c_void_p) for name in (
+        "logits", "out", "requests", "history", "starts", "lengths", "prompts", "contexts", "repetition", "frequency", "presence", "bias_ids",
+        "bias_values", "bias_starts", "mask_words", "mask_rows", "ancestors", "token_ids", "cu_seqlens", "nodes", "err")] + \
+        [(name, c_longlong) for name in ("stride", "out_stride", "history_tokens", "bias_count")] + \
+        [(name, c_int) for name in ("rows", "vocab", "num_requests", "masks", "mask_width", "words", "tokens", "each", "penalised")]
+
+
+def adjust_logits(logits: torch.Tensor, *, history: TokenHistory | None = None, repetition: torch.Tensor | None = None,
+                  frequency: torch.Tensor | None = None, presence: torch.Tensor | None = None, contexts: torch.Tensor | None = None,
+                  requests: torch.Tensor | None = None, bias: LogitBias | None = None, masks: TokenMasks | None = None,
+                  drafted: DraftedRows | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """float32 logits [rows, vocab] (rows may lie apart) under their callers' options, in this order: for a token of the row's text z -> z / repetition
+    where z > 0, else z * repetition; for one that was generated n > 0 times z - frequency * n - presence; z + bias; -infinity where the row's mask
+    does not allow it. A row whose mask allows nothing is -infinity throughout.
+
+    `requests` int32 [rows]: the request that each row belongs to (None: row i is request i's); `repetition`, `frequency`, `presence` float32
+    [requests]: 1, 0 and 0 where None; `contexts` int32 [requests]: the repetition penalty sees so many of the last tokens (0 or None: all).
+    `out`: None for a new tensor; `logits` itself: in place, which reads and writes only what changes; or another tensor of the same shape that
+    shares no memory with it."""
+    what = "adjust_logits"
+    if logits.dim() != 2 or logits.dtype != torch.float32 or logits.stride(1) != 1:
+        raise KernelError(f"{what} takes float32 logits [rows, vocab] whose rows lie in one piece")
+    rows, vocab = logits.shape
+    if out is None:
+        out = torch.empty(rows, vocab, dtype=torch.float32, device=logits.device)
+    same = out is logits or (out.data_ptr() == logits.data_ptr() and out.shape == logits.shape and out.stride() == logits.stride())
+    if out.dtype != torch.float32 or out.shape != logits.shape or out.stride(1) != 1 or (rows > 1 and min(out.stride(0), logits.stride(0)) < vocab):
+        raise KernelError(f"{what} writes float32 rows that lie apart, in the logits' shape")
+    if not same:
+        a, b = logits.data_ptr(), out.data_ptr()
+        if rows and a < b + 4 * ((rows - 1) * out.stride(0) + vocab) and b < a + 4 * ((rows - 1) * logits.stride(0) + vocab):
+            raise KernelError(f"{what} writes to the logits themselves, or to a tensor that shares no memory with them")
+    penalties = [("repetition", repetition), ("frequency", frequency), ("presence", presence)]
+    given = [t for _, t in penalties if t is not None]
+    if (given or contexts is not None) and history is None:
+        raise KernelError(f"{what}: penalties go by the requests' history")
+    tensors = [logits, out, requests, contexts, *given]
+    num = rows
+    if history is not None:
+        num = history.lengths.shape[0]
+        tensors += [history.tokens, history.starts, history.lengths, history.prompts]
+        _flat(what, "tokens", history.tokens, torch.int32, None)
+        _flat(what, "starts", history.starts, torch.int64, num)
+        _flat(what, "lengths", history.lengths, torch.int32, num)
+        _flat(what, "prompts", history.prompts, torch.int32, num)
+    if bias is not None:
+        if history is None:
+            num = bias.starts.shape[0] - 1
+        tensors += [bias.ids, bias.values, bias.starts]
+        _flat(what, "ids", bias.ids, torch.int32, None)
+        _flat(what, "values", bias.values, torch.float32, bias.ids.shape[0])
+        _flat(what, "bias starts", bias.starts, torch.int32, num + 1)
+    for name, t in penalties:
+        if t is not None:
+            _flat(what, name, t, torch.float32, num)
+    if contexts is not None:
+        _flat(what, "contexts", contexts, torch.int32, num)
+    if requests is not None:
+        _flat(what, "requests", requests, torch.int32, rows)
+    elif (history is not None or bias is not None) and num < rows:
+        raise KernelError(f"{what}: {rows} rows of {num} requests need `requests`")
+    if masks is not None:
+        tensors += [masks.words, masks.rows]
+        _flat(what, "mask words", masks.words, torch.int32, None, None)
+        _flat(what, "mask rows", masks.rows, torch.int32, rows)
+        if masks.words.shape[1] * 32 < vocab:
+            raise KernelError(f"{what}: {masks.words.shape[1]} words do not hold {vocab} tokens")
+    if drafted is not None:
+        tensors += [drafted.tree.ancestors, drafted.token_ids, drafted.cu_seqlens, drafted.rows]
+        _flat(what, "ancestors", drafted.tree.ancestors, torch.int32, None, None)
+        _flat(what, "token_ids", drafted.token_ids, torch.int32, drafted.tree.ancestors.shape[0])
+        _flat(what, "cu_seqlens", drafted.cu_seqlens, torch.int32, None)
+        _flat(what, "drafted rows", drafted.rows, torch.int32, rows)
+        if history is not None and (requests is None or drafted.cu_seqlens.shape[0] != num + 1):
+            raise KernelError(f"{what}: drafted rows need `requests`, and the step of the same {num} requests")
+    _here(what, *tensors)
+    if rows == 0 or vocab == 0:
+        return out
+    a = _AdjustArgs(logits=logits.data_ptr(), out=out.data_ptr(), requests=_ptr(requests), repetition=_ptr(repetition), frequency=_ptr(frequency),
+                    presence=_ptr(presence), contexts=_ptr(contexts), err=error_word(logits.device).data_ptr(), stride=logits.stride(0),
+                    out_stride=out.stride(0), rows=rows, vocab=vocab, num_requests=num)
+    if history is not None and given:
+        a.history, a.starts, a.lengths, a.prompts = (t.data_ptr() for t in (history.tokens, history.starts, history.lengths, history.prompts))
+        a.history_tokens, a.penalised = history.tokens.shape[0], 1
+        if drafted is not None:
+            a.ancestors, a.token_ids, a.cu_seqlens, a.nodes = (t.data_ptr() for t in (drafted.tree.ancestors, drafted.token_ids, drafted.cu_seqlens,
+                                                                                      drafted.rows))
+            a.words, a.tokens = drafted.tree.ancestors.shape[1], drafted.tree.ancestors.shape[0]
+    if bias is not None:
+        a.bias_ids, a.bias_values, a.bias_starts, a.bias_count = bias.ids.data_ptr(), bias.values.data_ptr(), bias.starts.data_ptr(), bias.ids.shape[0]
+    if masks is not None:
+        a.mask_words, a.mask_rows = masks.words.data_ptr(), masks.rows.data_ptr()
+        a.masks, a.mask_width = masks.words.shape
+    fn = _function("logits", "omnia_adjust_logits", [c_void_p, c_int, c_void_p])
+    _check(fn(ctypes.addressof(a), int(same), _stream()), what)
     return out
 
 

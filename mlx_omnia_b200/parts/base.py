@@ -319,6 +319,17 @@ class KVView:
         heads, width = rows[index]
         return self.pages[:, start: start + heads * width * self.page_size].view(-1, heads, self.page_size, width)
 
+@dataclass(frozen=True)
+class StepTree:
+    """Of a step whose requests bring trees of drafted tokens: what each of them sees of its request's, itself too.
+
+    ancestors: int32 [tokens, words]; bit m of row t (the lowest bit of word 0 first): the row's token sees the m-th token that its
+               request brings to the step. At most 32 * words tokens a request, and 256.
+    """
+
+    ancestors: torch.Tensor
+
+
 @dataclass
 class StepContext:
     """The batch of one step: tokens of several requests, flattened.
@@ -352,6 +363,9 @@ class StepContext:
     # of what a request holds beyond its shared positions. None: from `shared` and `seq_lens_host`.
     shared_shape: "tuple[tuple[int, int], ...] | None" = None
     max_own: int | None = None
+    # Requests bring trees of drafted tokens (`positions` are then those in the tree, where tokens are stored is the order in which they are
+    # brought); a request that brings a plain run of tokens has the tree of a chain.
+    tree: StepTree | None = None
 
 
 @dataclass
