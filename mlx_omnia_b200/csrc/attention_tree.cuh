@@ -56,3 +56,82 @@ __device__ __forceinline__ int tree_low(const TreeAttention& a, int pos) {
   if (a.run > 0) low = max(low, pos - pos % a.run);
   return low;
 }
+
+// Equal shares of a step's work for the kernels that keep a fixed number of blocks busy. An item is a tile of rows of one request and one key/value
+// head; its keys come in tiles. All tiles of all items stand in one line (requests, then heads, then tiles of rows, then of keys), of which block
+// b takes [b T / G, (b + 1) T / G): contexts of unequal lengths cost no block more than another, and since lengths are read here, a captured
+// step has its shares right at every replay. An item that several blocks have part in is put together by the merge: block b leaves
+// what its first item came to in slot 2 b, and what its last one did in slot 2 b + 1.
+constexpr int TREE_MOST_REQUESTS = 1024;
+
+struct TreeShares {
+  int rows, keys;  // of a tile
+  __device__ __forceinline__ int row_tiles(const TreeAttention& a, const TreeKeys& k) const {
+    return k.total > 0 ? (k.count * (a.nq / a.nkv) + rows - 1) / rows : 0;
+  }
+  __device__ __forceinline__ int key_tiles(const TreeKeys& k) const { return (k.total + keys - 1) / keys; }
+
+  // ends[r]: tiles of all requests up to r, r among them (shared memory, of the whole block); -> tiles in all. `sums`: a word a warp.
+  __device__ __forceinline__ long long lay_out(const TreeAttention& a, long long* ends, long long* sums) const {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    long long before = 0;
+    for (int r0 = 0; r0 < a.requests; r0 += blockDim.x) {
+      const int r = r0 + threadIdx.x;
+      long long mine = 0;
+      if (r < a.requests) {
+        const TreeKeys k = tree_keys(a, r);
+        mine = (long long)row_tiles(a, k) * key_tiles(k) * a.nkv;
+      }
+#pragma unroll
+      for (int o = 1; o < 32; o *= 2) {
+        const long long other = __shfl_up_sync(0xffffffffu, mine, o);
+        if (lane >= o) mine += other;
+      }
+      if (lane == 31) sums[warp] = mine;
+      __syncthreads();
+      long long ahead = before;
+      for (int w = 0; w < warps; ++w) {
+        if (w < warp) ahead += sums[w];
+        before += sums[w];
+      }
+      if (r < a.requests) ends[r] = ahead + mine;
+      __syncthreads();
+    }
+    return before;
+  }
+};
+
+// A place in that line.
+struct TreePlace {
+  int request, head, row_tile, tile, row_tiles, tiles;
+  TreeKeys k;
+  __device__ __forceinline__ void enter(const TreeAttention& a, const TreeShares& s, int r) {
+    request = r;
+    k = tree_keys(a, r);
+    row_tiles = s.row_tiles(a, k), tiles = s.key_tiles(k);
+  }
+  __device__ __forceinline__ void find(const TreeAttention& a, const TreeShares& s, const long long* ends, long long at) {
+    int lo = 0, hi = a.requests - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (ends[mid] > at) hi = mid; else lo = mid + 1;
+    }
+    enter(a, s, lo);
+    const long long in = at - (lo ? ends[lo - 1] : 0);
+    const int each = row_tiles * tiles;
+    head = (int)(in / each);
+    const int rest = (int)(in % each);
+    row_tile = rest / tiles, tile = rest % tiles;
+  }
+  // To the next tile, which there is.
+  __device__ __forceinline__ void next(const TreeAttention& a, const TreeShares& s) {
+    if (++tile < tiles) return;
+    tile = 0;
+    if (++row_tile < row_tiles) return;
+    row_tile = 0;
+    if (++head < a.nkv) return;
+    head = 0;
+    do enter(a, s, request + 1);
+    while (row_tiles * tiles == 0 && request + 1 < a.requests);
+  }
+};

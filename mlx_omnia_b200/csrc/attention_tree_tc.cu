@@ -1,0 +1,461 @@
+// Attention of trees of drafted tokens in bfloat16 on the tensor cores (mma.sync m16n8k16, float32 sums and softmax), for requests that bring few rows.
+// Compiled for one head size:
+//   -DHEAD_DIM=d   (a multiple of 8, at most 256; rows are zero-padded to a multiple of 16; keys and values of equal width)
+//
+// Rows of a tile are (node, query head of the group) pairs of one request and key/value head, 16, 32 or 64 of them; four warps share a
+// tile of 64 keys, each with sixteen of the rows and all, half or a quarter of the keys, with a softmax state of its own; the states are brought
+// together when an item ends. Keys and values come by cp.async, row by row through the block table, so any page size works, three tiles deep, and
+// the loads run on across the items of a block's share (TreeShares).
+//
+// What a row does not see has no weight, whatever it holds: scores are replaced before the softmax, and where a tile has something that only some
+// rows see (nodes, the edge of a window) its values are looked through for ones that are no numbers, and if there are any, summed by hand.
+#include "attention_tree.cuh"
+
+#ifndef HEAD_DIM
+#define HEAD_DIM 128
+#endif
+
+namespace {
+
+typedef __nv_bfloat16 bf16;
+
+constexpr int D = HEAD_DIM;
+static_assert(D % 8 == 0 && D >= 8 && D <= 256, "head size must be a multiple of 8, at most 256");
+constexpr int DP = (D + 15) / 16 * 16, ROW = DP + 8;  // padded head size; shared-memory row stride (elements): odd in 16-byte units
+constexpr int CH = D / 8, KSTEPS = DP / 16, NT_O = DP / 8;
+constexpr int KEYS = 64, WARPS = 4, THREADS = 32 * WARPS, WARP_LOADS = KEYS / WARPS;  // keys whose rows a warp fetches
+constexpr int STAGES = D <= 128 ? 3 : 2;
+constexpr int STAGE = 2 * KEYS * ROW;                 // elements: keys, then values
+constexpr float LOG2E = 1.4426950408889634f;
+
+__device__ __forceinline__ void cp_async16(void* smem, const void* gmem, bool valid) {
+  const unsigned s = (unsigned)__cvta_generic_to_shared(smem);
+  const int bytes = valid ? 16 : 0;  // 0 source bytes: the 16 destination bytes are zero-filled
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(s), "l"(gmem), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldmatrix_x4(unsigned* r, const bf16* p) {
+  const unsigned s = (unsigned)__cvta_generic_to_shared(p);
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(s) : "memory");
+}
+__device__ __forceinline__ void ldmatrix_x4_trans(unsigned* r, const bf16* p) {
+  const unsigned s = (unsigned)__cvta_generic_to_shared(p);
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];\n" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(s) : "memory");
+}
+__device__ __forceinline__ void mma_bf16(float* c, const unsigned* a, unsigned b0, unsigned b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float fast_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float fast_rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ unsigned pack(float lo, float hi) {
+  __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<unsigned*>(&v);
+}
+__device__ __forceinline__ long long shfl64(long long v, int lane) { return __shfl_sync(0xffffffffu, v, lane); }
+
+}  // namespace
+
+// WR: warps side by side over the rows (a tile has 16 WR); the others share the keys.
+template <int WR>
+__global__ void __launch_bounds__(THREADS, D <= 128 ? 2 : 1) tree_shares_kernel(const __grid_constant__ TreeAttention a) {
+  constexpr int WK = WARPS / WR, KW = KEYS / WK, NT_S = KW / 8, ROWS = 16 * WR, HALF = NT_O > 8 ? (NT_O + 1) / 2 : NT_O;
+  extern __shared__ __align__(16) unsigned char raw[];
+  bf16* stages = reinterpret_cast<bf16*>(raw);
+  float* spare = reinterpret_cast<float*>(stages + STAGES * STAGE);  // [WR][16][8 HALF + 4], one warp's sums on their way to another
+  constexpr int SPARE = 8 * HALF + 4;
+  float* spare_ml = spare + WR * 16 * SPARE;                         // [WR][16][2]
+  __shared__ long long sums[WARPS];
+  long long* ends = reinterpret_cast<long long*>(raw);               // (where the stages are to be)
+  static_assert(STAGES * STAGE * sizeof(bf16) >= TREE_MOST_REQUESTS * sizeof(long long), "the requests' ends lie in the stages");
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, wr = warp % WR, wk = warp / WR, g = lane >> 2, t4 = lane & 3;
+  pdl_wait();
+  pdl_launch_dependents();
+  const TreeShares shares = {ROWS, KEYS};
+  const long long total = shares.lay_out(a, ends, sums);
+  const long long blocks = min((long long)gridDim.x, total);  // (a block more than there are tiles would leave its slots unwritten)
+  if (blockIdx.x >= blocks) return;
+  const long long t0 = total * blockIdx.x / blocks, t1 = total * (blockIdx.x + 1) / blocks;
+  const int group = a.nq / a.nkv;
+  const bf16 *kp = static_cast<const bf16*>(a.k_pages), *vp = static_cast<const bf16*>(a.v_pages);
+
+  // ---- loads: lane l < 16 knows where the l-th row of its warp's share of a tile lies ------------------------------------------------
+  TreePlace ahead;
+  ahead.find(a, shares, ends, t0);
+  TreePlace now = ahead;
+  __syncthreads();
+  if constexpr (D != DP) {  // the columns beyond a row: no load writes them
+    for (int i = tid; i < STAGES * 2 * KEYS; i += THREADS) *reinterpret_cast<uint4*>(stages + i * ROW + D) = make_uint4(0u, 0u, 0u, 0u);
+  }
+  long long loaded = t0;  // tiles asked for
+  auto where = [&]() -> long long {  // of this lane's key of the place `ahead`: elements from the pages' beginning; -1: none
+    const int x = ahead.tile * KEYS + warp * WARP_LOADS + lane;
+    if (lane >= WARP_LOADS || x >= ahead.k.total) return -1;
+    const int key = ahead.k.key(x), at = key / a.page_size;
+    const int page = at < a.max_pages ? a.block_table[(size_t)ahead.request * a.max_pages + at] : -1;
+    if (page < 0 || page >= a.num_pages) {
+      atomicOr(a.err, OMNIA_ERR_PAGE);
+      return -1;
+    }
+    return page * a.page_stride + (long long)(ahead.head * a.page_size + key % a.page_size) * D;
+  };
+  long long row_at = where();
+  auto fetch = [&]() {  // the tile at `ahead`, into the next stage; then on
+    if (loaded < t1) {
+      bf16* k_s = stages + (loaded - t0) % STAGES * STAGE + warp * WARP_LOADS * ROW;
+      bf16* v_s = k_s + KEYS * ROW;
+      constexpr int PIECES = WARP_LOADS * CH;
+#pragma unroll
+      for (int i0 = 0; i0 < PIECES; i0 += 32) {
+        const int i = i0 + lane, row = min(i / CH, WARP_LOADS - 1), c = i % CH;
+        const long long from = shfl64(row_at, row);
+        if (PIECES % 32 == 0 || i < PIECES) {
+          cp_async16(k_s + row * ROW + c * 8, kp + (from < 0 ? 0 : from) + c * 8, from >= 0);
+          cp_async16(v_s + row * ROW + c * 8, vp + (from < 0 ? 0 : from) + c * 8, from >= 0);
+        }
+      }
+      if (++loaded < t1) {
+        ahead.next(a, shares);
+        row_at = where();
+      }
+    }
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int s = 0; s < STAGES - 1; ++s) fetch();
+
+  const bool capped = a.softcap > 0.f;
+  const float cap = a.softcap * LOG2E, twice = capped ? 2.f * a.scale / a.softcap * LOG2E : 0.f, unit = a.scale * LOG2E;
+  unsigned qf[KSTEPS][4];
+  float o[NT_O][4], m[2], l[2];
+  int node[2], low[2];
+  bool first = true, entered = true;
+  for (long long t = t0; t < t1; ++t) {
+    const int rows = now.k.count * group, row0 = now.row_tile * ROWS + 16 * wr;
+    if (entered) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int row = row0 + g + 8 * h;
+        node[h] = row < rows ? row / group : -1;
+        low[h] = node[h] >= 0 ? tree_low(a, a.positions[now.k.first + node[h]]) : 0;
+        m[h] = -INFINITY, l[h] = 0.f;
+        const bf16* q = static_cast<const bf16*>(a.q) + ((size_t)(now.k.first + max(node[h], 0)) * a.nq + now.head * group + row % group) * D;
+#pragma unroll
+        for (int s = 0; s < KSTEPS; ++s) {
+          const int c = 16 * s + 2 * t4;
+          qf[s][h] = node[h] >= 0 && c < D ? *reinterpret_cast<const unsigned*>(q + c) : 0u;
+          qf[s][h + 2] = node[h] >= 0 && c + 8 < D ? *reinterpret_cast<const unsigned*>(q + c + 8) : 0u;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < NT_O; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+      entered = false;
+    }
+    cp_async_wait<STAGES - 2>();
+    __syncthreads();
+    fetch();
+    const bf16* k_s = stages + (t - t0) % STAGES * STAGE + wk * KW * ROW;
+    const bf16* v_s = k_s + KEYS * ROW;
+    float s[NT_S][4];
+#pragma unroll
+    for (int i = 0; i < NT_S; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < KSTEPS; ++ks)
+#pragma unroll
+      for (int i = 0; i < NT_S; i += 2) {
+        unsigned b[4];
+        ldmatrix_x4(b, k_s + (i * 8 + (lane & 7) + ((lane >> 4) << 3)) * ROW + ks * 16 + ((lane >> 3) & 1) * 8);
+        mma_bf16(s[i], qf[ks], b[0], b[1]);
+        mma_bf16(s[i + 1], qf[ks], b[2], b[3]);
+      }
+    // Scores in log2 units (a capped one that is infinite has the cap, of its sign: c tanh(x) = c - 2 c / (1 + e^2x)).
+    const int x0 = now.tile * KEYS + wk * KW;
+#pragma unroll
+    for (int i = 0; i < NT_S; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[i][j] = capped ? fmaf(-2.f * cap, fast_rcp(1.f + fast_exp2(s[i][j] * twice)), cap) : s[i][j] * unit;
+    // Whether every row sees every key of these.
+    const int last_key = now.k.key(min(x0 + KW, now.k.total) - 1);
+    const bool clear = x0 + KW <= now.k.total && last_key < now.k.held && x0 >= now.k.kept &&
+                       now.k.key(x0) >= tree_low(a, now.k.held + now.k.count - 1);
+    if (!clear) {
+#pragma unroll
+      for (int i = 0; i < NT_S; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int x = x0 + 8 * i + 2 * t4 + j;
+          int pos = 0, which = -1;
+          const bool real = x < now.k.total;
+          if (real) {
+            pos = now.k.key(x);
+            if (pos >= now.k.held) which = pos - now.k.held, pos = a.positions[now.k.first + which];
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            bool seen = real && node[h] >= 0 && (pos >= low[h] || (a.window > 0 && pos < a.keep));
+            if (seen && which >= 0)
+              seen = ((unsigned)a.ancestors[(size_t)(now.k.first + node[h]) * a.words + (which >> 5)] >> (which & 31)) & 1u;
+            if (!seen) s[i][2 * h + j] = -INFINITY;
+          }
+        }
+    }
+    unsigned pf[NT_S / 2][4];
+    float p[NT_S][4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float top = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < NT_S; ++i) top = fmaxf(top, fmaxf(s[i][2 * h], s[i][2 * h + 1]));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const float over = fmaxf(m[h], top), base = over == -INFINITY ? 0.f : over, f = fast_exp2(m[h] - base);
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < NT_S; ++i) {
+        p[i][2 * h] = fast_exp2(s[i][2 * h] - base), p[i][2 * h + 1] = fast_exp2(s[i][2 * h + 1] - base);
+        sum += p[i][2 * h] + p[i][2 * h + 1];
+      }
+      l[h] = l[h] * f + sum;  // (of this lane's keys)
+      m[h] = over;
+      if (f != 1.f) {
+#pragma unroll
+        for (int i = 0; i < NT_O; ++i) o[i][2 * h] *= f, o[i][2 * h + 1] *= f;
+      }
+      // Weights are rounded to bfloat16 for their product with the values, the sum is of what was not.
+#pragma unroll
+      for (int i = 0; i < NT_S; i += 2) {
+        pf[i / 2][h] = pack(p[i][2 * h], p[i][2 * h + 1]);
+        pf[i / 2][h + 2] = pack(p[i + 1][2 * h], p[i + 1][2 * h + 1]);
+      }
+    }
+    bool odd = false;
+    if (!clear) {
+#pragma unroll 1
+      for (int i = lane; i < KW * CH; i += 32) {
+        const uint4 v = *reinterpret_cast<const uint4*>(v_s + i / CH * ROW + i % CH * 8);
+        for (unsigned w : {v.x, v.y, v.z, v.w}) odd |= (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
+      }
+      odd = __any_sync(0xffffffffu, odd);
+    }
+    if (odd) {
+#pragma unroll
+      for (int i = 0; i < NT_S; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {  // the key that the lane c of a row has at i, j
+            const float p0 = __shfl_sync(0xffffffffu, p[i][j], (lane & ~3) | c), p1 = __shfl_sync(0xffffffffu, p[i][2 + j], (lane & ~3) | c);
+            const bf16* v = v_s + (8 * i + 2 * c + j) * ROW;
+#pragma unroll
+            for (int n = 0; n < NT_O; ++n) {
+              const float v0 = __bfloat162float(v[8 * n + 2 * t4]), v1 = __bfloat162float(v[8 * n + 2 * t4 + 1]);
+              if (p0 != 0.f) o[n][0] = fmaf(p0, v0, o[n][0]), o[n][1] = fmaf(p0, v1, o[n][1]);
+              if (p1 != 0.f) o[n][2] = fmaf(p1, v0, o[n][2]), o[n][3] = fmaf(p1, v1, o[n][3]);
+            }
+          }
+    } else {
+#pragma unroll
+      for (int ks = 0; ks < NT_S / 2; ++ks)
+#pragma unroll
+        for (int n = 0; n < NT_O; n += 2) {
+          unsigned b[4];
+          ldmatrix_x4_trans(b, v_s + (ks * 16 + (lane & 15)) * ROW + n * 8 + ((lane >> 4) << 3));
+          mma_bf16(o[n], pf[ks], b[0], b[1]);
+          mma_bf16(o[n + 1], pf[ks], b[2], b[3]);
+        }
+    }
+    if (now.tile + 1 < now.tiles && t + 1 < t1) {
+      ++now.tile;
+      continue;
+    }
+    // ---- the item's end in this block: the warps that shared the keys, then the slot or the answer ------------------------------------
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+    }
+#pragma unroll 1
+    for (int giver = WK - 1; giver > 0; --giver) {
+      float mine[2], other[2];
+#pragma unroll
+      for (int n0 = 0; n0 < NT_O; n0 += HALF) {
+        if (wk == giver) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float* to = spare + (wr * 16 + g + 8 * h) * SPARE;
+#pragma unroll
+            for (int n = 0; n < HALF; ++n)
+              if (n0 + n < NT_O) *reinterpret_cast<float2*>(to + 8 * n + 2 * t4) = make_float2(o[n0 + n][2 * h], o[n0 + n][2 * h + 1]);
+            if (n0 == 0 && t4 == 0) spare_ml[(wr * 16 + g + 8 * h) * 2] = m[h], spare_ml[(wr * 16 + g + 8 * h) * 2 + 1] = l[h];
+          }
+        }
+        __syncthreads();
+        if (wk == giver - 1) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float* from = spare + (wr * 16 + g + 8 * h) * SPARE;
+            if (n0 == 0) {
+              const float om = spare_ml[(wr * 16 + g + 8 * h) * 2], ol = spare_ml[(wr * 16 + g + 8 * h) * 2 + 1];
+              const float over = fmaxf(m[h], om), base = over == -INFINITY ? 0.f : over;
+              mine[h] = fast_exp2(m[h] - base), other[h] = fast_exp2(om - base);
+              l[h] = l[h] * mine[h] + ol * other[h];
+              m[h] = over;
+            }
+#pragma unroll
+            for (int n = 0; n < HALF; ++n)
+              if (n0 + n < NT_O) {
+                const float2 v = *reinterpret_cast<const float2*>(from + 8 * n + 2 * t4);
+                o[n0 + n][2 * h] = o[n0 + n][2 * h] * mine[h] + (other[h] != 0.f ? v.x * other[h] : 0.f);
+                o[n0 + n][2 * h + 1] = o[n0 + n][2 * h + 1] * mine[h] + (other[h] != 0.f ? v.y * other[h] : 0.f);
+              }
+          }
+        }
+        __syncthreads();
+      }
+    }
+    if (wk == 0) {
+      // The whole item is this block's where it begins and ends here.
+      const bool begins = !first || t - t0 >= now.tile, whole = begins && now.tile + 1 == now.tiles;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (!whole) {
+          const size_t slot = 2 * (size_t)blockIdx.x + (first ? 0 : 1), row = slot * ROWS + 16 * wr + g + 8 * h;
+          if (t4 == 0) a.part_ml[2 * row] = m[h], a.part_ml[2 * row + 1] = l[h];
+#pragma unroll
+          for (int n = 0; n < NT_O; ++n)
+            if (8 * n < D) *reinterpret_cast<float2*>(a.part_o + row * D + 8 * n + 2 * t4) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
+          continue;
+        }
+        if (node[h] < 0) continue;
+        const int token = now.k.first + node[h], head = now.head * group + (row0 + g + 8 * h) % group;
+        float over = l[h], f = 1.f;
+        if (a.sink) {
+          const float z = a.sink[head] * LOG2E, base = fmaxf(m[h], z);
+          f = fast_exp2(m[h] - base), over = l[h] * f + fast_exp2(z - base);
+        }
+        const float by = over > 0.f ? f / over : 0.f;
+        bf16* out = static_cast<bf16*>(a.out) + (size_t)token * a.nq * D + head * D;
+        const bf16* gate = a.gate ? static_cast<const bf16*>(a.gate) + (size_t)token * a.gate_stride + head * D : nullptr;
+#pragma unroll
+        for (int n = 0; n < NT_O; ++n)
+          if (8 * n < D) {
+            float y0 = o[n][2 * h] * by, y1 = o[n][2 * h + 1] * by;
+            if (by == 0.f) y0 = y1 = 0.f;
+            if (gate) {
+              y0 *= 1.f / (1.f + __expf(-__bfloat162float(gate[8 * n + 2 * t4])));
+              y1 *= 1.f / (1.f + __expf(-__bfloat162float(gate[8 * n + 2 * t4 + 1])));
+            }
+            *reinterpret_cast<unsigned*>(out + 8 * n + 2 * t4) = pack(y0, y1);
+          }
+      }
+    }
+    first = false, entered = true;
+    if (t + 1 < t1) now.next(a, shares);
+  }
+}
+
+// A block an item (a warp four of its rows in turn): the slots of the blocks that had part in it, in their order, the sink, the gate. A request
+// that sees nothing has zeros.
+__global__ void __launch_bounds__(THREADS) tree_join_kernel(const __grid_constant__ TreeAttention a, int rows_of_tile, int grid) {
+  __shared__ long long ends[TREE_MOST_REQUESTS], sums[WARPS];
+  pdl_wait();
+  pdl_launch_dependents();
+  const TreeShares shares = {rows_of_tile, KEYS};
+  const long long total = shares.lay_out(a, ends, sums);
+  const long long blocks = min((long long)grid, total);
+  const int request = blockIdx.z, head_kv = blockIdx.y, row_tile = blockIdx.x, group = a.nq / a.nkv;
+  const TreeKeys k = tree_keys(a, request);
+  const int tiles = shares.key_tiles(k), row_tiles = shares.row_tiles(a, k), here = min(rows_of_tile, k.count * group - row_tile * rows_of_tile);
+  if (row_tile == 0 && head_kv == 0 && threadIdx.x == 0 && row_tiles > (int)gridDim.x) atomicOr(a.err, OMNIA_ERR_WORK);
+  if (here <= 0) return;
+  const long long begin = (request ? ends[request - 1] : 0) + ((long long)head_kv * row_tiles + row_tile) * tiles, end = begin + tiles;
+  // Tile t is block b's where b T / G <= t < (b + 1) T / G.
+  auto block_of = [&](long long t) { return (int)(((t + 1) * blocks - 1) / total); };
+  const int b0 = tiles ? block_of(begin) : 0, b1 = tiles ? block_of(end - 1) : -1;
+  if (tiles && b0 == b1) return;
+  auto slot_of = [&](int b) { return 2 * (size_t)b + (begin <= total * b / blocks ? 0 : 1); };
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int r = warp; r < here; r += WARPS) {
+    const int row = row_tile * rows_of_tile + r, token = k.first + row / group, head = head_kv * group + row % group;
+    float base = a.sink ? a.sink[head] * LOG2E : -INFINITY;
+    for (int b = b0 + lane; b <= b1; b += 32) base = fmaxf(base, a.part_ml[2 * (slot_of(b) * rows_of_tile + r)]);
+    base = warp_max(base);
+    if (base == -INFINITY) base = 0.f;
+    float l = a.sink ? fast_exp2(a.sink[head] * LOG2E - base) : 0.f;
+    float sum[(D + 31) / 32];
+#pragma unroll
+    for (int i = 0; i < (D + 31) / 32; ++i) sum[i] = 0.f;
+    for (int b = b0; b <= b1; ++b) {
+      const size_t at = slot_of(b) * rows_of_tile + r;
+      const float w = fast_exp2(a.part_ml[2 * at] - base);
+      l += a.part_ml[2 * at + 1] * w;
+      if (w == 0.f) continue;
+#pragma unroll
+      for (int i = 0; i < (D + 31) / 32; ++i)
+        if (D % 32 == 0 || 32 * i + lane < D) sum[i] = fmaf(a.part_o[at * D + 32 * i + lane], w, sum[i]);
+    }
+    const float by = l > 0.f ? 1.f / l : 0.f;
+#pragma unroll
+    for (int i = 0; i < (D + 31) / 32; ++i) {
+      const int c = 32 * i + lane;
+      if (D % 32 != 0 && c >= D) continue;
+      float y = by == 0.f ? 0.f : sum[i] * by;
+      if (a.gate) y *= 1.f / (1.f + __expf(-__bfloat162float(static_cast<const bf16*>(a.gate)[(size_t)token * a.gate_stride + head * D + c])));
+      static_cast<bf16*>(a.out)[(size_t)token * a.nq * D + head * D + c] = __float2bfloat16_rn(y);
+    }
+  }
+}
+
+namespace {
+
+template <int WR>
+int launch(const TreeAttention& a, int blocks, cudaStream_t stream) {
+  constexpr int HALF = NT_O > 8 ? (NT_O + 1) / 2 : NT_O;
+  constexpr int bytes = STAGES * STAGE * 2 + (WR < WARPS ? WR * 16 * (8 * HALF + 4 + 2) * 4 : 0);
+  static bool ready[64] = {};
+  int device = 0;
+  cudaGetDevice(&device);
+  if (device < 0 || device >= 64) return (int)cudaErrorInvalidDevice;
+  if (!ready[device]) {
+    const cudaError_t e = cudaFuncSetAttribute(tree_shares_kernel<WR>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) return (int)e;
+    ready[device] = true;
+  }
+  launch_pdl(tree_shares_kernel<WR>, dim3(blocks), dim3(THREADS), bytes, stream, a);
+  return OMNIA_LAUNCH_RESULT();
+}
+
+}  // namespace
+
+// `rows`: of a tile, 16, 32 or 64; `blocks`: what the work is shared out over, with two slots of rows each in part_o and part_ml.
+extern "C" int omnia_tree_attention_tc(const TreeAttention* a, int most_nodes, int rows, int blocks, void* stream) {
+  if (a->d != D || a->dv != D || a->requests < 1 || a->requests > TREE_MOST_REQUESTS || a->nkv < 1 || a->nkv > 65535 || a->nq % a->nkv || blocks < 1 ||
+      most_nodes < 1)
+    return (int)cudaErrorInvalidValue;
+  const cudaStream_t s = (cudaStream_t)stream;
+  int code;
+  if (rows == 16) code = launch<1>(*a, blocks, s);
+  else if (rows == 32) code = launch<2>(*a, blocks, s);
+#if HEAD_DIM <= 128
+  else if (rows == 64) code = launch<4>(*a, blocks, s);
+#endif
+  else return (int)cudaErrorInvalidValue;
+  if (code) return code;
+  const dim3 grid((most_nodes * (a->nq / a->nkv) + rows - 1) / rows, a->nkv, a->requests);
+  launch_pdl(tree_join_kernel, grid, dim3(THREADS), 0, s, *a, rows, blocks);
+  return OMNIA_LAUNCH_RESULT();
+}

@@ -1495,9 +1495,18 @@ def tree_attention(q: torch.Tensor, kv: KVView, step: StepContext, scale: float,
                   table.data_ptr(), step.cu_seqlens.data_ptr(), step.seq_lens.data_ptr(), step.positions.data_ptr(), tree.ancestors.data_ptr(),
                   _ptr(sink), None, None, error_word(q.device).data_ptr(), page_stride, tokens, n, table.shape[1], pages.shape[0], nq, nkv, d, dv,
                   kv.page_size, 0 if gate is None else gate.stride(0), words, window, keep, run, 0, 0, scale, float(softcap or 0.0))
+    rows = step.max_q_len * (nq // nkv)
     # What the longest request can see: the plan is made for that, and from numbers that a captured step knows too.
     keys = min(max(step.max_seq_len, 1), window + keep + step.max_q_len if window else 1 << 30, run + step.max_q_len if run else 1 << 30)
-    tiles = -(-step.max_q_len * (nq // nkv) // 32) * n * nkv
+    if dv == d and q.dtype == torch.bfloat16 and d % 8 == 0 and d <= 256 and n <= 1024 and not k_ptr & 15 and not a.q & 3:
+        tile = 16 if rows <= 16 else 32 if rows <= 32 or d > 128 else 64
+        blocks = min((2 if d <= 128 else 1) * sm_count(q.device), n * nkv * -(-rows // tile) * -(-keys // 64))
+        parts = torch.empty(2 * blocks * tile * (d + 2), dtype=torch.float32, device=q.device)
+        a.part_o, a.part_ml = parts.data_ptr(), parts.data_ptr() + 2 * blocks * tile * d * 4
+        fn = _function("attention_tree_tc", "omnia_tree_attention_tc", [c_void_p, c_int, c_int, c_int, c_void_p], {"HEAD_DIM": d})
+        _check(fn(ctypes.addressof(a), step.max_q_len, tile, blocks, _stream()), what)
+        return out
+    tiles = -(-rows // 32) * n * nkv
     a.chunk, a.parts = tree_plan(tiles, keys, 64, 2 * sm_count(q.device))
     if a.parts > 1:
         parts = torch.empty(a.parts * tokens * nq * (dv + 2), dtype=torch.float32, device=q.device)

@@ -339,13 +339,21 @@ def test_a_captured_step_takes_the_lengths_of_its_replay():
         check(c, d ** -0.5, call=lambda **_: out)
 
 
-def test_lengths_beyond_the_plan_are_an_error():
-    nq, nkv, d, dtype, page = LAYOUTS[0]
+@pytest.mark.parametrize("layout", [LAYOUTS[0], (8, 1, 128, F32, 16)], ids=str)
+def test_lengths_beyond_the_plan(layout):
+    """The kernel for any type works by a plan for so many positions, the one of the tensor cores by the lengths themselves; both by the most tokens."""
+    nq, nkv, d, dtype, page = layout
     c = make(nq, nkv, d, dtype, page, [(900, refs.tree(16, 1))])
     c.step.max_seq_len = 300
+    if dtype == BF16:
+        check(c, d ** -0.5)
+    else:
+        ops.paged_attention(c.q, c.kv, c.step, d ** -0.5)
+        assert error_of(16)
+    c.step.max_seq_len, c.step.max_q_len = 916, 3
     ops.paged_attention(c.q, c.kv, c.step, d ** -0.5)
     assert error_of(16)
-    c.step.max_seq_len, c.step.seq_lens[0] = 916, 10  # fewer positions than tokens
+    c.step.max_q_len, c.step.seq_lens[0] = 16, 10  # fewer positions than tokens
     ops.paged_attention(c.q, c.kv, c.step, d ** -0.5)
     assert error_of(16)
     c = make(nq, nkv, d, dtype, page, [(900, refs.tree(16, 1))])
