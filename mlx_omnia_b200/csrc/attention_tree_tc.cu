@@ -27,6 +27,7 @@ constexpr int KEYS = 64, WARPS = 4, THREADS = 32 * WARPS, WARP_LOADS = KEYS / WA
 constexpr int STAGES = D <= 128 ? 3 : 2;
 constexpr int STAGE = 2 * KEYS * ROW;                 // elements: keys, then values
 constexpr float LOG2E = 1.4426950408889634f;
+constexpr float RESCALE_STEP = 8.f;  // log2 of how far a row's maximum may outgrow its exponent's offset
 
 __device__ __forceinline__ void cp_async16(void* smem, const void* gmem, bool valid) {
   const unsigned s = (unsigned)__cvta_generic_to_shared(smem);
@@ -92,6 +93,7 @@ __global__ void __launch_bounds__(THREADS, D <= 128 ? 2 : 1) tree_shares_kernel(
   const long long t0 = total * blockIdx.x / blocks, t1 = total * (blockIdx.x + 1) / blocks;
   const int group = a.nq / a.nkv;
   const bf16 *kp = static_cast<const bf16*>(a.k_pages), *vp = static_cast<const bf16*>(a.v_pages);
+  const long long apart = vp - kp;
 
   // ---- loads: lane l < 16 knows where the l-th row of its warp's share of a tile lies ------------------------------------------------
   TreePlace ahead;
@@ -101,7 +103,8 @@ __global__ void __launch_bounds__(THREADS, D <= 128 ? 2 : 1) tree_shares_kernel(
   if constexpr (D != DP) {  // the columns beyond a row: no load writes them
     for (int i = tid; i < STAGES * 2 * KEYS; i += THREADS) *reinterpret_cast<uint4*>(stages + i * ROW + D) = make_uint4(0u, 0u, 0u, 0u);
   }
-  long long loaded = t0;  // tiles asked for
+  const int share = (int)(t1 - t0);
+  int loaded = 0, load_stage = 0;  // tiles asked for
   auto where = [&]() -> long long {  // of this lane's key of the place `ahead`: elements from the pages' beginning; -1: none
     const int x = ahead.tile * KEYS + warp * WARP_LOADS + lane;
     if (lane >= WARP_LOADS || x >= ahead.k.total) return -1;
@@ -115,8 +118,9 @@ __global__ void __launch_bounds__(THREADS, D <= 128 ? 2 : 1) tree_shares_kernel(
   };
   long long row_at = where();
   auto fetch = [&]() {  // the tile at `ahead`, into the next stage; then on
-    if (loaded < t1) {
-      bf16* k_s = stages + (loaded - t0) % STAGES * STAGE + warp * WARP_LOADS * ROW;
+    if (loaded < share) {
+      bf16* k_s = stages + load_stage * STAGE + warp * WARP_LOADS * ROW;
+      if (++load_stage == STAGES) load_stage = 0;
       bf16* v_s = k_s + KEYS * ROW;
       constexpr int PIECES = WARP_LOADS * CH;
 #pragma unroll
@@ -124,11 +128,12 @@ __global__ void __launch_bounds__(THREADS, D <= 128 ? 2 : 1) tree_shares_kernel(
         const int i = i0 + lane, row = min(i / CH, WARP_LOADS - 1), c = i % CH;
         const long long from = shfl64(row_at, row);
         if (PIECES % 32 == 0 || i < PIECES) {
-          cp_async16(k_s + row * ROW + c * 8, kp + (from < 0 ? 0 : from) + c * 8, from >= 0);
-          cp_async16(v_s + row * ROW + c * 8, vp + (from < 0 ? 0 : from) + c * 8, from >= 0);
+          const bf16* at = kp + (from < 0 ? 0 : from) + c * 8;
+          cp_async16(k_s + row * ROW + c * 8, at, from >= 0);
+          cp_async16(v_s + row * ROW + c * 8, at + apart, from >= 0);
         }
       }
-      if (++loaded < t1) {
+      if (++loaded < share) {
         ahead.next(a, shares);
         row_at = where();
       }
@@ -139,12 +144,15 @@ __global__ void __launch_bounds__(THREADS, D <= 128 ? 2 : 1) tree_shares_kernel(
   for (int s = 0; s < STAGES - 1; ++s) fetch();
 
   const bool capped = a.softcap > 0.f;
-  const float cap = a.softcap * LOG2E, twice = capped ? 2.f * a.scale / a.softcap * LOG2E : 0.f, unit = a.scale * LOG2E;
+  // Scores keep the sign that they are compared by: a scale below zero turns the queries' signs instead.
+  const float size = fabsf(a.scale), cap = a.softcap * LOG2E, twice = capped ? 2.f * size / a.softcap * LOG2E : 0.f, unit = capped ? 1.f : size * LOG2E;
+  const unsigned turn = a.scale < 0.f ? 0x80008000u : 0u;
   unsigned qf[KSTEPS][4];
   float o[NT_O][4], m[2], l[2];
   int node[2], low[2];
   bool first = true, entered = true;
-  for (long long t = t0; t < t1; ++t) {
+  int stage = 0;
+  for (int t = 0; t < share; ++t) {
     const int rows = now.k.count * group, row0 = now.row_tile * ROWS + 16 * wr;
     if (entered) {
 #pragma unroll
@@ -157,8 +165,8 @@ __global__ void __launch_bounds__(THREADS, D <= 128 ? 2 : 1) tree_shares_kernel(
 #pragma unroll
         for (int s = 0; s < KSTEPS; ++s) {
           const int c = 16 * s + 2 * t4;
-          qf[s][h] = node[h] >= 0 && c < D ? *reinterpret_cast<const unsigned*>(q + c) : 0u;
-          qf[s][h + 2] = node[h] >= 0 && c + 8 < D ? *reinterpret_cast<const unsigned*>(q + c + 8) : 0u;
+          qf[s][h] = node[h] >= 0 && c < D ? *reinterpret_cast<const unsigned*>(q + c) ^ turn : 0u;
+          qf[s][h + 2] = node[h] >= 0 && c + 8 < D ? *reinterpret_cast<const unsigned*>(q + c + 8) ^ turn : 0u;
         }
       }
 #pragma unroll
@@ -168,7 +176,8 @@ __global__ void __launch_bounds__(THREADS, D <= 128 ? 2 : 1) tree_shares_kernel(
     cp_async_wait<STAGES - 2>();
     __syncthreads();
     fetch();
-    const bf16* k_s = stages + (t - t0) % STAGES * STAGE + wk * KW * ROW;
+    const bf16* k_s = stages + stage * STAGE + wk * KW * ROW;
+    if (++stage == STAGES) stage = 0;
     const bf16* v_s = k_s + KEYS * ROW;
     float s[NT_S][4];
 #pragma unroll
@@ -182,12 +191,13 @@ __global__ void __launch_bounds__(THREADS, D <= 128 ? 2 : 1) tree_shares_kernel(
         mma_bf16(s[i], qf[ks], b[0], b[1]);
         mma_bf16(s[i + 1], qf[ks], b[2], b[3]);
       }
-    // Scores in log2 units (a capped one that is infinite has the cap, of its sign: c tanh(x) = c - 2 c / (1 + e^2x)).
     const int x0 = now.tile * KEYS + wk * KW;
+    if (capped) {  // in log2 units (a score that is infinite has the cap, of its sign: c tanh(x) = c - 2 c / (1 + e^2x))
 #pragma unroll
-    for (int i = 0; i < NT_S; ++i)
+      for (int i = 0; i < NT_S; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) s[i][j] = capped ? fmaf(-2.f * cap, fast_rcp(1.f + fast_exp2(s[i][j] * twice)), cap) : s[i][j] * unit;
+        for (int j = 0; j < 4; ++j) s[i][j] = fmaf(-2.f * cap, fast_rcp(1.f + fast_exp2(s[i][j] * twice)), cap);
+    }
     // Whether every row sees every key of these.
     const int last_key = now.k.key(min(x0 + KW, now.k.total) - 1);
     const bool clear = x0 + KW <= now.k.total && last_key < now.k.held && x0 >= now.k.kept &&
@@ -222,19 +232,26 @@ __global__ void __launch_bounds__(THREADS, D <= 128 ? 2 : 1) tree_shares_kernel(
       for (int i = 0; i < NT_S; ++i) top = fmaxf(top, fmaxf(s[i][2 * h], s[i][2 * h + 1]));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const float over = fmaxf(m[h], top), base = over == -INFINITY ? 0.f : over, f = fast_exp2(m[h] - base);
+      top *= unit;
+      // The offset follows a row's maximum lazily: what was summed is brought to a new one only when the scores have outgrown the old.
+      if (top > m[h]) {
+        if (m[h] == -INFINITY) {
+          m[h] = top;  // (nothing was summed yet)
+        } else if (top - m[h] > RESCALE_STEP) {
+          const float f = fast_exp2(m[h] - top);
+          m[h] = top, l[h] *= f;
+#pragma unroll
+          for (int i = 0; i < NT_O; ++i) o[i][2 * h] *= f, o[i][2 * h + 1] *= f;
+        }
+      }
+      const float base = m[h] == -INFINITY ? 0.f : m[h];
       float sum = 0.f;
 #pragma unroll
       for (int i = 0; i < NT_S; ++i) {
-        p[i][2 * h] = fast_exp2(s[i][2 * h] - base), p[i][2 * h + 1] = fast_exp2(s[i][2 * h + 1] - base);
+        p[i][2 * h] = fast_exp2(fmaf(s[i][2 * h], unit, -base)), p[i][2 * h + 1] = fast_exp2(fmaf(s[i][2 * h + 1], unit, -base));
         sum += p[i][2 * h] + p[i][2 * h + 1];
       }
-      l[h] = l[h] * f + sum;  // (of this lane's keys)
-      m[h] = over;
-      if (f != 1.f) {
-#pragma unroll
-        for (int i = 0; i < NT_O; ++i) o[i][2 * h] *= f, o[i][2 * h + 1] *= f;
-      }
+      l[h] += sum;  // (of this lane's keys)
       // Weights are rounded to bfloat16 for their product with the values, the sum is of what was not.
 #pragma unroll
       for (int i = 0; i < NT_S; i += 2) {
@@ -278,7 +295,7 @@ __global__ void __launch_bounds__(THREADS, D <= 128 ? 2 : 1) tree_shares_kernel(
           mma_bf16(o[n + 1], pf[ks], b[2], b[3]);
         }
     }
-    if (now.tile + 1 < now.tiles && t + 1 < t1) {
+    if (now.tile + 1 < now.tiles && t + 1 < share) {
       ++now.tile;
       continue;
     }
@@ -329,7 +346,7 @@ __global__ void __launch_bounds__(THREADS, D <= 128 ? 2 : 1) tree_shares_kernel(
     }
     if (wk == 0) {
       // The whole item is this block's where it begins and ends here.
-      const bool begins = !first || t - t0 >= now.tile, whole = begins && now.tile + 1 == now.tiles;
+      const bool begins = !first || t >= now.tile, whole = begins && now.tile + 1 == now.tiles;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         if (!whole) {
@@ -364,59 +381,84 @@ __global__ void __launch_bounds__(THREADS, D <= 128 ? 2 : 1) tree_shares_kernel(
       }
     }
     first = false, entered = true;
-    if (t + 1 < t1) now.next(a, shares);
+    if (t + 1 < share) now.next(a, shares);
   }
 }
 
-// A block an item (a warp four of its rows in turn): the slots of the blocks that had part in it, in their order, the sink, the gate. A request
-// that sees nothing has zeros.
+// A warp a row of an item: the slots of the blocks that had part in it, in their order, the sink, the gate. A request that sees nothing
+// has zeros.
 __global__ void __launch_bounds__(THREADS) tree_join_kernel(const __grid_constant__ TreeAttention a, int rows_of_tile, int grid) {
   __shared__ long long ends[TREE_MOST_REQUESTS], sums[WARPS];
+  // (What is read ahead of the wait was there ahead of the kernel that this one waits for.)
+  const TreeShares shares = {rows_of_tile, KEYS};
+  const long long total = shares.lay_out(a, ends, sums), blocks = min((long long)grid, total);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int request = blockIdx.z, head_kv = blockIdx.y, group = a.nq / a.nkv, in = blockIdx.x * WARPS + warp, row_tile = in / rows_of_tile, r = in % rows_of_tile;
+  const TreeKeys k = tree_keys(a, request);
+  const int tiles = shares.key_tiles(k), row_tiles = shares.row_tiles(a, k);
+  if (blockIdx.x == 0 && head_kv == 0 && threadIdx.x == 0 && k.count * group > (int)gridDim.x * WARPS) atomicOr(a.err, OMNIA_ERR_WORK);
   pdl_wait();
   pdl_launch_dependents();
-  const TreeShares shares = {rows_of_tile, KEYS};
-  const long long total = shares.lay_out(a, ends, sums);
-  const long long blocks = min((long long)grid, total);
-  const int request = blockIdx.z, head_kv = blockIdx.y, row_tile = blockIdx.x, group = a.nq / a.nkv;
-  const TreeKeys k = tree_keys(a, request);
-  const int tiles = shares.key_tiles(k), row_tiles = shares.row_tiles(a, k), here = min(rows_of_tile, k.count * group - row_tile * rows_of_tile);
-  if (row_tile == 0 && head_kv == 0 && threadIdx.x == 0 && row_tiles > (int)gridDim.x) atomicOr(a.err, OMNIA_ERR_WORK);
-  if (here <= 0) return;
+  if (in >= k.count * group) return;
   const long long begin = (request ? ends[request - 1] : 0) + ((long long)head_kv * row_tiles + row_tile) * tiles, end = begin + tiles;
   // Tile t is block b's where b T / G <= t < (b + 1) T / G.
   auto block_of = [&](long long t) { return (int)(((t + 1) * blocks - 1) / total); };
   const int b0 = tiles ? block_of(begin) : 0, b1 = tiles ? block_of(end - 1) : -1;
   if (tiles && b0 == b1) return;
-  auto slot_of = [&](int b) { return 2 * (size_t)b + (begin <= total * b / blocks ? 0 : 1); };
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int r = warp; r < here; r += WARPS) {
-    const int row = row_tile * rows_of_tile + r, token = k.first + row / group, head = head_kv * group + row % group;
-    float base = a.sink ? a.sink[head] * LOG2E : -INFINITY;
-    for (int b = b0 + lane; b <= b1; b += 32) base = fmaxf(base, a.part_ml[2 * (slot_of(b) * rows_of_tile + r)]);
-    base = warp_max(base);
-    if (base == -INFINITY) base = 0.f;
-    float l = a.sink ? fast_exp2(a.sink[head] * LOG2E - base) : 0.f;
-    float sum[(D + 31) / 32];
+  // The item is the first of all blocks that have part in it but the one that it begins in, unless it begins that too.
+  const int slot0 = 2 * b0 + (tiles && begin <= total * b0 / blocks ? 0 : 1);
+  auto slot_of = [&](int b) { return b == b0 ? slot0 : 2 * b; };
+  const int token = k.first + in / group, head = head_kv * group + in % group;
+  const float sink = a.sink ? a.sink[head] * LOG2E : -INFINITY;
+  constexpr int PER = (D + 127) / 128;  // four dims a lane
+  float4 sum[PER];
 #pragma unroll
-    for (int i = 0; i < (D + 31) / 32; ++i) sum[i] = 0.f;
-    for (int b = b0; b <= b1; ++b) {
-      const size_t at = slot_of(b) * rows_of_tile + r;
-      const float w = fast_exp2(a.part_ml[2 * at] - base);
-      l += a.part_ml[2 * at + 1] * w;
-      if (w == 0.f) continue;
-#pragma unroll
-      for (int i = 0; i < (D + 31) / 32; ++i)
-        if (D % 32 == 0 || 32 * i + lane < D) sum[i] = fmaf(a.part_o[at * D + 32 * i + lane], w, sum[i]);
+  for (int i = 0; i < PER; ++i) sum[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  float base = -INFINITY, l = 0.f;
+  for (int c0 = b0; c0 <= b1; c0 += 32) {  // 32 slots at a time, a lane each for their offsets and sums
+    const int b = c0 + lane;
+    float ml = -INFINITY, ll = 0.f;
+    size_t row = 0;
+    if (b <= b1) {
+      row = (size_t)slot_of(b) * rows_of_tile + r;
+      const float2 x = reinterpret_cast<const float2*>(a.part_ml)[row];
+      ml = x.x, ll = x.y;
     }
-    const float by = l > 0.f ? 1.f / l : 0.f;
+    const float over = fmaxf(base, warp_max(ml)), offset = over == -INFINITY ? 0.f : over, f = fast_exp2(base - offset), w = fast_exp2(ml - offset);
+    l = l * f + warp_sum(ll * w);
 #pragma unroll
-    for (int i = 0; i < (D + 31) / 32; ++i) {
-      const int c = 32 * i + lane;
-      if (D % 32 != 0 && c >= D) continue;
-      float y = by == 0.f ? 0.f : sum[i] * by;
-      if (a.gate) y *= 1.f / (1.f + __expf(-__bfloat162float(static_cast<const bf16*>(a.gate)[(size_t)token * a.gate_stride + head * D + c])));
-      static_cast<bf16*>(a.out)[(size_t)token * a.nq * D + head * D + c] = __float2bfloat16_rn(y);
+    for (int i = 0; i < PER; ++i) sum[i].x *= f, sum[i].y *= f, sum[i].z *= f, sum[i].w *= f;
+    base = over;
+    const int here = min(32, b1 - c0 + 1);
+#pragma unroll 4
+    for (int p = 0; p < here; ++p) {
+      const float by = __shfl_sync(0xffffffffu, w, p);
+      const float* from = a.part_o + (size_t)((size_t)slot_of(c0 + p) * rows_of_tile + r) * D;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int c = (32 * i + lane) * 4;
+        if (c < D && by != 0.f) {
+          const float4 v = *reinterpret_cast<const float4*>(from + c);
+          sum[i].x = fmaf(v.x, by, sum[i].x), sum[i].y = fmaf(v.y, by, sum[i].y);
+          sum[i].z = fmaf(v.z, by, sum[i].z), sum[i].w = fmaf(v.w, by, sum[i].w);
+        }
+      }
     }
+  }
+  const float over = fmaxf(base, sink), offset = over == -INFINITY ? 0.f : over, f = fast_exp2(base - offset);
+  l = l * f + fast_exp2(sink - offset);
+  const float by = l > 0.f ? f / l : 0.f;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int c = (32 * i + lane) * 4;
+    if (c >= D) continue;
+    float y[4] = {sum[i].x * by, sum[i].y * by, sum[i].z * by, sum[i].w * by};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (by == 0.f) y[j] = 0.f;
+      if (a.gate) y[j] *= 1.f / (1.f + __expf(-__bfloat162float(static_cast<const bf16*>(a.gate)[(size_t)token * a.gate_stride + head * D + c + j])));
+    }
+    *reinterpret_cast<uint2*>(static_cast<bf16*>(a.out) + (size_t)token * a.nq * D + head * D + c) = make_uint2(pack(y[0], y[1]), pack(y[2], y[3]));
   }
 }
 
@@ -455,7 +497,7 @@ extern "C" int omnia_tree_attention_tc(const TreeAttention* a, int most_nodes, i
 #endif
   else return (int)cudaErrorInvalidValue;
   if (code) return code;
-  const dim3 grid((most_nodes * (a->nq / a->nkv) + rows - 1) / rows, a->nkv, a->requests);
+  const dim3 grid((most_nodes * (a->nq / a->nkv) + WARPS - 1) / WARPS, a->nkv, a->requests);
   launch_pdl(tree_join_kernel, grid, dim3(THREADS), 0, s, *a, rows, blocks);
   return OMNIA_LAUNCH_RESULT();
 }

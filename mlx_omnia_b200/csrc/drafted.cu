@@ -4,6 +4,9 @@
 //
 // A request's drafted tokens (its nodes) are numbered 0, 1, ... in the order they are brought; node 0 is known, each other one goes on from
 // an earlier one, its parent. What a node descends from, itself too, is a row of bits (its ancestors), `words` words of 32 bits.
+#include <stddef.h>
+#include <string.h>
+
 #include "common.cuh"
 
 namespace {
@@ -286,16 +289,20 @@ __global__ void __launch_bounds__(THREADS) keep_rows_kernel(const __grid_constan
 
 }  // namespace
 
-extern "C" int omnia_step_tables(const StepTables* a, void* stream) {
-  if (a->groups < 0 || a->groups > MOST_GROUPS || a->words < 0 || a->words > MOST_WORDS || a->requests < 1 || a->requests > 65534 || a->page_size < 1 ||
-      a->tokens < 0)
+// (What is given ends behind the last group.)
+extern "C" int omnia_step_tables(const void* given, void* stream) {
+  StepTables a = {};
+  memcpy(&a, given, offsetof(StepTables, group));
+  if (a.groups < 0 || a.groups > MOST_GROUPS || a.words < 0 || a.words > MOST_WORDS || a.requests < 1 || a.requests > 65534 || a.page_size < 1 ||
+      a.tokens < 0)
     return (int)cudaErrorInvalidValue;
-  int longest = a->tokens;
-  for (int g = 0; g < a->groups; ++g) longest = max(longest, a->group[g].width);
+  memcpy(a.group, static_cast<const char*>(given) + offsetof(StepTables, group), a.groups * sizeof(TableGroup));
+  int longest = a.tokens;
+  for (int g = 0; g < a.groups; ++g) longest = max(longest, a.group[g].width);
   // Blocks enough for the widest table or the longest request, and no more than fill the GPU.
-  const int wanted = (longest + 2 * THREADS - 1) / (2 * THREADS), room = 8 * omnia_sm_count() / (a->requests + 1);
+  const int wanted = (longest + 2 * THREADS - 1) / (2 * THREADS), room = 8 * omnia_sm_count() / (a.requests + 1);
   const int parts = max(1, min(wanted, room));
-  launch_pdl(step_tables_kernel, dim3(parts, a->requests + 1), dim3(THREADS), 0, (cudaStream_t)stream, *a);
+  launch_pdl(step_tables_kernel, dim3(parts, a.requests + 1), dim3(THREADS), 0, (cudaStream_t)stream, a);
   return OMNIA_LAUNCH_RESULT();
 }
 

@@ -15,6 +15,7 @@ import ctypes
 import functools
 import itertools
 import math
+import struct
 from ctypes import c_float, c_int, c_longlong, c_void_p
 
 import dataclasses
@@ -1273,24 +1274,58 @@ MOST_DRAFTED = 256
 """Tokens that a request brings to a step of drafted trees at most: eight words of bits, a thread each."""
 
 
-def _here(what: str, *tensors: "torch.Tensor | None") -> int:
-    """The index of the device that all of the tensors lie on, which has to be the current one (a launch goes to its stream)."""
-    index = torch.cuda.current_device()
-    for t in tensors:
-        if t is not None and (not t.is_cuda or t.get_device() != index):
-            raise KernelError(f"{what} takes tensors on the current CUDA device ({index}), not on {t.device}")
-    return index
+_entries: dict[str, ctypes._CFuncPtr] = {}
 
 
-def _flat(what: str, name: str, t: torch.Tensor, dtype: torch.dtype, *shape: "int | None") -> torch.Tensor:
-    """`t`, if it is contiguous, of this type and of this shape (None: any size)."""
-    if t.dtype != dtype or t.dim() != len(shape) or not t.is_contiguous() or any(n is not None and m != n for m, n in zip(t.shape, shape)):
-        raise KernelError(f"{what}: {name} is a contiguous {dtype} tensor of {[('any' if n is None else n) for n in shape]}, not {t.dtype} {list(t.shape)}")
-    return t
+def _entry(library: str, name: str, argtypes: list, defines: dict | None = None):
+    """`_function`, looked up by a name that costs less to make (these calls are bound by the host in small steps)."""
+    key = name if defines is None else name + str(defines["HEAD_DIM"])
+    fn = _entries.get(key)
+    if fn is None:
+        fn = _entries[key] = _function(library, name, argtypes, defines)
+    return fn
 
 
-@dataclass(frozen=True)
-class PageLists:
+def _wrong(what: str, name: str, t: torch.Tensor, dtype: torch.dtype, index: int, shape) -> KernelError:
+    if t.get_device() != index:
+        return KernelError(f"{what}: {name} lies on {t.device}, not with the other tensors")
+    return KernelError(f"{what}: {name} is a contiguous {dtype} tensor of {shape}, not {t.dtype} {list(t.shape)} with strides {list(t.stride())}")
+
+
+def _list_of(what: str, name: str, t: torch.Tensor, dtype: torch.dtype, index: int) -> int:
+    """The size of `t`, a contiguous tensor of one dimension on device `index`."""
+    if t.dtype is not dtype or t.dim() != 1 or not t.is_contiguous() or t.get_device() != index:
+        raise _wrong(what, name, t, dtype, index, "[n]")
+    return t.shape[0]
+
+
+def _like(what: str, name: str, t: torch.Tensor, dtype: torch.dtype, index: int, shape: tuple) -> None:
+    """`t` is a contiguous tensor of this shape on device `index`."""
+    if t.dtype is not dtype or t.shape != shape or not t.is_contiguous() or t.get_device() != index:
+        raise _wrong(what, name, t, dtype, index, list(shape))
+
+
+def _current(what: str, index: int) -> int:
+    """The current stream of the current device, which has to be device `index`, that of the tensors."""
+    if index < 0:
+        raise KernelError(f"{what} takes tensors on a CUDA device")
+    if torch._C._cuda_getDevice() != index:
+        raise KernelError(f"{what} takes tensors on the current CUDA device ({torch._C._cuda_getDevice()}), not on {index}")
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
+_error_addresses: dict[int, int] = {}
+
+
+def _error_address(index: int) -> int:
+    """Where `error_word` of a device lies (it is made once)."""
+    address = _error_addresses.get(index)
+    if address is None:
+        address = _error_addresses[index] = error_word(torch.device("cuda", index)).data_ptr()
+    return address
+
+
+class PageLists(NamedTuple):
     """Which physical pages requests hold in one group of caches: `pages` (int32, one dimension) has each request's from `starts[request]`
     (int64) on, in the order of its positions, -1 where one was given back; lists one behind the other, or the rows of a table that a program
     keeps. The block table that is made of them has `width` columns; `stride` positions share a stored row."""
@@ -1301,8 +1336,7 @@ class PageLists:
     stride: int = 1
 
 
-@dataclass(frozen=True)
-class StepTables:
+class StepTables(NamedTuple):
     """What `step_tables` makes: the fields of a `StepContext` and, for each group, (block table, slot mapping)."""
 
     positions: torch.Tensor
@@ -1312,13 +1346,8 @@ class StepTables:
     tree: StepTree | None
 
 
-class _TableGroup(ctypes.Structure):
-    _fields_ = [(name, c_void_p) for name in ("pages", "starts", "table", "slots")] + [("count", c_longlong), ("width", c_int), ("stride", c_int)]
-
-
-class _StepTablesArgs(ctypes.Structure):
-    _fields_ = [(name, c_void_p) for name in ("held", "brought", "parents", "positions", "cu_seqlens", "seq_lens", "ancestors", "err")] + \
-               [(name, c_int) for name in ("requests", "tokens", "page_size", "words", "groups")] + [("group", _TableGroup * 8)]
+_TABLES, _TABLE_GROUP = struct.Struct("8P5i4x"), struct.Struct("4Pq2i")  # StepTables, TableGroup in drafted.cu
+MOST_TABLE_GROUPS = 8
 
 
 def step_tables(held: torch.Tensor, brought: torch.Tensor, lists: "list[PageLists]", page_size: int, tokens: int,
@@ -1335,47 +1364,45 @@ def step_tables(held: torch.Tensor, brought: torch.Tensor, lists: "list[PageList
     A list too short or a table too narrow for its request, more tokens than rows, a parent that is no earlier token: the error word, and
     -1 in the request's tables (`raise_on_error`)."""
     what = "step_tables"
-    n = held.shape[0]
-    _here(what, held, brought, parents, *(t for x in lists for t in (x.pages, x.starts)))
-    _flat(what, "held", held, torch.int32, None)
-    _flat(what, "brought", brought, torch.int32, n)
-    words = 0
+    index, int32 = held.get_device(), torch.int32
+    n = _list_of(what, "held", held, int32, index)
+    _like(what, "brought", brought, int32, index, (n,))
+    words, count = 0, len(lists)
     if most is not None:
         if not 1 <= most <= MOST_DRAFTED:
             raise KernelError(f"{what}: a request brings 1 to {MOST_DRAFTED} drafted tokens, not {most}")
-        words = -(-most // 32)
+        words = (most + 31) // 32
     if parents is not None:
         if most is None:
             raise KernelError(f"{what}: parents go with `most`, the most tokens that a request brings")
-        _flat(what, "parents", parents, torch.int32, tokens)
-    if not 1 <= n <= 65534 or tokens < 0 or page_size < 1 or len(lists) > 8:
-        raise KernelError(f"{what} takes 1 to 65,534 requests, pages of a token or more and up to eight groups")
-    args = _StepTablesArgs(held=held.data_ptr(), brought=brought.data_ptr(), parents=_ptr(parents), requests=n, tokens=tokens, page_size=page_size,
-                           words=words, groups=len(lists))
-    # One buffer: the slots (8 bytes each) first, then all that has 4.
-    sizes = [2 * tokens] * len(lists) + [tokens, n + 1, n, tokens * words] + [n * x.width for x in lists]
+        _like(what, "parents", parents, int32, index, (tokens,))
+    if not 1 <= n <= 65534 or not 0 <= tokens < 1 << 31 or page_size < 1 or count > MOST_TABLE_GROUPS:
+        raise KernelError(f"{what} takes 1 to 65,534 requests, pages of a token or more and up to {MOST_TABLE_GROUPS} groups")
     for x in lists:
-        _flat(what, "pages", x.pages, torch.int32, None)
-        _flat(what, "starts", x.starts, torch.int64, n)
+        _list_of(what, "pages", x.pages, int32, index)
+        _like(what, "starts", x.starts, torch.int64, index, (n,))
         if x.width < 1 or x.stride < 1 or (x.stride > 1 and most is not None):
             raise KernelError(f"{what}: tables have a column or more, and drafted tokens a stored row each")
-    parts = torch.empty(sum(sizes), dtype=torch.int32, device=held.device).split(sizes)
-    count = len(lists)
-    positions, cu_seqlens, seq_lens, ancestors = parts[count: count + 4]
-    args.positions, args.cu_seqlens, args.seq_lens = positions.data_ptr(), cu_seqlens.data_ptr(), seq_lens.data_ptr()
-    args.ancestors, args.err = ancestors.data_ptr() if words else None, error_word(held.device).data_ptr()
+    stream, device = _current(what, index), held.device
+    buffer = torch.empty(tokens + 2 * n + 1, dtype=int32, device=device)
+    positions, cu_seqlens, seq_lens = buffer.split_with_sizes((tokens, n + 1, n))
+    at, ancestors, sees = buffer.data_ptr(), None, 0
+    if words:
+        ancestors = torch.empty(tokens, words, dtype=int32, device=device)
+        sees = ancestors.data_ptr()
+    packed = _TABLES.pack(held.data_ptr(), brought.data_ptr(), 0 if parents is None else parents.data_ptr(), at, at + 4 * tokens,
+                          at + 4 * (tokens + n + 1), sees, _error_address(index), n, tokens, page_size, words, count)
     groups = []
-    for i, x in enumerate(lists):
-        slots, table = parts[i], parts[count + 4 + i]
-        args.group[i] = _TableGroup(x.pages.data_ptr(), x.starts.data_ptr(), table.data_ptr(), slots.data_ptr(), x.pages.shape[0], x.width, x.stride)
-        groups.append((table.view(n, x.width), slots.view(torch.int64)))
-    fn = _function("drafted", "omnia_step_tables", [c_void_p, c_void_p])
-    _check(fn(ctypes.addressof(args), _stream()), what)
-    return StepTables(positions, cu_seqlens, seq_lens, groups, StepTree(ancestors.view(tokens, words)) if words else None)
+    for pages, starts, width, stride in lists:
+        table, slots = torch.empty(n, width, dtype=int32, device=device), torch.empty(tokens, dtype=torch.int64, device=device)
+        packed += _TABLE_GROUP.pack(pages.data_ptr(), starts.data_ptr(), table.data_ptr(), slots.data_ptr(), pages.shape[0], width, stride)
+        groups.append((table, slots))
+    # (The C side reads as many groups as it is told of.)
+    _check(_entry("drafted", "omnia_step_tables", [c_void_p, c_void_p])(packed, stream), what)
+    return StepTables(positions, cu_seqlens, seq_lens, groups, None if ancestors is None else StepTree(ancestors))
 
 
-@dataclass(frozen=True)
-class Accepted:
+class Accepted(NamedTuple):
     """What of a step's drafted tokens is kept: `path` int32 [requests, 32 * words], the kept ones' numbers within their request's, in order, -1
     behind them; `kept` int32 [requests], how many; `tokens` int32 [requests], what was chosen behind the last of them (-1: none was brought)."""
 
@@ -1389,20 +1416,31 @@ def accept_drafts(chosen: torch.Tensor, token_ids: torch.Tensor, tree: StepTree,
     (`chosen` int32 [tokens]: for every row of the step what its logits gave), as long as that was drafted there, of equal ones the first. Sampled
     choices keep the model's distribution: each is a draw from its own row, whatever was drafted."""
     what = "accept_drafts"
-    _here(what, chosen, token_ids, tree.ancestors, cu_seqlens)
-    tokens, words = tree.ancestors.shape if tree.ancestors.dim() == 2 else (0, 0)
-    _flat(what, "ancestors", tree.ancestors, torch.int32, None, None)
-    _flat(what, "chosen", chosen, torch.int32, tokens)
-    _flat(what, "token_ids", token_ids, torch.int32, tokens)
-    _flat(what, "cu_seqlens", cu_seqlens, torch.int32, None)
-    n = cu_seqlens.shape[0] - 1
+    ancestors = tree.ancestors
+    index, int32 = ancestors.get_device(), torch.int32
+    tokens, words = ancestors.shape if ancestors.dim() == 2 else (0, 0)
+    n = _list_of(what, "cu_seqlens", cu_seqlens, int32, index) - 1
     if n < 1 or not 1 <= words <= MOST_DRAFTED // 32:
         raise KernelError(f"{what} takes a request or more, of {MOST_DRAFTED} tokens at most")
-    path, kept, last = torch.empty(n * (32 * words + 2), dtype=torch.int32, device=chosen.device).split([n * 32 * words, n, n])
-    fn = _function("drafted", "omnia_accept_drafts", [c_void_p] * 4 + [c_int, c_int] + [c_void_p] * 3 + [c_int, c_void_p, c_void_p])
-    _check(fn(chosen.data_ptr(), token_ids.data_ptr(), tree.ancestors.data_ptr(), cu_seqlens.data_ptr(), n, words, path.data_ptr(), kept.data_ptr(),
-              last.data_ptr(), tokens, error_word(chosen.device).data_ptr(), _stream()), what)
-    return Accepted(path.view(n, 32 * words), kept, last)
+    _like(what, "ancestors", ancestors, int32, index, (tokens, words))
+    _like(what, "chosen", chosen, int32, index, (tokens,))
+    _like(what, "token_ids", token_ids, int32, index, (tokens,))
+    stream = _current(what, index)
+    path, buffer = torch.empty(n, 32 * words, dtype=int32, device=chosen.device), torch.empty(2, n, dtype=int32, device=chosen.device)
+    kept, last = buffer.unbind()
+    at = buffer.data_ptr()
+    fn = _entry("drafted", "omnia_accept_drafts", [c_void_p] * 4 + [c_int, c_int] + [c_void_p] * 3 + [c_int, c_void_p, c_void_p])
+    _check(fn(chosen.data_ptr(), token_ids.data_ptr(), ancestors.data_ptr(), cu_seqlens.data_ptr(), n, words, path.data_ptr(), at, at + 4 * n,
+              tokens, _error_address(index), stream), what)
+    return Accepted(path, kept, last)
+
+
+@functools.lru_cache(maxsize=256)
+def _page_kinds(rows: tuple[tuple[int, int], ...], page_size: int, elements: int, item: int) -> array.array:
+    """Of every kind of row: heads, then bytes of a head's row."""
+    if not 1 <= len(rows) <= 8 or any(h < 1 or w < 1 for h, w in rows) or sum(h * w for h, w in rows) * page_size != elements:
+        raise KernelError(f"pages of {elements} elements do not hold {page_size} rows of {rows}")
+    return array.array("i", [h for h, _ in rows] + [w * item for _, w in rows])
 
 
 def keep_rows(pages: torch.Tensor, rows: tuple[tuple[int, int], ...], page_size: int, block_table: torch.Tensor, held: torch.Tensor,
@@ -1411,32 +1449,30 @@ def keep_rows(pages: torch.Tensor, rows: tuple[tuple[int, int], ...], page_size:
     `copy_pages`), the i-th kept token's rows go to where the i-th token behind the request's `held` positions (int32 [requests]; below 0: nothing) is
     stored. Other drafted tokens' rows are what they were, or a kept one's. -> `pages`"""
     what = "keep_rows"
-    _here(what, pages, block_table, held, accepted.path, accepted.kept)
-    _flat(what, "block_table", block_table, torch.int32, None, None)
-    n, width = block_table.shape
-    _flat(what, "held", held, torch.int32, n)
-    _flat(what, "path", accepted.path, torch.int32, n, None)
-    _flat(what, "kept", accepted.kept, torch.int32, n)
-    shape, item = pages.shape, pages.element_size()
+    path, kept, int32 = accepted.path, accepted.kept, torch.int32
+    index = pages.get_device()
+    if block_table.dim() != 2 or path.dim() != 2 or pages.dim() < 3:
+        raise KernelError(f"{what} takes pages [layers, pages, ...], a block table [requests, pages] and paths [requests, tokens]")
+    (n, width), most, shape, item = block_table.shape, path.shape[1], pages.shape, pages.element_size()
+    _like(what, "block_table", block_table, int32, index, (n, width))
+    _like(what, "held", held, int32, index, (n,))
+    _like(what, "path", path, int32, index, (n, most))
+    _like(what, "kept", kept, int32, index, (n,))
+    if not pages.is_contiguous():
+        raise KernelError(f"{what} takes contiguous pages")
     elements = math.prod(shape[2:])
-    if not pages.is_contiguous() or pages.dim() < 3 or not 1 <= len(rows) <= 8 or sum(h * w for h, w in rows) * page_size != elements:
-        raise KernelError(f"{what} takes contiguous pages that hold {page_size} rows of {rows}")
-    if not 1 <= accepted.path.shape[1] <= MOST_DRAFTED:
-        raise KernelError(f"{what} takes paths of 1 to {MOST_DRAFTED} tokens")
-    heads, sizes = (c_int * len(rows))(*(h for h, _ in rows)), (c_int * len(rows))(*(w * item for _, w in rows))
-    fn = _function("drafted", "omnia_keep_rows", [c_void_p, c_longlong, c_longlong, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_int,
-                                                  c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p])
-    _check(fn(pages.data_ptr(), shape[1] * elements * item, elements * item, shape[0], shape[1], page_size, heads, sizes, len(rows),
-              block_table.data_ptr(), width, held.data_ptr(), accepted.path.data_ptr(), accepted.kept.data_ptr(), n, accepted.path.shape[1],
-              error_word(pages.device).data_ptr(), _stream()), what)
+    kinds = _page_kinds(rows, page_size, elements, item)
+    if not 1 <= most <= MOST_DRAFTED or not 1 <= n or width < 1 or not 1 <= shape[0] <= 65535 or shape[1] < 1:
+        raise KernelError(f"{what} takes a request or more, with paths of 1 to {MOST_DRAFTED} tokens, and pages of a layer or more")
+    stream, at = _current(what, index), kinds.buffer_info()[0]
+    fn = _entry("drafted", "omnia_keep_rows", [c_void_p, c_longlong, c_longlong, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_int,
+                                               c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p])
+    _check(fn(pages.data_ptr(), shape[1] * elements * item, elements * item, shape[0], shape[1], page_size, at, at + 4 * len(rows), len(rows),
+              block_table.data_ptr(), width, held.data_ptr(), path.data_ptr(), kept.data_ptr(), n, most, _error_address(index), stream), what)
     return pages
 
 
-class _TreeArgs(ctypes.Structure):  # TreeAttention in attention_tree.cuh
-    _fields_ = [(name, c_void_p) for name in ("q", "k_pages", "v_pages", "gate", "out", "block_table", "cu_seqlens", "seq_lens", "positions",
-                                              "ancestors", "sink", "part_o", "part_ml", "err")] + [("page_stride", c_longlong)] + \
-               [(name, c_int) for name in ("tokens", "requests", "max_pages", "num_pages", "nq", "nkv", "d", "dv", "page_size", "gate_stride", "words",
-                                           "window", "keep", "run", "chunk", "parts")] + [("scale", c_float), ("softcap", c_float)]
+_TREE = struct.Struct("14Pq16i2f")  # TreeAttention in attention_tree.cuh
 
 
 @functools.lru_cache(maxsize=4096)
@@ -1461,61 +1497,73 @@ def tree_attention(q: torch.Tensor, kv: KVView, step: StepContext, scale: float,
         raise KernelError(f"{what} takes a step of drafted trees")
     if q.dim() != 3 or not q.is_contiguous():
         raise KernelError(f"{what} takes contiguous queries [tokens, heads, width]")
+    index, int32 = q.get_device(), torch.int32
     tokens, nq, d = q.shape
+    dtype, pages, table, n, most = q.dtype, kv.pages, kv.block_table, step.num_seqs, step.max_q_len
     k_ptr, v_ptr, page_stride, nkv, dk, dv = kv_layout(kv)
-    code = _code(q.dtype)
-    pages, table, n = kv.pages, kv.block_table, step.num_seqs
-    if dk != d or nq % nkv or pages.dtype != q.dtype or not 1 <= d <= 512 or not 1 <= dv <= 512 or not pages.is_contiguous():
-        raise KernelError(f"{what}: {nq} heads of {d} ({q.dtype}) do not go with a cache of {nkv} heads of {dk} and {dv} ({pages.dtype})")
+    code = _code(dtype)
+    if dk != d or nq % nkv or pages.dtype is not dtype or not 1 <= d <= 512 or not 1 <= dv <= 512 or not pages.is_contiguous() or \
+            pages.get_device() != index:
+        raise KernelError(f"{what}: {nq} heads of {d} ({dtype}, {q.device}) do not go with a cache of {nkv} heads of {dk} and {dv} "
+                          f"({pages.dtype}, {pages.device})")
     if kv.spec is not None and kv.spec.stride != 1:
         raise KernelError(f"{what} takes a cache of a row for every position")
-    _here(what, q, pages, table, tree.ancestors, step.cu_seqlens, step.seq_lens, step.positions, gate, sink)
-    _flat(what, "ancestors", tree.ancestors, torch.int32, tokens, None)
-    _flat(what, "positions", step.positions, torch.int32, tokens)
-    _flat(what, "block_table", table, torch.int32, n, None)
-    _flat(what, "cu_seqlens", step.cu_seqlens, torch.int32, n + 1)
-    _flat(what, "seq_lens", step.seq_lens, torch.int32, n)
-    words = tree.ancestors.shape[1]
-    if not 1 <= step.max_q_len <= 32 * words <= MOST_DRAFTED:
-        raise KernelError(f"{what}: a request brings up to {step.max_q_len} tokens, the tree has {words} words for each ({MOST_DRAFTED} tokens at most)")
-    if gate is not None and (gate.dtype != q.dtype or gate.dim() != 2 or gate.stride(1) != 1 or gate.shape[0] != tokens or
-                             gate.shape[1] < gate_col + nq * dv or gate_col < 0):
-        raise KernelError(f"{what}: the gate's {nq * dv} columns from {gate_col} on lie outside rows of {list(gate.shape)}")
+    if table.dim() != 2 or tree.ancestors.dim() != 2:
+        raise KernelError(f"{what} takes a block table [requests, pages] and ancestors [tokens, words]")
+    width, words = table.shape[1], tree.ancestors.shape[1]
+    _like(what, "ancestors", tree.ancestors, int32, index, (tokens, words))
+    _like(what, "positions", step.positions, int32, index, (tokens,))
+    _like(what, "block_table", table, int32, index, (n, width))
+    _like(what, "cu_seqlens", step.cu_seqlens, int32, index, (n + 1,))
+    _like(what, "seq_lens", step.seq_lens, int32, index, (n,))
+    if not 1 <= most <= 32 * words <= MOST_DRAFTED or n < 1:
+        raise KernelError(f"{what}: a request brings up to {most} tokens, the tree has {words} words for each ({MOST_DRAFTED} tokens at most)")
+    gate_ptr = gate_stride = 0
+    if gate is not None:
+        if gate.dtype is not dtype or gate.dim() != 2 or gate.stride(1) != 1 or gate.shape[0] != tokens or gate.get_device() != index or \
+                not 0 <= gate_col <= gate.shape[1] - nq * dv:
+            raise KernelError(f"{what}: the gate's {nq * dv} columns from {gate_col} on lie outside rows of {list(gate.shape)}, or are no {dtype}")
+        gate_ptr, gate_stride = gate.data_ptr() + gate_col * dtype.itemsize, gate.stride(0)
     if sink is not None:
-        _flat(what, "sink", sink, torch.float32, nq)
+        _like(what, "sink", sink, torch.float32, index, (nq,))
     window = (kv.window if window == -1 else window) or 0
     keep = (kv.keep_first if keep_first is None else keep_first) if window else 0
     run = int(chunk or 0)
     if run and keep:
         raise KernelError("a mask of runs keeps no first positions")
-    out = torch.empty(tokens, nq * dv, dtype=q.dtype, device=q.device)
+    stream, device = _current(what, index), q.device
+    out = torch.empty(tokens, nq * dv, dtype=dtype, device=device)
     if tokens == 0:
         return out
-    a = _TreeArgs(q.data_ptr(), k_ptr, v_ptr, None if gate is None else gate.data_ptr() + gate_col * gate.element_size(), out.data_ptr(),
-                  table.data_ptr(), step.cu_seqlens.data_ptr(), step.seq_lens.data_ptr(), step.positions.data_ptr(), tree.ancestors.data_ptr(),
-                  _ptr(sink), None, None, error_word(q.device).data_ptr(), page_stride, tokens, n, table.shape[1], pages.shape[0], nq, nkv, d, dv,
-                  kv.page_size, 0 if gate is None else gate.stride(0), words, window, keep, run, 0, 0, scale, float(softcap or 0.0))
-    rows = step.max_q_len * (nq // nkv)
-    # What the longest request can see: the plan is made for that, and from numbers that a captured step knows too.
-    keys = min(max(step.max_seq_len, 1), window + keep + step.max_q_len if window else 1 << 30, run + step.max_q_len if run else 1 << 30)
-    if dv == d and q.dtype == torch.bfloat16 and d % 8 == 0 and d <= 256 and n <= 1024 and not k_ptr & 15 and not a.q & 3:
+    rows = most * (nq // nkv)
+    # What the longest request can see: plans are made for that, and from numbers that a captured step knows too.
+    keys = max(step.max_seq_len, 1)
+    if window:
+        keys = min(keys, window + keep + most)
+    if run:
+        keys = min(keys, run + most)
+    q_ptr, sms = q.data_ptr(), sm_count(device)
+    tensor_cores = dv == d and dtype is torch.bfloat16 and d % 8 == 0 and d <= 256 and n <= 1024 and not k_ptr & 15 and not q_ptr & 3
+    if tensor_cores:
         tile = 16 if rows <= 16 else 32 if rows <= 32 or d > 128 else 64
-        blocks = min((2 if d <= 128 else 1) * sm_count(q.device), n * nkv * -(-rows // tile) * -(-keys // 64))
-        parts = torch.empty(2 * blocks * tile * (d + 2), dtype=torch.float32, device=q.device)
-        a.part_o, a.part_ml = parts.data_ptr(), parts.data_ptr() + 2 * blocks * tile * d * 4
-        fn = _function("attention_tree_tc", "omnia_tree_attention_tc", [c_void_p, c_int, c_int, c_int, c_void_p], {"HEAD_DIM": d})
-        _check(fn(ctypes.addressof(a), step.max_q_len, tile, blocks, _stream()), what)
+        a_chunk, a_parts = 0, min((2 if d <= 128 else 1) * sms, n * nkv * -(-rows // tile) * -(-keys // 64))
+        slots = 2 * a_parts * tile
+    else:
+        a_chunk, a_parts = tree_plan(-(-rows // 32) * n * nkv, keys, 64, 2 * sms)
+        slots = a_parts * tokens * nq if a_parts > 1 else 0
+    part_o = torch.empty(slots * (dv + 2), dtype=torch.float32, device=device).data_ptr() if slots else 0
+    packed = _TREE.pack(
+        q_ptr, k_ptr, v_ptr, gate_ptr, out.data_ptr(), table.data_ptr(), step.cu_seqlens.data_ptr(), step.seq_lens.data_ptr(),
+        step.positions.data_ptr(), tree.ancestors.data_ptr(), 0 if sink is None else sink.data_ptr(), part_o, part_o + 4 * slots * dv,
+        _error_address(index), page_stride, tokens, n, width, pages.shape[0], nq, nkv, d, dv, kv.page_size, gate_stride, words, window, keep, run,
+        a_chunk, a_parts, scale, softcap or 0.0)
+    if tensor_cores:
+        fn = _entry("attention_tree_tc", "omnia_tree_attention_tc", [c_void_p, c_int, c_int, c_int, c_void_p], {"HEAD_DIM": d})
+        _check(fn(packed, most, tile, a_parts, stream), what)
         return out
-    tiles = -(-rows // 32) * n * nkv
-    a.chunk, a.parts = tree_plan(tiles, keys, 64, 2 * sm_count(q.device))
-    if a.parts > 1:
-        parts = torch.empty(a.parts * tokens * nq * (dv + 2), dtype=torch.float32, device=q.device)
-        a.part_o, a.part_ml = parts.data_ptr(), parts.data_ptr() + a.parts * tokens * nq * dv * 4
-    fn = _function("attention_tree", "omnia_tree_attention", [c_void_p, c_int, c_int, c_void_p])
-    _check(fn(ctypes.addressof(a), step.max_q_len, code, _stream()), what)
-    if a.parts > 1:
-        fn = _function("attention_tree", "omnia_tree_merge", [c_void_p, c_int, c_void_p])
-        _check(fn(ctypes.addressof(a), code, _stream()), what)
+    _check(_entry("attention_tree", "omnia_tree_attention", [c_void_p, c_int, c_int, c_void_p])(packed, most, code, stream), what)
+    if a_parts > 1:
+        _check(_entry("attention_tree", "omnia_tree_merge", [c_void_p, c_int, c_void_p])(packed, code, stream), what)
     return out
 
 
@@ -2082,8 +2130,7 @@ def sample(logits: torch.Tensor, temperature: torch.Tensor, top_k: torch.Tensor,
 # What a caller's options do to logits (csrc/logits.cu)
 
 
-@dataclass(frozen=True)
-class TokenHistory:
+class TokenHistory(NamedTuple):
     """Requests' texts: `tokens` (int32, one dimension) has request r's `lengths[r]` tokens from `starts[r]` on, the first `prompts[r]` of which
     were given to it and the rest generated (`starts` int64, the others int32 [requests])."""
 
@@ -2093,8 +2140,7 @@ class TokenHistory:
     prompts: torch.Tensor
 
 
-@dataclass(frozen=True)
-class LogitBias:
+class LogitBias(NamedTuple):
     """What requests add to tokens' logits: request r's entries are `starts[r]` to `starts[r + 1]` (int32 [requests + 1]) of `ids` (int32) and
     `values` (float32); of an id that is named twice, both count."""
 
@@ -2103,8 +2149,7 @@ class LogitBias:
     starts: torch.Tensor
 
 
-@dataclass(frozen=True)
-class TokenMasks:
+class TokenMasks(NamedTuple):
     """Which tokens are allowed: `words` int32 [masks, at least vocab / 32], a bit a token (the lowest of word 0 first), and `rows` int32 [rows], the
     mask of each row of logits (-1: none)."""
 
@@ -2112,8 +2157,7 @@ class TokenMasks:
     rows: torch.Tensor
 
 
-@dataclass(frozen=True)
-class DraftedRows:
+class DraftedRows(NamedTuple):
     """Rows of logits that belong to drafted tokens: `rows` int32 [rows of logits], each one's row of the step, whose tree, token ids and
     cu_seqlens these are. A request's history then ends ahead of what it brings to the step, and each row's text goes on with the tokens on its
     way through the tree, its own the last."""
@@ -2124,12 +2168,7 @@ class DraftedRows:
     rows: torch.Tensor
 
 
-class _AdjustArgs(ctypes.Structure):  # AdjustLogits in logits.cu
-    _fields_ = [(name, c_void_p) for name in (
-        "logits", "out", "requests", "history", "starts", "lengths", "prompts", "contexts", "repetition", "frequency", "presence", "bias_ids",
-        "bias_values", "bias_starts", "mask_words", "mask_rows", "ancestors", "token_ids", "cu_seqlens", "nodes", "err")] + \
-        [(name, c_longlong) for name in ("stride", "out_stride", "history_tokens", "bias_count")] + \
-        [(name, c_int) for name in ("rows", "vocab", "num_requests", "masks", "mask_width", "words", "tokens", "each", "penalised")]
+_ADJUST = struct.Struct("21P4q9i4x")  # AdjustLogits in logits.cu
 
 
 def adjust_logits(logits: torch.Tensor, *, history: TokenHistory | None = None, repetition: torch.Tensor | None = None,
@@ -2145,81 +2184,84 @@ def adjust_logits(logits: torch.Tensor, *, history: TokenHistory | None = None, 
     `out`: None for a new tensor; `logits` itself: in place, which reads and writes only what changes; or another tensor of the same shape that
     shares no memory with it."""
     what = "adjust_logits"
-    if logits.dim() != 2 or logits.dtype != torch.float32 or logits.stride(1) != 1:
+    if logits.dim() != 2 or logits.dtype is not torch.float32 or logits.stride(1) != 1:
         raise KernelError(f"{what} takes float32 logits [rows, vocab] whose rows lie in one piece")
-    rows, vocab = logits.shape
+    index, int32, (rows, vocab), stride = logits.get_device(), torch.int32, logits.shape, logits.stride(0)
+    if rows > 1 and stride < vocab:
+        raise KernelError(f"{what} takes rows that lie apart")
+    num, of_history, penalised = rows, (0, 0, 0, 0), 0
+    if history is not None:
+        num = _list_of(what, "lengths", history.lengths, int32, index)
+        _list_of(what, "tokens", history.tokens, int32, index)
+        _like(what, "starts", history.starts, torch.int64, index, (num,))
+        _like(what, "prompts", history.prompts, int32, index, (num,))
+        of_history = (history.tokens.data_ptr(), history.starts.data_ptr(), history.lengths.data_ptr(), history.prompts.data_ptr())
+    elif contexts is not None:
+        raise KernelError(f"{what}: penalties go by the requests' history")
+    of_penalties = []
+    for name, t in (("repetition", repetition), ("frequency", frequency), ("presence", presence)):
+        if t is None:
+            of_penalties.append(0)
+            continue
+        if history is None:
+            raise KernelError(f"{what}: penalties go by the requests' history")
+        _like(what, name, t, torch.float32, index, (num,))
+        of_penalties.append(t.data_ptr())
+        penalised = 1
+    if contexts is not None:
+        _like(what, "contexts", contexts, int32, index, (num,))
+    of_bias, entries = (0, 0, 0), 0
+    if bias is not None:
+        entries = _list_of(what, "ids", bias.ids, int32, index)
+        if history is None:
+            num = _list_of(what, "bias starts", bias.starts, int32, index) - 1
+        _like(what, "bias starts", bias.starts, int32, index, (num + 1,))
+        _like(what, "values", bias.values, torch.float32, index, (entries,))
+        of_bias = (bias.ids.data_ptr(), bias.values.data_ptr(), bias.starts.data_ptr())
+    if requests is not None:
+        _like(what, "requests", requests, int32, index, (rows,))
+    elif num < rows and (history is not None or bias is not None):
+        raise KernelError(f"{what}: {rows} rows of {num} requests need `requests`")
+    of_masks, count, width = (0, 0), 0, 0
+    if masks is not None:
+        if masks.words.dim() != 2 or masks.words.shape[1] * 32 < vocab:
+            raise KernelError(f"{what}: masks are [masks, words] of {vocab} tokens, 32 a word, not {list(masks.words.shape)}")
+        count, width = masks.words.shape
+        _like(what, "mask words", masks.words, int32, index, (count, width))
+        _like(what, "mask rows", masks.rows, int32, index, (rows,))
+        of_masks = (masks.words.data_ptr(), masks.rows.data_ptr())
+    of_drafted, words, tokens = (0, 0, 0, 0), 0, 0
+    if drafted is not None:
+        ancestors = drafted.tree.ancestors
+        if ancestors.dim() != 2 or (history is not None and requests is None):
+            raise KernelError(f"{what}: drafted rows need `requests`, and a tree of [tokens, words]")
+        tokens, words = ancestors.shape
+        _like(what, "ancestors", ancestors, int32, index, (tokens, words))
+        _like(what, "token_ids", drafted.token_ids, int32, index, (tokens,))
+        _like(what, "drafted rows", drafted.rows, int32, index, (rows,))
+        _like(what, "cu_seqlens", drafted.cu_seqlens, int32, index, (num + 1,) if history is not None else drafted.cu_seqlens.shape)
+        if penalised:
+            of_drafted = (ancestors.data_ptr(), drafted.token_ids.data_ptr(), drafted.cu_seqlens.data_ptr(), drafted.rows.data_ptr())
+    same = out is logits
     if out is None:
         out = torch.empty(rows, vocab, dtype=torch.float32, device=logits.device)
-    same = out is logits or (out.data_ptr() == logits.data_ptr() and out.shape == logits.shape and out.stride() == logits.stride())
-    if out.dtype != torch.float32 or out.shape != logits.shape or out.stride(1) != 1 or (rows > 1 and min(out.stride(0), logits.stride(0)) < vocab):
-        raise KernelError(f"{what} writes float32 rows that lie apart, in the logits' shape")
-    if not same:
-        a, b = logits.data_ptr(), out.data_ptr()
-        if rows and a < b + 4 * ((rows - 1) * out.stride(0) + vocab) and b < a + 4 * ((rows - 1) * logits.stride(0) + vocab):
+        out_ptr, out_stride, in_ptr = out.data_ptr(), vocab, logits.data_ptr()
+    else:
+        if out.dtype is not torch.float32 or out.shape != logits.shape or out.stride(1) != 1 or out.get_device() != index or \
+                (rows > 1 and out.stride(0) < vocab):
+            raise KernelError(f"{what} writes float32 rows that lie apart, in the logits' shape")
+        out_ptr, out_stride, in_ptr = out.data_ptr(), out.stride(0), logits.data_ptr()
+        same = same or (out_ptr == in_ptr and out_stride == stride)
+        if not same and rows and out_ptr < in_ptr + 4 * ((rows - 1) * stride + vocab) and in_ptr < out_ptr + 4 * ((rows - 1) * out_stride + vocab):
             raise KernelError(f"{what} writes to the logits themselves, or to a tensor that shares no memory with them")
-    penalties = [("repetition", repetition), ("frequency", frequency), ("presence", presence)]
-    given = [t for _, t in penalties if t is not None]
-    if (given or contexts is not None) and history is None:
-        raise KernelError(f"{what}: penalties go by the requests' history")
-    tensors = [logits, out, requests, contexts, *given]
-    num = rows
-    if history is not None:
-        num = history.lengths.shape[0]
-        tensors += [history.tokens, history.starts, history.lengths, history.prompts]
-        _flat(what, "tokens", history.tokens, torch.int32, None)
-        _flat(what, "starts", history.starts, torch.int64, num)
-        _flat(what, "lengths", history.lengths, torch.int32, num)
-        _flat(what, "prompts", history.prompts, torch.int32, num)
-    if bias is not None:
-        if history is None:
-            num = bias.starts.shape[0] - 1
-        tensors += [bias.ids, bias.values, bias.starts]
-        _flat(what, "ids", bias.ids, torch.int32, None)
-        _flat(what, "values", bias.values, torch.float32, bias.ids.shape[0])
-        _flat(what, "bias starts", bias.starts, torch.int32, num + 1)
-    for name, t in penalties:
-        if t is not None:
-            _flat(what, name, t, torch.float32, num)
-    if contexts is not None:
-        _flat(what, "contexts", contexts, torch.int32, num)
-    if requests is not None:
-        _flat(what, "requests", requests, torch.int32, rows)
-    elif (history is not None or bias is not None) and num < rows:
-        raise KernelError(f"{what}: {rows} rows of {num} requests need `requests`")
-    if masks is not None:
-        tensors += [masks.words, masks.rows]
-        _flat(what, "mask words", masks.words, torch.int32, None, None)
-        _flat(what, "mask rows", masks.rows, torch.int32, rows)
-        if masks.words.shape[1] * 32 < vocab:
-            raise KernelError(f"{what}: {masks.words.shape[1]} words do not hold {vocab} tokens")
-    if drafted is not None:
-        tensors += [drafted.tree.ancestors, drafted.token_ids, drafted.cu_seqlens, drafted.rows]
-        _flat(what, "ancestors", drafted.tree.ancestors, torch.int32, None, None)
-        _flat(what, "token_ids", drafted.token_ids, torch.int32, drafted.tree.ancestors.shape[0])
-        _flat(what, "cu_seqlens", drafted.cu_seqlens, torch.int32, None)
-        _flat(what, "drafted rows", drafted.rows, torch.int32, rows)
-        if history is not None and (requests is None or drafted.cu_seqlens.shape[0] != num + 1):
-            raise KernelError(f"{what}: drafted rows need `requests`, and the step of the same {num} requests")
-    _here(what, *tensors)
+    stream = _current(what, index)
     if rows == 0 or vocab == 0:
         return out
-    a = _AdjustArgs(logits=logits.data_ptr(), out=out.data_ptr(), requests=_ptr(requests), repetition=_ptr(repetition), frequency=_ptr(frequency),
-                    presence=_ptr(presence), contexts=_ptr(contexts), err=error_word(logits.device).data_ptr(), stride=logits.stride(0),
-                    out_stride=out.stride(0), rows=rows, vocab=vocab, num_requests=num)
-    if history is not None and given:
-        a.history, a.starts, a.lengths, a.prompts = (t.data_ptr() for t in (history.tokens, history.starts, history.lengths, history.prompts))
-        a.history_tokens, a.penalised = history.tokens.shape[0], 1
-        if drafted is not None:
-            a.ancestors, a.token_ids, a.cu_seqlens, a.nodes = (t.data_ptr() for t in (drafted.tree.ancestors, drafted.token_ids, drafted.cu_seqlens,
-                                                                                      drafted.rows))
-            a.words, a.tokens = drafted.tree.ancestors.shape[1], drafted.tree.ancestors.shape[0]
-    if bias is not None:
-        a.bias_ids, a.bias_values, a.bias_starts, a.bias_count = bias.ids.data_ptr(), bias.values.data_ptr(), bias.starts.data_ptr(), bias.ids.shape[0]
-    if masks is not None:
-        a.mask_words, a.mask_rows = masks.words.data_ptr(), masks.rows.data_ptr()
-        a.masks, a.mask_width = masks.words.shape
-    fn = _function("logits", "omnia_adjust_logits", [c_void_p, c_int, c_void_p])
-    _check(fn(ctypes.addressof(a), int(same), _stream()), what)
+    packed = _ADJUST.pack(
+        in_ptr, out_ptr, 0 if requests is None else requests.data_ptr(), *of_history, 0 if contexts is None else contexts.data_ptr(), *of_penalties,
+        *of_bias, *of_masks, *of_drafted, _error_address(index), stride, out_stride, 0 if history is None else history.tokens.shape[0], entries,
+        rows, vocab, num, count, width, words, tokens, 0, penalised)
+    _check(_entry("logits", "omnia_adjust_logits", [c_void_p, c_int, c_void_p])(packed, same, stream), what)
     return out
 
 

@@ -39,7 +39,7 @@ Block:        ``entry_norm`` and ``forward(x, h, ctx, exit_norm) -> (x, h_next)`
 from __future__ import annotations
 
 from dataclasses import dataclass, field
-from typing import Any, Callable
+from typing import Any, Callable, NamedTuple
 
 import torch
 
@@ -319,8 +319,7 @@ class KVView:
         heads, width = rows[index]
         return self.pages[:, start: start + heads * width * self.page_size].view(-1, heads, self.page_size, width)
 
-@dataclass(frozen=True)
-class StepTree:
+class StepTree(NamedTuple):
     """Of a step whose requests bring trees of drafted tokens: what each of them sees of its request's, itself too.
 
     ancestors: int32 [tokens, words]; bit m of row t (the lowest bit of word 0 first): the row's token sees the m-th token that its
