@@ -20,13 +20,14 @@ struct TreeAttention {
 };
 
 // The keys of a request that a step's rows can see, numbered 0, 1, ...: the kept first positions below `lo`, then the positions from `lo` on and
-// the nodes behind them. `lo` is where the window or the run of the earliest node, at position `held`, begins.
+// the nodes behind them. `lo` is where the window or the run of the earliest node, at position `held`, begins. For a kernel that fetches keys
+// `align` at a time, from a multiple of that on, both are rounded to such multiples (what that lets in no row sees).
 struct TreeKeys {
   int first, count, held, lo, kept, total;  // first: row of the request's node 0; total: keys, as numbered
   __device__ __forceinline__ int key(int x) const { return x < kept ? x : lo + (x - kept); }
 };
 
-__device__ __forceinline__ TreeKeys tree_keys(const TreeAttention& a, int request) {
+__device__ __forceinline__ TreeKeys tree_keys(const TreeAttention& a, int request, int align = 1) {
   TreeKeys k;
   k.first = a.cu_seqlens[request];
   k.count = a.cu_seqlens[request + 1] - k.first;
@@ -45,7 +46,8 @@ __device__ __forceinline__ TreeKeys tree_keys(const TreeAttention& a, int reques
   }
   if (a.window > 0) k.lo = max(0, k.held - a.window + 1);
   if (a.run > 0) k.lo = max(k.lo, k.held - k.held % a.run);
-  k.kept = min(a.window > 0 ? a.keep : 0, k.lo);
+  k.lo -= k.lo % align;
+  k.kept = min(a.window > 0 ? (a.keep + align - 1) / align * align : 0, k.lo);
   k.total = k.kept + held - k.lo;
   return k;
 }
@@ -65,7 +67,7 @@ __device__ __forceinline__ int tree_low(const TreeAttention& a, int pos) {
 constexpr int TREE_MOST_REQUESTS = 1024;
 
 struct TreeShares {
-  int rows, keys;  // of a tile
+  int rows, keys, align;  // of a tile, and of `tree_keys`
   __device__ __forceinline__ int row_tiles(const TreeAttention& a, const TreeKeys& k) const {
     return k.total > 0 ? (k.count * (a.nq / a.nkv) + rows - 1) / rows : 0;
   }
@@ -79,7 +81,7 @@ struct TreeShares {
       const int r = r0 + threadIdx.x;
       long long mine = 0;
       if (r < a.requests) {
-        const TreeKeys k = tree_keys(a, r);
+        const TreeKeys k = tree_keys(a, r, align);
         mine = (long long)row_tiles(a, k) * key_tiles(k) * a.nkv;
       }
 #pragma unroll
@@ -107,7 +109,7 @@ struct TreePlace {
   TreeKeys k;
   __device__ __forceinline__ void enter(const TreeAttention& a, const TreeShares& s, int r) {
     request = r;
-    k = tree_keys(a, r);
+    k = tree_keys(a, r, s.align);
     row_tiles = s.row_tiles(a, k), tiles = s.key_tiles(k);
   }
   __device__ __forceinline__ void find(const TreeAttention& a, const TreeShares& s, const long long* ends, long long at) {
@@ -135,3 +137,102 @@ struct TreePlace {
     while (row_tiles * tiles == 0 && request + 1 < a.requests);
   }
 };
+
+constexpr int TREE_JOIN_WARPS = 4;
+
+__device__ __forceinline__ float tree_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ unsigned tree_pair(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const unsigned*>(&v);
+}
+
+// A warp a row of an item: the slots of the blocks that had part in it, in their order, the sink, the gate. A request that sees nothing
+// has zeros.
+template <int D>
+__global__ void __launch_bounds__(32 * TREE_JOIN_WARPS) tree_join_kernel(const __grid_constant__ TreeAttention a, const TreeShares shares, int grid) {
+  constexpr int WARPS = TREE_JOIN_WARPS;
+  constexpr float LOG2E = 1.4426950408889634f;
+  __shared__ long long ends[TREE_MOST_REQUESTS], sums[WARPS];
+  // (What is read ahead of the wait was there ahead of the kernel that this one waits for.)
+  const int rows_of_tile = shares.rows;
+  const long long total = shares.lay_out(a, ends, sums), blocks = min((long long)grid, total);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int request = blockIdx.z, head_kv = blockIdx.y, group = a.nq / a.nkv, in = blockIdx.x * WARPS + warp, row_tile = in / rows_of_tile, r = in % rows_of_tile;
+  const TreeKeys k = tree_keys(a, request, shares.align);
+  const int tiles = shares.key_tiles(k), row_tiles = shares.row_tiles(a, k);
+  if (blockIdx.x == 0 && head_kv == 0 && threadIdx.x == 0 && k.count * group > (int)gridDim.x * WARPS) atomicOr(a.err, OMNIA_ERR_WORK);
+  pdl_wait();
+  pdl_launch_dependents();
+  if (in >= k.count * group) return;
+  const long long begin = (request ? ends[request - 1] : 0) + ((long long)head_kv * row_tiles + row_tile) * tiles, end = begin + tiles;
+  // Tile t is block b's where b T / G <= t < (b + 1) T / G.
+  auto block_of = [&](long long t) { return (int)(((t + 1) * blocks - 1) / total); };
+  const int b0 = tiles ? block_of(begin) : 0, b1 = tiles ? block_of(end - 1) : -1;
+  if (tiles && b0 == b1) return;
+  // The item is the first of all blocks that have part in it but the one that it begins in, unless it begins that too.
+  const int slot0 = 2 * b0 + (tiles && begin <= total * b0 / blocks ? 0 : 1);
+  auto slot_of = [&](int b) { return b == b0 ? slot0 : 2 * b; };
+  const int token = k.first + in / group, head = head_kv * group + in % group;
+  const float sink = a.sink ? a.sink[head] * LOG2E : -INFINITY;
+  constexpr int PER = (D + 127) / 128;  // four dims a lane
+  float4 sum[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) sum[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  float base = -INFINITY, l = 0.f;
+  for (int c0 = b0; c0 <= b1; c0 += 32) {  // 32 slots at a time, a lane each for their offsets and sums
+    const int b = c0 + lane;
+    float ml = -INFINITY, ll = 0.f;
+    size_t row = 0;
+    if (b <= b1) {
+      row = (size_t)slot_of(b) * rows_of_tile + r;
+      const float2 x = reinterpret_cast<const float2*>(a.part_ml)[row];
+      ml = x.x, ll = x.y;
+    }
+    const float over = fmaxf(base, warp_max(ml)), offset = over == -INFINITY ? 0.f : over, f = tree_exp2(base - offset), w = tree_exp2(ml - offset);
+    l = l * f + warp_sum(ll * w);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) sum[i].x *= f, sum[i].y *= f, sum[i].z *= f, sum[i].w *= f;
+    base = over;
+    const int here = min(32, b1 - c0 + 1);
+#pragma unroll 4
+    for (int p = 0; p < here; ++p) {
+      const float by = __shfl_sync(0xffffffffu, w, p);
+      const float* from = a.part_o + (size_t)((size_t)slot_of(c0 + p) * rows_of_tile + r) * D;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int c = (32 * i + lane) * 4;
+        if (c < D && by != 0.f) {
+          const float4 v = *reinterpret_cast<const float4*>(from + c);
+          sum[i].x = fmaf(v.x, by, sum[i].x), sum[i].y = fmaf(v.y, by, sum[i].y);
+          sum[i].z = fmaf(v.z, by, sum[i].z), sum[i].w = fmaf(v.w, by, sum[i].w);
+        }
+      }
+    }
+  }
+  const float over = fmaxf(base, sink), offset = over == -INFINITY ? 0.f : over, f = tree_exp2(base - offset);
+  l = l * f + tree_exp2(sink - offset);
+  const float by = l > 0.f ? f / l : 0.f;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int c = (32 * i + lane) * 4;
+    if (c >= D) continue;
+    float y[4] = {sum[i].x * by, sum[i].y * by, sum[i].z * by, sum[i].w * by};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (by == 0.f) y[j] = 0.f;
+      if (a.gate) y[j] *= 1.f / (1.f + __expf(-__bfloat162float(static_cast<const __nv_bfloat16*>(a.gate)[(size_t)token * a.gate_stride + head * D + c + j])));
+    }
+    *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + (size_t)token * a.nq * D + head * D + c) = make_uint2(tree_pair(y[0], y[1]), tree_pair(y[2], y[3]));
+  }
+}
+
+template <int D>
+int tree_join(const TreeAttention& a, const TreeShares& shares, int most_nodes, int blocks, cudaStream_t stream) {
+  const dim3 grid((most_nodes * (a.nq / a.nkv) + TREE_JOIN_WARPS - 1) / TREE_JOIN_WARPS, a.nkv, a.requests);
+  launch_pdl(tree_join_kernel<D>, grid, dim3(32 * TREE_JOIN_WARPS), 0, stream, a, shares, blocks);
+  return OMNIA_LAUNCH_RESULT();
+}

@@ -86,7 +86,7 @@ __global__ void __launch_bounds__(THREADS, D <= 128 ? 2 : 1) tree_shares_kernel(
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, wr = warp % WR, wk = warp / WR, g = lane >> 2, t4 = lane & 3;
   pdl_wait();
   pdl_launch_dependents();
-  const TreeShares shares = {ROWS, KEYS};
+  const TreeShares shares = {ROWS, KEYS, 1};
   const long long total = shares.lay_out(a, ends, sums);
   const long long blocks = min((long long)gridDim.x, total);  // (a block more than there are tiles would leave its slots unwritten)
   if (blockIdx.x >= blocks) return;
@@ -385,83 +385,6 @@ __global__ void __launch_bounds__(THREADS, D <= 128 ? 2 : 1) tree_shares_kernel(
   }
 }
 
-// A warp a row of an item: the slots of the blocks that had part in it, in their order, the sink, the gate. A request that sees nothing
-// has zeros.
-__global__ void __launch_bounds__(THREADS) tree_join_kernel(const __grid_constant__ TreeAttention a, int rows_of_tile, int grid) {
-  __shared__ long long ends[TREE_MOST_REQUESTS], sums[WARPS];
-  // (What is read ahead of the wait was there ahead of the kernel that this one waits for.)
-  const TreeShares shares = {rows_of_tile, KEYS};
-  const long long total = shares.lay_out(a, ends, sums), blocks = min((long long)grid, total);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int request = blockIdx.z, head_kv = blockIdx.y, group = a.nq / a.nkv, in = blockIdx.x * WARPS + warp, row_tile = in / rows_of_tile, r = in % rows_of_tile;
-  const TreeKeys k = tree_keys(a, request);
-  const int tiles = shares.key_tiles(k), row_tiles = shares.row_tiles(a, k);
-  if (blockIdx.x == 0 && head_kv == 0 && threadIdx.x == 0 && k.count * group > (int)gridDim.x * WARPS) atomicOr(a.err, OMNIA_ERR_WORK);
-  pdl_wait();
-  pdl_launch_dependents();
-  if (in >= k.count * group) return;
-  const long long begin = (request ? ends[request - 1] : 0) + ((long long)head_kv * row_tiles + row_tile) * tiles, end = begin + tiles;
-  // Tile t is block b's where b T / G <= t < (b + 1) T / G.
-  auto block_of = [&](long long t) { return (int)(((t + 1) * blocks - 1) / total); };
-  const int b0 = tiles ? block_of(begin) : 0, b1 = tiles ? block_of(end - 1) : -1;
-  if (tiles && b0 == b1) return;
-  // The item is the first of all blocks that have part in it but the one that it begins in, unless it begins that too.
-  const int slot0 = 2 * b0 + (tiles && begin <= total * b0 / blocks ? 0 : 1);
-  auto slot_of = [&](int b) { return b == b0 ? slot0 : 2 * b; };
-  const int token = k.first + in / group, head = head_kv * group + in % group;
-  const float sink = a.sink ? a.sink[head] * LOG2E : -INFINITY;
-  constexpr int PER = (D + 127) / 128;  // four dims a lane
-  float4 sum[PER];
-#pragma unroll
-  for (int i = 0; i < PER; ++i) sum[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-  float base = -INFINITY, l = 0.f;
-  for (int c0 = b0; c0 <= b1; c0 += 32) {  // 32 slots at a time, a lane each for their offsets and sums
-    const int b = c0 + lane;
-    float ml = -INFINITY, ll = 0.f;
-    size_t row = 0;
-    if (b <= b1) {
-      row = (size_t)slot_of(b) * rows_of_tile + r;
-      const float2 x = reinterpret_cast<const float2*>(a.part_ml)[row];
-      ml = x.x, ll = x.y;
-    }
-    const float over = fmaxf(base, warp_max(ml)), offset = over == -INFINITY ? 0.f : over, f = fast_exp2(base - offset), w = fast_exp2(ml - offset);
-    l = l * f + warp_sum(ll * w);
-#pragma unroll
-    for (int i = 0; i < PER; ++i) sum[i].x *= f, sum[i].y *= f, sum[i].z *= f, sum[i].w *= f;
-    base = over;
-    const int here = min(32, b1 - c0 + 1);
-#pragma unroll 4
-    for (int p = 0; p < here; ++p) {
-      const float by = __shfl_sync(0xffffffffu, w, p);
-      const float* from = a.part_o + (size_t)((size_t)slot_of(c0 + p) * rows_of_tile + r) * D;
-#pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        const int c = (32 * i + lane) * 4;
-        if (c < D && by != 0.f) {
-          const float4 v = *reinterpret_cast<const float4*>(from + c);
-          sum[i].x = fmaf(v.x, by, sum[i].x), sum[i].y = fmaf(v.y, by, sum[i].y);
-          sum[i].z = fmaf(v.z, by, sum[i].z), sum[i].w = fmaf(v.w, by, sum[i].w);
-        }
-      }
-    }
-  }
-  const float over = fmaxf(base, sink), offset = over == -INFINITY ? 0.f : over, f = fast_exp2(base - offset);
-  l = l * f + fast_exp2(sink - offset);
-  const float by = l > 0.f ? f / l : 0.f;
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int c = (32 * i + lane) * 4;
-    if (c >= D) continue;
-    float y[4] = {sum[i].x * by, sum[i].y * by, sum[i].z * by, sum[i].w * by};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (by == 0.f) y[j] = 0.f;
-      if (a.gate) y[j] *= 1.f / (1.f + __expf(-__bfloat162float(static_cast<const bf16*>(a.gate)[(size_t)token * a.gate_stride + head * D + c + j])));
-    }
-    *reinterpret_cast<uint2*>(static_cast<bf16*>(a.out) + (size_t)token * a.nq * D + head * D + c) = make_uint2(pack(y[0], y[1]), pack(y[2], y[3]));
-  }
-}
-
 namespace {
 
 template <int WR>
@@ -497,7 +420,5 @@ extern "C" int omnia_tree_attention_tc(const TreeAttention* a, int most_nodes, i
 #endif
   else return (int)cudaErrorInvalidValue;
   if (code) return code;
-  const dim3 grid((most_nodes * (a->nq / a->nkv) + WARPS - 1) / WARPS, a->nkv, a->requests);
-  launch_pdl(tree_join_kernel, grid, dim3(THREADS), 0, s, *a, rows, blocks);
-  return OMNIA_LAUNCH_RESULT();
+  return tree_join<D>(*a, {rows, KEYS, 1}, most_nodes, blocks, s);
 }

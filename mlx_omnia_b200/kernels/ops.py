@@ -1472,6 +1472,10 @@ def keep_rows(pages: torch.Tensor, rows: tuple[tuple[int, int], ...], page_size:
     return pages
 
 
+TREE_MANY_ROWS = 33
+"""From so many rows (query heads of a group times the most tokens that a request brings) attention of drafted trees runs on the tcgen05 kernel, where it
+takes the head size and the pages."""
+
 _TREE = struct.Struct("14Pq16i2f")  # TreeAttention in attention_tree.cuh
 
 
@@ -1544,7 +1548,12 @@ def tree_attention(q: torch.Tensor, kv: KVView, step: StepContext, scale: float,
         keys = min(keys, run + most)
     q_ptr, sms = q.data_ptr(), sm_count(device)
     tensor_cores = dv == d and dtype is torch.bfloat16 and d % 8 == 0 and d <= 256 and n <= 1024 and not k_ptr & 15 and not q_ptr & 3
-    if tensor_cores:
+    many = tensor_cores and rows >= TREE_MANY_ROWS and d in (64, 128) and kv.page_size % 16 == 0 and scale > 0 and not q_ptr & 15 and nq // nkv <= 128
+    if many:
+        tile = 2 * (128 // (nq // nkv) * (nq // nkv))
+        a_chunk, a_parts = 0, min(sms, n * nkv * -(-rows // tile) * -(-keys // 128))
+        slots = 2 * a_parts * tile
+    elif tensor_cores:
         tile = 16 if rows <= 16 else 32 if rows <= 32 or d > 128 else 64
         a_chunk, a_parts = 0, min((2 if d <= 128 else 1) * sms, n * nkv * -(-rows // tile) * -(-keys // 64))
         slots = 2 * a_parts * tile
@@ -1557,6 +1566,10 @@ def tree_attention(q: torch.Tensor, kv: KVView, step: StepContext, scale: float,
         step.positions.data_ptr(), tree.ancestors.data_ptr(), 0 if sink is None else sink.data_ptr(), part_o, part_o + 4 * slots * dv,
         _error_address(index), page_stride, tokens, n, width, pages.shape[0], nq, nkv, d, dv, kv.page_size, gate_stride, words, window, keep, run,
         a_chunk, a_parts, scale, softcap or 0.0)
+    if many:
+        fn = _entry("attention_tree_tcgen05", "omnia_tree_attention_tcgen05", [c_void_p, c_int, c_int, c_void_p], {"HEAD_DIM": d})
+        _check(fn(packed, most, a_parts, stream), what)
+        return out
     if tensor_cores:
         fn = _entry("attention_tree_tc", "omnia_tree_attention_tc", [c_void_p, c_int, c_int, c_int, c_void_p], {"HEAD_DIM": d})
         _check(fn(packed, most, tile, a_parts, stream), what)

@@ -24,6 +24,12 @@ def no_errors():
     ops.raise_on_error(torch.device("cuda:0"))
 
 
+@pytest.fixture(params=["few rows", "many rows"])
+def way(request, monkeypatch):
+    """Both kernels of the tensor cores, at every size that they take."""
+    monkeypatch.setattr(ops, "TREE_MANY_ROWS", {"few rows": 1 << 30, "many rows": 0}[request.param])
+
+
 def ints(values, dtype=torch.int32):
     return torch.as_tensor(np.asarray(values), device="cuda").to(dtype)
 
@@ -216,7 +222,7 @@ LAYOUTS = [(16, 8, 128, BF16, 16), (32, 8, 128, BF16, 16), (16, 4, 128, BF16, 32
 
 
 @pytest.mark.parametrize("layout", LAYOUTS, ids=str)
-def test_attention_of_trees(layout):
+def test_attention_of_trees(layout, way):
     nq, nkv, d, dtype, page = layout
     c = make(nq, nkv, d, dtype, page, [(500, refs.tree(13, 1)), (0, refs.tree(5, 2)), (1, [-1]), (63, refs.chain(64)), (130, refs.tree(70, 3)),
                                        (16, refs.tree(16, 4))], seed=d)
@@ -227,7 +233,7 @@ def test_attention_of_trees(layout):
 
 
 @pytest.mark.parametrize("layout", LAYOUTS[:6] + LAYOUTS[8:10], ids=str)
-def test_attention_of_trees_under_windows(layout):
+def test_attention_of_trees_under_windows(layout, way):
     nq, nkv, d, dtype, page = layout
     c = make(nq, nkv, d, dtype, page, [(500, refs.tree(33, 1)), (3, refs.chain(40)), (100, refs.tree(7, 2)), (36, refs.tree(9, 5))], seed=1)
     for window in (1, 5, 37, 400):
@@ -248,14 +254,14 @@ def check_run(c, d, run):
 
 
 @pytest.mark.parametrize("held,nodes", [(1, 1), (64, 1), (4097, 17), (20000, 3), (3000, 256), (0, 256), (1, 200)])
-def test_attention_of_trees_by_length(held, nodes):
+def test_attention_of_trees_by_length(held, nodes, way):
     for layout in ((16, 8, 128, BF16, 16), (6, 2, 64, BF16, 16)) + (((8, 1, 24, F32, 8),) if held < 10000 else ()):
         nq, nkv, d, dtype, page = layout
         check(make(nq, nkv, d, dtype, page, [(held, refs.tree(nodes, held)), (held // 2, refs.tree(max(nodes // 3, 1), 9))], seed=nodes), d ** -0.5, gated=True)
 
 
 @pytest.mark.parametrize("layout", LAYOUTS[:1] + LAYOUTS[3:5], ids=str)
-def test_attention_of_any_masks(layout):
+def test_attention_of_any_masks(layout, way):
     """Rows that see nothing have zeros, rows may see later tokens, and none knows of what it does not see."""
     nq, nkv, d, dtype, page = layout
     c = make(nq, nkv, d, dtype, page, [(0, refs.chain(9)), (40, refs.chain(3)), (0, refs.chain(40))],
@@ -267,7 +273,7 @@ def test_attention_of_any_masks(layout):
 
 @pytest.mark.parametrize("layout", LAYOUTS[:2] + LAYOUTS[3:5] + LAYOUTS[6:7], ids=str)
 @pytest.mark.parametrize("value", [math.nan, math.inf])
-def test_what_a_node_does_not_see_may_be_anything(layout, value):
+def test_what_a_node_does_not_see_may_be_anything(layout, value, way):
     nq, nkv, d, dtype, page = layout
     c = make(nq, nkv, d, dtype, page, [(70, [-1, 0, 0, 1, 2, 2]), (200, refs.tree(40, 2))], seed=5)
     for r, (bad, held) in enumerate(((2, 70), (11, 200))):
@@ -293,7 +299,7 @@ def check_some(c, d, bad):
     return got
 
 
-def test_padding_and_rows_behind_the_last_request():
+def test_padding_and_rows_behind_the_last_request(way):
     """A request of no positions is there for the step's shape; rows behind the last request are not written."""
     for layout in LAYOUTS[:1] + LAYOUTS[4:5]:
         nq, nkv, d, dtype, page = layout
@@ -305,7 +311,7 @@ def test_padding_and_rows_behind_the_last_request():
         assert float(got[6].abs().max()) == 0
 
 
-def test_a_captured_step_takes_the_lengths_of_its_replay():
+def test_a_captured_step_takes_the_lengths_of_its_replay(way):
     nq, nkv, d, dtype, page = LAYOUTS[0]
     big = make(nq, nkv, d, dtype, page, [(900, refs.tree(16, 1)), (300, refs.tree(16, 2))], seed=3)
     small = make(nq, nkv, d, dtype, page, [(200, refs.tree(16, 5)), (899, refs.tree(16, 7))], seed=4)
@@ -340,7 +346,7 @@ def test_a_captured_step_takes_the_lengths_of_its_replay():
 
 
 @pytest.mark.parametrize("layout", [LAYOUTS[0], (8, 1, 128, F32, 16)], ids=str)
-def test_lengths_beyond_the_plan(layout):
+def test_lengths_beyond_the_plan(layout, way):
     """The kernel for any type works by a plan for so many positions, the one of the tensor cores by the lengths themselves; both by the most tokens."""
     nq, nkv, d, dtype, page = layout
     c = make(nq, nkv, d, dtype, page, [(900, refs.tree(16, 1))])
