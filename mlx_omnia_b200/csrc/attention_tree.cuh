@@ -145,94 +145,116 @@ __device__ __forceinline__ float tree_exp2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// sigmoid(x) to some units of float32's last place.
+__device__ __forceinline__ float tree_sigmoid(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(1.f + tree_exp2(-1.4426950408889634f * x)));
+  return y;
+}
 __device__ __forceinline__ unsigned tree_pair(float lo, float hi) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const unsigned*>(&v);
 }
 
-// A warp a row of an item: the slots of the blocks that had part in it, in their order, the sink, the gate. A request that sees nothing
-// has zeros.
+// An item that several blocks had part in, put together by the blocks of the grid that stand for the first border in it (between block x and block
+// x + 1 of the kernel before): a warp a row at a time, the slots in the order of their blocks, the sink, the gate. The last `requests` blocks
+// write zeros for requests that see nothing. The rows of an item are shared out over the grid's other axis.
 template <int D>
-__global__ void __launch_bounds__(32 * TREE_JOIN_WARPS) tree_join_kernel(const __grid_constant__ TreeAttention a, const TreeShares shares, int grid) {
+__global__ void __launch_bounds__(32 * TREE_JOIN_WARPS) tree_join_kernel(const __grid_constant__ TreeAttention a, const TreeShares shares, int grid, int most) {
   constexpr int WARPS = TREE_JOIN_WARPS;
   constexpr float LOG2E = 1.4426950408889634f;
   __shared__ long long ends[TREE_MOST_REQUESTS], sums[WARPS];
   // (What is read ahead of the wait was there ahead of the kernel that this one waits for.)
-  const int rows_of_tile = shares.rows;
+  const int rows_of_tile = shares.rows, group = a.nq / a.nkv, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, step = WARPS * gridDim.y;
+  if ((int)blockIdx.x >= grid - 1) {
+    const TreeKeys k = tree_keys(a, blockIdx.x - (grid - 1), shares.align);
+    if (k.count > most && blockIdx.y == 0 && threadIdx.x == 0) atomicOr(a.err, OMNIA_ERR_WORK);
+    if (k.total > 0) return;
+    pdl_wait();
+    for (int r = blockIdx.y * WARPS + warp; r < k.count * a.nq; r += step)
+      for (int c = lane; c < D; c += 32) static_cast<__nv_bfloat16*>(a.out)[((size_t)k.first * a.nq + r) * D + c] = __float2bfloat16_rn(0.f);
+    return;
+  }
   const long long total = shares.lay_out(a, ends, sums), blocks = min((long long)grid, total);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int request = blockIdx.z, head_kv = blockIdx.y, group = a.nq / a.nkv, in = blockIdx.x * WARPS + warp, row_tile = in / rows_of_tile, r = in % rows_of_tile;
-  const TreeKeys k = tree_keys(a, request, shares.align);
-  const int tiles = shares.key_tiles(k), row_tiles = shares.row_tiles(a, k);
-  if (blockIdx.x == 0 && head_kv == 0 && threadIdx.x == 0 && k.count * group > (int)gridDim.x * WARPS) atomicOr(a.err, OMNIA_ERR_WORK);
+  const int border = blockIdx.x + 1;
+  if (border >= blocks) return;
+  // Tile t is block b's where b T / G <= t < (b + 1) T / G.
+  const long long at = total * border / blocks;
+  TreePlace place;
+  place.find(a, shares, ends, at);
+  const long long begin = at - place.tile, end = begin + place.tiles;
+  if (begin == at || begin < total * (border - 1) / blocks) return;  // no border in an item, or not its first
+  const int b0 = border - 1;
+  int b1 = border;
+  while (total * (b1 + 1) / blocks < end) ++b1;
+  // The item is the first of all blocks that have part in it but the one that it begins in, unless it begins that too.
+  const int slot0 = 2 * b0 + (begin == total * b0 / blocks ? 0 : 1);
+  auto slot_of = [&](int b) { return b == b0 ? slot0 : 2 * b; };
+  const TreeKeys& k = place.k;
+  const int head_kv = place.head, here = min(rows_of_tile, k.count * group - place.row_tile * rows_of_tile);
   pdl_wait();
   pdl_launch_dependents();
-  if (in >= k.count * group) return;
-  const long long begin = (request ? ends[request - 1] : 0) + ((long long)head_kv * row_tiles + row_tile) * tiles, end = begin + tiles;
-  // Tile t is block b's where b T / G <= t < (b + 1) T / G.
-  auto block_of = [&](long long t) { return (int)(((t + 1) * blocks - 1) / total); };
-  const int b0 = tiles ? block_of(begin) : 0, b1 = tiles ? block_of(end - 1) : -1;
-  if (tiles && b0 == b1) return;
-  // The item is the first of all blocks that have part in it but the one that it begins in, unless it begins that too.
-  const int slot0 = 2 * b0 + (tiles && begin <= total * b0 / blocks ? 0 : 1);
-  auto slot_of = [&](int b) { return b == b0 ? slot0 : 2 * b; };
-  const int token = k.first + in / group, head = head_kv * group + in % group;
-  const float sink = a.sink ? a.sink[head] * LOG2E : -INFINITY;
-  constexpr int PER = (D + 127) / 128;  // four dims a lane
-  float4 sum[PER];
+  for (int r = blockIdx.y * WARPS + warp; r < here; r += step) {
+    const int in = place.row_tile * rows_of_tile + r;
+    const int token = k.first + in / group, head = head_kv * group + in % group;
+    const float sink = a.sink ? a.sink[head] * LOG2E : -INFINITY;
+    constexpr int PER = (D + 127) / 128;  // four dims a lane
+    float4 sum[PER];
 #pragma unroll
-  for (int i = 0; i < PER; ++i) sum[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-  float base = -INFINITY, l = 0.f;
-  for (int c0 = b0; c0 <= b1; c0 += 32) {  // 32 slots at a time, a lane each for their offsets and sums
-    const int b = c0 + lane;
-    float ml = -INFINITY, ll = 0.f;
-    size_t row = 0;
-    if (b <= b1) {
-      row = (size_t)slot_of(b) * rows_of_tile + r;
-      const float2 x = reinterpret_cast<const float2*>(a.part_ml)[row];
-      ml = x.x, ll = x.y;
-    }
-    const float over = fmaxf(base, warp_max(ml)), offset = over == -INFINITY ? 0.f : over, f = tree_exp2(base - offset), w = tree_exp2(ml - offset);
-    l = l * f + warp_sum(ll * w);
+    for (int i = 0; i < PER; ++i) sum[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    float base = -INFINITY, l = 0.f;
+    for (int c0 = b0; c0 <= b1; c0 += 32) {  // 32 slots at a time, a lane each for their offsets and sums
+      const int b = c0 + lane;
+      float ml = -INFINITY, ll = 0.f;
+      size_t row = 0;
+      if (b <= b1) {
+        row = (size_t)slot_of(b) * rows_of_tile + r;
+        const float2 x = reinterpret_cast<const float2*>(a.part_ml)[row];
+        ml = x.x, ll = x.y;
+      }
+      const float over = fmaxf(base, warp_max(ml)), offset = over == -INFINITY ? 0.f : over, f = tree_exp2(base - offset), w = tree_exp2(ml - offset);
+      l = l * f + warp_sum(ll * w);
 #pragma unroll
-    for (int i = 0; i < PER; ++i) sum[i].x *= f, sum[i].y *= f, sum[i].z *= f, sum[i].w *= f;
-    base = over;
-    const int here = min(32, b1 - c0 + 1);
+      for (int i = 0; i < PER; ++i) sum[i].x *= f, sum[i].y *= f, sum[i].z *= f, sum[i].w *= f;
+      base = over;
+      const int here = min(32, b1 - c0 + 1);
 #pragma unroll 4
-    for (int p = 0; p < here; ++p) {
-      const float by = __shfl_sync(0xffffffffu, w, p);
-      const float* from = a.part_o + (size_t)((size_t)slot_of(c0 + p) * rows_of_tile + r) * D;
+      for (int p = 0; p < here; ++p) {
+        const float by = __shfl_sync(0xffffffffu, w, p);
+        const float* from = a.part_o + (size_t)((size_t)slot_of(c0 + p) * rows_of_tile + r) * D;
 #pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        const int c = (32 * i + lane) * 4;
-        if (c < D && by != 0.f) {
-          const float4 v = *reinterpret_cast<const float4*>(from + c);
-          sum[i].x = fmaf(v.x, by, sum[i].x), sum[i].y = fmaf(v.y, by, sum[i].y);
-          sum[i].z = fmaf(v.z, by, sum[i].z), sum[i].w = fmaf(v.w, by, sum[i].w);
+        for (int i = 0; i < PER; ++i) {
+          const int c = (32 * i + lane) * 4;
+          if (c < D && by != 0.f) {
+            const float4 v = *reinterpret_cast<const float4*>(from + c);
+            sum[i].x = fmaf(v.x, by, sum[i].x), sum[i].y = fmaf(v.y, by, sum[i].y);
+            sum[i].z = fmaf(v.z, by, sum[i].z), sum[i].w = fmaf(v.w, by, sum[i].w);
+          }
         }
       }
     }
-  }
-  const float over = fmaxf(base, sink), offset = over == -INFINITY ? 0.f : over, f = tree_exp2(base - offset);
-  l = l * f + tree_exp2(sink - offset);
-  const float by = l > 0.f ? f / l : 0.f;
+    const float over = fmaxf(base, sink), offset = over == -INFINITY ? 0.f : over, f = tree_exp2(base - offset);
+    l = l * f + tree_exp2(sink - offset);
+    const float by = l > 0.f ? f / l : 0.f;
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int c = (32 * i + lane) * 4;
-    if (c >= D) continue;
-    float y[4] = {sum[i].x * by, sum[i].y * by, sum[i].z * by, sum[i].w * by};
+    for (int i = 0; i < PER; ++i) {
+      const int c = (32 * i + lane) * 4;
+      if (c >= D) continue;
+      float y[4] = {sum[i].x * by, sum[i].y * by, sum[i].z * by, sum[i].w * by};
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (by == 0.f) y[j] = 0.f;
-      if (a.gate) y[j] *= 1.f / (1.f + __expf(-__bfloat162float(static_cast<const __nv_bfloat16*>(a.gate)[(size_t)token * a.gate_stride + head * D + c + j])));
+      for (int j = 0; j < 4; ++j) {
+        if (by == 0.f) y[j] = 0.f;
+        if (a.gate) y[j] *= tree_sigmoid(__bfloat162float(static_cast<const __nv_bfloat16*>(a.gate)[(size_t)token * a.gate_stride + head * D + c + j]));
+      }
+      *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + (size_t)token * a.nq * D + head * D + c) = make_uint2(tree_pair(y[0], y[1]), tree_pair(y[2], y[3]));
     }
-    *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + (size_t)token * a.nq * D + head * D + c) = make_uint2(tree_pair(y[0], y[1]), tree_pair(y[2], y[3]));
   }
 }
 
 template <int D>
 int tree_join(const TreeAttention& a, const TreeShares& shares, int most_nodes, int blocks, cudaStream_t stream) {
-  const dim3 grid((most_nodes * (a.nq / a.nkv) + TREE_JOIN_WARPS - 1) / TREE_JOIN_WARPS, a.nkv, a.requests);
-  launch_pdl(tree_join_kernel<D>, grid, dim3(32 * TREE_JOIN_WARPS), 0, stream, a, shares, blocks);
+  const int rows = min(shares.rows, most_nodes * (a.nq / a.nkv));
+  const dim3 grid(blocks - 1 + a.requests, min((rows + TREE_JOIN_WARPS - 1) / TREE_JOIN_WARPS, 16));
+  launch_pdl(tree_join_kernel<D>, grid, dim3(32 * TREE_JOIN_WARPS), 0, stream, a, shares, blocks, most_nodes);
   return OMNIA_LAUNCH_RESULT();
 }

@@ -373,8 +373,8 @@ __global__ void __launch_bounds__(THREADS, D <= 128 ? 2 : 1) tree_shares_kernel(
             float y0 = o[n][2 * h] * by, y1 = o[n][2 * h + 1] * by;
             if (by == 0.f) y0 = y1 = 0.f;
             if (gate) {
-              y0 *= 1.f / (1.f + __expf(-__bfloat162float(gate[8 * n + 2 * t4])));
-              y1 *= 1.f / (1.f + __expf(-__bfloat162float(gate[8 * n + 2 * t4 + 1])));
+              y0 *= tree_sigmoid(__bfloat162float(gate[8 * n + 2 * t4]));
+              y1 *= tree_sigmoid(__bfloat162float(gate[8 * n + 2 * t4 + 1]));
             }
             *reinterpret_cast<unsigned*>(out + 8 * n + 2 * t4) = pack(y0, y1);
           }

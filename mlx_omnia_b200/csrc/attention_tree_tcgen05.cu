@@ -29,7 +29,7 @@ namespace {
 constexpr int D = HEAD_DIM;
 static_assert(D == 64 || D == 128, "head sizes 64 and 128");
 constexpr int DH = D / 64;               // 64-wide halves of a head
-constexpr int BAR_BYTES = 384;           // of shared memory, for barriers
+constexpr int BAR_BYTES = 768;           // of shared memory, for two sets of barriers and the words behind them
 constexpr int BM = 128, BN = 128, HALF = 64;  // rows of a slot, keys of a tile, of the halves that are worked on
 // Seven tiles of shared memory: the rows (one tile where both slots hold the same, else two), the rest in stages of half a tile, as many for keys
 // as for values: five each that both slots read, or three each a slot where the slots take turns with the tiles.
@@ -85,7 +85,7 @@ struct Segment {
   int request, kvh, row0, rows, lo, hi;  // lo, hi: keys, as numbered; rows 0: nothing more
   bool whole, turns;
 };
-constexpr int TAIL_BYTES = 4 * BM * sizeof(float) + (sizeof(Segment) + 15) / 16 * 16;
+constexpr int TAIL_BYTES = 4 * BM * sizeof(float) + 2 * (sizeof(Segment) + 15) / 16 * 16;
 
 }  // namespace
 
@@ -99,23 +99,27 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_con
   }
   unsigned char* q_s = smem_raw;
   uint64_t* bars = reinterpret_cast<uint64_t*>(q_s + TILES * TILE_BYTES);
-  // bars: q_full | k_full[] | k_empty[] | v_full[] | v_empty[] | s_full[2][2] | p_full[2][2] | o_done[2][2] (slot, half) | began
+  // bars: q_full | k_full[] | k_empty[] | v_full[] | v_empty[] | s_full[2][2] | p_full[2][2] | o_done[2][2] (slot, half) | began; a set of them for
+  // every other segment, so that one is made while the other is in use
   constexpr int BARS = 1 + 4 * MOST_STAGES + 13;
-  static_assert(BARS * 8 + 24 <= BAR_BYTES, "barriers and the words behind them");
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + BARS);
+  static_assert(2 * BARS * 8 + 24 <= BAR_BYTES, "barriers and the words behind them");
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 2 * BARS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
   volatile int* by_hand = reinterpret_cast<volatile int*>(tmem_holder + 2);  // [2][2]: whether a slot's half has been summed without a product
   float* row_ml = reinterpret_cast<float*>(reinterpret_cast<unsigned char*>(bars) + BAR_BYTES);  // [2][128][2]: a slot's offset and sum, for the other one
-  Segment& s = *reinterpret_cast<Segment*>(row_ml + 4 * BM);
+  Segment* segments = reinterpret_cast<Segment*>(row_ml + 4 * BM);
   const int warp = omnia_warp_index(), lane = threadIdx.x & 31;
-  const uint32_t q_full = smem_u32(bars), k_full0 = q_full + 8, k_empty0 = k_full0 + 8 * MOST_STAGES, v_full0 = k_empty0 + 8 * MOST_STAGES,
-                 v_empty0 = v_full0 + 8 * MOST_STAGES, s_full0 = v_empty0 + 8 * MOST_STAGES, p_full0 = s_full0 + 32, o_done0 = p_full0 + 32,
-                 began = o_done0 + 32;
+  constexpr uint32_t K_FULL = 8, K_EMPTY = K_FULL + 8 * MOST_STAGES, V_FULL = K_EMPTY + 8 * MOST_STAGES, V_EMPTY = V_FULL + 8 * MOST_STAGES,
+                     S_FULL = V_EMPTY + 8 * MOST_STAGES, P_FULL = S_FULL + 32, O_DONE = P_FULL + 32, BEGAN = O_DONE + 32;
   if (warp == WARP_MMA) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)), "r"(TMEM_COLS));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
   }
-  if (threadIdx.x == 0) *abort_flag = 0;
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_kv) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_q) : "memory");
+  }
   // From here on what earlier kernels wrote is read; the launch is a programmatic dependent one.
   pdl_wait();
   pdl_launch_dependents();
@@ -130,55 +134,67 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_con
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem_base = *tmem_holder;
+  OMNIA_TRACE_BLOCK(2);  // the shares are known
   const int group = a.nq / a.nkv, slot_nodes = BM / group, slot_rows = slot_nodes * group;
 
   int stages = 1, issued = -1;  // of a ring; the last half tile that this warp has asked for
   uint32_t k_at = 0, v_at = 0;  // byte offsets of the rings in shared memory
+  const Segment* now = segments;
   // A slot's sequence of half tiles: half u is the (u & 1)th of the tile j0 + (u >> 1) * step.
   auto halves_of = [&](int j0) {
-    const int tiles = (s.hi - s.lo + BN - 1) / BN, step = s.turns ? 2 : 1;
+    const int tiles = (now->hi - now->lo + BN - 1) / BN, step = now->turns ? 2 : 1;
     const int mine = tiles > j0 ? (tiles - j0 + step - 1) / step : 0, last = j0 + (mine - 1) * step;
-    return mine < 1 ? 0 : 2 * mine - (s.hi - s.lo - last * BN <= HALF ? 1 : 0);
+    return mine < 1 ? 0 : 2 * mine - (now->hi - now->lo - last * BN <= HALF ? 1 : 0);
   };
-  auto first_of = [&](int j0, int u) { return s.lo + (j0 + (u >> 1) * (s.turns ? 2 : 1)) * BN + (u & 1) * HALF; };  // its first key
+  auto first_of = [&](int j0, int u) { return now->lo + (j0 + (u >> 1) * (now->turns ? 2 : 1)) * BN + (u & 1) * HALF; };  // its first key
   // Half u's stage, and the parity of the phase in which it is full.
-  auto stage_of = [&](int slot, int u) { return (s.turns ? slot * OWN_STAGES : 0) + u % stages; };
+  auto stage_of = [&](int slot, int u) { return (now->turns ? slot * OWN_STAGES : 0) + u % stages; };
   auto phase_of = [&](int u) { return (u / stages) & 1; };
-  // All warps go from segment to segment side by side: one of them makes the next, and the barriers anew, when all are done with the one before.
-  // -> whether there is one
-  bool made = false;
-  auto next_segment = [&]() {
-    block_sync();
-    if (warp == WARP_INIT && lane == 0) {
-      if (left > 0 && !*abort_flag) {
-        const int tiles = min(place.tiles - place.tile, left);
-        s.k = place.k, s.request = place.request, s.kvh = place.head;
-        s.row0 = place.row_tile * shares.rows, s.rows = min(shares.rows, place.k.count * group - s.row0);
-        s.lo = place.tile * BN, s.hi = min((place.tile + tiles) * BN, place.k.total);
-        s.whole = tiles == place.tiles, s.turns = s.rows <= slot_rows;
-        left -= tiles;
-        place.tile += tiles - 1;
-        if (left > 0) place.next(a, shares);
-        if (made)
-          for (int i = 0; i < BARS; ++i) mbar_inval(q_full + 8 * i);
-        mbar_init(q_full, 1);
-        const int readers = s.turns ? 1 : 2;
-        for (int i = 0; i < MOST_STAGES; ++i) mbar_init(k_full0 + 8 * i, 1), mbar_init(k_empty0 + 8 * i, readers);
-        for (int i = 0; i < MOST_STAGES; ++i) mbar_init(v_full0 + 8 * i, 1), mbar_init(v_empty0 + 8 * i, readers);
-        for (int i = 0; i < 4; ++i) mbar_init(s_full0 + 8 * i, 1), mbar_init(p_full0 + 8 * i, BM / 32), mbar_init(o_done0 + 8 * i, 1), by_hand[i] = 0;
-        mbar_init(began, BM / 32);
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      } else {
-        s.rows = 0;
-      }
-    }
-    block_sync();
-    if (s.rows == 0) return false;
-    made = true, issued = -1;
-    stages = s.turns ? OWN_STAGES : BOTH_STAGES;
-    k_at = (s.turns ? 1 : 2) * TILE_BYTES;
-    v_at = k_at + (s.turns ? MOST_STAGES : BOTH_STAGES) * STAGE_BYTES;
+  // All warps go from segment to segment side by side. One of them makes the next, and its barriers, while the others are at work.
+  int turn_of = -1;  // segments begun, less one
+  auto make_segment = [&](int which) {  // (a lane of the one warp)
+    Segment& n = segments[which & 1];
+    n.rows = 0;
+    if (left <= 0) return;
+    const int tiles = min(place.tiles - place.tile, left);
+    n.k = place.k, n.request = place.request, n.kvh = place.head;
+    n.row0 = place.row_tile * shares.rows;
+    n.lo = place.tile * BN, n.hi = min((place.tile + tiles) * BN, place.k.total);
+    const int rows = min(shares.rows, place.k.count * group - n.row0);
+    n.whole = tiles == place.tiles, n.turns = rows <= slot_rows;
+    left -= tiles;
+    place.tile += tiles - 1;
+    if (left > 0) place.next(a, shares);
+    const uint32_t set = smem_u32(bars) + (which & 1) * BARS * 8;
+    if (which > 1)
+      for (int i = 0; i < BARS; ++i) mbar_inval(set + 8 * i);
+    const int readers = n.turns ? 1 : 2;
+    mbar_init(set, 1);
+    for (int i = 0; i < MOST_STAGES; ++i) mbar_init(set + K_FULL + 8 * i, 1), mbar_init(set + K_EMPTY + 8 * i, readers);
+    for (int i = 0; i < MOST_STAGES; ++i) mbar_init(set + V_FULL + 8 * i, 1), mbar_init(set + V_EMPTY + 8 * i, readers);
+    for (int i = 0; i < 4; ++i) mbar_init(set + S_FULL + 8 * i, 1), mbar_init(set + P_FULL + 8 * i, BM / 32), mbar_init(set + O_DONE + 8 * i, 1);
+    mbar_init(set + BEGAN, BM / 32);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    n.rows = rows;
+  };
+  if (warp == WARP_INIT && lane == 0) {
+    for (int i = 0; i < 4; ++i) by_hand[i] = 0;
+    make_segment(0);
+  }
+  uint32_t q_full = 0, k_full0 = 0, k_empty0 = 0, v_full0 = 0, v_empty0 = 0, s_full0 = 0, p_full0 = 0, o_done0 = 0, began = 0;
+  auto next_segment = [&]() {  // -> whether there is one
+    block_sync();  // all are done with the one before
+    ++turn_of;
+    if (segments[turn_of & 1].rows == 0 || *abort_flag) return false;
+    issued = -1;
+    const bool turns = segments[turn_of & 1].turns;
+    stages = turns ? OWN_STAGES : BOTH_STAGES;
+    k_at = (turns ? 1 : 2) * TILE_BYTES;
+    v_at = k_at + (turns ? MOST_STAGES : BOTH_STAGES) * STAGE_BYTES;
+    q_full = smem_u32(bars) + (turn_of & 1) * BARS * 8;
+    k_full0 = q_full + K_FULL, k_empty0 = q_full + K_EMPTY, v_full0 = q_full + V_FULL, v_empty0 = q_full + V_EMPTY;
+    s_full0 = q_full + S_FULL, p_full0 = q_full + P_FULL, o_done0 = q_full + O_DONE, began = q_full + BEGAN;
     return true;
   };
 
@@ -186,6 +202,8 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_con
   else asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SLOT_REGS));
   if (warp >= WARP_MMA) {
     while (next_segment()) {
+      const Segment& s = segments[turn_of & 1];
+      now = &s;
       const int tiles = (s.hi - s.lo + BN - 1) / BN;
       if (warp == WARP_Q) {
         // ---- the rows' queries, a box the group's heads of a slot's nodes x 64 dims. The rows behind the last node are other requests' or zeros: no
@@ -241,6 +259,9 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_con
           issued = u;
           page_cur = page_next, key_cur = key_next;
         }
+      } else if (warp == WARP_INIT) {
+        if (lane == 0) make_segment(turn_of + 1);
+        __syncwarp();
       } else if (warp < WARP_K) {
         // ---- issuer of a slot's products -------------------------------------------------------------------------------
         const int slot = warp - WARP_MMA, j0 = s.turns ? slot : 0, halves = halves_of(j0);
@@ -295,6 +316,8 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_con
               if (ok) scores(u + 2);
             }
           }
+          // The last stage is free: this warp's products have told all barriers that wait for them, and the set may be made anew.
+          if (ok) wait_for(v_empty0 + 8 * stage_of(slot, halves - 1), phase_of(halves - 1), abort_flag);
         }
         __syncwarp();
       }
@@ -308,11 +331,14 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_con
     const float cap = a.softcap * LOG2E, twice = capped ? 2.f * a.scale / a.softcap * LOG2E : 0.f, unit = capped ? 1.f : a.scale * LOG2E;
     bool first = true;
     while (next_segment()) {
+      const Segment& s = segments[turn_of & 1];
+      now = &s;
       const int my_row = s.turns ? row : slot * slot_rows + row;   // among the segment's rows
       const bool live = row < slot_rows && my_row < s.rows;
       const int node = live ? (s.row0 + my_row) / group : 0, pos = a.positions[s.k.first + node], low = tree_low(a, pos);
       const int* sees = a.ancestors + (size_t)(s.k.first + node) * a.words;
       const int clear_from = tree_low(a, s.k.held + s.k.count - 1);  // what no row's window ends above
+      OMNIA_TRACE_BLOCK(3);  // a segment begins
       float m = -INFINITY, l = 0.f;  // the row's offset (log2 units), its sum against it
       bool ok = true;
       int done = 0;
@@ -324,29 +350,12 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_con
         const bool dry = u < 0;
         const int h = dry ? 0 : u & 1, t = u >> 1;
         const uint32_t half_addr = s_addr + h * HALF;
-        if (!dry) {
-          ok = __all_sync(0xffffffffu, wait_for(s_full0 + 8 * (2 * slot + h), t & 1, abort_flag));
-          if (!ok) break;
-        }
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const int x0 = dry ? 0 : first_of(j0, u), seen = dry ? HALF : min(HALF, s.hi - x0);  // keys of this half; the columns beyond hold whatever the stage held
         const bool clear = dry || (seen == HALF && x0 >= s.k.kept && s.k.key(x0) >= clear_from && s.k.key(x0 + HALF - 1) < s.k.held);
-        // All of the row's scores at once: a load from tensor memory takes some 0.35 us to arrive.
-        float z[HALF];
-        {
-          uint32_t raw[HALF];
-#pragma unroll
-          for (int c = 0; c < HALF; c += 32) tmem_load32(half_addr + c, raw + c);
-          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-          for (int c = 0; c < HALF; ++c) z[c] = __uint_as_float(raw[c]);
-        }
-        if (capped) {  // c tanh(x) = c - 2 c / (1 + e^2x), in log2 units (a score that is infinite has the cap, of its sign)
-#pragma unroll
-          for (int c = 0; c < HALF; ++c) z[c] = fmaf(-2.f * cap, fast_rcp(1.f + fast_exp2(z[c] * twice)), cap);
-        }
+        // What a row sees of a half that not all rows see all of, and whether one of its values is no number: asked for ahead of the scores.
+        uint32_t bits[2] = {~0u, ~0u};
+        bool odd = false;
         if (!clear) {
-          uint32_t bits[2];
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const int x = x0 + 32 * i, ends_at = s.hi - x;  // keys of these 32 that there are
@@ -367,6 +376,40 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_con
             }
             bits[i] = ends_at >= 32 ? b : ends_at > 0 ? b & ((1u << ends_at) - 1u) : 0u;
           }
+          const int st = stage_of(slot, u);
+          ok = __all_sync(0xffffffffu, wait_for(v_full0 + 8 * st, phase_of(u), abort_flag));
+          if (!ok) break;
+          const unsigned char* v = q_s + v_at + st * STAGE_BYTES;
+#pragma unroll
+          for (int side = 0; side < DH; ++side)
+#pragma unroll 4
+            for (int i = lane; i < seen * 8; i += 32) {
+              const uint4 x = *reinterpret_cast<const uint4*>(v + side * SIDE_BYTES + i * 16);
+              odd |= no_number(x.x) | no_number(x.y) | no_number(x.z) | no_number(x.w);
+            }
+          odd = __any_sync(0xffffffffu, odd);  // (the same for all of the slot's warps: the stage is what it is)
+        }
+        if (!dry) {
+          ok = __all_sync(0xffffffffu, wait_for(s_full0 + 8 * (2 * slot + h), t & 1, abort_flag));
+          if (!ok) break;
+          if (u == 0) OMNIA_TRACE_BLOCK(4);  // its first scores
+        }
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        // All of the row's scores at once: a load from tensor memory takes some 0.35 us to arrive.
+        float z[HALF];
+        {
+          uint32_t raw[HALF];
+#pragma unroll
+          for (int c = 0; c < HALF; c += 32) tmem_load32(half_addr + c, raw + c);
+          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+          for (int c = 0; c < HALF; ++c) z[c] = __uint_as_float(raw[c]);
+        }
+        if (capped) {  // c tanh(x) = c - 2 c / (1 + e^2x), in log2 units (a score that is infinite has the cap, of its sign)
+#pragma unroll
+          for (int c = 0; c < HALF; ++c) z[c] = fmaf(-2.f * cap, fast_rcp(1.f + fast_exp2(z[c] * twice)), cap);
+        }
+        if (!clear) {
 #pragma unroll
           for (int c = 0; c < HALF; ++c) z[c] = (bits[c / 32] >> (c % 32)) & 1u ? z[c] : -INFINITY;
         }
@@ -384,21 +427,6 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_con
             l *= alpha;
             m = top;
           }
-        }
-        // The values of a half that not all rows see all of: whether one is no number.
-        bool odd = false;
-        if (!clear) {
-          const int st = stage_of(slot, u);
-          ok = __all_sync(0xffffffffu, wait_for(v_full0 + 8 * st, phase_of(u), abort_flag));
-          if (!ok) break;
-          const unsigned char* v = q_s + v_at + st * STAGE_BYTES;
-#pragma unroll 1
-          for (int i = lane; i < seen * DH * 8; i += 32) {
-            const int side = i / (seen * 8), rest = i % (seen * 8);
-            const uint4 x = *reinterpret_cast<const uint4*>(v + side * SIDE_BYTES + rest * 16);
-            odd |= no_number(x.x) || no_number(x.y) || no_number(x.z) || no_number(x.w);
-          }
-          odd = __any_sync(0xffffffffu, odd);  // (the same for all of the slot's warps: the stage is what it is)
         }
         if (done > 0 && (odd || __any_sync(0xffffffffu, alpha != 1.f))) {
           // The products so far, the half before this one's among them, have to be done; the next one's wait for this warp.
@@ -485,6 +513,7 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_con
       // products are done behind the first barrier, and every load has landed, since products have read it), so that a warp writes a row at a time. ----
       if (ok && done > 0) ok = __all_sync(0xffffffffu, wait_for(o_done0 + 8 * (2 * slot + ((done - 1) & 1)), ((done - 1) >> 1) & 1, abort_flag));
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      OMNIA_TRACE_BLOCK(5);  // its last product
       constexpr int STRIDE = D + 4;  // floats: eight lanes' 16 bytes lie in different banks
       float* stage = reinterpret_cast<float*>(smem_raw) + (s.turns ? 0 : slot) * BM * STRIDE;
       static_assert(2 * BM * STRIDE * sizeof(float) <= TILES * TILE_BYTES, "both slots' rows fit where the tiles were");
@@ -538,24 +567,46 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_con
       // Rows out: a warp's own 32, or 16 of the rows that were both slots'.
       const int r0 = s.turns ? warp * 16 : quarter * 32, r1 = min(r0 + (s.turns ? 16 : 32), min(slot_rows, s.rows - (s.turns ? 0 : slot * slot_rows)));
       const int row_at = s.turns ? 0 : slot * slot_rows;
+      const bool mine = ok && lane < D / 4;
+      if (!s.whole) {
 #pragma unroll 4
-      for (int r = r0; r < r1; ++r) {
-        if (!ok || lane >= D / 4) continue;
-        const float4 y = reinterpret_cast<const float4*>(stage + r * STRIDE)[lane];
-        if (!s.whole) {
-          reinterpret_cast<float4*>(a.part_o + (part + row_at + r) * D)[lane] = y;
-          continue;
-        }
-        const int at = s.row0 + row_at + r, token = s.k.first + at / group, head = s.kvh * group + at % group;
-        float v[4] = {y.x, y.y, y.z, y.w};
-        if (a.gate) {
-          const bf16* gate = static_cast<const bf16*>(a.gate) + (size_t)token * a.gate_stride + head * D + 4 * lane;
+        for (int r = r0; r < r1; ++r)
+          if (mine) reinterpret_cast<float4*>(a.part_o + (part + row_at + r) * D)[lane] = reinterpret_cast<const float4*>(stage + r * STRIDE)[lane];
+      } else {
+        // A lane knows where the row that is as many behind the warp's first one goes.
+        const int at = s.row0 + row_at + min(r0 + lane, r1 - 1), my_token = s.k.first + at / group, my_head = s.kvh * group + at % group;
+        const bool pairs = ((reinterpret_cast<uintptr_t>(a.gate) | (uintptr_t)a.gate_stride * 2) & 7) == 0;
+#pragma unroll 1
+        for (int r = r0; r < r1; r += 4) {  // (four rows' gates on their way at once)
+          uint2 gates[4];
+          int tokens[4], heads[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) v[i] *= 1.f / (1.f + __expf(-__bfloat162float(gate[i])));
+          for (int i = 0; i < 4; ++i) {
+            tokens[i] = __shfl_sync(0xffffffffu, my_token, r - r0 + i), heads[i] = __shfl_sync(0xffffffffu, my_head, r - r0 + i);
+            if (a.gate && mine) {
+              const bf16* gate = static_cast<const bf16*>(a.gate) + (size_t)tokens[i] * a.gate_stride + heads[i] * D + 4 * lane;
+              if (pairs) {
+                gates[i] = *reinterpret_cast<const uint2*>(gate);
+              } else {
+                const unsigned short* g = reinterpret_cast<const unsigned short*>(gate);
+                gates[i] = make_uint2(g[0] | (uint32_t)g[1] << 16, g[2] | (uint32_t)g[3] << 16);
+              }
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (!mine || r + i >= r1) continue;
+            float4 y = reinterpret_cast<const float4*>(stage + (r + i) * STRIDE)[lane];
+            if (a.gate) {
+              y.x *= tree_sigmoid(__uint_as_float(gates[i].x << 16)), y.y *= tree_sigmoid(__uint_as_float(gates[i].x & 0xffff0000u));
+              y.z *= tree_sigmoid(__uint_as_float(gates[i].y << 16)), y.w *= tree_sigmoid(__uint_as_float(gates[i].y & 0xffff0000u));
+            }
+            *reinterpret_cast<uint2*>(static_cast<bf16*>(a.out) + ((size_t)tokens[i] * a.nq + heads[i]) * D + 4 * lane) =
+                make_uint2(pack_bf16(y.x, y.y), pack_bf16(y.z, y.w));
+          }
         }
-        *reinterpret_cast<uint2*>(static_cast<bf16*>(a.out) + (size_t)token * a.nq * D + head * D + 4 * lane) =
-            make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
       }
+      OMNIA_TRACE_BLOCK(6);  // its rows are out
       first = false;
     }
   }
@@ -566,11 +617,11 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_con
     // stage that the ring's other warp has filled since reads as not complete, so the wait is short.)
     const uint32_t full0 = warp >= WARP_V ? v_full0 : k_full0;
     const int turn = warp - (warp >= WARP_V ? WARP_V : WARP_K);
-    for (int u = issued; u >= 0 && u > issued - stages; u -= s.turns ? 1 : FEEDERS)
+    for (int u = issued; u >= 0 && u > issued - stages; u -= now->turns ? 1 : FEEDERS)
       for (uint32_t i = 0; i < WAIT_LIMIT / 1024 && !mbar_try(full0 + 8 * stage_of(turn, u), phase_of(u)); ++i) {
       }
   }
-  if (*abort_flag && warp == WARP_Q && lane == 0 && made)
+  if (*abort_flag && warp == WARP_Q && lane == 0 && q_full != 0)
     for (uint32_t i = 0; i < WAIT_LIMIT / 1024 && !mbar_try(q_full, 0); ++i) {
     }
   if (warp == WARP_MMA) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS));
