@@ -60,20 +60,25 @@ __device__ __forceinline__ int tree_low(const TreeAttention& a, int pos) {
 }
 
 // Equal shares of a step's work for the kernels that keep a fixed number of blocks busy. An item is a tile of rows of one request and one key/value
-// head; its keys come in tiles. All tiles of all items stand in one line (requests, then heads, then tiles of rows, then of keys), of which block
-// b takes [b T / G, (b + 1) T / G): contexts of unequal lengths cost no block more than another, and since lengths are read here, a captured
-// step has its shares right at every replay. An item that several blocks have part in is put together by the merge: block b leaves
-// what its first item came to in slot 2 b, and what its last one did in slot 2 b + 1.
+// head; its keys come in tiles. All tiles of all items stand in one line (requests, then heads, then tiles of rows, then of keys), ahead of each
+// item's as many empty places as its beginning and end cost in tiles, and block b takes [b T / G, (b + 1) T / G) of the T places: contexts of unequal lengths
+// cost no block more than another, and since lengths are read here, a captured step has its shares right at every replay. An item that several
+// blocks have part in is put together by the join: block b leaves in slot 2 b what the item came to that the block begins in (or ahead of, in its empty
+// places), and in slot 2 b + 1 what its last one did.
 constexpr int TREE_MOST_REQUESTS = 1024;
 
 struct TreeShares {
-  int rows, keys, align;  // of a tile, and of `tree_keys`
+  int rows, keys, align, extra;  // rows and keys of a tile; of `tree_keys`; empty places ahead of an item
   __device__ __forceinline__ int row_tiles(const TreeAttention& a, const TreeKeys& k) const {
     return k.total > 0 ? (k.count * (a.nq / a.nkv) + rows - 1) / rows : 0;
   }
   __device__ __forceinline__ int key_tiles(const TreeKeys& k) const { return (k.total + keys - 1) / keys; }
 
-  // ends[r]: tiles of all requests up to r, r among them (shared memory, of the whole block); -> tiles in all. `sums`: a word a warp.
+  __device__ __forceinline__ long long places(const TreeAttention& a, const TreeKeys& k) const {
+    return k.total > 0 ? (long long)row_tiles(a, k) * (key_tiles(k) + extra) * a.nkv : 0;
+  }
+
+  // ends[r]: places of all requests up to r, r among them (shared memory, of the whole block); -> places in all. `sums`: a word a warp.
   __device__ __forceinline__ long long lay_out(const TreeAttention& a, long long* ends, long long* sums) const {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     long long before = 0;
@@ -81,8 +86,7 @@ struct TreeShares {
       const int r = r0 + threadIdx.x;
       long long mine = 0;
       if (r < a.requests) {
-        const TreeKeys k = tree_keys(a, r, align);
-        mine = (long long)row_tiles(a, k) * key_tiles(k) * a.nkv;
+        mine = places(a, tree_keys(a, r, align));
       }
 #pragma unroll
       for (int o = 1; o < 32; o *= 2) {
@@ -103,16 +107,17 @@ struct TreeShares {
   }
 };
 
-// A place in that line.
+// A tile in that line, and how many places from it on are the block's (0: there is none).
 struct TreePlace {
-  int request, head, row_tile, tile, row_tiles, tiles;
+  int request, head, row_tile, tile, row_tiles, tiles, left;
   TreeKeys k;
   __device__ __forceinline__ void enter(const TreeAttention& a, const TreeShares& s, int r) {
     request = r;
     k = tree_keys(a, r, s.align);
     row_tiles = s.row_tiles(a, k), tiles = s.key_tiles(k);
   }
-  __device__ __forceinline__ void find(const TreeAttention& a, const TreeShares& s, const long long* ends, long long at) {
+  // The first tile of the `share` places from `at` on. -> where its item's places begin
+  __device__ __forceinline__ long long find(const TreeAttention& a, const TreeShares& s, const long long* ends, long long at, int share) {
     int lo = 0, hi = a.requests - 1;
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
@@ -120,15 +125,21 @@ struct TreePlace {
     }
     enter(a, s, lo);
     const long long in = at - (lo ? ends[lo - 1] : 0);
-    const int each = row_tiles * tiles;
+    const int item = tiles + s.extra, each = row_tiles * item;
     head = (int)(in / each);
     const int rest = (int)(in % each);
-    row_tile = rest / tiles, tile = rest % tiles;
+    row_tile = rest / item, tile = rest % item - s.extra;
+    const long long begin = at - (tile + s.extra);
+    left = share;
+    if (tile < 0) left = max(left + tile, 0), tile = 0;
+    return begin;
   }
-  // To the next tile, which there is.
-  __device__ __forceinline__ void next(const TreeAttention& a, const TreeShares& s) {
-    if (++tile < tiles) return;
-    tile = 0;
+  // `count` tiles on, to the next item at most.
+  __device__ __forceinline__ void next(const TreeAttention& a, const TreeShares& s, int count = 1) {
+    left -= count, tile += count;
+    if (tile < tiles) return;
+    left = max(left - s.extra, 0), tile = 0;
+    if (left == 0) return;
     if (++row_tile < row_tiles) return;
     row_tile = 0;
     if (++head < a.nkv) return;
@@ -178,22 +189,22 @@ __global__ void __launch_bounds__(32 * TREE_JOIN_WARPS) tree_join_kernel(const _
   const long long total = shares.lay_out(a, ends, sums), blocks = min((long long)grid, total);
   const int border = blockIdx.x + 1;
   if (border >= blocks) return;
-  // Tile t is block b's where b T / G <= t < (b + 1) T / G.
   const long long at = total * border / blocks;
   TreePlace place;
-  place.find(a, shares, ends, at);
-  const long long begin = at - place.tile, end = begin + place.tiles;
-  if (begin == at || begin < total * (border - 1) / blocks) return;  // no border in an item, or not its first
+  const long long begin = place.find(a, shares, ends, at, 1), first = begin + shares.extra, end = first + place.tiles;  // `first`: its first tile's
+  if (first >= at || first < total * (border - 1) / blocks) return;  // no border between tiles, or not the item's first
   const int b0 = border - 1;
   int b1 = border;
   while (total * (b1 + 1) / blocks < end) ++b1;
-  // The item is the first of all blocks that have part in it but the one that it begins in, unless it begins that too.
-  const int slot0 = 2 * b0 + (begin == total * b0 / blocks ? 0 : 1);
+  // The block that the item begins in may have begun in another item, the others have begun in this one.
+  const int slot0 = 2 * b0 + (begin <= total * b0 / blocks ? 0 : 1);
   auto slot_of = [&](int b) { return b == b0 ? slot0 : 2 * b; };
   const TreeKeys& k = place.k;
   const int head_kv = place.head, here = min(rows_of_tile, k.count * group - place.row_tile * rows_of_tile);
+  OMNIA_TRACE_BLOCK(2);
   pdl_wait();
   pdl_launch_dependents();
+  OMNIA_TRACE_BLOCK(3);
   for (int r = blockIdx.y * WARPS + warp; r < here; r += step) {
     const int in = place.row_tile * rows_of_tile + r;
     const int token = k.first + in / group, head = head_kv * group + in % group;
@@ -249,6 +260,7 @@ __global__ void __launch_bounds__(32 * TREE_JOIN_WARPS) tree_join_kernel(const _
       *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + (size_t)token * a.nq * D + head * D + c) = make_uint2(tree_pair(y[0], y[1]), tree_pair(y[2], y[3]));
     }
   }
+  OMNIA_TRACE_BLOCK(7);  // the rows are out
 }
 
 template <int D>

@@ -25,6 +25,7 @@ constexpr int DP = (D + 15) / 16 * 16, ROW = DP + 8;  // padded head size; share
 constexpr int CH = D / 8, KSTEPS = DP / 16, NT_O = DP / 8;
 constexpr int KEYS = 64, WARPS = 4, THREADS = 32 * WARPS, WARP_LOADS = KEYS / WARPS;  // keys whose rows a warp fetches
 constexpr int STAGES = D <= 128 ? 3 : 2;
+constexpr int EXTRA = 3;                              // tiles that an item's beginning and end cost
 constexpr int STAGE = 2 * KEYS * ROW;                 // elements: keys, then values
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float RESCALE_STEP = 8.f;  // log2 of how far a row's maximum may outgrow its exponent's offset
@@ -86,25 +87,26 @@ __global__ void __launch_bounds__(THREADS, D <= 128 ? 2 : 1) tree_shares_kernel(
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, wr = warp % WR, wk = warp / WR, g = lane >> 2, t4 = lane & 3;
   pdl_wait();
   pdl_launch_dependents();
-  const TreeShares shares = {ROWS, KEYS, 1};
+  const TreeShares shares = {ROWS, KEYS, 1, EXTRA};
   const long long total = shares.lay_out(a, ends, sums);
   const long long blocks = min((long long)gridDim.x, total);  // (a block more than there are tiles would leave its slots unwritten)
   if (blockIdx.x >= blocks) return;
-  const long long t0 = total * blockIdx.x / blocks, t1 = total * (blockIdx.x + 1) / blocks;
+  const long long t0 = total * blockIdx.x / blocks;
   const int group = a.nq / a.nkv;
   const bf16 *kp = static_cast<const bf16*>(a.k_pages), *vp = static_cast<const bf16*>(a.v_pages);
   const long long apart = vp - kp;
 
   // ---- loads: lane l < 16 knows where the l-th row of its warp's share of a tile lies ------------------------------------------------
   TreePlace ahead;
-  ahead.find(a, shares, ends, t0);
+  ahead.find(a, shares, ends, t0, (int)(total * (blockIdx.x + 1) / blocks - t0));
+  if (ahead.left == 0) return;
   TreePlace now = ahead;
+  OMNIA_TRACE_BLOCK(2);  // the shares are known
   __syncthreads();
   if constexpr (D != DP) {  // the columns beyond a row: no load writes them
     for (int i = tid; i < STAGES * 2 * KEYS; i += THREADS) *reinterpret_cast<uint4*>(stages + i * ROW + D) = make_uint4(0u, 0u, 0u, 0u);
   }
-  const int share = (int)(t1 - t0);
-  int loaded = 0, load_stage = 0;  // tiles asked for
+  int load_stage = 0;
   auto where = [&]() -> long long {  // of this lane's key of the place `ahead`: elements from the pages' beginning; -1: none
     const int x = ahead.tile * KEYS + warp * WARP_LOADS + lane;
     if (lane >= WARP_LOADS || x >= ahead.k.total) return -1;
@@ -118,7 +120,7 @@ __global__ void __launch_bounds__(THREADS, D <= 128 ? 2 : 1) tree_shares_kernel(
   };
   long long row_at = where();
   auto fetch = [&]() {  // the tile at `ahead`, into the next stage; then on
-    if (loaded < share) {
+    if (ahead.left > 0) {
       bf16* k_s = stages + load_stage * STAGE + warp * WARP_LOADS * ROW;
       if (++load_stage == STAGES) load_stage = 0;
       bf16* v_s = k_s + KEYS * ROW;
@@ -133,10 +135,8 @@ __global__ void __launch_bounds__(THREADS, D <= 128 ? 2 : 1) tree_shares_kernel(
           cp_async16(v_s + row * ROW + c * 8, at + apart, from >= 0);
         }
       }
-      if (++loaded < share) {
-        ahead.next(a, shares);
-        row_at = where();
-      }
+      ahead.next(a, shares);
+      if (ahead.left > 0) row_at = where();
     }
     cp_async_commit();
   };
@@ -152,7 +152,8 @@ __global__ void __launch_bounds__(THREADS, D <= 128 ? 2 : 1) tree_shares_kernel(
   int node[2], low[2];
   bool first = true, entered = true;
   int stage = 0;
-  for (int t = 0; t < share; ++t) {
+  const bool halfway = now.tile > 0;  // whether the first item began in another block
+  while (now.left > 0) {
     const int rows = now.k.count * group, row0 = now.row_tile * ROWS + 16 * wr;
     if (entered) {
 #pragma unroll
@@ -175,6 +176,7 @@ __global__ void __launch_bounds__(THREADS, D <= 128 ? 2 : 1) tree_shares_kernel(
     }
     cp_async_wait<STAGES - 2>();
     __syncthreads();
+    if (first) OMNIA_TRACE_BLOCK(4);  // a first tile is there
     fetch();
     const bf16* k_s = stages + stage * STAGE + wk * KW * ROW;
     if (++stage == STAGES) stage = 0;
@@ -295,10 +297,11 @@ __global__ void __launch_bounds__(THREADS, D <= 128 ? 2 : 1) tree_shares_kernel(
           mma_bf16(o[n + 1], pf[ks], b[2], b[3]);
         }
     }
-    if (now.tile + 1 < now.tiles && t + 1 < share) {
-      ++now.tile;
+    if (now.tile + 1 < now.tiles && now.left > 1) {
+      ++now.tile, --now.left;
       continue;
     }
+    OMNIA_TRACE_BLOCK(5);  // an item's last product
     // ---- the item's end in this block: the warps that shared the keys, then the slot or the answer ------------------------------------
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -346,7 +349,7 @@ __global__ void __launch_bounds__(THREADS, D <= 128 ? 2 : 1) tree_shares_kernel(
     }
     if (wk == 0) {
       // The whole item is this block's where it begins and ends here.
-      const bool begins = !first || t >= now.tile, whole = begins && now.tile + 1 == now.tiles;
+      const bool whole = !(first && halfway) && now.tile + 1 == now.tiles;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         if (!whole) {
@@ -380,8 +383,9 @@ __global__ void __launch_bounds__(THREADS, D <= 128 ? 2 : 1) tree_shares_kernel(
           }
       }
     }
+    OMNIA_TRACE_BLOCK(6);  // its rows are out
     first = false, entered = true;
-    if (t + 1 < share) now.next(a, shares);
+    now.next(a, shares);
   }
 }
 
@@ -420,5 +424,5 @@ extern "C" int omnia_tree_attention_tc(const TreeAttention* a, int most_nodes, i
 #endif
   else return (int)cudaErrorInvalidValue;
   if (code) return code;
-  return tree_join<D>(*a, {rows, KEYS, 1}, most_nodes, blocks, s);
+  return tree_join<D>(*a, {rows, KEYS, 1, EXTRA}, most_nodes, blocks, s);
 }

@@ -30,6 +30,7 @@ constexpr int D = HEAD_DIM;
 static_assert(D == 64 || D == 128, "head sizes 64 and 128");
 constexpr int DH = D / 64;               // 64-wide halves of a head
 constexpr int BAR_BYTES = 768;           // of shared memory, for two sets of barriers and the words behind them
+constexpr int EXTRA = 5;                 // tiles that an item's beginning and end cost
 constexpr int BM = 128, BN = 128, HALF = 64;  // rows of a slot, keys of a tile, of the halves that are worked on
 // Seven tiles of shared memory: the rows (one tile where both slots hold the same, else two), the rest in stages of half a tile, as many for keys
 // as for values: five each that both slots read, or three each a slot where the slots take turns with the tiles.
@@ -126,10 +127,12 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_con
   long long* ends = reinterpret_cast<long long*>(smem_raw);
   const long long total = shares.lay_out(a, ends, ends + TREE_MOST_REQUESTS);
   const long long blocks = min((long long)gridDim.x, total);
-  const long long t0 = blockIdx.x < blocks ? total * blockIdx.x / blocks : 0, t1 = blockIdx.x < blocks ? total * (blockIdx.x + 1) / blocks : 0;
-  int left = (int)(t1 - t0);
   TreePlace place;  // (one warp's)
-  if (left > 0 && warp == WARP_INIT) place.find(a, shares, ends, t0);
+  place.left = 0;
+  if (blockIdx.x < blocks && warp == WARP_INIT) {
+    const long long t0 = total * blockIdx.x / blocks;
+    place.find(a, shares, ends, t0, (int)(total * (blockIdx.x + 1) / blocks - t0));
+  }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -155,16 +158,14 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_con
   auto make_segment = [&](int which) {  // (a lane of the one warp)
     Segment& n = segments[which & 1];
     n.rows = 0;
-    if (left <= 0) return;
-    const int tiles = min(place.tiles - place.tile, left);
+    if (place.left == 0) return;
+    const int tiles = min(place.tiles - place.tile, place.left);
     n.k = place.k, n.request = place.request, n.kvh = place.head;
     n.row0 = place.row_tile * shares.rows;
     n.lo = place.tile * BN, n.hi = min((place.tile + tiles) * BN, place.k.total);
     const int rows = min(shares.rows, place.k.count * group - n.row0);
     n.whole = tiles == place.tiles, n.turns = rows <= slot_rows;
-    left -= tiles;
-    place.tile += tiles - 1;
-    if (left > 0) place.next(a, shares);
+    place.next(a, shares, tiles);
     const uint32_t set = smem_u32(bars) + (which & 1) * BARS * 8;
     if (which > 1)
       for (int i = 0; i < BARS; ++i) mbar_inval(set + 8 * i);
@@ -455,7 +456,7 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_con
           sums[c & 2] += p0, sums[(c & 2) + 1] += p1;
           packed[c / 2] = pack_bf16(p0, p1);
         }
-        if (!odd) tmem_store32(dry ? o_addr : half_addr, packed);
+        tmem_store32(dry ? o_addr : half_addr, packed);
         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         if (dry) {
           m = -INFINITY, l = 0.f;
@@ -463,7 +464,7 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_con
         }
         l += (sums[0] + sums[1]) + (sums[2] + sums[3]);
         if (odd) {
-          // The half by hand: a row's own sums over the keys that have a weight, eight dims at a time.
+          // The half by hand: a row's own sums over the keys that have a weight, eight dims and sixteen keys at a time.
           const unsigned char* v = q_s + v_at + stage_of(slot, u) * STAGE_BYTES;
 #pragma unroll 1
           for (int c = 0; c < D; c += 8) {
@@ -475,15 +476,24 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_con
 #pragma unroll
               for (int i = 0; i < 8; ++i) o[i] = 0u;
             }
+#pragma unroll 1
+            for (int k0 = 0; k0 < seen; k0 += 16) {
+              uint32_t pairs[8];
+              tmem_load8(half_addr + k0 / 2, pairs);
+              asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll 1
+              for (int k = 0; k < 16; ++k) {
+                uint32_t two = pairs[0];
 #pragma unroll
-            for (int k = 0; k < HALF; ++k) {
-              const float p = __uint_as_float(k & 1 ? packed[k / 2] & 0xffff0000u : packed[k / 2] << 16);
-              if (k < seen && p != 0.f) {
-                const uint4 x = *reinterpret_cast<const uint4*>(v + c / 64 * SIDE_BYTES + k * 128 + ((c / 8 % 8) ^ (k & 7)) * 16);
-                const uint32_t pairs[4] = {x.x, x.y, x.z, x.w};
+                for (int i = 1; i < 8; ++i) two = k / 2 == i ? pairs[i] : two;
+                const float p = __uint_as_float(k & 1 ? two & 0xffff0000u : two << 16);
+                if (k0 + k < seen && p != 0.f) {
+                  const uint4 x = *reinterpret_cast<const uint4*>(v + c / 64 * SIDE_BYTES + (k0 + k) * 128 + ((c / 8 % 8) ^ (k & 7)) * 16);
+                  const uint32_t values[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                  o[i] = __float_as_uint(fmaf(p, __uint_as_float(i & 1 ? pairs[i / 2] & 0xffff0000u : pairs[i / 2] << 16), __uint_as_float(o[i])));
+                  for (int i = 0; i < 8; ++i)
+                    o[i] = __float_as_uint(fmaf(p, __uint_as_float(i & 1 ? values[i / 2] & 0xffff0000u : values[i / 2] << 16), __uint_as_float(o[i])));
+                }
               }
             }
             tmem_store8(o_addr + c, o);
@@ -665,7 +675,7 @@ extern "C" int omnia_tree_attention_tcgen05(const TreeAttention* given, int most
     if (e != cudaSuccess) return (int)e;
     configured[device] = true;
   }
-  const TreeShares shares = {omnia_tree_tcgen05_rows(group), BN, 16};
+  const TreeShares shares = {omnia_tree_tcgen05_rows(group), BN, 16, EXTRA};
   const cudaError_t e = launch_pdl(tree_tcgen05_kernel, dim3(blocks), THREADS, smem, stream, map_kv, map_q, a, shares);
   if (e != cudaSuccess) return (int)e;
   return tree_join<D>(a, shares, most_nodes, blocks, stream);
