@@ -170,9 +170,10 @@ __device__ __forceinline__ unsigned tree_pair(float lo, float hi) {
 // An item that several blocks had part in, put together by the blocks of the grid that stand for the first border in it (between block x and block
 // x + 1 of the kernel before): a warp a row at a time, the slots in the order of their blocks, the sink, the gate. The last `requests` blocks
 // write zeros for requests that see nothing. The rows of an item are shared out over the grid's other axis.
-template <int D>
+template <typename T, int MOST>
 __global__ void __launch_bounds__(32 * TREE_JOIN_WARPS) tree_join_kernel(const __grid_constant__ TreeAttention a, const TreeShares shares, int grid, int most) {
   constexpr int WARPS = TREE_JOIN_WARPS;
+  const int D = a.d;  // a multiple of 4, MOST at most
   constexpr float LOG2E = 1.4426950408889634f;
   __shared__ long long ends[TREE_MOST_REQUESTS], sums[WARPS];
   // (What is read ahead of the wait was there ahead of the kernel that this one waits for.)
@@ -183,7 +184,7 @@ __global__ void __launch_bounds__(32 * TREE_JOIN_WARPS) tree_join_kernel(const _
     if (k.total > 0) return;
     pdl_wait();
     for (int r = blockIdx.y * WARPS + warp; r < k.count * a.nq; r += step)
-      for (int c = lane; c < D; c += 32) static_cast<__nv_bfloat16*>(a.out)[((size_t)k.first * a.nq + r) * D + c] = __float2bfloat16_rn(0.f);
+      for (int c = lane; c < D; c += 32) static_cast<T*>(a.out)[((size_t)k.first * a.nq + r) * D + c] = from_f32<T>(0.f);
     return;
   }
   const long long total = shares.lay_out(a, ends, sums), blocks = min((long long)grid, total);
@@ -209,7 +210,7 @@ __global__ void __launch_bounds__(32 * TREE_JOIN_WARPS) tree_join_kernel(const _
     const int in = place.row_tile * rows_of_tile + r;
     const int token = k.first + in / group, head = head_kv * group + in % group;
     const float sink = a.sink ? a.sink[head] * LOG2E : -INFINITY;
-    constexpr int PER = (D + 127) / 128;  // four dims a lane
+    constexpr int PER = (MOST + 127) / 128;  // four dims a lane
     float4 sum[PER];
 #pragma unroll
     for (int i = 0; i < PER; ++i) sum[i] = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -246,7 +247,7 @@ __global__ void __launch_bounds__(32 * TREE_JOIN_WARPS) tree_join_kernel(const _
     }
     const float over = fmaxf(base, sink), offset = over == -INFINITY ? 0.f : over, f = tree_exp2(base - offset);
     l = l * f + tree_exp2(sink - offset);
-    const float by = l > 0.f ? f / l : 0.f;
+    const float by = l > 0.f || l != l ? f / l : 0.f;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int c = (32 * i + lane) * 4;
@@ -255,18 +256,20 @@ __global__ void __launch_bounds__(32 * TREE_JOIN_WARPS) tree_join_kernel(const _
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         if (by == 0.f) y[j] = 0.f;
-        if (a.gate) y[j] *= tree_sigmoid(__bfloat162float(static_cast<const __nv_bfloat16*>(a.gate)[(size_t)token * a.gate_stride + head * D + c + j]));
+        if (a.gate) y[j] *= tree_sigmoid(to_f32(static_cast<const T*>(a.gate)[(size_t)token * a.gate_stride + head * D + c + j]));
       }
-      *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + (size_t)token * a.nq * D + head * D + c) = make_uint2(tree_pair(y[0], y[1]), tree_pair(y[2], y[3]));
+      T* to = static_cast<T*>(a.out) + (size_t)token * a.nq * D + head * D + c;
+      if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(to) = make_uint2(tree_pair(y[0], y[1]), tree_pair(y[2], y[3]));
+      else *reinterpret_cast<float4*>(to) = make_float4(y[0], y[1], y[2], y[3]);
     }
   }
   OMNIA_TRACE_BLOCK(7);  // the rows are out
 }
 
-template <int D>
+template <typename T, int MOST>
 int tree_join(const TreeAttention& a, const TreeShares& shares, int most_nodes, int blocks, cudaStream_t stream) {
   const int rows = min(shares.rows, most_nodes * (a.nq / a.nkv));
   const dim3 grid(blocks - 1 + a.requests, min((rows + TREE_JOIN_WARPS - 1) / TREE_JOIN_WARPS, 16));
-  launch_pdl(tree_join_kernel<D>, grid, dim3(32 * TREE_JOIN_WARPS), 0, stream, a, shares, blocks, most_nodes);
+  launch_pdl(tree_join_kernel<T, MOST>, grid, dim3(32 * TREE_JOIN_WARPS), 0, stream, a, shares, blocks, most_nodes);
   return OMNIA_LAUNCH_RESULT();
 }

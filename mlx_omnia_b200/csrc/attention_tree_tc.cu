@@ -367,7 +367,7 @@ __global__ void __launch_bounds__(THREADS, D <= 128 ? 2 : 1) tree_shares_kernel(
           const float z = a.sink[head] * LOG2E, base = fmaxf(m[h], z);
           f = fast_exp2(m[h] - base), over = l[h] * f + fast_exp2(z - base);
         }
-        const float by = over > 0.f ? f / over : 0.f;
+        const float by = over > 0.f || over != over ? f / over : 0.f;
         bf16* out = static_cast<bf16*>(a.out) + (size_t)token * a.nq * D + head * D;
         const bf16* gate = a.gate ? static_cast<const bf16*>(a.gate) + (size_t)token * a.gate_stride + head * D : nullptr;
 #pragma unroll
@@ -424,5 +424,5 @@ extern "C" int omnia_tree_attention_tc(const TreeAttention* a, int most_nodes, i
 #endif
   else return (int)cudaErrorInvalidValue;
   if (code) return code;
-  return tree_join<D>(*a, {rows, KEYS, 1, EXTRA}, most_nodes, blocks, s);
+  return tree_join<bf16, D>(*a, {rows, KEYS, 1, EXTRA}, most_nodes, blocks, s);
 }

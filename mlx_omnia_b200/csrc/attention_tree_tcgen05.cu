@@ -678,5 +678,5 @@ extern "C" int omnia_tree_attention_tcgen05(const TreeAttention* given, int most
   const TreeShares shares = {omnia_tree_tcgen05_rows(group), BN, 16, EXTRA};
   const cudaError_t e = launch_pdl(tree_tcgen05_kernel, dim3(blocks), THREADS, smem, stream, map_kv, map_q, a, shares);
   if (e != cudaSuccess) return (int)e;
-  return tree_join<D>(a, shares, most_nodes, blocks, stream);
+  return tree_join<bf16, D>(a, shares, most_nodes, blocks, stream);
 }

@@ -1482,8 +1482,8 @@ _TREE = struct.Struct("14Pq16i2f")  # TreeAttention in attention_tree.cuh
 @functools.lru_cache(maxsize=4096)
 def tree_plan(tiles: int, keys: int, step: int, places: int) -> tuple[int, int]:
     """(keys a block walks, blocks to a tile of rows) of attention over `keys` keys by `tiles` tiles of rows, in chunks of a multiple of `step` keys: as many
-    blocks as have a place at a time, no chunk shorter than four steps."""
-    parts = max(1, min(places // max(tiles, 1), -(-keys // (4 * step))))
+    blocks as have a place at a time."""
+    parts = max(1, min(places // max(tiles, 1), -(-keys // step)))
     chunk = -(-keys // (parts * step)) * step
     return chunk, -(-keys // chunk)
 
@@ -1549,6 +1549,7 @@ def tree_attention(q: torch.Tensor, kv: KVView, step: StepContext, scale: float,
     q_ptr, sms = q.data_ptr(), sm_count(device)
     tensor_cores = dv == d and dtype is torch.bfloat16 and d % 8 == 0 and d <= 256 and n <= 1024 and not k_ptr & 15 and not q_ptr & 3
     many = tensor_cores and rows >= TREE_MANY_ROWS and d in (64, 128) and kv.page_size % 16 == 0 and scale > 0 and not q_ptr & 15 and nq // nkv <= 128
+    shares32 = dv == d and dtype is torch.float32 and d % 4 == 0 and d <= 256 and n <= 1024 and not (k_ptr | v_ptr) & 15 and page_stride % 4 == 0
     if many:
         tile = 2 * (128 // (nq // nkv) * (nq // nkv))
         a_chunk, a_parts = 0, min(sms, n * nkv * -(-rows // tile) * -(-keys // 128))
@@ -1557,6 +1558,10 @@ def tree_attention(q: torch.Tensor, kv: KVView, step: StepContext, scale: float,
         tile = 16 if rows <= 16 else 32 if rows <= 32 or d > 128 else 64
         a_chunk, a_parts = 0, min((2 if d <= 128 else 1) * sms, n * nkv * -(-rows // tile) * -(-keys // 64))
         slots = 2 * a_parts * tile
+    elif shares32:
+        places = 4 if d <= 32 else 2 if d <= 128 else 1
+        a_chunk, a_parts = 0, min(places * sms, n * nkv * -(-rows // 32) * -(-keys // (64 if d <= 64 else 32)))
+        slots = 2 * a_parts * 32
     else:
         a_chunk, a_parts = tree_plan(-(-rows // 32) * n * nkv, keys, 64, 2 * sms)
         slots = a_parts * tokens * nq if a_parts > 1 else 0
@@ -1573,6 +1578,9 @@ def tree_attention(q: torch.Tensor, kv: KVView, step: StepContext, scale: float,
     if tensor_cores:
         fn = _entry("attention_tree_tc", "omnia_tree_attention_tc", [c_void_p, c_int, c_int, c_int, c_void_p], {"HEAD_DIM": d})
         _check(fn(packed, most, tile, a_parts, stream), what)
+        return out
+    if shares32:
+        _check(_entry("attention_tree", "omnia_tree_attention32", [c_void_p, c_int, c_int, c_void_p])(packed, most, a_parts, stream), what)
         return out
     _check(_entry("attention_tree", "omnia_tree_attention", [c_void_p, c_int, c_int, c_void_p])(packed, most, code, stream), what)
     if a_parts > 1:
