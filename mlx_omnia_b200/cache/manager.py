@@ -141,6 +141,7 @@ class RequestCache:
     # so that a step lays its block tables out with array copies instead of Python loops
     arrays: list[np.ndarray] = field(default_factory=list)
     runs: list[SharedRun] = field(default_factory=list)  # what it shares with others, shortest first
+    drafted: int = 0  # of its tokens, how many the last step brought as drafts of which none is kept yet
 
     def table_array(self, group: int) -> np.ndarray:
         return self.arrays[group][: len(self.tables[group])]
@@ -306,6 +307,8 @@ class CacheManager:
 
     def why_not_fork(self, request: RequestCache, positions: int) -> str | None:
         """Why `request` cannot be forked at `positions` (None: it can; pages and slots may still be short)."""
+        if request.drafted:
+            return f"request {request.request_id!r} holds drafted tokens that are not kept yet"
         if not 1 <= positions <= request.tokens:
             return f"a fork takes between 1 and the {request.tokens} positions that request {request.request_id!r} holds, not {positions}"
         # (The page that they end in is the fork's to write on, so its first rows have to be there. None is given back while it can be written to.)

@@ -15,7 +15,7 @@ from __future__ import annotations
 import dataclasses
 import itertools
 import secrets
-from collections.abc import Iterator, Sequence
+from collections.abc import Iterator, Mapping, Sequence
 from dataclasses import dataclass
 from pathlib import Path
 
@@ -26,7 +26,7 @@ from mlx_omnia_b200.engine.meter import Meter
 from mlx_omnia_b200.engine.scheduler import PlannedEntry, Request, Scheduler, StepOutput, StepPlan
 from mlx_omnia_b200.engine.step import StepEntry
 from mlx_omnia_b200.kernels import ops
-from mlx_omnia_b200.sampling.batch import sample_rows
+from mlx_omnia_b200.sampling.batch import allowed_ids, sample_drafted, sample_rows, text_of
 from mlx_omnia_b200.sampling.options import GenerationOptions
 from mlx_omnia_b200.text.bpe import Detokenizer
 from mlx_omnia_b200.text.defaults import GenerationDefaults
@@ -106,6 +106,8 @@ class Generator:
         vocab = self.engine.vocab_size
         if any(not 0 <= t < vocab for t in prompt):
             raise ValueError(f"a prompt token lies outside the vocabulary of {vocab}")
+        if any(token >= vocab for token in options.bias or ()):
+            raise ValueError(f"a bias names a token outside the vocabulary of {vocab}")
         budget = options.max_tokens
         if options.context_limit is not None:
             budget = min(budget, options.context_limit - len(prompt))
@@ -143,21 +145,14 @@ class Generator:
             tokens = [0] * planned.count if device_tokens is not None else \
                 planned.request.token_slice(planned.start, planned.count)
             entries.append(StepEntry(planned.request.cache, tokens, [planned.count - 1] if planned.samples else []))
+        sampling = [p.request for p in plan.entries if p.samples]
         try:
             logits = self.engine.runner.run(entries, copy=False, device_tokens=device_tokens)
+            chosen = self._choose(logits, sampling, 1 if device_tokens is not None else 0) if sampling else None
         except Exception:
             for planned in plan.entries:  # a failed step fails its requests and frees what they hold
                 self.scheduler._finish(planned.request, "abort")
             raise
-        sampling = [p.request for p in plan.entries if p.samples]
-        chosen = None
-        if sampling:
-            ahead = 1 if device_tokens is not None else 0  # draws already spent by the step not yet committed
-            histories = [r.token_slice(max(0, len(r.prompt) + len(r.generated) - r.sampling.penalty_context),
-                                       r.sampling.penalty_context) if r.sampling.repetition_penalty != 1.0 else []
-                         for r in sampling]
-            chosen = sample_rows(logits, [r.sampling for r in sampling], [self._seeds[r.request_id] for r in sampling],
-                                 [len(r.generated) + ahead for r in sampling], histories)
         launched = _Launched(plan, sampling, chosen)
         if chosen is not None and chosen.is_cuda:
             # The tokens start for the host at once, behind this step only. Read with a blocking copy
@@ -172,6 +167,17 @@ class Generator:
             launched.copied = torch.cuda.Event()
             launched.copied.record()
         return launched
+
+    def _choose(self, logits: torch.Tensor, sampling: list[Request], ahead: int) -> torch.Tensor:
+        """A token for every row of logits (`ahead`: draws already spent by a step that is not yet committed)."""
+        histories = [r.token_slice(max(0, len(r.prompt) + len(r.generated) - r.sampling.penalty_context),
+                                   r.sampling.penalty_context) if r.sampling.repetition_penalty != 1.0 else []
+                     for r in sampling]
+        adjusts = any(r.sampling.adjusts for r in sampling)
+        return sample_rows(logits, [r.sampling for r in sampling], [self._seeds[r.request_id] for r in sampling],
+                           [len(r.generated) + ahead for r in sampling], histories,
+                           [text_of(r.sampling, r.prompt, r.generated) for r in sampling] if adjusts else None,
+                           [allowed_ids(r.sampling, r.generated) for r in sampling] if adjusts else None)
 
     def _finalize(self, launched: "_Launched") -> list[StepOutput]:
         """Read the launched step's tokens (this waits for it) and commit them."""
@@ -195,7 +201,7 @@ class Generator:
     def _next_decode_plan(self, launched: "_Launched") -> StepPlan | None:
         """The plan of the step after `launched`, if it can be made before `launched`'s tokens
         are known: every entry decodes, nobody waits for admission, no request needs its own
-        last token on the host (repetition penalty), and the pages are there."""
+        last token on the host (penalties, constraints), and the pages are there."""
         if self.engine.runner.graphs is None or self.scheduler.waiting or not self.pipelined:
             return None
         entries = launched.plan.entries
@@ -205,7 +211,7 @@ class Generator:
         reserved = [0] * len(self.engine.cache.groups)
         for e in entries:
             r = e.request
-            if r.status != "running" or r.sampling.repetition_penalty != 1.0:
+            if r.status != "running" or r.sampling.needs_text:
                 return None
             if len(r.generated) + 2 > r.max_tokens:  # it ends with the launched step's token: plan normally
                 return None
@@ -230,6 +236,77 @@ class Generator:
         else:
             self._in_flight = None
         return self._finalize(launched)
+
+    def step_drafted(self, drafts: "Mapping[str, tuple[Sequence[int], Sequence[int] | None]]") -> list[StepOutput]:
+        """Run one step in which decoding requests bring drafted tokens, and return what it produced: for a request one token as ever, and one
+        more for every draft that it agrees with. The tokens are those of steps without drafts (drawn by the same numbers).
+
+        `drafts`: request id -> (tokens, parents): what may follow the request's latest token, as a tree: `parents[i]` is the earlier
+        draft that token i goes on from, -1 the latest token itself; None: each goes on from the one ahead of it. Drafts are left aside where
+        pages or the request's last tokens are short, in a step that reads prompts, and for requests that do not decode. ValueError for a
+        model whose layers keep other than keys and values."""
+        runner = self.engine.runner
+        why = runner.drafted.why_not()
+        if why is not None:
+            raise ValueError(why)
+        outputs = self.drain()
+        plan = self.scheduler.plan()
+        if not plan.entries:
+            return outputs
+        if any(e.count != 1 or not e.samples or not e.request.generated for e in plan.entries):
+            return outputs + self._finalize(self._launch(plan))
+        cache, vocab, entries = self.engine.cache, self.engine.vocab_size, []
+        reserved = [0] * len(cache.groups)
+        for planned in plan.entries:
+            self.scheduler._reserve(planned.request, 1, reserved)
+        for planned in plan.entries:
+            request = planned.request
+            tokens, parents = drafts.get(request.request_id, ((), None))
+            tokens = [int(t) for t in tokens]
+            parents = list(range(-1, len(tokens) - 1)) if parents is None else [int(p) for p in parents]
+            if len(parents) != len(tokens) or any(not -1 <= p < i for i, p in enumerate(parents)) or any(not 0 <= t < vocab for t in tokens) or \
+                    len(tokens) >= ops.MOST_DRAFTED:
+                raise ValueError(f"request {request.request_id!r}: up to {ops.MOST_DRAFTED - 1} drafts of the vocabulary, each with an earlier parent or -1")
+            count = 1 + len(tokens)
+            mine = [cache.pages_for(g, request.cache.tokens + count) - cache.pages_for(g, request.cache.tokens + 1) for g in range(len(cache.groups))]
+            if len(request.generated) + 1 >= request.max_tokens or any(r + m > g.pool.free for r, m, g in zip(reserved, mine, cache.groups)):
+                tokens, parents, count, mine = [], [], 1, [0] * len(mine)
+            reserved = [r + m for r, m in zip(reserved, mine)]
+            entries.append(StepEntry(request.cache, [request.token_slice(planned.start, 1)[0], *tokens], list(range(count)), [-1, *(p + 1 for p in parents)]))
+        requests = [planned.request for planned in plan.entries]
+        try:
+            logits = runner.run(entries)
+            rows, owners, depths, allowed = [], [], [], []
+            for r, (request, entry) in enumerate(zip(requests, entries)):
+                ways: list[list[int]] = []
+                for j, p in enumerate(entry.parents):
+                    ways.append([*ways[p], j] if p >= 0 else [j])
+                    rows.append(len(rows))
+                    owners.append(r)
+                    depths.append(len(ways[j]) - 1)
+                    allowed.append(allowed_ids(request.sampling, request.generated + [entry.tokens[i] for i in ways[j][1:]]))
+            params = [request.sampling for request in requests]
+            # (A request's text ends ahead of the step's tokens, the first of which is its latest one.)
+            texts = [text_of(p, request.prompt, request.generated[:-1]) for p, request in zip(params, requests)]
+            chosen = sample_drafted(logits, runner.drafted.last[1], rows, owners, depths, params, [self._seeds[r.request_id] for r in requests],
+                                    [len(r.generated) for r in requests], texts, allowed)
+            kept = runner.keep(entries, chosen)
+        except Exception:
+            for request in requests:  # a failed step fails its requests and frees what they hold
+                self.scheduler._finish(request, "abort")
+                self._seeds.pop(request.request_id, None)
+            raise
+        for request, mine in zip(requests, kept):
+            for token in [*mine.tokens, mine.next]:
+                some = self.scheduler.commit(StepPlan([PlannedEntry(request, request.computed, 1, True)], []), {request.request_id: token})
+                for output in some:
+                    if output.token is not None:
+                        request.meter.token()
+                outputs += some
+                if request.status != "running":
+                    self._seeds.pop(request.request_id, None)
+                    break
+        return outputs
 
     def resize_cache(self, tokens: int) -> None:
         """Give the page pools of a running engine room for `tokens` positions, more or fewer: what live requests hold is kept

@@ -21,6 +21,7 @@ import numpy as np
 import torch
 
 from mlx_omnia_b200.cache.manager import CacheManager, RequestCache
+from mlx_omnia_b200.kernels import ops
 from mlx_omnia_b200.parts.base import KVView, LayerContext, Runtime, StepContext
 from mlx_omnia_b200.parts.model import DecoderModel
 
@@ -30,6 +31,7 @@ class StepEntry:
     request: RequestCache
     tokens: list[int]
     want: list[int] = field(default_factory=list)  # indices into `tokens`
+    parents: list[int] | None = None  # drafted tokens: for each the earlier one that it goes on from; -1 for the first, which is known
 
 
 def shared_positions(entries: list[StepEntry]) -> tuple[tuple[int, tuple[int, ...]], ...]:
@@ -125,12 +127,133 @@ class StepLayout:
             fresh=self.view(device, "fresh"), logit_rows=self.view(device, "logit_rows"), groups=groups, **host_side)
 
 
+@dataclass(frozen=True)
+class Kept:
+    """What a request keeps of the tokens that it brought as drafts: the kept ones behind the first, and the token chosen behind the last of them."""
+
+    tokens: list[int]
+    next: int
+
+
+class DraftedSteps:
+    """Steps whose requests bring trees of drafted tokens. `run` reads all of them in one step; `keep` says which the model agrees with, moves
+    their keys and values to where a request that had brought only these would have them, and takes the others' room back."""
+
+    def __init__(self, runner: "StepRunner") -> None:
+        self.runner = runner
+        self.last: "tuple[list[StepEntry], StepContext, list[int]] | None" = None
+
+    def why_not(self) -> str | None:
+        """Why the model takes no drafted trees (None: it does). A tree's branches read the same positions and leave nothing behind but rows of the
+        cache, which state that goes from token to token does not."""
+        runner = self.runner
+        if runner.cache.has_state or not all(getattr(block.mixer, "tree_safe", False) for block in runner.model.blocks):
+            return "drafted trees take a model of attention over keys and values alone"
+        if any(g.spec.stride != 1 for g in runner.cache.groups):
+            return "drafted trees take caches with a row for every position"
+        return None
+
+    def run(self, entries: list[StepEntry]) -> torch.Tensor:
+        runner, cache, device = self.runner, self.runner.cache, self.runner.runtime.device
+        why = self.why_not()
+        if why is not None:
+            raise ValueError(why)
+        for e in entries:
+            n, parents = len(e.tokens), e.parents
+            if not 1 <= n <= ops.MOST_DRAFTED:
+                raise ValueError(f"request {e.request.request_id!r} brings {n} tokens to a step of drafted trees, which takes 1 to {ops.MOST_DRAFTED}")
+            if any(not 0 <= w < n for w in e.want):
+                raise ValueError(f"request {e.request.request_id!r}: a wanted place lies outside its tokens")
+            if parents is not None and (len(parents) != n or parents[0] != -1 or any(not 0 <= p < j for j, p in enumerate(parents) if j)):
+                raise ValueError(f"request {e.request.request_id!r}: a drafted token goes on from an earlier one, the first from none")
+            if parents is not None and e.want != list(range(n)):
+                raise ValueError(f"request {e.request.request_id!r}: drafted tokens want all their logits")
+        if len({id(e.request) for e in entries}) < len(entries):
+            raise ValueError("a request comes once to a step")
+        cache.reset_slots([e.request.slot for e in entries if e.request.fresh])
+        starts = runner.take_pages(entries)
+        brought = [len(e.tokens) for e in entries]
+        held, tokens = [s + b for s, b in zip(starts, brought)], sum(brought)
+        cu = np.cumsum([0, *brought])
+        rows = [int(c) + w for c, e in zip(cu, entries) for w in e.want]
+        lists = [[e.request.table_array(g) for e in entries] for g in range(len(cache.groups))]
+        n, groups = len(entries), len(cache.groups)
+        parts = {f"starts{g}": 2 * n for g in range(groups)} | {"held": n, "brought": n, "slots": n, "fresh": n, "parents": tokens, "ids": tokens,
+                                                               "rows": len(rows)} | {f"pages{g}": sum(map(len, x)) for g, x in enumerate(lists)}
+        where, at = {}, 0
+        for name, size in parts.items():
+            where[name] = slice(at, at + size)
+            at += size
+        host_tensor = torch.empty(at, dtype=torch.int32, pin_memory=device.type == "cuda")
+        host = host_tensor.numpy()
+        host[where["held"]], host[where["brought"]] = starts, brought
+        host[where["slots"]], host[where["fresh"]] = [e.request.slot for e in entries], [int(e.request.fresh) for e in entries]
+        host[where["parents"]] = [p for e in entries for p in (e.parents if e.parents is not None else range(-1, len(e.tokens) - 1))]
+        host[where["ids"]], host[where["rows"]] = [t for e in entries for t in e.tokens], rows
+        for g, x in enumerate(lists):
+            host[where[f"starts{g}"]].view(np.int64)[:] = np.cumsum([0, *map(len, x)])[:-1]
+            host[where[f"pages{g}"]] = np.concatenate(x)
+        packed = host_tensor.to(device, non_blocking=True) if device.type == "cuda" else host_tensor
+        part = {name: packed[w] for name, w in where.items()}
+        made = ops.step_tables(part["held"], part["brought"], [ops.PageLists(part[f"pages{g}"], part[f"starts{g}"].view(torch.int64), max(map(len, x)))
+                                                               for g, x in enumerate(lists)],
+                               cache.page_size, tokens, parents=part["parents"], most=max(brought))
+        step = StepContext(
+            num_tokens=tokens, num_seqs=n, token_ids=part["ids"], positions=made.positions, cu_seqlens=made.cu_seqlens, seq_lens=made.seq_lens,
+            state_slots=part["slots"], fresh=part["fresh"], logit_rows=part["rows"], q_lens=brought, seq_lens_host=held, max_q_len=max(brought),
+            max_seq_len=max(held), decode_only=False, groups=dict(enumerate(made.groups)), workspace=runner.ask_for_layers(), tree=made.tree)
+        logits = runner.model.forward(step, runner.layer_contexts(step))
+        runner.know_layers(step)
+        for e in entries:
+            e.request.fresh = False
+            if e.parents is not None:
+                e.request.drafted = len(e.tokens)
+            else:
+                cache.release_behind_window(e.request)
+        self.last = (list(entries), step, starts)
+        runner.steps_run += 1
+        return logits
+
+    def keep(self, entries: list[StepEntry], chosen: torch.Tensor) -> list[Kept | None]:
+        """`chosen`: int32 on the device, the token that was chosen from every row of the logits of `entries`' step, the one just run. Every drafted
+        token is kept whose way from the request's first is what was chosen; the requests hold these and no other from then on.
+        -> for each entry what it keeps (None: it brought no drafts)"""
+        if self.last is None or len(self.last[0]) != len(entries) or any(a is not b for a, b in zip(self.last[0], entries)):
+            raise ValueError("keep() takes the entries of the step of drafted trees that was run last, once")
+        cache, (_, step, starts) = self.runner.cache, self.last
+        if any(e.parents is not None and (e.request.request_id not in cache.requests or e.request.drafted != len(e.tokens)) for e in entries):
+            raise ValueError("a request of the step has ended")
+        if chosen.shape != step.logit_rows.shape:
+            raise ValueError("a token is chosen from every row of the step's logits")
+        picks = chosen
+        if step.logit_rows.shape[0] != step.num_tokens:
+            picks = torch.zeros(step.num_tokens, dtype=torch.int32, device=chosen.device)
+            picks[step.logit_rows.long()] = chosen
+        accepted = ops.accept_drafts(picks, step.token_ids, step.tree, step.cu_seqlens)
+        held = step.seq_lens - (step.cu_seqlens[1:] - step.cu_seqlens[:-1])
+        for g, group in enumerate(cache.groups):
+            ops.keep_rows(group.pages, group.spec.rows, cache.page_size, step.groups[g][0], held, accepted)
+        self.last = None
+        path, kept, last = accepted.path.tolist(), accepted.kept.tolist(), accepted.tokens.tolist()
+        found: list[Kept | None] = []
+        for i, e in enumerate(entries):
+            if e.parents is None:
+                found.append(None)
+                continue
+            self.runner._shrink(e.request, len(e.tokens) - kept[i])
+            e.request.drafted = 0
+            cache.release_behind_window(e.request)
+            found.append(Kept([e.tokens[j] for j in path[i][1: kept[i]]], last[i]))
+        return found
+
+
 class StepRunner:
     """Owns nothing but the glue: the model, the cache manager and the runtime."""
 
     def __init__(self, model: DecoderModel, cache: CacheManager, runtime: Runtime, cuda_graphs: bool = False) -> None:
         self.model, self.cache, self.runtime = model, cache, runtime
         self.steps_run = 0
+        self.drafted = DraftedSteps(self)
         self.attention_layers: Counter = Counter()  # kinds (`ops.AttentionLayer`) that a step was seen to run, and how often
         self.cuda_graphs = cuda_graphs
         self.graphs = self.mixed_graphs = None
@@ -228,7 +351,15 @@ class StepRunner:
         from a captured CUDA graph when graphs are on; `copy=False` then returns the
         graph's own logits buffer, which the next step overwrites. `device_tokens`
         (int32 on the device, one per entry; graph steps only) are the step's tokens when
-        the host does not know them yet."""
+        the host does not know them yet. Entries with `parents` bring drafted tokens: the step
+        is then one of drafted trees (`DraftedSteps`), and `keep` follows it."""
+        for e in entries:
+            if e.request.drafted:
+                raise ValueError(f"request {e.request.request_id!r} holds drafted tokens that are not kept yet")
+        if any(e.parents is not None for e in entries):
+            if device_tokens is not None:
+                raise ValueError("drafted tokens come from the host")
+            return self.drafted.run(entries)
         self.cache.reset_slots([e.request.slot for e in entries if e.request.fresh])
         if self.graphs is not None and entries and all(len(e.tokens) == 1 and e.want in ([], [0]) for e in entries):
             logits = self.graphs.run(entries, copy, device_tokens)
@@ -248,3 +379,7 @@ class StepRunner:
             self.cache.release_behind_window(entry.request)
         self.steps_run += 1
         return logits
+
+    def keep(self, entries: list[StepEntry], chosen: torch.Tensor) -> "list[Kept | None]":
+        """What becomes of the drafted tokens of the step just run (see `DraftedSteps.keep`)."""
+        return self.drafted.keep(entries, chosen)

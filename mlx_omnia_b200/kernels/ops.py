@@ -1115,7 +1115,7 @@ def paged_attention(q: torch.Tensor | None, kv: KVView, step: StepContext, scale
     cases (the 32-bit path among them) run on the generic kernel."""
     if step.workspace and "attention_layers" in step.workspace:  # the runner wants to know
         step.workspace["attention_layers"][attention_layer(kv, q.shape[1] if projection is None else projection.nq, window)] += 1
-    if step.tree is not None:
+    if getattr(step, "tree", None) is not None:
         if projection is not None or difference is not None:
             raise KernelError("attention of drafted trees takes queries, and no difference of maps")
         return tree_attention(q, kv, step, scale, gate=gate, gate_col=gate_col, sink=sink, window=window, keep_first=keep_first, chunk=chunk,

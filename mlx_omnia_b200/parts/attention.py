@@ -35,6 +35,7 @@ class GQAAttention(Mixer):
     """
 
     graph_safe = True  # no host-side work per request: a decode step can be captured
+    tree_safe = True  # branches of drafted tokens side by side: positions and slots come with the step
     graph_safe_mixed = True  # nor in a step of any other shape: repeated mixed steps can be captured too
     takes_pending = True  # h goes to the in-projection and nowhere else
 
@@ -266,6 +267,7 @@ class SinkWindowAttention(Mixer):
     `o` [hidden, heads * vdim]."""
 
     graph_safe = True
+    tree_safe = True
     graph_safe_mixed = True
 
     def __init__(self, hidden: int, heads: int, kv_heads: int, dim: int, vdim: int, scale: float,

@@ -14,7 +14,8 @@ Every part:
     ``load(tensors, runtime)``                  receives exactly those, on the device
 Mixer additionally (class attributes `graph_safe` / `graph_safe_mixed`: its forward does no
 host-side work per request in a step of single tokens / in any step, so such steps may be
-captured into CUDA graphs):
+captured into CUDA graphs; `tree_safe`: it takes a step of drafted trees, `StepContext.tree`: a token's
+keys and values go where its slot says, its position is what `positions` says, and attention is `ops.paged_attention`):
     ``kv_spec() -> KVSpec | None``              rows it keeps per position, in pages
     ``state_spec() -> StateSpec | {name: StateSpec} | None``  fixed-size state it keeps per request
                                                 (several named tensors when it gives a dict)

@@ -12,14 +12,15 @@ are refused rather than silently reordered.
 
 from __future__ import annotations
 
-from collections.abc import Collection
+import math
+from collections.abc import Callable, Collection, Mapping, Sequence
 from dataclasses import dataclass, replace
 
 
 @dataclass(frozen=True)
 class SamplingParams:
-    """temperature 0 means greedy; top_k 0, top_p 1, min_p 0 and repetition_penalty 1
-    switch the respective stage off. `seed` None draws a fresh seed per request."""
+    """temperature 0 means greedy; top_k 0, top_p 1, min_p 0, repetition_penalty 1, the other penalties 0, no bias and no
+    constraint switch the respective stage off. `seed` None draws a fresh seed per request."""
 
     temperature: float = 0.0
     top_k: int = 0
@@ -28,10 +29,29 @@ class SamplingParams:
     repetition_penalty: float = 1.0
     penalty_context: int = 20
     seed: int | None = None
+    frequency_penalty: float = 0.0
+    presence_penalty: float = 0.0
+    bias: tuple[tuple[int, float], ...] = ()
+    constraint: "Callable[[Sequence[int]], Collection[int] | None] | None" = None
 
     @property
     def greedy(self) -> bool:
         return self.temperature <= 0.0
+
+    @property
+    def counts(self) -> bool:
+        """Whether tokens weigh by how often they were generated."""
+        return self.frequency_penalty != 0.0 or self.presence_penalty != 0.0
+
+    @property
+    def adjusts(self) -> bool:
+        """Whether the logits are changed by more than the repetition penalty."""
+        return self.counts or bool(self.bias) or self.constraint is not None
+
+    @property
+    def needs_text(self) -> bool:
+        """Whether a choice depends on the tokens chosen before it (beside their number)."""
+        return self.counts or self.repetition_penalty != 1.0 or self.constraint is not None
 
 
 @dataclass(frozen=True)
@@ -116,11 +136,15 @@ class GenerationOptions:
     stop:           token ids that end the generation without being emitted; None means
                     the model's own (config.json's eos_token_id)
     penalty:        what `repetition_penalty(...)` returns, or None
+    frequency_penalty: subtracted from a token's logit for every time that it was generated
+    presence_penalty:  subtracted from a token's logit once if it was generated
+    bias:           {token id: what its logit is raised by} (-inf: never chosen), behind the penalties
+    constraint:     a function of the ids generated so far -> the ids that may come next (None: any); asked for every token
     context_limit:  ceiling on prompt and generation together, or None
     meter:          an `engine.meter.Meter` that the generation fills (token counts, time to the
                     first token, decode rate), or None
-    The reference's remaining fields (constraint, prefix, reasoning_budget, speculate) belong
-    to its server, grammar and drafter, which this engine leaves out.
+    The reference's remaining fields (prefix, reasoning_budget, speculate) belong
+    to its server and drafter, which this engine leaves out.
     """
 
     max_tokens: int
@@ -129,8 +153,26 @@ class GenerationOptions:
     penalty: Penalty | None = None
     context_limit: int | None = None
     meter: object | None = None
+    frequency_penalty: float = 0.0
+    presence_penalty: float = 0.0
+    bias: Mapping[int, float] | None = None
+    constraint: Callable[[Sequence[int]], Collection[int] | None] | None = None
+
+    def __post_init__(self) -> None:
+        if not all(math.isfinite(x) for x in (self.frequency_penalty, self.presence_penalty)):
+            raise ValueError("frequency_penalty and presence_penalty are finite numbers")
+        for token, value in (self.bias or {}).items():
+            if token < 0 or math.isnan(value) or value == math.inf:
+                raise ValueError(f"a bias names a token id and a finite number or -inf: {token}: {value}")
 
     def params(self) -> SamplingParams:
-        if self.penalty is None:
-            return self.sampler
-        return replace(self.sampler, repetition_penalty=self.penalty.value, penalty_context=self.penalty.context)
+        more: dict = {}
+        if self.penalty is not None:
+            more |= {"repetition_penalty": self.penalty.value, "penalty_context": self.penalty.context}
+        if self.frequency_penalty or self.presence_penalty:
+            more |= {"frequency_penalty": float(self.frequency_penalty), "presence_penalty": float(self.presence_penalty)}
+        if self.bias:
+            more["bias"] = tuple((int(token), float(value)) for token, value in self.bias.items())
+        if self.constraint is not None:
+            more["constraint"] = self.constraint
+        return replace(self.sampler, **more) if more else self.sampler
