@@ -133,6 +133,7 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_con
     const long long t0 = total * blockIdx.x / blocks;
     place.find(a, shares, ends, t0, (int)(total * (blockIdx.x + 1) / blocks - t0));
   }
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // (the ends lie where copies will come to)
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -616,6 +617,7 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_con
           }
         }
       }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // (the rows lay where the next segment's copies come to)
       OMNIA_TRACE_BLOCK(6);  // its rows are out
       first = false;
     }

@@ -1383,23 +1383,25 @@ def step_tables(held: torch.Tensor, brought: torch.Tensor, lists: "list[PageList
         _like(what, "starts", x.starts, torch.int64, index, (n,))
         if x.width < 1 or x.stride < 1 or (x.stride > 1 and most is not None):
             raise KernelError(f"{what}: tables have a column or more, and drafted tokens a stored row each")
-    stream, device = _current(what, index), held.device
-    buffer = torch.empty(tokens + 2 * n + 1, dtype=int32, device=device)
-    positions, cu_seqlens, seq_lens = buffer.split_with_sizes((tokens, n + 1, n))
-    at, ancestors, sees = buffer.data_ptr(), None, 0
+    stream = _current(what, index)
+    # One buffer: the slots (8 bytes each) first, then all that has 4.
+    sizes = [2 * tokens] * count + [x.width * n for x in lists] + [tokens, n + 1, n]
     if words:
-        ancestors = torch.empty(tokens, words, dtype=int32, device=device)
-        sees = ancestors.data_ptr()
-    packed = _TABLES.pack(held.data_ptr(), brought.data_ptr(), 0 if parents is None else parents.data_ptr(), at, at + 4 * tokens,
-                          at + 4 * (tokens + n + 1), sees, _error_address(index), n, tokens, page_size, words, count)
-    groups = []
-    for pages, starts, width, stride in lists:
-        table, slots = torch.empty(n, width, dtype=int32, device=device), torch.empty(tokens, dtype=torch.int64, device=device)
-        packed += _TABLE_GROUP.pack(pages.data_ptr(), starts.data_ptr(), table.data_ptr(), slots.data_ptr(), pages.shape[0], width, stride)
-        groups.append((table, slots))
+        sizes.append(tokens * words)
+    buffer = torch.empty(sum(sizes), dtype=int32, device=held.device)
+    parts, at, groups, packed = buffer.split_with_sizes(sizes), buffer.data_ptr(), [], b""
+    table_at = at + 8 * tokens * count
+    for i, (pages, starts, width, stride) in enumerate(lists):
+        packed += _TABLE_GROUP.pack(pages.data_ptr(), starts.data_ptr(), table_at, at + 8 * tokens * i, pages.shape[0], width, stride)
+        table_at += 4 * n * width
+        groups.append((parts[count + i].view(n, width), parts[i].view(torch.int64)))
+    positions, cu_seqlens, seq_lens = parts[2 * count: 2 * count + 3]
+    sees = table_at + 4 * (tokens + 2 * n + 1) if words else 0
+    packed = _TABLES.pack(held.data_ptr(), brought.data_ptr(), 0 if parents is None else parents.data_ptr(), table_at, table_at + 4 * tokens,
+                          table_at + 4 * (tokens + n + 1), sees, _error_address(index), n, tokens, page_size, words, count) + packed
     # (The C side reads as many groups as it is told of.)
     _check(_entry("drafted", "omnia_step_tables", [c_void_p, c_void_p])(packed, stream), what)
-    return StepTables(positions, cu_seqlens, seq_lens, groups, None if ancestors is None else StepTree(ancestors))
+    return StepTables(positions, cu_seqlens, seq_lens, groups, StepTree(parts[-1].view(tokens, words)) if words else None)
 
 
 class Accepted(NamedTuple):
@@ -1472,9 +1474,12 @@ def keep_rows(pages: torch.Tensor, rows: tuple[tuple[int, int], ...], page_size:
     return pages
 
 
-TREE_MANY_ROWS = 33
+TREE_MANY_ROWS, TREE_MANY_KEYS = 33, 2048
 """From so many rows (query heads of a group times the most tokens that a request brings) attention of drafted trees runs on the tcgen05 kernel, where it
-takes the head size and the pages."""
+takes the head size and the pages; with more than 16 rows from so many keys on, too. mma.sync gets to some 155 TFLOP/s on a B200, so that 16 rows to a key
+are as many as the memory's rate allows, and the tcgen05 kernel has a beginning and an end of 15 us. 16/8 heads of 128, us with mma.sync / tcgen05: 8
+requests of 500 positions with 8, 16, 32 tokens 29 / 30, 23 / 31, 33 / 31; of 4,096 46 / 51, 50 / 48, 69 / 55; of 20,000 141 / 138, 160 / 137, 210 / 139;
+one of 4,096 with 16 tokens 32 / 27, of 60,000 with 5 71 / 67, with 64 168 / 81."""
 
 _TREE = struct.Struct("14Pq16i2f")  # TreeAttention in attention_tree.cuh
 
@@ -1548,7 +1553,7 @@ def tree_attention(q: torch.Tensor, kv: KVView, step: StepContext, scale: float,
         keys = min(keys, run + most)
     q_ptr, sms = q.data_ptr(), sm_count(device)
     tensor_cores = dv == d and dtype is torch.bfloat16 and d % 8 == 0 and d <= 256 and n <= 1024 and not k_ptr & 15 and not q_ptr & 3
-    many = tensor_cores and rows >= TREE_MANY_ROWS and d in (64, 128) and kv.page_size % 16 == 0 and scale > 0 and not q_ptr & 15 and nq // nkv <= 128
+    many = tensor_cores and (rows >= TREE_MANY_ROWS or (rows > 16 and keys >= TREE_MANY_KEYS)) and d in (64, 128) and kv.page_size % 16 == 0 and scale > 0 and not q_ptr & 15 and nq // nkv <= 128
     shares32 = dv == d and dtype is torch.float32 and d % 4 == 0 and d <= 256 and n <= 1024 and not (k_ptr | v_ptr) & 15 and page_stride % 4 == 0
     if many:
         tile = 2 * (128 // (nq // nkv) * (nq // nkv))

@@ -28,6 +28,7 @@ def no_errors():
 def way(request, monkeypatch):
     """Both kernels of the tensor cores, at every size that they take."""
     monkeypatch.setattr(ops, "TREE_MANY_ROWS", {"few rows": 1 << 30, "many rows": 0}[request.param])
+    monkeypatch.setattr(ops, "TREE_MANY_KEYS", 1 << 30)
 
 
 def ints(values, dtype=torch.int32):
