@@ -7,13 +7,16 @@ the sources, keyed by a hash of the source text, the shared header and the flags
 If that folder cannot be written (a read-only checkout), a per-user folder under the
 temporary directory is used. While nvcc runs, a line is printed to stderr every few
 seconds. There is no fallback: if nvcc is missing or the compile fails, loading
-raises `KernelBuildError` with the compiler's output.
+raises `KernelBuildError` with the compiler's output. A `.cpp` file is a Python module of
+the host's side of calls (`load_module`), compiled with the host's compiler against the installed torch.
 """
 
 from __future__ import annotations
 
 import ctypes
 import hashlib
+import importlib.machinery
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -26,7 +29,10 @@ SOURCE_DIR = Path(__file__).resolve().parent
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 BASE_FLAGS = ["-O3", "-lineinfo", "-std=c++17", "--shared", "-Xcompiler", "-fPIC"]
 
+MODULE_FLAGS = ["-O2", "-std=c++17", "-shared", "-fPIC"]
+
 _loaded: dict[str, ctypes.CDLL] = {}
+_modules: dict = {}
 
 TIMELINE = int(os.environ.get("OMNIA_TIMELINE") or 0)
 """With OMNIA_TIMELINE=1 in the environment every library is the tracing build (see common.cuh):
@@ -121,6 +127,66 @@ def compile_library(name: str, defines: dict[str, object] | None = None, extra: 
     if verbose:
         print(f"[mlx_omnia_b200]   built {target.name} in {time.time() - started:.1f} s", file=sys.stderr, flush=True)
     return target
+
+
+def _module_command(source: Path, target: Path) -> list[str]:
+    import sysconfig
+
+    import torch
+
+    root = Path(torch.__file__).resolve().parent
+    cuda = Path(_nvcc()).resolve().parent.parent / "include"
+    includes = [root / "include", root / "include" / "torch" / "csrc" / "api" / "include", sysconfig.get_paths()["include"], cuda]
+    compiler = next((c for c in (os.environ.get("CXX"), shutil.which("g++"), shutil.which("c++")) if c), None)
+    if compiler is None:
+        raise KernelBuildError("no C++ compiler was found (looked at $CXX and for g++ and c++ on PATH)")
+    return [compiler, *MODULE_FLAGS, f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *[f"-I{p}" for p in includes], "-o", str(target),
+            str(source), f"-L{root / 'lib'}", *[f"-l{name}" for name in ("torch_python", "torch", "torch_cpu", "c10_cuda", "c10")]]
+
+
+def module_path(name: str) -> Path:
+    import torch
+
+    h = hashlib.sha256((SOURCE_DIR / f"{name}.cpp").read_bytes())
+    h.update(repr((torch.__version__, sys.version, MODULE_FLAGS)).encode())
+    return _build_dir() / f"omnia_{name}_{h.hexdigest()[:16]}.so"
+
+
+def compile_module(name: str, verbose: bool = True) -> Path:
+    """Compile the Python module `name`.cpp with the host's compiler, if it is not there yet; return its path."""
+    target = module_path(name)
+    if target.exists():
+        return target
+    partial = target.with_suffix(f".tmp{os.getpid()}.so")
+    command = _module_command(SOURCE_DIR / f"{name}.cpp", partial)
+    if verbose:
+        print(f"[mlx_omnia_b200] compiling {target.name} ...", file=sys.stderr, flush=True)
+    done = subprocess.run(command, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+    if done.returncode != 0:
+        partial.unlink(missing_ok=True)
+        raise KernelBuildError(f"the compiler failed for {name}.cpp:\n{' '.join(command)}\n{done.stdout}")
+    os.replace(partial, target)
+    for stale in target.parent.glob(f"omnia_{name}_*.so"):
+        if stale != target and ".tmp" not in stale.name:
+            stale.unlink(missing_ok=True)
+    return target
+
+
+def load_module(name: str):
+    """The Python module compiled from `name`.cpp (`omnia_<name>`), compiling it first if need be."""
+    key = f"module|{name}"
+    module = _modules.get(key)
+    if module is None:
+        path = compile_module(name)
+        loader = importlib.machinery.ExtensionFileLoader(f"omnia_{name}", str(path))
+        spec = importlib.util.spec_from_loader(f"omnia_{name}", loader)
+        try:
+            module = importlib.util.module_from_spec(spec)
+            loader.exec_module(module)
+        except ImportError as error:
+            raise KernelBuildError(f"could not load {path}: {error}") from error
+        _modules[key] = module
+    return module
 
 
 def load_library(name: str, defines: dict[str, object] | None = None, extra: list[str] | None = None) -> ctypes.CDLL:

@@ -15,7 +15,6 @@ import ctypes
 import functools
 import itertools
 import math
-import struct
 from ctypes import c_float, c_int, c_longlong, c_void_p
 
 import dataclasses
@@ -25,7 +24,7 @@ from typing import Callable, NamedTuple
 import numpy as np
 import torch
 
-from mlx_omnia_b200.csrc.build import load_library
+from mlx_omnia_b200.csrc.build import load_library, load_module
 from mlx_omnia_b200.parts.base import KVView, StepContext, StepTree
 
 _DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1}
@@ -1274,55 +1273,32 @@ MOST_DRAFTED = 256
 """Tokens that a request brings to a step of drafted trees at most: eight words of bits, a thread each."""
 
 
-_entries: dict[str, ctypes._CFuncPtr] = {}
+@functools.cache
+def _host():
+    """The host's side of these calls (csrc/host.cpp): checks, memory, the launch."""
+    module = load_module("host")
+    module.set_up(KernelError, lambda index: error_word(torch.device("cuda", index)).data_ptr())
+    return module
 
 
-def _entry(library: str, name: str, argtypes: list, defines: dict | None = None):
-    """`_function`, looked up by a name that costs less to make (these calls are bound by the host in small steps)."""
-    key = name if defines is None else name + str(defines["HEAD_DIM"])
-    fn = _entries.get(key)
-    if fn is None:
-        fn = _entries[key] = _function(library, name, argtypes, defines)
-    return fn
+_addresses: dict[str, int] = {}
 
 
-def _wrong(what: str, name: str, t: torch.Tensor, dtype: torch.dtype, index: int, shape) -> KernelError:
-    if t.get_device() != index:
-        return KernelError(f"{what}: {name} lies on {t.device}, not with the other tensors")
-    return KernelError(f"{what}: {name} is a contiguous {dtype} tensor of {shape}, not {t.dtype} {list(t.shape)} with strides {list(t.stride())}")
+def _address(library: str, name: str, head_dim: int = 0, index: int = 0) -> int:
+    """Where a launcher lies (0 for tensors on the host, which are refused before one is needed)."""
+    key = name if not head_dim else f"{name}{head_dim}"
+    found = _addresses.get(key)
+    if found is None:
+        if index < 0:
+            return 0
+        fn = getattr(load_library(library, {"HEAD_DIM": head_dim} if head_dim else None), name)
+        found = _addresses[key] = ctypes.cast(fn, c_void_p).value
+    return found
 
 
-def _list_of(what: str, name: str, t: torch.Tensor, dtype: torch.dtype, index: int) -> int:
-    """The size of `t`, a contiguous tensor of one dimension on device `index`."""
-    if t.dtype is not dtype or t.dim() != 1 or not t.is_contiguous() or t.get_device() != index:
-        raise _wrong(what, name, t, dtype, index, "[n]")
-    return t.shape[0]
-
-
-def _like(what: str, name: str, t: torch.Tensor, dtype: torch.dtype, index: int, shape: tuple) -> None:
-    """`t` is a contiguous tensor of this shape on device `index`."""
-    if t.dtype is not dtype or t.shape != shape or not t.is_contiguous() or t.get_device() != index:
-        raise _wrong(what, name, t, dtype, index, list(shape))
-
-
-def _current(what: str, index: int) -> int:
-    """The current stream of the current device, which has to be device `index`, that of the tensors."""
-    if index < 0:
-        raise KernelError(f"{what} takes tensors on a CUDA device")
-    if torch._C._cuda_getDevice() != index:
-        raise KernelError(f"{what} takes tensors on the current CUDA device ({torch._C._cuda_getDevice()}), not on {index}")
-    return torch._C._cuda_getCurrentRawStream(index)
-
-
-_error_addresses: dict[int, int] = {}
-
-
-def _error_address(index: int) -> int:
-    """Where `error_word` of a device lies (it is made once)."""
-    address = _error_addresses.get(index)
-    if address is None:
-        address = _error_addresses[index] = error_word(torch.device("cuda", index)).data_ptr()
-    return address
+def _launched() -> None:
+    global launches
+    launches += 1
 
 
 class PageLists(NamedTuple):
@@ -1346,10 +1322,6 @@ class StepTables(NamedTuple):
     tree: StepTree | None
 
 
-_TABLES, _TABLE_GROUP = struct.Struct("8P5i4x"), struct.Struct("4Pq2i")  # StepTables, TableGroup in drafted.cu
-MOST_TABLE_GROUPS = 8
-
-
 def step_tables(held: torch.Tensor, brought: torch.Tensor, lists: "list[PageLists]", page_size: int, tokens: int,
                 parents: torch.Tensor | None = None, most: int | None = None) -> StepTables:
     """The tables of a step whose requests hold `held` positions (int32 [requests]; below 0: a request that is there for the step's shape only) and
@@ -1363,45 +1335,10 @@ def step_tables(held: torch.Tensor, brought: torch.Tensor, lists: "list[PageList
 
     A list too short or a table too narrow for its request, more tokens than rows, a parent that is no earlier token: the error word, and
     -1 in the request's tables (`raise_on_error`)."""
-    what = "step_tables"
-    index, int32 = held.get_device(), torch.int32
-    n = _list_of(what, "held", held, int32, index)
-    _like(what, "brought", brought, int32, index, (n,))
-    words, count = 0, len(lists)
-    if most is not None:
-        if not 1 <= most <= MOST_DRAFTED:
-            raise KernelError(f"{what}: a request brings 1 to {MOST_DRAFTED} drafted tokens, not {most}")
-        words = (most + 31) // 32
-    if parents is not None:
-        if most is None:
-            raise KernelError(f"{what}: parents go with `most`, the most tokens that a request brings")
-        _like(what, "parents", parents, int32, index, (tokens,))
-    if not 1 <= n <= 65534 or not 0 <= tokens < 1 << 31 or page_size < 1 or count > MOST_TABLE_GROUPS:
-        raise KernelError(f"{what} takes 1 to 65,534 requests, pages of a token or more and up to {MOST_TABLE_GROUPS} groups")
-    for x in lists:
-        _list_of(what, "pages", x.pages, int32, index)
-        _like(what, "starts", x.starts, torch.int64, index, (n,))
-        if x.width < 1 or x.stride < 1 or (x.stride > 1 and most is not None):
-            raise KernelError(f"{what}: tables have a column or more, and drafted tokens a stored row each")
-    stream = _current(what, index)
-    # One buffer: the slots (8 bytes each) first, then all that has 4.
-    sizes = [2 * tokens] * count + [x.width * n for x in lists] + [tokens, n + 1, n]
-    if words:
-        sizes.append(tokens * words)
-    buffer = torch.empty(sum(sizes), dtype=int32, device=held.device)
-    parts, at, groups, packed = buffer.split_with_sizes(sizes), buffer.data_ptr(), [], b""
-    table_at = at + 8 * tokens * count
-    for i, (pages, starts, width, stride) in enumerate(lists):
-        packed += _TABLE_GROUP.pack(pages.data_ptr(), starts.data_ptr(), table_at, at + 8 * tokens * i, pages.shape[0], width, stride)
-        table_at += 4 * n * width
-        groups.append((parts[count + i].view(n, width), parts[i].view(torch.int64)))
-    positions, cu_seqlens, seq_lens = parts[2 * count: 2 * count + 3]
-    sees = table_at + 4 * (tokens + 2 * n + 1) if words else 0
-    packed = _TABLES.pack(held.data_ptr(), brought.data_ptr(), 0 if parents is None else parents.data_ptr(), table_at, table_at + 4 * tokens,
-                          table_at + 4 * (tokens + n + 1), sees, _error_address(index), n, tokens, page_size, words, count) + packed
-    # (The C side reads as many groups as it is told of.)
-    _check(_entry("drafted", "omnia_step_tables", [c_void_p, c_void_p])(packed, stream), what)
-    return StepTables(positions, cu_seqlens, seq_lens, groups, StepTree(parts[-1].view(tokens, words)) if words else None)
+    positions, cu_seqlens, seq_lens, groups, ancestors = _host().step_tables(_address("drafted", "omnia_step_tables", index=held.get_device()), held, brought,
+                                                                             lists, page_size, tokens, parents, most)
+    _launched()
+    return StepTables(positions, cu_seqlens, seq_lens, groups, None if ancestors is None else StepTree(ancestors))
 
 
 class Accepted(NamedTuple):
@@ -1417,32 +1354,9 @@ def accept_drafts(chosen: torch.Tensor, token_ids: torch.Tensor, tree: StepTree,
     """Which drafted tokens the model agrees with: from a request's first token, which is known, on to the one that was chosen behind it
     (`chosen` int32 [tokens]: for every row of the step what its logits gave), as long as that was drafted there, of equal ones the first. Sampled
     choices keep the model's distribution: each is a draw from its own row, whatever was drafted."""
-    what = "accept_drafts"
-    ancestors = tree.ancestors
-    index, int32 = ancestors.get_device(), torch.int32
-    tokens, words = ancestors.shape if ancestors.dim() == 2 else (0, 0)
-    n = _list_of(what, "cu_seqlens", cu_seqlens, int32, index) - 1
-    if n < 1 or not 1 <= words <= MOST_DRAFTED // 32:
-        raise KernelError(f"{what} takes a request or more, of {MOST_DRAFTED} tokens at most")
-    _like(what, "ancestors", ancestors, int32, index, (tokens, words))
-    _like(what, "chosen", chosen, int32, index, (tokens,))
-    _like(what, "token_ids", token_ids, int32, index, (tokens,))
-    stream = _current(what, index)
-    path, buffer = torch.empty(n, 32 * words, dtype=int32, device=chosen.device), torch.empty(2, n, dtype=int32, device=chosen.device)
-    kept, last = buffer.unbind()
-    at = buffer.data_ptr()
-    fn = _entry("drafted", "omnia_accept_drafts", [c_void_p] * 4 + [c_int, c_int] + [c_void_p] * 3 + [c_int, c_void_p, c_void_p])
-    _check(fn(chosen.data_ptr(), token_ids.data_ptr(), ancestors.data_ptr(), cu_seqlens.data_ptr(), n, words, path.data_ptr(), at, at + 4 * n,
-              tokens, _error_address(index), stream), what)
-    return Accepted(path, kept, last)
-
-
-@functools.lru_cache(maxsize=256)
-def _page_kinds(rows: tuple[tuple[int, int], ...], page_size: int, elements: int, item: int) -> array.array:
-    """Of every kind of row: heads, then bytes of a head's row."""
-    if not 1 <= len(rows) <= 8 or any(h < 1 or w < 1 for h, w in rows) or sum(h * w for h, w in rows) * page_size != elements:
-        raise KernelError(f"pages of {elements} elements do not hold {page_size} rows of {rows}")
-    return array.array("i", [h for h, _ in rows] + [w * item for _, w in rows])
+    made = _host().accept_drafts(_address("drafted", "omnia_accept_drafts", index=chosen.get_device()), chosen, token_ids, tree.ancestors, cu_seqlens)
+    _launched()
+    return Accepted(*made)
 
 
 def keep_rows(pages: torch.Tensor, rows: tuple[tuple[int, int], ...], page_size: int, block_table: torch.Tensor, held: torch.Tensor,
@@ -1450,27 +1364,8 @@ def keep_rows(pages: torch.Tensor, rows: tuple[tuple[int, int], ...], page_size:
     """In place: of every layer's pages (`pages` [layers, pages, ...], contiguous, of whatever type; `rows`: what a page holds, as for
     `copy_pages`), the i-th kept token's rows go to where the i-th token behind the request's `held` positions (int32 [requests]; below 0: nothing) is
     stored. Other drafted tokens' rows are what they were, or a kept one's. -> `pages`"""
-    what = "keep_rows"
-    path, kept, int32 = accepted.path, accepted.kept, torch.int32
-    index = pages.get_device()
-    if block_table.dim() != 2 or path.dim() != 2 or pages.dim() < 3:
-        raise KernelError(f"{what} takes pages [layers, pages, ...], a block table [requests, pages] and paths [requests, tokens]")
-    (n, width), most, shape, item = block_table.shape, path.shape[1], pages.shape, pages.element_size()
-    _like(what, "block_table", block_table, int32, index, (n, width))
-    _like(what, "held", held, int32, index, (n,))
-    _like(what, "path", path, int32, index, (n, most))
-    _like(what, "kept", kept, int32, index, (n,))
-    if not pages.is_contiguous():
-        raise KernelError(f"{what} takes contiguous pages")
-    elements = math.prod(shape[2:])
-    kinds = _page_kinds(rows, page_size, elements, item)
-    if not 1 <= most <= MOST_DRAFTED or not 1 <= n or width < 1 or not 1 <= shape[0] <= 65535 or shape[1] < 1:
-        raise KernelError(f"{what} takes a request or more, with paths of 1 to {MOST_DRAFTED} tokens, and pages of a layer or more")
-    stream, at = _current(what, index), kinds.buffer_info()[0]
-    fn = _entry("drafted", "omnia_keep_rows", [c_void_p, c_longlong, c_longlong, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_int,
-                                               c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p])
-    _check(fn(pages.data_ptr(), shape[1] * elements * item, elements * item, shape[0], shape[1], page_size, at, at + 4 * len(rows), len(rows),
-              block_table.data_ptr(), width, held.data_ptr(), path.data_ptr(), kept.data_ptr(), n, most, _error_address(index), stream), what)
+    _host().keep_rows(_address("drafted", "omnia_keep_rows", index=pages.get_device()), pages, rows, page_size, block_table, held, accepted.path, accepted.kept)
+    _launched()
     return pages
 
 
@@ -1480,9 +1375,6 @@ takes the head size and the pages; with more than 16 rows from so many keys on, 
 are as many as the memory's rate allows, and the tcgen05 kernel has a beginning and an end of 15 us. 16/8 heads of 128, us with mma.sync / tcgen05: 8
 requests of 500 positions with 8, 16, 32 tokens 29 / 30, 23 / 31, 33 / 31; of 4,096 46 / 51, 50 / 48, 69 / 55; of 20,000 141 / 138, 160 / 137, 210 / 139;
 one of 4,096 with 16 tokens 32 / 27, of 60,000 with 5 71 / 67, with 64 168 / 81."""
-
-_TREE = struct.Struct("14Pq16i2f")  # TreeAttention in attention_tree.cuh
-
 
 @functools.lru_cache(maxsize=4096)
 def tree_plan(tiles: int, keys: int, step: int, places: int) -> tuple[int, int]:
@@ -1501,49 +1393,21 @@ def tree_attention(q: torch.Tensor, kv: KVView, step: StepContext, scale: float,
     `gate`, `sink`, `window`, `keep_first`, `chunk`, `softcap` as for `paged_attention`, by the tokens' positions. A token that sees nothing
     has zeros. -> [tokens, nq * dv] (rows behind the last request's are not written)"""
     what = "tree_attention"
-    tree = step.tree
+    tree, pages, spec = step.tree, kv.pages, kv.spec
     if tree is None:
         raise KernelError(f"{what} takes a step of drafted trees")
-    if q.dim() != 3 or not q.is_contiguous():
+    if q.dim() != 3:
         raise KernelError(f"{what} takes contiguous queries [tokens, heads, width]")
-    index, int32 = q.get_device(), torch.int32
-    tokens, nq, d = q.shape
-    dtype, pages, table, n, most = q.dtype, kv.pages, kv.block_table, step.num_seqs, step.max_q_len
-    k_ptr, v_ptr, page_stride, nkv, dk, dv = kv_layout(kv)
-    code = _code(dtype)
-    if dk != d or nq % nkv or pages.dtype is not dtype or not 1 <= d <= 512 or not 1 <= dv <= 512 or not pages.is_contiguous() or \
-            pages.get_device() != index:
-        raise KernelError(f"{what}: {nq} heads of {d} ({dtype}, {q.device}) do not go with a cache of {nkv} heads of {dk} and {dv} "
-                          f"({pages.dtype}, {pages.device})")
-    if kv.spec is not None and kv.spec.stride != 1:
+    _, nq, d = q.shape
+    (nkv, dk), (_, dv) = spec.rows if spec is not None else ((pages.shape[2], pages.shape[4]),) * 2
+    if spec is not None and spec.stride != 1:
         raise KernelError(f"{what} takes a cache of a row for every position")
-    if table.dim() != 2 or tree.ancestors.dim() != 2:
-        raise KernelError(f"{what} takes a block table [requests, pages] and ancestors [tokens, words]")
-    width, words = table.shape[1], tree.ancestors.shape[1]
-    _like(what, "ancestors", tree.ancestors, int32, index, (tokens, words))
-    _like(what, "positions", step.positions, int32, index, (tokens,))
-    _like(what, "block_table", table, int32, index, (n, width))
-    _like(what, "cu_seqlens", step.cu_seqlens, int32, index, (n + 1,))
-    _like(what, "seq_lens", step.seq_lens, int32, index, (n,))
-    if not 1 <= most <= 32 * words <= MOST_DRAFTED or n < 1:
-        raise KernelError(f"{what}: a request brings up to {most} tokens, the tree has {words} words for each ({MOST_DRAFTED} tokens at most)")
-    gate_ptr = gate_stride = 0
-    if gate is not None:
-        if gate.dtype is not dtype or gate.dim() != 2 or gate.stride(1) != 1 or gate.shape[0] != tokens or gate.get_device() != index or \
-                not 0 <= gate_col <= gate.shape[1] - nq * dv:
-            raise KernelError(f"{what}: the gate's {nq * dv} columns from {gate_col} on lie outside rows of {list(gate.shape)}, or are no {dtype}")
-        gate_ptr, gate_stride = gate.data_ptr() + gate_col * dtype.itemsize, gate.stride(0)
-    if sink is not None:
-        _like(what, "sink", sink, torch.float32, index, (nq,))
     window = (kv.window if window == -1 else window) or 0
     keep = (kv.keep_first if keep_first is None else keep_first) if window else 0
-    run = int(chunk or 0)
+    run, page_size, n, most = int(chunk or 0), kv.page_size, step.num_seqs, step.max_q_len
     if run and keep:
         raise KernelError("a mask of runs keeps no first positions")
-    stream, device = _current(what, index), q.device
-    out = torch.empty(tokens, nq * dv, dtype=dtype, device=device)
-    if tokens == 0:
-        return out
+    index, base, bf16 = q.get_device(), pages.data_ptr(), q.dtype is torch.bfloat16
     rows = most * (nq // nkv)
     # What the longest request can see: plans are made for that, and from numbers that a captured step knows too.
     keys = max(step.max_seq_len, 1)
@@ -1551,45 +1415,29 @@ def tree_attention(q: torch.Tensor, kv: KVView, step: StepContext, scale: float,
         keys = min(keys, window + keep + most)
     if run:
         keys = min(keys, run + most)
-    q_ptr, sms = q.data_ptr(), sm_count(device)
-    tensor_cores = dv == d and dtype is torch.bfloat16 and d % 8 == 0 and d <= 256 and n <= 1024 and not k_ptr & 15 and not q_ptr & 3
-    many = tensor_cores and (rows >= TREE_MANY_ROWS or (rows > 16 and keys >= TREE_MANY_KEYS)) and d in (64, 128) and kv.page_size % 16 == 0 and scale > 0 and not q_ptr & 15 and nq // nkv <= 128
-    shares32 = dv == d and dtype is torch.float32 and d % 4 == 0 and d <= 256 and n <= 1024 and not (k_ptr | v_ptr) & 15 and page_stride % 4 == 0
-    if many:
-        tile = 2 * (128 // (nq // nkv) * (nq // nkv))
-        a_chunk, a_parts = 0, min(sms, n * nkv * -(-rows // tile) * -(-keys // 128))
-        slots = 2 * a_parts * tile
-    elif tensor_cores:
-        tile = 16 if rows <= 16 else 32 if rows <= 32 or d > 128 else 64
-        a_chunk, a_parts = 0, min((2 if d <= 128 else 1) * sms, n * nkv * -(-rows // tile) * -(-keys // 64))
-        slots = 2 * a_parts * tile
-    elif shares32:
-        places = 4 if d <= 32 else 2 if d <= 128 else 1
-        a_chunk, a_parts = 0, min(places * sms, n * nkv * -(-rows // 32) * -(-keys // (64 if d <= 64 else 32)))
-        slots = 2 * a_parts * 32
+    sms = sm_count(q.device) if index >= 0 else 1
+    equal = dv == d and n <= 1024 and not base & 15  # what every kernel by equal shares takes
+    chunk_keys = tile = merge = 0
+    if equal and bf16 and d % 8 == 0 and d <= 256 and not q.data_ptr() & 3:
+        if (rows >= TREE_MANY_ROWS or (rows > 16 and keys >= TREE_MANY_KEYS)) and d in (64, 128) and page_size % 16 == 0 and scale > 0 and \
+                not q.data_ptr() & 15 and nq // nkv <= 128:
+            kind, entry, tile = 0, _address("attention_tree_tcgen05", "omnia_tree_attention_tcgen05", d, index), 2 * (128 // (nq // nkv) * (nq // nkv))
+            parts = min(sms, n * nkv * -(-rows // tile) * -(-keys // 128))
+        else:
+            kind, entry, tile = 1, _address("attention_tree_tc", "omnia_tree_attention_tc", d, index), 16 if rows <= 16 else 32 if rows <= 32 or d > 128 else 64
+            parts = min((2 if d <= 128 else 1) * sms, n * nkv * -(-rows // tile) * -(-keys // 64))
+        slots = 2 * parts * tile
+    elif equal and q.dtype is torch.float32 and d % 4 == 0 and d <= 256:
+        kind, entry = 0, _address("attention_tree", "omnia_tree_attention32", index=index)
+        parts = min((4 if d <= 32 else 2 if d <= 128 else 1) * sms, n * nkv * -(-rows // 32) * -(-keys // (64 if d <= 64 else 32)))
+        slots = 2 * parts * 32
     else:
-        a_chunk, a_parts = tree_plan(-(-rows // 32) * n * nkv, keys, 64, 2 * sms)
-        slots = a_parts * tokens * nq if a_parts > 1 else 0
-    part_o = torch.empty(slots * (dv + 2), dtype=torch.float32, device=device).data_ptr() if slots else 0
-    packed = _TREE.pack(
-        q_ptr, k_ptr, v_ptr, gate_ptr, out.data_ptr(), table.data_ptr(), step.cu_seqlens.data_ptr(), step.seq_lens.data_ptr(),
-        step.positions.data_ptr(), tree.ancestors.data_ptr(), 0 if sink is None else sink.data_ptr(), part_o, part_o + 4 * slots * dv,
-        _error_address(index), page_stride, tokens, n, width, pages.shape[0], nq, nkv, d, dv, kv.page_size, gate_stride, words, window, keep, run,
-        a_chunk, a_parts, scale, softcap or 0.0)
-    if many:
-        fn = _entry("attention_tree_tcgen05", "omnia_tree_attention_tcgen05", [c_void_p, c_int, c_int, c_void_p], {"HEAD_DIM": d})
-        _check(fn(packed, most, a_parts, stream), what)
-        return out
-    if tensor_cores:
-        fn = _entry("attention_tree_tc", "omnia_tree_attention_tc", [c_void_p, c_int, c_int, c_int, c_void_p], {"HEAD_DIM": d})
-        _check(fn(packed, most, tile, a_parts, stream), what)
-        return out
-    if shares32:
-        _check(_entry("attention_tree", "omnia_tree_attention32", [c_void_p, c_int, c_int, c_void_p])(packed, most, a_parts, stream), what)
-        return out
-    _check(_entry("attention_tree", "omnia_tree_attention", [c_void_p, c_int, c_int, c_void_p])(packed, most, code, stream), what)
-    if a_parts > 1:
-        _check(_entry("attention_tree", "omnia_tree_merge", [c_void_p, c_int, c_void_p])(packed, code, stream), what)
+        kind, entry, merge = 2, _address("attention_tree", "omnia_tree_attention", index=index), _address("attention_tree", "omnia_tree_merge", index=index)
+        chunk_keys, parts = tree_plan(-(-rows // 32) * n * nkv, keys, 64, 2 * sms)
+        slots = parts * q.shape[0] * nq if parts > 1 else 0
+    out = _host().tree_attention(entry, merge, kind, q, pages, kv.block_table, step.cu_seqlens, step.seq_lens, step.positions, tree.ancestors, gate, gate_col,
+                                 sink, nkv, dk, dv, page_size, n, most, window, keep, run, chunk_keys, parts, slots, tile, scale, softcap or 0.0)
+    _launched()
     return out
 
 
@@ -2194,9 +2042,6 @@ class DraftedRows(NamedTuple):
     rows: torch.Tensor
 
 
-_ADJUST = struct.Struct("21P4q9i4x")  # AdjustLogits in logits.cu
-
-
 def adjust_logits(logits: torch.Tensor, *, history: TokenHistory | None = None, repetition: torch.Tensor | None = None,
                   frequency: torch.Tensor | None = None, presence: torch.Tensor | None = None, contexts: torch.Tensor | None = None,
                   requests: torch.Tensor | None = None, bias: LogitBias | None = None, masks: TokenMasks | None = None,
@@ -2209,86 +2054,10 @@ def adjust_logits(logits: torch.Tensor, *, history: TokenHistory | None = None, 
     [requests]: 1, 0 and 0 where None; `contexts` int32 [requests]: the repetition penalty sees so many of the last tokens (0 or None: all).
     `out`: None for a new tensor; `logits` itself: in place, which reads and writes only what changes; or another tensor of the same shape that
     shares no memory with it."""
-    what = "adjust_logits"
-    if logits.dim() != 2 or logits.dtype is not torch.float32 or logits.stride(1) != 1:
-        raise KernelError(f"{what} takes float32 logits [rows, vocab] whose rows lie in one piece")
-    index, int32, (rows, vocab), stride = logits.get_device(), torch.int32, logits.shape, logits.stride(0)
-    if rows > 1 and stride < vocab:
-        raise KernelError(f"{what} takes rows that lie apart")
-    num, of_history, penalised = rows, (0, 0, 0, 0), 0
-    if history is not None:
-        num = _list_of(what, "lengths", history.lengths, int32, index)
-        _list_of(what, "tokens", history.tokens, int32, index)
-        _like(what, "starts", history.starts, torch.int64, index, (num,))
-        _like(what, "prompts", history.prompts, int32, index, (num,))
-        of_history = (history.tokens.data_ptr(), history.starts.data_ptr(), history.lengths.data_ptr(), history.prompts.data_ptr())
-    elif contexts is not None:
-        raise KernelError(f"{what}: penalties go by the requests' history")
-    of_penalties = []
-    for name, t in (("repetition", repetition), ("frequency", frequency), ("presence", presence)):
-        if t is None:
-            of_penalties.append(0)
-            continue
-        if history is None:
-            raise KernelError(f"{what}: penalties go by the requests' history")
-        _like(what, name, t, torch.float32, index, (num,))
-        of_penalties.append(t.data_ptr())
-        penalised = 1
-    if contexts is not None:
-        _like(what, "contexts", contexts, int32, index, (num,))
-    of_bias, entries = (0, 0, 0), 0
-    if bias is not None:
-        entries = _list_of(what, "ids", bias.ids, int32, index)
-        if history is None:
-            num = _list_of(what, "bias starts", bias.starts, int32, index) - 1
-        _like(what, "bias starts", bias.starts, int32, index, (num + 1,))
-        _like(what, "values", bias.values, torch.float32, index, (entries,))
-        of_bias = (bias.ids.data_ptr(), bias.values.data_ptr(), bias.starts.data_ptr())
-    if requests is not None:
-        _like(what, "requests", requests, int32, index, (rows,))
-    elif num < rows and (history is not None or bias is not None):
-        raise KernelError(f"{what}: {rows} rows of {num} requests need `requests`")
-    of_masks, count, width = (0, 0), 0, 0
-    if masks is not None:
-        if masks.words.dim() != 2 or masks.words.shape[1] * 32 < vocab:
-            raise KernelError(f"{what}: masks are [masks, words] of {vocab} tokens, 32 a word, not {list(masks.words.shape)}")
-        count, width = masks.words.shape
-        _like(what, "mask words", masks.words, int32, index, (count, width))
-        _like(what, "mask rows", masks.rows, int32, index, (rows,))
-        of_masks = (masks.words.data_ptr(), masks.rows.data_ptr())
-    of_drafted, words, tokens = (0, 0, 0, 0), 0, 0
-    if drafted is not None:
-        ancestors = drafted.tree.ancestors
-        if ancestors.dim() != 2 or (history is not None and requests is None):
-            raise KernelError(f"{what}: drafted rows need `requests`, and a tree of [tokens, words]")
-        tokens, words = ancestors.shape
-        _like(what, "ancestors", ancestors, int32, index, (tokens, words))
-        _like(what, "token_ids", drafted.token_ids, int32, index, (tokens,))
-        _like(what, "drafted rows", drafted.rows, int32, index, (rows,))
-        _like(what, "cu_seqlens", drafted.cu_seqlens, int32, index, (num + 1,) if history is not None else drafted.cu_seqlens.shape)
-        if penalised:
-            of_drafted = (ancestors.data_ptr(), drafted.token_ids.data_ptr(), drafted.cu_seqlens.data_ptr(), drafted.rows.data_ptr())
-    same = out is logits
-    if out is None:
-        out = torch.empty(rows, vocab, dtype=torch.float32, device=logits.device)
-        out_ptr, out_stride, in_ptr = out.data_ptr(), vocab, logits.data_ptr()
-    else:
-        if out.dtype is not torch.float32 or out.shape != logits.shape or out.stride(1) != 1 or out.get_device() != index or \
-                (rows > 1 and out.stride(0) < vocab):
-            raise KernelError(f"{what} writes float32 rows that lie apart, in the logits' shape")
-        out_ptr, out_stride, in_ptr = out.data_ptr(), out.stride(0), logits.data_ptr()
-        same = same or (out_ptr == in_ptr and out_stride == stride)
-        if not same and rows and out_ptr < in_ptr + 4 * ((rows - 1) * stride + vocab) and in_ptr < out_ptr + 4 * ((rows - 1) * out_stride + vocab):
-            raise KernelError(f"{what} writes to the logits themselves, or to a tensor that shares no memory with them")
-    stream = _current(what, index)
-    if rows == 0 or vocab == 0:
-        return out
-    packed = _ADJUST.pack(
-        in_ptr, out_ptr, 0 if requests is None else requests.data_ptr(), *of_history, 0 if contexts is None else contexts.data_ptr(), *of_penalties,
-        *of_bias, *of_masks, *of_drafted, _error_address(index), stride, out_stride, 0 if history is None else history.tokens.shape[0], entries,
-        rows, vocab, num, count, width, words, tokens, 0, penalised)
-    _check(_entry("logits", "omnia_adjust_logits", [c_void_p, c_int, c_void_p])(packed, same, stream), what)
-    return out
+    made = _host().adjust_logits(_address("logits", "omnia_adjust_logits", index=logits.get_device()), logits, history, repetition, frequency, presence, contexts,
+                                 requests, bias, masks, drafted, out)
+    _launched()
+    return made
 
 
 # ------------------------------------------------------------------------------------
