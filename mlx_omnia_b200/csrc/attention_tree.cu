@@ -261,10 +261,14 @@ __global__ void __launch_bounds__(THREADS, Shares32<MOST>::PLACES) tree_shares32
   pdl_launch_dependents();
   const TreeShares shares = {ROWS, KEYS, 1, S::EXTRA};
   const long long total = shares.lay_out(a, ends, sums), blocks = min((long long)gridDim.x, total);
-  if (blockIdx.x >= blocks) return;
-  const long long t0 = total * blockIdx.x / blocks;
   TreePlace ahead;
-  ahead.find(a, shares, ends, t0, (int)(total * (blockIdx.x + 1) / blocks - t0));
+  if (blockIdx.x >= blocks) {
+    if (threadIdx.x == 0) tree_border(a, shares, total, blocks, 0, 0, ahead);
+    return;
+  }
+  const long long t0 = total * blockIdx.x / blocks;
+  const long long begin = ahead.find(a, shares, ends, t0, (int)(total * (blockIdx.x + 1) / blocks - t0));
+  if (threadIdx.x == 0) tree_border(a, shares, total, blocks, t0, begin, ahead);
   if (ahead.left == 0) return;
   TreePlace now = ahead;
   __syncthreads();

@@ -14,6 +14,7 @@ struct TreeAttention {
   const float* sink;                         // [nq] or null
   float *part_o, *part_ml;                   // [parts, tokens, nq, dv] unnormalised, [parts, tokens, nq, 2] (offset in log2 units, sum)
   int* err;
+  int4* borders;                             // of the kernels by equal shares: two a block, what the join does at the block's beginning
   long long page_stride;
   int tokens, requests, max_pages, num_pages, nq, nkv, d, dv, page_size, gate_stride, words, window, keep, run, chunk, parts;
   float scale, softcap;
@@ -149,6 +150,26 @@ struct TreePlace {
   }
 };
 
+// What the join does at the border ahead of block `block`, which begins at place `at` in an item whose places begin at `begin`: nothing, unless the border
+// lies between tiles of that item and is the first that does. (One thread of every block of the kernel, those that have no share too.)
+__device__ __forceinline__ void tree_border(const TreeAttention& a, const TreeShares& s, long long total, long long blocks, long long at, long long begin,
+                                            const TreePlace& place) {
+  const int block = blockIdx.x;
+  int4 item = make_int4(-1, 0, 0, 0), slots = make_int4(0, 0, 0, 0);
+  if (block > 0 && block < blocks) {
+    const long long first = begin + s.extra, end = first + place.tiles, before = total * (block - 1) / blocks;  // `first`: its first tile's place
+    if (first < at && first >= before) {
+      int last = block;
+      while (total * (last + 1) / blocks < end) ++last;
+      const int row0 = place.row_tile * s.rows, rows = min(s.rows, place.k.count * (a.nq / a.nkv) - row0);
+      item = make_int4(place.k.first, place.head, row0, rows);
+      // The block that the item begins in may have begun in another item, the others have begun in this one.
+      slots = make_int4(2 * (block - 1) + (begin <= before ? 0 : 1), 2 * block, last - block + 1, 0);
+    }
+  }
+  a.borders[2 * block] = item, a.borders[2 * block + 1] = slots;
+}
+
 constexpr int TREE_JOIN_WARPS = 4;
 
 __device__ __forceinline__ float tree_exp2(float x) {
@@ -167,16 +188,14 @@ __device__ __forceinline__ unsigned tree_pair(float lo, float hi) {
   return *reinterpret_cast<const unsigned*>(&v);
 }
 
-// An item that several blocks had part in, put together by the blocks of the grid that stand for the first border in it (between block x and block
-// x + 1 of the kernel before): a warp a row at a time, the slots in the order of their blocks, the sink, the gate. The last `requests` blocks
-// write zeros for requests that see nothing. The rows of an item are shared out over the grid's other axis.
+// An item that several blocks had part in, put together by the blocks of the grid that stand for the first border in it: a warp a row, the slots in the
+// order of their blocks, eight on their way at once, the sink, the gate. The last `requests` blocks write zeros for requests that see nothing. The rows of
+// an item are shared out over the grid's other axis.
 template <typename T, int MOST>
 __global__ void __launch_bounds__(32 * TREE_JOIN_WARPS) tree_join_kernel(const __grid_constant__ TreeAttention a, const TreeShares shares, int grid, int most) {
-  constexpr int WARPS = TREE_JOIN_WARPS;
-  const int D = a.d;  // a multiple of 4, MOST at most
+  constexpr int WARPS = TREE_JOIN_WARPS, PER = (MOST + 127) / 128;  // four dims a lane
   constexpr float LOG2E = 1.4426950408889634f;
-  __shared__ long long ends[TREE_MOST_REQUESTS], sums[WARPS];
-  // (What is read ahead of the wait was there ahead of the kernel that this one waits for.)
+  const int D = a.d;  // a multiple of 4, MOST at most
   const int rows_of_tile = shares.rows, group = a.nq / a.nkv, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, step = WARPS * gridDim.y;
   if ((int)blockIdx.x >= grid - 1) {
     const TreeKeys k = tree_keys(a, blockIdx.x - (grid - 1), shares.align);
@@ -187,61 +206,56 @@ __global__ void __launch_bounds__(32 * TREE_JOIN_WARPS) tree_join_kernel(const _
       for (int c = lane; c < D; c += 32) static_cast<T*>(a.out)[((size_t)k.first * a.nq + r) * D + c] = from_f32<T>(0.f);
     return;
   }
-  const long long total = shares.lay_out(a, ends, sums), blocks = min((long long)grid, total);
-  const int border = blockIdx.x + 1;
-  if (border >= blocks) return;
-  const long long at = total * border / blocks;
-  TreePlace place;
-  const long long begin = place.find(a, shares, ends, at, 1), first = begin + shares.extra, end = first + place.tiles;  // `first`: its first tile's
-  if (first >= at || first < total * (border - 1) / blocks) return;  // no border between tiles, or not the item's first
-  const int b0 = border - 1;
-  int b1 = border;
-  while (total * (b1 + 1) / blocks < end) ++b1;
-  // The block that the item begins in may have begun in another item, the others have begun in this one.
-  const int slot0 = 2 * b0 + (begin <= total * b0 / blocks ? 0 : 1);
-  auto slot_of = [&](int b) { return b == b0 ? slot0 : 2 * b; };
-  const TreeKeys& k = place.k;
-  const int head_kv = place.head, here = min(rows_of_tile, k.count * group - place.row_tile * rows_of_tile);
-  OMNIA_TRACE_BLOCK(2);
   pdl_wait();
   pdl_launch_dependents();
-  OMNIA_TRACE_BLOCK(3);
-  for (int r = blockIdx.y * WARPS + warp; r < here; r += step) {
-    const int in = place.row_tile * rows_of_tile + r;
-    const int token = k.first + in / group, head = head_kv * group + in % group;
+  const int4 item = a.borders[2 * (blockIdx.x + 1)], slots = a.borders[2 * (blockIdx.x + 1) + 1];
+  if (item.x < 0) return;
+  const int parts = slots.z + 1;
+  for (int r = blockIdx.y * WARPS + warp; r < item.w; r += step) {
+    const int in = item.z + r, token = item.x + in / group, head = item.y * group + in % group;
     const float sink = a.sink ? a.sink[head] * LOG2E : -INFINITY;
-    constexpr int PER = (MOST + 127) / 128;  // four dims a lane
+    float gates[PER][4];
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int c = (32 * i + lane) * 4 + j;
+        gates[i][j] = a.gate && c < D ? to_f32(static_cast<const T*>(a.gate)[(size_t)token * a.gate_stride + head * D + c]) : 0.f;
+      }
     float4 sum[PER];
 #pragma unroll
     for (int i = 0; i < PER; ++i) sum[i] = make_float4(0.f, 0.f, 0.f, 0.f);
     float base = -INFINITY, l = 0.f;
-    for (int c0 = b0; c0 <= b1; c0 += 32) {  // 32 slots at a time, a lane each for their offsets and sums
-      const int b = c0 + lane;
-      float ml = -INFINITY, ll = 0.f;
-      size_t row = 0;
-      if (b <= b1) {
-        row = (size_t)slot_of(b) * rows_of_tile + r;
-        const float2 x = reinterpret_cast<const float2*>(a.part_ml)[row];
-        ml = x.x, ll = x.y;
-      }
-      const float over = fmaxf(base, warp_max(ml)), offset = over == -INFINITY ? 0.f : over, f = tree_exp2(base - offset), w = tree_exp2(ml - offset);
-      l = l * f + warp_sum(ll * w);
+    for (int p0 = 0; p0 < parts; p0 += 8) {
+      float2 ml[8];
+      float4 x[8][PER];
 #pragma unroll
-      for (int i = 0; i < PER; ++i) sum[i].x *= f, sum[i].y *= f, sum[i].z *= f, sum[i].w *= f;
-      base = over;
-      const int here = min(32, b1 - c0 + 1);
-#pragma unroll 4
-      for (int p = 0; p < here; ++p) {
-        const float by = __shfl_sync(0xffffffffu, w, p);
-        const float* from = a.part_o + (size_t)((size_t)slot_of(c0 + p) * rows_of_tile + r) * D;
+      for (int u = 0; u < 8; ++u) {
+        const int p = p0 + u;
+        const size_t row = (size_t)(p == 0 ? slots.x : slots.y + 2 * (p - 1)) * rows_of_tile + r;
+        ml[u] = p < parts ? reinterpret_cast<const float2*>(a.part_ml)[row] : make_float2(-INFINITY, 0.f);
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
           const int c = (32 * i + lane) * 4;
-          if (c < D && by != 0.f) {
-            const float4 v = *reinterpret_cast<const float4*>(from + c);
-            sum[i].x = fmaf(v.x, by, sum[i].x), sum[i].y = fmaf(v.y, by, sum[i].y);
-            sum[i].z = fmaf(v.z, by, sum[i].z), sum[i].w = fmaf(v.w, by, sum[i].w);
-          }
+          x[u][i] = p < parts && c < D ? *reinterpret_cast<const float4*>(a.part_o + row * D + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+      }
+      float over = base;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) over = fmaxf(over, ml[u].x);
+      const float offset = over == -INFINITY ? 0.f : over, f = tree_exp2(base - offset);
+      base = over, l *= f;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) sum[i].x *= f, sum[i].y *= f, sum[i].z *= f, sum[i].w *= f;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const float w = tree_exp2(ml[u].x - offset);
+        if (w == 0.f) continue;  // (what it came to then need not be a number)
+        l = fmaf(ml[u].y, w, l);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          sum[i].x = fmaf(x[u][i].x, w, sum[i].x), sum[i].y = fmaf(x[u][i].y, w, sum[i].y);
+          sum[i].z = fmaf(x[u][i].z, w, sum[i].z), sum[i].w = fmaf(x[u][i].w, w, sum[i].w);
         }
       }
     }
@@ -256,7 +270,7 @@ __global__ void __launch_bounds__(32 * TREE_JOIN_WARPS) tree_join_kernel(const _
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         if (by == 0.f) y[j] = 0.f;
-        if (a.gate) y[j] *= tree_sigmoid(to_f32(static_cast<const T*>(a.gate)[(size_t)token * a.gate_stride + head * D + c + j]));
+        if (a.gate) y[j] *= tree_sigmoid(gates[i][j]);
       }
       T* to = static_cast<T*>(a.out) + (size_t)token * a.nq * D + head * D + c;
       if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(to) = make_uint2(tree_pair(y[0], y[1]), tree_pair(y[2], y[3]));

@@ -90,15 +90,19 @@ __global__ void __launch_bounds__(THREADS, D <= 128 ? 2 : 1) tree_shares_kernel(
   const TreeShares shares = {ROWS, KEYS, 1, EXTRA};
   const long long total = shares.lay_out(a, ends, sums);
   const long long blocks = min((long long)gridDim.x, total);  // (a block more than there are tiles would leave its slots unwritten)
-  if (blockIdx.x >= blocks) return;
+  TreePlace ahead;
+  if (blockIdx.x >= blocks) {
+    if (threadIdx.x == 0) tree_border(a, shares, total, blocks, 0, 0, ahead);
+    return;
+  }
   const long long t0 = total * blockIdx.x / blocks;
   const int group = a.nq / a.nkv;
   const bf16 *kp = static_cast<const bf16*>(a.k_pages), *vp = static_cast<const bf16*>(a.v_pages);
   const long long apart = vp - kp;
 
   // ---- loads: lane l < 16 knows where the l-th row of its warp's share of a tile lies ------------------------------------------------
-  TreePlace ahead;
-  ahead.find(a, shares, ends, t0, (int)(total * (blockIdx.x + 1) / blocks - t0));
+  const long long begin = ahead.find(a, shares, ends, t0, (int)(total * (blockIdx.x + 1) / blocks - t0));
+  if (tid == 0) tree_border(a, shares, total, blocks, t0, begin, ahead);
   if (ahead.left == 0) return;
   TreePlace now = ahead;
   OMNIA_TRACE_BLOCK(2);  // the shares are known

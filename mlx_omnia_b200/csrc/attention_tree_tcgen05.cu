@@ -129,9 +129,10 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_con
   const long long blocks = min((long long)gridDim.x, total);
   TreePlace place;  // (one warp's)
   place.left = 0;
-  if (blockIdx.x < blocks && warp == WARP_INIT) {
-    const long long t0 = total * blockIdx.x / blocks;
-    place.find(a, shares, ends, t0, (int)(total * (blockIdx.x + 1) / blocks - t0));
+  if (warp == WARP_INIT) {
+    long long t0 = 0, begin = 0;
+    if (blockIdx.x < blocks) t0 = total * blockIdx.x / blocks, begin = place.find(a, shares, ends, t0, (int)(total * (blockIdx.x + 1) / blocks - t0));
+    if (lane == 0) tree_border(a, shares, total, blocks, t0, begin, place);
   }
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // (the ends lie where copies will come to)
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");

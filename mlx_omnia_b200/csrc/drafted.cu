@@ -225,12 +225,12 @@ struct KeepRows {
   const int *table, *held, *path, *kept;
   int* err;
   long long layer_bytes, page_bytes;
-  int requests, num_pages, page_size, width, most, kinds, units;  // units: of U bytes, of a position's rows of all kinds
+  int requests, layers, num_pages, page_size, width, most, kinds, units;  // units: of U bytes, of a position's rows of all kinds
   int heads[MOST_KINDS], row_units[MOST_KINDS];                   // of each kind: heads, units of a head's row
 };
 
-// A block has one request's kept rows in one layer, a thread a unit of U bytes of a position's rows in turn: it reads eight kept positions' and
-// then writes them. A row goes to its own place or to an earlier one, and the rows of a path come in order, so what is written was
+// A block has one request's kept rows in some layers, a thread a unit of U bytes of a position's rows in turn: it reads four kept positions' in two
+// layers and then writes them. A row goes to its own place or to an earlier one, and the rows of a path come in order, so what is written was
 // read before, or belongs to a draft that is not kept.
 template <typename U>
 __global__ void __launch_bounds__(THREADS) keep_rows_kernel(const __grid_constant__ KeepRows a) {
@@ -261,7 +261,6 @@ __global__ void __launch_bounds__(THREADS) keep_rows_kernel(const __grid_constan
     to[j] = good ? (long long)target * a.page_size + ((long long)held + j) % a.page_size : -1;
   }
   __syncthreads();
-  char* layer = a.pages + blockIdx.y * a.layer_bytes;
   for (int unit = j; unit < a.units; unit += THREADS) {
     int rest = unit, kind = 0;
     long long base = 0;
@@ -272,18 +271,23 @@ __global__ void __launch_bounds__(THREADS) keep_rows_kernel(const __grid_constan
     }
     const int width = a.row_units[kind], head = rest / width, column = rest % width;
     base += (long long)head * a.page_size * width + column;
-    auto at = [&](long long row) {
-      return reinterpret_cast<U*>(layer + row / a.page_size * a.page_bytes) + base + row % a.page_size * width;
+    auto at = [&](int layer, long long row) {
+      return reinterpret_cast<U*>(a.pages + layer * a.layer_bytes + row / a.page_size * a.page_bytes) + base + row % a.page_size * width;
     };
-    for (int i0 = skip; i0 < count; i0 += 8) {
-      U held_rows[8];
+    for (int l0 = blockIdx.y; l0 < a.layers; l0 += 2 * gridDim.y)
+      for (int i0 = skip; i0 < count; i0 += 4) {
+        U held_rows[2][4];
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (i0 + i < count && from[i0 + i] >= 0) held_rows[i] = *at(from[i0 + i]);
+        for (int l = 0; l < 2; ++l)
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (i0 + i < count && from[i0 + i] >= 0) *at(to[i0 + i]) = held_rows[i];
-    }
+          for (int i = 0; i < 4; ++i)
+            if (l0 + l * (int)gridDim.y < a.layers && i0 + i < count && from[i0 + i] >= 0) held_rows[l][i] = *at(l0 + l * gridDim.y, from[i0 + i]);
+#pragma unroll
+        for (int l = 0; l < 2; ++l)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (l0 + l * (int)gridDim.y < a.layers && i0 + i < count && from[i0 + i] >= 0) *at(l0 + l * gridDim.y, to[i0 + i]) = held_rows[l][i];
+      }
   }
 }
 
@@ -323,12 +327,14 @@ extern "C" int omnia_keep_rows(void* pages, long long layer_bytes, long long pag
   KeepRows a = {};
   a.pages = (char*)pages, a.table = table, a.held = held, a.path = path, a.kept = kept, a.err = err;
   a.layer_bytes = layer_bytes, a.page_bytes = page_bytes;
-  a.requests = requests, a.num_pages = num_pages, a.page_size = page_size, a.width = width, a.most = most, a.kinds = kinds;
+  a.requests = requests, a.layers = layers, a.num_pages = num_pages, a.page_size = page_size, a.width = width, a.most = most, a.kinds = kinds;
   long long all = (long long)(uintptr_t)pages | layer_bytes | page_bytes;
   for (int k = 0; k < kinds; ++k) all |= bytes[k];
   const int unit = all % 16 == 0 ? 16 : all % 8 == 0 ? 8 : all % 4 == 0 ? 4 : all % 2 == 0 ? 2 : 1;
   for (int k = 0; k < kinds; ++k) a.heads[k] = heads[k], a.row_units[k] = bytes[k] / unit, a.units += heads[k] * a.row_units[k];
-  const dim3 grid(requests, layers);
+  // Blocks that the GPU holds at once, each with as many layers as that takes. (64 requests in 36 layers, a block each: 15 us.)
+  const int room = 6 * omnia_sm_count() / requests;
+  const dim3 grid(requests, room < 1 ? 1 : room < layers ? room : layers);
   const cudaStream_t s = (cudaStream_t)stream;
   if (unit == 16) launch_pdl(keep_rows_kernel<uint4>, grid, dim3(THREADS), 0, s, a);
   else if (unit == 8) launch_pdl(keep_rows_kernel<uint2>, grid, dim3(THREADS), 0, s, a);
