@@ -250,8 +250,8 @@ __global__ void __launch_bounds__(32 * TREE_JOIN_WARPS) tree_join_kernel(const _
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
         const float w = tree_exp2(ml[u].x - offset);
-        if (w == 0.f) continue;  // (what it came to then need not be a number)
-        l = fmaf(ml[u].y, w, l);
+        l = fmaf(ml[u].y, w, l);  // (no number where a row's scores are none: their maximum is then -infinity)
+        if (w == 0.f) continue;   // (what it came to then need not be a number)
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
           sum[i].x = fmaf(x[u][i].x, w, sum[i].x), sum[i].y = fmaf(x[u][i].y, w, sum[i].y);
