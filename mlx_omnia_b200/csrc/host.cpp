@@ -19,6 +19,7 @@ namespace {
 constexpr int64_t MOST_DRAFTED = 256, MOST_GROUPS = 8, MOST_KINDS = 8;
 
 PyObject* kernel_error = nullptr;   // ops.KernelError
+PyObject* memory_error = nullptr;   // torch.OutOfMemoryError
 PyObject* error_address = nullptr;  // device index -> address of the word that kernels report in
 int64_t error_addresses[64] = {};
 
@@ -66,6 +67,12 @@ int64_t whole(PyObject* o, const char* what, const char* name) {
     refuse(what, std::string(": ") + name + " is a whole number");
   }
   return v;
+}
+// So many positions, or (beyond 31 bits) more than a request holds.
+int positions(PyObject* o, const char* what, const char* name) {
+  const int64_t v = whole(o, what, name);
+  if (v < 0) refuse(what, std::string(": ") + name + " is no negative number");
+  return (int)(v < (1LL << 31) - MOST_DRAFTED ? v : (1LL << 31) - MOST_DRAFTED);
 }
 int64_t address(PyObject* o) { return (int64_t)PyLong_AsLongLong(o); }
 double real(PyObject* o, const char* what, const char* name) {
@@ -122,6 +129,8 @@ PyObject* guarded(F f) {
   } catch (const Refused& r) {
     PyErr_SetString(kernel_error, r.why.c_str());
   } catch (const Raised&) {
+  } catch (const c10::OutOfMemoryError& e) {
+    PyErr_SetString(memory_error, e.what_without_backtrace());
   } catch (const std::exception& e) {
     PyErr_SetString(PyExc_RuntimeError, e.what());
   }
@@ -358,8 +367,8 @@ PyObject* tree_attention(PyObject*, PyObject* const* args, Py_ssize_t given) {
     a.q = q.data_ptr(), a.k_pages = pages.data_ptr(), a.v_pages = (const char*)a.k_pages + nkv * dk * page_size * size, a.out = out.data_ptr();
     a.err = error_word(index), a.page_stride = nkv * (dk + dv) * page_size;
     a.tokens = (int)tokens, a.requests = (int)n, a.max_pages = (int)width, a.num_pages = (int)pages.size(0), a.nq = (int)nq, a.nkv = (int)nkv, a.d = (int)d;
-    a.dv = (int)dv, a.page_size = (int)page_size, a.words = (int)words, a.window = (int)whole(args[19], what, "window"), a.keep = (int)whole(args[20], what, "keep_first");
-    a.run = (int)whole(args[21], what, "chunk"), a.chunk = (int)whole(args[22], what, "plan"), a.parts = (int)parts;
+    a.dv = (int)dv, a.page_size = (int)page_size, a.words = (int)words, a.window = positions(args[19], what, "window"), a.keep = positions(args[20], what, "keep_first");
+    a.run = positions(args[21], what, "chunk"), a.chunk = (int)whole(args[22], what, "plan"), a.parts = (int)parts;
     a.scale = (float)real(args[26], what, "scale"), a.softcap = (float)real(args[27], what, "softcap");
     const int64_t entry = address(args[0]);
     const int dtype = type == at::kBFloat16;
@@ -482,14 +491,15 @@ PyObject* adjust_logits(PyObject*, PyObject* const* args, Py_ssize_t given) {
   });
 }
 
-// (KernelError, device index -> address of the error word)
+// (KernelError, torch.OutOfMemoryError, device index -> address of the error word)
 PyObject* set_up(PyObject*, PyObject* const* args, Py_ssize_t given) {
-  if (given != 2) {
-    PyErr_SetString(PyExc_TypeError, "set_up takes the error's class and a function");
+  if (given != 3) {
+    PyErr_SetString(PyExc_TypeError, "set_up takes two errors' classes and a function");
     return nullptr;
   }
   Py_XSETREF(kernel_error, Py_NewRef(args[0]));
-  Py_XSETREF(error_address, Py_NewRef(args[1]));
+  Py_XSETREF(memory_error, Py_NewRef(args[1]));
+  Py_XSETREF(error_address, Py_NewRef(args[2]));
   Py_RETURN_NONE;
 }
 

@@ -1277,7 +1277,7 @@ MOST_DRAFTED = 256
 def _host():
     """The host's side of these calls (csrc/host.cpp): checks, memory, the launch."""
     module = load_module("host")
-    module.set_up(KernelError, lambda index: error_word(torch.device("cuda", index)).data_ptr())
+    module.set_up(KernelError, torch.OutOfMemoryError, lambda index: error_word(torch.device("cuda", index)).data_ptr())
     return module
 
 
