@@ -394,12 +394,15 @@ class CacheManager:
 
     def resize(self, pages_per_group: "int | dict[KVSpec, int]") -> None:
         """Give every group's pool another number of pages, more or fewer, while requests live: what is held moves to the front of a
-        new tensor (old and new ones of all groups exist side by side meanwhile). CacheError where a pool would not take what it holds;
-        then, and where an allocation or a copy fails, nothing has changed. No step may be in flight, and
+        new tensor (old and new ones of all groups exist side by side meanwhile). CacheError where a pool would not take what it holds, or a
+        request holds drafted tokens that are not kept yet; then, and where an allocation or a copy fails, nothing has changed. No step may be in flight, and
         steps captured on the old tensors are dead afterwards (`StepRunner.forget_graphs`)."""
         counts = [pages_per_group[g.spec] if isinstance(pages_per_group, dict) else pages_per_group for g in self.groups]
         if any(count < 1 for count in counts):
             raise ValueError("a pool has at least one page")
+        for request in self.requests.values():
+            if request.drafted:
+                raise CacheError(f"request {request.request_id!r} holds drafted tokens that are not kept yet")
         pools = [group.pool.resized(count) for group, count in zip(self.groups, counts)]
         # Every group's new tensor is made and filled ahead of the first change: an allocation that fails leaves all as it was.
         tensors: list[torch.Tensor | None] = []

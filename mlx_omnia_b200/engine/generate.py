@@ -15,7 +15,7 @@ from __future__ import annotations
 import dataclasses
 import itertools
 import secrets
-from collections.abc import Iterator, Mapping, Sequence
+from collections.abc import Collection, Iterator, Mapping, Sequence
 from dataclasses import dataclass
 from pathlib import Path
 
@@ -243,48 +243,51 @@ class Generator:
 
         `drafts`: request id -> (tokens, parents): what may follow the request's latest token, as a tree: `parents[i]` is the earlier
         draft that token i goes on from, -1 the latest token itself; None: each goes on from the one ahead of it. Drafts are left aside where
-        pages or the request's last tokens are short, in a step that reads prompts, and for requests that do not decode. ValueError for a
+        pages are short, where generation ends with them or ahead of them, where the request's constraint does not let them come or lets nothing follow, in a step that
+        reads prompts, and for requests that do not decode. ValueError, and nothing has happened, for drafts that are no such trees and for a
         model whose layers keep other than keys and values."""
         runner = self.engine.runner
         why = runner.drafted.why_not()
         if why is not None:
             raise ValueError(why)
+        vocab, trees = self.engine.vocab_size, {}
+        for name, (tokens, parents) in drafts.items():
+            tokens = [int(t) for t in tokens]
+            parents = list(range(-1, len(tokens) - 1)) if parents is None else [int(p) for p in parents]
+            if len(parents) != len(tokens) or any(not -1 <= p < i for i, p in enumerate(parents)) or any(not 0 <= t < vocab for t in tokens) or \
+                    len(tokens) >= ops.MOST_DRAFTED:
+                raise ValueError(f"request {name!r}: up to {ops.MOST_DRAFTED - 1} drafts of the vocabulary, each with an earlier parent or -1")
+            trees[name] = tokens, parents
         outputs = self.drain()
         plan = self.scheduler.plan()
         if not plan.entries:
             return outputs
         if any(e.count != 1 or not e.samples or not e.request.generated for e in plan.entries):
             return outputs + self._finalize(self._launch(plan))
-        cache, vocab, entries = self.engine.cache, self.engine.vocab_size, []
+        cache, entries, allowed = self.engine.cache, [], []
         reserved = [0] * len(cache.groups)
         for planned in plan.entries:
             self.scheduler._reserve(planned.request, 1, reserved)
-        for planned in plan.entries:
-            request = planned.request
-            tokens, parents = drafts.get(request.request_id, ((), None))
-            tokens = [int(t) for t in tokens]
-            parents = list(range(-1, len(tokens) - 1)) if parents is None else [int(p) for p in parents]
-            if len(parents) != len(tokens) or any(not -1 <= p < i for i, p in enumerate(parents)) or any(not 0 <= t < vocab for t in tokens) or \
-                    len(tokens) >= ops.MOST_DRAFTED:
-                raise ValueError(f"request {request.request_id!r}: up to {ops.MOST_DRAFTED - 1} drafts of the vocabulary, each with an earlier parent or -1")
-            count = 1 + len(tokens)
-            mine = [cache.pages_for(g, request.cache.tokens + count) - cache.pages_for(g, request.cache.tokens + 1) for g in range(len(cache.groups))]
-            if len(request.generated) + 1 >= request.max_tokens or any(r + m > g.pool.free for r, m, g in zip(reserved, mine, cache.groups)):
-                tokens, parents, count, mine = [], [], 1, [0] * len(mine)
-            reserved = [r + m for r, m in zip(reserved, mine)]
-            entries.append(StepEntry(request.cache, [request.token_slice(planned.start, 1)[0], *tokens], list(range(count)), [-1, *(p + 1 for p in parents)]))
         requests = [planned.request for planned in plan.entries]
         try:
+            for planned in plan.entries:
+                request = planned.request
+                tokens, parents, lets = self._drafts_of(request, *trees.get(request.request_id, ((), ())))
+                held = request.cache.tokens
+                mine = [cache.pages_for(g, held + len(tokens)) - cache.pages_for(g, held + 1) for g in range(len(cache.groups))]
+                if any(r + m > g.pool.free for r, m, g in zip(reserved, mine, cache.groups)):
+                    tokens, parents, lets, mine = tokens[:1], parents[:1], lets[:1], [0] * len(mine)
+                reserved = [r + m for r, m in zip(reserved, mine)]
+                entries.append(StepEntry(request.cache, tokens, list(range(len(tokens))), parents))
+                allowed += lets
             logits = runner.run(entries)
-            rows, owners, depths, allowed = [], [], [], []
-            for r, (request, entry) in enumerate(zip(requests, entries)):
-                ways: list[list[int]] = []
-                for j, p in enumerate(entry.parents):
-                    ways.append([*ways[p], j] if p >= 0 else [j])
-                    rows.append(len(rows))
+            owners, depths = [], []
+            for r, entry in enumerate(entries):
+                first = len(depths)
+                for p in entry.parents:
                     owners.append(r)
-                    depths.append(len(ways[j]) - 1)
-                    allowed.append(allowed_ids(request.sampling, request.generated + [entry.tokens[i] for i in ways[j][1:]]))
+                    depths.append(depths[first + p] + 1 if p >= 0 else 0)
+            rows = list(range(len(depths)))
             params = [request.sampling for request in requests]
             # (A request's text ends ahead of the step's tokens, the first of which is its latest one.)
             texts = [text_of(p, request.prompt, request.generated[:-1]) for p, request in zip(params, requests)]
@@ -307,6 +310,31 @@ class Generator:
                     self._seeds.pop(request.request_id, None)
                     break
         return outputs
+
+    def _drafts_of(self, request: Request, drafts: Sequence[int], above: Sequence[int]) -> "tuple[list[int], list[int], list[Collection[int] | None]]":
+        """What a request brings to a step with these drafts: its latest token and the drafts that may come behind it, for each the one that it goes on
+        from and what may follow it. What is left out: the request's last token and its stop tokens, which nothing is chosen behind; drafts that its
+        constraint does not let come there (it is asked only about texts that it let come) or lets nothing follow; and what goes on from such."""
+        tokens, parents, allowed = [request.generated[-1]], [-1], [allowed_ids(request.sampling, request.generated)]
+        ways: list[list[int]] = [[]]
+        places = {-1: 0}  # of the drafts, those that stay: their place
+        for i, (token, p) in enumerate(zip(drafts, above)):
+            at = places.get(p)
+            if at is None or len(request.generated) + len(ways[at]) + 1 >= request.max_tokens or token in request.stop:
+                continue
+            if allowed[at] is not None and token not in allowed[at]:
+                continue
+            way, lets = [*ways[at], token], None
+            if request.sampling.constraint is not None:
+                lets = request.sampling.constraint([*request.generated, *way])
+                if lets is not None and not len(lets):
+                    continue
+            places[i] = len(tokens)
+            tokens.append(token)
+            parents.append(at)
+            allowed.append(lets)
+            ways.append(way)
+        return tokens, parents, allowed
 
     def resize_cache(self, tokens: int) -> None:
         """Give the page pools of a running engine room for `tokens` positions, more or fewer: what live requests hold is kept

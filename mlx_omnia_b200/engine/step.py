@@ -221,7 +221,7 @@ class DraftedSteps:
         if self.last is None or len(self.last[0]) != len(entries) or any(a is not b for a, b in zip(self.last[0], entries)):
             raise ValueError("keep() takes the entries of the step of drafted trees that was run last, once")
         cache, (_, step, starts) = self.runner.cache, self.last
-        if any(e.parents is not None and (e.request.request_id not in cache.requests or e.request.drafted != len(e.tokens)) for e in entries):
+        if any(e.parents is not None and (cache.requests.get(e.request.request_id) is not e.request or e.request.drafted != len(e.tokens)) for e in entries):
             raise ValueError("a request of the step has ended")
         if chosen.shape != step.logit_rows.shape:
             raise ValueError("a token is chosen from every row of the step's logits")

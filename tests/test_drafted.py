@@ -253,6 +253,77 @@ def test_drafts_that_are_refused(device):
     generator.abort(request.request_id)
 
 
+def test_a_rule_is_asked_only_about_what_it_let_come(device):
+    """A rule that knows no other texts than its own, and nothing that may follow some of them."""
+    engine, _, _ = engine_for("A", device)
+    prompt, asked = tiny_configs.prompt(9, engine.vocab_size, 4), []
+
+    def rule(made):
+        asked.append(list(made))
+        for i, token in enumerate(made):
+            if token % 3 != i % 3:
+                raise KeyError(token)
+        return [] if made and made[-1] < 30 else {t for t in range(engine.vocab_size) if t % 3 == len(made) % 3}
+
+    high = {t: -math.inf for t in range(30)}  # (nothing that ends is ever chosen)
+    for stop_at in (None, 4):
+        options = GenerationOptions(max_tokens=10, stop=(), bias=high, constraint=rule)
+        expect = Generator(engine).generate([prompt], options)[0]
+        if stop_at is not None:
+            options = GenerationOptions(max_tokens=10, stop=(expect[stop_at],), bias=high, constraint=rule)
+            expect = Generator(engine).generate([prompt], options)[0]
+        asked.clear()
+        generator, steps = Generator(engine), 0
+        request = generator.add(prompt, options)
+        while not generator.scheduler.idle:
+            at = len(request.generated)
+            ahead = expect[at: at + 3] + list(options.stop)
+            mine, parents, last = [], [], -1
+            for token in ahead:  # one that the rule does not let come and what goes on from it, one that nothing follows, the right one
+                depth = at + len(parents) // 4
+                mine += [token + 1, token, depth % 3, token]
+                parents += [last, len(mine) - 4, last, last]
+                last = len(mine) - 1
+            generator.step_drafted({request.request_id: (mine, parents)})
+            steps += 1
+        assert request.generated == expect and steps < len(expect) and request.finish_reason == ("length" if stop_at is None else "stop")
+        assert not any(t in options.stop for made in asked for t in made) and max(map(len, asked)) < 10
+    engine.cache.check()
+
+
+def test_refused_drafts_lose_nothing(device):
+    """A step in flight is still to come, and the tokens are what they would have been."""
+    engine, _, _ = engine_for("A", device)
+    prompt = tiny_configs.prompt(9, engine.vocab_size, 4)
+    expect = Generator(engine).generate([prompt], GenerationOptions(max_tokens=9, stop=()))[0]
+    generator, got = Generator(engine), []
+    request = generator.add(prompt, GenerationOptions(max_tokens=9, stop=()))
+    for _ in range(3):
+        got += generator.step()
+    with pytest.raises(ValueError, match="drafts"):
+        generator.step_drafted({request.request_id: ([1, 2], [0, 0])})
+    while not generator.scheduler.idle:
+        got += generator.step_drafted({request.request_id: ([1, 2], None)})
+    assert [o.token for o in got if o.token is not None] == request.generated == expect
+    engine.cache.check()
+
+
+def test_what_waits_for_drafts_to_be_kept(device):
+    engine, _, _ = engine_for("A", device)
+    request = engine.cache.open("r")
+    entries = [StepEntry(request, [1, 2], [0, 1], [-1, 0])]
+    engine.runner.run(entries)
+    with pytest.raises(ValueError, match="kept"):
+        engine.runner.run([StepEntry(request, [1])])
+    with pytest.raises(CacheError, match="kept"):
+        engine.cache.resize(64)
+    engine.cache.close("r")
+    engine.cache.open("r")  # another request of that name
+    with pytest.raises(ValueError, match="ended"):
+        engine.runner.keep(entries, chosen_on(device, [1, 1]))
+    engine.cache.check()
+
+
 def test_a_rule_that_fails_ends_its_step(device):
     engine, _, _ = engine_for("A", device)
     prompt = tiny_configs.prompt(5, engine.vocab_size, 4)
