@@ -42,6 +42,10 @@ bound of what requests hold beyond the groups) is captured when that amounts to 
 is taken off. Until then the step runs as one without groups, which needs nothing of them and whose
 results round otherwise (`ops.paged_attention`).
 
+Steps of drafted trees (`DraftedGraphs`). Their tables are made on the device from the requests' lengths and lists of pages, by the first kernel of
+the step, so one graph serves every step of as many requests, rows, drafts and pages, each rounded up; rows and requests beyond the step's belong to
+requests that hold nothing. Such a step too is captured at its third coming, in the way of mixed steps.
+
 The kernels and the model code are the same as in an uncaptured step; only the way
 they are launched differs, so logits agree bit for bit with an eager step of the same
 bucket, of groups or without. Capture is used only when every mixer of the model declares `graph_safe`
@@ -57,14 +61,14 @@ from __future__ import annotations
 
 import contextlib
 import gc
-from dataclasses import dataclass
+from dataclasses import dataclass, replace
 
 import numpy as np
 import torch
 
-from mlx_omnia_b200.engine.step import StepLayout, shared_positions
+from mlx_omnia_b200.engine.step import DraftedLayout, StepLayout, shared_positions
 from mlx_omnia_b200.kernels import ops
-from mlx_omnia_b200.parts.base import StepContext
+from mlx_omnia_b200.parts.base import StepContext, StepTree
 
 MAX_GRAPHS = 24
 CAPTURE_GAINS = 1152
@@ -102,7 +106,7 @@ def _bucket(n: int) -> int:
 class _Captured:
     graph: torch.cuda.CUDAGraph
     step: StepContext
-    layout: StepLayout
+    layout: StepLayout | DraftedLayout
     host_tensor: torch.Tensor  # pinned int32 mirror of `device`
     device: torch.Tensor
     logits: torch.Tensor
@@ -337,3 +341,88 @@ class MixedGraphs:
         self.replays += 1
         ops.launches += captured.launches
         return captured.logits.clone() if copy else captured.logits
+
+
+DRAFTED_MAX_TOKENS = 256
+"""Steps of more drafted tokens stay uncaptured: their kernels outlast the launching (28 layers: 4.2 ms; 64 requests of 2,000 positions with four tokens
+each take the GPU 7.8), and a graph keeps a row of logits for each."""
+
+
+class DraftedGraphs:
+    """Captured steps of drafted trees, keyed by their rounded shape (see the head of the file)."""
+
+    def __init__(self, runner) -> None:
+        self.runner = runner
+        self.seen: dict[tuple, int] = {}
+        self.captured: dict[tuple, _Captured] = {}  # in order of last use, oldest first
+        self.replays = 0
+
+    def wants(self, entries) -> tuple | None:
+        """(requests, rows, drafts of a request, width of the tables), where this step should run from a graph. (Their pages are taken.)"""
+        brought = [len(e.tokens) for e in entries]
+        if sum(brought) > DRAFTED_MAX_TOKENS or any(e.parents is None for e in entries):
+            return None
+        total = max(sum(brought), 8)
+        step = 1 << (total.bit_length() - 2)  # rows by two significant bits: products of 16 rows and of 13 stream the same weights
+        key = (_bucket(len(entries)), -(-total // step) * step, _bucket(max(brought)),
+               ops.width_bucket(max(len(t) for e in entries for t in e.request.tables)))
+        if key in self.captured:
+            return key
+        self.seen[key] = self.seen.get(key, 0) + 1
+        if len(self.seen) > 4096:
+            self.seen.clear()
+            return None
+        return key if self.seen[key] >= MIXED_CAPTURE_AT else None
+
+    def run(self, key: tuple, entries, starts: list[int], copy: bool = True) -> "tuple[torch.Tensor, StepContext]":
+        """-> logits of all the entries' tokens, and the step as these see it (its tables are the graph's own: the next step overwrites them)"""
+        runner, cache = self.runner, self.runner.cache
+        requests, tokens, most, width = key
+        captured = self.captured.pop(key, None)
+        fresh = captured is None
+        if fresh:
+            while len(self.captured) >= MIXED_MAX_GRAPHS:
+                torch.cuda.synchronize(runner.runtime.device)
+                del self.captured[next(iter(self.captured))]
+            # Requests that hold nothing for the rows that no entry brings: fewer than `tokens` of them.
+            layout = DraftedLayout(tokens, requests + -(-tokens // most), tokens, [width] * len(cache.groups), most)
+            host_tensor = torch.zeros(layout.words, dtype=torch.int32).pin_memory()
+            dev = torch.zeros(layout.words, dtype=torch.int32, device=runner.runtime.device)
+        else:
+            layout, host_tensor, dev = captured.layout, captured.host_tensor, captured.device
+            if captured.copied is not None:
+                captured.copied.synchronize()  # the pinned buffer is free to be written again
+        layout.fill(host_tensor.numpy(), cache, entries, starts, np.arange(tokens, dtype=np.int32))
+        dev.copy_(host_tensor, non_blocking=True)
+
+        def forward(workspace: dict) -> "tuple[torch.Tensor, StepContext]":
+            step = layout.context(dev, cache.page_size, width * cache.page_size, q_lens=[], seq_lens_host=[], workspace=workspace)
+            return runner.model.forward(step, runner.layer_contexts(step)), step
+
+        if fresh:
+            # This step runs kernel by kernel on the graph's buffers; then the same launches are captured.
+            workspace: dict = {"private": True}
+            logits, step = forward(workspace)
+            torch.cuda.synchronize(runner.runtime.device)
+            graph = torch.cuda.CUDAGraph()
+            before = ops.launches
+            with capturing(graph):
+                kept_logits, kept_step = forward(workspace)
+            launches = ops.launches - before
+            ops.launches = before  # the capture launched nothing
+            self.captured[key] = _Captured(graph, kept_step, layout, host_tensor, dev, kept_logits, launches)
+        else:
+            self.captured[key] = captured  # most recently used last
+            if captured.copied is None:
+                captured.copied = torch.cuda.Event()
+            captured.copied.record()
+            captured.graph.replay()
+            self.replays += 1
+            ops.launches += captured.launches
+            logits, step = captured.logits, captured.step
+        n, total = len(entries), sum(len(e.tokens) for e in entries)
+        mine = replace(step, num_tokens=total, num_seqs=n, token_ids=step.token_ids[:total], positions=step.positions[:total],
+                       cu_seqlens=step.cu_seqlens[: n + 1], seq_lens=step.seq_lens[:n], logit_rows=step.logit_rows[:total],
+                       groups={g: (table[:n], slots[:total]) for g, (table, slots) in step.groups.items()}, tree=StepTree(step.tree.ancestors[:total]))
+        logits = logits[:total]
+        return logits.clone() if copy and not fresh else logits, mine

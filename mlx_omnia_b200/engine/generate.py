@@ -280,7 +280,7 @@ class Generator:
                 reserved = [r + m for r, m in zip(reserved, mine)]
                 entries.append(StepEntry(request.cache, tokens, list(range(len(tokens))), parents))
                 allowed += lets
-            logits = runner.run(entries)
+            logits = runner.run(entries, copy=False)
             owners, depths = [], []
             for r, entry in enumerate(entries):
                 first = len(depths)

@@ -135,6 +135,56 @@ class Kept:
     next: int
 
 
+class DraftedLayout:
+    """Where what the host knows of a step of drafted trees lies in one buffer of int32 words: `tokens` rows of the batch, `seqs` requests, `wanted`
+    rows of logits, lists of `widths` pages. The tables are made from it on the device (`ops.step_tables`), in an eager step and in a captured one."""
+
+    def __init__(self, tokens: int, seqs: int, wanted: int, widths: list[int], most: int) -> None:
+        self.tokens, self.seqs, self.widths, self.most = tokens, seqs, list(widths), most
+        self.parts: dict[str, slice] = {}
+        at = 0
+        for name, size in ([(f"starts{g}", 2 * seqs) for g in range(len(widths))] +  # (8 bytes each)
+                           [("held", seqs), ("brought", seqs), ("slots", seqs), ("fresh", seqs), ("parents", tokens), ("ids", tokens), ("rows", wanted)] +
+                           [(f"pages{g}", seqs * w) for g, w in enumerate(widths)]):
+            self.parts[name] = slice(at, at + size)
+            at += size
+        self.words = at
+
+    def fill(self, host: np.ndarray, cache: CacheManager, entries: list[StepEntry], starts: list[int], rows) -> None:
+        """Requests beyond `entries` are there for the step's shape: rows that no entry brings are theirs, and see nothing."""
+        part = {name: host[where] for name, where in self.parts.items()}
+        n, brought = len(entries), [len(e.tokens) for e in entries]
+        total = sum(brought)
+        spare = [max(0, min(self.most, self.tokens - total - i * self.most)) for i in range(self.seqs - n)]
+        if max(brought) > self.most or total + sum(spare) != self.tokens:
+            raise ValueError("a step of drafted trees has more rows than its requests bring")
+        part["held"][:n], part["held"][n:] = starts, -1
+        part["brought"][:n], part["brought"][n:] = brought, spare
+        part["slots"][:n], part["slots"][n:] = [e.request.slot for e in entries], cache.scratch_slot
+        part["fresh"][:n], part["fresh"][n:] = [int(e.request.fresh) for e in entries], 0
+        part["parents"][:total] = [p for e in entries for p in (e.parents if e.parents is not None else range(-1, len(e.tokens) - 1))]
+        part["ids"][:total] = [t for e in entries for t in e.tokens]
+        part["parents"][total:], part["ids"][total:] = -1, 0
+        part["rows"][:] = rows
+        for g, width in enumerate(self.widths):
+            part[f"starts{g}"].view(np.int64)[:] = np.arange(self.seqs, dtype=np.int64) * width
+            table = part[f"pages{g}"].reshape(self.seqs, width)
+            table.fill(-1)
+            for i, e in enumerate(entries):
+                mine = e.request.table_array(g)
+                table[i, : len(mine)] = mine
+
+    def context(self, device: torch.Tensor, page_size: int, max_seq_len: int, **more) -> StepContext:
+        """The step, its tables made by a kernel from what the `device` buffer holds then."""
+        part = {name: device[where] for name, where in self.parts.items()}
+        lists = [ops.PageLists(part[f"pages{g}"], part[f"starts{g}"].view(torch.int64), width) for g, width in enumerate(self.widths)]
+        made = ops.step_tables(part["held"], part["brought"], lists, page_size, self.tokens, parents=part["parents"], most=self.most)
+        return StepContext(
+            num_tokens=self.tokens, num_seqs=self.seqs, token_ids=part["ids"], positions=made.positions, cu_seqlens=made.cu_seqlens,
+            seq_lens=made.seq_lens, state_slots=part["slots"], fresh=part["fresh"], logit_rows=part["rows"], max_q_len=self.most,
+            max_seq_len=max_seq_len, decode_only=False, groups=dict(enumerate(made.groups)), tree=made.tree, **more)
+
+
 class DraftedSteps:
     """Steps whose requests bring trees of drafted tokens. `run` reads all of them in one step; `keep` says which the model agrees with, moves
     their keys and values to where a request that had brought only these would have them, and takes the others' room back."""
@@ -153,7 +203,7 @@ class DraftedSteps:
             return "drafted trees take caches with a row for every position"
         return None
 
-    def run(self, entries: list[StepEntry]) -> torch.Tensor:
+    def run(self, entries: list[StepEntry], copy: bool = True) -> torch.Tensor:
         runner, cache, device = self.runner, self.runner.cache, self.runner.runtime.device
         why = self.why_not()
         if why is not None:
@@ -172,38 +222,22 @@ class DraftedSteps:
             raise ValueError("a request comes once to a step")
         cache.reset_slots([e.request.slot for e in entries if e.request.fresh])
         starts = runner.take_pages(entries)
-        brought = [len(e.tokens) for e in entries]
-        held, tokens = [s + b for s, b in zip(starts, brought)], sum(brought)
-        cu = np.cumsum([0, *brought])
-        rows = [int(c) + w for c, e in zip(cu, entries) for w in e.want]
-        lists = [[e.request.table_array(g) for e in entries] for g in range(len(cache.groups))]
-        n, groups = len(entries), len(cache.groups)
-        parts = {f"starts{g}": 2 * n for g in range(groups)} | {"held": n, "brought": n, "slots": n, "fresh": n, "parents": tokens, "ids": tokens,
-                                                               "rows": len(rows)} | {f"pages{g}": sum(map(len, x)) for g, x in enumerate(lists)}
-        where, at = {}, 0
-        for name, size in parts.items():
-            where[name] = slice(at, at + size)
-            at += size
-        host_tensor = torch.empty(at, dtype=torch.int32, pin_memory=device.type == "cuda")
-        host = host_tensor.numpy()
-        host[where["held"]], host[where["brought"]] = starts, brought
-        host[where["slots"]], host[where["fresh"]] = [e.request.slot for e in entries], [int(e.request.fresh) for e in entries]
-        host[where["parents"]] = [p for e in entries for p in (e.parents if e.parents is not None else range(-1, len(e.tokens) - 1))]
-        host[where["ids"]], host[where["rows"]] = [t for e in entries for t in e.tokens], rows
-        for g, x in enumerate(lists):
-            host[where[f"starts{g}"]].view(np.int64)[:] = np.cumsum([0, *map(len, x)])[:-1]
-            host[where[f"pages{g}"]] = np.concatenate(x)
-        packed = host_tensor.to(device, non_blocking=True) if device.type == "cuda" else host_tensor
-        part = {name: packed[w] for name, w in where.items()}
-        made = ops.step_tables(part["held"], part["brought"], [ops.PageLists(part[f"pages{g}"], part[f"starts{g}"].view(torch.int64), max(map(len, x)))
-                                                               for g, x in enumerate(lists)],
-                               cache.page_size, tokens, parents=part["parents"], most=max(brought))
-        step = StepContext(
-            num_tokens=tokens, num_seqs=n, token_ids=part["ids"], positions=made.positions, cu_seqlens=made.cu_seqlens, seq_lens=made.seq_lens,
-            state_slots=part["slots"], fresh=part["fresh"], logit_rows=part["rows"], q_lens=brought, seq_lens_host=held, max_q_len=max(brought),
-            max_seq_len=max(held), decode_only=False, groups=dict(enumerate(made.groups)), workspace=runner.ask_for_layers(), tree=made.tree)
-        logits = runner.model.forward(step, runner.layer_contexts(step))
-        runner.know_layers(step)
+        graphs = runner.drafted_graphs
+        key = graphs.wants(entries) if graphs is not None else None
+        if key is not None:
+            logits, step = graphs.run(key, entries, starts, copy)
+        else:
+            brought = [len(e.tokens) for e in entries]
+            cu, held = np.cumsum([0, *brought]), [s + b for s, b in zip(starts, brought)]
+            rows = [int(c) + w for c, e in zip(cu, entries) for w in e.want]
+            widths = [max(len(e.request.tables[g]) for e in entries) for g in range(len(cache.groups))]
+            layout = DraftedLayout(sum(brought), len(entries), len(rows), widths, max(brought))
+            host_tensor = torch.empty(layout.words, dtype=torch.int32, pin_memory=device.type == "cuda")
+            layout.fill(host_tensor.numpy(), cache, entries, starts, rows)
+            packed = host_tensor.to(device, non_blocking=True) if device.type == "cuda" else host_tensor
+            step = layout.context(packed, cache.page_size, max(held), q_lens=brought, seq_lens_host=held, workspace=runner.ask_for_layers())
+            logits = runner.model.forward(step, runner.layer_contexts(step))
+            runner.know_layers(step)
         for e in entries:
             e.request.fresh = False
             if e.parents is not None:
@@ -256,14 +290,14 @@ class StepRunner:
         self.drafted = DraftedSteps(self)
         self.attention_layers: Counter = Counter()  # kinds (`ops.AttentionLayer`) that a step was seen to run, and how often
         self.cuda_graphs = cuda_graphs
-        self.graphs = self.mixed_graphs = None
+        self.graphs = self.mixed_graphs = self.drafted_graphs = None
         self.forget_graphs()
 
     def forget_graphs(self) -> None:
         """Drop every captured step (they hold the addresses of the cache's tensors) and begin anew."""
         if not self.cuda_graphs or self.runtime.device.type != "cuda":
             return
-        from mlx_omnia_b200.engine.decode_graph import DecodeGraphs, MixedGraphs
+        from mlx_omnia_b200.engine.decode_graph import DecodeGraphs, DraftedGraphs, MixedGraphs
 
         if self.graphs is not None:
             torch.cuda.synchronize(self.runtime.device)  # nothing of them is still running
@@ -271,6 +305,8 @@ class StepRunner:
             self.graphs = DecodeGraphs(self)
             if MixedGraphs.supported(self.model):
                 self.mixed_graphs = MixedGraphs(self)
+                if self.drafted.why_not() is None:
+                    self.drafted_graphs = DraftedGraphs(self)
 
     def ask_for_layers(self) -> dict:
         """A step's workspace, in which attention notes its layers until these are known. (Every step runs all of them, and requests share positions
@@ -359,7 +395,7 @@ class StepRunner:
         if any(e.parents is not None for e in entries):
             if device_tokens is not None:
                 raise ValueError("drafted tokens come from the host")
-            return self.drafted.run(entries)
+            return self.drafted.run(entries, copy)
         self.cache.reset_slots([e.request.slot for e in entries if e.request.fresh])
         if self.graphs is not None and entries and all(len(e.tokens) == 1 and e.want in ([], [0]) for e in entries):
             logits = self.graphs.run(entries, copy, device_tokens)
