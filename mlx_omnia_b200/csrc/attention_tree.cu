@@ -261,14 +261,10 @@ __global__ void __launch_bounds__(THREADS, Shares32<MOST>::PLACES) tree_shares32
   pdl_launch_dependents();
   const TreeShares shares = {ROWS, KEYS, 1, S::EXTRA};
   const long long total = shares.lay_out(a, ends, sums), blocks = min((long long)gridDim.x, total);
+  if (blockIdx.x >= blocks) return;
+  const long long t0 = total * blockIdx.x / blocks, upto = total * (blockIdx.x + 1) / blocks;
   TreePlace ahead;
-  if (blockIdx.x >= blocks) {
-    if (threadIdx.x == 0) tree_border(a, shares, total, blocks, 0, 0, ahead);
-    return;
-  }
-  const long long t0 = total * blockIdx.x / blocks;
-  const long long begin = ahead.find(a, shares, ends, t0, (int)(total * (blockIdx.x + 1) / blocks - t0));
-  if (threadIdx.x == 0) tree_border(a, shares, total, blocks, t0, begin, ahead);
+  ahead.find(a, shares, ends, t0, (int)(upto - t0));
   if (ahead.left == 0) return;
   TreePlace now = ahead;
   __syncthreads();
@@ -324,6 +320,7 @@ __global__ void __launch_bounds__(THREADS, Shares32<MOST>::PLACES) tree_shares32
   while (now.left > 0) {
     const int rows = now.k.count * group, row0 = now.row_tile * ROWS, here = min(ROWS, rows - row0);
     if (entered) {
+      if (tid == 0 && now.tile == 0) tree_note(a, total, blocks, upto, now, first);
       for (int i = tid; i < ROWS * (MOST / 4); i += THREADS) {
         const int r = i / (MOST / 4), c = i % (MOST / 4) * 4, row = row0 + r;
         if (c >= d) continue;
@@ -584,8 +581,9 @@ int launch_tree(const TreeAttention& a, int most_nodes, cudaStream_t stream) {
 }
 
 template <int MOST>
-int launch_shares32(const TreeAttention& a, int most_nodes, int blocks, cudaStream_t stream) {
+int launch_shares32(TreeAttention a, int most_nodes, int blocks, cudaStream_t stream) {
   using S = Shares32<MOST>;
+  a.parts = tree_row_tiles(a, most_nodes, ROWS);
   constexpr int bytes = S::FLOATS * (int)sizeof(float);
   static bool ready[64] = {};
   int device = 0;
@@ -599,7 +597,7 @@ int launch_shares32(const TreeAttention& a, int most_nodes, int blocks, cudaStre
   launch_pdl(tree_shares32_kernel<MOST>, dim3(blocks), dim3(THREADS), bytes, stream, a);
   const int code = OMNIA_LAUNCH_RESULT();
   if (code) return code;
-  return tree_join<float, 256>(a, {ROWS, S::KEYS, 1, S::EXTRA}, most_nodes, blocks, stream);
+  return tree_join<float, MOST <= 128 ? 128 : 256>(a, {ROWS, S::KEYS, 1, S::EXTRA}, most_nodes, blocks, stream);
 }
 
 }  // namespace

@@ -14,8 +14,9 @@ struct TreeAttention {
   const float* sink;                         // [nq] or null
   float *part_o, *part_ml;                   // [parts, tokens, nq, dv] unnormalised, [parts, tokens, nq, 2] (offset in log2 units, sum)
   int* err;
-  int4* borders;                             // of the kernels by equal shares: two a block, what the join does at the block's beginning
+  int4* items;                               // [requests, nkv, parts], of the kernels by equal shares: where the join finds an item (tree_note)
   long long page_stride;
+  // chunk, parts: of the kernel for any shape; by equal shares `parts` is the most tiles of rows that a request has.
   int tokens, requests, max_pages, num_pages, nq, nkv, d, dv, page_size, gate_stride, words, window, keep, run, chunk, parts;
   float scale, softcap;
 };
@@ -150,24 +151,17 @@ struct TreePlace {
   }
 };
 
-// What the join does at the border ahead of block `block`, which begins at place `at` in an item whose places begin at `begin`: nothing, unless the border
-// lies between tiles of that item and is the first that does. (One thread of every block of the kernel, those that have no share too.)
-__device__ __forceinline__ void tree_border(const TreeAttention& a, const TreeShares& s, long long total, long long blocks, long long at, long long begin,
-                                            const TreePlace& place) {
+// Where the join finds an item, by the block that has its first tile and whose share of the line ends at place `upto` (one thread of it): in how many
+// pieces it is, in which slot the first one is, in which the next (one a block from there on).
+__device__ __forceinline__ void tree_note(const TreeAttention& a, long long total, long long blocks, long long upto, const TreePlace& now, bool first) {
+  if (now.row_tile >= a.parts) return;  // (more nodes than the call allows for, which the join reports)
   const int block = blockIdx.x;
-  int4 item = make_int4(-1, 0, 0, 0), slots = make_int4(0, 0, 0, 0);
-  if (block > 0 && block < blocks) {
-    const long long first = begin + s.extra, end = first + place.tiles, before = total * (block - 1) / blocks;  // `first`: its first tile's place
-    if (first < at && first >= before) {
-      int last = block;
-      while (total * (last + 1) / blocks < end) ++last;
-      const int row0 = place.row_tile * s.rows, rows = min(s.rows, place.k.count * (a.nq / a.nkv) - row0);
-      item = make_int4(place.k.first, place.head, row0, rows);
-      // The block that the item begins in may have begun in another item, the others have begun in this one.
-      slots = make_int4(2 * (block - 1) + (begin <= before ? 0 : 1), 2 * block, last - block + 1, 0);
-    }
+  int4 item = make_int4(1, 0, 0, 0);
+  if (now.tiles > now.left) {
+    const long long last = ((upto - now.left + now.tiles) * blocks - 1) / total;  // the block that has the item's last tile
+    item = make_int4((int)last - block + 1, 2 * block + (first ? 0 : 1), 2 * block + 2, 0);
   }
-  a.borders[2 * block] = item, a.borders[2 * block + 1] = slots;
+  a.items[((size_t)now.request * a.nkv + now.head) * a.parts + now.row_tile] = item;
 }
 
 constexpr int TREE_JOIN_WARPS = 4;
@@ -188,33 +182,24 @@ __device__ __forceinline__ unsigned tree_pair(float lo, float hi) {
   return *reinterpret_cast<const unsigned*>(&v);
 }
 
-// An item that several blocks had part in, put together by the blocks of the grid that stand for the first border in it: a warp a row, the slots in the
-// order of their blocks, eight on their way at once, the sink, the gate. The last `requests` blocks write zeros for requests that see nothing. The rows of
-// an item are shared out over the grid's other axis.
+// An item that several blocks had part in, put together: a warp a row, the slots in the order of their blocks, eight on their way at once, the sink, the
+// gate. A block of the grid's first axis has an item (a request's first one: its zeros, where it sees nothing), whose rows the second axis shares out. What
+// is read ahead of the wait was there ahead of the kernel that this one waits for. `slots`: how many there are.
 template <typename T, int MOST>
-__global__ void __launch_bounds__(32 * TREE_JOIN_WARPS) tree_join_kernel(const __grid_constant__ TreeAttention a, const TreeShares shares, int grid, int most) {
+__global__ void __launch_bounds__(32 * TREE_JOIN_WARPS) tree_join_kernel(const __grid_constant__ TreeAttention a, const TreeShares shares, int slots, int most) {
   constexpr int WARPS = TREE_JOIN_WARPS, PER = (MOST + 127) / 128;  // four dims a lane
   constexpr float LOG2E = 1.4426950408889634f;
   const int D = a.d;  // a multiple of 4, MOST at most
-  const int rows_of_tile = shares.rows, group = a.nq / a.nkv, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, step = WARPS * gridDim.y;
-  if ((int)blockIdx.x >= grid - 1) {
-    const TreeKeys k = tree_keys(a, blockIdx.x - (grid - 1), shares.align);
-    if (k.count > most && blockIdx.y == 0 && threadIdx.x == 0) atomicOr(a.err, OMNIA_ERR_WORK);
-    if (k.total > 0) return;
-    pdl_wait();
-    for (int r = blockIdx.y * WARPS + warp; r < k.count * a.nq; r += step)
-      for (int c = lane; c < D; c += 32) static_cast<T*>(a.out)[((size_t)k.first * a.nq + r) * D + c] = from_f32<T>(0.f);
-    return;
-  }
-  pdl_wait();
-  pdl_launch_dependents();
-  const int4 item = a.borders[2 * (blockIdx.x + 1)], slots = a.borders[2 * (blockIdx.x + 1) + 1];
-  if (item.x < 0) return;
-  const int parts = slots.z + 1;
-  for (int r = blockIdx.y * WARPS + warp; r < item.w; r += step) {
-    const int in = item.z + r, token = item.x + in / group, head = item.y * group + in % group;
-    const float sink = a.sink ? a.sink[head] * LOG2E : -INFINITY;
-    float gates[PER][4];
+  const int group = a.nq / a.nkv, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, step = WARPS * gridDim.y, r0 = blockIdx.y * WARPS + warp;
+  const int request = blockIdx.x / (a.nkv * a.parts), within = blockIdx.x % (a.nkv * a.parts), kvh = within / a.parts, row0 = within % a.parts * shares.rows;
+  const TreeKeys k = tree_keys(a, request, shares.align);
+  if (k.count > most && within == 0 && blockIdx.y == 0 && threadIdx.x == 0) atomicOr(a.err, OMNIA_ERR_WORK);
+  const int rows = k.total > 0 ? min(shares.rows, k.count * group - row0) : 0;
+  float gates[PER][4], sink = 0.f;
+  auto ahead = [&](int r) {  // what a row needs beside its pieces
+    if (r >= rows) return;
+    const int in = row0 + r, token = k.first + in / group, head = kvh * group + in % group;
+    sink = a.sink ? a.sink[head] * LOG2E : -INFINITY;
 #pragma unroll
     for (int i = 0; i < PER; ++i)
 #pragma unroll
@@ -222,6 +207,24 @@ __global__ void __launch_bounds__(32 * TREE_JOIN_WARPS) tree_join_kernel(const _
         const int c = (32 * i + lane) * 4 + j;
         gates[i][j] = a.gate && c < D ? to_f32(static_cast<const T*>(a.gate)[(size_t)token * a.gate_stride + head * D + c]) : 0.f;
       }
+  };
+  ahead(r0);
+  pdl_wait();
+  pdl_launch_dependents();
+  if (k.total <= 0) {
+    if (within > 0) return;
+    for (int r = r0; r < k.count * a.nq; r += step)
+      for (int c = lane; c < D; c += 32) static_cast<T*>(a.out)[((size_t)k.first * a.nq + r) * D + c] = from_f32<T>(0.f);
+    return;
+  }
+  if (rows <= 0) return;
+  const int4 item = a.items[blockIdx.x];
+  const int parts = item.x;
+  // One piece is its block's to write. (What lies outside the slots a kernel that gave up has left unwritten.)
+  if (parts < 2 || parts > slots || item.y < 0 || item.y >= slots || item.z < 0 || item.z + 2 * (parts - 2) >= slots) return;
+  for (int r = r0; r < rows; r += step) {
+    const int in = row0 + r, token = k.first + in / group, head = kvh * group + in % group;
+    if (r > r0) ahead(r);
     float4 sum[PER];
 #pragma unroll
     for (int i = 0; i < PER; ++i) sum[i] = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -232,7 +235,7 @@ __global__ void __launch_bounds__(32 * TREE_JOIN_WARPS) tree_join_kernel(const _
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
         const int p = p0 + u;
-        const size_t row = (size_t)(p == 0 ? slots.x : slots.y + 2 * (p - 1)) * rows_of_tile + r;
+        const size_t row = (size_t)(p == 0 ? item.y : item.z + 2 * (p - 1)) * shares.rows + r;
         ml[u] = p < parts ? reinterpret_cast<const float2*>(a.part_ml)[row] : make_float2(-INFINITY, 0.f);
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
@@ -280,10 +283,15 @@ __global__ void __launch_bounds__(32 * TREE_JOIN_WARPS) tree_join_kernel(const _
   OMNIA_TRACE_BLOCK(7);  // the rows are out
 }
 
+// The most tiles of rows that a request has.
+inline int tree_row_tiles(const TreeAttention& a, int most_nodes, int rows) { return (most_nodes * (a.nq / a.nkv) + rows - 1) / rows; }
+
+// (`a.parts` is that number.)
 template <typename T, int MOST>
 int tree_join(const TreeAttention& a, const TreeShares& shares, int most_nodes, int blocks, cudaStream_t stream) {
-  const int rows = min(shares.rows, most_nodes * (a.nq / a.nkv));
-  const dim3 grid(blocks - 1 + a.requests, min((rows + TREE_JOIN_WARPS - 1) / TREE_JOIN_WARPS, 16));
-  launch_pdl(tree_join_kernel<T, MOST>, grid, dim3(32 * TREE_JOIN_WARPS), 0, stream, a, shares, blocks, most_nodes);
+  const int rows = min(shares.rows, most_nodes * (a.nq / a.nkv)), items = a.requests * a.nkv * a.parts;
+  // A warp a row as long as blocks that have little to do are not many times what the GPU holds at once.
+  const dim3 grid(items, max(1, min(min((rows + TREE_JOIN_WARPS - 1) / TREE_JOIN_WARPS, 16), 4096 / items)));
+  launch_pdl(tree_join_kernel<T, MOST>, grid, dim3(32 * TREE_JOIN_WARPS), 0, stream, a, shares, 2 * blocks, most_nodes);
   return OMNIA_LAUNCH_RESULT();
 }

@@ -90,19 +90,15 @@ __global__ void __launch_bounds__(THREADS, D <= 128 ? 2 : 1) tree_shares_kernel(
   const TreeShares shares = {ROWS, KEYS, 1, EXTRA};
   const long long total = shares.lay_out(a, ends, sums);
   const long long blocks = min((long long)gridDim.x, total);  // (a block more than there are tiles would leave its slots unwritten)
-  TreePlace ahead;
-  if (blockIdx.x >= blocks) {
-    if (threadIdx.x == 0) tree_border(a, shares, total, blocks, 0, 0, ahead);
-    return;
-  }
-  const long long t0 = total * blockIdx.x / blocks;
+  if (blockIdx.x >= blocks) return;
+  const long long t0 = total * blockIdx.x / blocks, upto = total * (blockIdx.x + 1) / blocks;
   const int group = a.nq / a.nkv;
   const bf16 *kp = static_cast<const bf16*>(a.k_pages), *vp = static_cast<const bf16*>(a.v_pages);
   const long long apart = vp - kp;
 
   // ---- loads: lane l < 16 knows where the l-th row of its warp's share of a tile lies ------------------------------------------------
-  const long long begin = ahead.find(a, shares, ends, t0, (int)(total * (blockIdx.x + 1) / blocks - t0));
-  if (tid == 0) tree_border(a, shares, total, blocks, t0, begin, ahead);
+  TreePlace ahead;
+  ahead.find(a, shares, ends, t0, (int)(upto - t0));
   if (ahead.left == 0) return;
   TreePlace now = ahead;
   OMNIA_TRACE_BLOCK(2);  // the shares are known
@@ -160,6 +156,7 @@ __global__ void __launch_bounds__(THREADS, D <= 128 ? 2 : 1) tree_shares_kernel(
   while (now.left > 0) {
     const int rows = now.k.count * group, row0 = now.row_tile * ROWS + 16 * wr;
     if (entered) {
+      if (tid == 0 && now.tile == 0) tree_note(a, total, blocks, upto, now, first);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int row = row0 + g + 8 * h;
@@ -415,18 +412,20 @@ int launch(const TreeAttention& a, int blocks, cudaStream_t stream) {
 }  // namespace
 
 // `rows`: of a tile, 16, 32 or 64; `blocks`: what the work is shared out over, with two slots of rows each in part_o and part_ml.
-extern "C" int omnia_tree_attention_tc(const TreeAttention* a, int most_nodes, int rows, int blocks, void* stream) {
-  if (a->d != D || a->dv != D || a->requests < 1 || a->requests > TREE_MOST_REQUESTS || a->nkv < 1 || a->nkv > 65535 || a->nq % a->nkv || blocks < 1 ||
-      most_nodes < 1)
+extern "C" int omnia_tree_attention_tc(const TreeAttention* given, int most_nodes, int rows, int blocks, void* stream) {
+  TreeAttention a = *given;
+  if (a.d != D || a.dv != D || a.requests < 1 || a.requests > TREE_MOST_REQUESTS || a.nkv < 1 || a.nkv > 65535 || a.nq % a.nkv || blocks < 1 ||
+      most_nodes < 1 || (rows != 16 && rows != 32 && rows != 64))
     return (int)cudaErrorInvalidValue;
+  a.parts = tree_row_tiles(a, most_nodes, rows);
   const cudaStream_t s = (cudaStream_t)stream;
   int code;
-  if (rows == 16) code = launch<1>(*a, blocks, s);
-  else if (rows == 32) code = launch<2>(*a, blocks, s);
+  if (rows == 16) code = launch<1>(a, blocks, s);
+  else if (rows == 32) code = launch<2>(a, blocks, s);
 #if HEAD_DIM <= 128
-  else if (rows == 64) code = launch<4>(*a, blocks, s);
+  else if (rows == 64) code = launch<4>(a, blocks, s);
 #endif
   else return (int)cudaErrorInvalidValue;
   if (code) return code;
-  return tree_join<bf16, D>(*a, {rows, KEYS, 1, EXTRA}, most_nodes, blocks, s);
+  return tree_join<bf16, D>(a, {rows, KEYS, 1, EXTRA}, most_nodes, blocks, s);
 }

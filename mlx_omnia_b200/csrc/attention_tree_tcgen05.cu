@@ -129,10 +129,10 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_con
   const long long blocks = min((long long)gridDim.x, total);
   TreePlace place;  // (one warp's)
   place.left = 0;
-  if (warp == WARP_INIT) {
-    long long t0 = 0, begin = 0;
-    if (blockIdx.x < blocks) t0 = total * blockIdx.x / blocks, begin = place.find(a, shares, ends, t0, (int)(total * (blockIdx.x + 1) / blocks - t0));
-    if (lane == 0) tree_border(a, shares, total, blocks, t0, begin, place);
+  const long long upto = blocks ? total * (blockIdx.x + 1) / blocks : 0;
+  if (blockIdx.x < blocks && warp == WARP_INIT) {
+    const long long t0 = total * blockIdx.x / blocks;
+    place.find(a, shares, ends, t0, (int)(upto - t0));
   }
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // (the ends lie where copies will come to)
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -167,6 +167,7 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_con
     n.lo = place.tile * BN, n.hi = min((place.tile + tiles) * BN, place.k.total);
     const int rows = min(shares.rows, place.k.count * group - n.row0);
     n.whole = tiles == place.tiles, n.turns = rows <= slot_rows;
+    if (place.tile == 0) tree_note(a, total, blocks, upto, place, which == 0);
     place.next(a, shares, tiles);
     const uint32_t set = smem_u32(bars) + (which & 1) * BARS * 8;
     if (which > 1)
@@ -646,7 +647,7 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_con
 extern "C" int omnia_tree_tcgen05_rows(int group) { return 2 * (BM / group * group); }
 
 extern "C" int omnia_tree_attention_tcgen05(const TreeAttention* given, int most_nodes, int blocks, cudaStream_t stream) {
-  const TreeAttention a = *given;
+  TreeAttention a = *given;
   const int group = a.nkv > 0 ? a.nq / a.nkv : 0;
   if (a.requests < 1 || a.requests > TREE_MOST_REQUESTS || group < 1 || group > BM || a.nq != a.nkv * group || a.nkv > 65535 || a.d != D || a.dv != D ||
       a.page_size < 16 || a.page_size % 16 || a.max_pages < 1 || a.num_pages < 1 || ((uintptr_t)a.q & 15) || ((uintptr_t)a.k_pages & 15) ||
@@ -679,6 +680,7 @@ extern "C" int omnia_tree_attention_tcgen05(const TreeAttention* given, int most
     configured[device] = true;
   }
   const TreeShares shares = {omnia_tree_tcgen05_rows(group), BN, 16, EXTRA};
+  a.parts = tree_row_tiles(a, most_nodes, shares.rows);
   const cudaError_t e = launch_pdl(tree_tcgen05_kernel, dim3(blocks), THREADS, smem, stream, map_kv, map_q, a, shares);
   if (e != cudaSuccess) return (int)e;
   return tree_join<bf16, D>(a, shares, most_nodes, blocks, stream);

@@ -306,7 +306,7 @@ struct Tree {
   const void *q, *k_pages, *v_pages, *gate;
   void* out;
   const void *block_table, *cu_seqlens, *seq_lens, *positions, *ancestors, *sink;
-  void *part_o, *part_ml, *err, *borders;
+  void *part_o, *part_ml, *err, *items;
   long long page_stride;
   int tokens, requests, max_pages, num_pages, nq, nkv, d, dv, page_size, gate_stride, words, window, keep, run, chunk, parts;
   float scale, softcap;
@@ -359,10 +359,10 @@ PyObject* tree_attention(PyObject*, PyObject* const* args, Py_ssize_t given) {
     const int64_t slots = whole(args[24], what, "slots"), kind = whole(args[2], what, "kind"), parts = whole(args[23], what, "parts");
     at::Tensor part;
     if (slots) {
-      // Rows of sums, then their offsets and sums of weights; of the kernels by equal shares what the join does at each block's beginning, ahead of both.
-      const int64_t ahead = kind < 2 ? 8 * parts : 0;
+      // Rows of sums, then their offsets and sums of weights; of the kernels by equal shares where the join finds each tile of rows, ahead of both.
+      const int64_t tile = whole(args[25], what, "tile"), ahead = kind < 2 ? 4 * n * nkv * ((most * (nq / nkv) + tile - 1) / tile) : 0;
       part = empty(index, at::kFloat, {ahead + slots * (dv + 2)});
-      a.borders = part.data_ptr(), a.part_o = part.data_ptr<float>() + ahead, a.part_ml = part.data_ptr<float>() + ahead + slots * dv;
+      a.items = part.data_ptr(), a.part_o = part.data_ptr<float>() + ahead, a.part_ml = part.data_ptr<float>() + ahead + slots * dv;
     }
     a.q = q.data_ptr(), a.k_pages = pages.data_ptr(), a.v_pages = (const char*)a.k_pages + nkv * dk * page_size * size, a.out = out.data_ptr();
     a.err = error_word(index), a.page_stride = nkv * (dk + dv) * page_size;

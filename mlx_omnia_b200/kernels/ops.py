@@ -1417,24 +1417,25 @@ def tree_attention(q: torch.Tensor, kv: KVView, step: StepContext, scale: float,
         keys = min(keys, run + most)
     sms = sm_count(q.device) if index >= 0 else 1
     equal = dv == d and n <= 1024 and not base & 15  # what every kernel by equal shares takes
-    chunk_keys = tile = merge = 0
+    chunk_keys, tile, merge = 0, 32, 0
     if equal and bf16 and d % 8 == 0 and d <= 256 and not q.data_ptr() & 3:
         if (rows >= TREE_MANY_ROWS or (rows > 16 and keys >= TREE_MANY_KEYS)) and d in (64, 128) and page_size % 16 == 0 and scale > 0 and \
                 not q.data_ptr() & 15 and nq // nkv <= 128:
             kind, entry, tile = 0, _address("attention_tree_tcgen05", "omnia_tree_attention_tcgen05", d, index), 2 * (128 // (nq // nkv) * (nq // nkv))
-            parts = min(sms, n * nkv * -(-rows // tile) * -(-keys // 128))
+            parts, places = sms, -(-keys // 128) + 5
         else:
             kind, entry, tile = 1, _address("attention_tree_tc", "omnia_tree_attention_tc", d, index), 16 if rows <= 16 else 32 if rows <= 32 or d > 128 else 64
-            parts = min((2 if d <= 128 else 1) * sms, n * nkv * -(-rows // tile) * -(-keys // 64))
-        slots = 2 * parts * tile
+            parts, places = (2 if d <= 128 else 1) * sms, -(-keys // 64) + 3
     elif equal and q.dtype is torch.float32 and d % 4 == 0 and d <= 256:
         kind, entry = 0, _address("attention_tree", "omnia_tree_attention32", index=index)
-        parts = min((4 if d <= 32 else 2 if d <= 128 else 1) * sms, n * nkv * -(-rows // 32) * -(-keys // (64 if d <= 64 else 32)))
-        slots = 2 * parts * 32
+        parts, places = (4 if d <= 32 else 2 if d <= 128 else 1) * sms, -(-keys // (64 if d <= 64 else 32)) + 2
     else:
         kind, entry, merge = 2, _address("attention_tree", "omnia_tree_attention", index=index), _address("attention_tree", "omnia_tree_merge", index=index)
         chunk_keys, parts = tree_plan(-(-rows // 32) * n * nkv, keys, 64, 2 * sms)
         slots = parts * q.shape[0] * nq if parts > 1 else 0
+    if kind < 2:  # no more blocks than there are tiles, with the places that are kept for an item's beginning and end
+        parts = min(parts, n * nkv * -(-rows // tile) * places)
+        slots = 2 * parts * tile
     out = _host().tree_attention(entry, merge, kind, q, pages, kv.block_table, step.cu_seqlens, step.seq_lens, step.positions, tree.ancestors, gate, gate_col,
                                  sink, nkv, dk, dv, page_size, n, most, window, keep, run, chunk_keys, parts, slots, tile, scale, softcap or 0.0)
     _launched()
