@@ -50,6 +50,10 @@ __device__ long long tokens_ahead(const int* brought, int upto, long long* sums)
   return all;
 }
 
+// Bytes: 8 a token and table (its slot), 4 a column, 8 and the bits of its ancestors a token: 1.8 MB for 64 requests of 32,768 positions with 64 tokens in two
+// groups of caches, 0.3 us of memory; what it takes, 5.8 us of a replayed graph (8 requests with a token: 2.6), is a launch, a few dependent
+// reads of L2 (what is brought, where a list begins, the list) and, of trees, a round through shared memory for every doubling of a request's tokens.
+//
 // A block's row of the grid is a request (the last row: the tokens behind the last request's); the blocks of a row share its tokens and its
 // tables' columns. Each adds up for itself how many tokens come ahead: a few kilobytes out of L2, in place of a launch of its own.
 __global__ void __launch_bounds__(THREADS) step_tables_kernel(const __grid_constant__ StepTables a) {
@@ -148,7 +152,8 @@ __global__ void __launch_bounds__(THREADS) step_tables_kernel(const __grid_const
 }
 
 // A node is kept when every node on its way from node 0 is what was chosen behind its parent, the earliest of equal siblings. One
-// node at most of each depth is, so the kept ones are the ancestors of the last of them. A block a request, a node a thread.
+// node at most of each depth is, so the kept ones are the ancestors of the last of them. A block a request, a node a thread: a launch, two dependent reads
+// and the siblings' comparison in shared memory (64 requests of 64: 2.4 us of a replayed graph, one of 12 2.1; what it reads and writes are some kilobytes).
 __global__ void __launch_bounds__(THREADS)
 accept_drafts_kernel(const int* chosen, const int* ids, const int* ancestors, const int* cu_seqlens, int words, int* path, int* kept,
                      int* tokens, int rows, int* err) {
@@ -231,18 +236,21 @@ struct KeepRows {
 
 // A block has one request's kept rows in some layers, a thread a unit of U bytes of a position's rows in turn: it reads four kept positions' in two
 // layers and then writes them. A row goes to its own place or to an earlier one, and the rows of a path come in order, so what is written was
-// read before, or belongs to a draft that is not kept.
+// read before, or belongs to a draft that is not kept. Bytes: 2 rows of all layers a kept token that moves. One request's 3 in 28 layers are 0.7 MB and take 3.0 us
+// of a replayed graph, a launch and three dependent reads (which are kept, their pages, their rows); 64 requests' 76 in 36 layers 22 MB, 3.4 us at the memory's
+// rate, 6.0 here (10.1 with a division by the page's size at every access in place of one a row).
 template <typename U>
 __global__ void __launch_bounds__(THREADS) keep_rows_kernel(const __grid_constant__ KeepRows a) {
-  __shared__ long long from[MOST_NODES], to[MOST_NODES];  // rows of the whole pool: page * page_size + row
-  __shared__ int moves;
+  __shared__ long long from[MOST_NODES], to[MOST_NODES];  // where the page lies, in bytes from its layer's first one; -1: no move
+  __shared__ int from_row[MOST_NODES], to_row[MOST_NODES], path[MOST_NODES], moves;
   pdl_wait();
   pdl_launch_dependents();
   const int r = blockIdx.x, j = threadIdx.x;
   const int held = a.held[r], count = held < 0 ? 0 : min(max(a.kept[r], 0), a.most);
+  const int node = j < a.most ? a.path[(size_t)r * a.most + j] : -1;
+  path[j] = node;
   if (j == 0) moves = 0;
   __syncthreads();
-  const int node = j < count ? a.path[(size_t)r * a.most + j] : -1;
   const bool moved = j < count && node != j;
   if (moved) atomicAdd(&moves, 1);
   __syncthreads();
@@ -251,14 +259,14 @@ __global__ void __launch_bounds__(THREADS) keep_rows_kernel(const __grid_constan
   const int skip = count - moves;
   if (j < count) {
     int source = -1, target = -1;
-    if (moved && j >= skip && node > j && node < a.most && (j == 0 || node > a.path[(size_t)r * a.most + j - 1])) {
+    if (moved && j >= skip && node > j && node < a.most && (j == 0 || node > path[j - 1])) {
       const long long sp = ((long long)held + node) / a.page_size, dp = ((long long)held + j) / a.page_size;
       if (sp < a.width) source = a.table[(size_t)r * a.width + sp], target = a.table[(size_t)r * a.width + dp];
     }
     const bool good = source >= 0 && target >= 0 && source < a.num_pages && target < a.num_pages;
     if (moved && !good && blockIdx.y == 0) atomicOr(a.err, OMNIA_ERR_PAGE);
-    from[j] = good ? (long long)source * a.page_size + ((long long)held + node) % a.page_size : -1;
-    to[j] = good ? (long long)target * a.page_size + ((long long)held + j) % a.page_size : -1;
+    from[j] = good ? source * a.page_bytes : -1, from_row[j] = (int)(((long long)held + node) % a.page_size);
+    to[j] = good ? target * a.page_bytes : -1, to_row[j] = (int)(((long long)held + j) % a.page_size);
   }
   __syncthreads();
   for (int unit = j; unit < a.units; unit += THREADS) {
@@ -271,9 +279,7 @@ __global__ void __launch_bounds__(THREADS) keep_rows_kernel(const __grid_constan
     }
     const int width = a.row_units[kind], head = rest / width, column = rest % width;
     base += (long long)head * a.page_size * width + column;
-    auto at = [&](int layer, long long row) {
-      return reinterpret_cast<U*>(a.pages + layer * a.layer_bytes + row / a.page_size * a.page_bytes) + base + row % a.page_size * width;
-    };
+    auto at = [&](int layer, long long page, int row) { return reinterpret_cast<U*>(a.pages + layer * a.layer_bytes + page) + base + (long long)row * width; };
     for (int l0 = blockIdx.y; l0 < a.layers; l0 += 2 * gridDim.y)
       for (int i0 = skip; i0 < count; i0 += 4) {
         U held_rows[2][4];
@@ -281,12 +287,12 @@ __global__ void __launch_bounds__(THREADS) keep_rows_kernel(const __grid_constan
         for (int l = 0; l < 2; ++l)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if (l0 + l * (int)gridDim.y < a.layers && i0 + i < count && from[i0 + i] >= 0) held_rows[l][i] = *at(l0 + l * gridDim.y, from[i0 + i]);
+            if (l0 + l * (int)gridDim.y < a.layers && i0 + i < count && from[i0 + i] >= 0) held_rows[l][i] = *at(l0 + l * gridDim.y, from[i0 + i], from_row[i0 + i]);
 #pragma unroll
         for (int l = 0; l < 2; ++l)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if (l0 + l * (int)gridDim.y < a.layers && i0 + i < count && from[i0 + i] >= 0) *at(l0 + l * gridDim.y, to[i0 + i]) = held_rows[l][i];
+            if (l0 + l * (int)gridDim.y < a.layers && i0 + i < count && from[i0 + i] >= 0) *at(l0 + l * gridDim.y, to[i0 + i], to_row[i0 + i]) = held_rows[l][i];
       }
   }
 }
@@ -332,7 +338,7 @@ extern "C" int omnia_keep_rows(void* pages, long long layer_bytes, long long pag
   for (int k = 0; k < kinds; ++k) all |= bytes[k];
   const int unit = all % 16 == 0 ? 16 : all % 8 == 0 ? 8 : all % 4 == 0 ? 4 : all % 2 == 0 ? 2 : 1;
   for (int k = 0; k < kinds; ++k) a.heads[k] = heads[k], a.row_units[k] = bytes[k] / unit, a.units += heads[k] * a.row_units[k];
-  // Blocks that the GPU holds at once, each with as many layers as that takes. (64 requests in 36 layers, a block each: 15 us.)
+  // Blocks that the GPU holds at once, each with as many layers as that takes.
   const int room = 6 * omnia_sm_count() / requests;
   const dim3 grid(requests, room < 1 ? 1 : room < layers ? room : layers);
   const cudaStream_t s = (cudaStream_t)stream;
