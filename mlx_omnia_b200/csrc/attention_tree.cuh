@@ -183,7 +183,9 @@ __device__ __forceinline__ unsigned tree_pair(float lo, float hi) {
 }
 
 // An item that several blocks had part in, put together: a warp a row, the slots in the order of their blocks, eight on their way at once, the sink, the
-// gate. A block of the grid's first axis has an item (a request's first one: its zeros, where it sees nothing), whose rows the second axis shares out. What
+// gate. Bytes: 4 (D + 2) a row and piece, out of L2; what it takes, 3 to 5 us behind the kernel ahead, is the wait, where the item lies, and a round trip
+// for eight pieces. (Blocks by the borders of the kernel's blocks, most of which had nothing to do: 10 us for 592 blocks of 12 items' rows.) Offsets, sums and
+// what is summed are float32; one rounding to the output's type. A block of the grid's first axis has an item (a request's first one: its zeros, where it sees nothing), whose rows the second axis shares out. What
 // is read ahead of the wait was there ahead of the kernel that this one waits for. `slots`: how many there are.
 template <typename T, int MOST>
 __global__ void __launch_bounds__(32 * TREE_JOIN_WARPS) tree_join_kernel(const __grid_constant__ TreeAttention a, const TreeShares shares, int slots, int most) {

@@ -9,9 +9,12 @@
 // A block has a slice of SLICE tokens of a row. It asks for its logits, and while they come counts the occurrences of its own tokens in shared
 // memory: it reads the whole history (kilobytes, out of L2) and, of a drafted tree, the row's way, and keeps the entries of the biases' list that are
 // its own, in their order. So there are no counts in device memory to hold, clear or share, integers are all that is added without an order,
-// and no block waits for another. (Clusters whose blocks read a part of the history each and add to one another's counts: 64 rows of 24,000 tokens
-// 48 us in place of 53, but 21 in place of 14 where the history is short.) What bounds a new tensor of many rows is memory, 8 bytes a logit; in place
-// only what changes is touched.
+// and no block waits for another. A slice is 8,192 tokens: an SM holds five such blocks, and a
+// text is read by 19 of them where the vocabulary is 151,936. (Clusters whose blocks read a part of the history each and add to one another's counts: 64 rows of 24,000 tokens
+// 48 us in place of 53, but 21 in place of 14 where the history is short.) What bounds a new tensor of many rows is memory, 8 bytes a logit: 512
+// rows of 151,936 under masks, with texts of 2,000 tokens, 631 MB in 121 us (5.2 TB/s, 79 % of a copy's rate); 64 rows with texts of 6,000 and 40 biases
+// take 20.6 us of a replayed graph and 25.7 with cold caches, 12.0 of them memory, the rest the texts in all of a row's blocks; a row alone 5.0. In place only what changes is touched.
+// All is float32; what is counted are integers, so the order of additions to shared memory changes nothing.
 #include "common.cuh"
 
 struct AdjustLogits {
