@@ -1390,8 +1390,8 @@ def tree_attention(q: torch.Tensor, kv: KVView, step: StepContext, scale: float,
                    softcap: float | None = None) -> torch.Tensor:
     """Attention of the step's tokens where requests bring trees of drafted ones (`StepContext.tree`): a token sees the positions that its request
     holds and the tokens that its row of the tree names, whose keys and values are stored behind those in the order in which they are brought.
-    `gate`, `sink`, `window`, `keep_first`, `chunk`, `softcap` as for `paged_attention`, by the tokens' positions. A token that sees nothing
-    has zeros. -> [tokens, nq * dv] (rows behind the last request's are not written)"""
+    `gate`, `sink`, `window`, `keep_first`, `chunk`, `softcap` as for `paged_attention`, by the tokens' positions, which lie as `step_tables` makes them,
+    from `held` to `held` plus the tokens brought, less one. A token that sees nothing has zeros. -> [tokens, nq * dv] (rows behind the last request's are not written)"""
     what = "tree_attention"
     tree, pages, spec = step.tree, kv.pages, kv.spec
     if tree is None:
