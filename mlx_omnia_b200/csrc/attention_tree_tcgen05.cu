@@ -542,7 +542,7 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_con
         const float other_m = row_ml[((slot ^ 1) * BM + row) * 2], other_l = row_ml[((slot ^ 1) * BM + row) * 2 + 1];
         both = fmaxf(m, other_m);
         w = m == -INFINITY ? 0.f : fast_exp2(m - both);
-        l = l * w + (other_m == -INFINITY ? 0.f : other_l * fast_exp2(other_m - both));
+        l = l * w + other_l * (other_m == -INFINITY ? 0.f : fast_exp2(other_m - both));  // (a sum that is no number stays none)
       }
       const size_t part = (2 * (size_t)blockIdx.x + (first ? 0 : 1)) * shares.rows;
       if (ok && live && !s.whole && (!s.turns || slot == 0)) a.part_ml[2 * (part + my_row)] = both, a.part_ml[2 * (part + my_row) + 1] = l;

@@ -148,6 +148,21 @@ def test_a_query_that_is_no_number_has_no_number(layout, way):
         assert torch.isnan(got[bad]).all() and torch.equal(got[~bad], good[~bad])
 
 
+@pytest.mark.parametrize("layout", [(16, 8, 128, BF16, 16), (8, 2, 64, BF16, 16), (4, 4, 128, F32, 16), (4, 2, 130, F32, 16), (5, 1, 96, BF16, 8)], ids=str)
+@pytest.mark.parametrize("n", [3, 64])
+def test_a_key_that_is_no_number_reaches_all_who_see_it(layout, n, way):
+    """Also where it is all that a row sees of a tile, whoever has that tile."""
+    nq, nkv, d, dtype, page = layout
+    rng = random.Random(n)
+    c = make(nq, nkv, d, dtype, page, [(128 * rng.randint(1, 12), refs.chain(3) if r % 2 else [-1, -1, -1]) for r in range(n)], seed=n)
+    for r, (first, nodes, k, *_) in enumerate(c.requests):
+        held = len(k) - nodes
+        c.kv.row(0)[int(c.kv.block_table[r, held // page]), :, held % page, 1] = math.nan  # the first node's
+    got = ops.paged_attention(c.q, c.kv, c.step, d ** -0.5).view(n, 3, nq, d)
+    assert torch.isnan(got[1::2]).all()  # a chain: all see it
+    assert torch.isnan(got[0::2, 0]).all() and torch.isfinite(got[0::2, 1:]).all()
+
+
 def test_pages_beyond_31_bits(way):
     """A pool of 5 GB: pages whose first element lies beyond 2^31, attended to and moved within."""
     nkv, d, pages = 8, 128, 72_000
