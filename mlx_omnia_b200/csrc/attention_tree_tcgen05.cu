@@ -75,6 +75,20 @@ __device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, volatile
   *abort_flag = 1;
   return false;
 }
+// Whether three barriers' phases are complete: bits 0, 1, 2. A question takes some 300 cycles to be answered, so they are asked together.
+__device__ __forceinline__ uint32_t ask_three(uint32_t bar0, uint32_t parity0, uint32_t bar1, uint32_t parity1, uint32_t bar2, uint32_t parity2) {
+  uint32_t a, b, c;
+  asm volatile(
+      "{\n\t.reg .pred p, q, r;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%3], %4;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 q, [%5], %6;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 r, [%7], %8;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\tselp.u32 %1, 2, 0, q;\n\tselp.u32 %2, 4, 0, r;\n\t}"
+      : "=r"(a), "=r"(b), "=r"(c)
+      : "r"(bar0), "r"(parity0), "r"(bar1), "r"(parity1), "r"(bar2), "r"(parity2)
+      : "memory");
+  return a | b | c;
+}
 __device__ __forceinline__ void softmax_sync() { asm volatile("bar.sync 1, %0;" ::"n"(SOFTMAX_THREADS) : "memory"); }
 __device__ __forceinline__ void block_sync() { asm volatile("bar.sync 0, %0;" ::"n"(THREADS) : "memory"); }
 __device__ __forceinline__ void mbar_inval(uint32_t bar) { asm volatile("mbarrier.inval.shared::cta.b64 [%0];" ::"r"(bar) : "memory"); }
@@ -97,6 +111,8 @@ constexpr int TAIL_BYTES = 4 * BM * sizeof(float) + 2 * (sizeof(Segment) + 15) /
 
 }  // namespace
 
+// CAPPED: with a cap on the scores. (A kernel of its own: 300 instructions in the middle of a loop that is bound by fetching them, 2 % of long steps.)
+template <bool CAPPED>
 __global__ void __launch_bounds__(THREADS, 1)
 tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ TreeAttention a,
                     const TreeShares shares) {
@@ -285,32 +301,39 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_con
           // The second slot begins when the first one's first weights are there: its exponentials then run while the other one's products do, and
           // not beside the other one's exponentials.
           if (slot == 1 && tiles > 1 && ok) ok = wait_for(began, 0, abort_flag);
-          auto scores = [&](int u) {
-            const int h = u & 1, st = stage_of(slot, u);
-            ok = wait_for(k_full0 + 8 * st, phase_of(u), abort_flag);
+          // Stages are counted on, not divided out: this thread's instructions are what the slot's chain waits for.
+          const int base = s.turns ? slot * OWN_STAGES : 0;
+          int k_st = base, v_st = base;
+          uint32_t k_ph = 0, v_ph = 0;
+          auto scores = [&](int h, bool there) {  // of the next half; `there`: its keys have been seen to be
+            ok = there || wait_for(k_full0 + 8 * k_st, k_ph, abort_flag);
             if (!ok) return;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const uint64_t k_desc = desc_k_major(smem_u32(q_s + k_at + st * STAGE_BYTES));
+            const uint64_t k_desc = desc_k_major(smem_u32(q_s + k_at + k_st * STAGE_BYTES));
 #pragma unroll
             for (int kk = 0; kk < D / 16; ++kk)
               umma(s_tmem + h * HALF, q_desc + (((kk / 4) * HALF_BYTES + (kk % 4) * 32) >> 4),
                    k_desc + (((kk / 4) * SIDE_BYTES + (kk % 4) * 32) >> 4), instr_s, kk != 0);
             umma_commit(s_full0 + 8 * (2 * slot + h));
-            umma_commit(k_empty0 + 8 * st);
+            umma_commit(k_empty0 + 8 * k_st);
+            if (++k_st == base + stages) k_st = base, k_ph ^= 1;
           };
-          if (ok) scores(0);
-          if (ok && halves > 1) scores(1);
+          if (ok) scores(0, false);
+          if (ok && halves > 1) scores(1, false);
           for (int u = 0; u < halves && ok; ++u) {
-            const int h = u & 1, t = u >> 1, st = stage_of(slot, u);
-            ok = wait_for(v_full0 + 8 * st, phase_of(u), abort_flag) && wait_for(p_full0 + 8 * (2 * slot + h), t & 1, abort_flag);
+            const int h = u & 1;
+            const uint32_t t = (u >> 1) & 1, p_full = p_full0 + 8 * (2 * slot + h), o_done = o_done0 + 8 * (2 * slot + h);
+            const uint32_t there = ask_three(p_full, t, v_full0 + 8 * v_st, v_ph, k_full0 + 8 * k_st, k_ph);
+            ok = ((there & 2) || wait_for(v_full0 + 8 * v_st, v_ph, abort_flag)) && ((there & 1) || wait_for(p_full, t, abort_flag));
             if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             if (by_hand[2 * slot + h]) {
               by_hand[2 * slot + h] = 0;  // (the slot's warps write it again two halves on, behind products that come behind this)
               accumulate = 1;
             } else {
-              const uint64_t v_desc = desc_mn_major(smem_u32(q_s + v_at + st * STAGE_BYTES), SIDE_BYTES);
-              const int boxes = min(HALF, s.hi - first_of(j0, u) + 15) / 16;  // that were loaded: the rest of the stage is stale
+              const uint64_t v_desc = desc_mn_major(smem_u32(q_s + v_at + v_st * STAGE_BYTES), SIDE_BYTES);
+              // Boxes that were loaded: the rest of the stage, of a last half, is stale.
+              const int boxes = u + 1 < halves ? HALF / 16 : min(HALF, s.hi - first_of(j0, u) + 15) / 16;
 #pragma unroll
               for (int kk = 0; kk < HALF / 16; ++kk) {
                 if (kk >= boxes) break;
@@ -319,12 +342,13 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_con
                 accumulate = 1;
               }
             }
-            umma_commit(o_done0 + 8 * (2 * slot + h));
-            umma_commit(v_empty0 + 8 * st);
+            umma_commit(o_done);
+            umma_commit(v_empty0 + 8 * v_st);
+            if (++v_st == base + stages) v_st = base, v_ph ^= 1;
             // The half's columns are free once its weights have been read.
             if (u + 2 < halves) {
-              ok = wait_for(o_done0 + 8 * (2 * slot + h), t & 1, abort_flag);
-              if (ok) scores(u + 2);
+              ok = wait_for(o_done, t, abort_flag);
+              if (ok) scores(h, there & 4);
             }
           }
           // The last stage is free: this warp's products have told all barriers that wait for them, and the set may be made anew.
@@ -338,8 +362,7 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_con
     const int slot = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;
     const uint32_t lane_field = (uint32_t)(quarter * 32) << 16;
     const uint32_t s_addr = tmem_base + lane_field + slot * BN, o_addr = tmem_base + lane_field + O_COL + slot * D;
-    const bool capped = a.softcap > 0.f;
-    const float cap = a.softcap * LOG2E, twice = capped ? 2.f * a.scale / a.softcap * LOG2E : 0.f, unit = capped ? 1.f : a.scale * LOG2E;
+    const float cap = a.softcap * LOG2E, twice = CAPPED ? 2.f * a.scale / a.softcap * LOG2E : 0.f, unit = CAPPED ? 1.f : a.scale * LOG2E;
     bool first = true;
     while (next_segment()) {
       const Segment& s = segments[turn_of & 1];
@@ -416,7 +439,7 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_con
 #pragma unroll
           for (int c = 0; c < HALF; ++c) z[c] = __uint_as_float(raw[c]);
         }
-        if (capped) {  // c tanh(x) = c - 2 c / (1 + e^2x), in log2 units (a score that is infinite has the cap, of its sign)
+        if constexpr (CAPPED) {  // c tanh(x) = c - 2 c / (1 + e^2x), in log2 units (a score that is infinite has the cap, of its sign)
 #pragma unroll
           for (int c = 0; c < HALF; ++c) z[c] = fmaf(-2.f * cap, fast_rcp(1.f + fast_exp2(z[c] * twice)), cap);
         }
@@ -649,6 +672,24 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_con
   if (threadIdx.x == 0 && *abort_flag) atomicOr(a.err, OMNIA_ERR_TIMEOUT);
 }
 
+namespace {
+
+template <bool CAPPED>
+int launch(const CUtensorMap& map_kv, const CUtensorMap& map_q, const TreeAttention& a, const TreeShares& shares, int blocks, cudaStream_t stream) {
+  constexpr size_t smem = TILES * (size_t)TILE_BYTES + BAR_BYTES + TAIL_BYTES;
+  static bool configured[64] = {};
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) return (int)cudaErrorInvalidDevice;
+  if (!configured[device]) {
+    const cudaError_t e = cudaFuncSetAttribute(tree_tcgen05_kernel<CAPPED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return (int)e;
+    configured[device] = true;
+  }
+  return (int)launch_pdl(tree_tcgen05_kernel<CAPPED>, dim3(blocks), THREADS, smem, stream, map_kv, map_q, a, shares);
+}
+
+}  // namespace
+
 // Pages [num_pages, 2, nkv, page_size, D], page_size a multiple of 16; q [tokens, nq, D]. `blocks`: what the work is shared out over, an SM each, with
 // two slots of `omnia_tree_tcgen05_rows` rows in part_o and part_ml.
 extern "C" int omnia_tree_tcgen05_rows(int group) { return 2 * (BM / group * group); }
@@ -677,18 +718,9 @@ extern "C" int omnia_tree_attention_tcgen05(const TreeAttention* given, int most
   if (encode(&map_q, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(a.q), q_dims, q_strides, q_box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
     return (int)cudaErrorInvalidValue;
-  constexpr size_t smem = TILES * (size_t)TILE_BYTES + BAR_BYTES + TAIL_BYTES;
-  static bool configured[64] = {};
-  int device = 0;
-  if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) return (int)cudaErrorInvalidDevice;
-  if (!configured[device]) {
-    const cudaError_t e = cudaFuncSetAttribute(tree_tcgen05_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return (int)e;
-    configured[device] = true;
-  }
   const TreeShares shares = {omnia_tree_tcgen05_rows(group), BN, 16, EXTRA};
   a.parts = tree_row_tiles(a, most_nodes, shares.rows);
-  const cudaError_t e = launch_pdl(tree_tcgen05_kernel, dim3(blocks), THREADS, smem, stream, map_kv, map_q, a, shares);
-  if (e != cudaSuccess) return (int)e;
+  const int code = a.softcap > 0.f ? launch<true>(map_kv, map_q, a, shares, blocks, stream) : launch<false>(map_kv, map_q, a, shares, blocks, stream);
+  if (code) return code;
   return tree_join<bf16, D>(a, shares, most_nodes, blocks, stream);
 }
