@@ -4,13 +4,13 @@
 // Floor: a request's keys and values once (4 D bytes a position and key/value head) at the memory's rate, or the products' 4 D operations a row and
 // position, whichever is more; 256 rows are where the two meet.
 //
-// Measured (float32 softmax; error against 64 bits 0.0023 of the outputs' size where a 32-bit form rounded once has 0.0017): 32 / 8 heads of 128, 32 requests of
-// up to 8,192 positions with up to 64 tokens (795 MB, 0.14 PFLOP) 297 to 327 us: 0.46 PFLOP/s, 2.6 TB/s; what bounds it is a tile's chain, 2.7 us for 128 keys of 256 rows: scores, exponentials
-// of a row by the thread that has it, weights back to tensor memory, the product, where the two products alone would take 1.5. Of a half's 2,850 cycles a softmax warp asks whether its scores are there for 330, loads them for 170, has the maximum after 370,
-// the offset after 330, weights, sums and pairs after 1,350 (707 of them without the exponentials) and has stored these after 320; products, keys and values are ahead of it. Pairs of float32 in one
-// instruction and maxima of three made the weights 1,030, and everything beside them longer by what did not fit in registers: 339 us. A profiler counts 0.94
-// warps that wait for an instruction to be fetched for every one issued: what is taken out of the loop, though never run, is gained. 4 of up to 131,072 with up to 24
-// (1.49 GB) 270 to 328 us, 4.5 to 5.5 TB/s; 8 of up to 4,096 with up to 16, 16 / 8 heads (100 MB), 39 us, of which 12 to 15 are beginnings, ends and the join.
+// Measured, 32 / 8 heads of 128: 32 requests of up to 8,192 positions with up to 64 tokens (795 MB, 0.14 PFLOP) 297 to 327 us, 0.46 PFLOP/s, 2.6 TB/s; 4
+// of up to 131,072 with up to 24 (1.49 GB) 270 to 328, 4.5 to 5.5 TB/s. 16 / 8 heads, 8 of up to 4,096 with up to 16 (100 MB): 39, of which 12 to 15 are
+// beginnings, ends and the join. What bounds the long ones is a tile's chain, 2.7 us for 128 keys of 256 rows, where the products alone would take 1.5. Of
+// the 2,850 cycles that a softmax warp has for a half, 330 go to whether the scores are there, 170 to their load, 370 to the maximum, 330 to the offset,
+// 1,350 to weights, sums and pairs (707 without the exponentials), 320 to the store. For every instruction issued 0.94 warps wait for one to be fetched: code
+// taken out of the loop, though never run, is gained. Float32 in pairs and maxima of three: 1,030 for the weights, the same time in all. Error against
+// 64 bits 0.0023 of the outputs' size, where a 32-bit form rounded once has 0.0017.
 //
 // A block has an SM and an equal share of the step's tiles of 128 keys (TreeShares), and works it off item by item: up to 256 rows (node, query
 // head of the group) of one request and key/value head, in two slots of 128 that are two softmax chains. Each slot has a score tile of 128
