@@ -1407,6 +1407,8 @@ def tree_attention(q: torch.Tensor, kv: KVView, step: StepContext, scale: float,
     run, page_size, n, most = int(chunk or 0), kv.page_size, step.num_seqs, step.max_q_len
     if run and keep:
         raise KernelError("a mask of runs keeps no first positions")
+    if window < 0 or keep < 0 or run < 0:
+        raise KernelError(f"{what}: a window of {window} positions, {keep} kept ones, runs of {run}: none is below 0")
     index, base, bf16 = q.get_device(), pages.data_ptr(), q.dtype is torch.bfloat16
     rows = most * (nq // nkv)
     # What the longest request can see: plans are made for that, and from numbers that a captured step knows too.

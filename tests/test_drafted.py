@@ -430,7 +430,7 @@ def test_attention_of_trees_that_is_refused():
                   {"kv": view(spec=KVSpec(((2, 8), (2, 8)), stride=2))}, {"gate": torch.zeros(2, 32)[:, ::2]}, {"gate": torch.zeros(2, 31)},
                   {"gate": torch.zeros(2, 40), "gate_col": 9}, {"gate": torch.zeros(2, 40), "gate_col": -1}, {"gate": torch.zeros(3, 40)},
                   {"gate": torch.zeros(2, 40, dtype=torch.bfloat16)}, {"sink": torch.zeros(3)}, {"sink": torch.zeros(4, dtype=torch.bfloat16)},
-                  {"window": 4, "keep_first": 1, "chunk": 4}, {}):  # the last: on the CPU
+                  {"window": 4, "keep_first": 1, "chunk": 4}, {"window": -2}, {"window": 4, "keep_first": -1}, {"chunk": -4}, {}):  # the last: on the CPU
         with pytest.raises(ops.KernelError):
             ops.tree_attention(**good | wrong)
     with pytest.raises(ops.KernelError, match="difference"):

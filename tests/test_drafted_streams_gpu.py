@@ -13,7 +13,7 @@ import torch
 import drafted_refs as refs
 from mlx_omnia_b200.kernels import ops
 from mlx_omnia_b200.parts.base import KVSpec, KVView, StepContext
-from test_drafted_gpu import BF16, F32, check, ints, make, no_errors, way  # noqa: F401  (the fixtures too)
+from test_drafted_gpu import BF16, F32, check, check_window, ints, make, no_errors, way  # noqa: F401  (the fixtures too)
 
 pytestmark = pytest.mark.gpu
 PAGE, VOCAB, WORDS = 16, 9000, 1
@@ -194,6 +194,16 @@ def test_logits_beyond_31_bits():
     ops.adjust_logits(logits, masks=masks, out=logits)
     assert bool(torch.isfinite(logits[: rows - 2]).all())
     assert torch.isfinite(logits[rows - 2:]).sum(1).tolist() == [vocab // 32] * 2
+
+
+@pytest.mark.parametrize("layout", [(16, 8, 128, BF16, 16), (4, 4, 128, F32, 16), (4, 2, 130, F32, 16)], ids=str)
+def test_windows_beyond_31_bits(layout, way):
+    """As wide as a number can be said: all that is held, with or without kept positions."""
+    nq, nkv, d, dtype, page = layout
+    for window, keep in ((1 << 40, 0), ((1 << 31) - 1, 5), (1 << 31, 1 << 33)):
+        check_window(make(nq, nkv, d, dtype, page, [(300, refs.tree(9, 1)), (1, [-1])], window=window, keep=keep), d, window, keep)
+    with pytest.raises(ops.KernelError):
+        ops.tree_attention(*(lambda c: (c.q, c.kv, c.step, 0.1))(make(nq, nkv, d, dtype, page, [(30, [-1])])), window=-2)
 
 
 def test_the_most_requests_and_the_next():
