@@ -613,6 +613,7 @@ extern "C" int omnia_tree_attention(const TreeAttention* a, int most_nodes, int 
 }
 
 extern "C" int omnia_tree_merge(const TreeAttention* a, int dtype, void* stream) {
+  if ((uintptr_t)a->part_ml & 7) return (int)cudaErrorInvalidValue;  // (offsets and sums are read in pairs)
   const dim3 grid((a->tokens * a->nq + THREADS / 32 - 1) / (THREADS / 32));
   OMNIA_DISPATCH_DTYPE(dtype, launch_pdl(tree_merge_kernel<T>, grid, dim3(THREADS), 0, (cudaStream_t)stream, *a));
   return OMNIA_LAUNCH_RESULT();

@@ -359,10 +359,12 @@ PyObject* tree_attention(PyObject*, PyObject* const* args, Py_ssize_t given) {
     const int64_t slots = whole(args[24], what, "slots"), kind = whole(args[2], what, "kind"), parts = whole(args[23], what, "parts");
     at::Tensor part;
     if (slots) {
-      // Rows of sums, then their offsets and sums of weights; of the kernels by equal shares where the join finds each tile of rows, ahead of both.
+      // Rows of sums, then their offsets and sums of weights, which are read in pairs: on a multiple of 16 bytes whatever the widths. Of the kernels by
+      // equal shares where the join finds each tile of rows, ahead of both.
       const int64_t tile = whole(args[25], what, "tile"), ahead = kind < 2 ? 4 * n * nkv * ((most * (nq / nkv) + tile - 1) / tile) : 0;
-      part = empty(index, at::kFloat, {ahead + slots * (dv + 2)});
-      a.items = part.data_ptr(), a.part_o = part.data_ptr<float>() + ahead, a.part_ml = part.data_ptr<float>() + ahead + slots * dv;
+      const int64_t sums = (slots * dv + 3) / 4 * 4;
+      part = empty(index, at::kFloat, {ahead + sums + 2 * slots});
+      a.items = part.data_ptr(), a.part_o = part.data_ptr<float>() + ahead, a.part_ml = part.data_ptr<float>() + ahead + sums;
     }
     a.q = q.data_ptr(), a.k_pages = pages.data_ptr(), a.v_pages = (const char*)a.k_pages + nkv * dk * page_size * size, a.out = out.data_ptr();
     a.err = error_word(index), a.page_stride = nkv * (dk + dv) * page_size;

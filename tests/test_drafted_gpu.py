@@ -234,6 +234,21 @@ def test_attention_of_trees(layout, way):
     check(c, -0.3 * d ** -0.5, sink=True)
 
 
+WIDTHS = [(3, 1, 33, 33), (4, 2, 48, 32), (3, 3, 32, 80), (3, 1, 33, 17), (5, 1, 1, 7), (2, 1, 7, 300), (1, 1, 260, 129), (1, 1, 9, 511)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("layout", WIDTHS, ids=str)
+def test_keys_and_values_of_any_widths(layout, dtype):
+    """Keys and values that differ in width, odd widths: the kernel for any shape, its keys in one piece and in several (of an odd count too)."""
+    nq, nkv, d, dv = layout
+    for requests in ([(145, refs.tree(5, 1))], [(20, refs.tree(5, 2))], [(300, refs.chain(3)), (0, [-1]), (64, refs.tree(9, 3))], [(1000, [-1])]):
+        c = make(nq, nkv, d, dtype, 16, requests, dv=dv, seed=d + dv)
+        check(c, d ** -0.5)
+        check(c, d ** -0.5, gated=True, sink=True, softcap=2.0)
+        check_window(c, d, 150, keep=3, sink=True)
+
+
 @pytest.mark.parametrize("layout", LAYOUTS[:6] + LAYOUTS[8:10], ids=str)
 def test_attention_of_trees_under_windows(layout, way):
     nq, nkv, d, dtype, page = layout
