@@ -79,9 +79,11 @@ __global__ void __launch_bounds__(THREADS) step_tables_kernel(const __grid_const
     return;
   }
   const int held = a.held[r], wanted = max(a.brought[r], 0);
-  const bool padding = held < 0;  // a request that is there for the step's shape only
   int count = min(wanted, a.tokens - first);
+  const bool beyond = (long long)held + count > 0x7fffffffLL;  // positions are numbers of 31 bits
+  const bool padding = held < 0 || beyond;                     // a request that is there for the step's shape only
   if (part == 0 && threadIdx.x == 0) {
+    if (beyond) atomicOr(a.err, OMNIA_ERR_WORK);
     a.cu_seqlens[r] = first;
     a.seq_lens[r] = padding ? 0 : held + count;
   }
@@ -90,7 +92,7 @@ __global__ void __launch_bounds__(THREADS) step_tables_kernel(const __grid_const
     const long long start = group.starts[r];
     const int rows = padding ? 0 : (int)(((long long)held + count + group.stride - 1) / group.stride);
     const int pages = (int)(((long long)rows + a.page_size - 1) / a.page_size);
-    const bool fits = pages <= group.width && start >= 0 && start + pages <= group.count;
+    const bool fits = pages <= group.width && start >= 0 && start <= group.count - pages;
     if (!fits && pages && part == 0 && threadIdx.x == 0) atomicOr(a.err, OMNIA_ERR_WORK);
     int* table = group.table + (size_t)r * group.width;
     for (int c = part * THREADS + threadIdx.x; c < group.width; c += parts * THREADS)

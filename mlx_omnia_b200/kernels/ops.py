@@ -1333,8 +1333,9 @@ def step_tables(held: torch.Tensor, brought: torch.Tensor, lists: "list[PageList
     of it), a token's position is `held` plus the number of tokens on its way, and `tree` names what it sees. Slots go by the order in which tokens
     are brought, whatever their positions.
 
-    A list too short or a table too narrow for its request, more tokens than rows, a parent that is no earlier token: the error word, and
-    -1 in the request's tables (`raise_on_error`)."""
+    The error word (`raise_on_error`) reports a list too short or a table too narrow for its request (-1 in its tables), positions beyond 31 bits
+    (the request is one that holds nothing), more tokens than rows or than `most` (those behind are left out), a page that was given back (slot -1), and a
+    parent that is no earlier token (it goes on from what is held)."""
     positions, cu_seqlens, seq_lens, groups, ancestors = _host().step_tables(_address("drafted", "omnia_step_tables", index=held.get_device()), held, brought,
                                                                              lists, page_size, tokens, parents, most)
     _launched()

@@ -129,6 +129,20 @@ def test_tables_report_what_does_not_fit():
     assert error_of(16) and made.positions.tolist() == list(range(32)) + [-1] * 8
 
 
+def test_tables_of_numbers_at_the_end_of_their_types():
+    lists = lambda pages, width: [ops.PageLists(ints(pages), ints([0], torch.int64), width)]  # noqa: E731
+    for trees in ({}, {"most": 2}):  # positions beyond 31 bits, by one and by two
+        for held, brought in (([7, 2 ** 31 - 1, 3], [1, 1, 1]), ([7, 2 ** 31 - 2, 3], [1, 2, 1])):
+            made = ops.step_tables(ints(held), ints(brought), [ops.PageLists(ints([3, 4]), ints([0, 1, 1], torch.int64), 1)], 16, sum(brought), **trees)
+            n = brought[1]
+            assert error_of(16) and made.positions.tolist() == [7] + [-1] * n + [3] and made.seq_lens.tolist() == [8, 0, 4]
+            assert made.groups[0][0].tolist() == [[3], [-1], [4]] and made.groups[0][1].tolist() == [55] + [-1] * n + [67]
+    made = ops.step_tables(ints([2 ** 31 - 2]), ints([1]), lists([3, 4], 2), 16, 1)  # the last position of 31 bits, in a table too narrow
+    assert error_of(16) and made.seq_lens.tolist() == [2 ** 31 - 1] and made.groups[0][1].tolist() == [-1]
+    made = ops.step_tables(ints([20]), ints([1]), [ops.PageLists(ints([3, 4]), ints([2 ** 63 - 1], torch.int64), 2)], 16, 1)  # a list that begins nowhere
+    assert error_of(16) and made.groups[0][0].tolist() == [[-1, -1]] and made.groups[0][1].tolist() == [-1]
+
+
 # -- attention -------------------------------------------------------------------------------------------------------
 @dataclasses.dataclass
 class Case:
