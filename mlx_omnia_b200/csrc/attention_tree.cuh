@@ -36,13 +36,14 @@ __device__ __forceinline__ TreeKeys tree_keys(const TreeAttention& a, int reques
   const int held = a.seq_lens[request];
   k.held = held - k.count;
   k.lo = k.kept = k.total = 0;
-  if (held <= 0 || k.count <= 0) {  // a request that is there for the step's shape only
+  // Rows that are not the step's (also of a request that sees nothing, whose zeros are written), or more than there are bits for.
+  if (k.first < 0 || k.count < 0 || k.count > a.tokens - k.first || (held > 0 && (k.held < 0 || k.count > 32 * a.words))) {
+    atomicOr(a.err, OMNIA_ERR_WORK);
+    k.count = k.first < 0 ? 0 : max(0, min(k.count, a.tokens - k.first));
     k.held = 0;
     return k;
   }
-  if (k.held < 0 || k.count > 32 * a.words || k.first < 0 || k.first + k.count > a.tokens) {
-    atomicOr(a.err, OMNIA_ERR_WORK);
-    k.count = k.first < 0 ? 0 : min(k.count, a.tokens - k.first);
+  if (held <= 0 || k.count == 0) {  // a request that is there for the step's shape only
     k.held = 0;
     return k;
   }

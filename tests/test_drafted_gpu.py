@@ -344,6 +344,26 @@ def test_padding_and_rows_behind_the_last_request(way):
         assert float(got[6].abs().max()) == 0
 
 
+@pytest.mark.parametrize("layout", [LAYOUTS[0], LAYOUTS[4], LAYOUTS[9], LAYOUTS[7]], ids=str)
+def test_requests_whose_rows_are_not_the_steps(layout, way):
+    """Rows behind the step's last one, of a request that holds something and of one that is there for the shape only, and a list that goes back: reported,
+    and the other requests' rows are as ever."""
+    nq, nkv, d, dtype, page = layout
+    c = make(nq, nkv, d, dtype, page, [(20, refs.tree(6, 1)), (7, refs.tree(4, 2))], seed=2)  # (a tile of keys each: no sum is split otherwise)
+    expect = check(c, d ** -0.5)
+    lengths, ends = c.step.seq_lens.clone(), c.step.cu_seqlens.clone()
+    for held, cu in ((0, [0, 6, 13]), (11, [0, 6, 13]), (-1, [0, 6, 10 + 20]), (0, [0, 6, 2 ** 31 - 1]), (0, [0, 6, 5]), (11, [0, 6, 2]), (0, [0, 6, -4])):
+        c.step.seq_lens.copy_(ints([26, held]))
+        c.step.cu_seqlens.copy_(ints(cu))
+        got = ops.paged_attention(c.q, c.kv, c.step, d ** -0.5)
+        assert error_of(16) and torch.equal(got[:6], expect[:6])
+        if cu[2] > 10:
+            assert float(got[6:].abs().max()) == 0
+    c.step.seq_lens.copy_(lengths)
+    c.step.cu_seqlens.copy_(ends)
+    assert torch.equal(check(c, d ** -0.5), expect)
+
+
 def test_a_captured_step_takes_the_lengths_of_its_replay(way):
     nq, nkv, d, dtype, page = LAYOUTS[0]
     big = make(nq, nkv, d, dtype, page, [(900, refs.tree(16, 1)), (300, refs.tree(16, 2))], seed=3)
