@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(THREADS, 5) adjust_logits_kernel(const __grid_
       if (a.repetition) p.repetition = a.repetition[request];
       if (a.frequency) p.frequency = a.frequency[request];
       if (a.presence) p.presence = a.presence[request];
-      if (start < 0 || length < 0 || start + length > a.history_tokens) {
+      if (start < 0 || length < 0 || start > a.history_tokens - length) {
         if (tid == 0) atomicOr(a.err, OMNIA_ERR_WORK);
         length = 0;
       }

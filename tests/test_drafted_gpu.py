@@ -531,6 +531,15 @@ def test_a_bias_named_many_times_adds_in_order():
     assert np.array_equal(np.asarray(answers.pop(), dtype=np.float32), expect)
 
 
+@pytest.mark.parametrize("start,length", [(2 ** 63 - 1, 3), (2 ** 63 - 5, 2), (-1, 3), (-2 ** 63, 1), (8, 3), (0, 11), (11, 0), (0, -1)])
+def test_texts_that_lie_nowhere(start, length):
+    """Reported, and nothing is counted."""
+    logits = torch.ones(1, 50, device="cuda")
+    history = ops.TokenHistory(ints(list(range(10))), ints([start], torch.int64), ints([length]), ints([0]))
+    got = ops.adjust_logits(logits, history=history, frequency=torch.ones(1, device="cuda"))
+    assert error_of(16) and torch.equal(got, logits)
+
+
 def test_adjust_reports_bad_numbers():
     logits = torch.zeros(2, 100, device="cuda")
     run = lambda **more: call_adjust(logits, *({"texts": [[1], [2]], "prompts": [0, 0], "values": [[1.0] * 2] * 3, "bias": [[], []], "masks": [None] * 2} | more).values(), "pb")  # noqa: E731
