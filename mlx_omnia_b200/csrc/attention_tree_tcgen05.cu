@@ -352,8 +352,14 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_con
               if (ok) scores(h, there & 4);
             }
           }
-          // The last stage is free: this warp's products have told all barriers that wait for them, and the set may be made anew.
-          if (ok) wait_for(v_empty0 + 8 * stage_of(slot, halves - 1), phase_of(halves - 1), abort_flag);
+        }
+        __syncwarp();
+        // The set is made anew behind this segment, so whatever this slot's products tell a barrier has to have been told: the stages that they read
+        // last and the accumulator's last two halves, a lane a barrier. (What else arrives, another warp of the segment has waited for.)
+        const int back = lane & 7, last = halves - 1 - back;
+        if (last >= 0 && back < (lane < 16 ? stages : lane < 24 ? 2 : 0)) {
+          const uint32_t bar = lane < 16 ? (lane < 8 ? k_empty0 : v_empty0) + 8 * stage_of(slot, last) : o_done0 + 8 * (2 * slot + (last & 1));
+          wait_for(bar, lane < 16 ? phase_of(last) : (last >> 1) & 1, abort_flag);
         }
         __syncwarp();
       }

@@ -364,6 +364,16 @@ def test_requests_whose_rows_are_not_the_steps(layout, way):
     assert torch.equal(check(c, d ** -0.5), expect)
 
 
+@pytest.mark.parametrize("d", [64, 128])
+def test_blocks_of_many_items(d, way):
+    """Blocks that work off eight items and more each, of few rows and of many in turn, again and again."""
+    sizes = [(37 * i % 300, (5, 64, 1, 40, 33)[i % 5]) for i in range(300)]
+    c = make(16, 4, d, BF16, 16, [(held, refs.tree(nodes, held)) for held, nodes in sizes], seed=d)
+    expect = check(c, d ** -0.5)
+    for _ in range(10):
+        assert torch.equal(ops.paged_attention(c.q, c.kv, c.step, d ** -0.5), expect)
+
+
 def test_a_captured_step_takes_the_lengths_of_its_replay(way):
     nq, nkv, d, dtype, page = LAYOUTS[0]
     big = make(nq, nkv, d, dtype, page, [(900, refs.tree(16, 1)), (300, refs.tree(16, 2))], seed=3)
