@@ -23,7 +23,8 @@ namespace {
 constexpr int THREADS = 128, ROWS = 32;
 constexpr float LOG2E = 1.4426950408889634f;
 
-__device__ __forceinline__ bool tid0() { return threadIdx.x == 0 && blockIdx.x == 0 && blockIdx.y == 0; }
+// Of the kernel for any shape: one thread a request and key/value head.
+__device__ __forceinline__ bool tid0() { return threadIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0; }
 
 template <typename T>
 __device__ __forceinline__ void finish_dim(const TreeAttention& a, int token, int head, int dim, float value) {
@@ -45,7 +46,7 @@ __global__ void __launch_bounds__(THREADS) tree_pieces_kernel(const __grid_const
   __shared__ float top[ROWS], sum[ROWS], factor[ROWS];
   pdl_wait();
   pdl_launch_dependents();
-  const int request = blockIdx.z / a.nkv, kvh = blockIdx.z % a.nkv, part = blockIdx.x, group = a.nq / a.nkv;
+  const int request = blockIdx.x / a.nkv, kvh = blockIdx.x % a.nkv, part = blockIdx.z, group = a.nq / a.nkv;
   const TreeKeys k = tree_keys(a, request);
   if ((k.total > (long long)a.parts * a.chunk || k.count * group > (int)gridDim.y * ROWS) && tid0()) atomicOr(a.err, OMNIA_ERR_WORK);
   const int rows = k.count * group, row0 = blockIdx.y * ROWS, here = min(rows - row0, ROWS);
@@ -569,7 +570,8 @@ int launch_pieces(const TreeAttention& a, int most_nodes, cudaStream_t stream) {
     if (e != cudaSuccess) return (int)e;
     ready[device] = true;
   }
-  const dim3 grid(a.parts, (most_nodes * (a.nq / a.nkv) + ROWS - 1) / ROWS, a.requests * a.nkv);
+  // (The first axis of a grid takes 2^31 - 1 blocks, the others 65,535.)
+  const dim3 grid(a.requests * a.nkv, (most_nodes * (a.nq / a.nkv) + ROWS - 1) / ROWS, a.parts);
   launch_pdl(tree_pieces_kernel<T, MOST, KEYS>, grid, dim3(THREADS), bytes, stream, a);
   return OMNIA_LAUNCH_RESULT();
 }
@@ -606,8 +608,8 @@ int launch_shares32(TreeAttention a, int most_nodes, int blocks, cudaStream_t st
 }  // namespace
 
 extern "C" int omnia_tree_attention(const TreeAttention* a, int most_nodes, int dtype, void* stream) {
-  if (a->d < 1 || a->dv < 1 || a->d > 512 || a->dv > 512 || a->nkv < 1 || a->nq % a->nkv || a->requests < 1 || (long long)a->requests * a->nkv > 65535 ||
-      most_nodes < 1 || a->chunk < 1 || a->parts < 1 || a->page_size < 1)
+  if (a->d < 1 || a->dv < 1 || a->d > 512 || a->dv > 512 || a->nkv < 1 || a->nq % a->nkv || a->requests < 1 ||
+      (long long)a->requests * a->nkv > 0x7fffffffLL || a->parts > 65535 || most_nodes < 1 || a->chunk < 1 || a->parts < 1 || a->page_size < 1)
     return (int)cudaErrorInvalidValue;
   OMNIA_DISPATCH_DTYPE(dtype, return launch_tree<T>(*a, most_nodes, (cudaStream_t)stream));
 }

@@ -364,6 +364,14 @@ def test_requests_whose_rows_are_not_the_steps(layout, way):
     assert torch.equal(check(c, d ** -0.5), expect)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_more_requests_times_heads_than_an_axis_of_a_grid_takes(dtype):
+    """65,600 of them, for the kernel of any shape: more than 1,024 requests, with one piece of keys."""
+    c = make(8, 8, 8, dtype, 4, [(i % 7, refs.chain(1 + i % 2)) for i in range(8200)], seed=1)
+    c.requests = c.requests[::50] + c.requests[-3:]
+    check(c, 8 ** -0.5, sink=True)
+
+
 @pytest.mark.parametrize("d", [64, 128])
 def test_blocks_of_many_items(d, way):
     """Blocks that work off eight items and more each, of few rows and of many in turn, again and again."""
