@@ -150,8 +150,9 @@ __global__ void __launch_bounds__(THREADS, D <= 128 ? 2 : 1) tree_shares_kernel(
   for (int s = 0; s < STAGES - 1; ++s) fetch();
 
   const bool capped = a.softcap > 0.f;
-  // Scores keep the sign that they are compared by: a scale below zero turns the queries' signs instead.
-  const float size = fabsf(a.scale), cap = a.softcap * LOG2E, twice = capped ? 2.f * size / a.softcap * LOG2E : 0.f, unit = capped ? 1.f : size * LOG2E;
+  // Scores keep the sign that they are compared by: a scale below zero turns the queries' signs instead. (A scale of zero is float32's least number: what a
+  // row does not see is -infinity ahead of it, which zero would make no number.)
+  const float size = fabsf(a.scale), cap = a.softcap * LOG2E, twice = capped ? 2.f * size / a.softcap * LOG2E : 0.f, unit = capped ? 1.f : size == 0.f ? 1.17549435e-38f : size * LOG2E;
   const unsigned turn = a.scale < 0.f ? 0x80008000u : 0u;
   unsigned qf[KSTEPS][4];
   float o[NT_O][4], m[2], l[2];

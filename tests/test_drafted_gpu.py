@@ -248,6 +248,17 @@ def test_attention_of_trees(layout, way):
     check(c, -0.3 * d ** -0.5, sink=True)
 
 
+@pytest.mark.parametrize("layout", [LAYOUTS[0], LAYOUTS[3], LAYOUTS[4], LAYOUTS[8], LAYOUTS[9]], ids=str)
+def test_a_scale_of_zero(layout, way):
+    """All that a row sees weighs the same."""
+    nq, nkv, d, dtype, page = layout
+    c = make(nq, nkv, d, dtype, page, [(70, refs.tree(13, 1)), (0, refs.tree(5, 2)), (1, [-1])], seed=d)
+    for scale in (0.0, -0.0, 1e-42):
+        for options in ({}, {"sink": True}, {"softcap": 3.0}):
+            check(c, scale, **options)
+        check(c, scale, window=9, keep=2, call=lambda **more: ops.paged_attention(c.q, c.kv, c.step, scale, window=9, keep_first=2, **more))
+
+
 WIDTHS = [(3, 1, 33, 33), (4, 2, 48, 32), (3, 3, 32, 80), (3, 1, 33, 17), (5, 1, 1, 7), (2, 1, 7, 300), (1, 1, 260, 129), (1, 1, 9, 511)]
 
 
