@@ -106,13 +106,13 @@ class Generator:
         vocab = self.engine.vocab_size
         if any(not 0 <= t < vocab for t in prompt):
             raise ValueError(f"a prompt token lies outside the vocabulary of {vocab}")
-        if any(token >= vocab for token in options.bias or ()):
+        params = options.params()
+        if any(token >= vocab for token, _ in params.bias):
             raise ValueError(f"a bias names a token outside the vocabulary of {vocab}")
         budget = options.max_tokens
         if options.context_limit is not None:
             budget = min(budget, options.context_limit - len(prompt))
         stop = options.stop if options.stop is not None else self.default_stop
-        params = options.params()
         request = Request(request_id or f"req-{next(self._ids)}", prompt, max(budget, 0), params, frozenset(stop))
         if leader is not None:
             request.fork_at = common_start([leader.prompt, prompt[:-1]]) if fork_at is None else int(fork_at)

@@ -34,6 +34,13 @@ class SamplingParams:
     bias: tuple[tuple[int, float], ...] = ()
     constraint: "Callable[[Sequence[int]], Collection[int] | None] | None" = None
 
+    def __post_init__(self) -> None:
+        if not all(math.isfinite(x) for x in (self.frequency_penalty, self.presence_penalty)):
+            raise ValueError("frequency_penalty and presence_penalty are finite numbers")
+        for token, value in self.bias:
+            if token < 0 or math.isnan(value) or value == math.inf:
+                raise ValueError(f"a bias names a token id and a finite number or -inf: {token}: {value}")
+
     @property
     def greedy(self) -> bool:
         return self.temperature <= 0.0
@@ -169,8 +176,10 @@ class GenerationOptions:
         more: dict = {}
         if self.penalty is not None:
             more |= {"repetition_penalty": self.penalty.value, "penalty_context": self.penalty.context}
-        if self.frequency_penalty or self.presence_penalty:
-            more |= {"frequency_penalty": float(self.frequency_penalty), "presence_penalty": float(self.presence_penalty)}
+        if self.frequency_penalty:
+            more["frequency_penalty"] = float(self.frequency_penalty)
+        if self.presence_penalty:
+            more["presence_penalty"] = float(self.presence_penalty)
         if self.bias:
             more["bias"] = tuple((int(token), float(value)) for token, value in self.bias.items())
         if self.constraint is not None:

@@ -375,6 +375,23 @@ def test_options_that_are_refused():
     assert GenerationOptions(max_tokens=1).params() is GenerationOptions(max_tokens=1).sampler
 
 
+def test_options_that_the_sampler_brings(device):
+    """They count as the generation's own do: checked, and kept beside these."""
+    for wrong in ({"bias": ((-1, 1.0),)}, {"bias": ((1, math.nan),)}, {"bias": ((1, math.inf),)}, {"frequency_penalty": math.nan}, {"presence_penalty": -math.inf}):
+        with pytest.raises(ValueError):
+            SamplingParams(**wrong)
+    own = SamplingParams(frequency_penalty=0.5, presence_penalty=0.25, bias=((4, 100.0),))
+    made = GenerationOptions(max_tokens=1, sampler=own, presence_penalty=1.0).params()
+    assert (made.frequency_penalty, made.presence_penalty, made.bias) == (0.5, 1.0, ((4, 100.0),))
+    engine, _, _ = engine_for("A", device)
+    generator, prompt = Generator(engine), tiny_configs.prompt(5, engine.vocab_size, 4)
+    for options in ({"sampler": SamplingParams(bias=((engine.vocab_size, 1.0),))}, {"bias": {engine.vocab_size: 1.0}}):
+        with pytest.raises(ValueError, match="outside the vocabulary"):
+            generator.add(prompt, GenerationOptions(max_tokens=2, stop=(), **options))
+    assert generator.scheduler.idle
+    assert generator.generate([prompt], GenerationOptions(max_tokens=3, stop=(), sampler=SamplingParams(bias=((4, 100.0),)))) == [[4] * 3]
+
+
 def test_the_text_that_penalties_go_by():
     prompt, made = list(range(100, 110)), [1, 2, 3]
     assert text_of(SamplingParams(), prompt, made).tokens == []
