@@ -82,7 +82,8 @@ def adjust_rows(logits: torch.Tensor, params: Sequence[SamplingParams], texts: S
         words[place["starts"]].view(np.int64)[:] = np.cumsum([0, *lengths])[:-1]
         words[place["lengths"]], words[place["prompts"]] = lengths, [x.prompt for x in texts]
         words[place["contexts"]] = [p.penalty_context if p.repetition_penalty != 1.0 else 0 for p in params]
-        real[place["repetition"]] = [p.repetition_penalty for p in params]
+        # (A context of 0 sees nothing, and is all of the text to the kernel.)
+        real[place["repetition"]] = [p.repetition_penalty if p.penalty_context > 0 else 1.0 for p in params]
         real[place["frequency"]] = [p.frequency_penalty for p in params]
         real[place["presence"]] = [p.presence_penalty for p in params]
         words[place["tokens"]] = [t for x in texts for t in x.tokens]

@@ -392,6 +392,23 @@ def test_options_that_the_sampler_brings(device):
     assert generator.generate([prompt], GenerationOptions(max_tokens=3, stop=(), sampler=SamplingParams(bias=((4, 100.0),)))) == [[4] * 3]
 
 
+def test_a_repetition_penalty_that_sees_nothing(device):
+    """A context of no tokens: beside other penalties and with drafts it does what it does by itself."""
+    engine, _, _ = engine_for("A", device)
+    prompt = tiny_configs.prompt(5, engine.vocab_size, 4)
+    blind = SamplingParams(repetition_penalty=50.0, penalty_context=0)
+    for more in ({}, {"frequency_penalty": 1e-3}):
+        expect = Generator(engine).generate([prompt], GenerationOptions(max_tokens=8, stop=(), **more))[0]
+        options = GenerationOptions(max_tokens=8, stop=(), sampler=blind, **more)
+        assert Generator(engine).generate([prompt], options)[0] == expect
+        generator = Generator(engine)
+        request = generator.add(prompt, options)
+        while not generator.scheduler.idle:
+            at = len(request.generated)
+            generator.step_drafted({request.request_id: (expect[at: at + 3], None)} if at else {})
+        assert request.generated == expect
+
+
 def test_the_text_that_penalties_go_by():
     prompt, made = list(range(100, 110)), [1, 2, 3]
     assert text_of(SamplingParams(), prompt, made).tokens == []
