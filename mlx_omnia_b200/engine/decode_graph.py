@@ -44,7 +44,8 @@ results round otherwise (`ops.paged_attention`).
 
 Steps of drafted trees (`DraftedGraphs`). Their tables are made on the device from the requests' lengths and lists of pages, by the first kernel of
 the step, so one graph serves every step of as many requests, rows, drafts and pages, each rounded up; rows and requests beyond the step's belong to
-requests that hold nothing. Such a step too is captured at its third coming, in the way of mixed steps.
+requests that hold nothing. Such a step too is captured at its third coming, in the way of mixed steps; ahead of that it runs kernel by kernel in the
+same rounded shape, since kernels are chosen and their work is cut by it.
 
 The kernels and the model code are the same as in an uncaptured step; only the way
 they are launched differs, so logits agree bit for bit with an eager step of the same
@@ -357,36 +358,41 @@ class DraftedGraphs:
         self.captured: dict[tuple, _Captured] = {}  # in order of last use, oldest first
         self.replays = 0
 
-    def wants(self, entries) -> tuple | None:
-        """(requests, rows, drafts of a request, width of the tables), where this step should run from a graph. (Their pages are taken.)"""
+    def shape(self, entries) -> tuple | None:
+        """(requests, rows, drafts of a request, width of the tables), rounded, of a step that is captured when it comes often enough (None: never).
+        (Their pages are taken.)"""
         brought = [len(e.tokens) for e in entries]
         if sum(brought) > DRAFTED_MAX_TOKENS or any(e.parents is None for e in entries):
             return None
         total = max(sum(brought), 8)
         step = 1 << (total.bit_length() - 2)  # rows by two significant bits: products of 16 rows and of 13 stream the same weights
-        key = (_bucket(len(entries)), -(-total // step) * step, _bucket(max(brought)),
-               ops.width_bucket(max(len(t) for e in entries for t in e.request.tables)))
+        return (_bucket(len(entries)), -(-total // step) * step, _bucket(max(brought)),
+                ops.width_bucket(max(len(t) for e in entries for t in e.request.tables)))
+
+    def _comes_often(self, key: tuple) -> bool:
         if key in self.captured:
-            return key
+            return True
         self.seen[key] = self.seen.get(key, 0) + 1
         if len(self.seen) > 4096:
             self.seen.clear()
-            return None
-        return key if self.seen[key] >= MIXED_CAPTURE_AT else None
+            return False
+        return self.seen[key] >= MIXED_CAPTURE_AT
 
     def run(self, key: tuple, entries, starts: list[int], copy: bool = True) -> "tuple[torch.Tensor, StepContext]":
-        """-> logits of all the entries' tokens, and the step as these see it (its tables are the graph's own: the next step overwrites them)"""
+        """A step of this shape. -> logits of all the entries' tokens, and the step as these see it (of a captured step its tables are the graph's own:
+        the next step overwrites them)"""
         runner, cache = self.runner, self.runner.cache
         requests, tokens, most, width = key
+        often = self._comes_often(key)
         captured = self.captured.pop(key, None)
         fresh = captured is None
         if fresh:
-            while len(self.captured) >= MIXED_MAX_GRAPHS:
+            while often and len(self.captured) >= MIXED_MAX_GRAPHS:
                 torch.cuda.synchronize(runner.runtime.device)
                 del self.captured[next(iter(self.captured))]
             # Requests that hold nothing for the rows that no entry brings: fewer than `tokens` of them.
             layout = DraftedLayout(tokens, requests + -(-tokens // most), tokens, [width] * len(cache.groups), most)
-            host_tensor = torch.zeros(layout.words, dtype=torch.int32).pin_memory()
+            host_tensor = torch.zeros(layout.words, dtype=torch.int32, pin_memory=True)
             dev = torch.zeros(layout.words, dtype=torch.int32, device=runner.runtime.device)
         else:
             layout, host_tensor, dev = captured.layout, captured.host_tensor, captured.device
@@ -399,7 +405,10 @@ class DraftedGraphs:
             step = layout.context(dev, cache.page_size, width * cache.page_size, q_lens=[], seq_lens_host=[], workspace=workspace)
             return runner.model.forward(step, runner.layer_contexts(step)), step
 
-        if fresh:
+        if not often:
+            logits, step = forward(runner.ask_for_layers())
+            runner.know_layers(step)
+        elif fresh:
             # This step runs kernel by kernel on the graph's buffers; then the same launches are captured.
             workspace: dict = {"private": True}
             logits, step = forward(workspace)

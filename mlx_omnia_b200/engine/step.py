@@ -223,7 +223,7 @@ class DraftedSteps:
         cache.reset_slots([e.request.slot for e in entries if e.request.fresh])
         starts = runner.take_pages(entries)
         graphs = runner.drafted_graphs
-        key = graphs.wants(entries) if graphs is not None else None
+        key = graphs.shape(entries) if graphs is not None else None
         if key is not None:
             logits, step = graphs.run(key, entries, starts, copy)
         else:

@@ -98,6 +98,29 @@ def test_generation_with_captured_steps_of_drafts():
     ops.raise_on_error(torch.device(DEVICE))
 
 
+@pytest.mark.parametrize("held,sizes", [(300, [9]), (2030, [9]), (700, [3, 12, 1]), (60, [17])])
+def test_a_step_has_the_same_logits_captured_or_not(held, sizes):
+    """In bfloat16, bit for bit, at every coming: 9 tokens of 3 query heads are 27 rows of attention and 48 as they are rounded, on the two sides of the
+    choice between its kernels."""
+    engine, _, _ = engine_for("C", DEVICE, cache_tokens=8192, page_size=16, max_requests=8, dtype="bfloat16")
+    vocab, graphs, found = engine.vocab_size, engine.runner.drafted_graphs, []
+    bases = [engine.cache.open(f"base {i}") for i in range(len(sizes))]
+    for i, base in enumerate(bases):
+        engine.runner.run([StepEntry(base, tiny_configs.prompt(held + 5 * i, vocab, 7 + i))])
+    for turn in range(6):
+        entries = [StepEntry(engine.cache.fork(base, f"fork {i}"), tiny_configs.prompt(n, vocab, 40 + i), list(range(n)), refs.tree(n, i, 4))
+                   for i, (base, n) in enumerate(zip(bases, sizes))]
+        found.append(engine.runner.run(entries).clone())
+        kept = engine.runner.keep(entries, chosen_on(DEVICE, [vocab - 1] * sum(sizes)))
+        assert [k.next for k in kept] == [vocab - 1] * len(sizes)
+        for i in range(len(sizes)):
+            engine.cache.close(f"fork {i}")
+    assert graphs.replays == 3 and len(graphs.captured) == 1
+    assert all(torch.equal(x, found[0]) for x in found)
+    engine.cache.check()
+    ops.raise_on_error(torch.device(DEVICE))
+
+
 def test_what_is_not_captured():
     engine, _, _ = engine_for("A", DEVICE, cache_tokens=2048)
     graphs, request, other = engine.runner.drafted_graphs, engine.cache.open("r"), engine.cache.open("o")
