@@ -93,6 +93,7 @@ class Generator:
         self._ids = itertools.count()
         self._seeds: dict[str, int] = {}
         self._in_flight: _Launched | None = None
+        self._held: list[StepOutput] = []  # committed, but not returned yet: a step that fails behind them leaves them to the next call
         self._token_slots: list[torch.Tensor] = []  # pinned buffers the chosen tokens come back in, used in turn
         self._token_slot = 0
         self.pipelined = True  # launch the next decode step before reading this one's tokens
@@ -128,9 +129,18 @@ class Generator:
         self._seeds.pop(request_id, None)
 
     def drain(self) -> list[StepOutput]:
-        """Commit the step that is still in flight, if any."""
+        """Commit the step that is still in flight, if any. -> its outputs, behind those of a call that failed"""
+        self._land()
+        return self._hand_out()
+
+    def _land(self) -> None:
         launched, self._in_flight = self._in_flight, None
-        return self._finalize(launched) if launched is not None else []
+        if launched is not None:
+            self._held += self._finalize(launched)
+
+    def _hand_out(self) -> list[StepOutput]:
+        outputs, self._held = self._held, []
+        return outputs
 
     # -- one step -----------------------------------------------------------------------------
     # A decode step's tokens are chosen on the GPU and can feed the next step from there, so the
@@ -223,11 +233,11 @@ class Generator:
 
     def step(self) -> list[StepOutput]:
         """Run one step (or, in steady decoding, launch the next one and) return what the oldest
-        step in flight produced for each sampling request."""
+        step in flight produced for each sampling request. (What a call that failed had committed comes first.)"""
         if self._in_flight is None:
             plan = self.scheduler.plan()
             if not plan.entries:
-                return []
+                return self._hand_out()
             self._in_flight = self._launch(plan)
         launched = self._in_flight
         following = self._next_decode_plan(launched)
@@ -235,7 +245,8 @@ class Generator:
             self._in_flight = self._launch(following, device_tokens=launched.chosen)
         else:
             self._in_flight = None
-        return self._finalize(launched)
+        self._held += self._finalize(launched)
+        return self._hand_out()
 
     def step_drafted(self, drafts: "Mapping[str, tuple[Sequence[int], Sequence[int] | None]]") -> list[StepOutput]:
         """Run one step in which decoding requests bring drafted tokens, and return what it produced: for a request one token as ever, and one
@@ -245,7 +256,8 @@ class Generator:
         draft that token i goes on from, -1 the latest token itself; None: each goes on from the one ahead of it. Drafts are left aside where
         pages are short, where generation ends with them or ahead of them, where the request's constraint does not let them come or lets nothing follow, in a step that
         reads prompts, and for requests that do not decode. ValueError, and nothing has happened, for drafts that are no such trees and for a
-        model whose layers keep other than keys and values."""
+        model whose layers keep other than keys and values. What was committed ahead of a step that fails is the next call's (`step`, `step_drafted`,
+        `drain`) to return."""
         runner = self.engine.runner
         why = runner.drafted.why_not()
         if why is not None:
@@ -258,12 +270,13 @@ class Generator:
                     len(tokens) >= ops.MOST_DRAFTED:
                 raise ValueError(f"request {name!r}: up to {ops.MOST_DRAFTED - 1} drafts of the vocabulary, each with an earlier parent or -1")
             trees[name] = tokens, parents
-        outputs = self.drain()
+        self._land()
         plan = self.scheduler.plan()
         if not plan.entries:
-            return outputs
+            return self._hand_out()
         if any(e.count != 1 or not e.samples or not e.request.generated for e in plan.entries):
-            return outputs + self._finalize(self._launch(plan))
+            self._held += self._finalize(self._launch(plan))
+            return self._hand_out()
         cache, entries, allowed = self.engine.cache, [], []
         reserved = [0] * len(cache.groups)
         for planned in plan.entries:
@@ -305,11 +318,11 @@ class Generator:
                 for output in some:
                     if output.token is not None:
                         request.meter.token()
-                outputs += some
+                self._held += some
                 if request.status != "running":
                     self._seeds.pop(request.request_id, None)
                     break
-        return outputs
+        return self._hand_out()
 
     def _drafts_of(self, request: Request, drafts: Sequence[int], above: Sequence[int]) -> "tuple[list[int], list[int], list[Collection[int] | None]]":
         """What a request brings to a step with these drafts: its latest token and the drafts that may come behind it, for each the one that it goes on

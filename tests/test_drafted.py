@@ -340,6 +340,41 @@ def test_a_rule_that_fails_ends_its_step(device):
     engine.cache.check()
 
 
+def test_a_step_that_fails_loses_no_output(device, monkeypatch):
+    """Of the step in flight ahead of it, in which one request ended."""
+    engine, _, _ = engine_for("A", device)
+    prompts, options = [tiny_configs.prompt(n, engine.vocab_size, n) for n in (5, 7)], [GenerationOptions(max_tokens=n, stop=()) for n in (2, 9)]
+    expect = [Generator(engine).generate([p], o)[0] for p, o in zip(prompts, options)]
+    for failing in ("run", "keep"):
+        generator = Generator(engine)
+        generator.pipelined = False
+        requests = [generator.add(p, o) for p, o in zip(prompts, options)]
+        assert len(generator.step()) == 2
+        generator._in_flight = generator._launch(generator.scheduler.plan())
+        with monkeypatch.context() as patch:
+            patch.setattr(engine.runner.drafted, failing, lambda *a, **k: (_ for _ in ()).throw(RuntimeError("no more")))
+            with pytest.raises(RuntimeError, match="no more"):
+                generator.step_drafted({requests[1].request_id: ([1, 2], None)})
+        assert requests[1].status == "finished" and requests[1].finish_reason == "abort"
+        outputs = generator.drain()
+        assert [(o.request, o.token, o.finished) for o in outputs] == [(requests[0], expect[0][1], True), (requests[1], expect[1][1], False)]
+        assert not generator.drain() and not generator.step() and not engine.cache.requests
+    # ... and what is handed out by the next step.
+    generator = Generator(engine)
+    generator.pipelined = False
+    first, second = (generator.add(p, o) for p, o in zip(prompts, options))
+    generator.step()
+    generator._in_flight = generator._launch(generator.scheduler.plan())
+    with monkeypatch.context() as patch:
+        patch.setattr(engine.runner.drafted, "run", lambda *a, **k: (_ for _ in ()).throw(RuntimeError("no more")))
+        with pytest.raises(RuntimeError, match="no more"):
+            generator.step_drafted({})
+    third = generator.add(prompts[0], options[0])
+    assert [(o.request, o.token) for o in generator.step()] == [(first, expect[0][1]), (second, expect[1][1]), (third, expect[0][0])]
+    generator.run()
+    engine.cache.check()
+
+
 def test_options_on_logits_by_their_definition(device):
     """Greedy choices, redrawn from the plain implementation's logits."""
     engine, raw, weights = engine_for("B", device)
