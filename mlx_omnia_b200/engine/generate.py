@@ -19,6 +19,7 @@ from collections.abc import Collection, Iterator, Mapping, Sequence
 from dataclasses import dataclass
 from pathlib import Path
 
+import numpy as np
 import torch
 
 from mlx_omnia_b200.engine.engine import DTYPES, Engine, EngineArgs
@@ -26,7 +27,7 @@ from mlx_omnia_b200.engine.meter import Meter
 from mlx_omnia_b200.engine.scheduler import PlannedEntry, Request, Scheduler, StepOutput, StepPlan
 from mlx_omnia_b200.engine.step import StepEntry
 from mlx_omnia_b200.kernels import ops
-from mlx_omnia_b200.sampling.batch import allowed_ids, sample_drafted, sample_rows, text_of
+from mlx_omnia_b200.sampling.batch import allowed_ids, id_array, sample_drafted, sample_rows, text_of
 from mlx_omnia_b200.sampling.options import GenerationOptions
 from mlx_omnia_b200.text.bpe import Detokenizer
 from mlx_omnia_b200.text.defaults import GenerationDefaults
@@ -94,6 +95,7 @@ class Generator:
         self._seeds: dict[str, int] = {}
         self._in_flight: _Launched | None = None
         self._held: list[StepOutput] = []  # committed, but not returned yet: a step that fails behind them leaves them to the next call
+        self._failed: list[Request] = []  # ended by constraints of their own, which no call has raised yet
         self._token_slots: list[torch.Tensor] = []  # pinned buffers the chosen tokens come back in, used in turn
         self._token_slot = 0
         self.pipelined = True  # launch the next decode step before reading this one's tokens
@@ -142,6 +144,25 @@ class Generator:
         outputs, self._held = self._held, []
         return outputs
 
+    def _deliver(self) -> list[StepOutput]:
+        """What a step returns. Where a request's constraint failed in it, that error is raised and the outputs, the request's end among them, are
+        the next call's."""
+        failed, self._failed = self._failed, []
+        if failed:
+            raise failed[0].error
+        return self._hand_out()
+
+    def _fail(self, request: Request, error: Exception) -> None:
+        self.scheduler._finish(request, "abort")  # (frees what it holds)
+        request.error = error
+        self._seeds.pop(request.request_id, None)
+
+    def _fail_alone(self, request: Request, error: Exception) -> None:
+        """End a request by its own constraint's error: the step goes on for the others."""
+        self._fail(request, error)
+        self._held.append(StepOutput(request, None, True))
+        self._failed.append(request)
+
     # -- one step -----------------------------------------------------------------------------
     # A decode step's tokens are chosen on the GPU and can feed the next step from there, so the
     # host need not wait for them before it launches that step: while the GPU runs step n + 1 the
@@ -159,9 +180,10 @@ class Generator:
         try:
             logits = self.engine.runner.run(entries, copy=False, device_tokens=device_tokens)
             chosen = self._choose(logits, sampling, 1 if device_tokens is not None else 0) if sampling else None
-        except Exception:
-            for planned in plan.entries:  # a failed step fails its requests and frees what they hold
-                self.scheduler._finish(planned.request, "abort")
+        except Exception as error:
+            for planned in plan.entries:  # a failed step fails its requests
+                if planned.request.error is None:
+                    self._fail(planned.request, error)
             raise
         launched = _Launched(plan, sampling, chosen)
         if chosen is not None and chosen.is_cuda:
@@ -184,10 +206,18 @@ class Generator:
                                    r.sampling.penalty_context) if r.sampling.repetition_penalty != 1.0 else []
                      for r in sampling]
         adjusts = any(r.sampling.adjusts for r in sampling)
-        return sample_rows(logits, [r.sampling for r in sampling], [self._seeds[r.request_id] for r in sampling],
-                           [len(r.generated) + ahead for r in sampling], histories,
-                           [text_of(r.sampling, r.prompt, r.generated) for r in sampling] if adjusts else None,
-                           [allowed_ids(r.sampling, r.generated) for r in sampling] if adjusts else None)
+        params, seeds = [r.sampling for r in sampling], [self._seeds[r.request_id] for r in sampling]
+        draws = [len(r.generated) + ahead for r in sampling]
+        return sample_rows(logits, params, seeds, draws, histories, [text_of(r.sampling, r.prompt, r.generated) for r in sampling] if adjusts else None,
+                           [self._allowed(r) for r in sampling] if adjusts else None)
+
+    def _allowed(self, request: Request) -> np.ndarray | None:
+        """What the request's constraint lets come next. A constraint that fails ends its request, which is given any token then and keeps none."""
+        try:
+            return id_array(allowed_ids(request.sampling, request.generated), self.engine.vocab_size)
+        except Exception as error:
+            self._fail_alone(request, error)
+            return None
 
     def _finalize(self, launched: "_Launched") -> list[StepOutput]:
         """Read the launched step's tokens (this waits for it) and commit them."""
@@ -233,11 +263,16 @@ class Generator:
 
     def step(self) -> list[StepOutput]:
         """Run one step (or, in steady decoding, launch the next one and) return what the oldest
-        step in flight produced for each sampling request. (What a call that failed had committed comes first.)"""
+        step in flight produced for each sampling request. (What a call that failed had committed comes first.) A request whose constraint
+        fails ends, with the error as its `error`; the step goes on for the others and then raises it, and what it produced is the next call's to return."""
+        self._advance()
+        return self._deliver()
+
+    def _advance(self) -> None:
         if self._in_flight is None:
             plan = self.scheduler.plan()
             if not plan.entries:
-                return self._hand_out()
+                return
             self._in_flight = self._launch(plan)
         launched = self._in_flight
         following = self._next_decode_plan(launched)
@@ -246,7 +281,6 @@ class Generator:
         else:
             self._in_flight = None
         self._held += self._finalize(launched)
-        return self._hand_out()
 
     def step_drafted(self, drafts: "Mapping[str, tuple[Sequence[int], Sequence[int] | None]]") -> list[StepOutput]:
         """Run one step in which decoding requests bring drafted tokens, and return what it produced: for a request one token as ever, and one
@@ -276,23 +310,30 @@ class Generator:
             return self._hand_out()
         if any(e.count != 1 or not e.samples or not e.request.generated for e in plan.entries):
             self._held += self._finalize(self._launch(plan))
-            return self._hand_out()
+            return self._deliver()
         cache, entries, allowed = self.engine.cache, [], []
         reserved = [0] * len(cache.groups)
         for planned in plan.entries:
             self.scheduler._reserve(planned.request, 1, reserved)
-        requests = [planned.request for planned in plan.entries]
-        try:
-            for planned in plan.entries:
-                request = planned.request
+        requests: list[Request] = []
+        for planned in plan.entries:
+            request = planned.request
+            try:
                 tokens, parents, lets = self._drafts_of(request, *trees.get(request.request_id, ((), ())))
-                held = request.cache.tokens
-                mine = [cache.pages_for(g, held + len(tokens)) - cache.pages_for(g, held + 1) for g in range(len(cache.groups))]
-                if any(r + m > g.pool.free for r, m, g in zip(reserved, mine, cache.groups)):
-                    tokens, parents, lets, mine = tokens[:1], parents[:1], lets[:1], [0] * len(mine)
-                reserved = [r + m for r, m in zip(reserved, mine)]
-                entries.append(StepEntry(request.cache, tokens, list(range(len(tokens))), parents))
-                allowed += lets
+            except Exception as error:
+                self._fail_alone(request, error)
+                continue
+            held = request.cache.tokens
+            mine = [cache.pages_for(g, held + len(tokens)) - cache.pages_for(g, held + 1) for g in range(len(cache.groups))]
+            if any(r + m > g.pool.free for r, m, g in zip(reserved, mine, cache.groups)):
+                tokens, parents, lets, mine = tokens[:1], parents[:1], lets[:1], [0] * len(mine)
+            reserved = [r + m for r, m in zip(reserved, mine)]
+            requests.append(request)
+            entries.append(StepEntry(request.cache, tokens, list(range(len(tokens))), parents))
+            allowed += lets
+        if not entries:
+            return self._deliver()
+        try:
             logits = runner.run(entries, copy=False)
             owners, depths = [], []
             for r, entry in enumerate(entries):
@@ -307,10 +348,9 @@ class Generator:
             chosen = sample_drafted(logits, runner.drafted.last[1], rows, owners, depths, params, [self._seeds[r.request_id] for r in requests],
                                     [len(r.generated) for r in requests], texts, allowed)
             kept = runner.keep(entries, chosen)
-        except Exception:
-            for request in requests:  # a failed step fails its requests and frees what they hold
-                self.scheduler._finish(request, "abort")
-                self._seeds.pop(request.request_id, None)
+        except Exception as error:
+            for request in requests:  # a failed step fails its requests
+                self._fail(request, error)
             raise
         for request, mine in zip(requests, kept):
             for token in [*mine.tokens, mine.next]:
@@ -322,30 +362,35 @@ class Generator:
                 if request.status != "running":
                     self._seeds.pop(request.request_id, None)
                     break
-        return self._hand_out()
+        return self._deliver()
 
-    def _drafts_of(self, request: Request, drafts: Sequence[int], above: Sequence[int]) -> "tuple[list[int], list[int], list[Collection[int] | None]]":
+    def _drafts_of(self, request: Request, drafts: Sequence[int], above: Sequence[int]) -> "tuple[list[int], list[int], list[np.ndarray | None]]":
         """What a request brings to a step with these drafts: its latest token and the drafts that may come behind it, for each the one that it goes on
         from and what may follow it. What is left out: the request's last token and its stop tokens, which nothing is chosen behind; drafts that its
-        constraint does not let come there (it is asked only about texts that it let come) or lets nothing follow; and what goes on from such."""
-        tokens, parents, allowed = [request.generated[-1]], [-1], [allowed_ids(request.sampling, request.generated)]
+        constraint does not let come there (it is asked only about texts that it let come), lets nothing follow or fails at (should such a text
+        come, it ends the request then); and what goes on from such."""
+        vocab = self.engine.vocab_size
+        lets = allowed_ids(request.sampling, request.generated)
+        tokens, parents, rules, allowed = [request.generated[-1]], [-1], [lets], [id_array(lets, vocab)]
         ways: list[list[int]] = [[]]
         places = {-1: 0}  # of the drafts, those that stay: their place
         for i, (token, p) in enumerate(zip(drafts, above)):
             at = places.get(p)
             if at is None or len(request.generated) + len(ways[at]) + 1 >= request.max_tokens or token in request.stop:
                 continue
-            if allowed[at] is not None and token not in allowed[at]:
+            if rules[at] is not None and token not in rules[at]:
                 continue
             way, lets = [*ways[at], token], None
-            if request.sampling.constraint is not None:
-                lets = request.sampling.constraint([*request.generated, *way])
-                if lets is not None and not len(lets):
-                    continue
+            try:
+                lets = allowed_ids(request.sampling, [*request.generated, *way])
+                ids = id_array(lets, vocab)
+            except Exception:
+                continue
             places[i] = len(tokens)
             tokens.append(token)
             parents.append(at)
-            allowed.append(lets)
+            rules.append(lets)
+            allowed.append(ids)
             ways.append(way)
         return tokens, parents, allowed
 
@@ -365,8 +410,17 @@ class Generator:
     def run(self) -> None:
         """Step until every request has finished."""
         while not self.scheduler.idle or self._in_flight is not None:
-            if not self.step() and self._in_flight is None and not self.scheduler.running and self.scheduler.waiting:
-                raise RuntimeError("the scheduler can admit nothing: the cache pool is too small")
+            self._idle(self.step())
+
+    def _idle(self, outputs: list[StepOutput]) -> None:
+        if not outputs and self._in_flight is None and not self.scheduler.running and self.scheduler.waiting:
+            raise RuntimeError("the scheduler can admit nothing: the cache pool is too small")
+
+    def advance_for(self, requests: Sequence[Request]) -> list[StepOutput]:
+        """`step` for a caller that goes by its own requests: of constraints that failed, only theirs are raised."""
+        self._advance()
+        self._failed = [r for r in self._failed if any(r is mine for mine in requests)]
+        return self._deliver()
 
     def generate(self, prompts: Sequence[Sequence[int]], options: GenerationOptions, *, samples: int = 1,
                  share: bool = False) -> list[list[int]]:
@@ -392,7 +446,14 @@ class Generator:
                 draws = options if seed is None else \
                     dataclasses.replace(options, sampler=dataclasses.replace(options.sampler, seed=seed + i))
                 requests.append(self.add(prompt, draws, leader=first))
-        self.run()
+        try:
+            while not self.scheduler.idle or self._in_flight is not None:
+                self._idle(self.advance_for(requests))
+        except BaseException:
+            for request in requests:  # the others are not left behind
+                if request.status != "finished":
+                    self.abort(request.request_id)
+            raise
         ops.raise_on_error(self.engine.runtime.device)
         return [r.generated for r in requests]
 
@@ -419,9 +480,11 @@ class LanguageModel:
         pieces = Detokenizer(self.tokenizer)
         try:
             while request.status != "finished":
-                for output in self.generator.step():
+                for output in self.generator.advance_for([request]):
                     if output.request is request and output.token is not None:
                         yield Segment(pieces.feed(output.token), output.token)
+            if request.error is not None:  # (met in a step that another stream took)
+                raise request.error
             rest = pieces.flush()
             if rest:
                 yield Segment(rest, -1)

@@ -59,6 +59,7 @@ class Request:
     cache: RequestCache | None = None
     status: str = "waiting"  # waiting | running | finished
     finish_reason: str | None = None  # stop | length | abort
+    error: Exception | None = None  # what ended it, where that was its own constraint or a step that failed
     preemptions: int = 0
     order: int = 0
     meter: object | None = None  # an engine.meter.Meter, filled by the generation loop

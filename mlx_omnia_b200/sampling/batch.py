@@ -41,6 +41,17 @@ def allowed_ids(params: SamplingParams, generated: Sequence[int]) -> "Collection
     return allowed
 
 
+def id_array(allowed: "Collection[int] | None", vocab: int) -> np.ndarray | None:
+    """What a constraint lets come next as an array. ValueError for a token that there is not."""
+    if allowed is None:
+        return None
+    ids = allowed if isinstance(allowed, np.ndarray) else np.asarray(list(allowed))
+    ids = ids.astype(np.int64, copy=False)
+    if ids.min() < 0 or ids.max() >= vocab:
+        raise ValueError(f"a constraint allows a token outside the vocabulary of {vocab}")
+    return ids
+
+
 def _masks(allowed: "Sequence[Collection[int] | None]", vocab: int, device: torch.device) -> "ops.TokenMasks | None":
     """A mask of bits for every row that has one."""
     some = [i for i, a in enumerate(allowed) if a is not None]
@@ -50,9 +61,7 @@ def _masks(allowed: "Sequence[Collection[int] | None]", vocab: int, device: torc
     words = np.empty(len(allowed) + len(some) * width, dtype=np.int32)
     words[: len(allowed)] = -1
     for k, i in enumerate(some):
-        ids = np.asarray(list(allowed[i]), dtype=np.int64)
-        if ids.min() < 0 or ids.max() >= vocab:
-            raise ValueError(f"a constraint allows a token outside the vocabulary of {vocab}")
+        ids = id_array(allowed[i], vocab)
         row = np.zeros(width * 32, dtype=bool)
         row[ids] = True
         words[i] = k

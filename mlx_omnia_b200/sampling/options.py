@@ -146,7 +146,8 @@ class GenerationOptions:
     frequency_penalty: subtracted from a token's logit for every time that it was generated
     presence_penalty:  subtracted from a token's logit once if it was generated
     bias:           {token id: what its logit is raised by} (-inf: never chosen), behind the penalties
-    constraint:     a function of the ids generated so far -> the ids that may come next (None: any); asked for every token
+    constraint:     a function of the ids generated so far -> the ids that may come next (None: any); asked for every token. An error of its own, no
+                    ids, or ids that there are not end its request, and no other one
     context_limit:  ceiling on prompt and generation together, or None
     meter:          an `engine.meter.Meter` that the generation fills (token counts, time to the
                     first token, decode rate), or None

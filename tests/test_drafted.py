@@ -17,7 +17,7 @@ import tiny_configs
 from mlx_omnia_b200 import GenerationOptions, min_p, repetition_penalty, sampler, temperature, top_k
 from mlx_omnia_b200.cache import CacheError
 from mlx_omnia_b200.engine.engine import Engine, EngineArgs
-from mlx_omnia_b200.engine.generate import Generator
+from mlx_omnia_b200.engine.generate import Generator, LanguageModel
 from mlx_omnia_b200.engine.step import StepEntry
 from mlx_omnia_b200.kernels import ops
 from mlx_omnia_b200.parts.base import KVSpec, KVView, StepContext
@@ -372,6 +372,91 @@ def test_a_step_that_fails_loses_no_output(device, monkeypatch):
     third = generator.add(prompts[0], options[0])
     assert [(o.request, o.token) for o in generator.step()] == [(first, expect[0][1]), (second, expect[1][1]), (third, expect[0][0])]
     generator.run()
+    engine.cache.check()
+
+
+RULES = {"nothing": lambda made: [] if len(made) == 3 else None, "no token": lambda made: [10 ** 6] if len(made) == 3 else None,
+         "an error": lambda made: {}["gone"] if len(made) == 3 else range(400), "no ids": lambda made: ["x"] if len(made) == 3 else None}
+
+
+@pytest.mark.parametrize("which", list(RULES))
+@pytest.mark.parametrize("drafted", [False, True])
+def test_a_rule_that_fails_ends_its_own_request_alone(device, which, drafted):
+    """The others have the tokens that they would have had, none of which is lost."""
+    engine, _, _ = engine_for("A", device)
+    prompts = [tiny_configs.prompt(n, engine.vocab_size, n) for n in (5, 9, 12)]
+    options = [GenerationOptions(max_tokens=8, stop=(), sampler=sampler(temperature(0.8), seed=3), frequency_penalty=0.2),
+               GenerationOptions(max_tokens=8, stop=(), constraint=RULES[which]), GenerationOptions(max_tokens=8, stop=())]
+    expect = [Generator(engine).generate([p], o)[0] if o.constraint is None else None for p, o in zip(prompts, options)]
+    generator, outputs, errors = Generator(engine), [], []
+    requests = [generator.add(p, o) for p, o in zip(prompts, options)]
+    while not generator.scheduler.idle or generator._in_flight is not None:
+        drafts = {r.request_id: (e[len(r.generated): len(r.generated) + 2], None) for r, e in zip(requests, expect) if e is not None and r.generated}
+        try:
+            outputs += generator.step_drafted(drafts) if drafted else generator.step()
+        except Exception as error:  # noqa: BLE001
+            errors.append(error)
+    outputs += generator.drain()
+    assert [r.generated for r in requests[::2]] == expect[::2] and [r.finish_reason for r in requests] == ["length", "abort", "length"]
+    assert errors == [requests[1].error] and len(requests[1].generated) == 3 and requests[0].error is None and requests[2].error is None
+    for r in requests:
+        mine = [o for o in outputs if o.request is r]
+        assert [o.token for o in mine if o.token is not None] == r.generated
+        assert [o.finished for o in mine] == [False] * (len(mine) - 1) + [True]
+    assert not engine.cache.requests and not generator._seeds
+    engine.cache.check()
+
+
+def test_a_rule_that_fails_is_its_callers(device):
+    """`generate` and streams beside a request whose rule fails go on; its own stream, and the call that it belongs to, raise the error."""
+    engine, _, _ = engine_for("A", device)
+    prompts = [tiny_configs.prompt(n, engine.vocab_size, n) for n in (5, 9, 12)]
+    plain, wrong = GenerationOptions(max_tokens=6, stop=()), GenerationOptions(max_tokens=6, stop=(), constraint=RULES["an error"])
+    expect = Generator(engine).generate(prompts[::2], plain)
+    generator = Generator(engine)
+    odd = generator.add(prompts[1], wrong)
+    assert generator.generate(prompts[::2], plain) == expect
+    assert isinstance(odd.error, KeyError) and odd.status == "finished"
+    bystander = generator.add(prompts[2], plain)
+    late = [r for r in generator.scheduler.waiting]
+    with pytest.raises(KeyError):
+        generator.generate(prompts[:2], wrong)
+    assert late == [bystander] and bystander.status == "running" and generator.scheduler.running == [bystander] and not generator.scheduler.waiting
+    generator.run()
+    assert bystander.generated == expect[1]
+    model = LanguageModel(engine)
+    streams = [model.stream(prompts[0], plain), model.stream(prompts[1], wrong)]
+    first, second = [next(streams[0]).token_id], []
+    with pytest.raises(KeyError):
+        while True:
+            second.append(next(streams[1]).token_id)  # (takes the steps of both)
+    with pytest.raises(StopIteration):
+        while True:
+            next(streams[0])
+    assert model.generator.scheduler.idle and first == expect[0][:1]
+    streams = [model.stream(prompts[1], wrong), model.stream(prompts[0], plain)]
+    next(streams[0])
+    assert [s.token_id for s in streams[1] if s.token_id >= 0] == expect[0]
+    with pytest.raises(KeyError):
+        list(streams[0])
+    assert not engine.cache.requests
+    engine.cache.check()
+
+
+def test_a_rule_that_fails_at_a_draft_fails_when_it_comes(device):
+    """A draft of a text that the rule fails at is left aside: the tokens and the end are those of steps without drafts."""
+    engine, _, _ = engine_for("A", device)
+    prompt = tiny_configs.prompt(9, engine.vocab_size, 4)
+    free = Generator(engine).generate([prompt], GenerationOptions(max_tokens=8, stop=()))[0]
+    never = next(t for t in range(engine.vocab_size) if t not in free)
+    for rule in (lambda made: {}["gone"] if never in made else None, lambda made: [-1] if never in made else None):
+        generator = Generator(engine)
+        request = generator.add(prompt, GenerationOptions(max_tokens=8, stop=(), constraint=rule))
+        while not generator.scheduler.idle:
+            at = len(request.generated)
+            ahead = free[at: at + 2]  # (as many as there are)
+            generator.step_drafted({request.request_id: ([never, 5, *ahead], [-1, 0, -1, 2][: 2 + len(ahead)])} if at else {})
+        assert request.generated == free and request.error is None
     engine.cache.check()
 
 
