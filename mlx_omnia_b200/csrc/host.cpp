@@ -443,8 +443,12 @@ PyObject* adjust_logits(PyObject*, PyObject* const* args, Py_ssize_t given) {
       a.bias_values = like(item(bias, 1, 3, what), what, "values", at::kFloat, index, {(int64_t)a.bias_count});
       a.bias_ids = THPVariable_Unpack(ids).data_ptr();
     }
-    if (args[7] != Py_None) a.requests = like(args[7], what, "requests", at::kInt, index, {rows});
-    else if (num < rows && (text || biased)) refuse(what, ": " + std::to_string(rows) + " rows of " + std::to_string(num) + " requests need `requests`");
+    if (args[7] != Py_None) {
+      const void* requests = like(args[7], what, "requests", at::kInt, index, {rows});
+      if (text || biased) a.requests = requests;  // (nothing else goes by them, and there is no number of requests then)
+    } else if (num < rows && (text || biased)) {
+      refuse(what, ": " + std::to_string(rows) + " rows of " + std::to_string(num) + " requests need `requests`");
+    }
     if (masks != Py_None) {
       const at::Tensor& words = tensor(item(masks, 0, 2, what), what, "mask words");
       if (words.dim() != 2 || words.size(1) * 32 < vocab)

@@ -569,6 +569,16 @@ def test_texts_that_lie_nowhere(start, length):
     assert error_of(16) and torch.equal(got, logits)
 
 
+def test_masks_alone_go_by_no_requests():
+    """Rows of requests of which nothing is given but masks: whose rows they are changes nothing."""
+    logits = torch.randn(3, 70, device="cuda")
+    masks = ops.TokenMasks(ints([[-1, 0, 63], [5, 0, 0]]), ints([0, -1, 1]))
+    expect = ops.adjust_logits(logits, masks=masks)
+    assert torch.equal(expect[1], logits[1]) and torch.isinf(expect[2]).sum() == 68 and torch.isinf(expect[0]).sum() == 32
+    for requests in ([0, 0, 1], [9, 4, 100], [-1, 5, 2]):
+        assert torch.equal(ops.adjust_logits(logits, masks=masks, requests=ints(requests)), expect)
+
+
 def test_adjust_reports_bad_numbers():
     logits = torch.zeros(2, 100, device="cuda")
     run = lambda **more: call_adjust(logits, *({"texts": [[1], [2]], "prompts": [0, 0], "values": [[1.0] * 2] * 3, "bias": [[], []], "masks": [None] * 2} | more).values(), "pb")  # noqa: E731
