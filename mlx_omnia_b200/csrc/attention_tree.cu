@@ -1,5 +1,5 @@
-// Attention of trees of drafted tokens for any head sizes (<= 512; keys and values may differ in width), page size and element type, and the
-// merge of the pieces that all kernels of such attention leave behind.
+// Attention of trees of drafted tokens for any head sizes (<= 512; keys and values may differ in width), page size, element type and number of requests, with
+// the merge of its pieces, and the 32-bit path's kernel by equal shares (whose items the join of attention_tree.cuh puts together).
 //
 //   out[i, h] = sigmoid(gate) * sum_k p_k v_k / (sum_k p_k + exp(sink_h)),  p_k = exp(s_k), s_k = scale q_i . k (softcap tanh(s / softcap))
 //
@@ -622,7 +622,7 @@ extern "C" int omnia_tree_merge(const TreeAttention* a, int dtype, void* stream)
 }
 
 // The 32-bit path: keys and values of one width, a multiple of 4 up to 256. `blocks`: what the work is shared out over, with two slots of
-// omnia_tree32_rows rows each in part_o and part_ml.
+// ROWS rows each in part_o and part_ml.
 extern "C" int omnia_tree_attention32(const TreeAttention* a, int most_nodes, int blocks, void* stream) {
   if (a->d != a->dv || a->d % 4 || a->d < 4 || a->d > 256 || a->nkv < 1 || a->nkv > 65535 || a->nq % a->nkv || a->requests < 1 ||
       a->requests > TREE_MOST_REQUESTS || most_nodes < 1 || blocks < 1 || a->page_size < 1 || a->page_stride % 4 ||

@@ -4,10 +4,11 @@
 // Floor: a request's keys and values once (4 D bytes a position and key/value head) at the memory's rate, or the products' 4 D operations a row and
 // position, whichever is more; 256 rows are where the two meet.
 //
-// Measured, 32 / 8 heads of 128: 32 requests of up to 8,192 positions with up to 64 tokens (795 MB, 0.14 PFLOP) 297 to 327 us, 0.46 PFLOP/s, 2.6 TB/s; 4
-// of up to 131,072 with up to 24 (1.49 GB) 270 to 328, 4.5 to 5.5 TB/s. 16 / 8 heads, 8 of up to 4,096 with up to 16 (100 MB): 39, of which 12 to 15 are
-// beginnings, ends and the join. What bounds the long ones is a tile's chain, 2.7 us for 128 keys of 256 rows, where the products alone would take 1.5. Of
-// the 2,850 cycles that a softmax warp has for a half, 330 go to whether the scores are there, 170 to their load, 370 to the maximum, 330 to the offset,
+// Measured, 32 / 8 heads of 128: 32 requests of up to 8,192 positions with up to 64 tokens (795 MB, 0.14 PFLOP) 298 us, 325 as the GPU gets to its power limit
+// (1,000 W, 1.97 -> 1.79 GHz), 0.47 PFLOP/s, 2.7 TB/s; 4 of up to 131,072 with up to 24 (1.49 GB) 268, 300 to 330 at the limit (1.49 GHz), 4.5 to 5.6 TB/s.
+// 16 / 8 heads, 8 of up to 4,096 with up to 16 (100 MB): 40.5, of which 12 to 15 are beginnings, ends and the join. What bounds the first is a tile's chain:
+// 5,700 cycles for 128 keys of 256 rows, 2.9 us at 1.97 GHz where the products alone would take 1.5; 79 tiles an SM are 230 us, the rest the
+// beginnings and ends of an SM's two to four segments. Of the 2,850 cycles that a softmax warp has for a half, 330 go to whether the scores are there, 170 to their load, 370 to the maximum, 330 to the offset,
 // 1,350 to weights, sums and pairs (707 without the exponentials), 320 to the store. For every instruction issued 0.94 warps wait for one to be fetched: code
 // taken out of the loop, though never run, is gained. Float32 in pairs and maxima of three: 1,030 for the weights, the same time in all. Error against
 // 64 bits 0.0023 of the outputs' size, where a 32-bit form rounded once has 0.0017.

@@ -284,14 +284,15 @@ class Generator:
 
     def step_drafted(self, drafts: "Mapping[str, tuple[Sequence[int], Sequence[int] | None]]") -> list[StepOutput]:
         """Run one step in which decoding requests bring drafted tokens, and return what it produced: for a request one token as ever, and one
-        more for every draft that it agrees with. The tokens are those of steps without drafts (drawn by the same numbers).
+        more for every draft that it agrees with. The tokens are those of steps without drafts (drawn by the same numbers): a step of
+        several rows rounds its sums otherwise than one of single tokens, so in bfloat16 an answer may part where two tokens are as good as equal.
 
         `drafts`: request id -> (tokens, parents): what may follow the request's latest token, as a tree: `parents[i]` is the earlier
         draft that token i goes on from, -1 the latest token itself; None: each goes on from the one ahead of it. Drafts are left aside where
-        pages are short, where generation ends with them or ahead of them, where the request's constraint does not let them come or lets nothing follow, in a step that
+        pages are short, where generation ends with them or ahead of them, where the request's constraint does not let them come, lets nothing follow or fails at them, in a step that
         reads prompts, and for requests that do not decode. ValueError, and nothing has happened, for drafts that are no such trees and for a
         model whose layers keep other than keys and values. What was committed ahead of a step that fails is the next call's (`step`, `step_drafted`,
-        `drain`) to return."""
+        `drain`) to return. A constraint that fails ends its request, as in `step`."""
         runner = self.engine.runner
         why = runner.drafted.why_not()
         if why is not None:
