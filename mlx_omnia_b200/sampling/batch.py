@@ -111,6 +111,11 @@ def adjust_rows(logits: torch.Tensor, params: Sequence[SamplingParams], texts: S
         masks=_masks(allowed, logits.shape[1], logits.device), drafted=drafted if counting else None, out=logits)
 
 
+def _adjusted(params: SamplingParams) -> SamplingParams:
+    """What is left to do on adjusted logits. (No bias: new parameters check theirs, at every step.)"""
+    return params if params.repetition_penalty == 1.0 else replace(params, repetition_penalty=1.0, bias=())
+
+
 def sample_drafted(logits: torch.Tensor, step, rows: Sequence[int], requests: Sequence[int], depths: Sequence[int], params: Sequence[SamplingParams],
                    seeds: Sequence[int], draws: Sequence[int], texts: Sequence[Text], allowed: "Sequence[Collection[int] | None]") -> torch.Tensor:
     """Choose one token for every row of a step of drafted trees: `rows[i]` the step's row that logits row i belongs to, `requests[i]` its
@@ -119,7 +124,7 @@ def sample_drafted(logits: torch.Tensor, step, rows: Sequence[int], requests: Se
     if any(p.adjusts or p.repetition_penalty != 1.0 for p in params):
         at = torch.as_tensor(np.asarray(rows, dtype=np.int32)).to(logits.device, non_blocking=True)
         adjust_rows(logits, params, texts, allowed, requests, ops.DraftedRows(step.tree, step.token_ids, step.cu_seqlens, at))
-    plain = [replace(p, repetition_penalty=1.0) for p in params]
+    plain = [_adjusted(p) for p in params]
     return _choose(logits, [plain[r] for r in requests], [seeds[r] for r in requests], [draws[r] + d for r, d in zip(requests, depths)], [[]] * len(requests))
 
 
@@ -133,7 +138,7 @@ def sample_rows(logits: torch.Tensor, params: list[SamplingParams], seeds: list[
     -> int32 [rows] on the device."""
     if any(p.adjusts for p in params):
         adjust_rows(logits, params, texts, allowed)
-        params, histories = [replace(p, repetition_penalty=1.0) for p in params], [[]] * len(params)
+        params, histories = [_adjusted(p) for p in params], [[]] * len(params)
     return _choose(logits, params, seeds, draws, histories)
 
 
